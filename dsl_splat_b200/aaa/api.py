@@ -20,6 +20,7 @@ import torch
 from torch import Tensor
 
 from ..cameras import validate_camera_options
+from ..features import FeatureDecoder
 from ..inputs import batch_item, normalize_inputs, spherical_harmonics
 from ..statistics import StatisticsRequest, prepare_statistics
 from ..training import prepare_training_metadata
@@ -50,6 +51,11 @@ class RasterizationResult:
     @property
     def extra_features(self) -> Tensor | None:
         return self.meta.get("render_extra_signals")
+
+    @property
+    def decoded_features(self) -> Tensor | None:
+        """The feature decoder's image (None without a feature_decoder)."""
+        return self.meta.get("decoded_features")
 
 
 def _check_arguments(features, sh_coeffs, sh_degree):
@@ -96,7 +102,8 @@ def rasterize(means: Tensor, quats: Tensor, scales: Tensor, opacities: Tensor, v
               filter3d: Tensor | None = None, near_plane: float = 0.01, far_plane: float = 1e10,
               radius_clip: float = 0.0, packed: bool = False, absgrad: bool = False,
               settings: ExtendedSettings | None = None,
-              statistics: Sequence[StatisticsRequest] = ()) -> RasterizationResult:
+              statistics: Sequence[StatisticsRequest] = (),
+              feature_decoder: FeatureDecoder | None = None) -> RasterizationResult:
     """Render AAA Gaussians with OpenCV world-to-camera poses and zero-skew K.
 
     Pass features (...,N,D) / (...,C,N,D), or SH coefficients (...,N,K,3) /
@@ -104,7 +111,11 @@ def rasterize(means: Tensor, quats: Tensor, scales: Tensor, opacities: Tensor, v
     are normalised differentiably.  Defaults: AAA's antialiased HIER 64/8/4
     configuration.  First-order gradients reach the Gaussian parameters,
     features/SH, extras and poses; K, background and filter gradients are
-    not supported (as in the reference)."""
+    not supported (as in the reference).
+
+    feature_decoder (features.FeatureDecoder; no counterpart in the reference)
+    is called on the extra feature image, or on the features without extras,
+    and gives meta["decoded_features"]."""
     validate_camera_options(width, height, near_plane, far_plane, radius_clip)
     sh_degree = _check_arguments(features, sh_coeffs, sh_degree)
     # the raw quaternions go to the kernels, which normalise them with
@@ -189,7 +200,10 @@ def rasterize(means: Tensor, quats: Tensor, scales: Tensor, opacities: Tensor, v
     if extras:
         meta["render_extra_signals"] = torch.stack(extras).reshape(
             shape + (layout.extras.channels,))
-    return RasterizationResult(torch.stack(outputs).reshape(shape + (channels,)),
+    main = torch.stack(outputs).reshape(shape + (channels,))
+    if feature_decoder is not None:
+        meta["decoded_features"] = feature_decoder(meta.get("render_extra_signals", main))
+    return RasterizationResult(main,
                                torch.stack(alphas).reshape(shape + (1,)), meta,
                                statistics_outputs)
 

@@ -18,6 +18,7 @@ from torch import Tensor
 
 from ..camera_prep import ViewConfig, prepare_cameras, prepare_cameras_with_centers
 from ..cameras import validate_camera_options
+from ..features import FeatureDecoder
 from ..inputs import batch_item, normalize_inputs
 from ..statistics import StatisticsRequest, prepare_statistics
 from ..training import prepare_training_metadata
@@ -53,6 +54,11 @@ class RasterizationResult:
     @property
     def extra_features(self) -> Tensor | None:
         return self.meta.get("render_extra_signals")
+
+    @property
+    def decoded_features(self) -> Tensor | None:
+        """The feature decoder's image (None without a feature_decoder)."""
+        return self.meta.get("decoded_features")
 
 
 def _check_sh(sh_coeffs, sh_degree, features):
@@ -91,13 +97,18 @@ def rasterize(means: Tensor, quats: Tensor, scales: Tensor, opacities: Tensor, v
               near_plane: float = 0.2, far_plane: float = math.inf, radius_clip: float = 0.0,
               packed: bool = False, absgrad: bool = False,
               statistics: Sequence[StatisticsRequest] = (),
-              tile_mode: str = "radius") -> RasterizationResult:
+              tile_mode: str = "radius",
+              feature_decoder: FeatureDecoder | None = None) -> RasterizationResult:
     """Render original 3DGS (centre-depth order, square tile bounds).
 
     Inputs are activated scales/opacities and wxyz quaternions (normalised
     here).  means2d is in CUDA raster coordinates (integer pixel centres,
     K-projected position minus 0.5), zero for culled rows.  Gradients reach
     means, quats, scales, opacities, features/SH, extras and viewmats.
+
+    feature_decoder (features.FeatureDecoder; no counterpart in the reference)
+    is called on the extra feature image, or on the features without extras,
+    and gives meta["decoded_features"].
     """
     validate_tile_mode(tile_mode)
     validate_camera_options(width, height, near_plane, far_plane, radius_clip)
@@ -235,4 +246,6 @@ def rasterize(means: Tensor, quats: Tensor, scales: Tensor, opacities: Tensor, v
     if layout.extras is not None:
         meta["render_extra_signals"] = main[..., channels:]
         features = main[..., :channels]
+    if feature_decoder is not None:
+        meta["decoded_features"] = feature_decoder(meta.get("render_extra_signals", features))
     return RasterizationResult(features, alpha, meta, statistics_outputs)

@@ -21,6 +21,7 @@ from .. import stages
 from ..camera_prep import prepare_cameras, prepare_cameras_with_centers
 from ..cameras import validate_camera_options
 from ..gs3d.api import _check_sh
+from ..features import FeatureDecoder
 from ..inputs import batch_item, normalize_inputs
 from ..statistics import StatisticsRequest, prepare_statistics
 from ..training import prepare_training_metadata
@@ -53,6 +54,11 @@ class RasterizationResult:
     def extra_features(self) -> Tensor | None:
         return self.meta.get("render_extra_signals")
 
+    @property
+    def decoded_features(self) -> Tensor | None:
+        """The feature decoder's image (None without a feature_decoder)."""
+        return self.meta.get("decoded_features")
+
 
 def validate_kernel_size(kernel_size) -> None:
     """rade/api.py:82-83."""
@@ -66,7 +72,8 @@ def rasterize(means: Tensor, quats: Tensor, scales: Tensor, opacities: Tensor, v
               backgrounds: Tensor | None = None, extra_features: Tensor | None = None,
               near_plane: float = 0.2, far_plane: float = math.inf, radius_clip: float = 0.0,
               kernel_size: float = 0.0, packed: bool = False, absgrad: bool = False,
-              statistics: Sequence[StatisticsRequest] = ()) -> RasterizationResult:
+              statistics: Sequence[StatisticsRequest] = (),
+              feature_decoder: FeatureDecoder | None = None) -> RasterizationResult:
     """Render RaDe-GS features, alpha, expected/median Z depth and normals.
 
     Inputs use OpenCV world-to-camera matrices and channel-last images.
@@ -75,7 +82,9 @@ def rasterize(means: Tensor, quats: Tensor, scales: Tensor, opacities: Tensor, v
     the last contributor whose incoming transmittance exceeds 0.5, normals
     unit camera-space vectors (zero where nothing was blended).  kernel_size
     dilates the 2D covariance and compensates opacity.  Intrinsics/background
-    gradients are unsupported.
+    gradients are unsupported.  feature_decoder (features.FeatureDecoder; no
+    counterpart in the reference) is called on the extra feature image, or on
+    the features without extras, and gives meta["decoded_features"].
     """
     validate_kernel_size(kernel_size)
     validate_camera_options(width, height, near_plane, far_plane, radius_clip)
@@ -178,6 +187,9 @@ def rasterize(means: Tensor, quats: Tensor, scales: Tensor, opacities: Tensor, v
         assemble(v) for v in zip(*images))
     if layout.extras is not None:
         meta["render_extra_signals"] = extra_image
+    if feature_decoder is not None:
+        meta["decoded_features"] = feature_decoder(
+            meta.get("render_extra_signals", main_features))
     meta.update(depth=depth, median_depth=median, normals=normals)
     return RasterizationResult(main_features, alpha, depth, median, normals, meta,
                                statistics_outputs)

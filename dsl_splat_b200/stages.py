@@ -669,3 +669,100 @@ def render_backward(state: ProjectedFootprint, bins: dict, feat_a: Tensor,
             ptr(gb), ptr(absolute), constant_tail, ptr(tile_order(bins)), nv.stream(a.device)),
             "render_backward")
     return centers, conics, ga, gb, absolute
+
+
+# ---- feature operators -------------------------------------------------------
+
+FEATURE_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATIONS = ("none", "relu", "silu", "gelu", "sigmoid")
+
+
+def _workspace(nbytes: int, like: Tensor) -> Tensor:
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+
+
+def feature_linear(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None,
+                   activation: str) -> Tensor:
+    """act(x weight^T + bias) + residual for x (M,K), weight (N,K)."""
+    pin = Args()
+    (m, k), n = x.shape, len(weight)
+    y = x.new_empty((m, n))
+    if y.numel():
+        with torch.cuda.device(x.device):
+            check(lib.splat_feature_linear(
+                FEATURE_DTYPES[x.dtype], m, k, n, pin(x), pin(weight), pin(bias), pin(residual),
+                ACTIVATIONS.index(activation), ptr(y), _stream(x)), "feature_linear")
+    return y
+
+
+def feature_linear_backward(x: Tensor, weight: Tensor, bias: Tensor | None, activation: str,
+                            upstream: Tensor, needs: tuple[bool, bool, bool]
+                            ) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
+    """Gradients of x, weight and bias (None where not needed)."""
+    pin = Args()
+    (m, k), n = x.shape, len(weight)
+    dx = x.new_empty((m, k)) if needs[0] else None
+    dweight = x.new_empty((n, k)) if needs[1] else None
+    dbias = x.new_empty((n,)) if needs[2] else None
+    if m == 0:
+        for g in (dweight, dbias):
+            if g is not None:
+                g.zero_()
+    elif any(needs):
+        dtype, act = FEATURE_DTYPES[x.dtype], ACTIVATIONS.index(activation)
+        size = lib.splat_feature_linear_backward_workspace_bytes(dtype, m, k, n, act)
+        ws = _workspace(size, x)
+        with torch.cuda.device(x.device):
+            check(lib.splat_feature_linear_backward(
+                dtype, m, k, n, pin(x), pin(weight), pin(bias), act, pin(upstream), ptr(dx),
+                ptr(dweight), ptr(dbias), ptr(ws), size, _stream(x)), "feature_linear_backward")
+    return dx, dweight, dbias
+
+
+def feature_norm(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None, eps: float,
+                 activation: str) -> tuple[Tensor, Tensor, Tensor]:
+    """Group norm with an activation of x (B,S,C): y and the (B,groups) fp32 mean
+    and reciprocal deviation."""
+    pin = Args()
+    samples, positions, channels = x.shape
+    y = torch.empty((samples, positions, channels), dtype=x.dtype, device=x.device)
+    mean, rstd = torch.empty((2, samples, groups), dtype=torch.float32, device=x.device)
+    if y.numel():
+        dtype = FEATURE_DTYPES[x.dtype]
+        size = lib.splat_feature_norm_workspace_bytes(dtype, samples, positions, channels,
+                                                      groups, 0)
+        ws = _workspace(size, x)
+        with torch.cuda.device(x.device):
+            check(lib.splat_feature_norm(
+                dtype, samples, positions, channels, groups, pin(x), pin(weight), pin(bias), eps,
+                ACTIVATIONS.index(activation), ptr(y), ptr(mean), ptr(rstd), ptr(ws), size,
+                _stream(x)), "feature_norm")
+    return y, mean, rstd
+
+
+def feature_norm_backward(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None,
+                          mean: Tensor, rstd: Tensor, activation: str, upstream: Tensor,
+                          needs: tuple[bool, bool, bool]
+                          ) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
+    """Gradients of x, weight and bias (None where not needed)."""
+    pin = Args()
+    samples, positions, channels = x.shape
+    dx = (torch.empty((samples, positions, channels), dtype=x.dtype, device=x.device)
+          if needs[0] else None)
+    dweight = x.new_empty((channels,)) if needs[1] else None
+    dbias = x.new_empty((channels,)) if needs[2] else None
+    if samples * positions == 0:
+        for g in (dweight, dbias):
+            if g is not None:
+                g.zero_()
+    elif any(needs):
+        dtype = FEATURE_DTYPES[x.dtype]
+        size = lib.splat_feature_norm_workspace_bytes(dtype, samples, positions, channels,
+                                                      groups, 1)
+        ws = _workspace(size, x)
+        with torch.cuda.device(x.device):
+            check(lib.splat_feature_norm_backward(
+                dtype, samples, positions, channels, groups, pin(x), pin(weight), pin(bias),
+                ptr(mean), ptr(rstd), ACTIVATIONS.index(activation), pin(upstream), ptr(dx),
+                ptr(dweight), ptr(dbias), ptr(ws), size, _stream(x)), "feature_norm_backward")
+    return dx, dweight, dbias

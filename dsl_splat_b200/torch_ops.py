@@ -27,6 +27,8 @@ Operator <- reference code it stands for:
   rade_project_backward  rade/projection.py:475-551
   rade_render         rade/render.py:550-601 (colour, alpha, depths, normals)
   rade_render_backward   rade/render.py:604-670
+  feature_linear, feature_norm and their _backward: no counterpart (features.linear,
+                      features.group_norm)
 """
 
 from __future__ import annotations
@@ -498,7 +500,90 @@ def _rade_render_backward(ctx, g_feat, g_alpha, g_depth, g_median, g_normals, g_
 
 rade_render.register_autograd(_rade_render_backward, setup_context=_rade_render_setup)
 
+
+# ---- feature operators ----------------------------------------------------------
+
+@torch.library.custom_op(f"{_NS}::feature_linear", mutates_args=())
+def feature_linear(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None,
+                   activation: str) -> Tensor:
+    return stages.feature_linear(x, weight, bias, residual, activation)
+
+
+@feature_linear.register_fake
+def _(x, weight, bias, residual, activation):
+    return x.new_empty((x.shape[0], weight.shape[0]))
+
+
+@torch.library.custom_op(f"{_NS}::feature_linear_backward", mutates_args=())
+def feature_linear_backward(x: Tensor, weight: Tensor, bias: Tensor | None, activation: str,
+                            upstream: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    return stages.feature_linear_backward(x, weight, bias, activation, upstream,
+                                          (True, True, True))
+
+
+@feature_linear_backward.register_fake
+def _(x, weight, bias, activation, upstream):
+    return x.new_empty(x.shape), weight.new_empty(weight.shape), x.new_empty((weight.shape[0],))
+
+
+def _feature_linear_setup(ctx, inputs, output):
+    x, weight, bias, residual, ctx.activation = inputs
+    ctx.save_for_backward(x, weight, bias)
+    ctx.with_residual = residual is not None
+
+
+def _feature_linear_backward(ctx, upstream):
+    x, weight, bias = ctx.saved_tensors
+    dx, dw, db = torch.ops.splat200.feature_linear_backward(x, weight, bias, ctx.activation,
+                                                            upstream)
+    return (dx, dw, None if bias is None else db, upstream if ctx.with_residual else None, None)
+
+
+feature_linear.register_autograd(_feature_linear_backward, setup_context=_feature_linear_setup)
+
+
+@torch.library.custom_op(f"{_NS}::feature_norm", mutates_args=())
+def feature_norm(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None, eps: float,
+                 activation: str) -> tuple[Tensor, Tensor, Tensor]:
+    y, mean, rstd = stages.feature_norm(x, groups, weight, bias, eps, activation)
+    return y, mean, rstd.clone()  # an operator's outputs share no storage
+
+
+@feature_norm.register_fake
+def _(x, groups, weight, bias, eps, activation):
+    moments = x.new_empty((x.shape[0], groups), dtype=torch.float32)
+    return x.new_empty(x.shape), moments, torch.empty_like(moments)
+
+
+@torch.library.custom_op(f"{_NS}::feature_norm_backward", mutates_args=())
+def feature_norm_backward(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None,
+                          mean: Tensor, rstd: Tensor, activation: str, upstream: Tensor
+                          ) -> tuple[Tensor, Tensor, Tensor]:
+    return stages.feature_norm_backward(x, groups, weight, bias, mean, rstd, activation,
+                                        upstream, (True, True, True))
+
+
+@feature_norm_backward.register_fake
+def _(x, groups, weight, bias, mean, rstd, activation, upstream):
+    return (x.new_empty(x.shape), x.new_empty((x.shape[-1],)), x.new_empty((x.shape[-1],)))
+
+
+def _feature_norm_setup(ctx, inputs, output):
+    x, ctx.groups, weight, bias, _eps, ctx.activation = inputs
+    ctx.save_for_backward(x, weight, bias, output[1], output[2])
+
+
+def _feature_norm_backward(ctx, upstream, _mean, _rstd):
+    x, weight, bias, mean, rstd = ctx.saved_tensors
+    dx, dw, db = torch.ops.splat200.feature_norm_backward(x, ctx.groups, weight, bias, mean,
+                                                          rstd, ctx.activation, upstream)
+    return (dx, None, None if weight is None else dw, None if bias is None else db, None, None)
+
+
+feature_norm.register_autograd(_feature_norm_backward, setup_context=_feature_norm_setup)
+
 OPERATORS = ("cameras_prepare", "project", "project_backward", "project_views",
              "project_views_backward", "sh_forward", "sh_backward", "bin_and_sort", "render",
              "render_backward", "rade_project", "rade_project_backward", "rade_render",
-             "rade_render_backward")
+             "rade_render_backward", "feature_linear", "feature_linear_backward", "feature_norm",
+             "feature_norm_backward")

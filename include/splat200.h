@@ -564,6 +564,48 @@ int splat_aaa_camera_backward(const SplatAaaFrame* frame, const int* radii,
 /* Diagnostic: ours[i] = the blend's exp, cuda_exp[i] = CUDA expf, for x (n). */
 int splat_debug_expf(int n, const float* x, float* ours, float* cuda_exp, void* stream);
 
+/* ---- feature operators ----------------------------------------------------
+ * No counterpart in the reference: what decodes blended feature images
+ * (channel-last rows of pixels) and per-Gaussian features.  dtype of every
+ * tensor of a call: 0 float32, 1 bfloat16, 2 float16 (row-major, contiguous,
+ * 16-byte aligned bases).  activation: 0 none, 1 relu, 2 silu, 3 gelu (erf),
+ * 4 sigmoid.  Sums are held in fp32 or more and rounded once, so results do
+ * not depend on the order in which blocks run. */
+
+/* y = act(x weight^T + bias) + residual; x (rows, k), weight (n, k), bias (n)
+ * or NULL, residual (rows, n) or NULL, y (rows, n). */
+int splat_feature_linear(int dtype, long long rows, int k, int n, const void* x,
+                         const void* weight, const void* bias, const void* residual,
+                         int activation, void* y, void* stream);
+
+/* Gradients of the above for the upstream dy (rows, n): dx (rows, k),
+ * dweight (n, k), dbias (n), each NULL to skip it (the residual's gradient is
+ * dy).  The pre-activation is recomputed from x, weight and bias. */
+size_t splat_feature_linear_backward_workspace_bytes(int dtype, long long rows, int k, int n,
+                                                     int activation);
+int splat_feature_linear_backward(int dtype, long long rows, int k, int n, const void* x,
+                                  const void* weight, const void* bias, int activation,
+                                  const void* dy, void* dx, void* dweight, void* dbias,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* y = act((x - mean) rstd weight_c + bias_c); x, y (samples, positions,
+ * channels); mean and rstd (samples, groups) float32 over the positions of a
+ * sample and the channels of a group, written for the backward; weight, bias
+ * (channels) or NULL. */
+size_t splat_feature_norm_workspace_bytes(int dtype, int samples, long long positions,
+                                          int channels, int groups, int backward);
+int splat_feature_norm(int dtype, int samples, long long positions, int channels, int groups,
+                       const void* x, const void* weight, const void* bias, float eps,
+                       int activation, void* y, float* mean, float* rstd, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* Gradients of the above for dy: dx, dweight, dbias, each NULL to skip it. */
+int splat_feature_norm_backward(int dtype, int samples, long long positions, int channels,
+                                int groups, const void* x, const void* weight, const void* bias,
+                                const float* mean, const float* rstd, int activation,
+                                const void* dy, void* dx, void* dweight, void* dbias,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
