@@ -38,7 +38,7 @@ SOURCES = {"splat200.cu": ["-fmad=false"],
 HEADERS = ["splat_common.cuh", "cameras.cuh", "project.cuh", "binning.cuh", "render.cuh",
            "footprint.cuh", "tile_modes.cuh", "host_runtime.h", "rade.cuh", "rade_project.cuh",
            "aaa.cuh", "aaa_render.cuh", "aaa_api.cuh", "aaa_blend_params.cuh",
-           "aaa_backward.cuh", "feature_common.cuh"]
+           "aaa_backward.cuh", "feature_common.cuh", "feature_product.cuh", "tensor_core.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

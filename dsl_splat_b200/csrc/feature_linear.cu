@@ -10,105 +10,122 @@
 #include <algorithm>
 
 #include "feature_common.cuh"
+#include "feature_product.cuh"
 #include "host_runtime.h"
 #include "splat200.h"
 
 namespace splat {
 namespace feature {
 
-constexpr int kTileM = 64, kTileN = 64, kTileK = 16;
+// ---- launching a product -------------------------------------------------------
 
-// C(i, j) = sum_k A(i, k) B(j, k) with element strides, in 64x64 tiles of
-// fp32 sums; blockIdx.z takes a range of k and then writes fp32 partial sums.
-struct ProductParams {
-  long long m, k;
-  int n;
-  const void* a;
-  long long a_row, a_k;
-  const void* b;
-  long long b_row, b_k;
-  long long k_per_split;
-  // epilogue
-  const void* bias;      // (n), added to C
-  const void* residual;  // (m, n), added after the activation
-  const void* dy;        // (m, n): C becomes dy * act'(C)
-  void* out;             // (m, n); (splits, m, n) fp32 with several splits
-};
+// The widest of 16, 8, 4 and 2 bytes that rows of ld values start on.
+template <class S>
+int row_vector(const void* base, long long ld) {
+  int v = 16;
+  while (v > static_cast<int>(sizeof(S)) &&
+         ((ld * static_cast<long long>(sizeof(S))) % v || !host::aligned(base, v)))
+    v /= 2;
+  return v;
+}
 
-enum Epilogue : int { kForward = 0, kSlope = 1, kPlain = 2 };
+// Shared memory of a block when one or two share an SM (228 KB, of which each
+// block costs 1 KB besides its own), less the barriers and the rounding of the
+// base to 1 KB.
+constexpr int kOneBlockBytes = 225 * 1024, kTwoBlocksBytes = 110 * 1024;
+constexpr int kMaxResidentBytes = 128 * 1024;
 
-template <class TA, class TB, class TO, int EPI, int ACT>
-__global__ void __launch_bounds__(256) product_kernel(const ProductParams p) {
-  __shared__ float as[kTileK][kTileM + 1], bs[kTileK][kTileN + 1];
-  const TA* a = static_cast<const TA*>(p.a);
-  const TB* b = static_cast<const TB*>(p.b);
-  const long long row0 = static_cast<long long>(blockIdx.x) * kTileM;
-  const int col0 = blockIdx.y * kTileN;
-  const long long k_begin = blockIdx.z * p.k_per_split;
-  const long long k_end = min(k_begin + p.k_per_split, p.k);
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  float acc[4][4] = {};
-  for (long long k0 = k_begin; k0 < k_end; k0 += kTileK) {
-    for (int i = threadIdx.x; i < kTileM * kTileK; i += 256) {
-      // neighbouring threads take neighbouring addresses of either layout
-      const int r = p.a_k == 1 ? i / kTileK : i % kTileM;
-      const int k = p.a_k == 1 ? i % kTileK : i / kTileM;
-      const bool in = row0 + r < p.m && k0 + k < k_end;
-      as[k][r] = in ? to_float(a[(row0 + r) * p.a_row + (k0 + k) * p.a_k]) : 0.0f;
-    }
-    for (int i = threadIdx.x; i < kTileN * kTileK; i += 256) {
-      const int r = p.b_k == 1 ? i / kTileK : i % kTileN;
-      const int k = p.b_k == 1 ? i % kTileK : i / kTileN;
-      const bool in = col0 + r < p.n && k0 + k < k_end;
-      bs[k][r] = in ? to_float(b[(col0 + r) * p.b_row + (k0 + k) * p.b_k]) : 0.0f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kTileK; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += as[k][ty * 4 + i] * bs[k][tx * 4 + j];
-    __syncthreads();
-  }
-  TO* out = static_cast<TO*>(p.out) + blockIdx.z * p.m * p.n;
-  for (int i = 0; i < 4; ++i) {
-    const long long row = row0 + ty * 4 + i;
-    if (row >= p.m) break;
-    for (int j = 0; j < 4; ++j) {
-      const int col = col0 + tx * 4 + j;
-      if (col >= p.n) break;
-      float z = acc[i][j];
-      if (p.bias) z += to_float(static_cast<const TB*>(p.bias)[col]);
-      if constexpr (EPI == kForward) {
-        z = activate<ACT>(z);
-        if (p.residual) z += to_float(static_cast<const TA*>(p.residual)[row * p.n + col]);
-      }
-      if constexpr (EPI == kSlope)
-        z = to_float(static_cast<const TA*>(p.dy)[row * p.n + col]) * slope<ACT>(z);
-      out[row * p.n + col] = from_float<TO>(z);
-    }
+// Fills in the tiling of p (its sources, sizes and epilogue set) and launches.
+template <class SA, int PA, bool AMN, class SB, int PB, bool BMN, class TE, class TO, int EPI>
+int launch_product(ProductParams p, cudaStream_t s) {
+  const int widest = PA == 1 && PB == 1 ? 256 : 128;
+  p.tiles_n = (p.n + widest - 1) / widest;
+  p.tile_n = ((p.n + p.tiles_n - 1) / p.tiles_n + 31) / 32 * 32;
+  p.tiles_m = (p.m + kTileRows - 1) / kTileRows;
+  p.tiles = p.tiles_m * p.tiles_n * p.splits;
+  p.a_vector = row_vector<SA>(p.a, p.a_ld);
+  p.b_vector = row_vector<SB>(p.b, p.b_ld);
+  constexpr int V = sizeof(TE) == 2 ? 8 : 4;
+  p.out_vector = p.n % V == 0 && host::aligned(p.bias, 16) && host::aligned(p.extra, 16) &&
+                 host::aligned(p.out, 16);
+  p.tmem_columns = 32;
+  constexpr int kAcc = accumulators(PA, PB);
+  while (p.tmem_columns < 2u * kAcc * p.tile_n) p.tmem_columns *= 2;
+  // sums of several accumulators are joined in fp32 outputs; an operand row of
+  // more values than kExactSum is summed in one
+  p.k_per_sum = kAcc == 2 && EPI == kPlain && sizeof(TO) == 4 ? kExactSum : p.k_per_split;
+  const int b_bytes = PB * b_plane_bytes<BMN>(p.tile_n), a_bytes = PA * kAPlane;
+  const long long chunks = (p.k + kChunk - 1) / kChunk;
+  const long long whole_b = chunks * b_bytes;
+  p.resident = p.splits == 1 && p.tiles_n == 1 && whole_b <= kMaxResidentBytes;
+  const int fixed = kEpilogueWarps * kStagingBytes + (p.resident ? static_cast<int>(whole_b) : 0);
+  const int stage = a_bytes + (p.resident ? 0 : b_bytes);
+  int blocks = 2, budget = kTwoBlocksBytes;
+  if (producers(PA, PB) > 128 || p.tmem_columns > 256 || fixed + 2 * stage > budget)
+    blocks = 1, budget = kOneBlockBytes;
+  p.stages = std::min(kMaxStages, (budget - fixed) / stage);
+  if (p.stages < 1) return host::fail(kTooLarge, "feature_linear: no room for a stage");
+  const bool copied = PA == 1 && PB == 1 && p.a_vector == 16 &&
+                      (p.resident || p.b_vector == 16) && sizeof(SA) == 2;
+  p.lag = copied ? p.stages - 1 : 0;
+  p.error = host::device_error_word();
+  if (!p.error) return kCudaError;
+  const int bytes = fixed + p.stages * stage + 1024;
+  auto* kernel = product_kernel<SA, PA, AMN, SB, PB, BMN, TE, TO, EPI>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+      cudaSuccess)
+    return host::check_launch("feature_linear: shared memory");
+  const long long grid = std::min<long long>(p.tiles, host::sm_count() * blocks);
+  kernel<<<static_cast<unsigned>(grid), kEpilogueWarps * 32 + producers(PA, PB) + 32, bytes, host::counted(s)>>>(p);
+  return host::check_launch("feature_linear");
+}
+
+// Parts of an operand that is T in memory (beside a one-part operand f16 goes
+// as it is), and of the fp32 dz: a 16-bit gradient's products take dz in two
+// parts (2^-16), so that it is rounded once, at the end.
+template <class T>
+constexpr int kSourceParts = sizeof(T) == 4 ? 3 : kIsF16<T> ? 2 : 1;
+template <class T>
+constexpr int kNativeParts = sizeof(T) == 4 ? 3 : 1;
+template <class T>
+constexpr int kGradientParts = sizeof(T) == 4 ? 3 : 2;
+
+// ---- sums over splits and rows ---------------------------------------------------
+
+// Adds the splits' partial sums in a fixed order: 8 threads to a value.
+template <class T>
+__global__ void __launch_bounds__(256)
+    join_splits_kernel(const float* partial, long long count, int splits, T* out) {
+  const long long i = blockIdx.x * 32LL + threadIdx.x;
+  float s = 0.0f;
+  if (i < count)
+    for (int k = threadIdx.y; k < splits; k += 8) s += partial[k * count + i];
+  __shared__ float sums[8][32];
+  sums[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && i < count) {
+    for (int k = 1; k < 8; ++k) s += sums[k][threadIdx.x];
+    out[i] = from_float<T>(s);
   }
 }
 
-// Adds the splits' partial sums in order.
 template <class T>
-__global__ void join_splits_kernel(const float* partial, long long count, int splits, T* out) {
-  const long long i = blockIdx.x * 256LL + threadIdx.x;
-  if (i >= count) return;
-  float s = 0.0f;
-  for (int k = 0; k < splits; ++k) s += partial[k * count + i];
-  out[i] = from_float<T>(s);
+void join_splits(const float* partial, long long count, int splits, void* out, cudaStream_t s) {
+  join_splits_kernel<T><<<host::blocks_for(count, 32), dim3(32, 8), 0, host::counted(s)>>>(
+      partial, count, splits, static_cast<T*>(out));
 }
 
 // Column sums of dz (m, n) over ranges of rows.
-__global__ void column_sums_kernel(const float* dz, long long m, int n, long long rows,
-                                   float* partial) {
+template <class S>
+__global__ void __launch_bounds__(256) column_sums_kernel(const S* dz, long long m, int n,
+                                                          long long rows, float* partial) {
   const int c = blockIdx.x * 32 + threadIdx.x;
   const long long begin = blockIdx.y * rows, end = min(begin + rows, m);
   float s = 0.0f;
-  if (c < n)
-    for (long long r = begin + threadIdx.y; r < end; r += 8) s += dz[r * n + c];
+  if (c < n) {
+#pragma unroll 8
+    for (long long r = begin + threadIdx.y; r < end; r += 8) s += to_float(dz[r * n + c]);
+  }
   __shared__ float sums[8][32];
   sums[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
@@ -128,13 +145,76 @@ int check_linear(int dtype, long long rows, int k, int n, int activation) {
   return kOk;
 }
 
-constexpr int kMaxSplits = 256;
-
-int dweight_splits(long long rows) {
-  return static_cast<int>(std::min<long long>(kMaxSplits, (rows + 4095) / 4096));
+// Ranges of rows whose sums of dz^T x (and of dz) are joined afterwards:
+// enough tiles for two blocks on every SM, 512 rows to a range at least.
+struct Splits {
+  int count;
+  long long rows;
+};
+Splits weight_splits(long long rows, int k, int n) {
+  const long long tiles = ((n + 127LL) / 128) * ((k + 127) / 128);
+  const long long wanted = std::max(1LL, 2LL * host::sm_count() / tiles);
+  const long long most = (rows + 511) / 512;
+  const long long per = (rows + std::min(wanted, most) - 1) / std::min(wanted, most);
+  Splits s;
+  s.rows = (per + kChunk - 1) / kChunk * kChunk;
+  s.count = static_cast<int>((rows + s.rows - 1) / s.rows);
+  return s;
 }
 
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
+size_t dz_bytes(long long rows, int n, int activation) {
+  return activation == kNone ? 0 : round16(static_cast<size_t>(rows) * n * 4);
+}
+
+// The two products of the backward, from dz as S.
+template <class T, class S, int PZ, int PT>
+int launch_gradients(long long rows, int k, int n, const S* dz, const void* x,
+                     const void* weight, void* dx, void* dweight, void* dbias, float* partial,
+                     cudaStream_t s) {
+  if (dx) {
+    ProductParams p{};
+    p.m = rows, p.k = n, p.n = k;
+    p.a = dz, p.a_ld = n;
+    p.b = weight, p.b_ld = k;
+    p.k_per_split = n, p.splits = 1;
+    p.out = dx;
+    const int status = launch_product<S, PZ, false, T, PT, true, T, T, kPlain>(p, s);
+    if (status != kOk) return status;
+  }
+  const Splits splits = weight_splits(rows, k, n);
+  if (dweight) {
+    ProductParams p{};
+    p.m = n, p.k = rows, p.n = k;
+    p.a = dz, p.a_ld = n;
+    p.b = x, p.b_ld = k;
+    p.k_per_split = splits.rows, p.splits = splits.count;
+    p.out = partial;
+    const int status = launch_product<S, PZ, true, T, PT, true, float, float, kPlain>(p, s);
+    if (status != kOk) return status;
+    join_splits<T>(partial, static_cast<long long>(n) * k, splits.count, dweight, s);
+  }
+  if (dbias) {
+    float* sums = partial + static_cast<long long>(splits.count) * n * k;
+    column_sums_kernel<S><<<dim3(host::blocks_for(n, 32), splits.count), dim3(32, 8), 0,
+                            host::counted(s)>>>(dz, rows, n, splits.rows, sums);
+    join_splits<T>(sums, n, splits.count, dbias, s);
+  }
+  return host::check_launch("feature_linear_backward");
+}
+
+template <class T>
+ProductParams forward_params(long long rows, int k, int n, const void* x, const void* weight,
+                             const void* bias, const void* extra, int activation, void* out) {
+  ProductParams p{};
+  p.m = rows, p.k = k, p.n = n;
+  p.a = x, p.a_ld = k;
+  p.b = weight, p.b_ld = k;
+  p.k_per_split = k, p.splits = 1;
+  p.bias = bias, p.extra = extra, p.activation = activation, p.out = out;
+  return p;
+}
 
 }  // namespace feature
 }  // namespace splat
@@ -150,27 +230,20 @@ int splat_feature_linear(int dtype, long long rows, int k, int n, const void* x,
   const int bad = check_linear(dtype, rows, k, n, activation);
   if (bad != kOk) return bad;
   if (!x || !weight || !y) return host::fail(kInvalidArgument, "feature_linear: null pointer");
-  ProductParams p{};
-  p.m = rows, p.k = k, p.n = n;
-  p.a = x, p.a_row = k, p.a_k = 1;
-  p.b = weight, p.b_row = k, p.b_k = 1;
-  p.k_per_split = k;
-  p.bias = bias, p.residual = residual, p.out = y;
-  const dim3 grid(host::blocks_for(rows, kTileM), host::blocks_for(n, kTileN));
   auto s = static_cast<cudaStream_t>(stream);
   return SPLAT_FEATURE_TYPE(dtype, [&] {
-    return SPLAT_FEATURE_ACT(activation, [&] {
-      product_kernel<T, T, T, kForward, ACT><<<grid, 256, 0, host::counted(s)>>>(p);
-      return host::check_launch("feature_linear");
-    });
+    constexpr int P = kNativeParts<T>;
+    return launch_product<T, P, false, T, P, false, T, T, kForward>(
+        forward_params<T>(rows, k, n, x, weight, bias, residual, activation, y), s);
   });
 }
 
 size_t splat_feature_linear_backward_workspace_bytes(int dtype, long long rows, int k, int n,
                                                      int activation) {
   if (check_linear(dtype, rows, k, n, activation) != kOk) return 0;
-  const size_t splits = dweight_splits(rows);
-  return round16(static_cast<size_t>(rows) * n * 4) + splits * n * (static_cast<size_t>(k) + 1) * 4;
+  const Splits splits = weight_splits(rows, k, n);
+  return dz_bytes(rows, n, activation) +
+         static_cast<size_t>(splits.count) * n * (static_cast<size_t>(k) + 1) * 4;
 }
 
 int splat_feature_linear_backward(int dtype, long long rows, int k, int n, const void* x,
@@ -181,57 +254,25 @@ int splat_feature_linear_backward(int dtype, long long rows, int k, int n, const
   if (bad != kOk) return bad;
   if (!x || !weight || !dy || !workspace)
     return host::fail(kInvalidArgument, "feature_linear_backward: null pointer");
+  if (!host::aligned(workspace, 16))
+    return host::fail(kInvalidArgument, "feature_linear_backward: workspace not 16-byte aligned");
   if (workspace_bytes <
       splat_feature_linear_backward_workspace_bytes(dtype, rows, k, n, activation))
     return host::fail(kWorkspaceTooSmall, "feature_linear_backward: workspace");
   auto s = static_cast<cudaStream_t>(stream);
   float* dz = static_cast<float*>(workspace);
-  float* partial =
-      reinterpret_cast<float*>(static_cast<char*>(workspace) + round16(rows * n * 4));
-  const int splits = dweight_splits(rows);
-  const long long rows_per_split = (rows + splits - 1) / splits;
+  float* partial = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                            dz_bytes(rows, n, activation));
   return SPLAT_FEATURE_TYPE(dtype, [&] {
-    ProductParams p{};
-    p.m = rows, p.k = k, p.n = n;
-    p.a = x, p.a_row = k, p.a_k = 1;
-    p.b = weight, p.b_row = k, p.b_k = 1;
-    p.k_per_split = k;
-    p.bias = bias, p.dy = dy, p.out = dz;
-    SPLAT_FEATURE_ACT(activation, [&] {
-      const dim3 grid(host::blocks_for(rows, kTileM), host::blocks_for(n, kTileN));
-      product_kernel<T, T, float, kSlope, ACT><<<grid, 256, 0, host::counted(s)>>>(p);
-    });
-    if (dx) {
-      ProductParams q{};
-      q.m = rows, q.k = n, q.n = k;
-      q.a = dz, q.a_row = n, q.a_k = 1;
-      q.b = weight, q.b_row = 1, q.b_k = k;
-      q.k_per_split = n;
-      q.out = dx;
-      const dim3 grid(host::blocks_for(rows, kTileM), host::blocks_for(k, kTileN));
-      product_kernel<float, T, T, kPlain, kNone><<<grid, 256, 0, host::counted(s)>>>(q);
-    }
-    if (dweight) {
-      ProductParams q{};
-      q.m = n, q.k = rows, q.n = k;
-      q.a = dz, q.a_row = 1, q.a_k = n;
-      q.b = x, q.b_row = 1, q.b_k = k;
-      q.k_per_split = rows_per_split;
-      q.out = partial;
-      const dim3 grid(host::blocks_for(n, kTileM), host::blocks_for(k, kTileN), splits);
-      product_kernel<float, T, float, kPlain, kNone><<<grid, 256, 0, host::counted(s)>>>(q);
-      const long long count = static_cast<long long>(n) * k;
-      join_splits_kernel<T><<<host::blocks_for(count, 256), 256, 0, host::counted(s)>>>(
-          partial, count, splits, static_cast<T*>(dweight));
-    }
-    if (dbias) {
-      float* sums = partial + static_cast<long long>(splits) * n * k;
-      column_sums_kernel<<<dim3(host::blocks_for(n, 32), splits), dim3(32, 8), 0,
-                           host::counted(s)>>>(dz, rows, n, rows_per_split, sums);
-      join_splits_kernel<T><<<host::blocks_for(n, 256), 256, 0, host::counted(s)>>>(
-          sums, n, splits, static_cast<T*>(dbias));
-    }
-    return host::check_launch("feature_linear_backward");
+    constexpr int P = kNativeParts<T>;
+    if (activation == kNone)  // dz is dy
+      return launch_gradients<T, T, P, P>(rows, k, n, static_cast<const T*>(dy), x, weight, dx,
+                                          dweight, dbias, partial, s);
+    const int status = launch_product<T, P, false, T, P, false, T, float, kSlope>(
+        forward_params<T>(rows, k, n, x, weight, bias, dy, activation, dz), s);
+    if (status != kOk) return status;
+    return launch_gradients<T, float, kGradientParts<T>, kSourceParts<T>>(
+        rows, k, n, dz, x, weight, dx, dweight, dbias, partial, s);
   });
 }
 

@@ -17,6 +17,9 @@ int check_launch(const char* what);
 // Counts one kernel launch and returns its stream; every launch passes its
 // stream through here.
 cudaStream_t counted(cudaStream_t s);
+// The current device's error word (splat_device_error), or NULL with the CUDA
+// error recorded.
+int* device_error_word();
 // Streaming multiprocessors of the current device (148 on B200).
 int sm_count();
 

@@ -54,6 +54,15 @@ cudaStream_t counted(cudaStream_t s) {
   return s;
 }
 
+int* device_error_word() {
+  void* word = nullptr;
+  if (cudaGetSymbolAddress(&word, g_splat_device_error) != cudaSuccess) {
+    check_launch("device_error_word");
+    return nullptr;
+  }
+  return static_cast<int*>(word);
+}
+
 int sm_count() {
   int sms = 148, dev = 0;
   if (cudaGetDevice(&dev) == cudaSuccess)
