@@ -32,6 +32,11 @@ SPLAT_DEV bf16 from_float<bf16>(float v) { return __float2bfloat16_rn(v); }
 template <>
 SPLAT_DEV f16 from_float<f16>(float v) { return __float2half_rn(v); }
 
+template <class T>
+constexpr bool kIsF16 = false;
+template <>
+inline constexpr bool kIsF16<f16> = true;
+
 // V consecutive values, loaded and stored as one access of V * sizeof(T)
 // bytes (at most 16), which the address must be a multiple of.
 template <class T, int V>
@@ -39,16 +44,93 @@ struct alignas(sizeof(T) * V) Vec {
   T v[V];
 };
 
-// 1 / (1 + exp(-z)): exp2 of a scaled argument and a reciprocal, each within
-// a few units of 2^-23; exp(-z) overflowing to infinity gives 0.
-SPLAT_DEV float logistic(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+// The same for V values at once: 16-bit ones are rounded in pairs.
+template <class T, int V>
+SPLAT_DEV Vec<T, V> round_values(const float (&v)[V]) {
+  Vec<T, V> r;
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) {
+      if constexpr (kIsF16<T>) {
+        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = reinterpret_cast<const uint32_t&>(h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = reinterpret_cast<const uint32_t&>(h);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) r.v[j] = from_float<T>(v[j]);
+  }
+  return r;
+}
+
+template <class T, int V>
+SPLAT_DEV void widen(const Vec<T, V>& r, float (&v)[V]) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) {
+      if constexpr (kIsF16<T>) {
+        const float2 f = __half22float2(reinterpret_cast<const __half2&>(w[j]));
+        v[2 * j] = f.x;
+        v[2 * j + 1] = f.y;
+      } else {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = to_float(r.v[j]);
+  }
+}
+
+// 2^x and 1/x in one instruction each, within 2 units of 2^-23; results below
+// the normal range are 0.
+SPLAT_DEV float fast_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+SPLAT_DEV float fast_reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// 1 / (1 + exp(-z)); exp(-z) overflowing to infinity gives 0.
+SPLAT_DEV float logistic(float z) {
+  return fast_reciprocal(1.0f + fast_exp2(z * -1.44269504088896341f));
+}
+
+// The normal distribution's upper tail at |z| and its density: with
+// x = |z| / sqrt 2 and t = 1 / (1 + 0.3275911 x), erfc(x) is
+// t (a1 + a2 t + .. + a5 t^4) exp(-x^2) within 1.5e-7 (Abramowitz and Stegun,
+// Handbook of Mathematical Functions, 7.1.26).
+SPLAT_DEV void normal_tail(float z, float& tail, float& density) {
+  const float e = fast_exp2(z * z * -0.72134752044448170f);
+  const float t = fast_reciprocal(__fmaf_rn(fabsf(z), 0.23164189f, 1.0f));
+  float q = __fmaf_rn(t, 1.061405429f, -1.453152027f);
+  q = __fmaf_rn(q, t, 1.421413741f);
+  q = __fmaf_rn(q, t, -0.284496736f);
+  q = __fmaf_rn(q, t, 0.254829592f);
+  tail = 0.5f * q * t * e;
+  density = 0.39894228040143268f * e;
+}
 
 // NaN passes through every activation.
 template <int ACT>
 SPLAT_DEV float activate(float z) {
   if constexpr (ACT == kRelu) return z < 0.0f ? 0.0f : z;
   if constexpr (ACT == kSilu) return z * logistic(z);
-  if constexpr (ACT == kGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+  if constexpr (ACT == kGelu) {
+    float tail, density;
+    normal_tail(z, tail, density);
+    return z * (z < 0.0f ? tail : 1.0f - tail);
+  }
   if constexpr (ACT == kSigmoid) return logistic(z);
   return z;
 }
@@ -61,14 +143,37 @@ SPLAT_DEV float slope(float z) {
     const float s = logistic(z);
     return s * (1.0f + z * (1.0f - s));
   }
-  if constexpr (ACT == kGelu)
-    return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) +
-           z * 0.39894228040143268f * __expf(-0.5f * z * z);
+  if constexpr (ACT == kGelu) {
+    float tail, density;
+    normal_tail(z, tail, density);
+    return (z < 0.0f ? tail : 1.0f - tail) + z * density;
+  }
   if constexpr (ACT == kSigmoid) {
     const float s = logistic(z);
     return s * (1.0f - s);
   }
   return 1.0f;
+}
+
+// Packed pairs: one instruction for both where there is one.
+SPLAT_DEV void logistic2(float& a, float& b) {
+  unpack2(mul2(pack2(a, b), pack2(-1.44269504088896341f, -1.44269504088896341f)), a, b);
+  unpack2(add2(pack2(fast_exp2(a), fast_exp2(b)), pack2(1.0f, 1.0f)), a, b);
+  a = fast_reciprocal(a);
+  b = fast_reciprocal(b);
+}
+template <int ACT>
+SPLAT_DEV void activate2(float& a, float& b) {
+  if constexpr (ACT == kSilu) {
+    float s = a, t = b;
+    logistic2(s, t);
+    unpack2(mul2(pack2(a, b), pack2(s, t)), a, b);
+  } else if constexpr (ACT == kSigmoid) {
+    logistic2(a, b);
+  } else {
+    a = activate<ACT>(a);
+    b = activate<ACT>(b);
+  }
 }
 
 }  // namespace feature

@@ -33,6 +33,7 @@ int row_vector(const void* base, long long ld) {
 // block costs 1 KB besides its own), less the barriers and the rounding of the
 // base to 1 KB.
 constexpr int kOneBlockBytes = 225 * 1024, kTwoBlocksBytes = 110 * 1024;
+constexpr int kMaxSharedBias = 4096;  // values
 constexpr int kMaxResidentBytes = 128 * 1024;
 
 // Fills in the tiling of p (its sources, sizes and epilogue set) and launches.
@@ -41,13 +42,18 @@ int launch_product(ProductParams p, cudaStream_t s) {
   const int widest = PA == 1 && PB == 1 ? 256 : 128;
   p.tiles_n = (p.n + widest - 1) / widest;
   p.tile_n = ((p.n + p.tiles_n - 1) / p.tiles_n + 31) / 32 * 32;
-  p.tiles_m = (p.m + kTileRows - 1) / kTileRows;
+  const long long tiles_m = (p.m + kTileRows - 1) / kTileRows;
+  if (tiles_m * p.tiles_n * p.splits >= 1LL << 31)
+    return host::fail(kTooLarge, "feature_linear: too many tiles");
+  p.tiles_m = static_cast<uint32_t>(tiles_m);
   p.tiles = p.tiles_m * p.tiles_n * p.splits;
   p.a_vector = row_vector<SA>(p.a, p.a_ld);
   p.b_vector = row_vector<SB>(p.b, p.b_ld);
-  constexpr int V = sizeof(TE) == 2 ? 8 : 4;
-  p.out_vector = p.n % V == 0 && host::aligned(p.bias, 16) && host::aligned(p.extra, 16) &&
-                 host::aligned(p.out, 16);
+  p.extra_vector =
+      p.n * static_cast<long long>(sizeof(TE)) % 16 == 0 && host::aligned(p.extra, 16);
+  p.out_vector = p.n * static_cast<long long>(sizeof(TO)) % 16 == 0 && host::aligned(p.out, 16);
+  const int columns = static_cast<int>(p.tiles_n) * p.tile_n;
+  p.bias_shared = p.bias && columns <= kMaxSharedBias ? columns : 0;
   p.tmem_columns = 32;
   constexpr int kAcc = accumulators(PA, PB);
   while (p.tmem_columns < 2u * kAcc * p.tile_n) p.tmem_columns *= 2;
@@ -58,7 +64,7 @@ int launch_product(ProductParams p, cudaStream_t s) {
   const long long chunks = (p.k + kChunk - 1) / kChunk;
   const long long whole_b = chunks * b_bytes;
   p.resident = p.splits == 1 && p.tiles_n == 1 && whole_b <= kMaxResidentBytes;
-  const int fixed = kEpilogueWarps * kStagingBytes + (p.resident ? static_cast<int>(whole_b) : 0);
+  const int fixed = kEpilogueWarps * kStagingBytes + (p.bias_shared * 4 + 1023) / 1024 * 1024 + (p.resident ? static_cast<int>(whole_b) : 0);
   const int stage = a_bytes + (p.resident ? 0 : b_bytes);
   int blocks = 2, budget = kTwoBlocksBytes;
   if (producers(PA, PB) > 128 || p.tmem_columns > 256 || fixed + 2 * stage > budget)
@@ -75,7 +81,7 @@ int launch_product(ProductParams p, cudaStream_t s) {
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
       cudaSuccess)
     return host::check_launch("feature_linear: shared memory");
-  const long long grid = std::min<long long>(p.tiles, host::sm_count() * blocks);
+  const long long grid = std::min<long long>(p.tiles, static_cast<long long>(host::sm_count()) * blocks);
   kernel<<<static_cast<unsigned>(grid), kEpilogueWarps * 32 + producers(PA, PB) + 32, bytes, host::counted(s)>>>(p);
   return host::check_launch("feature_linear");
 }

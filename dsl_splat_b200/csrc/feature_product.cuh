@@ -53,15 +53,16 @@ struct ProductParams {
   int a_vector, b_vector;  // bytes that every row start and chunk is aligned to
   long long k_per_split;   // a multiple of kChunk unless there is one split
   long long k_per_sum;     // of one accumulator; the tile's sums are added in `out` (fp32)
-  int splits, tile_n, tiles_n;
-  long long tiles_m, tiles;
+  int splits, tile_n;
+  uint32_t tiles_n, tiles_m, tiles;  // tiles = splits * tiles_m * tiles_n, below 2^31
   int stages, resident, activation;
   int lag;                 // stages whose copies may be in flight; 0: through registers
   uint32_t tmem_columns;
   const void* bias;   // (n) or NULL
   const void* extra;  // residual or dy (m, n), or NULL
   void* out;          // (splits, m, n)
-  int out_vector;     // rows of extra and out start on whole vectors
+  int extra_vector, out_vector;  // their rows are whole 16-byte pieces
+  int bias_shared;    // values of the bias kept in shared memory (0: too many)
   int* error;
 };
 
@@ -258,123 +259,120 @@ SPLAT_DEV void fill_chunk(bool async, int vector, uint32_t dst, uint32_t plane, 
 
 // ---- epilogue ------------------------------------------------------------------
 
-template <int EPI, int ACT>
-SPLAT_DEV float finish(float z, float extra) {
-  if constexpr (EPI == kForward) return activate<ACT>(z) + extra;
-  if constexpr (EPI == kSlope) return extra * slope<ACT>(z);
-  return z;
-}
+// A 32 x 32 patch of values of T in a warp's staging memory: 16-byte pieces,
+// permuted so that both a lane's own row and 16 bytes per lane along rows are
+// accessed without bank conflicts.
+template <class T>
+struct Patch {
+  static constexpr int kPieces = 2 * sizeof(T);  // of a row
+  static constexpr int V = 16 / sizeof(T);       // values of a piece
+  uint32_t base;
+  SPLAT_DEV uint32_t at(int row, int piece) const {
+    const int turn = kPieces == 4 ? (row >> 1) & 3 : row & 7;
+    return base + row * (32 * sizeof(T)) + ((piece ^ turn) << 4);
+  }
 
-// A 32 x 32 patch of the accumulator: staged through the warp's shared memory
-// so that global accesses run along rows.
-SPLAT_DEV void stage_patch(uint32_t staging, const float (&v)[32]) {
-  const int lane = threadIdx.x & 31;
-  __syncwarp();
+  // Global memory (its corner, rows of ld values) -> staging.  vector: rows
+  // start on 16 bytes and cols is a whole number of pieces.
+  SPLAT_DEV void load(const T* src, long long ld, int rows, int cols, bool vector) const {
+    const int lane = threadIdx.x & 31;
+    if (vector) {
+      constexpr int kRows = 32 / kPieces;
+      const int piece = lane % kPieces, r0 = lane / kPieces;
+      uint4 v[kPieces];
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    store_shared(staging + lane * 128 + ((j ^ (lane & 7)) << 4),
-                 make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
-                            __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3])));
-  __syncwarp();
-}
-
-template <int EPI, int ACT, class TE, class TO>
-SPLAT_DEV void write_patch(const ProductParams& p, uint32_t staging, long long row0, int col0,
-                           TO* out, bool add) {
-  const int lane = threadIdx.x & 31;
-  const TE* extra = static_cast<const TE*>(p.extra);
-  const TE* bias = static_cast<const TE*>(p.bias);
-  if (p.out_vector) {
-    constexpr int V = sizeof(TE) == 2 ? 8 : 4;  // columns of a lane
-    constexpr int kLanes = 32 / V, kRows = 32 / kLanes;
-    const int c = lane % kLanes, col = col0 + c * V;
-    if (col < p.n) {
-      float b[V] = {};
-      if (bias) {
-        const Vec<TE, V> raw = *reinterpret_cast<const Vec<TE, V>*>(bias + col);
-#pragma unroll
-        for (int j = 0; j < V; ++j) b[j] = to_float(raw.v[j]);
+      for (int i = 0; i < kPieces; ++i) {
+        const int r = i * kRows + r0;
+        v[i] = make_uint4(0, 0, 0, 0);
+        if (r < rows && piece * V < cols)
+          v[i] = __ldg(reinterpret_cast<const uint4*>(src + r * ld + piece * V));
       }
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) store_shared(at(i * kRows + r0, piece), v[i]);
+    } else {
 #pragma unroll 4
-      for (int i = 0; i < 32 / kRows; ++i) {
-        const int r = i * kRows + lane / kLanes;
-        const long long row = row0 + r;
-        if (row >= p.m) break;
-        Vec<TE, V> e;
-        if (extra) e = *reinterpret_cast<const Vec<TE, V>*>(extra + row * p.n + col);
-        float z[V];
-#pragma unroll
-        for (int j = 0; j < V / 4; ++j) {
-          const float4 q = load_shared(staging + r * 128 + (((c * (V / 4) + j) ^ (r & 7)) << 4));
-          z[4 * j] = q.x, z[4 * j + 1] = q.y, z[4 * j + 2] = q.z, z[4 * j + 3] = q.w;
-        }
-        constexpr int W = 16 / sizeof(TO);  // values of one store
-#pragma unroll
-        for (int h = 0; h < V; h += W < V ? W : V) {
-          Vec<TO, (W < V ? W : V)> o;
-#pragma unroll
-          for (int j = 0; j < (W < V ? W : V); ++j)
-            o.v[j] = from_float<TO>(finish<EPI, ACT>(z[h + j] + b[h + j],
-                                                extra ? to_float(e.v[h + j]) : 0.0f));
-          auto* at = reinterpret_cast<Vec<TO, (W < V ? W : V)>*>(out + row * p.n + col + h);
-          if constexpr (EPI == kPlain && sizeof(TO) == 4) {
-            if (add) {
-              const Vec<TO, (W < V ? W : V)> sum = *at;
-#pragma unroll
-              for (int j = 0; j < (W < V ? W : V); ++j) o.v[j] += sum.v[j];
-            }
-          }
-          *at = o;
-        }
-      }
-    }
-  } else {
-    const int col = col0 + lane;
-    if (col < p.n) {
-      const float b = bias ? to_float(bias[col]) : 0.0f;
-#pragma unroll 8
-      for (int r = 0; r < 32; ++r) {
-        const long long row = row0 + r;
-        if (row >= p.m) break;
-        const float e = extra ? to_float(extra[row * p.n + col]) : 0.0f;
-        float z;
-        asm volatile("ld.shared.f32 %0, [%1];"
-                     : "=f"(z)
-                     : "r"(staging + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4)
-                     : "memory");
-        float value = finish<EPI, ACT>(z + b, e);
-        if constexpr (EPI == kPlain && sizeof(TO) == 4) {
-          if (add) value += out[row * p.n + col];
-        }
-        out[row * p.n + col] = from_float<TO>(value);
+      for (int r = 0; r < rows; ++r) {
+        const T v = lane < cols ? src[r * ld + lane] : from_float<T>(0.0f);
+        const uint32_t to = at(r, lane / V) + lane % V * sizeof(T);
+        if constexpr (sizeof(T) == 4)
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
+        else
+          asm volatile("st.shared.u16 [%0], %1;" ::"r"(to),
+                       "h"(reinterpret_cast<const unsigned short&>(v))
+                       : "memory");
       }
     }
   }
-}
 
-template <int EPI, class TE, class TO>
-SPLAT_DEV void store_patch(const ProductParams& p, uint32_t staging, const float (&v)[32],
-                           long long row0, int col0, TO* out, bool add) {
-  stage_patch(staging, v);
-  if constexpr (EPI == kPlain) {
-    write_patch<EPI, kNone, TE, TO>(p, staging, row0, col0, out, add);
-  } else {
-    switch (p.activation) {
-      case kRelu: write_patch<EPI, kRelu, TE, TO>(p, staging, row0, col0, out, false); break;
-      case kSilu: write_patch<EPI, kSilu, TE, TO>(p, staging, row0, col0, out, false); break;
-      case kGelu: write_patch<EPI, kGelu, TE, TO>(p, staging, row0, col0, out, false); break;
-      case kSigmoid: write_patch<EPI, kSigmoid, TE, TO>(p, staging, row0, col0, out, false); break;
-      default: write_patch<EPI, kNone, TE, TO>(p, staging, row0, col0, out, false);
+  // Staging -> global memory; add (fp32 only): onto what is there.
+  SPLAT_DEV void store(T* dst, long long ld, int rows, int cols, bool vector, bool add) const {
+    const int lane = threadIdx.x & 31;
+    if (vector) {
+      constexpr int kRows = 32 / kPieces;
+      const int piece = lane % kPieces, r0 = lane / kPieces;
+      if (piece * V >= cols) return;
+      dst += r0 * ld + piece * V;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i, dst += kRows * ld) {
+        if (i * kRows + r0 >= rows) break;
+        float4 v = load_shared(at(i * kRows + r0, piece));
+        if constexpr (sizeof(T) == 4) {
+          if (add) {
+            const float4 o = *reinterpret_cast<const float4*>(dst);
+            v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+          }
+        }
+        *reinterpret_cast<float4*>(dst) = v;
+      }
+    } else if (lane < cols) {
+      dst += lane;
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r, dst += ld) {
+        const uint32_t from = at(r, lane / V) + lane % V * sizeof(T);
+        if constexpr (sizeof(T) == 4) {
+          float v;
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(from) : "memory");
+          *dst = add ? v + *dst : v;
+        } else {
+          unsigned short v;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
+          *dst = reinterpret_cast<const T&>(v);
+        }
+      }
+    }
+  }
+};
+
+// The epilogue's arithmetic on a lane's row: v becomes act(v) + e, or
+// e act'(v); the extra values e lie in the patch.
+template <int EPI, int ACT, class TE>
+SPLAT_DEV void finish_row(const Patch<TE>& extra, bool with_extra, float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+  constexpr int V = Patch<TE>::V;
+#pragma unroll
+  for (int piece = 0; piece < Patch<TE>::kPieces; ++piece) {
+    float* z = v + piece * V;
+    if constexpr (EPI == kForward) {
+#pragma unroll
+      for (int j = 0; j < V; j += 2) activate2<ACT>(z[j], z[j + 1]);
+    }
+    if (EPI == kSlope || with_extra) {
+      const float4 raw = load_shared(extra.at(lane, piece));
+      float e[V];
+      widen<TE, V>(reinterpret_cast<const Vec<TE, V>&>(raw), e);
+#pragma unroll
+      for (int j = 0; j < V; j += 2) {
+        if constexpr (EPI == kForward)
+          unpack2(add2(pack2(z[j], z[j + 1]), pack2(e[j], e[j + 1])), z[j], z[j + 1]);
+        else
+          unpack2(mul2(pack2(slope<ACT>(z[j]), slope<ACT>(z[j + 1])), pack2(e[j], e[j + 1])), z[j],
+                  z[j + 1]);
+      }
     }
   }
 }
 
 // ---- the kernel ------------------------------------------------------------------
-
-template <class S>
-constexpr bool kIsF16 = false;
-template <>
-inline constexpr bool kIsF16<f16> = true;
 
 // Bytes of a plane of B's chunk.
 template <bool MN>
@@ -385,11 +383,20 @@ __host__ __device__ constexpr int b_plane_bytes(int tile_n) {
 struct ProductTile {
   long long m0, k0, k1;
   int n0, split;
-  SPLAT_DEV ProductTile(const ProductParams& p, long long t) {
-    n0 = static_cast<int>(t % p.tiles_n) * p.tile_n;
-    t /= p.tiles_n;
-    m0 = (t % p.tiles_m) * kTileRows;
-    split = static_cast<int>(t / p.tiles_m);
+  // divisions only where there is something to divide: every warp passes here
+  // for every tile
+  SPLAT_DEV ProductTile(const ProductParams& p, uint32_t t) {
+    uint32_t rest = t;
+    n0 = split = 0;
+    if (p.tiles_n > 1) {
+      rest = t / p.tiles_n;
+      n0 = (t - rest * p.tiles_n) * p.tile_n;
+    }
+    if (p.splits > 1) {
+      split = rest / p.tiles_m;
+      rest -= split * p.tiles_m;
+    }
+    m0 = static_cast<long long>(rest) * kTileRows;
     k0 = split * p.k_per_split;
     k1 = min(k0 + p.k_per_split, p.k);
   }
@@ -407,8 +414,8 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
   const uint32_t base = (tc::shared_address(dynamic) + 1023u) & ~1023u;
   const uint32_t b_plane = b_plane_bytes<BMN>(p.tile_n);
   const uint32_t a_bytes = PA * kAPlane, b_bytes = PB * b_plane;
-  const uint32_t staging = base;
-  const uint32_t resident = staging + kEpilogueWarps * kStagingBytes;
+  const uint32_t bias_at = base + kEpilogueWarps * kStagingBytes;
+  const uint32_t resident = bias_at + (p.bias_shared * 4 + 1023) / 1024 * 1024;
   const int chunks_all = static_cast<int>((p.k + kChunk - 1) / kChunk);
   const uint32_t ring = resident + (p.resident ? chunks_all * b_bytes : 0);
   const uint32_t stage_bytes = a_bytes + (p.resident ? 0 : b_bytes);
@@ -426,6 +433,12 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
     tc::barrier_init(tc::shared_address(&resident_full), kProducers);
     tc::barrier_init(tc::shared_address(&drained), 1);
     tc::barrier_init_fence();
+  }
+  if (p.bias) {
+    for (int i = threadIdx.x; i < p.bias_shared; i += blockDim.x)
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(bias_at + i * 4),
+                   "f"(i < p.n ? to_float(static_cast<const TE*>(p.bias)[i]) : 0.0f)
+                   : "memory");
   }
   if (warp == 0) tc::tmem_alloc(tc::shared_address(&tmem_base), p.tmem_columns);
   tc::fence_before_sync();
@@ -451,7 +464,7 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
     }
     int stage = 0, in_flight = 0, landed = 0;
     uint32_t parity = 1;  // a fresh barrier's previous phase counts as complete
-    for (long long t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+    for (uint32_t t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
       const ProductTile tile(p, t);
       for (long long k = tile.k0; k < tile.k1; k += kChunk) {
         if (!(ok = tc::barrier_wait(tc::shared_address(&empty[stage]), parity))) break;
@@ -500,7 +513,7 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
       if (p.resident) ok = tc::barrier_wait(tc::shared_address(&resident_full), 0);
       int stage = 0;
       uint32_t parity = 0, acc = 0, acc_parity = 1;
-      for (long long t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+      for (uint32_t t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
         const ProductTile tile(p, t);
         int c = 0;
         for (long long sum_k = tile.k0; sum_k < tile.k1 && ok; sum_k += p.k_per_sum) {
@@ -549,17 +562,30 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
   } else if (warp < kEpilogueWarps) {
     // ---- epilogue
     const int lane_block = warp & 3, half = warp >> 2;
+    const Patch<TE> extra_patch{base + warp * kStagingBytes};
+    const Patch<TO> out_patch{base + warp * kStagingBytes};
     uint32_t acc = 0, parity = 0;
-    for (long long t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+    for (uint32_t t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
       const ProductTile tile(p, t);
       const long long row0 = tile.m0 + lane_block * 32;
-      TO* out = static_cast<TO*>(p.out) + static_cast<long long>(tile.split) * p.m * p.n;
+      const int rows = static_cast<int>(min(p.m - row0, 32LL));
+      TO* out = static_cast<TO*>(p.out) + (tile.split * p.m + row0) * p.n;
       for (long long sum_k = tile.k0; sum_k < tile.k1; sum_k += p.k_per_sum) {
-        if (!(ok = tc::barrier_wait(tc::shared_address(&acc_full[acc]), parity))) break;
-        tc::fence_after_sync();
+        bool waited = false;
         for (int c = half; c * 32 < p.tile_n; c += kEpilogueWarps / 4) {
-          const int col0 = tile.n0 + c * 32;
-          if (col0 >= p.n || row0 >= p.m) break;
+          const int col0 = tile.n0 + c * 32, cols = min(p.n - col0, 32);
+          if (cols <= 0 || rows <= 0) break;
+          __syncwarp();  // the patch before has been read
+          if (EPI != kPlain && p.extra) {
+            extra_patch.load(static_cast<const TE*>(p.extra) + row0 * p.n + col0, p.n, rows, cols,
+                             p.extra_vector);
+            __syncwarp();
+          }
+          if (!waited) {
+            if (!(ok = tc::barrier_wait(tc::shared_address(&acc_full[acc]), parity))) break;
+            tc::fence_after_sync();
+            waited = true;
+          }
           const uint32_t from = tmem + (lane_block << 21) + acc * kAcc * p.tile_n + c * 32;
           float v[32];
           tc::tmem_load32(from, v);
@@ -569,8 +595,49 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] += low[i];
           }
-          store_patch<EPI, TE, TO>(p, staging + warp * kStagingBytes, v, row0, col0, out,
-                                   sum_k != tile.k0);
+          if constexpr (EPI != kPlain) {
+            if (p.bias) {
+              if (p.bias_shared) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  const float4 b = load_shared(bias_at + (col0 + j * 4) * 4);
+                  unpack2(add2(pack2(v[4 * j], v[4 * j + 1]), pack2(b.x, b.y)), v[4 * j],
+                          v[4 * j + 1]);
+                  unpack2(add2(pack2(v[4 * j + 2], v[4 * j + 3]), pack2(b.z, b.w)), v[4 * j + 2],
+                          v[4 * j + 3]);
+                }
+              } else {
+                const TE* bias = static_cast<const TE*>(p.bias) + col0;
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (j < cols) v[j] += to_float(bias[j]);
+              }
+            }
+            const bool e = p.extra;
+            switch (p.activation) {
+              case kRelu: finish_row<EPI, kRelu, TE>(extra_patch, e, v); break;
+              case kSilu: finish_row<EPI, kSilu, TE>(extra_patch, e, v); break;
+              case kGelu: finish_row<EPI, kGelu, TE>(extra_patch, e, v); break;
+              case kSigmoid: finish_row<EPI, kSigmoid, TE>(extra_patch, e, v); break;
+              default: finish_row<EPI, kNone, TE>(extra_patch, e, v);
+            }
+            if (sizeof(TE) != sizeof(TO)) __syncwarp();  // the two patches' rows differ
+          }
+#pragma unroll
+          for (int j = 0; j < Patch<TO>::kPieces; ++j) {
+            constexpr int V = Patch<TO>::V;
+            float o[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = v[j * V + i];
+            const Vec<TO, V> r = round_values<TO, V>(o);
+            store_shared(out_patch.at(threadIdx.x & 31, j), reinterpret_cast<const uint4&>(r));
+          }
+          __syncwarp();
+          out_patch.store(out + col0, p.n, rows, cols, p.out_vector, sum_k != tile.k0);
+        }
+        if (!ok) break;
+        if (!waited) {  // a warp without a patch still takes part
+          if (!(ok = tc::barrier_wait(tc::shared_address(&acc_full[acc]), parity))) break;
         }
         tc::fence_before_sync();
         tc::barrier_arrive(tc::shared_address(&acc_empty[acc]));
