@@ -1,6 +1,6 @@
 """Builds libsplat200.so in place for sm_100a (nvcc, no JIT cache).
 
-Five translation units, compiled in parallel and linked into one library:
+Six translation units, compiled in parallel and linked into one library:
 
 * splat200.cu (entry points, forward kernels, binning, blending) with
   -fmad=false: every multiply-add stays two IEEE roundings unless the source
@@ -11,8 +11,9 @@ Five translation units, compiled in parallel and linked into one library:
   -prec-sqrt=false: their outputs are gradients, compared within a relative
   tolerance, and contraction plus the approximate divide and square root (a
   few ulp) remove a large part of their arithmetic;
-* feature_linear.cu and feature_norm.cu (the feature operators) with
-  -fmad=true: their results are compared within their types' rounding.
+* feature_linear.cu, feature_linear_backward.cu and feature_norm.cu (the
+  feature operators) with -fmad=true: their results are compared within their
+  types' rounding.
 
 splat200.cu keeps IEEE-rounded division and square root (the nvcc defaults
 -prec-div=true -prec-sqrt=true); nothing is built with --use_fast_math.
@@ -34,11 +35,13 @@ SOURCES = {"splat200.cu": ["-fmad=false"],
            "project_backward.cu": ["-fmad=true", "-prec-div=false", "-prec-sqrt=false"],
            "aaa_backward.cu": ["-fmad=true", "-prec-div=false", "-prec-sqrt=false"],
            "feature_linear.cu": ["-fmad=true"],
+           "feature_linear_backward.cu": ["-fmad=true"],
            "feature_norm.cu": ["-fmad=true"]}
 HEADERS = ["splat_common.cuh", "cameras.cuh", "project.cuh", "binning.cuh", "render.cuh",
            "footprint.cuh", "tile_modes.cuh", "host_runtime.h", "rade.cuh", "rade_project.cuh",
            "aaa.cuh", "aaa_render.cuh", "aaa_api.cuh", "aaa_blend_params.cuh",
-           "aaa_backward.cuh", "feature_common.cuh", "feature_product.cuh", "tensor_core.cuh"]
+           "aaa_backward.cuh", "feature_common.cuh", "feature_product.cuh", "feature_fused.cuh",
+           "feature_launch.cuh", "tensor_core.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

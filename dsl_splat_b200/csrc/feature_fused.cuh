@@ -1,0 +1,369 @@
+// The backward of a linear layer in one pass over its rows:
+//
+//   z = x W^T + b, dz = dy act'(z), dx = dz W, dW += dz^T x, db += dz^T 1
+//
+// for layers whose W and one 128-row tile of x and dz fit in shared memory.
+// x and dy are read once and dx is written once; the three products of a tile
+// take the same copies of x, dz and W, as K-major operands in one and MN-major
+// ones in the other, and dW stays in tensor memory (16-bit types: 2^-10 of the
+// result's rounding at 10^5 additions) or is added up in registers after every
+// tile (fp32: the tensor core truncates its sums).
+//
+// A block of eight warps does each tile's steps together: load, product,
+// activation slope, products, store.  What overlaps one block's steps is the
+// other blocks of its SM, and copies of the next tile's x.
+#pragma once
+#include "feature_product.cuh"
+
+namespace splat {
+namespace feature {
+
+struct FusedParams {
+  long long rows;
+  int k, n, k32, n32;  // widths rounded up to 32
+  const void *x, *weight, *bias, *dy;
+  void* dx;        // (rows, k) or NULL
+  float* partial;  // per block: (n, k) of dW, then (n) of db; NULL: neither
+  int activation, x_vector, w_vector, dy_vector, dx_vector;
+  int buffers;  // of x: 2 when the next tile's is copied ahead
+  uint32_t tiles, tmem_columns;
+  int* error;
+};
+
+constexpr int kFusedThreads = 256;
+constexpr int kFusedWidth = 128;        // widest k and n
+constexpr int kOnesBytes = 16 * 128;    // 16 rows of 64 ones
+
+// PT parts of x and W, PZ of dz.
+template <class T, int PT, int PZ>
+struct Fused {
+  static constexpr int kAcc = sizeof(T) == 4 ? 2 : 1;  // accumulators of dW and db
+  static constexpr bool kNative16 = PT == 1 && PZ == 1 && kIsF16<T>;
+  __host__ __device__ static int blocks64(int n) { return (n + 63) / 64; }
+  __host__ __device__ static int staging_bytes() { return 8 * 1024 * sizeof(T); }
+  __host__ __device__ static int x_plane(int k) { return blocks64(k) * kAPlane; }
+  __host__ __device__ static int w_plane(int k, int n32) { return blocks64(k) * n32 * 128; }
+  static size_t shared_bytes(int k, int n, int n32, int buffers) {
+    return staging_bytes() + static_cast<size_t>(buffers) * PT * x_plane(k) +
+           PZ * x_plane(n) + PT * w_plane(k, n32) + kOnesBytes + 1024 + kFusedWidth * 4;
+  }
+};
+
+template <class T, int PT, int PZ>
+__global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
+    fused_backward_kernel(const __grid_constant__ FusedParams p) {
+  using F = Fused<T, PT, PZ>;
+  constexpr int kAcc = F::kAcc;
+  constexpr int kParts = PT > PZ ? PT : PZ;
+  extern __shared__ unsigned char dynamic[];
+  __shared__ alignas(8) unsigned long long z_done, dx_done, dw_done, drained;
+  __shared__ uint32_t tmem_base;
+  const uint32_t base = (tc::shared_address(dynamic) + 1023u) & ~1023u;
+  const uint32_t x_plane = F::x_plane(p.k), z_plane = F::x_plane(p.n);
+  const uint32_t w_plane = F::w_plane(p.k, p.n32);
+  const uint32_t x_at = base + F::staging_bytes();
+  const uint32_t z_at = x_at + p.buffers * PT * x_plane;
+  const uint32_t w_at = z_at + PZ * z_plane;
+  const uint32_t ones_at = w_at + PT * w_plane;
+  const uint32_t bias_at = ones_at + kOnesBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane_block = warp & 3, half = warp >> 2;
+  const Patch<T> patch{base + warp * static_cast<uint32_t>(1024 * sizeof(T))};
+  const T* x = static_cast<const T*>(p.x);
+  const bool with_z = p.activation != kNone;
+  const bool ahead = p.buffers == 2;
+
+  if (threadIdx.x == 0) {
+    tc::barrier_init(tc::shared_address(&z_done), 1);
+    tc::barrier_init(tc::shared_address(&dx_done), 1);
+    tc::barrier_init(tc::shared_address(&dw_done), 1);
+    tc::barrier_init(tc::shared_address(&drained), 1);
+    tc::barrier_init_fence();
+  }
+  if (warp == 0) tc::tmem_alloc(tc::shared_address(&tmem_base), p.tmem_columns);
+  // W, a block of ones and the bias stay for all tiles
+  for (int c = 0; c * 64 < p.k; ++c)
+    fill<T, PT>(p.w_vector, w_at + c * p.n32 * 128, w_plane, p.n32, 8,
+                static_cast<const T*>(p.weight) + c * 64, p.k, p.n, p.k - c * 64, threadIdx.x,
+                kFusedThreads);
+  {
+    const uint32_t one = F::kNative16 ? 0x3c003c00u : 0x3f803f80u;
+    if (threadIdx.x < kOnesBytes / 16)
+      store_shared(ones_at + threadIdx.x * 16, make_uint4(one, one, one, one));
+  }
+  for (int i = threadIdx.x; i < p.n32; i += kFusedThreads)
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(bias_at + i * 4),
+                 "f"(p.bias && i < p.n ? to_float(static_cast<const T*>(p.bias)[i]) : 0.0f)
+                 : "memory");
+
+  const auto load_x = [&](uint32_t tile, uint32_t at, bool async) {
+    const long long m0 = static_cast<long long>(tile) * kTileRows;
+    for (int c = 0; c * 64 < p.k; ++c) {
+      const int valid = p.k - c * 64;
+      const int pieces = min((valid + 15) / 16 * 2, 8);
+      const T* src = x + m0 * p.k + c * 64;
+      if constexpr (PT == 1 && sizeof(T) == 2) {
+        if (async) {
+          fill_async<T>(at + c * kAPlane, kTileRows, pieces, src, p.k, p.rows - m0, valid,
+                        threadIdx.x, kFusedThreads);
+          continue;
+        }
+      }
+      fill<T, PT>(p.x_vector, at + c * kAPlane, x_plane, kTileRows, pieces, src, p.k,
+                  p.rows - m0, valid, threadIdx.x, kFusedThreads);
+    }
+  };
+  if (ahead) {
+    load_x(blockIdx.x, x_at, true);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_base;
+  const uint32_t acc_w = tmem + max(p.k32, p.n32), acc_b = acc_w + kAcc * p.k32;
+
+  float sum_w[kAcc == 2 ? 2 : 1][32] = {};  // fp32: this thread's part of dW
+  float sum_b = 0.0f;
+  uint32_t parity = 0;
+  int buffer = 0;
+  bool ok = true, fresh = true;
+  for (uint32_t t = blockIdx.x; t < p.tiles; t += gridDim.x, parity ^= 1) {
+    const long long row0 = static_cast<long long>(t) * kTileRows + lane_block * 32;
+    const int rows = static_cast<int>(max(min(p.rows - row0, 32LL), 0LL));
+    const uint32_t x_now = x_at + buffer * PT * x_plane;
+    if (ahead)
+      wait_copies(0);
+    else
+      load_x(t, x_now, false);
+    tc::fence_async_proxy();
+    tc::fence_before_sync();
+    // x is there, and the previous tile's accumulators have been read
+    if (__syncthreads_or(!ok)) break;
+    if (threadIdx.x == 0 && with_z) {
+      tc::fence_after_sync();
+      const uint32_t instruction = tc::instruction(!F::kNative16, false, false, p.n32);
+      bool first = true;
+#pragma unroll
+      for (int sum = PT - 1; sum >= 0; --sum)
+#pragma unroll
+        for (int i = 0; i <= sum; ++i)
+          for (int s = 0; s * 16 < p.k; ++s) {
+            const uint32_t o = (s & 3) * tc::kStepK;
+            tc::mma(tmem,
+                    tc::descriptor_k_major(x_now + i * x_plane + (s >> 2) * kAPlane + o),
+                    tc::descriptor_k_major(w_at + (sum - i) * w_plane + (s >> 2) * p.n32 * 128 + o),
+                    instruction, !first);
+            first = false;
+          }
+      tc::commit(tc::shared_address(&z_done));
+    }
+    if (ahead) {
+      buffer ^= 1;
+      if (t + gridDim.x < p.tiles) load_x(t + gridDim.x, x_at + buffer * PT * x_plane, true);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    // dz: a lane's row of each 32-wide patch
+    bool waited = !with_z;
+    for (int c = half; c * 32 < p.n32; c += 2) {
+      __syncwarp();
+      patch.load(static_cast<const T*>(p.dy) + row0 * p.n + c * 32, p.n, rows,
+                 min(p.n - c * 32, 32), p.dy_vector);
+      __syncwarp();
+      float v[32];
+      if (!waited) {
+        ok = tc::barrier_wait(tc::shared_address(&z_done), parity) && ok;
+        tc::fence_after_sync();
+        waited = true;
+      }
+      if (with_z) {
+        tc::tmem_load32(tmem + (lane_block << 21) + c * 32, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float4 b = load_shared(bias_at + (c * 32 + j * 4) * 4);
+          unpack2(add2(pack2(v[4 * j], v[4 * j + 1]), pack2(b.x, b.y)), v[4 * j], v[4 * j + 1]);
+          unpack2(add2(pack2(v[4 * j + 2], v[4 * j + 3]), pack2(b.z, b.w)), v[4 * j + 2],
+                  v[4 * j + 3]);
+        }
+      }
+      switch (p.activation) {
+        case kRelu: finish_row<kSlope, kRelu, T>(patch, true, v); break;
+        case kSilu: finish_row<kSlope, kSilu, T>(patch, true, v); break;
+        case kGelu: finish_row<kSlope, kGelu, T>(patch, true, v); break;
+        case kSigmoid: finish_row<kSlope, kSigmoid, T>(patch, true, v); break;
+        default: finish_row<kSlope, kNone, T>(patch, true, v);
+      }
+      if (lane >= rows) {  // rows past the end add nothing to dW
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+      }
+      const int row = lane_block * 32 + lane;
+      const uint32_t at = z_at + (c >> 1) * kAPlane + row * 128;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint4 parts[PZ];
+        if constexpr (F::kNative16) {
+          float o[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = v[j * 8 + i];
+          const Vec<T, 8> r = round_values<T, 8>(o);
+          parts[0] = reinterpret_cast<const uint4&>(r);
+        } else {
+          Vec<float, 8> o;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o.v[i] = v[j * 8 + i];
+          to_parts<float, PZ>(o, parts);
+        }
+#pragma unroll
+        for (int q = 0; q < PZ; ++q)
+          store_shared(at + q * z_plane + ((((c & 1) * 4 + j) ^ (row & 7)) << 4), parts[q]);
+      }
+    }
+    tc::fence_async_proxy();
+    tc::fence_before_sync();
+    __syncthreads();  // dz is there, z has been read
+    if (threadIdx.x == 0) {
+      tc::fence_after_sync();
+      if (p.dx) {
+        const uint32_t instruction = tc::instruction(!F::kNative16, false, true, p.k32);
+        bool first = true;
+#pragma unroll
+        for (int sum = kParts - 1; sum >= 0; --sum)
+#pragma unroll
+          for (int i = 0; i < PZ; ++i) {
+            const int j = sum - i;
+            if (j < 0 || j >= PT) continue;
+            for (int s = 0; s * 16 < p.n; ++s) {
+              tc::mma(tmem,
+                      tc::descriptor_k_major(z_at + i * z_plane + (s >> 2) * kAPlane +
+                                             (s & 3) * tc::kStepK),
+                      tc::descriptor_mn_major(w_at + j * w_plane + s * tc::kStepMn, p.n32 * 128),
+                      instruction, !first);
+              first = false;
+            }
+          }
+      }
+      tc::commit(tc::shared_address(&dx_done));
+      if (p.partial) {
+        // n of up to 64 take one block of dz twice; the upper lanes are not read
+        const uint32_t z_block = p.n > 64 ? kAPlane : 0;
+        const uint32_t wide = tc::instruction(!F::kNative16, true, true, p.k32);
+        const uint32_t narrow = tc::instruction(!F::kNative16, true, false, 16);
+        const bool start = kAcc == 2 || fresh;
+#pragma unroll
+        for (int sum = kParts - 1; sum >= 0; --sum)
+#pragma unroll
+          for (int i = 0; i < PZ; ++i) {
+            const int j = sum - i;
+            if (j < 0 || j >= PT) continue;
+            const bool own = sum == 0 && kAcc == 2;
+            const int first_part = kParts - 1 < PT ? 0 : kParts - PT;
+            const bool first = start && (own || (sum == kParts - 1 && i == first_part));
+            for (int s = 0; s < kTileRows / 16; ++s)
+              tc::mma(acc_w + (own ? 0 : (kAcc - 1) * p.k32),
+                      tc::descriptor_mn_major(z_at + i * z_plane + s * tc::kStepMn, z_block),
+                      tc::descriptor_mn_major(x_now + j * x_plane + s * tc::kStepMn, kAPlane),
+                      wide, !(first && s == 0));
+          }
+#pragma unroll
+        for (int i = PZ - 1; i >= 0; --i) {
+          const bool own = i == 0 && kAcc == 2;
+          const bool first = start && (own || i == PZ - 1);
+          for (int s = 0; s < kTileRows / 16; ++s)
+            tc::mma(acc_b + (own ? 0 : (kAcc - 1) * 32),
+                    tc::descriptor_mn_major(z_at + i * z_plane + s * tc::kStepMn, z_block),
+                    tc::descriptor_k_major(ones_at + (s & 3) * tc::kStepK), narrow,
+                    !(first && s == 0));
+        }
+      }
+      tc::commit(tc::shared_address(&dw_done));
+    }
+    fresh = false;
+    if (p.dx) {
+      ok = tc::barrier_wait(tc::shared_address(&dx_done), parity) && ok;
+      tc::fence_after_sync();
+      for (int c = half; c * 32 < p.k32; c += 2) {
+        float v[32];
+        tc::tmem_load32(tmem + (lane_block << 21) + c * 32, v);
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < Patch<T>::kPieces; ++j) {
+          constexpr int V = Patch<T>::V;
+          float o[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) o[i] = v[j * V + i];
+          const Vec<T, V> r = round_values<T, V>(o);
+          store_shared(patch.at(lane, j), reinterpret_cast<const uint4&>(r));
+        }
+        __syncwarp();
+        patch.store(static_cast<T*>(p.dx) + row0 * p.k + c * 32, p.k, rows,
+                    min(p.k - c * 32, 32), p.dx_vector, false);
+      }
+    }
+    // the tile's operands are free once its last products are done
+    ok = tc::barrier_wait(tc::shared_address(&dw_done), parity) && ok;
+    tc::fence_after_sync();
+    if constexpr (kAcc == 2) {
+      if (p.partial && lane_block * 32 < p.n) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = half + 2 * i;
+          if (c * 32 < p.k32) {
+            float v[32];
+            tc::tmem_load32(acc_w + (lane_block << 21) + c * 32, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum_w[i][j] += v[j];
+            tc::tmem_load32(acc_w + (lane_block << 21) + p.k32 + c * 32, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum_w[i][j] += v[j];
+          }
+        }
+        if (half == 0)
+          sum_b += tc::tmem_load1(acc_b + (lane_block << 21)) +
+                   tc::tmem_load1(acc_b + (lane_block << 21) + 32);
+      }
+    }
+  }
+
+  // this block's sums
+  if (p.partial && !fresh) {
+    float* out = p.partial + static_cast<size_t>(blockIdx.x) * p.n * (p.k + 1);
+    const int row = lane_block * 32 + lane;
+    if (lane_block * 32 < p.n) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = half + 2 * i;
+        if (c * 32 < p.k32) {
+          float v[32];
+          if constexpr (kAcc == 2) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = sum_w[i][j];
+          } else {
+            tc::tmem_load32(acc_w + (lane_block << 21) + c * 32, v);
+          }
+          if (row < p.n) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c * 32 + j < p.k) out[row * p.k + c * 32 + j] = v[j];
+          }
+        }
+      }
+      if (half == 0) {
+        if constexpr (kAcc == 1) sum_b = tc::tmem_load1(acc_b + (lane_block << 21));
+        if (row < p.n) out[p.n * p.k + row] = sum_b;
+      }
+    }
+  }
+  if (ahead) wait_copies(0);
+  if (threadIdx.x == 0) {  // also after a wait that ran out
+    tc::commit(tc::shared_address(&drained));
+    ok = tc::barrier_wait(tc::shared_address(&drained), 0) && ok;
+  }
+  if (!ok) atomicCAS(p.error, 0, kDeviceTimeout);
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 0) tc::tmem_free(tmem, p.tmem_columns);
+}
+
+}  // namespace feature
+}  // namespace splat

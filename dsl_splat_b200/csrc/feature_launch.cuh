@@ -1,0 +1,105 @@
+// Host side of the linear layer's products: tiling and launch.
+#pragma once
+#include <algorithm>
+
+#include "feature_product.cuh"
+#include "host_runtime.h"
+
+namespace splat {
+namespace feature {
+
+// ---- launching a product -------------------------------------------------------
+
+// The widest of 16, 8, 4 and 2 bytes that rows of ld values start on.
+template <class S>
+int row_vector(const void* base, long long ld) {
+  int v = 16;
+  while (v > static_cast<int>(sizeof(S)) &&
+         ((ld * static_cast<long long>(sizeof(S))) % v || !host::aligned(base, v)))
+    v /= 2;
+  return v;
+}
+
+// Shared memory of a block when one or two share an SM (228 KB, of which each
+// block costs 1 KB besides its own), less the barriers and the rounding of the
+// base to 1 KB.
+constexpr int kOneBlockBytes = 225 * 1024, kTwoBlocksBytes = 110 * 1024;
+constexpr int kMaxSharedBias = 4096;  // values
+constexpr int kMaxResidentBytes = 128 * 1024;
+
+// Fills in the tiling of p (its sources, sizes and epilogue set) and launches.
+template <class SA, int PA, bool AMN, class SB, int PB, bool BMN, class TE, class TO, int EPI>
+int launch_product(ProductParams p, cudaStream_t s) {
+  const int widest = PA == 1 && PB == 1 ? 256 : 128;
+  p.tiles_n = (p.n + widest - 1) / widest;
+  p.tile_n = ((p.n + p.tiles_n - 1) / p.tiles_n + 31) / 32 * 32;
+  const long long tiles_m = (p.m + kTileRows - 1) / kTileRows;
+  if (tiles_m * p.tiles_n * p.splits >= 1LL << 31)
+    return host::fail(kTooLarge, "feature_linear: too many tiles");
+  p.tiles_m = static_cast<uint32_t>(tiles_m);
+  p.tiles = p.tiles_m * p.tiles_n * p.splits;
+  p.a_vector = row_vector<SA>(p.a, p.a_ld);
+  p.b_vector = row_vector<SB>(p.b, p.b_ld);
+  p.extra_vector =
+      p.n * static_cast<long long>(sizeof(TE)) % 16 == 0 && host::aligned(p.extra, 16);
+  p.out_vector = p.n * static_cast<long long>(sizeof(TO)) % 16 == 0 && host::aligned(p.out, 16);
+  const int columns = static_cast<int>(p.tiles_n) * p.tile_n;
+  p.bias_shared = p.bias && columns <= kMaxSharedBias ? columns : 0;
+  p.tmem_columns = 32;
+  constexpr int kAcc = accumulators(PA, PB);
+  while (p.tmem_columns < 2u * kAcc * p.tile_n) p.tmem_columns *= 2;
+  // sums of several accumulators are joined in fp32 outputs; an operand row of
+  // more values than kExactSum is summed in one
+  p.k_per_sum = kAcc == 2 && EPI == kPlain && sizeof(TO) == 4 ? kExactSum : p.k_per_split;
+  const int b_bytes = PB * b_plane_bytes<BMN>(p.tile_n), a_bytes = PA * kAPlane;
+  const long long chunks = (p.k + kChunk - 1) / kChunk;
+  const long long whole_b = chunks * b_bytes;
+  p.resident = p.splits == 1 && p.tiles_n == 1 && whole_b <= kMaxResidentBytes;
+  const int fixed = kEpilogueWarps * kStagingBytes + (p.bias_shared * 4 + 1023) / 1024 * 1024 + (p.resident ? static_cast<int>(whole_b) : 0);
+  const int stage = a_bytes + (p.resident ? 0 : b_bytes);
+  int blocks = 2, budget = kTwoBlocksBytes;
+  if (producers(PA, PB) > 128 || p.tmem_columns > 256 || fixed + 2 * stage > budget)
+    blocks = 1, budget = kOneBlockBytes;
+  p.stages = std::min(kMaxStages, (budget - fixed) / stage);
+  if (p.stages < 1) return host::fail(kTooLarge, "feature_linear: no room for a stage");
+  const bool copied = PA == 1 && PB == 1 && p.a_vector == 16 &&
+                      (p.resident || p.b_vector == 16) && sizeof(SA) == 2;
+  p.lag = copied ? p.stages - 1 : 0;
+  p.error = host::device_error_word();
+  if (!p.error) return kCudaError;
+  const int bytes = fixed + p.stages * stage + 1024;
+  auto* kernel = product_kernel<SA, PA, AMN, SB, PB, BMN, TE, TO, EPI>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+      cudaSuccess)
+    return host::check_launch("feature_linear: shared memory");
+  const long long grid = std::min<long long>(p.tiles, static_cast<long long>(host::sm_count()) * blocks);
+  kernel<<<static_cast<unsigned>(grid), kEpilogueWarps * 32 + producers(PA, PB) + 32, bytes, host::counted(s)>>>(p);
+  return host::check_launch("feature_linear");
+}
+
+// Parts of an operand that is T in memory (beside a one-part operand f16 goes
+// as it is), and of the fp32 dz: a 16-bit gradient's products take dz in two
+// parts (2^-16), so that it is rounded once, at the end.
+template <class T>
+constexpr int kSourceParts = sizeof(T) == 4 ? 3 : kIsF16<T> ? 2 : 1;
+template <class T>
+constexpr int kNativeParts = sizeof(T) == 4 ? 3 : 1;
+template <class T>
+constexpr int kGradientParts = sizeof(T) == 4 ? 3 : 2;
+
+template <class T>
+ProductParams forward_params(long long rows, int k, int n, const void* x, const void* weight,
+                             const void* bias, const void* extra, int activation, void* out) {
+  ProductParams p{};
+  p.m = rows, p.k = k, p.n = n;
+  p.a = x, p.a_ld = k;
+  p.b = weight, p.b_ld = k;
+  p.k_per_split = k, p.splits = 1;
+  p.bias = bias, p.extra = extra, p.activation = activation, p.out = out;
+  return p;
+}
+
+int check_linear(int dtype, long long rows, int k, int n, int activation);
+
+}  // namespace feature
+}  // namespace splat

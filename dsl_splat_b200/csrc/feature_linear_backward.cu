@@ -1,0 +1,266 @@
+// The backward of a linear layer (feature_linear.cu):
+//
+//   z = x W^T + b,  dz = dy act'(z)
+//   dx = dz W,  dW = dz^T x,  db = sum over rows of dz,  dr = dy
+//
+// Narrow layers take one pass over the rows (feature_fused.cuh).  Wider ones
+// form dz in fp32 and take a product each for dx and dW, the latter over
+// ranges of rows whose sums are joined in a fixed order.
+#include <algorithm>
+
+#include "feature_fused.cuh"
+#include "feature_launch.cuh"
+#include "splat200.h"
+
+namespace splat {
+namespace feature {
+
+// ---- sums over splits and rows ---------------------------------------------------
+
+// Adds the splits' partial sums, `stride` values apart, in a fixed order: 8
+// threads to a value.  The first count_a values go to a, the rest to b.
+template <class T>
+__global__ void __launch_bounds__(256)
+    join_splits_kernel(const float* partial, long long stride, int splits, long long count_a,
+                       long long count_b, T* a, T* b) {
+  const long long i = blockIdx.x * 32LL + threadIdx.x, count = count_a + count_b;
+  float s = 0.0f;
+  if (i < count) {
+#pragma unroll 4
+    for (int k = threadIdx.y; k < splits; k += 8) s += partial[k * stride + i];
+  }
+  __shared__ float sums[8][32];
+  sums[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && i < count) {
+    for (int k = 1; k < 8; ++k) s += sums[k][threadIdx.x];
+    T* to = i < count_a ? a : b;
+    if (to) to[i < count_a ? i : i - count_a] = from_float<T>(s);
+  }
+}
+
+template <class T>
+void join_splits(const float* partial, long long stride, int splits, long long count_a,
+                 long long count_b, void* a, void* b, cudaStream_t s) {
+  join_splits_kernel<T>
+      <<<host::blocks_for(count_a + count_b, 32), dim3(32, 8), 0, host::counted(s)>>>(
+          partial, stride, splits, count_a, count_b, static_cast<T*>(a), static_cast<T*>(b));
+}
+
+// Column sums of dz (m, n) over ranges of rows.
+template <class S>
+__global__ void __launch_bounds__(256) column_sums_kernel(const S* dz, long long m, int n,
+                                                          long long rows, float* partial) {
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  const long long begin = blockIdx.y * rows, end = min(begin + rows, m);
+  float s = 0.0f;
+  if (c < n) {
+#pragma unroll 8
+    for (long long r = begin + threadIdx.y; r < end; r += 8) s += to_float(dz[r * n + c]);
+  }
+  __shared__ float sums[8][32];
+  sums[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < n) {
+    for (int i = 1; i < 8; ++i) s += sums[i][threadIdx.x];
+    partial[static_cast<long long>(blockIdx.y) * n + c] = s;
+  }
+}
+
+// Ranges of rows whose sums of dz^T x (and of dz) are joined afterwards:
+// enough tiles for two blocks on every SM, 512 rows to a range at least.
+struct Splits {
+  int count;
+  long long rows;
+};
+Splits weight_splits(long long rows, int k, int n) {
+  const long long tiles = ((n + 127LL) / 128) * ((k + 127) / 128);
+  const long long wanted = std::max(1LL, 2LL * host::sm_count() / tiles);
+  const long long most = (rows + 511) / 512;
+  const long long per = (rows + std::min(wanted, most) - 1) / std::min(wanted, most);
+  Splits s;
+  s.rows = (per + kChunk - 1) / kChunk * kChunk;
+  s.count = static_cast<int>((rows + s.rows - 1) / s.rows);
+  return s;
+}
+
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
+size_t dz_bytes(long long rows, int n, int activation) {
+  return activation == kNone ? 0 : round16(static_cast<size_t>(rows) * n * 4);
+}
+
+// The two products of the backward, from dz as S.
+template <class T, class S, int PZ, int PT>
+int launch_gradients(long long rows, int k, int n, const S* dz, const void* x,
+                     const void* weight, void* dx, void* dweight, void* dbias, float* partial,
+                     cudaStream_t s) {
+  if (dx) {
+    ProductParams p{};
+    p.m = rows, p.k = n, p.n = k;
+    p.a = dz, p.a_ld = n;
+    p.b = weight, p.b_ld = k;
+    p.k_per_split = n, p.splits = 1;
+    p.out = dx;
+    const int status = launch_product<S, PZ, false, T, PT, true, T, T, kPlain>(p, s);
+    if (status != kOk) return status;
+  }
+  const Splits splits = weight_splits(rows, k, n);
+  if (dweight) {
+    ProductParams p{};
+    p.m = n, p.k = rows, p.n = k;
+    p.a = dz, p.a_ld = n;
+    p.b = x, p.b_ld = k;
+    p.k_per_split = splits.rows, p.splits = splits.count;
+    p.out = partial;
+    const int status = launch_product<S, PZ, true, T, PT, true, float, float, kPlain>(p, s);
+    if (status != kOk) return status;
+    const long long count = static_cast<long long>(n) * k;
+    join_splits<T>(partial, count, splits.count, count, 0, dweight, nullptr, s);
+  }
+  if (dbias) {
+    float* sums = partial + static_cast<long long>(splits.count) * n * k;
+    column_sums_kernel<S><<<dim3(host::blocks_for(n, 32), splits.count), dim3(32, 8), 0,
+                            host::counted(s)>>>(dz, rows, n, splits.rows, sums);
+    join_splits<T>(sums, n, splits.count, n, 0, dbias, nullptr, s);
+  }
+  return host::check_launch("feature_linear_backward");
+}
+
+// ---- narrow layers: one pass -----------------------------------------------------
+
+// How a narrow layer's pass is launched; blocks == 0: the layer is too wide.
+struct FusedPlan {
+  int blocks, buffers;
+  size_t bytes;
+  uint32_t tmem_columns;
+};
+
+int round32(int n) { return (n + 31) / 32 * 32; }
+
+template <class T, int PT, int PZ>
+FusedPlan plan_fused(long long rows, int k, int n) {
+  using F = Fused<T, PT, PZ>;
+  FusedPlan plan{};
+  if (k > kFusedWidth || n > kFusedWidth) return plan;
+  const int k32 = round32(k), n32 = round32(n);
+  plan.tmem_columns = 32;
+  while (plan.tmem_columns < static_cast<uint32_t>(std::max(k32, n32) + F::kAcc * (k32 + 32)))
+    plan.tmem_columns *= 2;
+  plan.buffers = 1;
+  plan.bytes = F::shared_bytes(k, n, n32, 1);
+  if (plan.tmem_columns > 512 || plan.bytes > kOneBlockBytes) return plan;
+  int per_sm = 1;
+  if (sizeof(T) == 2 && plan.tmem_columns <= 256 && plan.bytes <= kTwoBlocksBytes) per_sm = 2;
+  // x is copied ahead where that costs no block
+  if (sizeof(T) == 2 && PT == 1 && k % 8 == 0) {
+    const size_t two = F::shared_bytes(k, n, n32, 2);
+    if (two <= static_cast<size_t>(per_sm == 2 ? kTwoBlocksBytes : kOneBlockBytes))
+      plan.buffers = 2, plan.bytes = two;
+  }
+  plan.blocks = static_cast<int>(std::min<long long>(
+      (rows + kTileRows - 1) / kTileRows, static_cast<long long>(host::sm_count()) * per_sm));
+  return plan;
+}
+
+template <class T, int PT, int PZ>
+int launch_fused(const FusedPlan& plan, long long rows, int k, int n, const void* x,
+                 const void* weight, const void* bias, int activation, const void* dy, void* dx,
+                 void* dweight, void* dbias, float* partial, cudaStream_t s) {
+  FusedParams p{};
+  p.rows = rows, p.k = k, p.n = n, p.k32 = round32(k), p.n32 = round32(n);
+  p.x = x, p.weight = weight, p.bias = bias, p.dy = dy, p.dx = dx;
+  p.partial = dweight || dbias ? partial : nullptr;
+  p.activation = activation;
+  p.x_vector = row_vector<T>(x, k);
+  p.w_vector = row_vector<T>(weight, k);
+  p.dy_vector = n * sizeof(T) % 16 == 0 && host::aligned(dy, 16);
+  p.dx_vector = k * sizeof(T) % 16 == 0 && host::aligned(dx, 16);
+  if (plan.buffers == 2 && p.x_vector != 16)
+    return host::fail(kInvalidArgument, "feature_linear_backward: x must be 16-byte aligned");
+  p.buffers = plan.buffers;
+  p.tiles = static_cast<uint32_t>((rows + kTileRows - 1) / kTileRows);
+  p.tmem_columns = plan.tmem_columns;
+  p.error = host::device_error_word();
+  if (!p.error) return kCudaError;
+  auto* kernel = fused_backward_kernel<T, PT, PZ>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(plan.bytes)) != cudaSuccess)
+    return host::check_launch("feature_linear_backward: shared memory");
+  kernel<<<plan.blocks, kFusedThreads, plan.bytes, host::counted(s)>>>(p);
+  if (p.partial) {
+    const long long count = static_cast<long long>(n) * k;
+    join_splits<T>(partial, count + n, plan.blocks, count, n, dweight, dbias, s);
+  }
+  return host::check_launch("feature_linear_backward");
+}
+
+// Calls f with the part counts of T and the activation.
+template <class T, class F>
+auto with_parts(int activation, F f) {
+  constexpr int P = kNativeParts<T>;
+  if (activation == kNone)
+    return f(std::integral_constant<int, P>{}, std::integral_constant<int, P>{});
+  return f(std::integral_constant<int, kSourceParts<T>>{},
+           std::integral_constant<int, kGradientParts<T>>{});
+}
+
+}  // namespace feature
+}  // namespace splat
+
+using namespace splat;
+using namespace splat::feature;
+
+extern "C" {
+
+size_t splat_feature_linear_backward_workspace_bytes(int dtype, long long rows, int k, int n,
+                                                     int activation) {
+  if (check_linear(dtype, rows, k, n, activation) != kOk) return 0;
+  const FusedPlan plan = SPLAT_FEATURE_TYPE(dtype, [&] {
+    return with_parts<T>(activation, [&](auto pt, auto pz) {
+      return plan_fused<T, decltype(pt)::value, decltype(pz)::value>(rows, k, n);
+    });
+  });
+  const size_t sums = static_cast<size_t>(n) * (static_cast<size_t>(k) + 1) * 4;
+  if (plan.blocks) return plan.blocks * sums;
+  return dz_bytes(rows, n, activation) + weight_splits(rows, k, n).count * sums;
+}
+
+int splat_feature_linear_backward(int dtype, long long rows, int k, int n, const void* x,
+                                  const void* weight, const void* bias, int activation,
+                                  const void* dy, void* dx, void* dweight, void* dbias,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  const int bad = check_linear(dtype, rows, k, n, activation);
+  if (bad != kOk) return bad;
+  if (!x || !weight || !dy || !workspace)
+    return host::fail(kInvalidArgument, "feature_linear_backward: null pointer");
+  if (!host::aligned(workspace, 16))
+    return host::fail(kInvalidArgument, "feature_linear_backward: workspace not 16-byte aligned");
+  if (workspace_bytes <
+      splat_feature_linear_backward_workspace_bytes(dtype, rows, k, n, activation))
+    return host::fail(kWorkspaceTooSmall, "feature_linear_backward: workspace");
+  auto s = static_cast<cudaStream_t>(stream);
+  return SPLAT_FEATURE_TYPE(dtype, [&] {
+    return with_parts<T>(activation, [&](auto pt, auto pz) {
+      constexpr int PT = decltype(pt)::value, PZ = decltype(pz)::value;
+      const FusedPlan plan = plan_fused<T, PT, PZ>(rows, k, n);
+      if (plan.blocks)
+        return launch_fused<T, PT, PZ>(plan, rows, k, n, x, weight, bias, activation, dy, dx,
+                                       dweight, dbias, static_cast<float*>(workspace), s);
+      float* dz = static_cast<float*>(workspace);
+      float* partial = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                                dz_bytes(rows, n, activation));
+      if (activation == kNone)  // dz is dy
+        return launch_gradients<T, T, kNativeParts<T>, kNativeParts<T>>(
+            rows, k, n, static_cast<const T*>(dy), x, weight, dx, dweight, dbias, partial, s);
+      constexpr int P = kNativeParts<T>;
+      const int status = launch_product<T, P, false, T, P, false, T, float, kSlope>(
+          forward_params<T>(rows, k, n, x, weight, bias, dy, activation, dz), s);
+      if (status != kOk) return status;
+      return launch_gradients<T, float, kGradientParts<T>, kSourceParts<T>>(
+          rows, k, n, dz, x, weight, dx, dweight, dbias, partial, s);
+    });
+  });
+}
+
+}  // extern "C"
