@@ -176,6 +176,21 @@ SPLAT_DEV void activate2(float& a, float& b) {
   }
 }
 
+template <int ACT>
+SPLAT_DEV void slope2(float& a, float& b) {
+  if constexpr (ACT == kSilu || ACT == kSigmoid) {
+    float s = a, t = b;
+    logistic2(s, t);
+    const f32x2 p = pack2(s, t), z = pack2(a, b);
+    // s + s z (1 - s), and s (1 - s)
+    const f32x2 q = fma2(pack2(-s, -t), ACT == kSilu ? z : p, ACT == kSilu ? z : p);
+    unpack2(ACT == kSilu ? fma2(p, q, p) : q, a, b);
+  } else {
+    a = slope<ACT>(a);
+    b = slope<ACT>(b);
+  }
+}
+
 }  // namespace feature
 }  // namespace splat
 

@@ -25,7 +25,7 @@ struct FusedParams {
   void* dx;        // (rows, k) or NULL
   float* partial;  // per block: (n, k) of dW, then (n) of db; NULL: neither
   int activation, x_vector, w_vector, dy_vector, dx_vector;
-  int buffers;  // of x: 2 when the next tile's is copied ahead
+  int buffers;  // of x: 2 when the next tile's x and dy are copied ahead
   uint32_t tiles, tmem_columns;
   int* error;
 };
@@ -34,27 +34,32 @@ constexpr int kFusedThreads = 256;
 constexpr int kFusedWidth = 128;        // widest k and n
 constexpr int kOnesBytes = 16 * 128;    // 16 rows of 64 ones
 
-// PT parts of x and W, PZ of dz.
-template <class T, int PT, int PZ>
+template <class T>
 struct Fused {
+  static constexpr int P = sizeof(T) == 4 ? 3 : 1;  // parts of every operand
   static constexpr int kAcc = sizeof(T) == 4 ? 2 : 1;  // accumulators of dW and db
-  static constexpr bool kNative16 = PT == 1 && PZ == 1 && kIsF16<T>;
   __host__ __device__ static int blocks64(int n) { return (n + 63) / 64; }
+  // a patch of 32 x 32 values for each warp
   __host__ __device__ static int staging_bytes() { return 8 * 1024 * sizeof(T); }
+  // and, when the next tile is copied ahead, the warps' patches of its dy
+  __host__ __device__ static int ahead_bytes(int n32) {
+    return (n32 + 63) / 64 * staging_bytes();
+  }
   __host__ __device__ static int x_plane(int k) { return blocks64(k) * kAPlane; }
   __host__ __device__ static int w_plane(int k, int n32) { return blocks64(k) * n32 * 128; }
   static size_t shared_bytes(int k, int n, int n32, int buffers) {
-    return staging_bytes() + static_cast<size_t>(buffers) * PT * x_plane(k) +
-           PZ * x_plane(n) + PT * w_plane(k, n32) + kOnesBytes + 1024 + kFusedWidth * 4;
+    return staging_bytes() + static_cast<size_t>(buffers) * P * x_plane(k) +
+           P * x_plane(n) + P * w_plane(k, n32) + (buffers == 2 ? ahead_bytes(n32) : 0) +
+           kOnesBytes + 1024 + kFusedWidth * 4;
   }
 };
 
-template <class T, int PT, int PZ>
+template <class T>
 __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
     fused_backward_kernel(const __grid_constant__ FusedParams p) {
-  using F = Fused<T, PT, PZ>;
+  using F = Fused<T>;
   constexpr int kAcc = F::kAcc;
-  constexpr int kParts = PT > PZ ? PT : PZ;
+  constexpr int P = F::P;
   extern __shared__ unsigned char dynamic[];
   __shared__ alignas(8) unsigned long long z_done, dx_done, dw_done, drained;
   __shared__ uint32_t tmem_base;
@@ -62,9 +67,10 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
   const uint32_t x_plane = F::x_plane(p.k), z_plane = F::x_plane(p.n);
   const uint32_t w_plane = F::w_plane(p.k, p.n32);
   const uint32_t x_at = base + F::staging_bytes();
-  const uint32_t z_at = x_at + p.buffers * PT * x_plane;
-  const uint32_t w_at = z_at + PZ * z_plane;
-  const uint32_t ones_at = w_at + PT * w_plane;
+  const uint32_t z_at = x_at + p.buffers * P * x_plane;
+  const uint32_t w_at = z_at + P * z_plane;
+  const uint32_t dy_at = w_at + P * w_plane;
+  const uint32_t ones_at = dy_at + (p.buffers == 2 ? F::ahead_bytes(p.n32) : 0);
   const uint32_t bias_at = ones_at + kOnesBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int lane_block = warp & 3, half = warp >> 2;
@@ -83,11 +89,11 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
   if (warp == 0) tc::tmem_alloc(tc::shared_address(&tmem_base), p.tmem_columns);
   // W, a block of ones and the bias stay for all tiles
   for (int c = 0; c * 64 < p.k; ++c)
-    fill<T, PT>(p.w_vector, w_at + c * p.n32 * 128, w_plane, p.n32, 8,
+    fill<T, P>(p.w_vector, w_at + c * p.n32 * 128, w_plane, p.n32, 8,
                 static_cast<const T*>(p.weight) + c * 64, p.k, p.n, p.k - c * 64, threadIdx.x,
                 kFusedThreads);
   {
-    const uint32_t one = F::kNative16 ? 0x3c003c00u : 0x3f803f80u;
+    const uint32_t one = kIsF16<T> ? 0x3c003c00u : 0x3f803f80u;
     if (threadIdx.x < kOnesBytes / 16)
       store_shared(ones_at + threadIdx.x * 16, make_uint4(one, one, one, one));
   }
@@ -102,19 +108,32 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
       const int valid = p.k - c * 64;
       const int pieces = min((valid + 15) / 16 * 2, 8);
       const T* src = x + m0 * p.k + c * 64;
-      if constexpr (PT == 1 && sizeof(T) == 2) {
+      if constexpr (sizeof(T) == 2) {
         if (async) {
           fill_async<T>(at + c * kAPlane, kTileRows, pieces, src, p.k, p.rows - m0, valid,
                         threadIdx.x, kFusedThreads);
           continue;
         }
       }
-      fill<T, PT>(p.x_vector, at + c * kAPlane, x_plane, kTileRows, pieces, src, p.k,
+      fill<T, P>(p.x_vector, at + c * kAPlane, x_plane, kTileRows, pieces, src, p.k,
                   p.rows - m0, valid, threadIdx.x, kFusedThreads);
+    }
+  };
+  // copies of this warp's patches of dy, into memory that only it touches
+  const auto copy_dy = [&](uint32_t tile) {
+    if constexpr (sizeof(T) == 2) {
+      const long long from = static_cast<long long>(tile) * kTileRows + lane_block * 32;
+      const int left = static_cast<int>(max(min(p.rows - from, 32LL), 0LL));
+      for (int c = half; c * 32 < p.n32; c += 2)
+        Patch<T>{dy_at + ((c >> 1) * 8 + warp) * static_cast<uint32_t>(1024 * sizeof(T))}
+            .load_async(left ? static_cast<const T*>(p.dy) + from * p.n + c * 32
+                             : static_cast<const T*>(p.dy),
+                        p.n, left, min(p.n - c * 32, 32));
     }
   };
   if (ahead) {
     load_x(blockIdx.x, x_at, true);
+    copy_dy(blockIdx.x);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   tc::fence_before_sync();
@@ -131,7 +150,7 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
   for (uint32_t t = blockIdx.x; t < p.tiles; t += gridDim.x, parity ^= 1) {
     const long long row0 = static_cast<long long>(t) * kTileRows + lane_block * 32;
     const int rows = static_cast<int>(max(min(p.rows - row0, 32LL), 0LL));
-    const uint32_t x_now = x_at + buffer * PT * x_plane;
+    const uint32_t x_now = x_at + buffer * P * x_plane;
     if (ahead)
       wait_copies(0);
     else
@@ -142,10 +161,10 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
     if (__syncthreads_or(!ok)) break;
     if (threadIdx.x == 0 && with_z) {
       tc::fence_after_sync();
-      const uint32_t instruction = tc::instruction(!F::kNative16, false, false, p.n32);
+      const uint32_t instruction = tc::instruction(!kIsF16<T>, false, false, p.n32);
       bool first = true;
 #pragma unroll
-      for (int sum = PT - 1; sum >= 0; --sum)
+      for (int sum = P - 1; sum >= 0; --sum)
 #pragma unroll
         for (int i = 0; i <= sum; ++i)
           for (int s = 0; s * 16 < p.k; ++s) {
@@ -160,16 +179,20 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
     }
     if (ahead) {
       buffer ^= 1;
-      if (t + gridDim.x < p.tiles) load_x(t + gridDim.x, x_at + buffer * PT * x_plane, true);
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (t + gridDim.x < p.tiles) load_x(t + gridDim.x, x_at + buffer * P * x_plane, true);
     }
     // dz: a lane's row of each 32-wide patch
     bool waited = !with_z;
     for (int c = half; c * 32 < p.n32; c += 2) {
-      __syncwarp();
-      patch.load(static_cast<const T*>(p.dy) + row0 * p.n + c * 32, p.n, rows,
-                 min(p.n - c * 32, 32), p.dy_vector);
-      __syncwarp();
+      const Patch<T> dy{ahead ? dy_at + ((c >> 1) * 8 + warp) * static_cast<uint32_t>(
+                                                                   1024 * sizeof(T))
+                              : patch.base};
+      if (!ahead) {
+        __syncwarp();
+        dy.load(static_cast<const T*>(p.dy) + row0 * p.n + c * 32, p.n, rows,
+                min(p.n - c * 32, 32), p.dy_vector);
+        __syncwarp();
+      }
       float v[32];
       if (!waited) {
         ok = tc::barrier_wait(tc::shared_address(&z_done), parity) && ok;
@@ -187,11 +210,11 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
         }
       }
       switch (p.activation) {
-        case kRelu: finish_row<kSlope, kRelu, T>(patch, true, v); break;
-        case kSilu: finish_row<kSlope, kSilu, T>(patch, true, v); break;
-        case kGelu: finish_row<kSlope, kGelu, T>(patch, true, v); break;
-        case kSigmoid: finish_row<kSlope, kSigmoid, T>(patch, true, v); break;
-        default: finish_row<kSlope, kNone, T>(patch, true, v);
+        case kRelu: finish_row<kSlope, kRelu, T>(dy, true, v); break;
+        case kSilu: finish_row<kSlope, kSilu, T>(dy, true, v); break;
+        case kGelu: finish_row<kSlope, kGelu, T>(dy, true, v); break;
+        case kSigmoid: finish_row<kSlope, kSigmoid, T>(dy, true, v); break;
+        default: finish_row<kSlope, kNone, T>(dy, true, v);
       }
       if (lane >= rows) {  // rows past the end add nothing to dW
 #pragma unroll
@@ -201,8 +224,8 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
       const uint32_t at = z_at + (c >> 1) * kAPlane + row * 128;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        uint4 parts[PZ];
-        if constexpr (F::kNative16) {
+        uint4 parts[P];
+        if constexpr (sizeof(T) == 2) {
           float o[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) o[i] = v[j * 8 + i];
@@ -212,12 +235,17 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
           Vec<float, 8> o;
 #pragma unroll
           for (int i = 0; i < 8; ++i) o.v[i] = v[j * 8 + i];
-          to_parts<float, PZ>(o, parts);
+          to_parts<float, P>(o, parts);
         }
 #pragma unroll
-        for (int q = 0; q < PZ; ++q)
+        for (int q = 0; q < P; ++q)
           store_shared(at + q * z_plane + ((((c & 1) * 4 + j) ^ (row & 7)) << 4), parts[q]);
       }
+    }
+    if (ahead) {
+      __syncwarp();  // this tile's dy has been read
+      if (t + gridDim.x < p.tiles) copy_dy(t + gridDim.x);
+      asm volatile("cp.async.commit_group;" ::: "memory");
     }
     tc::fence_async_proxy();
     tc::fence_before_sync();
@@ -225,14 +253,14 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
     if (threadIdx.x == 0) {
       tc::fence_after_sync();
       if (p.dx) {
-        const uint32_t instruction = tc::instruction(!F::kNative16, false, true, p.k32);
+        const uint32_t instruction = tc::instruction(!kIsF16<T>, false, true, p.k32);
         bool first = true;
 #pragma unroll
-        for (int sum = kParts - 1; sum >= 0; --sum)
+        for (int sum = P - 1; sum >= 0; --sum)
 #pragma unroll
-          for (int i = 0; i < PZ; ++i) {
+          for (int i = 0; i < P; ++i) {
             const int j = sum - i;
-            if (j < 0 || j >= PT) continue;
+            if (j < 0 || j >= P) continue;
             for (int s = 0; s * 16 < p.n; ++s) {
               tc::mma(tmem,
                       tc::descriptor_k_major(z_at + i * z_plane + (s >> 2) * kAPlane +
@@ -247,18 +275,17 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
       if (p.partial) {
         // n of up to 64 take one block of dz twice; the upper lanes are not read
         const uint32_t z_block = p.n > 64 ? kAPlane : 0;
-        const uint32_t wide = tc::instruction(!F::kNative16, true, true, p.k32);
-        const uint32_t narrow = tc::instruction(!F::kNative16, true, false, 16);
+        const uint32_t wide = tc::instruction(!kIsF16<T>, true, true, p.k32);
+        const uint32_t narrow = tc::instruction(!kIsF16<T>, true, false, 16);
         const bool start = kAcc == 2 || fresh;
 #pragma unroll
-        for (int sum = kParts - 1; sum >= 0; --sum)
+        for (int sum = P - 1; sum >= 0; --sum)
 #pragma unroll
-          for (int i = 0; i < PZ; ++i) {
+          for (int i = 0; i < P; ++i) {
             const int j = sum - i;
-            if (j < 0 || j >= PT) continue;
+            if (j < 0 || j >= P) continue;
             const bool own = sum == 0 && kAcc == 2;
-            const int first_part = kParts - 1 < PT ? 0 : kParts - PT;
-            const bool first = start && (own || (sum == kParts - 1 && i == first_part));
+            const bool first = start && (own || (sum == P - 1 && i == 0));
             for (int s = 0; s < kTileRows / 16; ++s)
               tc::mma(acc_w + (own ? 0 : (kAcc - 1) * p.k32),
                       tc::descriptor_mn_major(z_at + i * z_plane + s * tc::kStepMn, z_block),
@@ -266,9 +293,9 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
                       wide, !(first && s == 0));
           }
 #pragma unroll
-        for (int i = PZ - 1; i >= 0; --i) {
+        for (int i = P - 1; i >= 0; --i) {
           const bool own = i == 0 && kAcc == 2;
-          const bool first = start && (own || i == PZ - 1);
+          const bool first = start && (own || i == P - 1);
           for (int s = 0; s < kTileRows / 16; ++s)
             tc::mma(acc_b + (own ? 0 : (kAcc - 1) * 32),
                     tc::descriptor_mn_major(z_at + i * z_plane + s * tc::kStepMn, z_block),

@@ -37,7 +37,7 @@ int splat_feature_linear(int dtype, long long rows, int k, int n, const void* x,
   if (!x || !weight || !y) return host::fail(kInvalidArgument, "feature_linear: null pointer");
   auto s = static_cast<cudaStream_t>(stream);
   return SPLAT_FEATURE_TYPE(dtype, [&] {
-    constexpr int P = kNativeParts<T>;
+    constexpr int P = kOperandParts<T>;
     return launch_product<T, P, false, T, P, false, T, T, kForward>(
         forward_params<T>(rows, k, n, x, weight, bias, residual, activation, y), s);
   });

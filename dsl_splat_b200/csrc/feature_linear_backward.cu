@@ -4,7 +4,7 @@
 //   dx = dz W,  dW = dz^T x,  db = sum over rows of dz,  dr = dy
 //
 // Narrow layers take one pass over the rows (feature_fused.cuh).  Wider ones
-// form dz in fp32 and take a product each for dx and dW, the latter over
+// form dz (in x's type) and take a product each for dx and dW, the latter over
 // ranges of rows whose sums are joined in a fixed order.
 #include <algorithm>
 
@@ -86,15 +86,16 @@ Splits weight_splits(long long rows, int k, int n) {
 
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
-size_t dz_bytes(long long rows, int n, int activation) {
-  return activation == kNone ? 0 : round16(static_cast<size_t>(rows) * n * 4);
+size_t dz_bytes(int dtype, long long rows, int n, int activation) {
+  return activation == kNone ? 0 : round16(static_cast<size_t>(rows) * n * (dtype == kF32 ? 4 : 2));
 }
 
-// The two products of the backward, from dz as S.
-template <class T, class S, int PZ, int PT>
-int launch_gradients(long long rows, int k, int n, const S* dz, const void* x,
+// The two products of the backward.
+template <class T>
+int launch_gradients(long long rows, int k, int n, const T* dz, const void* x,
                      const void* weight, void* dx, void* dweight, void* dbias, float* partial,
                      cudaStream_t s) {
+  constexpr int P = kOperandParts<T>;
   if (dx) {
     ProductParams p{};
     p.m = rows, p.k = n, p.n = k;
@@ -102,7 +103,7 @@ int launch_gradients(long long rows, int k, int n, const S* dz, const void* x,
     p.b = weight, p.b_ld = k;
     p.k_per_split = n, p.splits = 1;
     p.out = dx;
-    const int status = launch_product<S, PZ, false, T, PT, true, T, T, kPlain>(p, s);
+    const int status = launch_product<T, P, false, T, P, true, T, T, kPlain>(p, s);
     if (status != kOk) return status;
   }
   const Splits splits = weight_splits(rows, k, n);
@@ -113,14 +114,14 @@ int launch_gradients(long long rows, int k, int n, const S* dz, const void* x,
     p.b = x, p.b_ld = k;
     p.k_per_split = splits.rows, p.splits = splits.count;
     p.out = partial;
-    const int status = launch_product<S, PZ, true, T, PT, true, float, float, kPlain>(p, s);
+    const int status = launch_product<T, P, true, T, P, true, float, float, kPlain>(p, s);
     if (status != kOk) return status;
     const long long count = static_cast<long long>(n) * k;
     join_splits<T>(partial, count, splits.count, count, 0, dweight, nullptr, s);
   }
   if (dbias) {
     float* sums = partial + static_cast<long long>(splits.count) * n * k;
-    column_sums_kernel<S><<<dim3(host::blocks_for(n, 32), splits.count), dim3(32, 8), 0,
+    column_sums_kernel<T><<<dim3(host::blocks_for(n, 32), splits.count), dim3(32, 8), 0,
                             host::counted(s)>>>(dz, rows, n, splits.rows, sums);
     join_splits<T>(sums, n, splits.count, n, 0, dbias, nullptr, s);
   }
@@ -138,9 +139,9 @@ struct FusedPlan {
 
 int round32(int n) { return (n + 31) / 32 * 32; }
 
-template <class T, int PT, int PZ>
+template <class T>
 FusedPlan plan_fused(long long rows, int k, int n) {
-  using F = Fused<T, PT, PZ>;
+  using F = Fused<T>;
   FusedPlan plan{};
   if (k > kFusedWidth || n > kFusedWidth) return plan;
   const int k32 = round32(k), n32 = round32(n);
@@ -152,8 +153,8 @@ FusedPlan plan_fused(long long rows, int k, int n) {
   if (plan.tmem_columns > 512 || plan.bytes > kOneBlockBytes) return plan;
   int per_sm = 1;
   if (sizeof(T) == 2 && plan.tmem_columns <= 256 && plan.bytes <= kTwoBlocksBytes) per_sm = 2;
-  // x is copied ahead where that costs no block
-  if (sizeof(T) == 2 && PT == 1 && k % 8 == 0) {
+  // x and dy are copied ahead where that costs no block
+  if (sizeof(T) == 2 && k % 8 == 0 && n % 8 == 0) {
     const size_t two = F::shared_bytes(k, n, n32, 2);
     if (two <= static_cast<size_t>(per_sm == 2 ? kTwoBlocksBytes : kOneBlockBytes))
       plan.buffers = 2, plan.bytes = two;
@@ -163,7 +164,7 @@ FusedPlan plan_fused(long long rows, int k, int n) {
   return plan;
 }
 
-template <class T, int PT, int PZ>
+template <class T>
 int launch_fused(const FusedPlan& plan, long long rows, int k, int n, const void* x,
                  const void* weight, const void* bias, int activation, const void* dy, void* dx,
                  void* dweight, void* dbias, float* partial, cudaStream_t s) {
@@ -176,14 +177,15 @@ int launch_fused(const FusedPlan& plan, long long rows, int k, int n, const void
   p.w_vector = row_vector<T>(weight, k);
   p.dy_vector = n * sizeof(T) % 16 == 0 && host::aligned(dy, 16);
   p.dx_vector = k * sizeof(T) % 16 == 0 && host::aligned(dx, 16);
-  if (plan.buffers == 2 && p.x_vector != 16)
-    return host::fail(kInvalidArgument, "feature_linear_backward: x must be 16-byte aligned");
+  if (plan.buffers == 2 && (p.x_vector != 16 || !p.dy_vector))
+    return host::fail(kInvalidArgument,
+                      "feature_linear_backward: x and dy must be 16-byte aligned");
   p.buffers = plan.buffers;
   p.tiles = static_cast<uint32_t>((rows + kTileRows - 1) / kTileRows);
   p.tmem_columns = plan.tmem_columns;
   p.error = host::device_error_word();
   if (!p.error) return kCudaError;
-  auto* kernel = fused_backward_kernel<T, PT, PZ>;
+  auto* kernel = fused_backward_kernel<T>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(plan.bytes)) != cudaSuccess)
     return host::check_launch("feature_linear_backward: shared memory");
@@ -193,16 +195,6 @@ int launch_fused(const FusedPlan& plan, long long rows, int k, int n, const void
     join_splits<T>(partial, count + n, plan.blocks, count, n, dweight, dbias, s);
   }
   return host::check_launch("feature_linear_backward");
-}
-
-// Calls f with the part counts of T and the activation.
-template <class T, class F>
-auto with_parts(int activation, F f) {
-  constexpr int P = kNativeParts<T>;
-  if (activation == kNone)
-    return f(std::integral_constant<int, P>{}, std::integral_constant<int, P>{});
-  return f(std::integral_constant<int, kSourceParts<T>>{},
-           std::integral_constant<int, kGradientParts<T>>{});
 }
 
 }  // namespace feature
@@ -216,14 +208,10 @@ extern "C" {
 size_t splat_feature_linear_backward_workspace_bytes(int dtype, long long rows, int k, int n,
                                                      int activation) {
   if (check_linear(dtype, rows, k, n, activation) != kOk) return 0;
-  const FusedPlan plan = SPLAT_FEATURE_TYPE(dtype, [&] {
-    return with_parts<T>(activation, [&](auto pt, auto pz) {
-      return plan_fused<T, decltype(pt)::value, decltype(pz)::value>(rows, k, n);
-    });
-  });
+  const FusedPlan plan = SPLAT_FEATURE_TYPE(dtype, [&] { return plan_fused<T>(rows, k, n); });
   const size_t sums = static_cast<size_t>(n) * (static_cast<size_t>(k) + 1) * 4;
   if (plan.blocks) return plan.blocks * sums;
-  return dz_bytes(rows, n, activation) + weight_splits(rows, k, n).count * sums;
+  return dz_bytes(dtype, rows, n, activation) + weight_splits(rows, k, n).count * sums;
 }
 
 int splat_feature_linear_backward(int dtype, long long rows, int k, int n, const void* x,
@@ -241,25 +229,21 @@ int splat_feature_linear_backward(int dtype, long long rows, int k, int n, const
     return host::fail(kWorkspaceTooSmall, "feature_linear_backward: workspace");
   auto s = static_cast<cudaStream_t>(stream);
   return SPLAT_FEATURE_TYPE(dtype, [&] {
-    return with_parts<T>(activation, [&](auto pt, auto pz) {
-      constexpr int PT = decltype(pt)::value, PZ = decltype(pz)::value;
-      const FusedPlan plan = plan_fused<T, PT, PZ>(rows, k, n);
-      if (plan.blocks)
-        return launch_fused<T, PT, PZ>(plan, rows, k, n, x, weight, bias, activation, dy, dx,
-                                       dweight, dbias, static_cast<float*>(workspace), s);
-      float* dz = static_cast<float*>(workspace);
-      float* partial = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                                dz_bytes(rows, n, activation));
-      if (activation == kNone)  // dz is dy
-        return launch_gradients<T, T, kNativeParts<T>, kNativeParts<T>>(
-            rows, k, n, static_cast<const T*>(dy), x, weight, dx, dweight, dbias, partial, s);
-      constexpr int P = kNativeParts<T>;
-      const int status = launch_product<T, P, false, T, P, false, T, float, kSlope>(
-          forward_params<T>(rows, k, n, x, weight, bias, dy, activation, dz), s);
+    const FusedPlan plan = plan_fused<T>(rows, k, n);
+    if (plan.blocks)
+      return launch_fused<T>(plan, rows, k, n, x, weight, bias, activation, dy, dx, dweight,
+                             dbias, static_cast<float*>(workspace), s);
+    const T* dz = static_cast<const T*>(dy);
+    if (activation != kNone) {
+      constexpr int P = kOperandParts<T>;
+      const int status = launch_product<T, P, false, T, P, false, T, T, kSlope>(
+          forward_params<T>(rows, k, n, x, weight, bias, dy, activation, workspace), s);
       if (status != kOk) return status;
-      return launch_gradients<T, float, kGradientParts<T>, kSourceParts<T>>(
-          rows, k, n, dz, x, weight, dx, dweight, dbias, partial, s);
-    });
+      dz = static_cast<const T*>(workspace);
+    }
+    float* partial = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                              dz_bytes(dtype, rows, n, activation));
+    return launch_gradients<T>(rows, k, n, dz, x, weight, dx, dweight, dbias, partial, s);
   });
 }
 

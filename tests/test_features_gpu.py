@@ -8,8 +8,8 @@ step) and h = eps(dtype) / 2 for the one rounding to the output's type:
   products' magnitudes;
 * an activation and its slope, 16 u relative, and what their argument is off
   by times their Lipschitz constants (both at most 1.2);
-* a 16-bit upstream times a slope may be held as a pair of 8- or 11-bit
-  parts: 2^-16 relative.
+* 16-bit types take dz = dy act'(z) in their own type: half a step relative
+  (and half their smallest value) of each dz, besides the above.
 """
 
 import math
@@ -95,7 +95,7 @@ def check_linear(x, w, b, r, act, y, grads=None, dy=None):
     if act == "relu":  # the slope jumps where z is within its own error of 0
         e_dz = dyd.abs() * ((z.abs() <= e_z).double() + U)
     if x.dtype != torch.float32:
-        e_dz = e_dz + 2.0 ** -16 * dz.abs()
+        e_dz = e_dz + half_step(x.dtype) * (dz.abs() + e_dz) + smallest(x.dtype)
     dx, dw, db = grads
     if dx is not None:
         check(dx, dz @ wd, (n + 8) * U * (dz.abs() @ wd.abs()) + e_dz @ wd.abs(), "dx")
