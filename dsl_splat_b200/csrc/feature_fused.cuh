@@ -30,6 +30,44 @@ struct FusedParams {
   int* error;
 };
 
+// The same for one-part operands whose rows are 16-byte aligned, by copies that
+// the thread does not wait for.
+template <class S>
+SPLAT_DEV void fill_async(uint32_t dst, int rows, int pieces, const S* src, long long ld,
+                          long long rows_valid, long long cols_valid, int thread, int threads) {
+  const int shift = pieces <= 1 ? 0 : pieces <= 2 ? 1 : pieces <= 4 ? 2 : 3;
+  const int total = rows << shift;
+  const int piece = thread & ((1 << shift) - 1);  // threads is a multiple of 8
+  if (piece >= pieces) return;
+  const long long left = cols_valid - piece * 8;
+  const int bytes = left <= 0 ? 0 : static_cast<int>(left < 8 ? left : 8) * 2;
+  src += piece * 8;
+#pragma unroll 4
+  for (int i = thread; i < total; i += threads) {
+    const int row = i >> shift;
+    const bool in = row < rows_valid && bytes;
+    // a copy of no bytes fills with zeros; its address stays inside the source
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                     dst + row * 128 + ((piece ^ (row & 7)) << 4)),
+                 "l"(in ? src + row * ld : src - piece * 8), "r"(in ? bytes : 0)
+                 : "memory");
+  }
+}
+
+// Waits until at most `lag` groups of the thread's copies are in flight.
+SPLAT_DEV void wait_copies(int lag) {
+  switch (lag) {
+    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+    case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+    case 5: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
+    case 6: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
+    default: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
+  }
+}
+
 constexpr int kFusedThreads = 256;
 constexpr int kFusedWidth = 128;        // widest k and n
 constexpr int kOnesBytes = 16 * 128;    // 16 rows of 64 ones

@@ -20,6 +20,23 @@ int row_vector(const void* base, long long ld) {
   return v;
 }
 
+// The map of a row-major matrix (rows x columns, ld values between rows) for
+// tensor copies of boxes of box_columns x box_rows, swizzled over their row
+// length (64 or 128 bytes) as the kernels' shared layouts are.  False where
+// the matrix cannot be copied so.
+template <class T>
+bool make_map(CUtensorMap& map, const void* base, long long rows, long long columns, long long ld,
+              int box_columns, int box_rows) {
+  if (!base || rows >= 1LL << 31 || !host::aligned(base, 16) || ld * sizeof(T) % 16) return false;
+  return host::encode_map(&map,
+                          sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                          : kIsF16<T>    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                          base, rows, columns, ld * sizeof(T), box_columns, box_rows,
+                          box_columns * sizeof(T) == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                                         : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
 // Shared memory of a block when one or two share an SM (228 KB, of which each
 // block costs 1 KB besides its own), less the barriers and the rounding of the
 // base to 1 KB.
@@ -55,16 +72,24 @@ int launch_product(ProductParams p, cudaStream_t s) {
   const long long chunks = (p.k + kChunk - 1) / kChunk;
   const long long whole_b = chunks * b_bytes;
   p.resident = p.splits == 1 && p.tiles_n == 1 && whole_b <= kMaxResidentBytes;
-  const int fixed = kEpilogueWarps * kStagingBytes + (p.bias_shared * 4 + 1023) / 1024 * 1024 + (p.resident ? static_cast<int>(whole_b) : 0);
+  const int fixed = kEpilogueWarps * staging_bytes<TE, TO, EPI>() + (p.bias_shared * 4 + 1023) / 1024 * 1024 + (p.resident ? static_cast<int>(whole_b) : 0);
   const int stage = a_bytes + (p.resident ? 0 : b_bytes);
   int blocks = 2, budget = kTwoBlocksBytes;
   if (producers(PA, PB) > 128 || p.tmem_columns > 256 || fixed + 2 * stage > budget)
     blocks = 1, budget = kOneBlockBytes;
   p.stages = std::min(kMaxStages, (budget - fixed) / stage);
   if (p.stages < 1) return host::fail(kTooLarge, "feature_linear: no room for a stage");
-  const bool copied = PA == 1 && PB == 1 && p.a_vector == 16 &&
-                      (p.resident || p.b_vector == 16) && sizeof(SA) == 2;
-  p.lag = copied ? p.stages - 1 : 0;
+  if constexpr (PA == 1 && PB == 1) {
+    p.copy_operands =
+        make_map<SA>(p.a_map, p.a, AMN ? p.k : p.m, AMN ? p.m : p.k, p.a_ld, kChunk,
+                     AMN ? kChunk : kTileRows) &&
+        make_map<SB>(p.b_map, p.b, BMN ? p.k : p.n, BMN ? p.n : p.k, p.b_ld, kChunk,
+                     BMN ? kChunk : p.tile_n);
+  }
+  if (EPI != kPlain) p.copy_extra = make_map<TE>(p.extra_map, p.extra, p.m, p.n, p.n, 32, 32);
+  // partial sums are added to or lie one split behind the other
+  if (p.splits == 1 && p.k_per_sum >= p.k)
+    p.copy_out = make_map<TO>(p.out_map, p.out, p.m, p.n, p.n, 32, 32);
   p.error = host::device_error_word();
   if (!p.error) return kCudaError;
   const int bytes = fixed + p.stages * stage + 1024;

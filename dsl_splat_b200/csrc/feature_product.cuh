@@ -7,9 +7,11 @@
 // i + j < parts are summed: three parts reproduce an fp32 product to 2^-24, two
 // a 16-bit value exactly.  Accumulators are fp32 in tensor memory.
 //
-// Work.  A persistent block takes 128 x NT tiles.  Four producer warps move
-// 64-wide chunks of k from global memory into a ring of stages (converting and
-// zero-filling on the way: any row length, any row count), one thread issues
+// Work.  A persistent block takes 128 x NT tiles.  64-wide chunks of k go from
+// global memory into a ring of stages: 16-bit operands with 16-byte rows by
+// tensor copies that one thread starts, all others through four or eight
+// producer warps (converting and zero-filling on the way: any row length, any
+// row count).  One thread issues
 // the products, and eight epilogue warps take the finished accumulator, of which
 // there are two, so that loads, products and epilogues of neighbouring tiles
 // overlap.  Where the whole of B fits beside the ring it is loaded once per
@@ -25,12 +27,16 @@ constexpr int kTileRows = 128;
 constexpr int kChunk = 64;             // k of a stage: 128 bytes of 16-bit values
 constexpr int kEpilogueWarps = 8;                  // epilogue warps
 constexpr int kMaxStages = 8;
-constexpr int kStagingBytes = 4096;    // of an epilogue warp: 32 x 32 fp32
+// Staging memory of an epilogue warp: a patch of the extra values and one of
+// the results.
+template <class TE, class TO, int EPI>
+__host__ __device__ constexpr int staging_bytes() {
+  return 1024 * ((EPI == 2 ? 0 : sizeof(TE)) + sizeof(TO));
+}
 constexpr int kAPlane = kTileRows * 128;
 
-// Producer threads.  One-part operands are copied as they are and the copies
-// wait in the ring; those that are split pass through registers, so there it
-// is threads that keep loads in flight.
+// Producer threads: operands that are split always pass through registers, so
+// there it is threads that keep loads in flight.
 __host__ __device__ constexpr int producers(int pa, int pb) { return pa == 1 && pb == 1 ? 128 : 256; }
 // fp32 operands keep the products of lower parts in an accumulator of their
 // own: the tensor core truncates its sums, so each addition at full magnitude
@@ -44,6 +50,8 @@ constexpr int kExactSum = 512;
 enum Epilogue : int { kForward = 0, kSlope = 1, kPlain = 2 };
 
 struct ProductParams {
+  CUtensorMap a_map, b_map, extra_map, out_map;
+  int copy_operands, copy_extra, copy_out;  // by tensor copies
   long long m, k;  // k of all splits
   int n;
   // row-major sources: A is (m, k) rows or, transposed, (k, m); B likewise
@@ -56,7 +64,6 @@ struct ProductParams {
   int splits, tile_n;
   uint32_t tiles_n, tiles_m, tiles;  // tiles = splits * tiles_m * tiles_n, below 2^31
   int stages, resident, activation;
-  int lag;                 // stages whose copies may be in flight; 0: through registers
   uint32_t tmem_columns;
   const void* bias;   // (n) or NULL
   const void* extra;  // residual or dy (m, n), or NULL
@@ -194,49 +201,11 @@ SPLAT_DEV void fill(int vector, uint32_t dst, uint32_t plane, int rows, int piec
                                 threads);
 }
 
-// The same for one-part operands whose rows are 16-byte aligned, by copies that
-// the thread does not wait for.
-template <class S>
-SPLAT_DEV void fill_async(uint32_t dst, int rows, int pieces, const S* src, long long ld,
-                          long long rows_valid, long long cols_valid, int thread, int threads) {
-  const int shift = pieces <= 1 ? 0 : pieces <= 2 ? 1 : pieces <= 4 ? 2 : 3;
-  const int total = rows << shift;
-  const int piece = thread & ((1 << shift) - 1);  // threads is a multiple of 8
-  if (piece >= pieces) return;
-  const long long left = cols_valid - piece * 8;
-  const int bytes = left <= 0 ? 0 : static_cast<int>(left < 8 ? left : 8) * 2;
-  src += piece * 8;
-#pragma unroll 4
-  for (int i = thread; i < total; i += threads) {
-    const int row = i >> shift;
-    const bool in = row < rows_valid && bytes;
-    // a copy of no bytes fills with zeros; its address stays inside the source
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                     dst + row * 128 + ((piece ^ (row & 7)) << 4)),
-                 "l"(in ? src + row * ld : src - piece * 8), "r"(in ? bytes : 0)
-                 : "memory");
-  }
-}
-
-// Waits until at most `lag` groups of the thread's copies are in flight.
-SPLAT_DEV void wait_copies(int lag) {
-  switch (lag) {
-    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-    case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-    case 5: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
-    case 6: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
-    default: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
-  }
-}
-
 // One operand's chunk: `width` m or n from mn0 and kChunk k from k0 (k_valid of
 // them real).  K-major operands are one block of `width` rows; MN-major ones
 // are blocks of 64 m or n, each of kChunk rows.
 template <class S, int P, bool MN>
-SPLAT_DEV void fill_chunk(bool async, int vector, uint32_t dst, uint32_t plane, int width,
+SPLAT_DEV void fill_chunk(int vector, uint32_t dst, uint32_t plane, int width,
                           const S* src, long long ld, long long mn0, long long mn_valid,
                           long long k0, int k_valid, int thread, int threads) {
   const int rows = MN ? min((k_valid + 15) / 16 * 16, kChunk) : width;
@@ -246,14 +215,27 @@ SPLAT_DEV void fill_chunk(bool async, int vector, uint32_t dst, uint32_t plane, 
     const long long rows_valid = MN ? k_valid : mn_valid;
     const long long cols_valid = MN ? mn_valid - b * 64 : k_valid;
     const uint32_t at = dst + b * (kChunk * 128);
-    if constexpr (P == 1) {
-      if (async) {
-        fill_async<S>(at, rows, pieces, corner, ld, rows_valid, cols_valid, thread, threads);
-        continue;
-      }
-    }
     fill<S, P>(vector, at, plane, rows, pieces, corner, ld, rows_valid, cols_valid, thread,
                threads);
+  }
+}
+
+// The same by tensor copies of boxes of 64 columns (MN-major: of 64 k rows);
+// returns the bytes that will arrive.
+template <bool MN>
+SPLAT_DEV uint32_t chunk_bytes(int width, long long mn_valid) {
+  return MN ? static_cast<uint32_t>(min((mn_valid + 63) / 64, (width + 63LL) / 64)) * (kChunk * 128)
+            : width * 128;
+}
+template <bool MN>
+SPLAT_DEV void copy_chunk(const CUtensorMap* map, uint32_t dst, int width, long long mn0,
+                          long long mn_valid, long long k0, uint32_t bar) {
+  if constexpr (MN) {
+    for (int b = 0; b * 64 < width && b * 64 < mn_valid; ++b)
+      tc::copy_in(dst + b * (kChunk * 128), map, static_cast<int>(mn0) + b * 64,
+                  static_cast<int>(k0), bar);
+  } else {
+    tc::copy_in(dst, map, static_cast<int>(k0), static_cast<int>(mn0), bar);
   }
 }
 
@@ -425,12 +407,13 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
   constexpr int kProducers = producers(PA, PB), kAcc = accumulators(PA, PB);
   extern __shared__ unsigned char dynamic[];
   __shared__ alignas(8) unsigned long long full[kMaxStages], empty[kMaxStages], acc_full[2],
-      acc_empty[2], resident_full, drained;
+      acc_empty[2], resident_full, drained, extra_full[kEpilogueWarps];
   __shared__ uint32_t tmem_base;
   const uint32_t base = (tc::shared_address(dynamic) + 1023u) & ~1023u;
   const uint32_t b_plane = b_plane_bytes<BMN>(p.tile_n);
   const uint32_t a_bytes = PA * kAPlane, b_bytes = PB * b_plane;
-  const uint32_t bias_at = base + kEpilogueWarps * kStagingBytes;
+  constexpr int kStaging = staging_bytes<TE, TO, EPI>();
+  const uint32_t bias_at = base + kEpilogueWarps * kStaging;
   const uint32_t resident = bias_at + (p.bias_shared * 4 + 1023) / 1024 * 1024;
   const int chunks_all = static_cast<int>((p.k + kChunk - 1) / kChunk);
   const uint32_t ring = resident + (p.resident ? chunks_all * b_bytes : 0);
@@ -438,15 +421,18 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
   const int warp = threadIdx.x >> 5;
 
   if (threadIdx.x == 0) {
+    const int arrivals = p.copy_operands ? 1 : kProducers;
+    for (int i = 0; i < kEpilogueWarps; ++i)
+      tc::barrier_init(tc::shared_address(&extra_full[i]), 1);
     for (int i = 0; i < p.stages; ++i) {
-      tc::barrier_init(tc::shared_address(&full[i]), kProducers);
+      tc::barrier_init(tc::shared_address(&full[i]), arrivals);
       tc::barrier_init(tc::shared_address(&empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       tc::barrier_init(tc::shared_address(&acc_full[i]), 1);
       tc::barrier_init(tc::shared_address(&acc_empty[i]), kEpilogueWarps * 32);
     }
-    tc::barrier_init(tc::shared_address(&resident_full), kProducers);
+    tc::barrier_init(tc::shared_address(&resident_full), arrivals);
     tc::barrier_init(tc::shared_address(&drained), 1);
     tc::barrier_init_fence();
   }
@@ -466,53 +452,67 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
   if (warp >= kEpilogueWarps && warp < kEpilogueWarps + kProducers / 32) {
     // ---- producers
     const int thread = threadIdx.x - kEpilogueWarps * 32;
-    const SA* a = static_cast<const SA*>(p.a);
-    const SB* b = static_cast<const SB*>(p.b);
-    if (p.resident) {
-      for (int c = 0; c < chunks_all; ++c)
-        fill_chunk<SB, PB, BMN>(false, p.b_vector, resident + c * b_bytes, b_plane, p.tile_n, b, p.b_ld,
-                                0, p.n, static_cast<long long>(c) * kChunk,
-                                static_cast<int>(min(p.k - static_cast<long long>(c) * kChunk,
-                                                     static_cast<long long>(kChunk))),
-                                thread, kProducers);
-      tc::fence_async_proxy();
-      tc::barrier_arrive(tc::shared_address(&resident_full));
-    }
-    int stage = 0, in_flight = 0, landed = 0;
+    int stage = 0;
     uint32_t parity = 1;  // a fresh barrier's previous phase counts as complete
-    for (uint32_t t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
-      const ProductTile tile(p, t);
-      for (long long k = tile.k0; k < tile.k1; k += kChunk) {
-        if (!(ok = tc::barrier_wait(tc::shared_address(&empty[stage]), parity))) break;
-        const uint32_t at = ring + stage * stage_bytes;
-        const int k_valid = static_cast<int>(min(tile.k1 - k, static_cast<long long>(kChunk)));
-        fill_chunk<SA, PA, AMN>(p.lag, p.a_vector, at, kAPlane, kTileRows, a, p.a_ld, tile.m0,
-                                p.m - tile.m0, k, k_valid, thread, kProducers);
-        if (!p.resident)
-          fill_chunk<SB, PB, BMN>(p.lag, p.b_vector, at + a_bytes, b_plane, p.tile_n, b, p.b_ld,
-                                  tile.n0, p.n - tile.n0, k, k_valid, thread, kProducers);
-        if (p.lag) {
-          asm volatile("cp.async.commit_group;" ::: "memory");
-          if (++in_flight > p.lag) {
-            wait_copies(p.lag);
-            tc::fence_async_proxy();
-            tc::barrier_arrive(tc::shared_address(&full[landed]));
-            if (++landed == p.stages) landed = 0;
-            --in_flight;
+    if (PA == 1 && PB == 1 && p.copy_operands) {
+      if (thread == 0) {
+        if (p.resident) {
+          const uint32_t bar = tc::shared_address(&resident_full);
+          tc::barrier_expect(bar, chunks_all * chunk_bytes<BMN>(p.tile_n, p.n));
+          for (int c = 0; c < chunks_all; ++c)
+            copy_chunk<BMN>(&p.b_map, resident + c * b_bytes, p.tile_n, 0, p.n,
+                            static_cast<long long>(c) * kChunk, bar);
+        }
+        int started = 0;  // stages that have been filled at least once
+        for (uint32_t t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+          const ProductTile tile(p, t);
+          for (long long k = tile.k0; k < tile.k1; k += kChunk) {
+            if (!(ok = tc::barrier_wait(tc::shared_address(&empty[stage]), parity))) break;
+            const uint32_t at = ring + stage * stage_bytes, bar = tc::shared_address(&full[stage]);
+            tc::barrier_expect(bar,
+                               chunk_bytes<AMN>(kTileRows, p.m - tile.m0) +
+                                   (p.resident ? 0 : chunk_bytes<BMN>(p.tile_n, p.n - tile.n0)));
+            copy_chunk<AMN>(&p.a_map, at, kTileRows, tile.m0, p.m - tile.m0, k, bar);
+            if (!p.resident)
+              copy_chunk<BMN>(&p.b_map, at + a_bytes, p.tile_n, tile.n0, p.n - tile.n0, k, bar);
+            started = max(started, stage + 1);
+            if (++stage == p.stages) stage = 0, parity ^= 1;
           }
-        } else {
+        }
+        // no copy is in flight past this point, also after a wait that ran out:
+        // parity ^ 1 is the phase of the ring's current round, parity the last one's
+        if (p.resident) ok = tc::barrier_wait(tc::shared_address(&resident_full), 0) && ok;
+        for (int i = 0; i < started; ++i)
+          ok = tc::barrier_wait(tc::shared_address(&full[i]), i < stage ? parity ^ 1 : parity) && ok;
+      }
+    } else {
+      const SA* a = static_cast<const SA*>(p.a);
+      const SB* b = static_cast<const SB*>(p.b);
+      if (p.resident) {
+        for (int c = 0; c < chunks_all; ++c)
+          fill_chunk<SB, PB, BMN>(p.b_vector, resident + c * b_bytes, b_plane, p.tile_n, b, p.b_ld,
+                                  0, p.n, static_cast<long long>(c) * kChunk,
+                                  static_cast<int>(min(p.k - static_cast<long long>(c) * kChunk,
+                                                       static_cast<long long>(kChunk))),
+                                  thread, kProducers);
+        tc::fence_async_proxy();
+        tc::barrier_arrive(tc::shared_address(&resident_full));
+      }
+      for (uint32_t t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+        const ProductTile tile(p, t);
+        for (long long k = tile.k0; k < tile.k1; k += kChunk) {
+          if (!(ok = tc::barrier_wait(tc::shared_address(&empty[stage]), parity))) break;
+          const uint32_t at = ring + stage * stage_bytes;
+          const int k_valid = static_cast<int>(min(tile.k1 - k, static_cast<long long>(kChunk)));
+          fill_chunk<SA, PA, AMN>(p.a_vector, at, kAPlane, kTileRows, a, p.a_ld, tile.m0,
+                                  p.m - tile.m0, k, k_valid, thread, kProducers);
+          if (!p.resident)
+            fill_chunk<SB, PB, BMN>(p.b_vector, at + a_bytes, b_plane, p.tile_n, b, p.b_ld,
+                                    tile.n0, p.n - tile.n0, k, k_valid, thread, kProducers);
           tc::fence_async_proxy();
           tc::barrier_arrive(tc::shared_address(&full[stage]));
+          if (++stage == p.stages) stage = 0, parity ^= 1;
         }
-        if (++stage == p.stages) stage = 0, parity ^= 1;
-      }
-    }
-    if (p.lag) {
-      wait_copies(0);
-      tc::fence_async_proxy();
-      for (; in_flight; --in_flight) {
-        tc::barrier_arrive(tc::shared_address(&full[landed]));
-        if (++landed == p.stages) landed = 0;
       }
     }
   } else if (warp == kEpilogueWarps + kProducers / 32) {
@@ -578,9 +578,25 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
   } else if (warp < kEpilogueWarps) {
     // ---- epilogue
     const int lane_block = warp & 3, half = warp >> 2;
-    const Patch<TE> extra_patch{base + warp * kStagingBytes};
-    const Patch<TO> out_patch{base + warp * kStagingBytes};
-    uint32_t acc = 0, parity = 0;
+    constexpr bool kExtra = EPI != kPlain;
+    const Patch<TE> extra_patch{base + warp * kStaging + 1024 * static_cast<int>(sizeof(TO))};
+    const Patch<TO> out_patch{base + warp * kStaging};
+    const bool leader = (threadIdx.x & 31) == 0;
+    const uint32_t extra_bar = tc::shared_address(&extra_full[warp]);
+    uint32_t acc = 0, parity = 0, extra_parity = 0;
+    bool extra_coming = false;
+    // starts the copy of the extra values of a tile's patch
+    const auto fetch_extra = [&](const ProductTile& tile, int c) {
+      const long long row0 = tile.m0 + lane_block * 32;
+      if (c * 32 >= p.tile_n || tile.n0 + c * 32 >= p.n || row0 >= p.m) return;
+      if (leader) {
+        tc::barrier_expect(extra_bar, 1024 * sizeof(TE));
+        tc::copy_in(extra_patch.base, &p.extra_map, tile.n0 + c * 32, static_cast<int>(row0),
+                    extra_bar);
+      }
+      extra_coming = true;
+    };
+    if (kExtra && p.copy_extra) fetch_extra(ProductTile(p, blockIdx.x), half);
     for (uint32_t t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
       const ProductTile tile(p, t);
       const long long row0 = tile.m0 + lane_block * 32;
@@ -591,8 +607,8 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
         for (int c = half; c * 32 < p.tile_n; c += kEpilogueWarps / 4) {
           const int col0 = tile.n0 + c * 32, cols = min(p.n - col0, 32);
           if (cols <= 0 || rows <= 0) break;
-          __syncwarp();  // the patch before has been read
-          if (EPI != kPlain && p.extra) {
+          if (kExtra && p.extra && !p.copy_extra) {
+            __syncwarp();  // the patch before has been read
             extra_patch.load(static_cast<const TE*>(p.extra) + row0 * p.n + col0, p.n, rows, cols,
                              p.extra_vector);
             __syncwarp();
@@ -611,7 +627,7 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] += low[i];
           }
-          if constexpr (EPI != kPlain) {
+          if constexpr (kExtra) {
             if (p.bias) {
               if (p.bias_shared) {
 #pragma unroll
@@ -629,6 +645,11 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
                   if (j < cols) v[j] += to_float(bias[j]);
               }
             }
+            if (p.copy_extra) {
+              if (!(ok = tc::barrier_wait(extra_bar, extra_parity))) break;
+              extra_parity ^= 1;
+              extra_coming = false;
+            }
             const bool e = p.extra;
             switch (p.activation) {
               case kRelu: finish_row<EPI, kRelu, TE>(extra_patch, e, v); break;
@@ -637,8 +658,17 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
               case kSigmoid: finish_row<EPI, kSigmoid, TE>(extra_patch, e, v); break;
               default: finish_row<EPI, kNone, TE>(extra_patch, e, v);
             }
-            if (sizeof(TE) != sizeof(TO)) __syncwarp();  // the two patches' rows differ
+            if (p.copy_extra) {  // the next patch's, once this one has been read
+              __syncwarp();
+              const int next = c + kEpilogueWarps / 4;
+              if (next * 32 < p.tile_n && tile.n0 + next * 32 < p.n)
+                fetch_extra(tile, next);
+              else if (p.tiles - t > gridDim.x)
+                fetch_extra(ProductTile(p, t + gridDim.x), half);
+            }
           }
+          if (leader && p.copy_out) tc::copies_out_read();
+          __syncwarp();  // the results before have left the patch
 #pragma unroll
           for (int j = 0; j < Patch<TO>::kPieces; ++j) {
             constexpr int V = Patch<TO>::V;
@@ -648,12 +678,20 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
             const Vec<TO, V> r = round_values<TO, V>(o);
             store_shared(out_patch.at(threadIdx.x & 31, j), reinterpret_cast<const uint4&>(r));
           }
-          __syncwarp();
-          out_patch.store(out + col0, p.n, rows, cols, p.out_vector, sum_k != tile.k0);
+          if (p.copy_out) {
+            tc::fence_async_proxy();
+            __syncwarp();
+            if (leader) tc::copy_out(&p.out_map, col0, static_cast<int>(row0), out_patch.base);
+          } else {
+            __syncwarp();
+            out_patch.store(out + col0, p.n, rows, cols, p.out_vector, sum_k != tile.k0);
+          }
         }
         if (!ok) break;
         if (!waited) {  // a warp without a patch still takes part
           if (!(ok = tc::barrier_wait(tc::shared_address(&acc_full[acc]), parity))) break;
+          if (kExtra && p.copy_extra && !extra_coming && p.tiles - t > gridDim.x)
+            fetch_extra(ProductTile(p, t + gridDim.x), half);
         }
         tc::fence_before_sync();
         tc::barrier_arrive(tc::shared_address(&acc_empty[acc]));
@@ -661,6 +699,8 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
         if (acc == 0) parity ^= 1;
       }
     }
+    if (extra_coming) ok = tc::barrier_wait(extra_bar, extra_parity) && ok;
+    if (leader && p.copy_out) tc::copies_out_read();
   }
   if (!ok) atomicCAS(p.error, 0, kDeviceTimeout);
   tc::fence_before_sync();

@@ -2,6 +2,7 @@
 // reporting (splat_last_error), the launch counter (splat_launch_count) and
 // argument checks.  Defined in splat200.cu.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstddef>
@@ -20,6 +21,11 @@ cudaStream_t counted(cudaStream_t s);
 // The current device's error word (splat_device_error), or NULL with the CUDA
 // error recorded.
 int* device_error_word();
+// A tensor map of a row-major matrix for boxes of box_columns x box_rows;
+// false when the driver does not make one.
+bool encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows,
+                long long columns, long long row_bytes, int box_columns, int box_rows,
+                CUtensorMapSwizzle swizzle);
 // Streaming multiprocessors of the current device (148 on B200).
 int sm_count();
 

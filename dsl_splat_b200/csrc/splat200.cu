@@ -63,6 +63,33 @@ int* device_error_word() {
   return static_cast<int*>(word);
 }
 
+bool encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows,
+                long long columns, long long row_bytes, int box_columns, int box_rows,
+                CUtensorMapSwizzle swizzle) {
+  using Encode = decltype(&cuTensorMapEncodeTiled);
+  // the driver is reached through the runtime, so that the library links
+  // without libcuda
+  static const Encode encode = [] {
+    void* entry = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000,
+                                         cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      entry = nullptr;
+    cudaGetLastError();
+    return reinterpret_cast<Encode>(entry);
+  }();
+  if (!encode) return false;
+  const cuuint64_t size[2] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t stride[1] = {static_cast<cuuint64_t>(row_bytes)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_columns),
+                             static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t step[2] = {1, 1};
+  return encode(map, type, 2, const_cast<void*>(base), size, stride, box, step,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int sm_count() {
   int sms = 148, dev = 0;
   if (cudaGetDevice(&dev) == cudaSuccess)

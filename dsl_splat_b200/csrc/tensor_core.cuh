@@ -2,6 +2,7 @@
 // mbarriers with bounded waits, tensor memory, and tcgen05.mma on operands in
 // 128-byte-swizzled shared memory.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -26,25 +27,66 @@ SPLAT_DEV void barrier_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// Polls of one wait before it gives up; each poll suspends for a while in
-// hardware, so this is seconds.
-constexpr int kPollLimit = 1 << 22;
+// Nanoseconds after which a wait gives up, and the time that one poll may
+// sleep in hardware.
+constexpr unsigned long long kWaitLimit = 2000000000ull;
+constexpr uint32_t kPollSleep = 100000;
+
+SPLAT_DEV bool barrier_poll(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity), "r"(kPollSleep)
+      : "memory");
+  return done;
+}
+SPLAT_DEV unsigned long long nanoseconds() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
 
 // Waits for the phase of the given parity to complete.  False when the limit
 // runs out: the caller records an error and leaves.
 SPLAT_DEV bool barrier_wait(uint32_t bar, uint32_t parity) {
-  for (int i = 0; i < kPollLimit; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (done) return true;
-  }
-  return false;
+  if (barrier_poll(bar, parity)) return true;
+  const unsigned long long start = nanoseconds();
+  while (!barrier_poll(bar, parity))
+    if (nanoseconds() - start > kWaitLimit) return false;
+  return true;
+}
+
+// One arrival, and bytes that copies will bring before the phase completes.
+SPLAT_DEV void barrier_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+
+// ---- tensor copies -----------------------------------------------------------
+
+// A box of a row-major matrix at (column, row) of global memory, whose
+// out-of-range values read as zeros, into shared memory; the barrier is told.
+SPLAT_DEV void copy_in(uint32_t dst, const CUtensorMap* map, int column, int row, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(column), "r"(row), "r"(bar)
+      : "memory");
+}
+// The reverse; out-of-range values are not written.
+SPLAT_DEV void copy_out(const CUtensorMap* map, int column, int row, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   map),
+               "r"(column), "r"(row), "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// Until the sources of this thread's copy_outs may be written again.
+SPLAT_DEV void copies_out_read() {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
 // Orders this thread's shared-memory accesses before later accesses of the
