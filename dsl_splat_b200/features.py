@@ -39,50 +39,57 @@ from . import stages
 ACTIVATIONS = stages.ACTIVATIONS
 
 
+def _once(backward):
+    """once_differentiable, whose cost only a backward that is recorded pays."""
+    recorded = once_differentiable(backward)
+
+    def run(ctx, *upstream):
+        return (recorded if torch.is_grad_enabled() else backward)(ctx, *upstream)
+
+    return run
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: Tensor, weight: Tensor, bias: Tensor | None,
-                residual: Tensor | None, activation: str, grad_enabled: bool) -> Tensor:
-        y = stages.feature_linear(x, weight, bias, residual, activation)
-        if grad_enabled and any(ctx.needs_input_grad[:4]):
-            ctx.save_for_backward(x, weight, bias)
-            ctx.activation = activation
+                residual: Tensor | None, activation: str) -> Tensor:
+        ctx.save_for_backward(x, weight, bias)
+        ctx.activation = activation
         ctx.set_materialize_grads(False)
-        return y
+        return stages.feature_linear(x, weight, bias, residual, activation)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx: Any, upstream: Tensor | None):
         if upstream is None:
-            return (None,) * 6
+            return (None,) * 5
         x, weight, bias = ctx.saved_tensors
         needs = ctx.needs_input_grad
         dx, dweight, dbias = stages.feature_linear_backward(
-            x, weight, bias, ctx.activation, upstream, tuple(needs[:3]))
-        return dx, dweight, dbias, upstream if needs[3] else None, None, None
+            x, weight, bias, ctx.activation, upstream, needs[:3])
+        return dx, dweight, dbias, upstream if needs[3] else None, None
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: Tensor, weight: Tensor | None, bias: Tensor | None, groups: int,
-                eps: float, activation: str, grad_enabled: bool) -> Tensor:
-        y, mean, rstd = stages.feature_norm(x, groups, weight, bias, eps, activation)
-        if grad_enabled and any(ctx.needs_input_grad[:3]):
-            ctx.save_for_backward(x, weight, bias, mean, rstd)
-            ctx.groups, ctx.activation = groups, activation
+                eps: float, activation: str) -> Tensor:
+        y, moments = stages.feature_norm(x, groups, weight, bias, eps, activation)
+        ctx.save_for_backward(x, weight, bias, moments)
+        ctx.groups, ctx.activation = groups, activation
         ctx.set_materialize_grads(False)
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx: Any, upstream: Tensor | None):
         if upstream is None:
-            return (None,) * 7
-        x, weight, bias, mean, rstd = ctx.saved_tensors
+            return (None,) * 6
+        x, weight, bias, moments = ctx.saved_tensors
         dx, dweight, dbias = stages.feature_norm_backward(
-            x, ctx.groups, weight, bias, mean, rstd, ctx.activation, upstream,
-            tuple(ctx.needs_input_grad[:3]))
-        return dx, dweight, dbias, None, None, None, None
+            x, ctx.groups, weight, bias, moments, ctx.activation, upstream,
+            ctx.needs_input_grad[:3])
+        return dx, dweight, dbias, None, None, None
 
 
 def _check_activation(activation: str) -> None:
@@ -98,10 +105,15 @@ def _check_input(x: Tensor) -> None:
 def _check_like(t: Tensor | None, x: Tensor, shape: tuple, name: str) -> None:
     if t is None:
         return
-    if not isinstance(t, Tensor) or t.device != x.device or t.dtype != x.dtype:
+    if not isinstance(t, Tensor) or t.dtype is not x.dtype or t.device != x.device:
         raise ValueError(f"{name} must have x's dtype and device")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _recorded(*tensors: Tensor | None) -> bool:
+    """Whether autograd has to know of a call."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *,
@@ -121,15 +133,20 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *,
     n = weight.shape[0]
     _check_like(weight, x, (n, k), "weight")
     _check_like(bias, x, (n,), "bias")
-    shape = tuple(x.shape[:-1]) + (n,)
+    shape = x.shape[:-1] + (n,)
     _check_like(residual, x, shape, "residual")
-    if max(k, n) > 65535:
+    if k > 65535 or n > 65535:
         raise ValueError("at most 65535 input and output features")
-    rows = math.prod(x.shape[:-1])  # explicit: with no rows a -1 dimension is ambiguous
-    y = _Linear.apply(x.reshape(rows, k), weight, bias,
-                      None if residual is None else residual.reshape(rows, n), activation,
-                      torch.is_grad_enabled())
-    return y.reshape(shape)
+    flat = x.ndim == 2
+    if not flat:
+        rows = math.prod(x.shape[:-1])  # explicit: with no rows a -1 dimension is ambiguous
+        x = x.reshape(rows, k)
+        residual = None if residual is None else residual.reshape(rows, n)
+    if _recorded(x, weight, bias, residual):
+        y = _Linear.apply(x, weight, bias, residual, activation)
+    else:
+        y = stages.feature_linear(x, weight, bias, residual, activation)
+    return y if flat else y.reshape(shape)
 
 
 def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tensor | None = None,
@@ -161,9 +178,13 @@ def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tenso
     positions = math.prod(x.shape[-1 - spatial_dims:-1])
     if positions > (1 << 31) - 1 or positions * channels > 1 << 40 or samples * channels > 1 << 30:
         raise ValueError("too many positions or samples")
-    y = _GroupNorm.apply(x.reshape(samples, positions, channels), weight, bias, int(groups),
-                         float(eps), activation, torch.is_grad_enabled())
-    return y.reshape(x.shape)
+    shape = x.shape
+    x = x.reshape(samples, positions, channels)
+    if _recorded(x, weight, bias):
+        y = _GroupNorm.apply(x, weight, bias, int(groups), float(eps), activation)
+    else:
+        y = stages.feature_norm(x, groups, weight, bias, eps, activation)[0]
+    return y.reshape(shape)
 
 
 @dataclass(slots=True)

@@ -672,26 +672,61 @@ def render_backward(state: ProjectedFootprint, bins: dict, feat_a: Tensor,
 
 
 # ---- feature operators -------------------------------------------------------
+#
+# Small calls are bound by the host, so these spare what a call does not need:
+# a device guard on the current device, a Stream object, copies of references.
 
 FEATURE_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = ("none", "relu", "silu", "gelu", "sigmoid")
+_ACTIVATION_CODES = {name: code for code, name in enumerate(ACTIVATIONS)}
 
 
-def _workspace(nbytes: int, like: Tensor) -> Tensor:
-    return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+def _call(fn, what: str, device: torch.device, *args) -> None:
+    """fn(*args, stream) on the device's current stream."""
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        status = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, stream)
+    if status:
+        check(status, what)
+
+
+def _query(fn, what: str, device: torch.device, *args) -> int:
+    """A workspace size, which goes by the device's number of multiprocessors."""
+    if torch._C._cuda_getDevice() == device.index:
+        size = fn(*args)
+    else:
+        with torch.cuda.device(device.index):
+            size = fn(*args)
+    if not size:
+        raise nv.SplatError(f"{what}: {lib.splat_last_error().decode(errors='replace')}")
+    return size
+
+
+def _dense(t: Tensor | None) -> Tensor | None:
+    """_c without the call where nothing is to be done."""
+    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
+        return t
+    return _c(t)
+
+
+def _address(t: Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 def feature_linear(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None,
                    activation: str) -> Tensor:
     """act(x weight^T + bias) + residual for x (M,K), weight (N,K)."""
-    pin = Args()
-    (m, k), n = x.shape, len(weight)
+    (m, k), n = x.shape, weight.shape[0]
     y = x.new_empty((m, n))
-    if y.numel():
-        with torch.cuda.device(x.device):
-            check(lib.splat_feature_linear(
-                FEATURE_DTYPES[x.dtype], m, k, n, pin(x), pin(weight), pin(bias), pin(residual),
-                ACTIVATIONS.index(activation), ptr(y), _stream(x)), "feature_linear")
+    if m:
+        x, weight, bias, residual = _dense(x), _dense(weight), _dense(bias), _dense(residual)
+        _call(lib.splat_feature_linear, "feature_linear", x.device, FEATURE_DTYPES[x.dtype], m, k,
+              n, x.data_ptr(), weight.data_ptr(), _address(bias), _address(residual),
+              _ACTIVATION_CODES[activation], y.data_ptr())
     return y
 
 
@@ -699,70 +734,64 @@ def feature_linear_backward(x: Tensor, weight: Tensor, bias: Tensor | None, acti
                             upstream: Tensor, needs: tuple[bool, bool, bool]
                             ) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
     """Gradients of x, weight and bias (None where not needed)."""
-    pin = Args()
-    (m, k), n = x.shape, len(weight)
-    dx = x.new_empty((m, k)) if needs[0] else None
-    dweight = x.new_empty((n, k)) if needs[1] else None
-    dbias = x.new_empty((n,)) if needs[2] else None
-    if m == 0:
-        for g in (dweight, dbias):
-            if g is not None:
-                g.zero_()
-    elif any(needs):
-        dtype, act = FEATURE_DTYPES[x.dtype], ACTIVATIONS.index(activation)
-        size = lib.splat_feature_linear_backward_workspace_bytes(dtype, m, k, n, act)
-        ws = _workspace(size, x)
-        with torch.cuda.device(x.device):
-            check(lib.splat_feature_linear_backward(
-                dtype, m, k, n, pin(x), pin(weight), pin(bias), act, pin(upstream), ptr(dx),
-                ptr(dweight), ptr(dbias), ptr(ws), size, _stream(x)), "feature_linear_backward")
+    (m, k), n = x.shape, weight.shape[0]
+    make = x.new_empty if m else x.new_zeros
+    dx = make((m, k)) if needs[0] else None
+    dweight = make((n, k)) if needs[1] else None
+    dbias = make((n,)) if needs[2] else None
+    if m and any(needs):
+        dtype, act, device = FEATURE_DTYPES[x.dtype], _ACTIVATION_CODES[activation], x.device
+        size = _query(lib.splat_feature_linear_backward_workspace_bytes,
+                      "feature_linear_backward", device, dtype, m, k, n, act)
+        ws = x.new_empty((size,), dtype=torch.uint8)
+        x, weight, bias, upstream = _dense(x), _dense(weight), _dense(bias), _dense(upstream)
+        _call(lib.splat_feature_linear_backward, "feature_linear_backward", device, dtype, m, k,
+              n, x.data_ptr(), weight.data_ptr(), _address(bias), act, upstream.data_ptr(),
+              _address(dx), _address(dweight), _address(dbias), ws.data_ptr(), size)
     return dx, dweight, dbias
 
 
 def feature_norm(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None, eps: float,
-                 activation: str) -> tuple[Tensor, Tensor, Tensor]:
-    """Group norm with an activation of x (B,S,C): y and the (B,groups) fp32 mean
-    and reciprocal deviation."""
-    pin = Args()
+                 activation: str) -> tuple[Tensor, Tensor]:
+    """Group norm with an activation of x (B,S,C): y, and the fp32 means and
+    reciprocal deviations (2,B,groups)."""
     samples, positions, channels = x.shape
-    y = torch.empty((samples, positions, channels), dtype=x.dtype, device=x.device)
-    mean, rstd = torch.empty((2, samples, groups), dtype=torch.float32, device=x.device)
-    if y.numel():
-        dtype = FEATURE_DTYPES[x.dtype]
-        size = lib.splat_feature_norm_workspace_bytes(dtype, samples, positions, channels,
-                                                      groups, 0)
-        ws = _workspace(size, x)
-        with torch.cuda.device(x.device):
-            check(lib.splat_feature_norm(
-                dtype, samples, positions, channels, groups, pin(x), pin(weight), pin(bias), eps,
-                ACTIVATIONS.index(activation), ptr(y), ptr(mean), ptr(rstd), ptr(ws), size,
-                _stream(x)), "feature_norm")
-    return y, mean, rstd
+    y = x.new_empty((samples, positions, channels))
+    moments = x.new_empty((2, samples, groups), dtype=torch.float32)
+    if samples and positions:
+        dtype, device = FEATURE_DTYPES[x.dtype], x.device
+        size = _query(lib.splat_feature_norm_workspace_bytes, "feature_norm", device, dtype,
+                      samples, positions, channels, groups, 0)
+        ws = x.new_empty((size,), dtype=torch.uint8)
+        x, weight, bias = _dense(x), _dense(weight), _dense(bias)
+        mean = moments.data_ptr()
+        _call(lib.splat_feature_norm, "feature_norm", device, dtype, samples, positions, channels,
+              groups, x.data_ptr(), _address(weight), _address(bias), eps,
+              _ACTIVATION_CODES[activation], y.data_ptr(), mean, mean + 4 * samples * groups,
+              ws.data_ptr(), size)
+    return y, moments
 
 
 def feature_norm_backward(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None,
-                          mean: Tensor, rstd: Tensor, activation: str, upstream: Tensor,
+                          moments: Tensor, activation: str, upstream: Tensor,
                           needs: tuple[bool, bool, bool]
                           ) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
     """Gradients of x, weight and bias (None where not needed)."""
-    pin = Args()
     samples, positions, channels = x.shape
-    dx = (torch.empty((samples, positions, channels), dtype=x.dtype, device=x.device)
-          if needs[0] else None)
-    dweight = x.new_empty((channels,)) if needs[1] else None
-    dbias = x.new_empty((channels,)) if needs[2] else None
-    if samples * positions == 0:
-        for g in (dweight, dbias):
-            if g is not None:
-                g.zero_()
-    elif any(needs):
-        dtype = FEATURE_DTYPES[x.dtype]
-        size = lib.splat_feature_norm_workspace_bytes(dtype, samples, positions, channels,
-                                                      groups, 1)
-        ws = _workspace(size, x)
-        with torch.cuda.device(x.device):
-            check(lib.splat_feature_norm_backward(
-                dtype, samples, positions, channels, groups, pin(x), pin(weight), pin(bias),
-                ptr(mean), ptr(rstd), ACTIVATIONS.index(activation), pin(upstream), ptr(dx),
-                ptr(dweight), ptr(dbias), ptr(ws), size, _stream(x)), "feature_norm_backward")
+    values = samples and positions
+    make = x.new_empty if values else x.new_zeros
+    dx = make((samples, positions, channels)) if needs[0] else None
+    dweight = make((channels,)) if needs[1] else None
+    dbias = make((channels,)) if needs[2] else None
+    if values and any(needs):
+        dtype, device = FEATURE_DTYPES[x.dtype], x.device
+        size = _query(lib.splat_feature_norm_workspace_bytes, "feature_norm_backward", device,
+                      dtype, samples, positions, channels, groups, 1)
+        ws = x.new_empty((size,), dtype=torch.uint8)
+        x, weight, bias, upstream = _dense(x), _dense(weight), _dense(bias), _dense(upstream)
+        mean = moments.data_ptr()
+        _call(lib.splat_feature_norm_backward, "feature_norm_backward", device, dtype, samples,
+              positions, channels, groups, x.data_ptr(), _address(weight), _address(bias), mean,
+              mean + 4 * samples * groups, _ACTIVATION_CODES[activation], upstream.data_ptr(),
+              _address(dx), _address(dweight), _address(dbias), ws.data_ptr(), size)
     return dx, dweight, dbias

@@ -544,39 +544,37 @@ feature_linear.register_autograd(_feature_linear_backward, setup_context=_featur
 
 @torch.library.custom_op(f"{_NS}::feature_norm", mutates_args=())
 def feature_norm(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None, eps: float,
-                 activation: str) -> tuple[Tensor, Tensor, Tensor]:
-    y, mean, rstd = stages.feature_norm(x, groups, weight, bias, eps, activation)
-    return y, mean, rstd.clone()  # an operator's outputs share no storage
+                 activation: str) -> tuple[Tensor, Tensor]:
+    return stages.feature_norm(x, groups, weight, bias, eps, activation)
 
 
 @feature_norm.register_fake
 def _(x, groups, weight, bias, eps, activation):
-    moments = x.new_empty((x.shape[0], groups), dtype=torch.float32)
-    return x.new_empty(x.shape), moments, torch.empty_like(moments)
+    return x.new_empty(x.shape), x.new_empty((2, x.shape[0], groups), dtype=torch.float32)
 
 
 @torch.library.custom_op(f"{_NS}::feature_norm_backward", mutates_args=())
 def feature_norm_backward(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None,
-                          mean: Tensor, rstd: Tensor, activation: str, upstream: Tensor
+                          moments: Tensor, activation: str, upstream: Tensor
                           ) -> tuple[Tensor, Tensor, Tensor]:
-    return stages.feature_norm_backward(x, groups, weight, bias, mean, rstd, activation,
-                                        upstream, (True, True, True))
+    return stages.feature_norm_backward(x, groups, weight, bias, moments, activation, upstream,
+                                        (True, True, True))
 
 
 @feature_norm_backward.register_fake
-def _(x, groups, weight, bias, mean, rstd, activation, upstream):
+def _(x, groups, weight, bias, moments, activation, upstream):
     return (x.new_empty(x.shape), x.new_empty((x.shape[-1],)), x.new_empty((x.shape[-1],)))
 
 
 def _feature_norm_setup(ctx, inputs, output):
     x, ctx.groups, weight, bias, _eps, ctx.activation = inputs
-    ctx.save_for_backward(x, weight, bias, output[1], output[2])
+    ctx.save_for_backward(x, weight, bias, output[1])
 
 
-def _feature_norm_backward(ctx, upstream, _mean, _rstd):
-    x, weight, bias, mean, rstd = ctx.saved_tensors
-    dx, dw, db = torch.ops.splat200.feature_norm_backward(x, ctx.groups, weight, bias, mean,
-                                                          rstd, ctx.activation, upstream)
+def _feature_norm_backward(ctx, upstream, _moments):
+    x, weight, bias, moments = ctx.saved_tensors
+    dx, dw, db = torch.ops.splat200.feature_norm_backward(x, ctx.groups, weight, bias, moments,
+                                                          ctx.activation, upstream)
     return (dx, None, None if weight is None else dw, None if bias is None else db, None, None)
 
 

@@ -82,11 +82,11 @@ def test_fake_shapes():
         dx, dw, db = torch.ops.splat200.feature_linear_backward(x, w, None, "silu", y)
         assert dx.shape == x.shape and dw.shape == w.shape and db.shape == (6,)
         v = torch.empty(2, 50, 12, device="cuda", dtype=torch.float16)
-        y, mean, rstd = torch.ops.splat200.feature_norm(v, 3, None, None, 1e-5, "none")
-        assert y.shape == v.shape and mean.shape == rstd.shape == (2, 3)
-        assert mean.dtype == torch.float32
-        dx, dw, db = torch.ops.splat200.feature_norm_backward(v, 3, None, None, mean, rstd,
-                                                              "none", y)
+        y, moments = torch.ops.splat200.feature_norm(v, 3, None, None, 1e-5, "none")
+        assert y.shape == v.shape and moments.shape == (2, 2, 3)
+        assert moments.dtype == torch.float32
+        dx, dw, db = torch.ops.splat200.feature_norm_backward(v, 3, None, None, moments, "none",
+                                                              y)
         assert dx.shape == v.shape and dw.shape == db.shape == (12,)
 
 
