@@ -62,48 +62,152 @@ struct NormParams {
   float eps;
 };
 
-template <class T, int V>
-SPLAT_DEV void load_values(const T* base, long long at, long long span, float (&v)[V], float fill) {
-  if (at + V <= span) {
-    const Vec<T, V> r = *reinterpret_cast<const Vec<T, V>*>(base + at);
+// V fp32 values as packed pairs (one plain value when V is 1): what a thread
+// keeps of its channels, and the arithmetic on them.
+template <int V>
+struct Pairs {
+  static constexpr int N = (V + 1) / 2;
+  f32x2 v[N];
+  SPLAT_DEV void set(const float (&x)[V]) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = to_float(r.v[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = at + j < span ? to_float(base[at + j]) : fill;
+    for (int i = 0; i < N; ++i) v[i] = pack2(x[2 * i], V == 1 ? 0.0f : x[2 * i + 1 < V ? 2 * i + 1 : 0]);
   }
+  SPLAT_DEV void get(float (&x)[V]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float a, b;
+      unpack2(v[i], a, b);
+      x[2 * i] = a;
+      if (2 * i + 1 < V) x[2 * i + 1] = b;
+    }
+  }
+};
+template <int V>
+SPLAT_DEV Pairs<V> operator+(Pairs<V> a, const Pairs<V>& b) {
+#pragma unroll
+  for (int i = 0; i < Pairs<V>::N; ++i) a.v[i] = add2(a.v[i], b.v[i]);
+  return a;
+}
+template <int V>
+SPLAT_DEV Pairs<V> operator*(Pairs<V> a, const Pairs<V>& b) {
+#pragma unroll
+  for (int i = 0; i < Pairs<V>::N; ++i) a.v[i] = mul2(a.v[i], b.v[i]);
+  return a;
+}
+template <int V>
+SPLAT_DEV Pairs<V> fma(Pairs<V> a, const Pairs<V>& b, const Pairs<V>& c) {
+#pragma unroll
+  for (int i = 0; i < Pairs<V>::N; ++i) a.v[i] = fma2(a.v[i], b.v[i], c.v[i]);
+  return a;
+}
+template <int ACT, int V>
+SPLAT_DEV Pairs<V> activate(Pairs<V> x) {
+#pragma unroll
+  for (int i = 0; i < Pairs<V>::N; ++i) {
+    float a, b;
+    unpack2(x.v[i], a, b);
+    if constexpr (V == 1) a = activate<ACT>(a);
+    else activate2<ACT>(a, b);
+    x.v[i] = pack2(a, b);
+  }
+  return x;
+}
+template <int ACT, int V>
+SPLAT_DEV Pairs<V> slope(Pairs<V> x) {
+#pragma unroll
+  for (int i = 0; i < Pairs<V>::N; ++i) {
+    float a, b;
+    unpack2(x.v[i], a, b);
+    if constexpr (V == 1) a = slope<ACT>(a);
+    else slope2<ACT>(a, b);
+    x.v[i] = pack2(a, b);
+  }
+  return x;
 }
 
 template <class T, int V>
-SPLAT_DEV void store_values(T* base, long long at, long long span, const float (&v)[V]) {
-  if (at + V <= span) {
-    Vec<T, V> r;
-#pragma unroll
-    for (int j = 0; j < V; ++j) r.v[j] = from_float<T>(v[j]);
-    *reinterpret_cast<Vec<T, V>*>(base + at) = r;
+SPLAT_DEV Pairs<V> widen_pairs(const Vec<T, V>& r) {
+  float f[V];
+  widen<T, V>(r, f);
+  Pairs<V> p;
+  p.set(f);
+  return p;
+}
+// Values read for the last time, and results, which need not stay in the L2.
+template <class V>
+SPLAT_DEV V load_last(const V* p) {
+  if constexpr (sizeof(V) == 16) {
+    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
+    return reinterpret_cast<const V&>(u);
   } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (at + j < span) base[at + j] = from_float<T>(v[j]);
+    return *p;
   }
 }
+template <class V>
+SPLAT_DEV void store_streaming(V* p, const V& v) {
+  if constexpr (sizeof(V) == 16)
+    __stcs(reinterpret_cast<uint4*>(p), reinterpret_cast<const uint4&>(v));
+  else
+    *p = v;
+}
+template <class T, int V>
+SPLAT_DEV Vec<T, V> round_pairs(const Pairs<V>& p) {
+  float f[V];
+  p.get(f);
+  return round_values<T, V>(f);
+}
+// The vector that a lone sample may end inside: its `left` values.
+template <class T, int V>
+SPLAT_DEV Vec<T, V> load_part(const T* p, int left) {
+  Vec<T, V> r;
+#pragma unroll
+  for (int j = 0; j < V; ++j) r.v[j] = j < left ? p[j] : from_float<T>(0.0f);
+  return r;
+}
+template <class T, int V>
+SPLAT_DEV void store_part(T* p, const Vec<T, V>& r, int left) {
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    if (j < left) p[j] = r.v[j];
+}
 
-// What a thread of any of the passes works on.
+// What a thread of any of the passes works on: `count` whole vectors, the
+// first at `first` (values from the sample's start) and `stride` values apart,
+// and the part of a last one (`left` values, usually none) behind them.
 struct Place {
   int sample, part, column;  // part: the block along the sample's rows
   int vector;                // of the period(s) at a step
-  bool active;
+  int count, left;
+  long long first, stride;
 };
 
+template <int V>
 SPLAT_DEV Place place(const Layout& l) {
   Place p;
-  long long b = blockIdx.x;
-  p.column = static_cast<int>(b % l.columns);
-  b /= l.columns;
-  p.part = static_cast<int>(b % l.blocks);
-  p.sample = static_cast<int>(b / l.blocks);
+  unsigned b = blockIdx.x;
+  p.column = 0;
+  if (l.columns > 1) {
+    p.column = b % l.columns;
+    b /= l.columns;
+  }
+  p.sample = b / l.blocks;
+  p.part = b - p.sample * l.blocks;
   p.vector = p.column * l.threads + threadIdx.x;
-  p.active = p.vector < l.step;
+  const int begin = p.part * l.per_block, end = min(begin + l.per_block, l.steps);
+  p.first = (static_cast<long long>(begin) * l.step + p.vector) * V;
+  p.stride = static_cast<long long>(l.step) * V;
+  p.count = p.left = 0;
+  if (p.vector < l.step) {
+    // every step but the sample's last is whole
+    p.count = end - begin;
+    if (end == l.steps) {
+      const long long o = p.first + (p.count - 1) * p.stride;
+      if (o + V > l.span) {
+        --p.count;
+        p.left = static_cast<int>(max(l.span - o, 0LL));
+      }
+    }
+  }
   return p;
 }
 
@@ -137,41 +241,53 @@ SPLAT_DEV void write_partial(const NormParams& p, const Place& at, const float (
 // Sums of x - pivot and its square per channel; the pivot is the sample's
 // first row, so that a large common offset does not cancel.
 template <class T, int V>
-__global__ void __launch_bounds__(kMaxThreads) norm_sums_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kMaxThreads, 4) norm_sums_kernel(const NormParams p) {
+  using Values = Vec<T, V>;
   const Layout& l = p.l;
-  const Place at = place(l);
+  const Place at = place<V>(l);
   const T* x = static_cast<const T*>(p.x) + at.sample * l.span;
-  float s1[V] = {}, s2[V] = {};
-  if (at.active) {
-    float pivot[V];
+  float zero[V] = {}, pivot[V];
+  Pairs<V> minus, s1, s2;
+  s1.set(zero);
+  s2.set(zero);
+  const bool active = at.count || at.left;
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      pivot[j] = to_float(x[(static_cast<long long>(at.vector) * V + j) % l.channels]);
-    const int begin = at.part * l.per_block, end = min(begin + l.per_block, l.steps);
-#pragma unroll 4
-    for (int i = begin; i < end; ++i) {
-      const long long o = (static_cast<long long>(i) * l.step + at.vector) * V;
-      if (o + V <= l.span) {
-        float v[V];
-        load_values<T, V>(x, o, l.span, v, 0.0f);
+  for (int j = 0; j < V; ++j)
+    pivot[j] =
+        active ? -to_float(x[(static_cast<long long>(at.vector) * V + j) % l.channels]) : 0.0f;
+  minus.set(pivot);
+  const T* from = x + at.first;
+  constexpr int U = 4;
+  int i = 0;
+  for (; i + U <= at.count; i += U) {
+    Values v[U];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float d = v[j] - pivot[j];
-          s1[j] += d;
-          s2[j] += d * d;
-        }
-      } else {
+    for (int u = 0; u < U; ++u)
+      v[u] = *reinterpret_cast<const Values*>(from + u * at.stride);
+    from += U * at.stride;
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (o + j < l.span) {
-            const float d = to_float(x[o + j]) - pivot[j];
-            s1[j] += d;
-            s2[j] += d * d;
-          }
-      }
+    for (int u = 0; u < U; ++u) {
+      const Pairs<V> d = widen_pairs<T, V>(v[u]) + minus;
+      s1 = s1 + d;
+      s2 = fma(d, d, s2);
     }
   }
-  write_partial<V>(p, at, s1, s2);
+  for (; i < at.count; ++i, from += at.stride) {
+    const Pairs<V> d = widen_pairs<T, V>(*reinterpret_cast<const Values*>(from)) + minus;
+    s1 = s1 + d;
+    s2 = fma(d, d, s2);
+  }
+  float a[V], b[V];
+  s1.get(a);
+  s2.get(b);
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    if (j < at.left) {
+      const float d = to_float(from[j]) + pivot[j];
+      a[j] += d;
+      b[j] += d * d;
+    }
+  write_partial<V>(p, at, a, b);
 }
 
 SPLAT_DEV double warp_sum(double v) {
@@ -180,58 +296,71 @@ SPLAT_DEV double warp_sum(double v) {
   return v;
 }
 
-// Joins the blocks' sums of one channel (a warp per call).
-SPLAT_DEV double2 channel_sums(const NormParams& p, int sample, int c) {
+// The blocks' sums of up to kJoinChannels channels from c0 on, joined in
+// shared memory: neighbouring threads read neighbouring channels of a block's
+// row, and the threads of a channel are added up in a fixed order.
+constexpr int kJoinThreads = 256, kJoinChannels = 32;
+
+SPLAT_DEV void channel_sums(const NormParams& p, int sample, int c0, int count,
+                            double2 (&joined)[kJoinChannels]) {
+  __shared__ double2 sums[kJoinThreads];
   const int parts = p.l.blocks * p.l.columns;
-  const float2* in = p.partial + static_cast<long long>(sample) * parts * p.l.channels + c;
+  const float2* in =
+      p.partial + static_cast<long long>(sample) * parts * p.l.channels + c0;
+  const int lanes = kJoinThreads / count, c = threadIdx.x % count, lane = threadIdx.x / count;
   double a = 0.0, b = 0.0;
-  for (int i = threadIdx.x & 31; i < parts; i += 32) {
-    const float2 v = in[static_cast<long long>(i) * p.l.channels];
-    a += v.x;
-    b += v.y;
+  if (lane < lanes) {
+#pragma unroll 8
+    for (int i = lane; i < parts; i += lanes) {
+      const float2 v = in[static_cast<long long>(i) * p.l.channels + c];
+      a += v.x;
+      b += v.y;
+    }
   }
-  return make_double2(warp_sum(a), warp_sum(b));
+  __syncthreads();
+  sums[threadIdx.x] = make_double2(a, b);
+  __syncthreads();
+  // a warp to a channel: its lanes' sums, then those of the warp
+  for (int k = threadIdx.x >> 5; k < count; k += kJoinThreads / 32) {
+    a = b = 0.0;
+    for (int i = threadIdx.x & 31; i < lanes; i += 32) {
+      a += sums[i * count + k].x;
+      b += sums[i * count + k].y;
+    }
+    a = warp_sum(a);
+    b = warp_sum(b);
+    if ((threadIdx.x & 31) == 0) joined[k] = make_double2(a, b);
+  }
+  __syncthreads();
 }
 
-constexpr int kJoinWarps = 8;
-
-// Mean and reciprocal deviation of one group: each channel's (count, mean,
-// sum of squared deviations) joined pairwise, in doubles:
+// Mean and reciprocal deviation of one group: the channels' (count, mean, sum
+// of squared deviations) joined one after another, in doubles:
 //   M = M_a + M_b + (mean_b - mean_a)^2 n_a n_b / (n_a + n_b).
 template <class T>
-__global__ void __launch_bounds__(kJoinWarps * 32) norm_join_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(const NormParams p) {
+  __shared__ double2 joined[kJoinChannels];
   const int sample = blockIdx.x / p.groups, g = blockIdx.x % p.groups;
-  const int warp = threadIdx.x >> 5;
   const double rows = static_cast<double>(p.l.span / p.l.channels);
   const T* x = static_cast<const T*>(p.x) + sample * p.l.span;
   double n = 0.0, mean = 0.0, m2 = 0.0;
-  for (int k = warp; k < p.group_channels; k += kJoinWarps) {
-    const int c = g * p.group_channels + k;
-    const double2 s = channel_sums(p, sample, c);
-    const double channel_mean = s.x / rows + static_cast<double>(to_float(x[c]));
-    const double channel_m2 = s.y - s.x * s.x / rows;
-    const double d = channel_mean - mean, total = n + rows;
-    m2 += channel_m2 + d * d * n * rows / total;
-    mean += d * rows / total;
-    n = total;
-  }
-  __shared__ double joined[kJoinWarps][3];
-  if ((threadIdx.x & 31) == 0) {
-    joined[warp][0] = n;
-    joined[warp][1] = mean;
-    joined[warp][2] = m2;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    n = joined[0][0], mean = joined[0][1], m2 = joined[0][2];
-    for (int w = 1; w < kJoinWarps; ++w) {
-      const double nb = joined[w][0];
-      if (nb == 0.0) continue;
-      const double d = joined[w][1] - mean, total = n + nb;
-      m2 += joined[w][2] + d * d * n * nb / total;
-      mean += d * nb / total;
-      n = total;
+  for (int k0 = 0; k0 < p.group_channels; k0 += kJoinChannels) {
+    const int c0 = g * p.group_channels + k0, count = min(kJoinChannels, p.group_channels - k0);
+    channel_sums(p, sample, c0, count, joined);
+    if (threadIdx.x == 0) {
+      for (int k = 0; k < count; ++k) {
+        const double2 s = joined[k];
+        const double channel_mean = s.x / rows + static_cast<double>(to_float(x[c0 + k]));
+        const double channel_m2 = s.y - s.x * s.x / rows;
+        const double d = channel_mean - mean, total = n + rows;
+        m2 += channel_m2 + d * d * n * rows / total;
+        mean += d * rows / total;
+        n = total;
+      }
     }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
     // rounding can leave a constant group a hair below zero; NaN stays
     const double var = m2 < 0.0 ? 0.0 : m2 / n;
     p.mean[blockIdx.x] = static_cast<float>(mean);
@@ -239,103 +368,145 @@ __global__ void __launch_bounds__(kJoinWarps * 32) norm_join_kernel(const NormPa
   }
 }
 
-// The parameters of a thread's V channels.
-template <class T, int V>
+// The parameters of a thread's V channels: -mean, rstd w, b, and for the
+// backward -rstd m1 and -rstd^2 m2, so that with d = x - mean
+//   u = d (rstd w) + b,  dx = du (rstd w) - d rstd^2 m2 - rstd m1.
+template <class T, int V, bool BACKWARD>
 struct Channels {
-  float mean[V], rstd[V], weight[V], bias[V];
+  Pairs<V> minus, scale, bias, k1, k2;
   SPLAT_DEV void load(const NormParams& p, const Place& at) {
+    float m[V], s[V], b[V], x1[V], x2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int c = static_cast<int>((static_cast<long long>(at.vector) * V + j) % p.l.channels);
       const int g = at.sample * p.groups + c / p.group_channels;
-      mean[j] = p.mean[g];
-      rstd[j] = p.rstd[g];
-      weight[j] = p.weight ? to_float(static_cast<const T*>(p.weight)[c]) : 1.0f;
-      bias[j] = p.bias ? to_float(static_cast<const T*>(p.bias)[c]) : 0.0f;
+      const float rstd = p.rstd[g];
+      m[j] = -p.mean[g];
+      s[j] = rstd * (p.weight ? to_float(static_cast<const T*>(p.weight)[c]) : 1.0f);
+      b[j] = p.bias ? to_float(static_cast<const T*>(p.bias)[c]) : 0.0f;
+      if constexpr (BACKWARD) {
+        const float2 sums = p.moments[g];
+        x1[j] = -rstd * sums.x;
+        x2[j] = -rstd * rstd * sums.y;
+      }
+    }
+    minus.set(m);
+    scale.set(s);
+    bias.set(b);
+    if constexpr (BACKWARD) {
+      k1.set(x1);
+      k2.set(x2);
     }
   }
 };
 
+// The passes that write go through a block's steps backwards: what the pass
+// before read last is still in the L2.
 template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kMaxThreads) norm_apply_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kMaxThreads, 4) norm_apply_kernel(const NormParams p) {
+  using Values = Vec<T, V>;
   const Layout& l = p.l;
-  const Place at = place(l);
-  if (!at.active) return;
-  const T* x = static_cast<const T*>(p.x) + at.sample * l.span;
-  T* y = static_cast<T*>(p.out) + at.sample * l.span;
-  Channels<T, V> ch;
+  const Place at = place<V>(l);
+  if (!at.count && !at.left) return;
+  const long long end = at.sample * l.span + at.first + at.count * at.stride;
+  const T* from = static_cast<const T*>(p.x) + end;
+  T* to = static_cast<T*>(p.out) + end;
+  Channels<T, V, false> ch;
   ch.load(p, at);
-  const int begin = at.part * l.per_block, end = min(begin + l.per_block, l.steps);
-#pragma unroll 4
-  for (int i = begin; i < end; ++i) {
-    const long long o = (static_cast<long long>(i) * l.step + at.vector) * V;
-    if (o >= l.span) break;
-    float v[V];
-    load_values<T, V>(x, o, l.span, v, 0.0f);
+  const auto result = [&](const Values& v) {
+    return round_pairs<T, V>(
+        activate<ACT, V>(fma(widen_pairs<T, V>(v) + ch.minus, ch.scale, ch.bias)));
+  };
+  if (at.left) store_part<T, V>(to, result(load_part<T, V>(from, at.left)), at.left);
+  constexpr int U = 4;
+  int i = at.count;
+  for (; i >= U; i -= U) {
+    Values v[U];
+    from -= U * at.stride;
+    to -= U * at.stride;
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      v[j] = activate<ACT>((v[j] - ch.mean[j]) * ch.rstd[j] * ch.weight[j] + ch.bias[j]);
-    store_values<T, V>(y, o, l.span, v);
+    for (int u = 0; u < U; ++u)
+      v[u] = load_last(reinterpret_cast<const Values*>(from + u * at.stride));
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      store_streaming(reinterpret_cast<Values*>(to + u * at.stride), result(v[u]));
+  }
+  for (; i > 0; --i) {
+    from -= at.stride;
+    to -= at.stride;
+    store_streaming(reinterpret_cast<Values*>(to),
+                    result(load_last(reinterpret_cast<const Values*>(from))));
   }
 }
 
-// Sums of du and du xhat per channel.
+// Sums of du and du (x - mean) per channel.
 template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kMaxThreads) norm_backward_sums_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kMaxThreads, 3) norm_backward_sums_kernel(const NormParams p) {
+  using Values = Vec<T, V>;
   const Layout& l = p.l;
-  const Place at = place(l);
-  float s1[V] = {}, s2[V] = {};
-  if (at.active) {
-    const T* x = static_cast<const T*>(p.x) + at.sample * l.span;
-    const T* dy = static_cast<const T*>(p.dy) + at.sample * l.span;
-    Channels<T, V> ch;
+  const Place at = place<V>(l);
+  float a[V] = {}, b[V] = {};
+  Pairs<V> s1, s2;
+  s1.set(a);
+  s2.set(a);
+  if (at.count || at.left) {
+    const T* from = static_cast<const T*>(p.x) + at.sample * l.span + at.first;
+    const T* grad = static_cast<const T*>(p.dy) + at.sample * l.span + at.first;
+    Channels<T, V, false> ch;
     ch.load(p, at);
-    const int begin = at.part * l.per_block, end = min(begin + l.per_block, l.steps);
-#pragma unroll 2
-    for (int i = begin; i < end; ++i) {
-      const long long o = (static_cast<long long>(i) * l.step + at.vector) * V;
-      if (o >= l.span) break;
-      float v[V], d[V];
-      load_values<T, V>(x, o, l.span, v, 0.0f);
-      load_values<T, V>(dy, o, l.span, d, 0.0f);  // 0 past the end: adds nothing
+    const auto add = [&](const Values& v, const Values& g) {
+      const Pairs<V> d = widen_pairs<T, V>(v) + ch.minus;
+      const Pairs<V> du = slope<ACT, V>(fma(d, ch.scale, ch.bias)) * widen_pairs<T, V>(g);
+      s1 = s1 + du;
+      s2 = fma(du, d, s2);
+    };
+    constexpr int U = 2;
+    int i = 0;
+    for (; i + U <= at.count; i += U, from += U * at.stride, grad += U * at.stride) {
+      Values v[U], g[U];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float hat = (v[j] - ch.mean[j]) * ch.rstd[j];
-        const float du = d[j] * slope<ACT>(hat * ch.weight[j] + ch.bias[j]);
-        s1[j] += o + j < l.span ? du : 0.0f;
-        s2[j] += o + j < l.span ? du * hat : 0.0f;
+      for (int u = 0; u < U; ++u) {
+        v[u] = *reinterpret_cast<const Values*>(from + u * at.stride);
+        g[u] = *reinterpret_cast<const Values*>(grad + u * at.stride);
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u) add(v[u], g[u]);
     }
+    for (; i < at.count; ++i, from += at.stride, grad += at.stride)
+      add(*reinterpret_cast<const Values*>(from), *reinterpret_cast<const Values*>(grad));
+    // an upstream of 0 behind the end adds nothing unless x - mean is not
+    // finite, which the sums of the values before it are not then either
+    if (at.left) add(load_part<T, V>(from, at.left), load_part<T, V>(grad, at.left));
   }
-  write_partial<V>(p, at, s1, s2);
+  s1.get(a);
+  s2.get(b);
+  write_partial<V>(p, at, a, b);
 }
 
 template <class T>
-__global__ void __launch_bounds__(kJoinWarps * 32) norm_backward_join_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kJoinThreads) norm_backward_join_kernel(const NormParams p) {
+  __shared__ double2 joined[kJoinChannels];
   const int sample = blockIdx.x / p.groups, g = blockIdx.x % p.groups;
-  const int warp = threadIdx.x >> 5;
+  const double rstd = p.rstd[blockIdx.x];
   double m1 = 0.0, m2 = 0.0;
-  for (int k = warp; k < p.group_channels; k += kJoinWarps) {
-    const int c = g * p.group_channels + k;
-    const double2 s = channel_sums(p, sample, c);
-    const double w = p.weight ? to_float(static_cast<const T*>(p.weight)[c]) : 1.0;
-    m1 += w * s.x;
-    m2 += w * s.y;
-    if ((threadIdx.x & 31) == 0)
-      p.channel[static_cast<long long>(sample) * p.l.channels + c] = s;
-  }
-  __shared__ double joined[kJoinWarps][2];
-  if ((threadIdx.x & 31) == 0) {
-    joined[warp][0] = m1;
-    joined[warp][1] = m2;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    m1 = m2 = 0.0;
-    for (int w = 0; w < kJoinWarps; ++w) {
-      m1 += joined[w][0];
-      m2 += joined[w][1];
+  for (int k0 = 0; k0 < p.group_channels; k0 += kJoinChannels) {
+    const int c0 = g * p.group_channels + k0, count = min(kJoinChannels, p.group_channels - k0);
+    channel_sums(p, sample, c0, count, joined);
+    if (threadIdx.x < count) {
+      joined[threadIdx.x].y *= rstd;  // of du (x - mean) to du xhat
+      p.channel[static_cast<long long>(sample) * p.l.channels + c0 + threadIdx.x] =
+          joined[threadIdx.x];
     }
+    __syncthreads();
+    if (threadIdx.x == 0)
+      for (int k = 0; k < count; ++k) {
+        const double w = p.weight ? to_float(static_cast<const T*>(p.weight)[c0 + k]) : 1.0;
+        m1 += w * joined[k].x;
+        m2 += w * joined[k].y;
+      }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
     const double n = static_cast<double>(p.l.span / p.l.channels) * p.group_channels;
     p.moments[blockIdx.x] = make_float2(static_cast<float>(m1 / n), static_cast<float>(m2 / n));
   }
@@ -357,38 +528,48 @@ __global__ void norm_parameters_kernel(const NormParams p, T* dweight, T* dbias)
 }
 
 template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kMaxThreads) norm_backward_apply_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kMaxThreads, 3) norm_backward_apply_kernel(const NormParams p) {
+  using Values = Vec<T, V>;
   const Layout& l = p.l;
-  const Place at = place(l);
-  if (!at.active) return;
-  const T* x = static_cast<const T*>(p.x) + at.sample * l.span;
-  const T* dy = static_cast<const T*>(p.dy) + at.sample * l.span;
-  T* dx = static_cast<T*>(p.out) + at.sample * l.span;
-  Channels<T, V> ch;
+  const Place at = place<V>(l);
+  if (!at.count && !at.left) return;
+  const long long end = at.sample * l.span + at.first + at.count * at.stride;
+  const T* from = static_cast<const T*>(p.x) + end;
+  const T* grad = static_cast<const T*>(p.dy) + end;
+  T* to = static_cast<T*>(p.out) + end;
+  Channels<T, V, true> ch;
   ch.load(p, at);
-  float m1[V], m2[V];
+  const auto result = [&](const Values& v, const Values& g) {
+    const Pairs<V> d = widen_pairs<T, V>(v) + ch.minus;
+    const Pairs<V> du = slope<ACT, V>(fma(d, ch.scale, ch.bias)) * widen_pairs<T, V>(g);
+    return round_pairs<T, V>(fma(du, ch.scale, fma(d, ch.k2, ch.k1)));
+  };
+  if (at.left)
+    store_part<T, V>(to, result(load_part<T, V>(from, at.left), load_part<T, V>(grad, at.left)),
+                     at.left);
+  constexpr int U = 2;
+  int i = at.count;
+  for (; i >= U; i -= U) {
+    Values v[U], g[U];
+    from -= U * at.stride;
+    grad -= U * at.stride;
+    to -= U * at.stride;
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int c = static_cast<int>((static_cast<long long>(at.vector) * V + j) % l.channels);
-    const float2 m = p.moments[at.sample * p.groups + c / p.group_channels];
-    m1[j] = m.x;
-    m2[j] = m.y;
-  }
-  const int begin = at.part * l.per_block, end = min(begin + l.per_block, l.steps);
-#pragma unroll 2
-  for (int i = begin; i < end; ++i) {
-    const long long o = (static_cast<long long>(i) * l.step + at.vector) * V;
-    if (o >= l.span) break;
-    float v[V], d[V];
-    load_values<T, V>(x, o, l.span, v, 0.0f);
-    load_values<T, V>(dy, o, l.span, d, 0.0f);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float hat = (v[j] - ch.mean[j]) * ch.rstd[j];
-      const float du = d[j] * slope<ACT>(hat * ch.weight[j] + ch.bias[j]);
-      v[j] = ch.rstd[j] * (ch.weight[j] * du - m1[j] - hat * m2[j]);
+    for (int u = 0; u < U; ++u) {
+      v[u] = load_last(reinterpret_cast<const Values*>(from + u * at.stride));
+      g[u] = load_last(reinterpret_cast<const Values*>(grad + u * at.stride));
     }
-    store_values<T, V>(dx, o, l.span, v);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      store_streaming(reinterpret_cast<Values*>(to + u * at.stride), result(v[u], g[u]));
+  }
+  for (; i > 0; --i) {
+    from -= at.stride;
+    grad -= at.stride;
+    to -= at.stride;
+    store_streaming(reinterpret_cast<Values*>(to),
+                    result(load_last(reinterpret_cast<const Values*>(from)),
+                           load_last(reinterpret_cast<const Values*>(grad))));
   }
 }
 
@@ -429,7 +610,8 @@ Layout make_layout(int samples, long long positions, int channels, int v, int pe
   return l;
 }
 
-constexpr int kBlocksPerSm = 6;
+// As many as the kernels' registers let share an SM.
+constexpr int kForwardBlocksPerSm = 4, kBackwardBlocksPerSm = 3;
 
 template <int V, class F>
 int with_width(int v, F f) {
@@ -476,7 +658,7 @@ size_t splat_feature_norm_workspace_bytes(int dtype, int samples, long long posi
                                           int channels, int groups, int backward) {
   if (check_norm(dtype, samples, positions, channels, groups, 0) != kOk) return 0;
   const int v = vector_width(bytes_of(dtype), samples, positions * channels);
-  const Layout l = make_layout(samples, positions, channels, v, kBlocksPerSm);
+  const Layout l = make_layout(samples, positions, channels, v, backward ? kBackwardBlocksPerSm : kForwardBlocksPerSm);
   size_t bytes = partial_bytes(samples, l);
   if (backward)
     bytes += round_up(static_cast<size_t>(samples) * groups * sizeof(float2)) +
@@ -499,7 +681,7 @@ int splat_feature_norm(int dtype, int samples, long long positions, int channels
     return host::fail(kWorkspaceTooSmall, "feature_norm: workspace");
   const int v = vector_width(bytes_of(dtype), samples, positions * channels);
   NormParams p{};
-  p.l = make_layout(samples, positions, channels, v, kBlocksPerSm);
+  p.l = make_layout(samples, positions, channels, v, kForwardBlocksPerSm);
   p.samples = samples;
   p.groups = groups;
   p.group_channels = channels / groups;
@@ -517,7 +699,7 @@ int splat_feature_norm(int dtype, int samples, long long positions, int channels
     return with_width<16 / sizeof(T)>(v, [&](auto width) {
       constexpr int V = decltype(width)::value;
       norm_sums_kernel<T, V><<<grid, p.l.threads, 0, host::counted(s)>>>(p);
-      norm_join_kernel<T><<<samples * groups, kJoinWarps * 32, 0, host::counted(s)>>>(p);
+      norm_join_kernel<T><<<samples * groups, kJoinThreads, 0, host::counted(s)>>>(p);
       return SPLAT_FEATURE_ACT(activation, [&] {
         norm_apply_kernel<T, V, ACT><<<grid, p.l.threads, 0, host::counted(s)>>>(p);
         return host::check_launch("feature_norm");
@@ -544,7 +726,7 @@ int splat_feature_norm_backward(int dtype, int samples, long long positions, int
     return host::fail(kWorkspaceTooSmall, "feature_norm_backward: workspace");
   const int v = vector_width(bytes_of(dtype), samples, positions * channels);
   NormParams p{};
-  p.l = make_layout(samples, positions, channels, v, kBlocksPerSm);
+  p.l = make_layout(samples, positions, channels, v, kBackwardBlocksPerSm);
   p.samples = samples;
   p.groups = groups;
   p.group_channels = channels / groups;
@@ -569,7 +751,7 @@ int splat_feature_norm_backward(int dtype, int samples, long long positions, int
       return SPLAT_FEATURE_ACT(activation, [&] {
         norm_backward_sums_kernel<T, V, ACT><<<grid, p.l.threads, 0, host::counted(s)>>>(p);
         norm_backward_join_kernel<T>
-            <<<samples * groups, kJoinWarps * 32, 0, host::counted(s)>>>(p);
+            <<<samples * groups, kJoinThreads, 0, host::counted(s)>>>(p);
         if (dweight || dbias)
           norm_parameters_kernel<T>
               <<<host::blocks_for(channels, 128), 128, 0, host::counted(s)>>>(
