@@ -13,7 +13,7 @@
 //
 // Both directions are a reduction of two sums per channel over the rows of a
 // sample, a small kernel that joins the blocks' sums, and a pass that writes
-// the result.  Sums over channels of a group are taken after the sums over
+// the result; small samples take one launch for all of it.  Sums over channels of a group are taken after the sums over
 // rows, so one layout serves any C and G: see Layout.
 #include <algorithm>
 #include <numeric>
@@ -193,11 +193,13 @@ SPLAT_DEV Place place(const Layout& l) {
   p.sample = b / l.blocks;
   p.part = b - p.sample * l.blocks;
   p.vector = p.column * l.threads + threadIdx.x;
-  const int begin = p.part * l.per_block, end = min(begin + l.per_block, l.steps);
+  // a cluster's last blocks may have no steps
+  const int begin = min(p.part * l.per_block, l.steps);
+  const int end = min(begin + l.per_block, l.steps);
   p.first = (static_cast<long long>(begin) * l.step + p.vector) * V;
   p.stride = static_cast<long long>(l.step) * V;
   p.count = p.left = 0;
-  if (p.vector < l.step) {
+  if (p.vector < l.step && begin < end) {
     // every step but the sample's last is whole
     p.count = end - begin;
     if (end == l.steps) {
@@ -334,38 +336,50 @@ SPLAT_DEV void channel_sums(const NormParams& p, int sample, int c0, int count,
   __syncthreads();
 }
 
-// Mean and reciprocal deviation of one group: the channels' (count, mean, sum
-// of squared deviations) joined one after another, in doubles:
+// A group's moments from its channels' sums of x - pivot: (count, mean, sum of
+// squared deviations) of up to 32 channels at a time, a lane to a channel, and
+// such blocks joined by
 //   M = M_a + M_b + (mean_b - mean_a)^2 n_a n_b / (n_a + n_b).
+struct Moments {
+  double n, mean, m2;
+  // Called by a whole warp; pivot and sums of lanes from `count` on are ignored.
+  SPLAT_DEV void join(double rows, int count, double2 sums, double pivot) {
+    const bool in = (threadIdx.x & 31) < count;
+    const double inverse = 1.0 / rows;
+    const double channel_mean = in ? sums.x * inverse + pivot : 0.0;
+    const double block_mean = warp_sum(channel_mean) / count, d = channel_mean - block_mean;
+    const double block_m2 =
+        warp_sum(in ? sums.y - sums.x * sums.x * inverse + rows * d * d : 0.0);
+    const double nb = rows * count, total = n + nb, apart = block_mean - mean;
+    m2 += block_m2 + apart * apart * (n * nb / total);
+    mean += apart * (nb / total);
+    n = total;
+  }
+  SPLAT_DEV void finish(float eps, float* mean_to, float* rstd_to) const {
+    // rounding can leave a constant group a hair below zero; NaN stays
+    const double var = m2 < 0.0 ? 0.0 : m2 / n;
+    *mean_to = static_cast<float>(mean);
+    *rstd_to = static_cast<float>(1.0 / sqrt(var + static_cast<double>(eps)));
+  }
+};
+
 template <class T>
 __global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(const NormParams p) {
   __shared__ double2 joined[kJoinChannels];
   const int sample = blockIdx.x / p.groups, g = blockIdx.x % p.groups;
   const double rows = static_cast<double>(p.l.span / p.l.channels);
   const T* x = static_cast<const T*>(p.x) + sample * p.l.span;
-  double n = 0.0, mean = 0.0, m2 = 0.0;
+  Moments m{};
   for (int k0 = 0; k0 < p.group_channels; k0 += kJoinChannels) {
     const int c0 = g * p.group_channels + k0, count = min(kJoinChannels, p.group_channels - k0);
     channel_sums(p, sample, c0, count, joined);
-    if (threadIdx.x == 0) {
-      for (int k = 0; k < count; ++k) {
-        const double2 s = joined[k];
-        const double channel_mean = s.x / rows + static_cast<double>(to_float(x[c0 + k]));
-        const double channel_m2 = s.y - s.x * s.x / rows;
-        const double d = channel_mean - mean, total = n + rows;
-        m2 += channel_m2 + d * d * n * rows / total;
-        mean += d * rows / total;
-        n = total;
-      }
+    if (threadIdx.x < 32) {
+      const int k = min(static_cast<int>(threadIdx.x), count - 1);
+      m.join(rows, count, joined[k], to_float(x[c0 + k]));
     }
     __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    // rounding can leave a constant group a hair below zero; NaN stays
-    const double var = m2 < 0.0 ? 0.0 : m2 / n;
-    p.mean[blockIdx.x] = static_cast<float>(mean);
-    p.rstd[blockIdx.x] = static_cast<float>(1.0 / sqrt(var + static_cast<double>(p.eps)));
-  }
+  if (threadIdx.x == 0) m.finish(p.eps, p.mean + blockIdx.x, p.rstd + blockIdx.x);
 }
 
 // The parameters of a thread's V channels: -mean, rstd w, b, and for the
@@ -374,20 +388,23 @@ __global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(const NormParam
 template <class T, int V, bool BACKWARD>
 struct Channels {
   Pairs<V> minus, scale, bias, k1, k2;
-  SPLAT_DEV void load(const NormParams& p, const Place& at) {
+  // moments: the sample's (mean, rstd) per group where they are not in p's
+  // arrays yet; sums: its (m1, m2) likewise
+  SPLAT_DEV void load(const NormParams& p, const Place& at, const float2* moments = nullptr,
+                      const float2* sums = nullptr) {
     float m[V], s[V], b[V], x1[V], x2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int c = static_cast<int>((static_cast<long long>(at.vector) * V + j) % p.l.channels);
-      const int g = at.sample * p.groups + c / p.group_channels;
-      const float rstd = p.rstd[g];
-      m[j] = -p.mean[g];
+      const int own = c / p.group_channels, g = at.sample * p.groups + own;
+      const float rstd = moments ? moments[own].y : p.rstd[g];
+      m[j] = -(moments ? moments[own].x : p.mean[g]);
       s[j] = rstd * (p.weight ? to_float(static_cast<const T*>(p.weight)[c]) : 1.0f);
       b[j] = p.bias ? to_float(static_cast<const T*>(p.bias)[c]) : 0.0f;
       if constexpr (BACKWARD) {
-        const float2 sums = p.moments[g];
-        x1[j] = -rstd * sums.x;
-        x2[j] = -rstd * rstd * sums.y;
+        const float2 s12 = sums ? sums[own] : p.moments[g];
+        x1[j] = -rstd * s12.x;
+        x2[j] = -rstd * rstd * s12.y;
       }
     }
     minus.set(m);
@@ -498,12 +515,14 @@ __global__ void __launch_bounds__(kJoinThreads) norm_backward_join_kernel(const 
           joined[threadIdx.x];
     }
     __syncthreads();
-    if (threadIdx.x == 0)
-      for (int k = 0; k < count; ++k) {
-        const double w = p.weight ? to_float(static_cast<const T*>(p.weight)[c0 + k]) : 1.0;
-        m1 += w * joined[k].x;
-        m2 += w * joined[k].y;
-      }
+    if (threadIdx.x < 32) {
+      const int k = threadIdx.x;
+      const double w =
+          k >= count ? 0.0
+                     : p.weight ? to_float(static_cast<const T*>(p.weight)[c0 + k]) : 1.0;
+      m1 += warp_sum(k < count ? w * joined[k].x : 0.0);
+      m2 += warp_sum(k < count ? w * joined[k].y : 0.0);
+    }
     __syncthreads();
   }
   if (threadIdx.x == 0) {
@@ -573,6 +592,264 @@ __global__ void __launch_bounds__(kMaxThreads, 3) norm_backward_apply_kernel(con
   }
 }
 
+// ---- small samples: one launch ---------------------------------------------------
+//
+// A sample that fits in the shared memory of a cluster of up to 8 blocks is
+// read once: every thread keeps its own values there, the blocks exchange
+// their channel sums through distributed shared memory, and each forms the
+// group's moments for itself.  For 37x53x35 fp32 (274 KB) 3 launches and
+// 12 us of device time become one of 6 us.
+
+constexpr int kMaxCluster = 8;
+constexpr int kSmallBytes = 64 * 1024;   // of a block's values
+constexpr int kSmallChannels = 1024;
+
+SPLAT_DEV uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+SPLAT_DEV void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// A pair in the shared memory of another block of the cluster, at the address
+// that it has in this one.
+SPLAT_DEV float2 load_cluster(const float2* own, uint32_t rank) {
+  const uint32_t here = static_cast<uint32_t>(__cvta_generic_to_shared(own));
+  uint32_t there;
+  float2 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(there)
+               : "memory");
+  return v;
+}
+
+// Sums the threads' sums over the block and then over the cluster; all blocks
+// end with the sample's sums per channel in `channel`.
+template <int V>
+SPLAT_DEV void cluster_sums(const Layout& l, const float (&s1)[V], const float (&s2)[V],
+                            float2* per_thread, float2* own, double2* channel) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) per_thread[threadIdx.x * V + j] = make_float2(s1[j], s2[j]);
+  __syncthreads();
+  const int count = l.threads * V;
+  for (int c = threadIdx.x; c < l.channels; c += l.threads) {
+    float a = 0.0f, b = 0.0f;
+    for (int i = c; i < count; i += l.channels) {
+      a += per_thread[i].x;
+      b += per_thread[i].y;
+    }
+    own[c] = make_float2(a, b);
+  }
+  cluster_sync();
+  for (int c = threadIdx.x; c < l.channels; c += l.threads) {
+    double a = 0.0, b = 0.0;
+    for (int r = 0; r < l.blocks; ++r) {
+      const float2 v = load_cluster(own + c, r);
+      a += v.x;
+      b += v.y;
+    }
+    channel[c] = make_double2(a, b);
+  }
+  cluster_sync();  // no block leaves while its sums are read
+}
+
+// Shared memory of the small kernels: the values, then the sums.
+__host__ __device__ inline size_t kept_bytes(const Layout& l, int vector_bytes, int arrays) {
+  return (static_cast<size_t>(arrays) * l.per_block * l.threads * vector_bytes + 15) / 16 * 16;
+}
+template <class T, int V>
+struct SmallShared {
+  float2* per_thread;
+  float2* own;
+  double2* channel;
+  float2* group;  // per group: mean and rstd, or m1 and m2
+  SPLAT_DEV SmallShared(unsigned char* base, const Layout& l, int arrays) {
+    base += kept_bytes(l, sizeof(Vec<T, V>), arrays);
+    channel = reinterpret_cast<double2*>(base);
+    per_thread = reinterpret_cast<float2*>(channel + l.channels);
+    own = per_thread + l.threads * V;
+    group = own + l.channels;
+  }
+};
+size_t small_bytes(const Layout& l, int v, int value_bytes, int groups, int arrays) {
+  return kept_bytes(l, v * value_bytes, arrays) +
+         static_cast<size_t>(l.channels) * (sizeof(double2) + sizeof(float2)) +
+         static_cast<size_t>(l.threads) * v * sizeof(float2) +
+         static_cast<size_t>(groups) * sizeof(float2);
+}
+
+template <class T, int V, int ACT>
+__global__ void __launch_bounds__(kMaxThreads) norm_small_kernel(const NormParams p) {
+  using Values = Vec<T, V>;
+  extern __shared__ __align__(16) unsigned char shared[];
+  const Layout& l = p.l;
+  const Place at = place<V>(l);
+  const SmallShared<T, V> mem(shared, l, 1);
+  Values* kept = reinterpret_cast<Values*>(shared) + threadIdx.x;
+  const T* x = static_cast<const T*>(p.x) + at.sample * l.span;
+  const T* from = x + at.first;
+  float a[V] = {}, b[V] = {}, pivot[V];
+  const bool active = at.count || at.left;
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    pivot[j] = active ? to_float(x[(at.vector * V + j) % l.channels]) : 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < at.count; ++i) {
+    const Values v = *reinterpret_cast<const Values*>(from + i * at.stride);
+    kept[i * l.threads] = v;
+    float f[V];
+    widen<T, V>(v, f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float d = f[j] - pivot[j];
+      a[j] += d;
+      b[j] += d * d;
+    }
+  }
+  if (at.left) {
+    const Values v = load_part<T, V>(from + at.count * at.stride, at.left);
+    kept[at.count * l.threads] = v;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j < at.left) {
+        const float d = to_float(v.v[j]) - pivot[j];
+        a[j] += d;
+        b[j] += d * d;
+      }
+  }
+  cluster_sums<V>(l, a, b, mem.per_thread, mem.own, mem.channel);
+  __syncthreads();
+  const double rows = static_cast<double>(l.span / l.channels);
+  // whole warps only (there is one: a block has more than 128 threads)
+  const int whole = l.threads / 32, lane = threadIdx.x & 31;
+  if (static_cast<int>(threadIdx.x >> 5) < whole) {
+    for (int g = threadIdx.x >> 5; g < p.groups; g += whole) {
+      Moments m{};
+      for (int k0 = 0; k0 < p.group_channels; k0 += 32) {
+        const int count = min(32, p.group_channels - k0);
+        const int c = g * p.group_channels + k0 + min(lane, count - 1);
+        m.join(rows, count, mem.channel[c], to_float(x[c]));
+      }
+      if (lane == 0) {
+        float2 r;
+        m.finish(p.eps, &r.x, &r.y);
+        mem.group[g] = r;
+        if (cluster_rank() == 0) {
+          p.mean[at.sample * p.groups + g] = r.x;
+          p.rstd[at.sample * p.groups + g] = r.y;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (!active) return;
+  Channels<T, V, false> ch;
+  ch.load(p, at, mem.group, nullptr);
+  T* to = static_cast<T*>(p.out) + at.sample * l.span + at.first;
+  const auto result = [&](const Values& v) {
+    return round_pairs<T, V>(
+        activate<ACT, V>(fma(widen_pairs<T, V>(v) + ch.minus, ch.scale, ch.bias)));
+  };
+#pragma unroll 2
+  for (int i = 0; i < at.count; ++i)
+    *reinterpret_cast<Values*>(to + i * at.stride) = result(kept[i * l.threads]);
+  if (at.left)
+    store_part<T, V>(to + at.count * at.stride, result(kept[at.count * l.threads]), at.left);
+}
+
+template <class T, int V, int ACT>
+__global__ void __launch_bounds__(kMaxThreads)
+    norm_backward_small_kernel(const NormParams p, T* dweight, T* dbias) {
+  using Values = Vec<T, V>;
+  extern __shared__ __align__(16) unsigned char shared[];
+  const Layout& l = p.l;
+  const Place at = place<V>(l);
+  const SmallShared<T, V> mem(shared, l, 2);
+  Values* kept_x = reinterpret_cast<Values*>(shared) + threadIdx.x;
+  Values* kept_g = kept_x + l.per_block * l.threads;
+  const long long offset = at.sample * l.span + at.first;
+  const T* from = static_cast<const T*>(p.x) + offset;
+  const T* grad = static_cast<const T*>(p.dy) + offset;
+  float a[V] = {}, b[V] = {};
+  Pairs<V> s1, s2;
+  s1.set(a);
+  s2.set(a);
+  const bool active = at.count || at.left;
+  Channels<T, V, false> ch;
+  if (active) {
+    ch.load(p, at, nullptr, nullptr);
+    const auto add = [&](const Values& v, const Values& g) {
+      const Pairs<V> d = widen_pairs<T, V>(v) + ch.minus;
+      const Pairs<V> du = slope<ACT, V>(fma(d, ch.scale, ch.bias)) * widen_pairs<T, V>(g);
+      s1 = s1 + du;
+      s2 = fma(du, d, s2);
+    };
+#pragma unroll 2
+    for (int i = 0; i < at.count; ++i) {
+      const Values v = *reinterpret_cast<const Values*>(from + i * at.stride);
+      const Values g = *reinterpret_cast<const Values*>(grad + i * at.stride);
+      kept_x[i * l.threads] = v;
+      kept_g[i * l.threads] = g;
+      add(v, g);
+    }
+    if (at.left) {
+      const Values v = load_part<T, V>(from + at.count * at.stride, at.left);
+      const Values g = load_part<T, V>(grad + at.count * at.stride, at.left);
+      kept_x[at.count * l.threads] = v;
+      kept_g[at.count * l.threads] = g;
+      add(v, g);
+    }
+  }
+  s1.get(a);
+  s2.get(b);
+  cluster_sums<V>(l, a, b, mem.per_thread, mem.own, mem.channel);
+  __syncthreads();
+  const bool first = cluster_rank() == 0;
+  const double n = static_cast<double>(l.span / l.channels) * p.group_channels;
+  for (int c = threadIdx.x; c < l.channels; c += l.threads) {
+    double2 s = mem.channel[c];
+    s.y *= p.rstd[at.sample * p.groups + c / p.group_channels];
+    mem.channel[c] = s;
+    if (first) {
+      if (p.samples > 1) p.channel[static_cast<long long>(at.sample) * l.channels + c] = s;
+      if (dbias) dbias[c] = from_float<T>(static_cast<float>(s.x));
+      if (dweight) dweight[c] = from_float<T>(static_cast<float>(s.y));
+    }
+  }
+  if (!p.out) return;
+  __syncthreads();
+  for (int g = threadIdx.x; g < p.groups; g += l.threads) {
+    double m1 = 0.0, m2 = 0.0;
+    for (int k = 0; k < p.group_channels; ++k) {
+      const int c = g * p.group_channels + k;
+      const double w = p.weight ? to_float(static_cast<const T*>(p.weight)[c]) : 1.0;
+      m1 += w * mem.channel[c].x;
+      m2 += w * mem.channel[c].y;
+    }
+    mem.group[g] = make_float2(static_cast<float>(m1 / n), static_cast<float>(m2 / n));
+  }
+  __syncthreads();
+  if (!active) return;
+  Channels<T, V, true> k;
+  k.load(p, at, nullptr, mem.group);
+  T* to = static_cast<T*>(p.out) + offset;
+  const auto result = [&](const Values& v, const Values& g) {
+    const Pairs<V> d = widen_pairs<T, V>(v) + k.minus;
+    const Pairs<V> du = slope<ACT, V>(fma(d, k.scale, k.bias)) * widen_pairs<T, V>(g);
+    return round_pairs<T, V>(fma(du, k.scale, fma(d, k.k2, k.k1)));
+  };
+#pragma unroll 2
+  for (int i = 0; i < at.count; ++i)
+    *reinterpret_cast<Values*>(to + i * at.stride) =
+        result(kept_x[i * l.threads], kept_g[i * l.threads]);
+  if (at.left)
+    store_part<T, V>(to + at.count * at.stride,
+                     result(kept_x[at.count * l.threads], kept_g[at.count * l.threads]), at.left);
+}
+
 // ---- host ------------------------------------------------------------------
 
 // Values per vector: 16 bytes' worth, halved until every sample starts on a
@@ -612,6 +889,58 @@ Layout make_layout(int samples, long long positions, int channels, int v, int pe
 
 // As many as the kernels' registers let share an SM.
 constexpr int kForwardBlocksPerSm = 4, kBackwardBlocksPerSm = 3;
+
+// How a call is run: in clusters of l.blocks (small), or in passes.
+struct Plan {
+  Layout l;
+  int vector;
+  bool small;
+  size_t shared_bytes;
+};
+
+Plan make_plan(int value_bytes, int samples, long long positions, int channels, int groups,
+               bool backward) {
+  Plan plan;
+  plan.vector = vector_width(value_bytes, samples, positions * channels);
+  plan.l = make_layout(samples, positions, channels, plan.vector,
+                       backward ? kBackwardBlocksPerSm : kForwardBlocksPerSm);
+  const long long bytes = positions * channels * value_bytes * (backward ? 2 : 1);
+  plan.small = plan.l.columns == 1 && channels <= kSmallChannels &&
+               bytes <= static_cast<long long>(kMaxCluster) * kSmallBytes;
+  plan.shared_bytes = 0;
+  if (plan.small) {
+    // 8 KB to a block at least, where the sample has them
+    int blocks = 1;
+    while (blocks < kMaxCluster && blocks * 8192LL < bytes && blocks < plan.l.steps) blocks *= 2;
+    plan.l.blocks = blocks;
+    plan.l.per_block = (plan.l.steps + blocks - 1) / blocks;
+    plan.shared_bytes = small_bytes(plan.l, plan.vector, value_bytes, groups, backward ? 2 : 1);
+  }
+  return plan;
+}
+
+// Launches a small sample's kernel as clusters of `blocks`.
+template <class... A, class... B>
+int launch_cluster(void (*kernel)(A...), const Plan& plan, int samples, cudaStream_t s,
+                   B... args) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(plan.shared_bytes)) != cudaSuccess)
+    return host::check_launch("feature_norm: shared memory");
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = plan.l.blocks;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(samples) * plan.l.blocks);
+  config.blockDim = dim3(plan.l.threads);
+  config.dynamicSmemBytes = plan.shared_bytes;
+  config.stream = host::counted(s);
+  config.attrs = &cluster;
+  config.numAttrs = 1;
+  if (cudaLaunchKernelEx(&config, kernel, args...) != cudaSuccess)
+    return host::check_launch("feature_norm");
+  return kOk;
+}
 
 template <int V, class F>
 int with_width(int v, F f) {
@@ -657,9 +986,10 @@ extern "C" {
 size_t splat_feature_norm_workspace_bytes(int dtype, int samples, long long positions,
                                           int channels, int groups, int backward) {
   if (check_norm(dtype, samples, positions, channels, groups, 0) != kOk) return 0;
-  const int v = vector_width(bytes_of(dtype), samples, positions * channels);
-  const Layout l = make_layout(samples, positions, channels, v, backward ? kBackwardBlocksPerSm : kForwardBlocksPerSm);
-  size_t bytes = partial_bytes(samples, l);
+  const Plan plan =
+      make_plan(bytes_of(dtype), samples, positions, channels, groups, backward != 0);
+  // never 0, which means an error
+  size_t bytes = plan.small ? 16 : partial_bytes(samples, plan.l);
   if (backward)
     bytes += round_up(static_cast<size_t>(samples) * groups * sizeof(float2)) +
              static_cast<size_t>(samples) * channels * sizeof(double2);
@@ -679,9 +1009,9 @@ int splat_feature_norm(int dtype, int samples, long long positions, int channels
   if (workspace_bytes <
       splat_feature_norm_workspace_bytes(dtype, samples, positions, channels, groups, 0))
     return host::fail(kWorkspaceTooSmall, "feature_norm: workspace");
-  const int v = vector_width(bytes_of(dtype), samples, positions * channels);
+  const Plan plan = make_plan(bytes_of(dtype), samples, positions, channels, groups, false);
   NormParams p{};
-  p.l = make_layout(samples, positions, channels, v, kForwardBlocksPerSm);
+  p.l = plan.l;
   p.samples = samples;
   p.groups = groups;
   p.group_channels = channels / groups;
@@ -696,8 +1026,12 @@ int splat_feature_norm(int dtype, int samples, long long positions, int channels
   auto s = static_cast<cudaStream_t>(stream);
   const unsigned grid = static_cast<unsigned>(samples) * p.l.blocks * p.l.columns;
   return SPLAT_FEATURE_TYPE(dtype, [&] {
-    return with_width<16 / sizeof(T)>(v, [&](auto width) {
+    return with_width<16 / sizeof(T)>(plan.vector, [&](auto width) {
       constexpr int V = decltype(width)::value;
+      if (plan.small)
+        return SPLAT_FEATURE_ACT(activation, [&] {
+          return launch_cluster(norm_small_kernel<T, V, ACT>, plan, samples, s, p);
+        });
       norm_sums_kernel<T, V><<<grid, p.l.threads, 0, host::counted(s)>>>(p);
       norm_join_kernel<T><<<samples * groups, kJoinThreads, 0, host::counted(s)>>>(p);
       return SPLAT_FEATURE_ACT(activation, [&] {
@@ -724,9 +1058,9 @@ int splat_feature_norm_backward(int dtype, int samples, long long positions, int
   if (workspace_bytes <
       splat_feature_norm_workspace_bytes(dtype, samples, positions, channels, groups, 1))
     return host::fail(kWorkspaceTooSmall, "feature_norm_backward: workspace");
-  const int v = vector_width(bytes_of(dtype), samples, positions * channels);
+  const Plan plan = make_plan(bytes_of(dtype), samples, positions, channels, groups, true);
   NormParams p{};
-  p.l = make_layout(samples, positions, channels, v, kBackwardBlocksPerSm);
+  p.l = plan.l;
   p.samples = samples;
   p.groups = groups;
   p.group_channels = channels / groups;
@@ -739,23 +1073,34 @@ int splat_feature_norm_backward(int dtype, int samples, long long positions, int
   p.rstd = const_cast<float*>(rstd);
   char* at = static_cast<char*>(workspace);
   p.partial = reinterpret_cast<float2*>(at);
-  at += partial_bytes(samples, p.l);
+  at += plan.small ? 16 : partial_bytes(samples, p.l);
   p.moments = reinterpret_cast<float2*>(at);
   at += round_up(static_cast<size_t>(samples) * groups * sizeof(float2));
   p.channel = reinterpret_cast<double2*>(at);
   auto s = static_cast<cudaStream_t>(stream);
   const unsigned grid = static_cast<unsigned>(samples) * p.l.blocks * p.l.columns;
   return SPLAT_FEATURE_TYPE(dtype, [&] {
-    return with_width<16 / sizeof(T)>(v, [&](auto width) {
+    return with_width<16 / sizeof(T)>(plan.vector, [&](auto width) {
       constexpr int V = decltype(width)::value;
+      T *dw = static_cast<T*>(dweight), *db = static_cast<T*>(dbias);
       return SPLAT_FEATURE_ACT(activation, [&] {
+        if (plan.small) {
+          const bool one = samples == 1;
+          const int status =
+              launch_cluster(norm_backward_small_kernel<T, V, ACT>, plan, samples, s, p,
+                             one ? dw : nullptr, one ? db : nullptr);
+          if (status != kOk || one || !(dw || db)) return status;
+          norm_parameters_kernel<T>
+              <<<host::blocks_for(channels, 128), 128, 0, host::counted(s)>>>(p, dw, db);
+          return host::check_launch("feature_norm_backward");
+        }
         norm_backward_sums_kernel<T, V, ACT><<<grid, p.l.threads, 0, host::counted(s)>>>(p);
         norm_backward_join_kernel<T>
             <<<samples * groups, kJoinThreads, 0, host::counted(s)>>>(p);
         if (dweight || dbias)
           norm_parameters_kernel<T>
               <<<host::blocks_for(channels, 128), 128, 0, host::counted(s)>>>(
-                  p, static_cast<T*>(dweight), static_cast<T*>(dbias));
+                  p, dw, db);
         if (dx)
           norm_backward_apply_kernel<T, V, ACT><<<grid, p.l.threads, 0, host::counted(s)>>>(p);
         return host::check_launch("feature_norm_backward");
