@@ -312,11 +312,20 @@ SPLAT_DEV void channel_sums(const NormParams& p, int sample, int c0, int count,
   const int lanes = kJoinThreads / count, c = threadIdx.x % count, lane = threadIdx.x / count;
   double a = 0.0, b = 0.0;
   if (lane < lanes) {
-#pragma unroll 8
-    for (int i = lane; i < parts; i += lanes) {
-      const float2 v = in[static_cast<long long>(i) * p.l.channels + c];
-      a += v.x;
-      b += v.y;
+    constexpr int U = 8;  // reads in flight
+    for (int i0 = lane; i0 < parts; i0 += U * lanes) {
+      float2 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * lanes;
+        v[u] = i < parts ? in[static_cast<long long>(i) * p.l.channels + c]
+                         : make_float2(0.0f, 0.0f);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        a += v[u].x;
+        b += v[u].y;
+      }
     }
   }
   __syncthreads();
@@ -501,7 +510,8 @@ __global__ void __launch_bounds__(kMaxThreads, 3) norm_backward_sums_kernel(cons
 }
 
 template <class T>
-__global__ void __launch_bounds__(kJoinThreads) norm_backward_join_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kJoinThreads)
+    norm_backward_join_kernel(const NormParams p, T* dweight, T* dbias) {
   __shared__ double2 joined[kJoinChannels];
   const int sample = blockIdx.x / p.groups, g = blockIdx.x % p.groups;
   const double rstd = p.rstd[blockIdx.x];
@@ -511,8 +521,11 @@ __global__ void __launch_bounds__(kJoinThreads) norm_backward_join_kernel(const 
     channel_sums(p, sample, c0, count, joined);
     if (threadIdx.x < count) {
       joined[threadIdx.x].y *= rstd;  // of du (x - mean) to du xhat
-      p.channel[static_cast<long long>(sample) * p.l.channels + c0 + threadIdx.x] =
-          joined[threadIdx.x];
+      const double2 v = joined[threadIdx.x];
+      if (p.samples > 1)
+        p.channel[static_cast<long long>(sample) * p.l.channels + c0 + threadIdx.x] = v;
+      if (dbias) dbias[c0 + threadIdx.x] = from_float<T>(static_cast<float>(v.x));
+      if (dweight) dweight[c0 + threadIdx.x] = from_float<T>(static_cast<float>(v.y));
     }
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -696,18 +709,26 @@ __global__ void __launch_bounds__(kMaxThreads) norm_small_kernel(const NormParam
 #pragma unroll
   for (int j = 0; j < V; ++j)
     pivot[j] = active ? to_float(x[(at.vector * V + j) % l.channels]) : 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < at.count; ++i) {
-    const Values v = *reinterpret_cast<const Values*>(from + i * at.stride);
-    kept[i * l.threads] = v;
-    float f[V];
-    widen<T, V>(v, f);
+  constexpr int U = 8;  // reads in flight
+  for (int i0 = 0; i0 < at.count; i0 += U) {
+    Values v[U];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float d = f[j] - pivot[j];
-      a[j] += d;
-      b[j] += d * d;
-    }
+    for (int u = 0; u < U; ++u)
+      if (i0 + u < at.count)
+        v[u] = *reinterpret_cast<const Values*>(from + (i0 + u) * at.stride);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u < at.count) {
+        kept[(i0 + u) * l.threads] = v[u];
+        float f[V];
+        widen<T, V>(v[u], f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float d = f[j] - pivot[j];
+          a[j] += d;
+          b[j] += d * d;
+        }
+      }
   }
   if (at.left) {
     const Values v = load_part<T, V>(from + at.count * at.stride, at.left);
@@ -737,7 +758,7 @@ __global__ void __launch_bounds__(kMaxThreads) norm_small_kernel(const NormParam
         float2 r;
         m.finish(p.eps, &r.x, &r.y);
         mem.group[g] = r;
-        if (cluster_rank() == 0) {
+        if (p.mean && cluster_rank() == 0) {
           p.mean[at.sample * p.groups + g] = r.x;
           p.rstd[at.sample * p.groups + g] = r.y;
         }
@@ -787,13 +808,22 @@ __global__ void __launch_bounds__(kMaxThreads)
       s1 = s1 + du;
       s2 = fma(du, d, s2);
     };
-#pragma unroll 2
-    for (int i = 0; i < at.count; ++i) {
-      const Values v = *reinterpret_cast<const Values*>(from + i * at.stride);
-      const Values g = *reinterpret_cast<const Values*>(grad + i * at.stride);
-      kept_x[i * l.threads] = v;
-      kept_g[i * l.threads] = g;
-      add(v, g);
+    constexpr int U = 4;  // pairs of reads in flight
+    for (int i0 = 0; i0 < at.count; i0 += U) {
+      Values v[U], g[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u < at.count) {
+          v[u] = *reinterpret_cast<const Values*>(from + (i0 + u) * at.stride);
+          g[u] = *reinterpret_cast<const Values*>(grad + (i0 + u) * at.stride);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u < at.count) {
+          kept_x[(i0 + u) * l.threads] = v[u];
+          kept_g[(i0 + u) * l.threads] = g[u];
+          add(v[u], g[u]);
+        }
     }
     if (at.left) {
       const Values v = load_part<T, V>(from + at.count * at.stride, at.left);
@@ -988,12 +1018,10 @@ size_t splat_feature_norm_workspace_bytes(int dtype, int samples, long long posi
   if (check_norm(dtype, samples, positions, channels, groups, 0) != kOk) return 0;
   const Plan plan =
       make_plan(bytes_of(dtype), samples, positions, channels, groups, backward != 0);
-  // never 0, which means an error
-  size_t bytes = plan.small ? 16 : partial_bytes(samples, plan.l);
-  if (backward)
-    bytes += round_up(static_cast<size_t>(samples) * groups * sizeof(float2)) +
-             static_cast<size_t>(samples) * channels * sizeof(double2);
-  return bytes;
+  const size_t moments = round_up(static_cast<size_t>(samples) * groups * sizeof(float2));
+  if (!backward) return plan.small ? 16 : partial_bytes(samples, plan.l) + moments;
+  return (plan.small ? 0 : partial_bytes(samples, plan.l)) + moments +
+         static_cast<size_t>(samples) * channels * sizeof(double2);
 }
 
 int splat_feature_norm(int dtype, int samples, long long positions, int channels, int groups,
@@ -1002,14 +1030,15 @@ int splat_feature_norm(int dtype, int samples, long long positions, int channels
                        size_t workspace_bytes, void* stream) {
   const int bad = check_norm(dtype, samples, positions, channels, groups, activation);
   if (bad != kOk) return bad;
-  if (!x || !y || !mean || !rstd || !workspace)
+  if (!x || !y || !mean != !rstd)
     return host::fail(kInvalidArgument, "feature_norm: null pointer");
   if (!host::aligned(x, 16) || !host::aligned(y, 16) || !host::aligned(workspace, 16))
     return host::fail(kInvalidArgument, "feature_norm: x, y and workspace must be 16-byte aligned");
-  if (workspace_bytes <
-      splat_feature_norm_workspace_bytes(dtype, samples, positions, channels, groups, 0))
-    return host::fail(kWorkspaceTooSmall, "feature_norm: workspace");
   const Plan plan = make_plan(bytes_of(dtype), samples, positions, channels, groups, false);
+  const size_t partial = plan.small ? 0 : partial_bytes(samples, plan.l);
+  const size_t moments = round_up(static_cast<size_t>(samples) * groups * sizeof(float2));
+  if (!plan.small && (!workspace || workspace_bytes < partial + moments))
+    return host::fail(kWorkspaceTooSmall, "feature_norm: workspace");
   NormParams p{};
   p.l = plan.l;
   p.samples = samples;
@@ -1022,6 +1051,10 @@ int splat_feature_norm(int dtype, int samples, long long positions, int channels
   p.mean = mean;
   p.rstd = rstd;
   p.partial = static_cast<float2*>(workspace);
+  if (!mean && !plan.small) {  // the passes hand them on all the same
+    p.mean = reinterpret_cast<float*>(static_cast<char*>(workspace) + partial);
+    p.rstd = p.mean + static_cast<size_t>(samples) * groups;
+  }
   p.eps = eps;
   auto s = static_cast<cudaStream_t>(stream);
   const unsigned grid = static_cast<unsigned>(samples) * p.l.blocks * p.l.columns;
@@ -1055,10 +1088,11 @@ int splat_feature_norm_backward(int dtype, int samples, long long positions, int
       !host::aligned(workspace, 16))
     return host::fail(kInvalidArgument,
                       "feature_norm_backward: tensors and workspace must be 16-byte aligned");
-  if (workspace_bytes <
-      splat_feature_norm_workspace_bytes(dtype, samples, positions, channels, groups, 1))
-    return host::fail(kWorkspaceTooSmall, "feature_norm_backward: workspace");
   const Plan plan = make_plan(bytes_of(dtype), samples, positions, channels, groups, true);
+  if (workspace_bytes < (plan.small ? 0 : partial_bytes(samples, plan.l)) +
+                            round_up(static_cast<size_t>(samples) * groups * sizeof(float2)) +
+                            static_cast<size_t>(samples) * channels * sizeof(double2))
+    return host::fail(kWorkspaceTooSmall, "feature_norm_backward: workspace");
   NormParams p{};
   p.l = plan.l;
   p.samples = samples;
@@ -1073,7 +1107,7 @@ int splat_feature_norm_backward(int dtype, int samples, long long positions, int
   p.rstd = const_cast<float*>(rstd);
   char* at = static_cast<char*>(workspace);
   p.partial = reinterpret_cast<float2*>(at);
-  at += plan.small ? 16 : partial_bytes(samples, p.l);
+  at += plan.small ? 0 : partial_bytes(samples, p.l);
   p.moments = reinterpret_cast<float2*>(at);
   at += round_up(static_cast<size_t>(samples) * groups * sizeof(float2));
   p.channel = reinterpret_cast<double2*>(at);
@@ -1084,24 +1118,22 @@ int splat_feature_norm_backward(int dtype, int samples, long long positions, int
       constexpr int V = decltype(width)::value;
       T *dw = static_cast<T*>(dweight), *db = static_cast<T*>(dbias);
       return SPLAT_FEATURE_ACT(activation, [&] {
+        // a lone sample's sums are the parameters' gradients
+        const bool one = samples == 1;
+        T *dw1 = one ? dw : nullptr, *db1 = one ? db : nullptr;
         if (plan.small) {
-          const bool one = samples == 1;
-          const int status =
-              launch_cluster(norm_backward_small_kernel<T, V, ACT>, plan, samples, s, p,
-                             one ? dw : nullptr, one ? db : nullptr);
-          if (status != kOk || one || !(dw || db)) return status;
+          const int status = launch_cluster(norm_backward_small_kernel<T, V, ACT>, plan, samples,
+                                            s, p, dw1, db1);
+          if (status != kOk) return status;
+        } else {
+          norm_backward_sums_kernel<T, V, ACT><<<grid, p.l.threads, 0, host::counted(s)>>>(p);
+          norm_backward_join_kernel<T>
+              <<<samples * groups, kJoinThreads, 0, host::counted(s)>>>(p, dw1, db1);
+        }
+        if (!one && (dw || db))
           norm_parameters_kernel<T>
               <<<host::blocks_for(channels, 128), 128, 0, host::counted(s)>>>(p, dw, db);
-          return host::check_launch("feature_norm_backward");
-        }
-        norm_backward_sums_kernel<T, V, ACT><<<grid, p.l.threads, 0, host::counted(s)>>>(p);
-        norm_backward_join_kernel<T>
-            <<<samples * groups, kJoinThreads, 0, host::counted(s)>>>(p);
-        if (dweight || dbias)
-          norm_parameters_kernel<T>
-              <<<host::blocks_for(channels, 128), 128, 0, host::counted(s)>>>(
-                  p, dw, db);
-        if (dx)
+        if (dx && !plan.small)
           norm_backward_apply_kernel<T, V, ACT><<<grid, p.l.threads, 0, host::counted(s)>>>(p);
         return host::check_launch("feature_norm_backward");
       });

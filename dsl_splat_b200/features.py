@@ -183,7 +183,7 @@ def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tenso
     if _recorded(x, weight, bias):
         y = _GroupNorm.apply(x, weight, bias, int(groups), float(eps), activation)
     else:
-        y = stages.feature_norm(x, groups, weight, bias, eps, activation)[0]
+        y = stages.feature_norm(x, groups, weight, bias, eps, activation, False)[0]
     return y.reshape(shape)
 
 

@@ -752,23 +752,25 @@ def feature_linear_backward(x: Tensor, weight: Tensor, bias: Tensor | None, acti
 
 
 def feature_norm(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None, eps: float,
-                 activation: str) -> tuple[Tensor, Tensor]:
-    """Group norm with an activation of x (B,S,C): y, and the fp32 means and
-    reciprocal deviations (2,B,groups)."""
+                 activation: str, save: bool = True) -> tuple[Tensor, Tensor | None]:
+    """Group norm with an activation of x (B,S,C): y, and (save) the fp32 means
+    and reciprocal deviations (2,B,groups)."""
     samples, positions, channels = x.shape
     y = x.new_empty((samples, positions, channels))
-    moments = x.new_empty((2, samples, groups), dtype=torch.float32)
+    moments = x.new_empty((2, samples, groups), dtype=torch.float32) if save else None
     if samples and positions:
         dtype, device = FEATURE_DTYPES[x.dtype], x.device
         size = _query(lib.splat_feature_norm_workspace_bytes, "feature_norm", device, dtype,
                       samples, positions, channels, groups, 0)
-        ws = x.new_empty((size,), dtype=torch.uint8)
+        ws = x.new_empty((size,), dtype=torch.uint8) if size > 16 else None
         x, weight, bias = _dense(x), _dense(weight), _dense(bias)
-        mean = moments.data_ptr()
+        mean = rstd = None
+        if save:
+            mean = moments.data_ptr()
+            rstd = mean + 4 * samples * groups
         _call(lib.splat_feature_norm, "feature_norm", device, dtype, samples, positions, channels,
               groups, x.data_ptr(), _address(weight), _address(bias), eps,
-              _ACTIVATION_CODES[activation], y.data_ptr(), mean, mean + 4 * samples * groups,
-              ws.data_ptr(), size)
+              _ACTIVATION_CODES[activation], y.data_ptr(), mean, rstd, _address(ws), size)
     return y, moments
 
 

@@ -590,8 +590,9 @@ int splat_feature_linear_backward(int dtype, long long rows, int k, int n, const
 
 /* y = act((x - mean) rstd weight_c + bias_c); x, y (samples, positions,
  * channels); mean and rstd (samples, groups) float32 over the positions of a
- * sample and the channels of a group, written for the backward; weight, bias
- * (channels) or NULL. */
+ * sample and the channels of a group, written for the backward, or both NULL;
+ * weight, bias (channels) or NULL.  A forward workspace of 16 bytes or less
+ * may be NULL. */
 size_t splat_feature_norm_workspace_bytes(int dtype, int samples, long long positions,
                                           int channels, int groups, int backward);
 int splat_feature_norm(int dtype, int samples, long long positions, int channels, int groups,

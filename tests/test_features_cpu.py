@@ -105,7 +105,9 @@ def test_entry_points_refuse_before_any_launch():
                                   None) == -1
     assert lib.splat_feature_norm(0, 1, 4, 8, 2, P + 4, None, None, 1e-5, 0, P, P, P, P, 1 << 20,
                                   None) == -1
-    assert lib.splat_feature_norm(0, 1, 4, 8, 2, P, None, None, 1e-5, 0, P, P, P, P, 0,
+    assert lib.splat_feature_norm(0, 1, 4, 8, 2, P, None, None, 1e-5, 0, P, P, None, P, 1 << 20,
+                                  None) == -1
+    assert lib.splat_feature_norm(0, 1, 1 << 20, 8, 2, P, None, None, 1e-5, 0, P, P, P, P, 0,
                                   None) == -5
     assert lib.splat_feature_norm(0, 1, 1 << 32, 8, 2, P, None, None, 1e-5, 0, P, P, P, P, 0,
                                   None) == -4
