@@ -41,7 +41,7 @@ HEADERS = ["splat_common.cuh", "cameras.cuh", "project.cuh", "binning.cuh", "ren
            "footprint.cuh", "tile_modes.cuh", "host_runtime.h", "rade.cuh", "rade_project.cuh",
            "aaa.cuh", "aaa_render.cuh", "aaa_api.cuh", "aaa_blend_params.cuh",
            "aaa_backward.cuh", "feature_common.cuh", "feature_product.cuh", "feature_fused.cuh",
-           "feature_launch.cuh", "tensor_core.cuh"]
+           "feature_launch.cuh", "feature_narrow.cuh", "tensor_core.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -10,8 +10,8 @@
 // tile (fp32: the tensor core truncates its sums).
 //
 // A block of eight warps does each tile's steps together: load, product,
-// activation slope, products, store.  What overlaps one block's steps is the
-// other blocks of its SM, and copies of the next tile's x.
+// activation slope, products, store; other blocks of its SM overlap them.
+// 16-bit types with 16-byte rows take the pass of feature_narrow.cuh instead.
 #pragma once
 #include "feature_product.cuh"
 
@@ -25,48 +25,9 @@ struct FusedParams {
   void* dx;        // (rows, k) or NULL
   float* partial;  // per block: (n, k) of dW, then (n) of db; NULL: neither
   int activation, x_vector, w_vector, dy_vector, dx_vector;
-  int buffers;  // of x: 2 when the next tile's x and dy are copied ahead
   uint32_t tiles, tmem_columns;
   int* error;
 };
-
-// The same for one-part operands whose rows are 16-byte aligned, by copies that
-// the thread does not wait for.
-template <class S>
-SPLAT_DEV void fill_async(uint32_t dst, int rows, int pieces, const S* src, long long ld,
-                          long long rows_valid, long long cols_valid, int thread, int threads) {
-  const int shift = pieces <= 1 ? 0 : pieces <= 2 ? 1 : pieces <= 4 ? 2 : 3;
-  const int total = rows << shift;
-  const int piece = thread & ((1 << shift) - 1);  // threads is a multiple of 8
-  if (piece >= pieces) return;
-  const long long left = cols_valid - piece * 8;
-  const int bytes = left <= 0 ? 0 : static_cast<int>(left < 8 ? left : 8) * 2;
-  src += piece * 8;
-#pragma unroll 4
-  for (int i = thread; i < total; i += threads) {
-    const int row = i >> shift;
-    const bool in = row < rows_valid && bytes;
-    // a copy of no bytes fills with zeros; its address stays inside the source
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                     dst + row * 128 + ((piece ^ (row & 7)) << 4)),
-                 "l"(in ? src + row * ld : src - piece * 8), "r"(in ? bytes : 0)
-                 : "memory");
-  }
-}
-
-// Waits until at most `lag` groups of the thread's copies are in flight.
-SPLAT_DEV void wait_copies(int lag) {
-  switch (lag) {
-    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-    case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-    case 5: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
-    case 6: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
-    default: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
-  }
-}
 
 constexpr int kFusedThreads = 256;
 constexpr int kFusedWidth = 128;        // widest k and n
@@ -79,16 +40,11 @@ struct Fused {
   __host__ __device__ static int blocks64(int n) { return (n + 63) / 64; }
   // a patch of 32 x 32 values for each warp
   __host__ __device__ static int staging_bytes() { return 8 * 1024 * sizeof(T); }
-  // and, when the next tile is copied ahead, the warps' patches of its dy
-  __host__ __device__ static int ahead_bytes(int n32) {
-    return (n32 + 63) / 64 * staging_bytes();
-  }
   __host__ __device__ static int x_plane(int k) { return blocks64(k) * kAPlane; }
   __host__ __device__ static int w_plane(int k, int n32) { return blocks64(k) * n32 * 128; }
-  static size_t shared_bytes(int k, int n, int n32, int buffers) {
-    return staging_bytes() + static_cast<size_t>(buffers) * P * x_plane(k) +
-           P * x_plane(n) + P * w_plane(k, n32) + (buffers == 2 ? ahead_bytes(n32) : 0) +
-           kOnesBytes + 1024 + kFusedWidth * 4;
+  static size_t shared_bytes(int k, int n, int n32) {
+    return static_cast<size_t>(staging_bytes()) + P * x_plane(k) + P * x_plane(n) +
+           P * w_plane(k, n32) + kOnesBytes + 1024 + kFusedWidth * 4;
   }
 };
 
@@ -105,17 +61,15 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
   const uint32_t x_plane = F::x_plane(p.k), z_plane = F::x_plane(p.n);
   const uint32_t w_plane = F::w_plane(p.k, p.n32);
   const uint32_t x_at = base + F::staging_bytes();
-  const uint32_t z_at = x_at + p.buffers * P * x_plane;
+  const uint32_t z_at = x_at + P * x_plane;
   const uint32_t w_at = z_at + P * z_plane;
-  const uint32_t dy_at = w_at + P * w_plane;
-  const uint32_t ones_at = dy_at + (p.buffers == 2 ? F::ahead_bytes(p.n32) : 0);
+  const uint32_t ones_at = w_at + P * w_plane;
   const uint32_t bias_at = ones_at + kOnesBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int lane_block = warp & 3, half = warp >> 2;
   const Patch<T> patch{base + warp * static_cast<uint32_t>(1024 * sizeof(T))};
   const T* x = static_cast<const T*>(p.x);
   const bool with_z = p.activation != kNone;
-  const bool ahead = p.buffers == 2;
 
   if (threadIdx.x == 0) {
     tc::barrier_init(tc::shared_address(&z_done), 1);
@@ -140,40 +94,6 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
                  "f"(p.bias && i < p.n ? to_float(static_cast<const T*>(p.bias)[i]) : 0.0f)
                  : "memory");
 
-  const auto load_x = [&](uint32_t tile, uint32_t at, bool async) {
-    const long long m0 = static_cast<long long>(tile) * kTileRows;
-    for (int c = 0; c * 64 < p.k; ++c) {
-      const int valid = p.k - c * 64;
-      const int pieces = min((valid + 15) / 16 * 2, 8);
-      const T* src = x + m0 * p.k + c * 64;
-      if constexpr (sizeof(T) == 2) {
-        if (async) {
-          fill_async<T>(at + c * kAPlane, kTileRows, pieces, src, p.k, p.rows - m0, valid,
-                        threadIdx.x, kFusedThreads);
-          continue;
-        }
-      }
-      fill<T, P>(p.x_vector, at + c * kAPlane, x_plane, kTileRows, pieces, src, p.k,
-                  p.rows - m0, valid, threadIdx.x, kFusedThreads);
-    }
-  };
-  // copies of this warp's patches of dy, into memory that only it touches
-  const auto copy_dy = [&](uint32_t tile) {
-    if constexpr (sizeof(T) == 2) {
-      const long long from = static_cast<long long>(tile) * kTileRows + lane_block * 32;
-      const int left = static_cast<int>(max(min(p.rows - from, 32LL), 0LL));
-      for (int c = half; c * 32 < p.n32; c += 2)
-        Patch<T>{dy_at + ((c >> 1) * 8 + warp) * static_cast<uint32_t>(1024 * sizeof(T))}
-            .load_async(left ? static_cast<const T*>(p.dy) + from * p.n + c * 32
-                             : static_cast<const T*>(p.dy),
-                        p.n, left, min(p.n - c * 32, 32));
-    }
-  };
-  if (ahead) {
-    load_x(blockIdx.x, x_at, true);
-    copy_dy(blockIdx.x);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -183,16 +103,17 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
   float sum_w[kAcc == 2 ? 2 : 1][32] = {};  // fp32: this thread's part of dW
   float sum_b = 0.0f;
   uint32_t parity = 0;
-  int buffer = 0;
   bool ok = true, fresh = true;
   for (uint32_t t = blockIdx.x; t < p.tiles; t += gridDim.x, parity ^= 1) {
     const long long row0 = static_cast<long long>(t) * kTileRows + lane_block * 32;
     const int rows = static_cast<int>(max(min(p.rows - row0, 32LL), 0LL));
-    const uint32_t x_now = x_at + buffer * P * x_plane;
-    if (ahead)
-      wait_copies(0);
-    else
-      load_x(t, x_now, false);
+    const long long m0 = static_cast<long long>(t) * kTileRows;
+    for (int c = 0; c * 64 < p.k; ++c) {
+      const int valid = p.k - c * 64;
+      fill<T, P>(p.x_vector, x_at + c * kAPlane, x_plane, kTileRows,
+                 min((valid + 15) / 16 * 2, 8), x + m0 * p.k + c * 64, p.k, p.rows - m0, valid,
+                 threadIdx.x, kFusedThreads);
+    }
     tc::fence_async_proxy();
     tc::fence_before_sync();
     // x is there, and the previous tile's accumulators have been read
@@ -208,29 +129,20 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
           for (int s = 0; s * 16 < p.k; ++s) {
             const uint32_t o = (s & 3) * tc::kStepK;
             tc::mma(tmem,
-                    tc::descriptor_k_major(x_now + i * x_plane + (s >> 2) * kAPlane + o),
+                    tc::descriptor_k_major(x_at + i * x_plane + (s >> 2) * kAPlane + o),
                     tc::descriptor_k_major(w_at + (sum - i) * w_plane + (s >> 2) * p.n32 * 128 + o),
                     instruction, !first);
             first = false;
           }
       tc::commit(tc::shared_address(&z_done));
     }
-    if (ahead) {
-      buffer ^= 1;
-      if (t + gridDim.x < p.tiles) load_x(t + gridDim.x, x_at + buffer * P * x_plane, true);
-    }
     // dz: a lane's row of each 32-wide patch
     bool waited = !with_z;
     for (int c = half; c * 32 < p.n32; c += 2) {
-      const Patch<T> dy{ahead ? dy_at + ((c >> 1) * 8 + warp) * static_cast<uint32_t>(
-                                                                   1024 * sizeof(T))
-                              : patch.base};
-      if (!ahead) {
-        __syncwarp();
-        dy.load(static_cast<const T*>(p.dy) + row0 * p.n + c * 32, p.n, rows,
-                min(p.n - c * 32, 32), p.dy_vector);
-        __syncwarp();
-      }
+      __syncwarp();
+      patch.load(static_cast<const T*>(p.dy) + row0 * p.n + c * 32, p.n, rows,
+                 min(p.n - c * 32, 32), p.dy_vector);
+      __syncwarp();
       float v[32];
       if (!waited) {
         ok = tc::barrier_wait(tc::shared_address(&z_done), parity) && ok;
@@ -248,11 +160,11 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
         }
       }
       switch (p.activation) {
-        case kRelu: finish_row<kSlope, kRelu, T>(dy, true, v); break;
-        case kSilu: finish_row<kSlope, kSilu, T>(dy, true, v); break;
-        case kGelu: finish_row<kSlope, kGelu, T>(dy, true, v); break;
-        case kSigmoid: finish_row<kSlope, kSigmoid, T>(dy, true, v); break;
-        default: finish_row<kSlope, kNone, T>(dy, true, v);
+        case kRelu: finish_row<kSlope, kRelu, T>(patch, true, v); break;
+        case kSilu: finish_row<kSlope, kSilu, T>(patch, true, v); break;
+        case kGelu: finish_row<kSlope, kGelu, T>(patch, true, v); break;
+        case kSigmoid: finish_row<kSlope, kSigmoid, T>(patch, true, v); break;
+        default: finish_row<kSlope, kNone, T>(patch, true, v);
       }
       if (lane >= rows) {  // rows past the end add nothing to dW
 #pragma unroll
@@ -279,11 +191,6 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
         for (int q = 0; q < P; ++q)
           store_shared(at + q * z_plane + ((((c & 1) * 4 + j) ^ (row & 7)) << 4), parts[q]);
       }
-    }
-    if (ahead) {
-      __syncwarp();  // this tile's dy has been read
-      if (t + gridDim.x < p.tiles) copy_dy(t + gridDim.x);
-      asm volatile("cp.async.commit_group;" ::: "memory");
     }
     tc::fence_async_proxy();
     tc::fence_before_sync();
@@ -327,7 +234,7 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
             for (int s = 0; s < kTileRows / 16; ++s)
               tc::mma(acc_w + (own ? 0 : (kAcc - 1) * p.k32),
                       tc::descriptor_mn_major(z_at + i * z_plane + s * tc::kStepMn, z_block),
-                      tc::descriptor_mn_major(x_now + j * x_plane + s * tc::kStepMn, kAPlane),
+                      tc::descriptor_mn_major(x_at + j * x_plane + s * tc::kStepMn, kAPlane),
                       wide, !(first && s == 0));
           }
 #pragma unroll
@@ -419,7 +326,6 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
       }
     }
   }
-  if (ahead) wait_copies(0);
   if (threadIdx.x == 0) {  // also after a wait that ran out
     tc::commit(tc::shared_address(&drained));
     ok = tc::barrier_wait(tc::shared_address(&drained), 0) && ok;

@@ -10,6 +10,7 @@
 
 #include "feature_fused.cuh"
 #include "feature_launch.cuh"
+#include "feature_narrow.cuh"
 #include "splat200.h"
 
 namespace splat {
@@ -132,7 +133,8 @@ int launch_gradients(long long rows, int k, int n, const T* dz, const void* x,
 
 // How a narrow layer's pass is launched; blocks == 0: the layer is too wide.
 struct FusedPlan {
-  int blocks, buffers;
+  int blocks;
+  bool copies;  // by tensor copies
   size_t bytes;
   uint32_t tmem_columns;
 };
@@ -148,16 +150,18 @@ FusedPlan plan_fused(long long rows, int k, int n) {
   plan.tmem_columns = 32;
   while (plan.tmem_columns < static_cast<uint32_t>(std::max(k32, n32) + F::kAcc * (k32 + 32)))
     plan.tmem_columns *= 2;
-  plan.buffers = 1;
-  plan.bytes = F::shared_bytes(k, n, n32, 1);
-  if (plan.tmem_columns > 512 || plan.bytes > kOneBlockBytes) return plan;
+  const int row_align = 16 / static_cast<int>(sizeof(T));
+  plan.copies = sizeof(T) == 2 && k % row_align == 0 && n % row_align == 0 && rows < 1LL << 31;
   int per_sm = 1;
-  if (sizeof(T) == 2 && plan.tmem_columns <= 256 && plan.bytes <= kTwoBlocksBytes) per_sm = 2;
-  // x and dy are copied ahead where that costs no block
-  if (sizeof(T) == 2 && k % 8 == 0 && n % 8 == 0) {
-    const size_t two = F::shared_bytes(k, n, n32, 2);
-    if (two <= static_cast<size_t>(per_sm == 2 ? kTwoBlocksBytes : kOneBlockBytes))
-      plan.buffers = 2, plan.bytes = two;
+  if (plan.copies) {
+    plan.bytes = narrow_bytes(k, n, n32);
+    plan.tmem_columns = 32;
+    while (plan.tmem_columns < static_cast<uint32_t>(n32 + 2 * k32)) plan.tmem_columns *= 2;
+    if (k <= 64 && n <= 64) per_sm = 2;
+  } else {
+    plan.bytes = F::shared_bytes(k, n, n32);
+    if (plan.tmem_columns > 512 || plan.bytes > kOneBlockBytes) return plan;
+    if (sizeof(T) == 2 && plan.tmem_columns <= 256 && plan.bytes <= kTwoBlocksBytes) per_sm = 2;
   }
   plan.blocks = static_cast<int>(std::min<long long>(
       (rows + kTileRows - 1) / kTileRows, static_cast<long long>(host::sm_count()) * per_sm));
@@ -165,32 +169,64 @@ FusedPlan plan_fused(long long rows, int k, int n) {
 }
 
 template <class T>
-int launch_fused(const FusedPlan& plan, long long rows, int k, int n, const void* x,
-                 const void* weight, const void* bias, int activation, const void* dy, void* dx,
-                 void* dweight, void* dbias, float* partial, cudaStream_t s) {
-  FusedParams p{};
+int launch_narrow(const FusedPlan& plan, long long rows, int k, int n, const void* x,
+                  const void* weight, const void* bias, int activation, const void* dy, void* dx,
+                  float* partial, cudaStream_t s) {
+  NarrowParams p{};
   p.rows = rows, p.k = k, p.n = n, p.k32 = round32(k), p.n32 = round32(n);
-  p.x = x, p.weight = weight, p.bias = bias, p.dy = dy, p.dx = dx;
-  p.partial = dweight || dbias ? partial : nullptr;
-  p.activation = activation;
-  p.x_vector = row_vector<T>(x, k);
-  p.w_vector = row_vector<T>(weight, k);
-  p.dy_vector = n * sizeof(T) % 16 == 0 && host::aligned(dy, 16);
-  p.dx_vector = k * sizeof(T) % 16 == 0 && host::aligned(dx, 16);
-  if (plan.buffers == 2 && (p.x_vector != 16 || !p.dy_vector))
-    return host::fail(kInvalidArgument,
-                      "feature_linear_backward: x and dy must be 16-byte aligned");
-  p.buffers = plan.buffers;
+  p.bias = bias, p.with_dx = dx != nullptr, p.partial = partial, p.activation = activation;
   p.tiles = static_cast<uint32_t>((rows + kTileRows - 1) / kTileRows);
   p.tmem_columns = plan.tmem_columns;
   p.error = host::device_error_word();
   if (!p.error) return kCudaError;
-  auto* kernel = fused_backward_kernel<T>;
+  if (!make_map<T>(p.x_map, x, rows, k, k, 64, kTileRows) ||
+      !make_map<T>(p.dy_map, dy, rows, n, n, 64, kTileRows) ||
+      !make_map<T>(p.w_map, weight, n, k, k, 64, p.n32) ||
+      (dx && !make_map<T>(p.dx_map, dx, rows, k, k, 32, 32)))
+    return host::fail(kInvalidArgument,
+                      "feature_linear_backward: tensors must be 16-byte aligned");
+  const bool wide = k > 64 || n > 64;
+  auto* kernel = wide ? narrow_backward_kernel<T, true> : narrow_backward_kernel<T, false>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(plan.bytes)) != cudaSuccess)
     return host::check_launch("feature_linear_backward: shared memory");
-  kernel<<<plan.blocks, kFusedThreads, plan.bytes, host::counted(s)>>>(p);
-  if (p.partial) {
+  kernel<<<plan.blocks, kNarrowThreads, plan.bytes, host::counted(s)>>>(p);
+  return host::check_launch("feature_linear_backward");
+}
+
+template <class T>
+int launch_fused(const FusedPlan& plan, long long rows, int k, int n, const void* x,
+                 const void* weight, const void* bias, int activation, const void* dy, void* dx,
+                 void* dweight, void* dbias, float* partial, cudaStream_t s) {
+  if (!dweight && !dbias) partial = nullptr;
+  if constexpr (sizeof(T) == 2) {
+    if (plan.copies) {
+      const int status =
+          launch_narrow<T>(plan, rows, k, n, x, weight, bias, activation, dy, dx, partial, s);
+      if (status != kOk) return status;
+    }
+  }
+  if (!plan.copies) {
+    FusedParams p{};
+    p.rows = rows, p.k = k, p.n = n, p.k32 = round32(k), p.n32 = round32(n);
+    p.x = x, p.weight = weight, p.bias = bias, p.dy = dy, p.dx = dx;
+    p.partial = partial;
+    p.activation = activation;
+    p.x_vector = row_vector<T>(x, k);
+    p.w_vector = row_vector<T>(weight, k);
+    p.dy_vector = n * sizeof(T) % 16 == 0 && host::aligned(dy, 16);
+    p.dx_vector = k * sizeof(T) % 16 == 0 && host::aligned(dx, 16);
+    p.tiles = static_cast<uint32_t>((rows + kTileRows - 1) / kTileRows);
+    p.tmem_columns = plan.tmem_columns;
+    p.error = host::device_error_word();
+    if (!p.error) return kCudaError;
+    auto* kernel = fused_backward_kernel<T>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(plan.bytes)) != cudaSuccess)
+      return host::check_launch("feature_linear_backward: shared memory");
+    kernel<<<plan.blocks, kFusedThreads, plan.bytes, host::counted(s)>>>(p);
+  }
+  if (partial) {
     const long long count = static_cast<long long>(n) * k;
     join_splits<T>(partial, count + n, plan.blocks, count, n, dweight, dbias, s);
   }

@@ -286,21 +286,6 @@ struct Patch {
     }
   }
 
-  // The same by copies that the thread does not wait for; 16-bit types whose
-  // rows are whole pieces.
-  SPLAT_DEV void load_async(const T* src, long long ld, int rows, int cols) const {
-    constexpr int kRows = 32 / kPieces;
-    const int lane = threadIdx.x & 31, piece = lane % kPieces, r0 = lane / kPieces;
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int r = i * kRows + r0;
-      const bool in = r < rows && piece * V < cols;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at(r, piece)),
-                   "l"(in ? src + r * ld + piece * V : src), "r"(in ? 16 : 0)
-                   : "memory");
-    }
-  }
-
   // Staging -> global memory; add (fp32 only): onto what is there.
   SPLAT_DEV void store(T* dst, long long ld, int rows, int cols, bool vector, bool add) const {
     const int lane = threadIdx.x & 31;
