@@ -9,8 +9,10 @@
 // result's rounding at 10^5 additions) or is added up in registers after every
 // tile (fp32: the tensor core truncates its sums).
 //
-// A block of eight warps does each tile's steps together: load, product,
-// activation slope, products, store; other blocks of its SM overlap them.
+// A block of 16 warps does each tile's steps together: load, product,
+// activation slope, products, store, while bulk copies bring the next tile's x
+// and dy (contiguous whatever their row lengths) to shared memory; where those
+// do not fit beside the operands, the steps read global memory.
 // 16-bit types with 16-byte rows take the pass of feature_narrow.cuh instead.
 #pragma once
 #include "feature_product.cuh"
@@ -25,11 +27,12 @@ struct FusedParams {
   void* dx;        // (rows, k) or NULL
   float* partial;  // per block: (n, k) of dW, then (n) of db; NULL: neither
   int activation, x_vector, w_vector, dy_vector, dx_vector;
+  int raw;  // x and dy are copied ahead
   uint32_t tiles, tmem_columns;
   int* error;
 };
 
-constexpr int kFusedThreads = 256;
+constexpr int kFusedThreads = 512, kFusedWarps = kFusedThreads / 32;
 constexpr int kFusedWidth = 128;        // widest k and n
 constexpr int kOnesBytes = 16 * 128;    // 16 rows of 64 ones
 
@@ -38,13 +41,18 @@ struct Fused {
   static constexpr int P = sizeof(T) == 4 ? 3 : 1;  // parts of every operand
   static constexpr int kAcc = sizeof(T) == 4 ? 2 : 1;  // accumulators of dW and db
   __host__ __device__ static int blocks64(int n) { return (n + 63) / 64; }
-  // a patch of 32 x 32 values for each warp
-  __host__ __device__ static int staging_bytes() { return 8 * 1024 * sizeof(T); }
+  // a patch of 32 x 16 values for each warp
+  __host__ __device__ static int staging_bytes() { return kFusedWarps * 512 * sizeof(T); }
+  // a tile of rows of n values as it is in memory
+  __host__ __device__ static int raw_bytes(int n) {
+    return (kTileRows * n * static_cast<int>(sizeof(T)) + 127) / 128 * 128;
+  }
   __host__ __device__ static int x_plane(int k) { return blocks64(k) * kAPlane; }
   __host__ __device__ static int w_plane(int k, int n32) { return blocks64(k) * n32 * 128; }
-  static size_t shared_bytes(int k, int n, int n32) {
+  static size_t shared_bytes(int k, int n, int n32, bool raw) {
     return static_cast<size_t>(staging_bytes()) + P * x_plane(k) + P * x_plane(n) +
-           P * w_plane(k, n32) + kOnesBytes + 1024 + kFusedWidth * 4;
+           P * w_plane(k, n32) + kOnesBytes + 1024 + kFusedWidth * 4 +
+           (raw ? raw_bytes(k) + raw_bytes(n) : 0);
   }
 };
 
@@ -55,7 +63,7 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
   constexpr int kAcc = F::kAcc;
   constexpr int P = F::P;
   extern __shared__ unsigned char dynamic[];
-  __shared__ alignas(8) unsigned long long z_done, dx_done, dw_done, drained;
+  __shared__ alignas(8) unsigned long long z_done, dx_done, dw_done, drained, x_raw, dy_raw;
   __shared__ uint32_t tmem_base;
   const uint32_t base = (tc::shared_address(dynamic) + 1023u) & ~1023u;
   const uint32_t x_plane = F::x_plane(p.k), z_plane = F::x_plane(p.n);
@@ -66,9 +74,20 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
   const uint32_t ones_at = w_at + P * w_plane;
   const uint32_t bias_at = ones_at + kOnesBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int lane_block = warp & 3, half = warp >> 2;
-  const Patch<T> patch{base + warp * static_cast<uint32_t>(1024 * sizeof(T))};
+  // a warp's patches: 16 columns from 16 group on, and from 64 + 16 group on
+  const int lane_block = warp & 3, group = warp >> 2;
+  const Patch<T, 16> patch{base + warp * static_cast<uint32_t>(512 * sizeof(T))};
+  const uint32_t x_raw_at = bias_at + kFusedWidth * 4;
+  const uint32_t dy_raw_at = x_raw_at + F::raw_bytes(p.k);
   const T* x = static_cast<const T*>(p.x);
+  // thread 0: copies of a tile
+  const auto copy_rows = [&](const void* from, int width, uint32_t tile, uint32_t to,
+                             unsigned long long& bar) {
+    const long long m0 = static_cast<long long>(tile) * kTileRows;
+    copy_run<T>(to, static_cast<const T*>(from) + m0 * width,
+                static_cast<int>(min(p.rows - m0, static_cast<long long>(kTileRows))) * width,
+                tc::shared_address(&bar));
+  };
   const bool with_z = p.activation != kNone;
 
   if (threadIdx.x == 0) {
@@ -76,7 +95,13 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
     tc::barrier_init(tc::shared_address(&dx_done), 1);
     tc::barrier_init(tc::shared_address(&dw_done), 1);
     tc::barrier_init(tc::shared_address(&drained), 1);
+    tc::barrier_init(tc::shared_address(&x_raw), 1);
+    tc::barrier_init(tc::shared_address(&dy_raw), 1);
     tc::barrier_init_fence();
+    if (p.raw) {
+      copy_rows(p.x, p.k, blockIdx.x, x_raw_at, x_raw);
+      copy_rows(p.dy, p.n, blockIdx.x, dy_raw_at, dy_raw);
+    }
   }
   if (warp == 0) tc::tmem_alloc(tc::shared_address(&tmem_base), p.tmem_columns);
   // W, a block of ones and the bias stay for all tiles
@@ -100,7 +125,7 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
   const uint32_t tmem = tmem_base;
   const uint32_t acc_w = tmem + max(p.k32, p.n32), acc_b = acc_w + kAcc * p.k32;
 
-  float sum_w[kAcc == 2 ? 2 : 1][32] = {};  // fp32: this thread's part of dW
+  float sum_w[kAcc == 2 ? 2 : 1][16] = {};  // fp32: this thread's part of dW
   float sum_b = 0.0f;
   uint32_t parity = 0;
   bool ok = true, fresh = true;
@@ -108,16 +133,26 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
     const long long row0 = static_cast<long long>(t) * kTileRows + lane_block * 32;
     const int rows = static_cast<int>(max(min(p.rows - row0, 32LL), 0LL));
     const long long m0 = static_cast<long long>(t) * kTileRows;
+    const bool next = p.tiles - t > gridDim.x;
+    if (p.raw) ok = tc::barrier_wait(tc::shared_address(&x_raw), parity) && ok;
     for (int c = 0; c * 64 < p.k; ++c) {
-      const int valid = p.k - c * 64;
-      fill<T, P>(p.x_vector, x_at + c * kAPlane, x_plane, kTileRows,
-                 min((valid + 15) / 16 * 2, 8), x + m0 * p.k + c * 64, p.k, p.rows - m0, valid,
-                 threadIdx.x, kFusedThreads);
+      const int valid = p.k - c * 64, pieces = min((valid + 15) / 16 * 2, 8);
+      if (p.raw)
+        fill_shared<T, P>(p.x_vector, x_at + c * kAPlane, x_plane, kTileRows, pieces,
+                          x_raw_at + c * 64 * static_cast<int>(sizeof(T)),
+                          p.k * static_cast<int>(sizeof(T)),
+                          static_cast<int>(min(p.rows - m0, static_cast<long long>(kTileRows))),
+                          valid, threadIdx.x, kFusedThreads);
+      else
+        fill<T, P>(p.x_vector, x_at + c * kAPlane, x_plane, kTileRows, pieces, x + m0 * p.k + c * 64,
+                   p.k, p.rows - m0, valid, threadIdx.x, kFusedThreads);
     }
     tc::fence_async_proxy();
     tc::fence_before_sync();
     // x is there, and the previous tile's accumulators have been read
     if (__syncthreads_or(!ok)) break;
+    if (threadIdx.x == 0 && p.raw && next)
+      copy_rows(p.x, p.k, t + gridDim.x, x_raw_at, x_raw);
     if (threadIdx.x == 0 && with_z) {
       tc::fence_after_sync();
       const uint32_t instruction = tc::instruction(!kIsF16<T>, false, false, p.n32);
@@ -136,24 +171,30 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
           }
       tc::commit(tc::shared_address(&z_done));
     }
-    // dz: a lane's row of each 32-wide patch
+    // dz: a lane's row of each patch
     bool waited = !with_z;
-    for (int c = half; c * 32 < p.n32; c += 2) {
+    if (p.raw) ok = tc::barrier_wait(tc::shared_address(&dy_raw), parity) && ok;
+    for (int c = group * 16; c < p.n32; c += 64) {
+      const int cols = min(p.n - c, 16);
       __syncwarp();
-      patch.load(static_cast<const T*>(p.dy) + row0 * p.n + c * 32, p.n, rows,
-                 min(p.n - c * 32, 32), p.dy_vector);
+      if (p.raw)
+        patch.load_shared_rows(
+            dy_raw_at + ((lane_block * 32) * p.n + c) * static_cast<int>(sizeof(T)), p.n, rows, cols,
+            p.dy_vector);
+      else
+        patch.load(static_cast<const T*>(p.dy) + row0 * p.n + c, p.n, rows, cols, p.dy_vector);
       __syncwarp();
-      float v[32];
+      float v[16];
       if (!waited) {
         ok = tc::barrier_wait(tc::shared_address(&z_done), parity) && ok;
         tc::fence_after_sync();
         waited = true;
       }
       if (with_z) {
-        tc::tmem_load32(tmem + (lane_block << 21) + c * 32, v);
+        tc::tmem_load16(tmem + (lane_block << 21) + c, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float4 b = load_shared(bias_at + (c * 32 + j * 4) * 4);
+        for (int j = 0; j < 4; ++j) {
+          const float4 b = load_shared(bias_at + (c + j * 4) * 4);
           unpack2(add2(pack2(v[4 * j], v[4 * j + 1]), pack2(b.x, b.y)), v[4 * j], v[4 * j + 1]);
           unpack2(add2(pack2(v[4 * j + 2], v[4 * j + 3]), pack2(b.z, b.w)), v[4 * j + 2],
                   v[4 * j + 3]);
@@ -168,12 +209,12 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
       }
       if (lane >= rows) {  // rows past the end add nothing to dW
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+        for (int j = 0; j < 16; ++j) v[j] = 0.0f;
       }
       const int row = lane_block * 32 + lane;
-      const uint32_t at = z_at + (c >> 1) * kAPlane + row * 128;
+      const uint32_t at = z_at + (c >> 6) * kAPlane + row * 128;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 2; ++j) {
         uint4 parts[P];
         if constexpr (sizeof(T) == 2) {
           float o[8];
@@ -189,13 +230,14 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
         }
 #pragma unroll
         for (int q = 0; q < P; ++q)
-          store_shared(at + q * z_plane + ((((c & 1) * 4 + j) ^ (row & 7)) << 4), parts[q]);
+          store_shared(at + q * z_plane + ((((c & 63) / 8 + j) ^ (row & 7)) << 4), parts[q]);
       }
     }
     tc::fence_async_proxy();
     tc::fence_before_sync();
     __syncthreads();  // dz is there, z has been read
     if (threadIdx.x == 0) {
+      if (p.raw && next) copy_rows(p.dy, p.n, t + gridDim.x, dy_raw_at, dy_raw);
       tc::fence_after_sync();
       if (p.dx) {
         const uint32_t instruction = tc::instruction(!kIsF16<T>, false, true, p.k32);
@@ -254,13 +296,13 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
     if (p.dx) {
       ok = tc::barrier_wait(tc::shared_address(&dx_done), parity) && ok;
       tc::fence_after_sync();
-      for (int c = half; c * 32 < p.k32; c += 2) {
-        float v[32];
-        tc::tmem_load32(tmem + (lane_block << 21) + c * 32, v);
+      for (int c = group * 16; c < p.k; c += 64) {
+        float v[16];
+        tc::tmem_load16(tmem + (lane_block << 21) + c, v);
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < Patch<T>::kPieces; ++j) {
-          constexpr int V = Patch<T>::V;
+        for (int j = 0; j < Patch<T, 16>::kPieces; ++j) {
+          constexpr int V = Patch<T, 16>::V;
           float o[V];
 #pragma unroll
           for (int i = 0; i < V; ++i) o[i] = v[j * V + i];
@@ -268,8 +310,8 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
           store_shared(patch.at(lane, j), reinterpret_cast<const uint4&>(r));
         }
         __syncwarp();
-        patch.store(static_cast<T*>(p.dx) + row0 * p.k + c * 32, p.k, rows,
-                    min(p.k - c * 32, 32), p.dx_vector, false);
+        patch.store(static_cast<T*>(p.dx) + row0 * p.k + c, p.k, rows, min(p.k - c, 16),
+                    p.dx_vector, false);
       }
     }
     // the tile's operands are free once its last products are done
@@ -279,18 +321,18 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
       if (p.partial && lane_block * 32 < p.n) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int c = half + 2 * i;
-          if (c * 32 < p.k32) {
-            float v[32];
-            tc::tmem_load32(acc_w + (lane_block << 21) + c * 32, v);
+          const int c = group * 16 + 64 * i;
+          if (c < p.k) {
+            float v[16];
+            tc::tmem_load16(acc_w + (lane_block << 21) + c, v);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) sum_w[i][j] += v[j];
-            tc::tmem_load32(acc_w + (lane_block << 21) + p.k32 + c * 32, v);
+            for (int j = 0; j < 16; ++j) sum_w[i][j] += v[j];
+            tc::tmem_load16(acc_w + (lane_block << 21) + p.k32 + c, v);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) sum_w[i][j] += v[j];
+            for (int j = 0; j < 16; ++j) sum_w[i][j] += v[j];
           }
         }
-        if (half == 0)
+        if (group == 0)
           sum_b += tc::tmem_load1(acc_b + (lane_block << 21)) +
                    tc::tmem_load1(acc_b + (lane_block << 21) + 32);
       }
@@ -304,29 +346,35 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
     if (lane_block * 32 < p.n) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int c = half + 2 * i;
-        if (c * 32 < p.k32) {
-          float v[32];
+        const int c = group * 16 + 64 * i;
+        if (c < p.k) {
+          float v[16];
           if constexpr (kAcc == 2) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = sum_w[i][j];
+            for (int j = 0; j < 16; ++j) v[j] = sum_w[i][j];
           } else {
-            tc::tmem_load32(acc_w + (lane_block << 21) + c * 32, v);
+            tc::tmem_load16(acc_w + (lane_block << 21) + c, v);
           }
           if (row < p.n) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (c * 32 + j < p.k) out[row * p.k + c * 32 + j] = v[j];
+            for (int j = 0; j < 16; ++j)
+              if (c + j < p.k) out[row * p.k + c + j] = v[j];
           }
         }
       }
-      if (half == 0) {
+      if (group == 0) {
         if constexpr (kAcc == 1) sum_b = tc::tmem_load1(acc_b + (lane_block << 21));
         if (row < p.n) out[p.n * p.k + row] = sum_b;
       }
     }
   }
-  if (threadIdx.x == 0) {  // also after a wait that ran out
+  if (threadIdx.x == 0) {  // nothing is in flight past this, also after a wait that ran out
+    if (p.raw && !ok) {
+      tc::barrier_wait(tc::shared_address(&x_raw), parity);
+      tc::barrier_wait(tc::shared_address(&dy_raw), parity);
+      tc::barrier_wait(tc::shared_address(&x_raw), parity ^ 1);
+      tc::barrier_wait(tc::shared_address(&dy_raw), parity ^ 1);
+    }
     tc::commit(tc::shared_address(&drained));
     ok = tc::barrier_wait(tc::shared_address(&drained), 0) && ok;
   }

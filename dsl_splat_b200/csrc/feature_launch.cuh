@@ -47,7 +47,10 @@ constexpr int kMaxResidentBytes = 128 * 1024;
 // Fills in the tiling of p (its sources, sizes and epilogue set) and launches.
 template <class SA, int PA, bool AMN, class SB, int PB, bool BMN, class TE, class TO, int EPI>
 int launch_product(ProductParams p, cudaStream_t s) {
-  const int widest = PA == 1 && PB == 1 ? 256 : 128;
+  // a plain product's tiles are as wide as they can be; one with arithmetic
+  // behind it is faster with two blocks' epilogues on an SM (512 -> 512 fp16
+  // gelu over 131072 rows: see the sizes in the measurements)
+  const int widest = PA == 1 && PB == 1 && EPI == kPlain ? 256 : 128;
   p.tiles_n = (p.n + widest - 1) / widest;
   p.tile_n = ((p.n + p.tiles_n - 1) / p.tiles_n + 31) / 32 * 32;
   const long long tiles_m = (p.m + kTileRows - 1) / kTileRows;
@@ -72,13 +75,13 @@ int launch_product(ProductParams p, cudaStream_t s) {
   const long long chunks = (p.k + kChunk - 1) / kChunk;
   const long long whole_b = chunks * b_bytes;
   p.resident = p.splits == 1 && p.tiles_n == 1 && whole_b <= kMaxResidentBytes;
-  const int fixed = kEpilogueWarps * staging_bytes<TE, TO, EPI>() + (p.bias_shared * 4 + 1023) / 1024 * 1024 + (p.resident ? static_cast<int>(whole_b) : 0);
+  // a patch of results, and one of the extra values
+  p.staging = 1024 * static_cast<int>(sizeof(TO) + (p.extra ? sizeof(TE) : 0));
+  const int fixed = kEpilogueWarps * p.staging + (p.bias_shared * 4 + 1023) / 1024 * 1024 + (p.resident ? static_cast<int>(whole_b) : 0);
   const int stage = a_bytes + (p.resident ? 0 : b_bytes);
   int blocks = 2, budget = kTwoBlocksBytes;
   if (producers(PA, PB) > 128 || p.tmem_columns > 256 || fixed + 2 * stage > budget)
     blocks = 1, budget = kOneBlockBytes;
-  p.stages = std::min(kMaxStages, (budget - fixed) / stage);
-  if (p.stages < 1) return host::fail(kTooLarge, "feature_linear: no room for a stage");
   if constexpr (PA == 1 && PB == 1) {
     p.copy_operands =
         make_map<SA>(p.a_map, p.a, AMN ? p.k : p.m, AMN ? p.m : p.k, p.a_ld, kChunk,
@@ -86,13 +89,21 @@ int launch_product(ProductParams p, cudaStream_t s) {
         make_map<SB>(p.b_map, p.b, BMN ? p.k : p.n, BMN ? p.n : p.k, p.b_ld, kChunk,
                      BMN ? kChunk : p.tile_n);
   }
+  // two tiles of A as they are in memory, where two stages fit beside them
+  if (!p.copy_operands && !AMN && p.tiles_n == 1 && p.a_ld == p.k && host::aligned(p.a, 16)) {
+    const long long raw = (kTileRows * p.k * static_cast<long long>(sizeof(SA)) + 127) / 128 * 128;
+    if (fixed + 2 * stage + 2 * raw > budget && blocks == 2) blocks = 1, budget = kOneBlockBytes;
+    if (fixed + 2 * stage + 2 * raw <= budget) p.raw_bytes = static_cast<int>(raw);
+  }
+  p.stages = std::min(kMaxStages, (budget - fixed - 2 * p.raw_bytes) / stage);
+  if (p.stages < 1) return host::fail(kTooLarge, "feature_linear: no room for a stage");
   if (EPI != kPlain) p.copy_extra = make_map<TE>(p.extra_map, p.extra, p.m, p.n, p.n, 32, 32);
   // partial sums are added to or lie one split behind the other
   if (p.splits == 1 && p.k_per_sum >= p.k)
     p.copy_out = make_map<TO>(p.out_map, p.out, p.m, p.n, p.n, 32, 32);
   p.error = host::device_error_word();
   if (!p.error) return kCudaError;
-  const int bytes = fixed + p.stages * stage + 1024;
+  const int bytes = fixed + p.stages * stage + 2 * p.raw_bytes + 1024;
   auto* kernel = product_kernel<SA, PA, AMN, SB, PB, BMN, TE, TO, EPI>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
       cudaSuccess)

@@ -135,6 +135,7 @@ int launch_gradients(long long rows, int k, int n, const T* dz, const void* x,
 struct FusedPlan {
   int blocks;
   bool copies;  // by tensor copies
+  bool raw;     // or by bulk copies
   size_t bytes;
   uint32_t tmem_columns;
 };
@@ -159,9 +160,12 @@ FusedPlan plan_fused(long long rows, int k, int n) {
     while (plan.tmem_columns < static_cast<uint32_t>(n32 + 2 * k32)) plan.tmem_columns *= 2;
     if (k <= 64 && n <= 64) per_sm = 2;
   } else {
-    plan.bytes = F::shared_bytes(k, n, n32);
+    plan.bytes = F::shared_bytes(k, n, n32, false);
     if (plan.tmem_columns > 512 || plan.bytes > kOneBlockBytes) return plan;
     if (sizeof(T) == 2 && plan.tmem_columns <= 256 && plan.bytes <= kTwoBlocksBytes) per_sm = 2;
+    const size_t raw = F::shared_bytes(k, n, n32, true);
+    plan.raw = raw <= static_cast<size_t>(per_sm == 2 ? kTwoBlocksBytes : kOneBlockBytes);
+    if (plan.raw) plan.bytes = raw;
   }
   plan.blocks = static_cast<int>(std::min<long long>(
       (rows + kTileRows - 1) / kTileRows, static_cast<long long>(host::sm_count()) * per_sm));
@@ -212,6 +216,10 @@ int launch_fused(const FusedPlan& plan, long long rows, int k, int n, const void
     p.x = x, p.weight = weight, p.bias = bias, p.dy = dy, p.dx = dx;
     p.partial = partial;
     p.activation = activation;
+    p.raw = plan.raw;
+    if (p.raw && !(host::aligned(x, 16) && host::aligned(dy, 16)))
+      return host::fail(kInvalidArgument,
+                        "feature_linear_backward: x and dy must be 16-byte aligned");
     p.x_vector = row_vector<T>(x, k);
     p.w_vector = row_vector<T>(weight, k);
     p.dy_vector = n * sizeof(T) % 16 == 0 && host::aligned(dy, 16);

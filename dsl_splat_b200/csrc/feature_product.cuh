@@ -11,12 +11,15 @@
 // global memory into a ring of stages: 16-bit operands with 16-byte rows by
 // tensor copies that one thread starts, all others through four or eight
 // producer warps (converting and zero-filling on the way: any row length, any
-// row count).  One thread issues
+// row count).  These take the tiles of a short-rowed A, which are contiguous,
+// from bulk copies that run two tiles ahead.  One thread issues
 // the products, and eight epilogue warps take the finished accumulator, of which
 // there are two, so that loads, products and epilogues of neighbouring tiles
 // overlap.  Where the whole of B fits beside the ring it is loaded once per
 // block.
 #pragma once
+#include <type_traits>
+
 #include "feature_common.cuh"
 #include "tensor_core.cuh"
 
@@ -27,12 +30,6 @@ constexpr int kTileRows = 128;
 constexpr int kChunk = 64;             // k of a stage: 128 bytes of 16-bit values
 constexpr int kEpilogueWarps = 8;                  // epilogue warps
 constexpr int kMaxStages = 8;
-// Staging memory of an epilogue warp: a patch of the extra values and one of
-// the results.
-template <class TE, class TO, int EPI>
-__host__ __device__ constexpr int staging_bytes() {
-  return 1024 * ((EPI == 2 ? 0 : sizeof(TE)) + sizeof(TO));
-}
 constexpr int kAPlane = kTileRows * 128;
 
 // Producer threads: operands that are split always pass through registers, so
@@ -52,6 +49,8 @@ enum Epilogue : int { kForward = 0, kSlope = 1, kPlain = 2 };
 struct ProductParams {
   CUtensorMap a_map, b_map, extra_map, out_map;
   int copy_operands, copy_extra, copy_out;  // by tensor copies
+  int raw_bytes;   // of a tile of A as it is in memory, copied ahead; 0: none
+  int staging;     // bytes of an epilogue warp
   long long m, k;  // k of all splits
   int n;
   // row-major sources: A is (m, k) rows or, transposed, (k, m); B likewise
@@ -72,6 +71,20 @@ struct ProductParams {
   int bias_shared;    // values of the bias kept in shared memory (0: too many)
   int* error;
 };
+
+SPLAT_DEV void store_shared(uint32_t address, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(address), "r"(v.x), "r"(v.y),
+               "r"(v.z), "r"(v.w)
+               : "memory");
+}
+SPLAT_DEV float4 load_shared(uint32_t address) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(address)
+               : "memory");
+  return v;
+}
 
 // ---- global memory -> operand planes -----------------------------------------
 
@@ -134,45 +147,68 @@ SPLAT_DEV void to_parts(const Vec<S, 8>& v, uint4 (&out)[P]) {
   }
 }
 
-SPLAT_DEV void store_shared(uint32_t address, uint4 v) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(address), "r"(v.x), "r"(v.y),
-               "r"(v.z), "r"(v.w)
-               : "memory");
-}
-SPLAT_DEV float4 load_shared(uint32_t address) {
-  float4 v;
-  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(address)
-               : "memory");
-  return v;
+// The same from shared memory.
+template <class S, int VB>
+SPLAT_DEV Vec<S, 8> load8_shared(uint32_t p, int valid) {
+  Vec<S, 8> r;
+  constexpr int E = VB / static_cast<int>(sizeof(S));  // values per load
+#pragma unroll
+  for (int j = 0; j < 8 / E; ++j) {
+    Vec<S, E> part;
+    if (j * E < valid) {
+      if constexpr (VB == 16) {
+        const float4 u = load_shared(p + j * 16);
+        part = reinterpret_cast<const Vec<S, E>&>(u);
+      } else if constexpr (VB == 8) {
+        float2 u;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                     : "=f"(u.x), "=f"(u.y)
+                     : "r"(p + j * 8)
+                     : "memory");
+        part = reinterpret_cast<const Vec<S, E>&>(u);
+      } else if constexpr (VB == 4) {
+        float u;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(u) : "r"(p + j * 4) : "memory");
+        part = reinterpret_cast<const Vec<S, E>&>(u);
+      } else {
+        unsigned short u;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(p + j * 2) : "memory");
+        part = reinterpret_cast<const Vec<S, E>&>(u);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) part.v[e] = from_float<S>(0.0f);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) r.v[j * E + e] = part.v[e];
+  }
+  return r;
 }
 
 // Fills `rows` rows of a block (and of its parts' planes, `plane` bytes apart)
-// with `pieces` 16-byte pieces each from src (already at the block's corner):
-// rows from rows_valid and columns from cols_valid on are zero.
-template <class S, int P, int VB>
-SPLAT_DEV void fill_block(uint32_t dst, uint32_t plane, int rows, int pieces, const S* src,
-                          long long ld, long long rows_valid, long long cols_valid, int thread,
-                          int threads) {
-  constexpr int U = P == 1 && VB == 16 ? 8 : 4;  // pieces in flight per thread
-  const int shift = pieces <= 1 ? 0 : pieces <= 2 ? 1 : pieces <= 4 ? 2 : 3;
-  const int total = rows << shift;
+// with `pieces` (2, 4, 6 or 8) 16-byte pieces each; load(row, piece, valid)
+// gives a piece's values.  Rows from rows_valid and columns from cols_valid on
+// are zero.
+template <class S, int P, int U, class L>
+SPLAT_DEV void fill_pieces(uint32_t dst, uint32_t plane, int rows, int pieces,
+                           long long rows_valid, long long cols_valid, int thread, int threads,
+                           L load) {
+  // i / pieces as a product and a shift, exact for i < 2^15
+  const int factor = pieces == 6 ? 10923 : 65536 / pieces;
+  const int total = rows * pieces;
   for (int i0 = thread; i0 < total; i0 += U * threads) {
     Vec<S, 8> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * threads, row = i >> shift, piece = i & ((1 << shift) - 1);
-      const long long left = cols_valid - piece * 8;
-      const int valid = i < total && row < rows_valid && piece < pieces && left > 0
-                            ? static_cast<int>(left < 8 ? left : 8)
-                            : 0;
-      v[u] = load8<S, VB>(src + row * ld + piece * 8, valid);
+      const int i = i0 + u * threads, row = (i * factor) >> 16, piece = i - row * pieces;
+      const int left = static_cast<int>(min(cols_valid, 1LL << 20)) - piece * 8;
+      const int valid = i < total && row < rows_valid && left > 0 ? min(left, 8) : 0;
+      v[u] = load(row, piece, valid);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * threads, row = i >> shift, piece = i & ((1 << shift) - 1);
-      if (i < total && piece < pieces) {
+      const int i = i0 + u * threads, row = (i * factor) >> 16, piece = i - row * pieces;
+      if (i < total) {
         uint4 parts[P];
         to_parts<S, P>(v[u], parts);
         const uint32_t at = dst + row * 128 + ((piece ^ (row & 7)) << 4);
@@ -187,18 +223,62 @@ template <class S, int P>
 SPLAT_DEV void fill(int vector, uint32_t dst, uint32_t plane, int rows, int pieces, const S* src,
                     long long ld, long long rows_valid, long long cols_valid, int thread,
                     int threads) {
-  if (vector >= 16)
-    fill_block<S, P, 16>(dst, plane, rows, pieces, src, ld, rows_valid, cols_valid, thread,
-                         threads);
-  else if (vector >= 8)
-    fill_block<S, P, 8>(dst, plane, rows, pieces, src, ld, rows_valid, cols_valid, thread,
-                        threads);
-  else if (vector >= 4 || sizeof(S) == 4)
-    fill_block<S, P, 4>(dst, plane, rows, pieces, src, ld, rows_valid, cols_valid, thread,
-                        threads);
-  else
-    fill_block<S, P, sizeof(S)>(dst, plane, rows, pieces, src, ld, rows_valid, cols_valid, thread,
-                                threads);
+  const auto run = [&](auto bytes) {
+    constexpr int VB = decltype(bytes)::value;
+    // pieces in flight per thread
+    fill_pieces<S, P, P == 1 && VB == 16 ? 8 : 4>(
+        dst, plane, rows, pieces, rows_valid, cols_valid, thread, threads,
+        [&](int row, int piece, int valid) {
+          return load8<S, VB>(src + row * ld + piece * 8, valid);
+        });
+  };
+  if (vector >= 16) run(std::integral_constant<int, 16>{});
+  else if (vector >= 8) run(std::integral_constant<int, 8>{});
+  else if (vector >= 4 || sizeof(S) == 4) run(std::integral_constant<int, 4>{});
+  else run(std::integral_constant<int, static_cast<int>(sizeof(S))>{});
+}
+
+// From rows of row_bytes in shared memory.
+template <class S, int P>
+SPLAT_DEV void fill_shared(int vector, uint32_t dst, uint32_t plane, int rows, int pieces,
+                           uint32_t src, int row_bytes, int rows_valid, int cols_valid,
+                           int thread, int threads) {
+  const auto run = [&](auto bytes) {
+    constexpr int VB = decltype(bytes)::value;
+    fill_pieces<S, P, 2>(dst, plane, rows, pieces, rows_valid, cols_valid, thread, threads,
+                         [&](int row, int piece, int valid) {
+                           return load8_shared<S, VB>(
+                               src + row * row_bytes + piece * 8 * static_cast<int>(sizeof(S)),
+                               valid);
+                         });
+  };
+  if (vector >= 16) run(std::integral_constant<int, 16>{});
+  else if (vector >= 8) run(std::integral_constant<int, 8>{});
+  else if (vector >= 4 || sizeof(S) == 4) run(std::integral_constant<int, 4>{});
+  else run(std::integral_constant<int, static_cast<int>(sizeof(S))>{});
+}
+
+// A contiguous run of values (its start 16-byte aligned) into shared memory by
+// one bulk copy; the values behind its last whole 16 bytes are stored by the
+// calling thread.  The barrier takes this thread's arrival.
+template <class S>
+SPLAT_DEV void copy_run(uint32_t dst, const S* src, int values, uint32_t bar) {
+  const int bytes = values * static_cast<int>(sizeof(S)), whole = bytes & ~15;
+  for (int i = whole / static_cast<int>(sizeof(S)); i < values; ++i) {
+    const uint32_t to = dst + i * static_cast<int>(sizeof(S));
+    if constexpr (sizeof(S) == 4)
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(to), "f"(src[i]) : "memory");
+    else
+      asm volatile("st.shared.u16 [%0], %1;" ::"r"(to),
+                   "h"(reinterpret_cast<const unsigned short&>(src[i]))
+                   : "memory");
+  }
+  if (whole) {
+    tc::barrier_expect(bar, whole);
+    tc::bulk_in(dst, src, whole, bar);
+  } else {
+    tc::barrier_arrive(bar);
+  }
 }
 
 // One operand's chunk: `width` m or n from mn0 and kChunk k from k0 (k_valid of
@@ -241,17 +321,53 @@ SPLAT_DEV void copy_chunk(const CUtensorMap* map, uint32_t dst, int width, long 
 
 // ---- epilogue ------------------------------------------------------------------
 
-// A 32 x 32 patch of values of T in a warp's staging memory: 16-byte pieces,
-// permuted so that both a lane's own row and 16 bytes per lane along rows are
-// accessed without bank conflicts.
-template <class T>
+// A patch of 32 rows x W values of T in a warp's staging memory: 16-byte
+// pieces, permuted so that both a lane's own row and 16 bytes per lane along
+// rows are accessed without bank conflicts.
+template <class T, int W = 32>
 struct Patch {
-  static constexpr int kPieces = 2 * sizeof(T);  // of a row
-  static constexpr int V = 16 / sizeof(T);       // values of a piece
+  static constexpr int kPieces = W * sizeof(T) / 16;  // of a row
+  static constexpr int V = 16 / sizeof(T);            // values of a piece
   uint32_t base;
   SPLAT_DEV uint32_t at(int row, int piece) const {
-    const int turn = kPieces == 4 ? (row >> 1) & 3 : row & 7;
-    return base + row * (32 * sizeof(T)) + ((piece ^ turn) << 4);
+    const int turn = kPieces == 2 ? (row >> 2) & 1 : kPieces == 4 ? (row >> 1) & 3 : row & 7;
+    return base + row * (W * sizeof(T)) + ((piece ^ turn) << 4);
+  }
+
+  // Rows of ld values in shared memory -> staging.
+  SPLAT_DEV void load_shared_rows(uint32_t src, int ld, int rows, int cols, bool vector) const {
+    const int lane = threadIdx.x & 31;
+    constexpr int kSize = sizeof(T);
+    if (vector) {
+      constexpr int kRows = 32 / kPieces;
+      const int piece = lane % kPieces, r0 = lane / kPieces;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int r = i * kRows + r0;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (r < rows && piece * V < cols) v = load_shared(src + (r * ld + piece * V) * kSize);
+        store_shared(at(r, piece), reinterpret_cast<const uint4&>(v));
+      }
+    } else {
+      constexpr int kRows = 32 / W;
+      const int col = lane % W;
+#pragma unroll 8
+      for (int i = 0; i < W; ++i) {
+        const int r = i * kRows + lane / W;
+        const uint32_t from = src + (r * ld + col) * kSize;
+        const uint32_t to = at(r, col / V) + col % V * kSize;
+        const bool in = r < rows && col < cols;
+        if constexpr (kSize == 4) {
+          float v = 0.0f;
+          if (in) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(from) : "memory");
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
+        } else {
+          unsigned short v = 0;
+          if (in) asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
+          asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(v) : "memory");
+        }
+      }
+    }
   }
 
   // Global memory (its corner, rows of ld values) -> staging.  vector: rows
@@ -272,10 +388,14 @@ struct Patch {
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) store_shared(at(i * kRows + r0, piece), v[i]);
     } else {
-#pragma unroll 4
-      for (int r = 0; r < rows; ++r) {
-        const T v = lane < cols ? src[r * ld + lane] : from_float<T>(0.0f);
-        const uint32_t to = at(r, lane / V) + lane % V * sizeof(T);
+      constexpr int kRows = 32 / W;
+      const int col = lane % W;
+      src += lane / W * ld + col;
+#pragma unroll 8
+      for (int i = 0; i < W; ++i) {
+        const int r = i * kRows + lane / W;
+        const T v = r < rows && col < cols ? src[i * kRows * ld] : from_float<T>(0.0f);
+        const uint32_t to = at(r, col / V) + col % V * sizeof(T);
         if constexpr (sizeof(T) == 4)
           asm volatile("st.shared.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
         else
@@ -306,11 +426,14 @@ struct Patch {
         }
         *reinterpret_cast<float4*>(dst) = v;
       }
-    } else if (lane < cols) {
-      dst += lane;
+    } else {
+      constexpr int kRows = 32 / W;
+      const int col = lane % W;
+      if (col >= cols) return;
+      dst += lane / W * ld + col;
 #pragma unroll 4
-      for (int r = 0; r < rows; ++r, dst += ld) {
-        const uint32_t from = at(r, lane / V) + lane % V * sizeof(T);
+      for (int r = lane / W; r < rows; r += kRows, dst += kRows * ld) {
+        const uint32_t from = at(r, col / V) + col % V * sizeof(T);
         if constexpr (sizeof(T) == 4) {
           float v;
           asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(from) : "memory");
@@ -327,12 +450,12 @@ struct Patch {
 
 // The epilogue's arithmetic on a lane's row: v becomes act(v) + e, or
 // e act'(v); the extra values e lie in the patch.
-template <int EPI, int ACT, class TE>
-SPLAT_DEV void finish_row(const Patch<TE>& extra, bool with_extra, float (&v)[32]) {
+template <int EPI, int ACT, class TE, int W>
+SPLAT_DEV void finish_row(const Patch<TE, W>& extra, bool with_extra, float (&v)[W]) {
   const int lane = threadIdx.x & 31;
-  constexpr int V = Patch<TE>::V;
+  constexpr int V = Patch<TE, W>::V;
 #pragma unroll
-  for (int piece = 0; piece < Patch<TE>::kPieces; ++piece) {
+  for (int piece = 0; piece < Patch<TE, W>::kPieces; ++piece) {
     float* z = v + piece * V;
     if constexpr (EPI == kForward) {
 #pragma unroll
@@ -392,13 +515,13 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
   constexpr int kProducers = producers(PA, PB), kAcc = accumulators(PA, PB);
   extern __shared__ unsigned char dynamic[];
   __shared__ alignas(8) unsigned long long full[kMaxStages], empty[kMaxStages], acc_full[2],
-      acc_empty[2], resident_full, drained, extra_full[kEpilogueWarps];
+      acc_empty[2], resident_full, drained, extra_full[kEpilogueWarps], raw_full[2],
+      raw_read[2];
   __shared__ uint32_t tmem_base;
   const uint32_t base = (tc::shared_address(dynamic) + 1023u) & ~1023u;
   const uint32_t b_plane = b_plane_bytes<BMN>(p.tile_n);
   const uint32_t a_bytes = PA * kAPlane, b_bytes = PB * b_plane;
-  constexpr int kStaging = staging_bytes<TE, TO, EPI>();
-  const uint32_t bias_at = base + kEpilogueWarps * kStaging;
+  const uint32_t bias_at = base + kEpilogueWarps * p.staging;
   const uint32_t resident = bias_at + (p.bias_shared * 4 + 1023) / 1024 * 1024;
   const int chunks_all = static_cast<int>((p.k + kChunk - 1) / kChunk);
   const uint32_t ring = resident + (p.resident ? chunks_all * b_bytes : 0);
@@ -414,6 +537,8 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
       tc::barrier_init(tc::shared_address(&empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
+      tc::barrier_init(tc::shared_address(&raw_full[i]), 1);
+      tc::barrier_init(tc::shared_address(&raw_read[i]), kProducers);
       tc::barrier_init(tc::shared_address(&acc_full[i]), 1);
       tc::barrier_init(tc::shared_address(&acc_empty[i]), kEpilogueWarps * 32);
     }
@@ -483,14 +608,41 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
         tc::fence_async_proxy();
         tc::barrier_arrive(tc::shared_address(&resident_full));
       }
-      for (uint32_t t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+      // the tiles of A by bulk copies, two ahead
+      const uint32_t raw_at = ring + p.stages * stage_bytes;
+      const int row_bytes = static_cast<int>(p.k) * static_cast<int>(sizeof(SA));
+      const auto copy_tile = [&](uint32_t t, uint32_t buffer) {
+        const long long m0 = ProductTile(p, t).m0;
+        copy_run<SA>(raw_at + buffer * p.raw_bytes, a + m0 * p.k,
+                     static_cast<int>(min(p.m - m0, static_cast<long long>(kTileRows)) * p.k),
+                     tc::shared_address(&raw_full[buffer]));
+      };
+      uint32_t started = 0;  // copies, by thread 0
+      if (!AMN && p.raw_bytes && thread == 0)
+        for (; started < 2 && blockIdx.x + started * gridDim.x < p.tiles; ++started)
+          copy_tile(blockIdx.x + started * gridDim.x, started);
+      uint32_t i = 0;
+      for (uint32_t t = blockIdx.x; t < p.tiles && ok; t += gridDim.x, ++i) {
         const ProductTile tile(p, t);
+        const uint32_t buffer = i & 1;
+        if (!AMN && p.raw_bytes &&
+            !(ok = tc::barrier_wait(tc::shared_address(&raw_full[buffer]), (i >> 1) & 1)))
+          break;
         for (long long k = tile.k0; k < tile.k1; k += kChunk) {
           if (!(ok = tc::barrier_wait(tc::shared_address(&empty[stage]), parity))) break;
           const uint32_t at = ring + stage * stage_bytes;
           const int k_valid = static_cast<int>(min(tile.k1 - k, static_cast<long long>(kChunk)));
-          fill_chunk<SA, PA, AMN>(p.a_vector, at, kAPlane, kTileRows, a, p.a_ld, tile.m0,
-                                  p.m - tile.m0, k, k_valid, thread, kProducers);
+          if (!AMN && p.raw_bytes)
+            fill_shared<SA, PA>(p.a_vector, at, kAPlane, kTileRows,
+                                min((k_valid + 15) / 16 * 2, 8),
+                                raw_at + buffer * p.raw_bytes +
+                                    static_cast<int>(k) * static_cast<int>(sizeof(SA)),
+                                row_bytes,
+                                static_cast<int>(min(p.m - tile.m0, static_cast<long long>(kTileRows))),
+                                k_valid, thread, kProducers);
+          else
+            fill_chunk<SA, PA, AMN>(p.a_vector, at, kAPlane, kTileRows, a, p.a_ld, tile.m0,
+                                    p.m - tile.m0, k, k_valid, thread, kProducers);
           if (!p.resident)
             fill_chunk<SB, PB, BMN>(p.b_vector, at + a_bytes, b_plane, p.tile_n, b, p.b_ld,
                                     tile.n0, p.n - tile.n0, k, k_valid, thread, kProducers);
@@ -498,7 +650,19 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
           tc::barrier_arrive(tc::shared_address(&full[stage]));
           if (++stage == p.stages) stage = 0, parity ^= 1;
         }
+        if (!AMN && p.raw_bytes && ok) {
+          const uint32_t read = tc::shared_address(&raw_read[buffer]);
+          tc::barrier_arrive(read);
+          if (thread == 0 && p.tiles - t > 2ull * gridDim.x) {
+            if (!(ok = tc::barrier_wait(read, (i >> 1) & 1))) break;
+            copy_tile(t + 2 * gridDim.x, buffer);
+            ++started;
+          }
+        }
       }
+      // no copy is in flight past this point, also after a wait that ran out
+      for (uint32_t j = started < 2 ? 0 : started - 2; j < started; ++j)
+        ok = tc::barrier_wait(tc::shared_address(&raw_full[j & 1]), (j >> 1) & 1) && ok;
     }
   } else if (warp == kEpilogueWarps + kProducers / 32) {
     // ---- one thread issues the products
@@ -564,8 +728,8 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
     // ---- epilogue
     const int lane_block = warp & 3, half = warp >> 2;
     constexpr bool kExtra = EPI != kPlain;
-    const Patch<TE> extra_patch{base + warp * kStaging + 1024 * static_cast<int>(sizeof(TO))};
-    const Patch<TO> out_patch{base + warp * kStaging};
+    const Patch<TE> extra_patch{base + warp * p.staging + 1024 * static_cast<int>(sizeof(TO))};
+    const Patch<TO> out_patch{base + warp * p.staging};
     const bool leader = (threadIdx.x & 31) == 0;
     const uint32_t extra_bar = tc::shared_address(&extra_full[warp]);
     uint32_t acc = 0, parity = 0, extra_parity = 0;
