@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
   const uint32_t w_at = z_at + P * z_plane;
   const uint32_t ones_at = w_at + P * w_plane;
   const uint32_t bias_at = ones_at + kOnesBytes;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = tc::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   // a warp's patches: 16 columns from 16 group on, and from 64 + 16 group on
   const int lane_block = warp & 3, group = warp >> 2;
   const Patch<T, 16> patch{base + warp * static_cast<uint32_t>(512 * sizeof(T))};
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = tmem_base;
+  const uint32_t tmem = tc::uniform(tmem_base);
   const uint32_t acc_w = tmem + max(p.k32, p.n32), acc_b = acc_w + kAcc * p.k32;
 
   float sum_w[kAcc == 2 ? 2 : 1][16] = {};  // fp32: this thread's part of dW
@@ -151,9 +151,10 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
     tc::fence_before_sync();
     // x is there, and the previous tile's accumulators have been read
     if (__syncthreads_or(!ok)) break;
-    if (threadIdx.x == 0 && p.raw && next)
+    if (threadIdx.x == 32 && p.raw && next)
       copy_rows(p.x, p.k, t + gridDim.x, x_raw_at, x_raw);
-    if (threadIdx.x == 0 && with_z) {
+    if (warp == 0 && with_z) {
+      const uint32_t lead = tc::elected();
       tc::fence_after_sync();
       const uint32_t instruction = tc::instruction(!kIsF16<T>, false, false, p.n32);
       bool first = true;
@@ -161,15 +162,14 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
       for (int sum = P - 1; sum >= 0; --sum)
 #pragma unroll
         for (int i = 0; i <= sum; ++i)
-          for (int s = 0; s * 16 < p.k; ++s) {
-            const uint32_t o = (s & 3) * tc::kStepK;
-            tc::mma(tmem,
-                    tc::descriptor_k_major(x_at + i * x_plane + (s >> 2) * kAPlane + o),
-                    tc::descriptor_k_major(w_at + (sum - i) * w_plane + (s >> 2) * p.n32 * 128 + o),
-                    instruction, !first);
+          for (int c = 0; c * 64 < p.k; ++c) {
+            tc::mma_steps(lead, tmem, tc::descriptor_k_major(x_at + i * x_plane + c * kAPlane),
+                          tc::descriptor_k_major(w_at + (sum - i) * w_plane + c * p.n32 * 128),
+                          tc::kStepK, tc::kStepK, min((p.k - c * 64 + 15) / 16, 4), instruction,
+                          !first);
             first = false;
           }
-      tc::commit(tc::shared_address(&z_done));
+      tc::commit(lead, tc::shared_address(&z_done));
     }
     // dz: a lane's row of each patch
     bool waited = !with_z;
@@ -236,8 +236,10 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
     tc::fence_async_proxy();
     tc::fence_before_sync();
     __syncthreads();  // dz is there, z has been read
-    if (threadIdx.x == 0) {
-      if (p.raw && next) copy_rows(p.dy, p.n, t + gridDim.x, dy_raw_at, dy_raw);
+    if (threadIdx.x == 32 && p.raw && next)
+      copy_rows(p.dy, p.n, t + gridDim.x, dy_raw_at, dy_raw);
+    if (warp == 0) {
+      const uint32_t lead = tc::elected();
       tc::fence_after_sync();
       if (p.dx) {
         const uint32_t instruction = tc::instruction(!kIsF16<T>, false, true, p.k32);
@@ -248,17 +250,17 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
           for (int i = 0; i < P; ++i) {
             const int j = sum - i;
             if (j < 0 || j >= P) continue;
-            for (int s = 0; s * 16 < p.n; ++s) {
-              tc::mma(tmem,
-                      tc::descriptor_k_major(z_at + i * z_plane + (s >> 2) * kAPlane +
-                                             (s & 3) * tc::kStepK),
-                      tc::descriptor_mn_major(w_at + j * w_plane + s * tc::kStepMn, p.n32 * 128),
-                      instruction, !first);
+            for (int c = 0; c * 64 < p.n; ++c) {
+              tc::mma_steps(lead, tmem, tc::descriptor_k_major(z_at + i * z_plane + c * kAPlane),
+                            tc::descriptor_mn_major(w_at + j * w_plane + c * 4 * tc::kStepMn,
+                                                    p.n32 * 128),
+                            tc::kStepK, tc::kStepMn, min((p.n - c * 64 + 15) / 16, 4),
+                            instruction, !first);
               first = false;
             }
           }
       }
-      tc::commit(tc::shared_address(&dx_done));
+      tc::commit(lead, tc::shared_address(&dx_done));
       if (p.partial) {
         // n of up to 64 take one block of dz twice; the upper lanes are not read
         const uint32_t z_block = p.n > 64 ? kAPlane : 0;
@@ -273,24 +275,24 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
             if (j < 0 || j >= P) continue;
             const bool own = sum == 0 && kAcc == 2;
             const bool first = start && (own || (sum == P - 1 && i == 0));
-            for (int s = 0; s < kTileRows / 16; ++s)
-              tc::mma(acc_w + (own ? 0 : (kAcc - 1) * p.k32),
-                      tc::descriptor_mn_major(z_at + i * z_plane + s * tc::kStepMn, z_block),
-                      tc::descriptor_mn_major(x_at + j * x_plane + s * tc::kStepMn, kAPlane),
-                      wide, !(first && s == 0));
+            tc::mma_steps(lead, acc_w + (own ? 0 : (kAcc - 1) * p.k32),
+                          tc::descriptor_mn_major(z_at + i * z_plane, z_block),
+                          tc::descriptor_mn_major(x_at + j * x_plane, kAPlane), tc::kStepMn,
+                          tc::kStepMn, kTileRows / 16, wide, !first);
           }
 #pragma unroll
         for (int i = P - 1; i >= 0; --i) {
           const bool own = i == 0 && kAcc == 2;
           const bool first = start && (own || i == P - 1);
-          for (int s = 0; s < kTileRows / 16; ++s)
-            tc::mma(acc_b + (own ? 0 : (kAcc - 1) * 32),
-                    tc::descriptor_mn_major(z_at + i * z_plane + s * tc::kStepMn, z_block),
-                    tc::descriptor_k_major(ones_at + (s & 3) * tc::kStepK), narrow,
-                    !(first && s == 0));
+          for (int h = 0; h < 2; ++h)
+            tc::mma_steps(lead, acc_b + (own ? 0 : (kAcc - 1) * 32),
+                          tc::descriptor_mn_major(z_at + i * z_plane + h * 4 * tc::kStepMn,
+                                                  z_block),
+                          tc::descriptor_k_major(ones_at), tc::kStepMn, tc::kStepK, 4, narrow,
+                          !(first && h == 0));
         }
       }
-      tc::commit(tc::shared_address(&dw_done));
+      tc::commit(lead, tc::shared_address(&dw_done));
     }
     fresh = false;
     if (p.dx) {
@@ -375,7 +377,9 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
       tc::barrier_wait(tc::shared_address(&x_raw), parity ^ 1);
       tc::barrier_wait(tc::shared_address(&dy_raw), parity ^ 1);
     }
-    tc::commit(tc::shared_address(&drained));
+  }
+  if (warp == 0) {
+    tc::commit(tc::elected(), tc::shared_address(&drained));
     ok = tc::barrier_wait(tc::shared_address(&drained), 0) && ok;
   }
   if (!ok) atomicCAS(p.error, 0, kDeviceTimeout);

@@ -48,25 +48,64 @@ void join_splits(const float* partial, long long stride, int splits, long long c
           partial, stride, splits, count_a, count_b, static_cast<T*>(a), static_cast<T*>(b));
 }
 
-// Column sums of dz (m, n) over ranges of rows.
-template <class S>
+// Column sums of dz (m, n) over ranges of rows: a thread adds V neighbouring
+// columns (V is 1 where rows are not whole 16-byte pieces), the block's eight
+// rows of threads are joined in a fixed order.
+template <class S, int V>
 __global__ void __launch_bounds__(256) column_sums_kernel(const S* dz, long long m, int n,
                                                           long long rows, float* partial) {
-  const int c = blockIdx.x * 32 + threadIdx.x;
+  const int c = (blockIdx.x * 32 + threadIdx.x) * V;
   const long long begin = blockIdx.y * rows, end = min(begin + rows, m);
-  float s = 0.0f;
+  float s[V] = {};
   if (c < n) {
-#pragma unroll 8
-    for (long long r = begin + threadIdx.y; r < end; r += 8) s += to_float(dz[r * n + c]);
+    constexpr int U = 4;  // rows in flight
+    const S* from = dz + (begin + threadIdx.y) * n + c;
+    const long long stride = 8LL * n;
+    for (long long r = begin + threadIdx.y; r < end; r += 8 * U, from += U * stride) {
+      Vec<S, V> v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + 8 * u < end) v[u] = *reinterpret_cast<const Vec<S, V>*>(from + u * stride);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + 8 * u < end) {
+          float f[V];
+          widen<S, V>(v[u], f);
+#pragma unroll
+          for (int j = 0; j < V; ++j) s[j] += f[j];
+        }
+    }
   }
-  __shared__ float sums[8][32];
-  sums[threadIdx.y][threadIdx.x] = s;
+  __shared__ float sums[8][32 * V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) sums[threadIdx.y][threadIdx.x * V + j] = s[j];
   __syncthreads();
-  if (threadIdx.y == 0 && c < n) {
-    for (int i = 1; i < 8; ++i) s += sums[i][threadIdx.x];
-    partial[static_cast<long long>(blockIdx.y) * n + c] = s;
+  const int t = threadIdx.y * 32 + threadIdx.x, col = blockIdx.x * 32 * V + t;
+  if (t < 32 * V && col < n) {
+    float a = 0.0f;
+    for (int i = 0; i < 8; ++i) a += sums[i][t];
+    partial[static_cast<long long>(blockIdx.y) * n + col] = a;
   }
 }
+
+// Their ranges of rows: eight blocks to an SM, 256 rows to a range at least.
+template <class T>
+int sum_columns(const T* dz, long long rows, int n, float* partial, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const bool vector = n % V == 0 && host::aligned(dz, 16);
+  const int blocks = host::blocks_for(n, vector ? 32 * V : 32);
+  const long long wanted = std::max(1LL, 8LL * host::sm_count() / blocks);
+  const long long count = std::min({wanted, (rows + 255) / 256, 1024LL});
+  const long long per = (rows + count - 1) / count;
+  const int splits = static_cast<int>((rows + per - 1) / per);
+  const dim3 grid(blocks, splits), block(32, 8);
+  if (vector)
+    column_sums_kernel<T, V><<<grid, block, 0, host::counted(s)>>>(dz, rows, n, per, partial);
+  else
+    column_sums_kernel<T, 1><<<grid, block, 0, host::counted(s)>>>(dz, rows, n, per, partial);
+  return splits;
+}
+constexpr int kMaxColumnSplits = 1024;
 
 // Ranges of rows whose sums of dz^T x (and of dz) are joined afterwards:
 // enough tiles for two blocks on every SM, 512 rows to a range at least.
@@ -122,9 +161,8 @@ int launch_gradients(long long rows, int k, int n, const T* dz, const void* x,
   }
   if (dbias) {
     float* sums = partial + static_cast<long long>(splits.count) * n * k;
-    column_sums_kernel<T><<<dim3(host::blocks_for(n, 32), splits.count), dim3(32, 8), 0,
-                            host::counted(s)>>>(dz, rows, n, splits.rows, sums);
-    join_splits<T>(sums, n, splits.count, n, 0, dbias, nullptr, s);
+    const int count = sum_columns<T>(dz, rows, n, sums, s);
+    join_splits<T>(sums, n, count, n, 0, dbias, nullptr, s);
   }
   return host::check_launch("feature_linear_backward");
 }
@@ -255,7 +293,9 @@ size_t splat_feature_linear_backward_workspace_bytes(int dtype, long long rows, 
   const FusedPlan plan = SPLAT_FEATURE_TYPE(dtype, [&] { return plan_fused<T>(rows, k, n); });
   const size_t sums = static_cast<size_t>(n) * (static_cast<size_t>(k) + 1) * 4;
   if (plan.blocks) return plan.blocks * sums;
-  return dz_bytes(dtype, rows, n, activation) + weight_splits(rows, k, n).count * sums;
+  return dz_bytes(dtype, rows, n, activation) +
+         static_cast<size_t>(weight_splits(rows, k, n).count) * n * k * 4 +
+         static_cast<size_t>(kMaxColumnSplits) * n * 4;
 }
 
 int splat_feature_linear_backward(int dtype, long long rows, int k, int n, const void* x,

@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
   const uint32_t w_block = p.n32 * 128;
   const uint32_t patch_at = w_at + blocks64(p.k) * w_block;
   const uint32_t bias_at = patch_at + 8 * 2048, join_at = bias_at + kNarrowWidth * 4;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = tc::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const bool with_z = p.activation != kNone;
   const auto bar = [](const unsigned long long& b) { return tc::shared_address(&b); };
 
@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = tmem_base;
+  const uint32_t tmem = tc::uniform(tmem_base);
   const uint32_t z_tmem = tmem, dx_tmem = z_tmem + p.n32, w_tmem = dx_tmem + p.k32;
   const uint32_t count = (p.tiles - blockIdx.x + gridDim.x - 1) / gridDim.x;  // of this block
   bool ok = true;
@@ -108,7 +108,8 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
     }
   } else if (warp == 8) {
     // ---- products
-    if (lane == 0) {
+    {
+      const uint32_t lead = tc::elected();
       const uint32_t z_instruction = tc::instruction(!kIsF16<T>, false, false, p.n32);
       const uint32_t dx_instruction = tc::instruction(!kIsF16<T>, false, true, p.k32);
       const uint32_t w_instruction = tc::instruction(!kIsF16<T>, true, true, p.k32);
@@ -119,12 +120,11 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
         if (!(ok = tc::barrier_wait(bar(full[b]), (i >> 1) & 1) && ok)) return;
         tc::fence_after_sync();
         if (!with_z) return;
-        for (int s = 0; s * 16 < p.k; ++s) {
-          const uint32_t o = (s & 3) * tc::kStepK;
-          tc::mma(z_tmem, tc::descriptor_k_major(x_at + b * x_bytes + (s >> 2) * kAPlane + o),
-                  tc::descriptor_k_major(w_at + (s >> 2) * w_block + o), z_instruction, s > 0);
-        }
-        tc::commit(bar(z_done));
+        for (int c = 0; c * 64 < p.k; ++c)
+          tc::mma_steps(lead, z_tmem, tc::descriptor_k_major(x_at + b * x_bytes + c * kAPlane),
+                        tc::descriptor_k_major(w_at + c * w_block), tc::kStepK, tc::kStepK,
+                        min((p.k - c * 64 + 15) / 16, 4), z_instruction, c > 0);
+        tc::commit(lead, bar(z_done));
       };
       ok = tc::barrier_wait(bar(w_full), 0);
       if (ok) form_z(0);
@@ -135,25 +135,24 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
         if (i + 1 < count) form_z(i + 1);
         const uint32_t x_now = x_at + b * x_bytes, z_now = z_at + b * z_bytes;
         if (p.partial) {
-          for (int s = 0; s < kTileRows / 16; ++s)
-            tc::mma(w_tmem, tc::descriptor_mn_major(z_now + s * tc::kStepMn, z_block),
-                    tc::descriptor_mn_major(x_now + s * tc::kStepMn, kAPlane), w_instruction,
-                    i > 0 || s > 0);
+          tc::mma_steps(lead, w_tmem, tc::descriptor_mn_major(z_now, z_block),
+                        tc::descriptor_mn_major(x_now, kAPlane), tc::kStepMn, tc::kStepMn,
+                        kTileRows / 16, w_instruction, i > 0);
         }
         if (p.with_dx) {
           if (i > 0 && !(ok = tc::barrier_wait(bar(dx_read), (i - 1) & 1) && ok)) break;
           tc::fence_after_sync();
-          for (int s = 0; s * 16 < p.n; ++s)
-            tc::mma(dx_tmem,
-                    tc::descriptor_k_major(z_now + (s >> 2) * kAPlane + (s & 3) * tc::kStepK),
-                    tc::descriptor_mn_major(w_at + s * tc::kStepMn, w_block), dx_instruction,
-                    s > 0);
+          for (int c = 0; c * 64 < p.n; ++c)
+            tc::mma_steps(lead, dx_tmem, tc::descriptor_k_major(z_now + c * kAPlane),
+                          tc::descriptor_mn_major(w_at + c * 4 * tc::kStepMn, w_block),
+                          tc::kStepK, tc::kStepMn, min((p.n - c * 64 + 15) / 16, 4),
+                          dx_instruction, c > 0);
         }
-        tc::commit(bar(dx_done));
-        tc::commit(bar(spent[b]));
+        tc::commit(lead, bar(dx_done));
+        tc::commit(lead, bar(spent[b]));
       }
       // whichever way the loop ended, no product is in flight past this point
-      tc::commit(bar(all_done));
+      tc::commit(lead, bar(all_done));
       ok = tc::barrier_wait(bar(all_done), 0) && ok;
     }
   } else {

@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
   const int chunks_all = static_cast<int>((p.k + kChunk - 1) / kChunk);
   const uint32_t ring = resident + (p.resident ? chunks_all * b_bytes : 0);
   const uint32_t stage_bytes = a_bytes + (p.resident ? 0 : b_bytes);
-  const int warp = threadIdx.x >> 5;
+  const int warp = tc::uniform(threadIdx.x >> 5);
 
   if (threadIdx.x == 0) {
     const int arrivals = p.copy_operands ? 1 : kProducers;
@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = tmem_base;
+  const uint32_t tmem = tc::uniform(tmem_base);
   bool ok = true;
 
   if (warp >= kEpilogueWarps && warp < kEpilogueWarps + kProducers / 32) {
@@ -665,8 +665,9 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
         ok = tc::barrier_wait(tc::shared_address(&raw_full[j & 1]), (j >> 1) & 1) && ok;
     }
   } else if (warp == kEpilogueWarps + kProducers / 32) {
-    // ---- one thread issues the products
-    if ((threadIdx.x & 31) == 0) {
+    // ---- one warp issues the products
+    {
+      const uint32_t lead = tc::elected();
       constexpr bool kBf16 = !(PA == 1 && PB == 1 && kIsF16<SA>);
       constexpr int kParts = PA > PB ? PA : PB;
       // the part of A in the first product of the smallest kind
@@ -702,26 +703,25 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
                 // the first product into an accumulator overwrites it
                 const bool own = sum == 0 && kAcc == 2;
                 const bool first = k == sum_k && (own || (sum == kParts - 1 && i == first_part));
-                for (int s = 0; s < steps; ++s) {
-                  const uint32_t ao = at + i * kAPlane + s * (AMN ? tc::kStepMn : tc::kStepK);
-                  const uint32_t bo = b_at + j * b_plane + s * (BMN ? tc::kStepMn : tc::kStepK);
-                  tc::mma(d + (own ? 0 : (kAcc - 1) * p.tile_n),
-                          AMN ? tc::descriptor_mn_major(ao, a_block) : tc::descriptor_k_major(ao),
-                          BMN ? tc::descriptor_mn_major(bo, kChunk * 128)
-                              : tc::descriptor_k_major(bo),
-                          instruction, !(first && s == 0));
-                }
+                const uint32_t ao = at + i * kAPlane, bo = b_at + j * b_plane;
+                tc::mma_steps(lead, d + (own ? 0 : (kAcc - 1) * p.tile_n),
+                              AMN ? tc::descriptor_mn_major(ao, a_block)
+                                  : tc::descriptor_k_major(ao),
+                              BMN ? tc::descriptor_mn_major(bo, kChunk * 128)
+                                  : tc::descriptor_k_major(bo),
+                              AMN ? tc::kStepMn : tc::kStepK, BMN ? tc::kStepMn : tc::kStepK,
+                              steps, instruction, !first);
               }
-            tc::commit(tc::shared_address(&empty[stage]));
+            tc::commit(lead, tc::shared_address(&empty[stage]));
             if (++stage == p.stages) stage = 0, parity ^= 1;
           }
-          tc::commit(tc::shared_address(&acc_full[acc]));
+          tc::commit(lead, tc::shared_address(&acc_full[acc]));
           acc ^= 1;
           if (acc == 0) acc_parity ^= 1;
         }
       }
       // whichever way the loop ended, no product is in flight past this point
-      tc::commit(tc::shared_address(&drained));
+      tc::commit(lead, tc::shared_address(&drained));
       ok = tc::barrier_wait(tc::shared_address(&drained), 0) && ok;
     }
   } else if (warp < kEpilogueWarps) {

@@ -194,20 +194,54 @@ __host__ __device__ constexpr uint32_t instruction(bool is_bf16, bool a_mn, bool
          (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-// D (tensor memory) = A B^T, or += with accumulate; one thread.
-SPLAT_DEV void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, bool accumulate) {
+// One lane of a warp, chosen by the hardware: 1 there, 0 in the others.  What
+// issues products runs in the whole warp, its instructions guarded by this
+// value: the operands then live in uniform registers, while in one lane's
+// branch each of them is moved there for every instruction (about 100 cycles a
+// product).
+SPLAT_DEV uint32_t elected() {
+  uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r;
+}
+// A value that all lanes of the warp have, as the compiler does not know.
+SPLAT_DEV uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// D (tensor memory) = A B^T, or += with accumulate; issued by the elected lane.
+SPLAT_DEV void mma(uint32_t elected, uint32_t d, uint64_t a, uint64_t b, uint32_t instruction,
+                   bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(instruction), "r"(static_cast<uint32_t>(accumulate))
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(instruction), "r"(static_cast<uint32_t>(accumulate)), "r"(elected)
       : "memory");
 }
-// The barrier gets one arrival when all earlier mma of this thread are done.
-SPLAT_DEV void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   bar)
-               : "memory");
+// A run of products over `steps` steps of 16 k: descriptors advance by da and
+// db (bytes) a step.
+SPLAT_DEV void mma_steps(uint32_t elected, uint32_t d, uint64_t a, uint64_t b, uint32_t da,
+                         uint32_t db, int steps, uint32_t instruction, bool accumulate) {
+#pragma unroll 4
+  for (int s = 0; s < steps; ++s) {
+    mma(elected, d, a, b, instruction, accumulate || s > 0);
+    a += da >> 4;
+    b += db >> 4;
+  }
+}
+// The barrier gets one arrival when all earlier mma of this lane are done.
+SPLAT_DEV void commit(uint32_t elected, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          bar),
+      "r"(elected)
+      : "memory");
 }
 
 }  // namespace tc
