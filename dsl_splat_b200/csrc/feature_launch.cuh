@@ -67,10 +67,13 @@ int launch_product(ProductParams p, cudaStream_t s) {
   p.bias_shared = p.bias && columns <= kMaxSharedBias ? columns : 0;
   p.tmem_columns = 32;
   constexpr int kAcc = accumulators(PA, PB);
-  while (p.tmem_columns < 2u * kAcc * p.tile_n) p.tmem_columns *= 2;
   // sums of several accumulators are joined in fp32 outputs; an operand row of
   // more values than kExactSum is summed in one
   p.k_per_sum = kAcc == 2 && EPI == kPlain && sizeof(TO) == 4 ? kExactSum : p.k_per_split;
+  p.alternate = p.tile_n == 32 && p.k_per_sum >= p.k_per_split;
+  p.accumulators = p.alternate ? 4 : 2;
+  while (p.tmem_columns < static_cast<uint32_t>(p.accumulators * kAcc * p.tile_n))
+    p.tmem_columns *= 2;
   const int b_bytes = PB * b_plane_bytes<BMN>(p.tile_n), a_bytes = PA * kAPlane;
   const long long chunks = (p.k + kChunk - 1) / kChunk;
   const long long whole_b = chunks * b_bytes;

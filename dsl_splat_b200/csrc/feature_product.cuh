@@ -13,10 +13,10 @@
 // producer warps (converting and zero-filling on the way: any row length, any
 // row count).  These take the tiles of a short-rowed A, which are contiguous,
 // from bulk copies that run two tiles ahead.  One thread issues
-// the products, and eight epilogue warps take the finished accumulator, of which
-// there are two, so that loads, products and epilogues of neighbouring tiles
-// overlap.  Where the whole of B fits beside the ring it is loaded once per
-// block.
+// the products, and eight epilogue warps take the finished accumulators, of
+// which there are two or four, so that loads, products and epilogues of
+// neighbouring tiles overlap.  Where the whole of B fits beside the ring it is
+// loaded once per block.
 #pragma once
 #include <type_traits>
 
@@ -29,7 +29,7 @@ namespace feature {
 constexpr int kTileRows = 128;
 constexpr int kChunk = 64;             // k of a stage: 128 bytes of 16-bit values
 constexpr int kEpilogueWarps = 8;                  // epilogue warps
-constexpr int kMaxStages = 8;
+constexpr int kMaxStages = 8, kMaxAccumulators = 4;
 constexpr int kAPlane = kTileRows * 128;
 
 // Producer threads: operands that are split always pass through registers, so
@@ -63,6 +63,10 @@ struct ProductParams {
   int splits, tile_n;
   uint32_t tiles_n, tiles_m, tiles;  // tiles = splits * tiles_m * tiles_n, below 2^31
   int stages, resident, activation;
+  // accumulators of a block: 2, whose columns the two groups of four epilogue
+  // warps share; or 4 (alternate), each finished by one group, for tiles of 32
+  // columns, which leave a second group nothing to do
+  int accumulators, alternate;
   uint32_t tmem_columns;
   const void* bias;   // (n) or NULL
   const void* extra;  // residual or dy (m, n), or NULL
@@ -514,8 +518,8 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
     product_kernel(const __grid_constant__ ProductParams p) {
   constexpr int kProducers = producers(PA, PB), kAcc = accumulators(PA, PB);
   extern __shared__ unsigned char dynamic[];
-  __shared__ alignas(8) unsigned long long full[kMaxStages], empty[kMaxStages], acc_full[2],
-      acc_empty[2], resident_full, drained, extra_full[kEpilogueWarps], raw_full[2],
+  __shared__ alignas(8) unsigned long long full[kMaxStages], empty[kMaxStages],
+      acc_full[kMaxAccumulators], acc_empty[kMaxAccumulators], resident_full, drained, extra_full[kEpilogueWarps], raw_full[2],
       raw_read[2];
   __shared__ uint32_t tmem_base;
   const uint32_t base = (tc::shared_address(dynamic) + 1023u) & ~1023u;
@@ -539,8 +543,11 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
     for (int i = 0; i < 2; ++i) {
       tc::barrier_init(tc::shared_address(&raw_full[i]), 1);
       tc::barrier_init(tc::shared_address(&raw_read[i]), kProducers);
+    }
+    for (int i = 0; i < p.accumulators; ++i) {
       tc::barrier_init(tc::shared_address(&acc_full[i]), 1);
-      tc::barrier_init(tc::shared_address(&acc_empty[i]), kEpilogueWarps * 32);
+      tc::barrier_init(tc::shared_address(&acc_empty[i]),
+                       kEpilogueWarps * (p.alternate ? 16 : 32));
     }
     tc::barrier_init(tc::shared_address(&resident_full), arrivals);
     tc::barrier_init(tc::shared_address(&drained), 1);
@@ -678,12 +685,14 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
       const uint32_t a_block = p.m > 64 ? kChunk * 128 : 0;
       if (p.resident) ok = tc::barrier_wait(tc::shared_address(&resident_full), 0);
       int stage = 0;
-      uint32_t parity = 0, acc = 0, acc_parity = 1;
+      uint32_t parity = 0, i_acc = 0;  // accumulators filled
       for (uint32_t t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
         const ProductTile tile(p, t);
         int c = 0;
         for (long long sum_k = tile.k0; sum_k < tile.k1 && ok; sum_k += p.k_per_sum) {
-          if (!(ok = tc::barrier_wait(tc::shared_address(&acc_empty[acc]), acc_parity))) break;
+          const uint32_t acc = i_acc & (p.accumulators - 1);
+          const uint32_t round = p.alternate ? i_acc >> 2 : i_acc >> 1;
+          if (!(ok = tc::barrier_wait(tc::shared_address(&acc_empty[acc]), (round & 1) ^ 1))) break;
           tc::fence_after_sync();
           const uint32_t d = tmem + acc * kAcc * p.tile_n;
           const long long sum_end = min(sum_k + p.k_per_sum, tile.k1);
@@ -716,8 +725,7 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
             if (++stage == p.stages) stage = 0, parity ^= 1;
           }
           tc::commit(lead, tc::shared_address(&acc_full[acc]));
-          acc ^= 1;
-          if (acc == 0) acc_parity ^= 1;
+          ++i_acc;
         }
       }
       // whichever way the loop ended, no product is in flight past this point
@@ -732,7 +740,11 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
     const Patch<TO> out_patch{base + warp * p.staging};
     const bool leader = (threadIdx.x & 31) == 0;
     const uint32_t extra_bar = tc::shared_address(&extra_full[warp]);
-    uint32_t acc = 0, parity = 0, extra_parity = 0;
+    // the accumulators and tiles of this warp, and its first chunk of columns
+    const uint32_t i_step = p.alternate ? 2 : 1, t_step = gridDim.x * i_step;
+    const uint32_t t_first = blockIdx.x + (p.alternate ? half * gridDim.x : 0);
+    const int c_first = p.alternate ? 0 : half;
+    uint32_t i_acc = p.alternate ? half : 0, extra_parity = 0;
     bool extra_coming = false;
     // starts the copy of the extra values of a tile's patch
     const auto fetch_extra = [&](const ProductTile& tile, int c) {
@@ -745,15 +757,18 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
       }
       extra_coming = true;
     };
-    if (kExtra && p.copy_extra) fetch_extra(ProductTile(p, blockIdx.x), half);
-    for (uint32_t t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+    if (kExtra && p.copy_extra && t_first < p.tiles)
+      fetch_extra(ProductTile(p, t_first), c_first);
+    for (uint32_t t = t_first; t < p.tiles && ok; t += t_step) {
       const ProductTile tile(p, t);
       const long long row0 = tile.m0 + lane_block * 32;
       const int rows = static_cast<int>(min(p.m - row0, 32LL));
       TO* out = static_cast<TO*>(p.out) + (tile.split * p.m + row0) * p.n;
       for (long long sum_k = tile.k0; sum_k < tile.k1; sum_k += p.k_per_sum) {
         bool waited = false;
-        for (int c = half; c * 32 < p.tile_n; c += kEpilogueWarps / 4) {
+        const uint32_t acc = i_acc & (p.accumulators - 1);
+        const uint32_t parity = (p.alternate ? i_acc >> 2 : i_acc >> 1) & 1;
+        for (int c = c_first; c * 32 < p.tile_n; c += kEpilogueWarps / 4) {
           const int col0 = tile.n0 + c * 32, cols = min(p.n - col0, 32);
           if (cols <= 0 || rows <= 0) break;
           if (kExtra && p.extra && !p.copy_extra) {
@@ -812,8 +827,8 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
               const int next = c + kEpilogueWarps / 4;
               if (next * 32 < p.tile_n && tile.n0 + next * 32 < p.n)
                 fetch_extra(tile, next);
-              else if (p.tiles - t > gridDim.x)
-                fetch_extra(ProductTile(p, t + gridDim.x), half);
+              else if (p.tiles - t > t_step)
+                fetch_extra(ProductTile(p, t + t_step), c_first);
             }
           }
           if (leader && p.copy_out) tc::copies_out_read();
@@ -839,13 +854,12 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
         if (!ok) break;
         if (!waited) {  // a warp without a patch still takes part
           if (!(ok = tc::barrier_wait(tc::shared_address(&acc_full[acc]), parity))) break;
-          if (kExtra && p.copy_extra && !extra_coming && p.tiles - t > gridDim.x)
-            fetch_extra(ProductTile(p, t + gridDim.x), half);
+          if (kExtra && p.copy_extra && !extra_coming && p.tiles - t > t_step)
+            fetch_extra(ProductTile(p, t + t_step), c_first);
         }
         tc::fence_before_sync();
         tc::barrier_arrive(tc::shared_address(&acc_empty[acc]));
-        acc ^= 1;
-        if (acc == 0) parity ^= 1;
+        i_acc += i_step;
       }
     }
     if (extra_coming) ok = tc::barrier_wait(extra_bar, extra_parity) && ok;
