@@ -95,7 +95,8 @@ SIGNATURES: dict[str, tuple] = {
                                        _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P]),
     "splat_aaa_preprocess_backward": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "splat_aaa_camera_backward": (_I, [_P, _P, _P, _P, _P, _P, _P]),
-    "splat_feature_linear": (_I, [_I, _L, _I, _I, _P, _P, _P, _P, _I, _P, _P]),
+    "splat_feature_linear_workspace_bytes": (_Z, [_I, _L, _I, _I]),
+    "splat_feature_linear": (_I, [_I, _L, _I, _I, _P, _P, _P, _P, _I, _P, _P, _Z, _P]),
     "splat_feature_linear_backward_workspace_bytes": (_Z, [_I, _L, _I, _I, _I]),
     "splat_feature_linear_backward": (_I, [_I, _L, _I, _I, _P, _P, _P, _I, _P, _P, _P, _P, _P,
                                            _Z, _P]),

@@ -1,6 +1,7 @@
 // Host side of the linear layer's products: tiling and launch.
 #pragma once
 #include <algorithm>
+#include <type_traits>
 
 #include "feature_product.cuh"
 #include "host_runtime.h"
@@ -42,6 +43,7 @@ bool make_map(CUtensorMap& map, const void* base, long long rows, long long colu
 // base to 1 KB.
 constexpr int kOneBlockBytes = 225 * 1024, kTwoBlocksBytes = 110 * 1024;
 constexpr int kMaxSharedBias = 4096;  // values
+constexpr long long kFewRows = 1024;
 constexpr int kMaxResidentBytes = 128 * 1024;
 
 // Fills in the tiling of p (its sources, sizes and epilogue set) and launches.
@@ -85,7 +87,16 @@ int launch_product(ProductParams p, cudaStream_t s) {
   int blocks = 2, budget = kTwoBlocksBytes;
   if (producers(PA, PB) > 128 || p.tmem_columns > 256 || fixed + 2 * stage > budget)
     blocks = 1, budget = kOneBlockBytes;
-  if constexpr (PA == 1 && PB == 1) {
+  if (p.a_plane_rows) {
+    // both operands are planes; f16 ones hold f16, all others bf16 parts
+    using H = std::conditional_t<kIsF16<SA>, f16, bf16>;
+    p.copy_operands =
+        make_map<H>(p.a_map, p.a, static_cast<long long>(p.a_plane_rows) * PA, AMN ? p.m : p.k,
+                    p.a_ld, kChunk, AMN ? kChunk : kTileRows) &&
+        make_map<H>(p.b_map, p.b, static_cast<long long>(p.b_plane_rows) * PB, BMN ? p.n : p.k,
+                    p.b_ld, kChunk, BMN ? kChunk : p.tile_n);
+    if (!p.copy_operands) return host::fail(kInvalidArgument, "feature_linear: operand planes");
+  } else if constexpr (PA == 1 && PB == 1) {
     p.copy_operands =
         make_map<SA>(p.a_map, p.a, AMN ? p.k : p.m, AMN ? p.m : p.k, p.a_ld, kChunk,
                      AMN ? kChunk : kTileRows) &&
@@ -125,6 +136,54 @@ int launch_product(ProductParams p, cudaStream_t s) {
 template <class T>
 constexpr int kOperandParts = sizeof(T) == 4 ? 3 : 1;
 
+// A matrix (rows, cols) of T as planes of its parts.
+struct Planes {
+  void* data = nullptr;
+  long long rows = 0;
+  int plane_rows = 0, ld = 0;
+};
+inline long long round_to(long long n, long long m) { return (n + m - 1) / m * m; }
+template <class T>
+size_t plane_bytes(long long rows, int cols) {
+  return static_cast<size_t>(kOperandParts<T>) * round_to(rows, 64) * round_to(cols, 8) * 2;
+}
+template <class T>
+Planes split(const void* src, long long rows, int cols, void* to, cudaStream_t s) {
+  Planes p;
+  if (sizeof(T) == 2 && row_vector<T>(src, cols) == 16) {  // it is one as it lies
+    p.data = const_cast<void*>(src);
+    p.rows = rows, p.plane_rows = static_cast<int>(rows), p.ld = cols;
+    return p;
+  }
+  p.data = to;
+  p.rows = rows;
+  p.plane_rows = static_cast<int>(round_to(rows, 64));
+  p.ld = static_cast<int>(round_to(cols, 8));
+  const int pieces = p.ld / 8;
+  const long long total = static_cast<long long>(p.plane_rows) * pieces;
+  const unsigned grid = static_cast<unsigned>(
+      std::min<long long>((total + 1023) / 1024, 8LL * host::sm_count()));
+  const auto run = [&](auto bytes) {
+    split_kernel<T, kOperandParts<T>, decltype(bytes)::value><<<grid, 256, 0, host::counted(s)>>>(
+        static_cast<const T*>(src), rows, cols, pieces, p.plane_rows, p.ld,
+        static_cast<uint16_t*>(to));
+  };
+  const int vector = row_vector<T>(src, cols);
+  if (vector == 16) run(std::integral_constant<int, 16>{});
+  else if (vector >= 4) run(std::integral_constant<int, 4>{});
+  else run(std::integral_constant<int, static_cast<int>(sizeof(T))>{});
+  return p;
+}
+
+// Whether the wide layers' products take planes: fp32 operands, and rows that
+// are not whole 16-byte pieces.  A pass over few rows would cost its launch.
+template <class T>
+bool wants_planes(long long rows, int k, int n) {
+  const int whole = 16 / static_cast<int>(sizeof(T));
+  return rows >= kFewRows && kOperandParts<T> * round_to(rows, 64) < 1LL << 31 &&
+         (sizeof(T) == 4 || k % whole || n % whole);
+}
+
 template <class T>
 ProductParams forward_params(long long rows, int k, int n, const void* x, const void* weight,
                              const void* bias, const void* extra, int activation, void* out) {
@@ -135,6 +194,11 @@ ProductParams forward_params(long long rows, int k, int n, const void* x, const 
   p.k_per_split = k, p.splits = 1;
   p.bias = bias, p.extra = extra, p.activation = activation, p.out = out;
   return p;
+}
+
+inline void use_planes(ProductParams& p, const Planes& a, const Planes& b) {
+  p.a = a.data, p.a_ld = a.ld, p.a_plane_rows = a.plane_rows;
+  p.b = b.data, p.b_ld = b.ld, p.b_plane_rows = b.plane_rows;
 }
 
 int check_linear(int dtype, long long rows, int k, int n, int activation);

@@ -130,19 +130,26 @@ size_t dz_bytes(int dtype, long long rows, int n, int activation) {
   return activation == kNone ? 0 : round16(static_cast<size_t>(rows) * n * (dtype == kF32 ? 4 : 2));
 }
 
+// What the wide layers' products read: the tensors, or planes of them.
+struct Sources {
+  const void *x, *weight, *dz;
+  Planes x_planes, weight_planes, dz_planes;  // data: NULL without planes
+};
+
 // The two products of the backward.
 template <class T>
-int launch_gradients(long long rows, int k, int n, const T* dz, const void* x,
-                     const void* weight, void* dx, void* dweight, void* dbias, float* partial,
-                     cudaStream_t s) {
+int launch_gradients(long long rows, int k, int n, const Sources& from, void* dx, void* dweight,
+                     void* dbias, float* partial, cudaStream_t s) {
   constexpr int P = kOperandParts<T>;
+  const bool planes = from.dz_planes.data != nullptr;
   if (dx) {
     ProductParams p{};
     p.m = rows, p.k = n, p.n = k;
-    p.a = dz, p.a_ld = n;
-    p.b = weight, p.b_ld = k;
+    p.a = from.dz, p.a_ld = n;
+    p.b = from.weight, p.b_ld = k;
     p.k_per_split = n, p.splits = 1;
     p.out = dx;
+    if (planes) use_planes(p, from.dz_planes, from.weight_planes);
     const int status = launch_product<T, P, false, T, P, true, T, T, kPlain>(p, s);
     if (status != kOk) return status;
   }
@@ -150,10 +157,11 @@ int launch_gradients(long long rows, int k, int n, const T* dz, const void* x,
   if (dweight) {
     ProductParams p{};
     p.m = n, p.k = rows, p.n = k;
-    p.a = dz, p.a_ld = n;
-    p.b = x, p.b_ld = k;
+    p.a = from.dz, p.a_ld = n;
+    p.b = from.x, p.b_ld = k;
     p.k_per_split = splits.rows, p.splits = splits.count;
     p.out = partial;
+    if (planes) use_planes(p, from.dz_planes, from.x_planes);
     const int status = launch_product<T, P, true, T, P, true, float, float, kPlain>(p, s);
     if (status != kOk) return status;
     const long long count = static_cast<long long>(n) * k;
@@ -161,7 +169,7 @@ int launch_gradients(long long rows, int k, int n, const T* dz, const void* x,
   }
   if (dbias) {
     float* sums = partial + static_cast<long long>(splits.count) * n * k;
-    const int count = sum_columns<T>(dz, rows, n, sums, s);
+    const int count = sum_columns<T>(static_cast<const T*>(from.dz), rows, n, sums, s);
     join_splits<T>(sums, n, count, n, 0, dbias, nullptr, s);
   }
   return host::check_launch("feature_linear_backward");
@@ -294,8 +302,13 @@ size_t splat_feature_linear_backward_workspace_bytes(int dtype, long long rows, 
   const size_t sums = static_cast<size_t>(n) * (static_cast<size_t>(k) + 1) * 4;
   if (plan.blocks) return plan.blocks * sums;
   return dz_bytes(dtype, rows, n, activation) +
-         static_cast<size_t>(weight_splits(rows, k, n).count) * n * k * 4 +
-         static_cast<size_t>(kMaxColumnSplits) * n * 4;
+         round16(static_cast<size_t>(weight_splits(rows, k, n).count) * n * k * 4) +
+         round16(static_cast<size_t>(kMaxColumnSplits) * n * 4) +
+         SPLAT_FEATURE_TYPE(dtype, [&] {
+           return wants_planes<T>(rows, k, n) ? plane_bytes<T>(rows, k) + plane_bytes<T>(n, k) +
+                                                    plane_bytes<T>(rows, n)
+                                              : static_cast<size_t>(0);
+         });
 }
 
 int splat_feature_linear_backward(int dtype, long long rows, int k, int n, const void* x,
@@ -317,17 +330,29 @@ int splat_feature_linear_backward(int dtype, long long rows, int k, int n, const
     if (plan.blocks)
       return launch_fused<T>(plan, rows, k, n, x, weight, bias, activation, dy, dx, dweight,
                              dbias, static_cast<float*>(workspace), s);
-    const T* dz = static_cast<const T*>(dy);
-    if (activation != kNone) {
-      constexpr int P = kOperandParts<T>;
-      const int status = launch_product<T, P, false, T, P, false, T, T, kSlope>(
-          forward_params<T>(rows, k, n, x, weight, bias, dy, activation, workspace), s);
-      if (status != kOk) return status;
-      dz = static_cast<const T*>(workspace);
+    constexpr int P = kOperandParts<T>;
+    char* at = static_cast<char*>(workspace);
+    void* dz = at;
+    at += dz_bytes(dtype, rows, n, activation);
+    float* partial = reinterpret_cast<float*>(at);
+    at += round16(static_cast<size_t>(weight_splits(rows, k, n).count) * n * k * 4) +
+          round16(static_cast<size_t>(kMaxColumnSplits) * n * 4);
+    Sources from{x, weight, activation == kNone ? dy : dz, {}, {}, {}};
+    const bool planes = wants_planes<T>(rows, k, n);
+    if (planes) {
+      if (dweight || activation != kNone) from.x_planes = split<T>(x, rows, k, at, s);
+      at += plane_bytes<T>(rows, k);
+      if (dx || activation != kNone) from.weight_planes = split<T>(weight, n, k, at, s);
+      at += plane_bytes<T>(n, k);
     }
-    float* partial = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                              dz_bytes(dtype, rows, n, activation));
-    return launch_gradients<T>(rows, k, n, dz, x, weight, dx, dweight, dbias, partial, s);
+    if (activation != kNone) {
+      ProductParams p = forward_params<T>(rows, k, n, x, weight, bias, dy, activation, dz);
+      if (planes) use_planes(p, from.x_planes, from.weight_planes);
+      const int status = launch_product<T, P, false, T, P, false, T, T, kSlope>(p, s);
+      if (status != kOk) return status;
+    }
+    if (planes && (dx || dweight)) from.dz_planes = split<T>(from.dz, rows, n, at, s);
+    return launch_gradients<T>(rows, k, n, from, dx, dweight, dbias, partial, s);
   });
 }
 

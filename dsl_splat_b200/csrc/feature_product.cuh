@@ -12,7 +12,9 @@
 // tensor copies that one thread starts, all others through four or eight
 // producer warps (converting and zero-filling on the way: any row length, any
 // row count).  These take the tiles of a short-rowed A, which are contiguous,
-// from bulk copies that run two tiles ahead.  One thread issues
+// from bulk copies that run two tiles ahead.  What would be converted again and
+// again (fp32 operands of several tiles, long unaligned rows) is laid out as
+// planes of parts by a pass before, and copied as well.  One warp issues
 // the products, and eight epilogue warps take the finished accumulators, of
 // which there are two or four, so that loads, products and epilogues of
 // neighbouring tiles overlap.  Where the whole of B fits beside the ring it is
@@ -49,6 +51,9 @@ enum Epilogue : int { kForward = 0, kSlope = 1, kPlain = 2 };
 struct ProductParams {
   CUtensorMap a_map, b_map, extra_map, out_map;
   int copy_operands, copy_extra, copy_out;  // by tensor copies
+  // the operands' parts lie in memory as 16-bit planes of so many rows (0: they
+  // are made on the way)
+  int a_plane_rows, b_plane_rows;
   int raw_bytes;   // of a tile of A as it is in memory, copied ahead; 0: none
   int staging;     // bytes of an epilogue warp
   long long m, k;  // k of all splits
@@ -311,15 +316,19 @@ SPLAT_DEV uint32_t chunk_bytes(int width, long long mn_valid) {
   return MN ? static_cast<uint32_t>(min((mn_valid + 63) / 64, (width + 63LL) / 64)) * (kChunk * 128)
             : width * 128;
 }
-template <bool MN>
-SPLAT_DEV void copy_chunk(const CUtensorMap* map, uint32_t dst, int width, long long mn0,
-                          long long mn_valid, long long k0, uint32_t bar) {
-  if constexpr (MN) {
-    for (int b = 0; b * 64 < width && b * 64 < mn_valid; ++b)
-      tc::copy_in(dst + b * (kChunk * 128), map, static_cast<int>(mn0) + b * 64,
-                  static_cast<int>(k0), bar);
-  } else {
-    tc::copy_in(dst, map, static_cast<int>(k0), static_cast<int>(mn0), bar);
+template <int P, bool MN>
+SPLAT_DEV void copy_chunk(const CUtensorMap* map, uint32_t dst, uint32_t plane, int plane_rows,
+                          int width, long long mn0, long long mn_valid, long long k0,
+                          uint32_t bar) {
+#pragma unroll
+  for (int i = 0; i < P; ++i, dst += plane) {
+    if constexpr (MN) {
+      for (int b = 0; b * 64 < width && b * 64 < mn_valid; ++b)
+        tc::copy_in(dst + b * (kChunk * 128), map, static_cast<int>(mn0) + b * 64,
+                    static_cast<int>(k0) + i * plane_rows, bar);
+    } else {
+      tc::copy_in(dst, map, static_cast<int>(k0), static_cast<int>(mn0) + i * plane_rows, bar);
+    }
   }
 }
 
@@ -482,6 +491,43 @@ SPLAT_DEV void finish_row(const Patch<TE, W>& extra, bool with_extra, float (&v)
   }
 }
 
+// ---- operands as planes ----------------------------------------------------------
+
+// src (rows, cols) as `P` planes of plane_rows x ld 16-bit parts; rows behind
+// the last are zero, columns behind the last are not written (nor read).
+template <class S, int P, int VB>
+__global__ void __launch_bounds__(256)
+    split_kernel(const S* src, long long rows, int cols, int pieces, long long plane_rows, int ld,
+                 uint16_t* dst) {
+  const long long total = plane_rows * pieces;
+  constexpr int U = 4;
+  for (long long i0 = blockIdx.x * 256LL + threadIdx.x; i0 < total; i0 += U * 256LL * gridDim.x) {
+    Vec<S, 8> v[U];
+    long long row[U];
+    int piece[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long i = i0 + u * 256LL * gridDim.x;
+      row[u] = i >= total ? plane_rows
+               : total <= 0xffffffffLL
+                   ? static_cast<uint32_t>(i) / static_cast<uint32_t>(pieces)
+                   : i / pieces;
+      piece[u] = static_cast<int>(i - row[u] * pieces);
+      v[u] = load8<S, VB>(src + row[u] * cols + piece[u] * 8,
+                          row[u] < rows ? min(cols - piece[u] * 8, 8) : 0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (row[u] < plane_rows) {
+        uint4 parts[P];
+        to_parts<S, P>(v[u], parts);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+          *reinterpret_cast<uint4*>(dst + (p * plane_rows + row[u]) * ld + piece[u] * 8) = parts[p];
+      }
+  }
+}
+
 // ---- the kernel ------------------------------------------------------------------
 
 // Bytes of a plane of B's chunk.
@@ -571,14 +617,14 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
     const int thread = threadIdx.x - kEpilogueWarps * 32;
     int stage = 0;
     uint32_t parity = 1;  // a fresh barrier's previous phase counts as complete
-    if (PA == 1 && PB == 1 && p.copy_operands) {
+    if (p.copy_operands) {
       if (thread == 0) {
         if (p.resident) {
           const uint32_t bar = tc::shared_address(&resident_full);
-          tc::barrier_expect(bar, chunks_all * chunk_bytes<BMN>(p.tile_n, p.n));
+          tc::barrier_expect(bar, chunks_all * PB * chunk_bytes<BMN>(p.tile_n, p.n));
           for (int c = 0; c < chunks_all; ++c)
-            copy_chunk<BMN>(&p.b_map, resident + c * b_bytes, p.tile_n, 0, p.n,
-                            static_cast<long long>(c) * kChunk, bar);
+            copy_chunk<PB, BMN>(&p.b_map, resident + c * b_bytes, b_plane, p.b_plane_rows, p.tile_n,
+                                0, p.n, static_cast<long long>(c) * kChunk, bar);
         }
         int started = 0;  // stages that have been filled at least once
         for (uint32_t t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
@@ -587,11 +633,14 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
             if (!(ok = tc::barrier_wait(tc::shared_address(&empty[stage]), parity))) break;
             const uint32_t at = ring + stage * stage_bytes, bar = tc::shared_address(&full[stage]);
             tc::barrier_expect(bar,
-                               chunk_bytes<AMN>(kTileRows, p.m - tile.m0) +
-                                   (p.resident ? 0 : chunk_bytes<BMN>(p.tile_n, p.n - tile.n0)));
-            copy_chunk<AMN>(&p.a_map, at, kTileRows, tile.m0, p.m - tile.m0, k, bar);
+                               PA * chunk_bytes<AMN>(kTileRows, p.m - tile.m0) +
+                                   (p.resident ? 0
+                                               : PB * chunk_bytes<BMN>(p.tile_n, p.n - tile.n0)));
+            copy_chunk<PA, AMN>(&p.a_map, at, kAPlane, p.a_plane_rows, kTileRows, tile.m0,
+                                p.m - tile.m0, k, bar);
             if (!p.resident)
-              copy_chunk<BMN>(&p.b_map, at + a_bytes, p.tile_n, tile.n0, p.n - tile.n0, k, bar);
+              copy_chunk<PB, BMN>(&p.b_map, at + a_bytes, b_plane, p.b_plane_rows, p.tile_n,
+                                  tile.n0, p.n - tile.n0, k, bar);
             started = max(started, stage + 1);
             if (++stage == p.stages) stage = 0, parity ^= 1;
           }

@@ -723,10 +723,14 @@ def feature_linear(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Ten
     (m, k), n = x.shape, weight.shape[0]
     y = x.new_empty((m, n))
     if m:
+        dtype, device = FEATURE_DTYPES[x.dtype], x.device
+        size = _query(lib.splat_feature_linear_workspace_bytes, "feature_linear", device, dtype, m,
+                      k, n)
+        ws = x.new_empty((size,), dtype=torch.uint8) if size > 16 else None
         x, weight, bias, residual = _dense(x), _dense(weight), _dense(bias), _dense(residual)
-        _call(lib.splat_feature_linear, "feature_linear", x.device, FEATURE_DTYPES[x.dtype], m, k,
-              n, x.data_ptr(), weight.data_ptr(), _address(bias), _address(residual),
-              _ACTIVATION_CODES[activation], y.data_ptr())
+        _call(lib.splat_feature_linear, "feature_linear", device, dtype, m, k, n, x.data_ptr(),
+              weight.data_ptr(), _address(bias), _address(residual),
+              _ACTIVATION_CODES[activation], y.data_ptr(), _address(ws), size)
     return y
 
 

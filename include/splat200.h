@@ -573,10 +573,13 @@ int splat_debug_expf(int n, const float* x, float* ours, float* cuda_exp, void* 
  * not depend on the order in which blocks run. */
 
 /* y = act(x weight^T + bias) + residual; x (rows, k), weight (n, k), bias (n)
- * or NULL, residual (rows, n) or NULL, y (rows, n). */
+ * or NULL, residual (rows, n) or NULL, y (rows, n).  A workspace of 16 bytes
+ * or less may be NULL. */
+size_t splat_feature_linear_workspace_bytes(int dtype, long long rows, int k, int n);
 int splat_feature_linear(int dtype, long long rows, int k, int n, const void* x,
                          const void* weight, const void* bias, const void* residual,
-                         int activation, void* y, void* stream);
+                         int activation, void* y, void* workspace, size_t workspace_bytes,
+                         void* stream);
 
 /* Gradients of the above for the upstream dy (rows, n): dx (rows, k),
  * dweight (n, k), dbias (n), each NULL to skip it (the residual's gradient is
