@@ -118,9 +118,8 @@ int launch_product(ProductParams p, cudaStream_t s) {
   p.error = host::device_error_word();
   if (!p.error) return kCudaError;
   const int bytes = fixed + p.stages * stage + 2 * p.raw_bytes + 1024;
-  auto* kernel = product_kernel<SA, PA, AMN, SB, PB, BMN, TE, TO, EPI>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
-      cudaSuccess)
+  constexpr auto* kernel = product_kernel<SA, PA, AMN, SB, PB, BMN, TE, TO, EPI>;
+  if (!host::allow_shared<kernel>())
     return host::check_launch("feature_linear: shared memory");
   const long long grid = std::min<long long>(p.tiles, static_cast<long long>(host::sm_count()) * blocks);
   kernel<<<static_cast<unsigned>(grid), kEpilogueWarps * 32 + producers(PA, PB) + 32, bytes, host::counted(s)>>>(p);

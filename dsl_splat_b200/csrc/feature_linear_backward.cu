@@ -40,9 +40,34 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// The same with four neighbouring values to a thread, for few splits and one
+// destination.
+template <class T>
+__global__ void __launch_bounds__(256)
+    join_quads_kernel(const float4* partial, long long stride, int splits, long long count, T* a) {
+  const long long i = blockIdx.x * 256LL + threadIdx.x;
+  if (i >= count) return;
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+  for (int k = 0; k < splits; ++k) {
+    const float4 v = partial[k * stride + i];
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  const float f[4] = {s.x, s.y, s.z, s.w};
+  reinterpret_cast<Vec<T, 4>*>(a)[i] = round_values<T, 4>(f);
+}
+
 template <class T>
 void join_splits(const float* partial, long long stride, int splits, long long count_a,
                  long long count_b, void* a, void* b, cudaStream_t s) {
+  // enough quads to fill the device without several threads to a value
+  if (!b && count_b == 0 && count_a % 4 == 0 && stride % 4 == 0 && count_a >= 1 << 16 &&
+      host::aligned(a, 16) && host::aligned(partial, 16)) {
+    join_quads_kernel<T><<<host::blocks_for(count_a / 4, 256), 256, 0, host::counted(s)>>>(
+        reinterpret_cast<const float4*>(partial), stride / 4, splits, count_a / 4,
+        static_cast<T*>(a));
+    return;
+  }
   join_splits_kernel<T>
       <<<host::blocks_for(count_a + count_b, 32), dim3(32, 8), 0, host::counted(s)>>>(
           partial, stride, splits, count_a, count_b, static_cast<T*>(a), static_cast<T*>(b));
@@ -88,6 +113,8 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const S* dz, long long
   }
 }
 
+constexpr int kMaxColumnSplits = 256;
+
 // Their ranges of rows: eight blocks to an SM, 256 rows to a range at least.
 template <class T>
 int sum_columns(const T* dz, long long rows, int n, float* partial, cudaStream_t s) {
@@ -95,7 +122,8 @@ int sum_columns(const T* dz, long long rows, int n, float* partial, cudaStream_t
   const bool vector = n % V == 0 && host::aligned(dz, 16);
   const int blocks = host::blocks_for(n, vector ? 32 * V : 32);
   const long long wanted = std::max(1LL, 8LL * host::sm_count() / blocks);
-  const long long count = std::min({wanted, (rows + 255) / 256, 1024LL});
+  const long long count =
+      std::min({wanted, (rows + 255) / 256, static_cast<long long>(kMaxColumnSplits)});
   const long long per = (rows + count - 1) / count;
   const int splits = static_cast<int>((rows + per - 1) / per);
   const dim3 grid(blocks, splits), block(32, 8);
@@ -105,8 +133,6 @@ int sum_columns(const T* dz, long long rows, int n, float* partial, cudaStream_t
     column_sums_kernel<T, 1><<<grid, block, 0, host::counted(s)>>>(dz, rows, n, per, partial);
   return splits;
 }
-constexpr int kMaxColumnSplits = 1024;
-
 // Ranges of rows whose sums of dz^T x (and of dz) are joined afterwards:
 // enough tiles for two blocks on every SM, 512 rows to a range at least.
 struct Splits {
@@ -236,10 +262,10 @@ int launch_narrow(const FusedPlan& plan, long long rows, int k, int n, const voi
     return host::fail(kInvalidArgument,
                       "feature_linear_backward: tensors must be 16-byte aligned");
   const bool wide = k > 64 || n > 64;
-  auto* kernel = wide ? narrow_backward_kernel<T, true> : narrow_backward_kernel<T, false>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(plan.bytes)) != cudaSuccess)
+  if (!(wide ? host::allow_shared<narrow_backward_kernel<T, true>>()
+             : host::allow_shared<narrow_backward_kernel<T, false>>()))
     return host::check_launch("feature_linear_backward: shared memory");
+  auto* kernel = wide ? narrow_backward_kernel<T, true> : narrow_backward_kernel<T, false>;
   kernel<<<plan.blocks, kNarrowThreads, plan.bytes, host::counted(s)>>>(p);
   return host::check_launch("feature_linear_backward");
 }
@@ -274,11 +300,9 @@ int launch_fused(const FusedPlan& plan, long long rows, int k, int n, const void
     p.tmem_columns = plan.tmem_columns;
     p.error = host::device_error_word();
     if (!p.error) return kCudaError;
-    auto* kernel = fused_backward_kernel<T>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(plan.bytes)) != cudaSuccess)
+    if (!host::allow_shared<fused_backward_kernel<T>>())
       return host::check_launch("feature_linear_backward: shared memory");
-    kernel<<<plan.blocks, kFusedThreads, plan.bytes, host::counted(s)>>>(p);
+    fused_backward_kernel<T><<<plan.blocks, kFusedThreads, plan.bytes, host::counted(s)>>>(p);
   }
   if (partial) {
     const long long count = static_cast<long long>(n) * k;

@@ -950,11 +950,9 @@ Plan make_plan(int value_bytes, int samples, long long positions, int channels, 
 }
 
 // Launches a small sample's kernel as clusters of `blocks`.
-template <class... A, class... B>
-int launch_cluster(void (*kernel)(A...), const Plan& plan, int samples, cudaStream_t s,
-                   B... args) {
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(plan.shared_bytes)) != cudaSuccess)
+template <auto* kernel, class... A>
+int launch_cluster(const Plan& plan, int samples, cudaStream_t s, A... args) {
+  if (!host::allow_shared<kernel>())
     return host::check_launch("feature_norm: shared memory");
   cudaLaunchAttribute cluster;
   cluster.id = cudaLaunchAttributeClusterDimension;
@@ -1063,7 +1061,7 @@ int splat_feature_norm(int dtype, int samples, long long positions, int channels
       constexpr int V = decltype(width)::value;
       if (plan.small)
         return SPLAT_FEATURE_ACT(activation, [&] {
-          return launch_cluster(norm_small_kernel<T, V, ACT>, plan, samples, s, p);
+          return launch_cluster<norm_small_kernel<T, V, ACT>>(plan, samples, s, p);
         });
       norm_sums_kernel<T, V><<<grid, p.l.threads, 0, host::counted(s)>>>(p);
       norm_join_kernel<T><<<samples * groups, kJoinThreads, 0, host::counted(s)>>>(p);
@@ -1122,8 +1120,8 @@ int splat_feature_norm_backward(int dtype, int samples, long long positions, int
         const bool one = samples == 1;
         T *dw1 = one ? dw : nullptr, *db1 = one ? db : nullptr;
         if (plan.small) {
-          const int status = launch_cluster(norm_backward_small_kernel<T, V, ACT>, plan, samples,
-                                            s, p, dw1, db1);
+          const int status = launch_cluster<norm_backward_small_kernel<T, V, ACT>>(
+              plan, samples, s, p, dw1, db1);
           if (status != kOk) return status;
         } else {
           norm_backward_sums_kernel<T, V, ACT><<<grid, p.l.threads, 0, host::counted(s)>>>(p);

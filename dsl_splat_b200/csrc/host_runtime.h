@@ -29,6 +29,23 @@ bool encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, lo
 // Streaming multiprocessors of the current device (148 on B200).
 int sm_count();
 
+// Lets a kernel (of less than 1 KB of static shared memory) take as much
+// dynamic shared memory as a block can have, once per device.
+template <auto* kernel>
+bool allow_shared() {
+  static unsigned long long done[2] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  unsigned long long* word = &done[(dev >> 6) & 1];
+  const unsigned long long bit = 1ULL << (dev & 63);
+  if (__atomic_load_n(word, __ATOMIC_ACQUIRE) & bit) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           226 * 1024) != cudaSuccess)
+    return false;
+  __atomic_fetch_or(word, bit, __ATOMIC_RELEASE);
+  return true;
+}
+
 inline unsigned blocks_for(long long n, int block) {
   return static_cast<unsigned>((n + block - 1) / block);
 }

@@ -11,6 +11,7 @@ stream; tensors must be CUDA float32/int32.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 
@@ -694,15 +695,13 @@ def _call(fn, what: str, device: torch.device, *args) -> None:
         check(status, what)
 
 
-def _query(fn, what: str, device: torch.device, *args) -> int:
-    """A workspace size, which goes by the device's number of multiprocessors."""
-    if torch._C._cuda_getDevice() == device.index:
-        size = fn(*args)
-    else:
-        with torch.cuda.device(device.index):
-            size = fn(*args)
+@functools.lru_cache(maxsize=1024)
+def _query(name: str, index: int, *args) -> int:
+    """A workspace size, which goes by the sizes and the device's multiprocessors."""
+    with torch.cuda.device(index):
+        size = getattr(lib, name)(*args)
     if not size:
-        raise nv.SplatError(f"{what}: {lib.splat_last_error().decode(errors='replace')}")
+        raise nv.SplatError(f"{name}: {lib.splat_last_error().decode(errors='replace')}")
     return size
 
 
@@ -724,8 +723,8 @@ def feature_linear(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Ten
     y = x.new_empty((m, n))
     if m:
         dtype, device = FEATURE_DTYPES[x.dtype], x.device
-        size = _query(lib.splat_feature_linear_workspace_bytes, "feature_linear", device, dtype, m,
-                      k, n)
+        size = _query("splat_feature_linear_workspace_bytes", device.index,
+                      dtype, m, k, n)
         ws = x.new_empty((size,), dtype=torch.uint8) if size > 16 else None
         x, weight, bias, residual = _dense(x), _dense(weight), _dense(bias), _dense(residual)
         _call(lib.splat_feature_linear, "feature_linear", device, dtype, m, k, n, x.data_ptr(),
@@ -745,8 +744,7 @@ def feature_linear_backward(x: Tensor, weight: Tensor, bias: Tensor | None, acti
     dbias = make((n,)) if needs[2] else None
     if m and any(needs):
         dtype, act, device = FEATURE_DTYPES[x.dtype], _ACTIVATION_CODES[activation], x.device
-        size = _query(lib.splat_feature_linear_backward_workspace_bytes,
-                      "feature_linear_backward", device, dtype, m, k, n, act)
+        size = _query("splat_feature_linear_backward_workspace_bytes", device.index, dtype, m, k, n, act)
         ws = x.new_empty((size,), dtype=torch.uint8)
         x, weight, bias, upstream = _dense(x), _dense(weight), _dense(bias), _dense(upstream)
         _call(lib.splat_feature_linear_backward, "feature_linear_backward", device, dtype, m, k,
@@ -764,8 +762,8 @@ def feature_norm(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | N
     moments = x.new_empty((2, samples, groups), dtype=torch.float32) if save else None
     if samples and positions:
         dtype, device = FEATURE_DTYPES[x.dtype], x.device
-        size = _query(lib.splat_feature_norm_workspace_bytes, "feature_norm", device, dtype,
-                      samples, positions, channels, groups, 0)
+        size = _query("splat_feature_norm_workspace_bytes", device.index,
+                      dtype, samples, positions, channels, groups, 0)
         ws = x.new_empty((size,), dtype=torch.uint8) if size > 16 else None
         x, weight, bias = _dense(x), _dense(weight), _dense(bias)
         mean = rstd = None
@@ -791,8 +789,7 @@ def feature_norm_backward(x: Tensor, groups: int, weight: Tensor | None, bias: T
     dbias = make((channels,)) if needs[2] else None
     if values and any(needs):
         dtype, device = FEATURE_DTYPES[x.dtype], x.device
-        size = _query(lib.splat_feature_norm_workspace_bytes, "feature_norm_backward", device,
-                      dtype, samples, positions, channels, groups, 1)
+        size = _query("splat_feature_norm_workspace_bytes", device.index, dtype, samples, positions, channels, groups, 1)
         ws = x.new_empty((size,), dtype=torch.uint8)
         x, weight, bias, upstream = _dense(x), _dense(weight), _dense(bias), _dense(upstream)
         mean = moments.data_ptr()
