@@ -44,7 +44,7 @@ struct Layout {
   int per_block;
 };
 
-constexpr int kMaxThreads = 256;
+constexpr int kMaxThreads = 512;
 
 struct NormParams {
   Layout l;
@@ -243,7 +243,7 @@ SPLAT_DEV void write_partial(const NormParams& p, const Place& at, const float (
 // Sums of x - pivot and its square per channel; the pivot is the sample's
 // first row, so that a large common offset does not cancel.
 template <class T, int V>
-__global__ void __launch_bounds__(kMaxThreads, 4) norm_sums_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kMaxThreads, 2) norm_sums_kernel(const NormParams p) {
   using Values = Vec<T, V>;
   const Layout& l = p.l;
   const Place at = place<V>(l);
@@ -292,6 +292,36 @@ __global__ void __launch_bounds__(kMaxThreads, 4) norm_sums_kernel(const NormPar
   write_partial<V>(p, at, a, b);
 }
 
+SPLAT_DEV uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+SPLAT_DEV void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// A value in the shared memory of another block of the cluster, at the address
+// that it has in this one.
+SPLAT_DEV double load_cluster(const double* own, uint32_t rank) {
+  const uint32_t here = static_cast<uint32_t>(__cvta_generic_to_shared(own));
+  uint32_t there;
+  double v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(rank));
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(there) : "memory");
+  return v;
+}
+SPLAT_DEV float2 load_cluster(const float2* own, uint32_t rank) {
+  const uint32_t here = static_cast<uint32_t>(__cvta_generic_to_shared(own));
+  uint32_t there;
+  float2 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(there)
+               : "memory");
+  return v;
+}
+
 SPLAT_DEV double warp_sum(double v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -301,7 +331,7 @@ SPLAT_DEV double warp_sum(double v) {
 // The blocks' sums of up to kJoinChannels channels from c0 on, joined in
 // shared memory: neighbouring threads read neighbouring channels of a block's
 // row, and the threads of a channel are added up in a fixed order.
-constexpr int kJoinThreads = 256, kJoinChannels = 32;
+constexpr int kJoinThreads = 1024, kJoinChannels = 32, kMaxCluster = 8;
 
 SPLAT_DEV void channel_sums(const NormParams& p, int sample, int c0, int count,
                             double2 (&joined)[kJoinChannels]) {
@@ -359,8 +389,12 @@ struct Moments {
     const double block_mean = warp_sum(channel_mean) / count, d = channel_mean - block_mean;
     const double block_m2 =
         warp_sum(in ? sums.y - sums.x * sums.x * inverse + rows * d * d : 0.0);
-    const double nb = rows * count, total = n + nb, apart = block_mean - mean;
-    m2 += block_m2 + apart * apart * (n * nb / total);
+    add(rows * count, block_mean, block_m2);
+  }
+  SPLAT_DEV void add(double nb, double mean_b, double m2_b) {
+    if (nb == 0.0) return;
+    const double total = n + nb, apart = mean_b - mean;
+    m2 += m2_b + apart * apart * (n * nb / total);
     mean += apart * (nb / total);
     n = total;
   }
@@ -372,14 +406,17 @@ struct Moments {
   }
 };
 
+// A cluster to a group, its blocks take 32 channels at a time in turn.
 template <class T>
-__global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(const NormParams p, int blocks) {
   __shared__ double2 joined[kJoinChannels];
-  const int sample = blockIdx.x / p.groups, g = blockIdx.x % p.groups;
+  __shared__ double mine[3];
+  const int group = blockIdx.x / blocks, rank = blockIdx.x - group * blocks;
+  const int sample = group / p.groups, g = group - sample * p.groups;
   const double rows = static_cast<double>(p.l.span / p.l.channels);
   const T* x = static_cast<const T*>(p.x) + sample * p.l.span;
   Moments m{};
-  for (int k0 = 0; k0 < p.group_channels; k0 += kJoinChannels) {
+  for (int k0 = rank * kJoinChannels; k0 < p.group_channels; k0 += blocks * kJoinChannels) {
     const int c0 = g * p.group_channels + k0, count = min(kJoinChannels, p.group_channels - k0);
     channel_sums(p, sample, c0, count, joined);
     if (threadIdx.x < 32) {
@@ -388,7 +425,14 @@ __global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(const NormParam
     }
     __syncthreads();
   }
-  if (threadIdx.x == 0) m.finish(p.eps, p.mean + blockIdx.x, p.rstd + blockIdx.x);
+  if (threadIdx.x == 0) mine[0] = m.n, mine[1] = m.mean, mine[2] = m.m2;
+  cluster_sync();
+  if (rank == 0 && threadIdx.x == 0) {
+    for (int r = 1; r < blocks; ++r) m.add(load_cluster(mine, r), load_cluster(mine + 1, r),
+                                           load_cluster(mine + 2, r));
+    m.finish(p.eps, p.mean + group, p.rstd + group);
+  }
+  cluster_sync();  // no block leaves while its sums are read
 }
 
 // The parameters of a thread's V channels: -mean, rstd w, b, and for the
@@ -429,7 +473,7 @@ struct Channels {
 // The passes that write go through a block's steps backwards: what the pass
 // before read last is still in the L2.
 template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kMaxThreads, 4) norm_apply_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kMaxThreads, 2) norm_apply_kernel(const NormParams p) {
   using Values = Vec<T, V>;
   const Layout& l = p.l;
   const Place at = place<V>(l);
@@ -467,7 +511,7 @@ __global__ void __launch_bounds__(kMaxThreads, 4) norm_apply_kernel(const NormPa
 
 // Sums of du and du (x - mean) per channel.
 template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kMaxThreads, 3) norm_backward_sums_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kMaxThreads, 1) norm_backward_sums_kernel(const NormParams p) {
   using Values = Vec<T, V>;
   const Layout& l = p.l;
   const Place at = place<V>(l);
@@ -486,7 +530,7 @@ __global__ void __launch_bounds__(kMaxThreads, 3) norm_backward_sums_kernel(cons
       s1 = s1 + du;
       s2 = fma(du, d, s2);
     };
-    constexpr int U = 2;
+    constexpr int U = 4;
     int i = 0;
     for (; i + U <= at.count; i += U, from += U * at.stride, grad += U * at.stride) {
       Values v[U], g[U];
@@ -511,37 +555,43 @@ __global__ void __launch_bounds__(kMaxThreads, 3) norm_backward_sums_kernel(cons
 
 template <class T>
 __global__ void __launch_bounds__(kJoinThreads)
-    norm_backward_join_kernel(const NormParams p, T* dweight, T* dbias) {
+    norm_backward_join_kernel(const NormParams p, int blocks, T* dweight, T* dbias) {
   __shared__ double2 joined[kJoinChannels];
-  const int sample = blockIdx.x / p.groups, g = blockIdx.x % p.groups;
-  const double rstd = p.rstd[blockIdx.x];
+  __shared__ double mine[2];
+  const int group = blockIdx.x / blocks, rank = blockIdx.x - group * blocks;
+  const int sample = group / p.groups, g = group - sample * p.groups;
+  const double rstd = p.rstd[group];
   double m1 = 0.0, m2 = 0.0;
-  for (int k0 = 0; k0 < p.group_channels; k0 += kJoinChannels) {
+  for (int k0 = rank * kJoinChannels; k0 < p.group_channels; k0 += blocks * kJoinChannels) {
     const int c0 = g * p.group_channels + k0, count = min(kJoinChannels, p.group_channels - k0);
     channel_sums(p, sample, c0, count, joined);
-    if (threadIdx.x < count) {
-      joined[threadIdx.x].y *= rstd;  // of du (x - mean) to du xhat
-      const double2 v = joined[threadIdx.x];
-      if (p.samples > 1)
-        p.channel[static_cast<long long>(sample) * p.l.channels + c0 + threadIdx.x] = v;
-      if (dbias) dbias[c0 + threadIdx.x] = from_float<T>(static_cast<float>(v.x));
-      if (dweight) dweight[c0 + threadIdx.x] = from_float<T>(static_cast<float>(v.y));
-    }
-    __syncthreads();
     if (threadIdx.x < 32) {
       const int k = threadIdx.x;
+      double2 v = joined[min(k, count - 1)];
+      v.y *= rstd;  // of du (x - mean) to du xhat
+      if (k < count) {
+        if (p.samples > 1) p.channel[static_cast<long long>(sample) * p.l.channels + c0 + k] = v;
+        if (dbias) dbias[c0 + k] = from_float<T>(static_cast<float>(v.x));
+        if (dweight) dweight[c0 + k] = from_float<T>(static_cast<float>(v.y));
+      }
       const double w =
-          k >= count ? 0.0
-                     : p.weight ? to_float(static_cast<const T*>(p.weight)[c0 + k]) : 1.0;
-      m1 += warp_sum(k < count ? w * joined[k].x : 0.0);
-      m2 += warp_sum(k < count ? w * joined[k].y : 0.0);
+          k < count && p.weight ? to_float(static_cast<const T*>(p.weight)[c0 + k]) : 1.0;
+      m1 += warp_sum(k < count ? w * v.x : 0.0);
+      m2 += warp_sum(k < count ? w * v.y : 0.0);
     }
     __syncthreads();
   }
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0) mine[0] = m1, mine[1] = m2;
+  cluster_sync();
+  if (rank == 0 && threadIdx.x == 0) {
+    for (int r = 1; r < blocks; ++r) {
+      m1 += load_cluster(mine, r);
+      m2 += load_cluster(mine + 1, r);
+    }
     const double n = static_cast<double>(p.l.span / p.l.channels) * p.group_channels;
-    p.moments[blockIdx.x] = make_float2(static_cast<float>(m1 / n), static_cast<float>(m2 / n));
+    p.moments[group] = make_float2(static_cast<float>(m1 / n), static_cast<float>(m2 / n));
   }
+  cluster_sync();  // no block leaves while its sums are read
 }
 
 // dw and db: the samples' channel sums added in order.
@@ -560,7 +610,7 @@ __global__ void norm_parameters_kernel(const NormParams p, T* dweight, T* dbias)
 }
 
 template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kMaxThreads, 3) norm_backward_apply_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kMaxThreads, 1) norm_backward_apply_kernel(const NormParams p) {
   using Values = Vec<T, V>;
   const Layout& l = p.l;
   const Place at = place<V>(l);
@@ -579,7 +629,7 @@ __global__ void __launch_bounds__(kMaxThreads, 3) norm_backward_apply_kernel(con
   if (at.left)
     store_part<T, V>(to, result(load_part<T, V>(from, at.left), load_part<T, V>(grad, at.left)),
                      at.left);
-  constexpr int U = 2;
+  constexpr int U = 4;
   int i = at.count;
   for (; i >= U; i -= U) {
     Values v[U], g[U];
@@ -613,31 +663,9 @@ __global__ void __launch_bounds__(kMaxThreads, 3) norm_backward_apply_kernel(con
 // group's moments for itself.  For 37x53x35 fp32 (274 KB) 3 launches and
 // 12 us of device time become one of 6 us.
 
-constexpr int kMaxCluster = 8;
+constexpr int kSmallThreads = 256;
 constexpr int kSmallBytes = 64 * 1024;   // of a block's values
 constexpr int kSmallChannels = 1024;
-
-SPLAT_DEV uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
-  return r;
-}
-SPLAT_DEV void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-// A pair in the shared memory of another block of the cluster, at the address
-// that it has in this one.
-SPLAT_DEV float2 load_cluster(const float2* own, uint32_t rank) {
-  const uint32_t here = static_cast<uint32_t>(__cvta_generic_to_shared(own));
-  uint32_t there;
-  float2 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(rank));
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
-               : "=f"(v.x), "=f"(v.y)
-               : "r"(there)
-               : "memory");
-  return v;
-}
 
 // Sums the threads' sums over the block and then over the cluster; all blocks
 // end with the sample's sums per channel in `channel`.
@@ -695,7 +723,7 @@ size_t small_bytes(const Layout& l, int v, int value_bytes, int groups, int arra
 }
 
 template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kMaxThreads) norm_small_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kSmallThreads) norm_small_kernel(const NormParams p) {
   using Values = Vec<T, V>;
   extern __shared__ __align__(16) unsigned char shared[];
   const Layout& l = p.l;
@@ -782,7 +810,7 @@ __global__ void __launch_bounds__(kMaxThreads) norm_small_kernel(const NormParam
 }
 
 template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kMaxThreads)
+__global__ void __launch_bounds__(kSmallThreads)
     norm_backward_small_kernel(const NormParams p, T* dweight, T* dbias) {
   using Values = Vec<T, V>;
   extern __shared__ __align__(16) unsigned char shared[];
@@ -891,18 +919,19 @@ int vector_width(int value_bytes, int samples, long long span) {
   return v;
 }
 
-Layout make_layout(int samples, long long positions, int channels, int v, int per_sm) {
+Layout make_layout(int samples, long long positions, int channels, int v, int per_sm,
+                   int threads) {
   Layout l;
   l.span = positions * channels;
   l.channels = channels;
   l.period = channels / std::gcd(channels, v);
-  if (l.period <= kMaxThreads) {
-    l.threads = l.period * std::max(1, kMaxThreads / l.period);
+  if (l.period <= threads) {
+    l.threads = l.period * std::max(1, threads / l.period);
     l.columns = 1;
     l.step = l.threads;
   } else {
-    l.threads = kMaxThreads;
-    l.columns = (l.period + kMaxThreads - 1) / kMaxThreads;
+    l.threads = threads;
+    l.columns = (l.period + threads - 1) / threads;
     l.step = l.period;
   }
   const long long vectors = (l.span + v - 1) / v;
@@ -918,7 +947,7 @@ Layout make_layout(int samples, long long positions, int channels, int v, int pe
 }
 
 // As many as the kernels' registers let share an SM.
-constexpr int kForwardBlocksPerSm = 4, kBackwardBlocksPerSm = 3;
+constexpr int kForwardBlocksPerSm = 2, kBackwardBlocksPerSm = 1;
 
 // How a call is run: in clusters of l.blocks (small), or in passes.
 struct Plan {
@@ -932,13 +961,15 @@ Plan make_plan(int value_bytes, int samples, long long positions, int channels, 
                bool backward) {
   Plan plan;
   plan.vector = vector_width(value_bytes, samples, positions * channels);
-  plan.l = make_layout(samples, positions, channels, plan.vector,
-                       backward ? kBackwardBlocksPerSm : kForwardBlocksPerSm);
+  const int per_sm = backward ? kBackwardBlocksPerSm : kForwardBlocksPerSm;
   const long long bytes = positions * channels * value_bytes * (backward ? 2 : 1);
+  plan.l = make_layout(samples, positions, channels, plan.vector, per_sm, kSmallThreads);
   plan.small = plan.l.columns == 1 && channels <= kSmallChannels &&
                bytes <= static_cast<long long>(kMaxCluster) * kSmallBytes;
   plan.shared_bytes = 0;
-  if (plan.small) {
+  if (!plan.small) {
+    plan.l = make_layout(samples, positions, channels, plan.vector, per_sm, kMaxThreads);
+  } else {
     // 8 KB to a block at least, where the sample has them
     int blocks = 1;
     while (blocks < kMaxCluster && blocks * 8192LL < bytes && blocks < plan.l.steps) blocks *= 2;
@@ -949,25 +980,36 @@ Plan make_plan(int value_bytes, int samples, long long positions, int channels, 
   return plan;
 }
 
-// Launches a small sample's kernel as clusters of `blocks`.
-template <auto* kernel, class... A>
-int launch_cluster(const Plan& plan, int samples, cudaStream_t s, A... args) {
-  if (!host::allow_shared<kernel>())
-    return host::check_launch("feature_norm: shared memory");
+template <class... A, class... B>
+int launch_cluster(void (*kernel)(A...), unsigned grid, int threads, int blocks,
+                   size_t shared_bytes, cudaStream_t s, B... args) {
   cudaLaunchAttribute cluster;
   cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = plan.l.blocks;
+  cluster.val.clusterDim.x = blocks;
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(samples) * plan.l.blocks);
-  config.blockDim = dim3(plan.l.threads);
-  config.dynamicSmemBytes = plan.shared_bytes;
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = shared_bytes;
   config.stream = host::counted(s);
   config.attrs = &cluster;
   config.numAttrs = 1;
   if (cudaLaunchKernelEx(&config, kernel, args...) != cudaSuccess)
     return host::check_launch("feature_norm");
   return kOk;
+}
+
+// A small sample's kernel, as clusters of the layout's blocks.
+template <auto* kernel, class... A>
+int launch_small(const Plan& plan, int samples, cudaStream_t s, A... args) {
+  if (!host::allow_shared<kernel>()) return host::check_launch("feature_norm: shared memory");
+  return launch_cluster(kernel, static_cast<unsigned>(samples) * plan.l.blocks, plan.l.threads,
+                        plan.l.blocks, plan.shared_bytes, s, args...);
+}
+
+// Blocks that join a group's channels.
+int join_blocks(int group_channels) {
+  return std::min(kMaxCluster, (group_channels + kJoinChannels - 1) / kJoinChannels);
 }
 
 template <int V, class F>
@@ -1061,10 +1103,14 @@ int splat_feature_norm(int dtype, int samples, long long positions, int channels
       constexpr int V = decltype(width)::value;
       if (plan.small)
         return SPLAT_FEATURE_ACT(activation, [&] {
-          return launch_cluster<norm_small_kernel<T, V, ACT>>(plan, samples, s, p);
+          return launch_small<norm_small_kernel<T, V, ACT>>(plan, samples, s, p);
         });
       norm_sums_kernel<T, V><<<grid, p.l.threads, 0, host::counted(s)>>>(p);
-      norm_join_kernel<T><<<samples * groups, kJoinThreads, 0, host::counted(s)>>>(p);
+      const int joins = join_blocks(p.group_channels);
+      const int status = launch_cluster(norm_join_kernel<T>,
+                                        static_cast<unsigned>(samples) * groups * joins,
+                                        kJoinThreads, joins, 0, s, p, joins);
+      if (status != kOk) return status;
       return SPLAT_FEATURE_ACT(activation, [&] {
         norm_apply_kernel<T, V, ACT><<<grid, p.l.threads, 0, host::counted(s)>>>(p);
         return host::check_launch("feature_norm");
@@ -1120,13 +1166,16 @@ int splat_feature_norm_backward(int dtype, int samples, long long positions, int
         const bool one = samples == 1;
         T *dw1 = one ? dw : nullptr, *db1 = one ? db : nullptr;
         if (plan.small) {
-          const int status = launch_cluster<norm_backward_small_kernel<T, V, ACT>>(
+          const int status = launch_small<norm_backward_small_kernel<T, V, ACT>>(
               plan, samples, s, p, dw1, db1);
           if (status != kOk) return status;
         } else {
           norm_backward_sums_kernel<T, V, ACT><<<grid, p.l.threads, 0, host::counted(s)>>>(p);
-          norm_backward_join_kernel<T>
-              <<<samples * groups, kJoinThreads, 0, host::counted(s)>>>(p, dw1, db1);
+          const int joins = join_blocks(p.group_channels);
+          const int status = launch_cluster(norm_backward_join_kernel<T>,
+                                            static_cast<unsigned>(samples) * groups * joins,
+                                            kJoinThreads, joins, 0, s, p, joins, dw1, db1);
+          if (status != kOk) return status;
         }
         if (!one && (dw || db))
           norm_parameters_kernel<T>
