@@ -38,10 +38,11 @@ bool make_map(CUtensorMap& map, const void* base, long long rows, long long colu
                                                          : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-// Shared memory of a block when one or two share an SM (228 KB, of which each
-// block costs 1 KB besides its own), less the barriers and the rounding of the
-// base to 1 KB.
-constexpr int kOneBlockBytes = 225 * 1024, kTwoBlocksBytes = 110 * 1024;
+// Shared memory of a block when one, two or three share an SM (228 KB, of which
+// each block costs 1 KB besides its own), less the barriers and the rounding
+// of the base to 1 KB.
+constexpr int kOneBlockBytes = 225 * 1024, kTwoBlocksBytes = 110 * 1024,
+              kThreeBlocksBytes = 73 * 1024;
 constexpr int kMaxSharedBias = 4096;  // values
 constexpr long long kFewRows = 1024;
 constexpr int kMaxResidentBytes = 128 * 1024;
@@ -109,6 +110,10 @@ int launch_product(ProductParams p, cudaStream_t s) {
     if (fixed + 2 * stage + 2 * raw > budget && blocks == 2) blocks = 1, budget = kOneBlockBytes;
     if (fixed + 2 * stage + 2 * raw <= budget) p.raw_bytes = static_cast<int>(raw);
   }
+  // blocks without register-filling producers are small enough for three
+  if (p.copy_operands && blocks == 2 && 3 * p.tmem_columns <= 512 &&
+      fixed + 2 * stage <= kThreeBlocksBytes)
+    blocks = 3, budget = kThreeBlocksBytes;
   p.stages = std::min(kMaxStages, (budget - fixed - 2 * p.raw_bytes) / stage);
   if (p.stages < 1) return host::fail(kTooLarge, "feature_linear: no room for a stage");
   if (EPI != kPlain) p.copy_extra = make_map<TE>(p.extra_map, p.extra, p.m, p.n, p.n, 32, 32);
@@ -121,8 +126,10 @@ int launch_product(ProductParams p, cudaStream_t s) {
   constexpr auto* kernel = product_kernel<SA, PA, AMN, SB, PB, BMN, TE, TO, EPI>;
   if (!host::allow_shared<kernel>())
     return host::check_launch("feature_linear: shared memory");
-  const long long grid = std::min<long long>(p.tiles, static_cast<long long>(host::sm_count()) * blocks);
-  kernel<<<static_cast<unsigned>(grid), kEpilogueWarps * 32 + producers(PA, PB) + 32, bytes, host::counted(s)>>>(p);
+  const long long grid =
+      std::min<long long>(p.tiles, static_cast<long long>(host::sm_count()) * blocks);
+  const int threads = kEpilogueWarps * 32 + (p.copy_operands ? 32 : producers(PA, PB)) + 32;
+  kernel<<<static_cast<unsigned>(grid), threads, bytes, host::counted(s)>>>(p);
   return host::check_launch("feature_linear");
 }
 

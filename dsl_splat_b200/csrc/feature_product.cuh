@@ -559,8 +559,8 @@ struct ProductTile {
 };
 
 template <class SA, int PA, bool AMN, class SB, int PB, bool BMN, class TE, class TO, int EPI>
-__global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
-                                  producers(PA, PB) == 128 ? 2 : 1)
+__global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
+                                  producers(PA, PB) == 128 ? 2 : 1)  // 64 and 120 registers
     product_kernel(const __grid_constant__ ProductParams p) {
   constexpr int kProducers = producers(PA, PB), kAcc = accumulators(PA, PB);
   extern __shared__ unsigned char dynamic[];
@@ -577,6 +577,8 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
   const uint32_t ring = resident + (p.resident ? chunks_all * b_bytes : 0);
   const uint32_t stage_bytes = a_bytes + (p.resident ? 0 : b_bytes);
   const int warp = tc::uniform(threadIdx.x >> 5);
+  // copies need no more than one producer warp
+  const int product_warp = kEpilogueWarps + (p.copy_operands ? 1 : kProducers / 32);
 
   if (threadIdx.x == 0) {
     const int arrivals = p.copy_operands ? 1 : kProducers;
@@ -612,7 +614,7 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
   const uint32_t tmem = tc::uniform(tmem_base);
   bool ok = true;
 
-  if (warp >= kEpilogueWarps && warp < kEpilogueWarps + kProducers / 32) {
+  if (warp >= kEpilogueWarps && warp < product_warp) {
     // ---- producers
     const int thread = threadIdx.x - kEpilogueWarps * 32;
     int stage = 0;
@@ -720,7 +722,7 @@ __global__ void __launch_bounds__(kEpilogueWarps * 32 + producers(PA, PB) + 32,
       for (uint32_t j = started < 2 ? 0 : started - 2; j < started; ++j)
         ok = tc::barrier_wait(tc::shared_address(&raw_full[j & 1]), (j >> 1) & 1) && ok;
     }
-  } else if (warp == kEpilogueWarps + kProducers / 32) {
+  } else if (warp == product_warp) {
     // ---- one warp issues the products
     {
       const uint32_t lead = tc::elected();
