@@ -80,10 +80,13 @@ int launch_product(ProductParams p, cudaStream_t s) {
   const int b_bytes = PB * b_plane_bytes<BMN>(p.tile_n), a_bytes = PA * kAPlane;
   const long long chunks = (p.k + kChunk - 1) / kChunk;
   const long long whole_b = chunks * b_bytes;
-  p.resident = p.splits == 1 && p.tiles_n == 1 && whole_b <= kMaxResidentBytes;
   // a patch of results, and one of the extra values
   p.staging = 1024 * static_cast<int>(sizeof(TO) + (p.extra ? sizeof(TE) : 0));
-  const int fixed = kEpilogueWarps * p.staging + (p.bias_shared * 4 + 1023) / 1024 * 1024 + (p.resident ? static_cast<int>(whole_b) : 0);
+  int fixed = kEpilogueWarps * p.staging + (p.bias_shared * 4 + 1023) / 1024 * 1024;
+  // B stays where two stages of A fit beside it
+  p.resident = p.splits == 1 && p.tiles_n == 1 && whole_b <= kMaxResidentBytes &&
+               fixed + whole_b + 2 * a_bytes <= kOneBlockBytes;
+  if (p.resident) fixed += static_cast<int>(whole_b);
   const int stage = a_bytes + (p.resident ? 0 : b_bytes);
   int blocks = 2, budget = kTwoBlocksBytes;
   if (producers(PA, PB) > 128 || p.tmem_columns > 256 || fixed + 2 * stage > budget)

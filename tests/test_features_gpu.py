@@ -135,6 +135,33 @@ def test_linear_sizes(m, k, n, dtype):
     linear_case(m, k, n, dtype, "silu", residual=True)
 
 
+# rows enough for several tiles of a block, and for operands laid out before
+# the products (1024): aligned and odd widths on either side of 64, 128 and 256
+MANY_ROWS = [(1024, 300, 17), (1500, 35, 300), (2001, 129, 130), (1300, 520, 264),
+             (1100, 264, 520), (50001, 40, 3), (60000, 33, 20), (120001, 64, 64),
+             (70001, 35, 64), (70000, 64, 35), (50000, 128, 128), (40000, 100, 72),
+             (30001, 96, 128), (4096, 256, 256), (9000, 16, 200)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m, k, n", MANY_ROWS)
+def test_linear_many_rows(m, k, n, dtype):
+    linear_case(m, k, n, dtype, "gelu", residual=True, seed=20)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m, k, n", [(3000, 300, 200), (3000, 301, 37), (70000, 48, 32)])
+def test_linear_many_rows_without_activation(m, k, n, dtype):
+    linear_case(m, k, n, dtype, "none", seed=21)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_very_wide(dtype):
+    """A bias of more values than a block keeps, and thousands of inputs."""
+    linear_case(40, 24, 5003, dtype, "silu", seed=22)
+    linear_case(40, 5003, 24, dtype, "silu", seed=23)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("bias, residual", [(True, False), (False, True), (False, False)])
@@ -156,6 +183,50 @@ def test_linear_single_gradients(dtype):
         grads = [None] * 3
         grads[which], = torch.autograd.grad(y, leaves[which], dy)
         check_linear(x, w, b, None, "gelu", y.detach(), grads, dy)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k, n", [(24, 40), (300, 200), (301, 33)])
+def test_linear_any_subset_of_gradients(k, n, dtype):
+    """Each subset's gradients are those of the whole set."""
+    normal = draws(24)
+    tensors = [normal(*s, dtype=dtype) for s in ((1200, k), (n, k), (n,), (1200, n))]
+    dy = normal(1200, n, dtype=dtype)
+
+    def grads(which):
+        leaves = [t.detach().clone().requires_grad_(i in which) for i, t in enumerate(tensors)]
+        y = features.linear(leaves[0], leaves[1], leaves[2], residual=leaves[3],
+                            activation="silu")
+        return dict(zip(which, torch.autograd.grad(y, [leaves[i] for i in which], dy)))
+
+    whole = grads((0, 1, 2, 3))
+    for which in ((0,), (1,), (2,), (3,), (0, 1), (1, 2), (0, 3)):
+        for i, g in grads(which).items():
+            assert torch.equal(g, whole[i])
+
+
+def test_no_second_derivative():
+    x = torch.ones(4, 8, device="cuda", requires_grad=True)
+    w = torch.ones(8, 8, device="cuda", requires_grad=True)
+    for y in (features.linear(x, w, activation="gelu"),
+              features.group_norm(x, 2, spatial_dims=1)):
+        g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_residual_is_the_input(dtype):
+    normal = draws(25)
+    x, w = normal(130, 32, dtype=dtype), normal(32, 32, dtype=dtype)
+    dy = normal(130, 32, dtype=dtype)
+    leaf = x.clone().requires_grad_()
+    y = features.linear(leaf, w, residual=leaf, activation="silu")
+    both, = torch.autograd.grad(y, leaf, dy)
+    apart = [x.clone().requires_grad_() for _ in range(2)]
+    y = features.linear(apart[0], w, residual=apart[1], activation="silu")
+    dx, dr = torch.autograd.grad(y, apart, dy)
+    assert torch.equal(both, dx + dr)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -264,6 +335,17 @@ def test_linear_long_rows():
     assert not y[:-5].any()
 
 
+def test_linear_more_rows_than_an_int():
+    """2^31 + 300 rows of one value."""
+    rows = (1 << 31) + 300
+    x = torch.zeros(rows, 1, device="cuda", dtype=torch.bfloat16)
+    x[-3:, 0] = torch.tensor([1.0, -2.0, 3.0])
+    w = torch.full((1, 1), 2.0, device="cuda", dtype=torch.bfloat16)
+    y = features.linear(x, w)
+    assert y[-3:, 0].tolist() == [2.0, -4.0, 6.0]
+    assert not y[:-3].any()
+
+
 # ---- group norm ----------------------------------------------------------------
 
 def norm_case(shape, groups, dtype, act, affine=True, spatial_dims=2, shift=0.0, seed=0):
@@ -339,7 +421,9 @@ NORM_SHAPES = [((1, 1, 1, 4), 2), ((1, 1, 1, 1), 1), ((2, 3, 5, 8), 8), ((1, 37,
                ((3, 17, 19, 35), 7), ((2, 16, 16, 32), 4), ((1, 100, 90, 64), 1),
                ((2, 31, 33, 48), 4), ((5, 8, 9, 6), 3), ((1, 9, 9, 1031), 1),
                ((1, 5, 7, 2050), 2), ((4, 2, 2, 512), 32), ((300, 2, 1, 8), 2),
-               ((2, 120, 160, 24), 8), ((1, 200, 300, 3), 1)]
+               ((2, 120, 160, 24), 8), ((1, 200, 300, 3), 1), ((1, 301, 211, 35), 5),
+               ((2, 300, 200, 35), 7), ((1, 150, 130, 149), 1), ((1, 40, 60, 600), 1),
+               ((3, 90, 110, 66), 2)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
