@@ -18,25 +18,37 @@ namespace feature {
 
 // ---- sums over splits and rows ---------------------------------------------------
 
-// Adds the splits' partial sums, `stride` values apart, in a fixed order: 8
+// Adds the splits' partial sums, `stride` values apart, in a fixed order: 32
 // threads to a value.  The first count_a values go to a, the rest to b.
+constexpr int kJoinLanes = 32;
 template <class T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(32 * kJoinLanes)
     join_splits_kernel(const float* partial, long long stride, int splits, long long count_a,
                        long long count_b, T* a, T* b) {
   const long long i = blockIdx.x * 32LL + threadIdx.x, count = count_a + count_b;
   float s = 0.0f;
   if (i < count) {
-#pragma unroll 4
-    for (int k = threadIdx.y; k < splits; k += 8) s += partial[k * stride + i];
+    constexpr int U = 8;  // reads in flight
+    for (int k0 = threadIdx.y; k0 < splits; k0 += U * kJoinLanes) {
+      float v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        v[u] = k0 + u * kJoinLanes < splits ? partial[(k0 + u * kJoinLanes) * stride + i] : 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) s += v[u];
+    }
   }
-  __shared__ float sums[8][32];
+  __shared__ float sums[kJoinLanes][33];
   sums[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
-  if (threadIdx.y == 0 && i < count) {
-    for (int k = 1; k < 8; ++k) s += sums[k][threadIdx.x];
-    T* to = i < count_a ? a : b;
-    if (to) to[i < count_a ? i : i - count_a] = from_float<T>(s);
+  // a warp to a value, its lanes' sums in a fixed tree
+  s = sums[threadIdx.x][threadIdx.y];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const long long j = blockIdx.x * 32LL + threadIdx.y;
+  if (threadIdx.x == 0 && j < count) {
+    T* to = j < count_a ? a : b;
+    if (to) to[j < count_a ? j : j - count_a] = from_float<T>(s);
   }
 }
 
@@ -69,7 +81,7 @@ void join_splits(const float* partial, long long stride, int splits, long long c
     return;
   }
   join_splits_kernel<T>
-      <<<host::blocks_for(count_a + count_b, 32), dim3(32, 8), 0, host::counted(s)>>>(
+      <<<host::blocks_for(count_a + count_b, 32), dim3(32, kJoinLanes), 0, host::counted(s)>>>(
           partial, stride, splits, count_a, count_b, static_cast<T*>(a), static_cast<T*>(b));
 }
 
