@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
   const int product_warp = kEpilogueWarps + (p.copy_operands ? 1 : kProducers / 32);
 
   if (threadIdx.x == 0) {
-    const int arrivals = p.copy_operands ? 1 : kProducers;
+    const int arrivals = p.copy_operands ? 1 : p.raw_bytes ? kProducers / 2 : kProducers;
     for (int i = 0; i < kEpilogueWarps; ++i)
       tc::barrier_init(tc::shared_address(&extra_full[i]), 1);
     for (int i = 0; i < p.stages; ++i) {
@@ -590,14 +590,14 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
     }
     for (int i = 0; i < 2; ++i) {
       tc::barrier_init(tc::shared_address(&raw_full[i]), 1);
-      tc::barrier_init(tc::shared_address(&raw_read[i]), kProducers);
+      tc::barrier_init(tc::shared_address(&raw_read[i]), kProducers / 2);
     }
     for (int i = 0; i < p.accumulators; ++i) {
       tc::barrier_init(tc::shared_address(&acc_full[i]), 1);
       tc::barrier_init(tc::shared_address(&acc_empty[i]),
                        kEpilogueWarps * (p.alternate ? 16 : 32));
     }
-    tc::barrier_init(tc::shared_address(&resident_full), arrivals);
+    tc::barrier_init(tc::shared_address(&resident_full), p.copy_operands ? 1 : kProducers);
     tc::barrier_init(tc::shared_address(&drained), 1);
     tc::barrier_init_fence();
   }
@@ -666,61 +666,79 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
         tc::fence_async_proxy();
         tc::barrier_arrive(tc::shared_address(&resident_full));
       }
-      // the tiles of A by bulk copies, two ahead
-      const uint32_t raw_at = ring + p.stages * stage_bytes;
-      const int row_bytes = static_cast<int>(p.k) * static_cast<int>(sizeof(SA));
-      const auto copy_tile = [&](uint32_t t, uint32_t buffer) {
-        const long long m0 = ProductTile(p, t).m0;
-        copy_run<SA>(raw_at + buffer * p.raw_bytes, a + m0 * p.k,
-                     static_cast<int>(min(p.m - m0, static_cast<long long>(kTileRows)) * p.k),
-                     tc::shared_address(&raw_full[buffer]));
-      };
-      uint32_t started = 0;  // copies, by thread 0
-      if (!AMN && p.raw_bytes && thread == 0)
-        for (; started < 2 && blockIdx.x + started * gridDim.x < p.tiles; ++started)
-          copy_tile(blockIdx.x + started * gridDim.x, started);
-      uint32_t i = 0;
-      for (uint32_t t = blockIdx.x; t < p.tiles && ok; t += gridDim.x, ++i) {
-        const ProductTile tile(p, t);
-        const uint32_t buffer = i & 1;
-        if (!AMN && p.raw_bytes &&
-            !(ok = tc::barrier_wait(tc::shared_address(&raw_full[buffer]), (i >> 1) & 1)))
-          break;
-        for (long long k = tile.k0; k < tile.k1; k += kChunk) {
-          if (!(ok = tc::barrier_wait(tc::shared_address(&empty[stage]), parity))) break;
-          const uint32_t at = ring + stage * stage_bytes;
-          const int k_valid = static_cast<int>(min(tile.k1 - k, static_cast<long long>(kChunk)));
-          if (!AMN && p.raw_bytes)
+      if (!AMN && p.raw_bytes) {
+        // two groups of producers take turns at the tiles, whose fixed costs
+        // (waits, the proxy fence) then overlap; each has a buffer of its own,
+        // which bulk copies fill while the other group converts
+        constexpr int kGroup = kProducers / 2;
+        const int group = thread / kGroup, own = thread % kGroup;
+        const uint32_t raw_at = ring + p.stages * stage_bytes + group * p.raw_bytes;
+        const uint32_t raw_bar = tc::shared_address(&raw_full[group]);
+        const uint32_t read_bar = tc::shared_address(&raw_read[group]);
+        const int row_bytes = static_cast<int>(p.k) * static_cast<int>(sizeof(SA));
+        uint32_t copied = 0;  // tiles, by the group's first thread
+        const auto copy_tile = [&](uint32_t t) {
+          const long long m0 = ProductTile(p, t).m0;
+          copy_run<SA>(raw_at, a + m0 * p.k,
+                       static_cast<int>(min(p.m - m0, static_cast<long long>(kTileRows)) * p.k),
+                       raw_bar);
+          ++copied;
+        };
+        const auto advance = [&](int stages) {
+          for (stage += stages; stage >= p.stages; stage -= p.stages) parity ^= 1;
+        };
+        const uint32_t step = 2 * gridDim.x, first = blockIdx.x + group * gridDim.x;
+        if (own == 0 && first < p.tiles) copy_tile(first);
+        advance(group * chunks_all);
+        uint32_t round = 0;
+        for (uint32_t t = first; t < p.tiles && ok; t += step, round ^= 1) {
+          const ProductTile tile(p, t);
+          const int rows =
+              static_cast<int>(min(p.m - tile.m0, static_cast<long long>(kTileRows)));
+          if (!(ok = tc::barrier_wait(raw_bar, round))) break;
+          for (int c = 0; c < chunks_all; ++c) {
+            if (!(ok = tc::barrier_wait(tc::shared_address(&empty[stage]), parity))) break;
+            const uint32_t at = ring + stage * stage_bytes;
+            const int k_valid = min(static_cast<int>(p.k) - c * kChunk, kChunk);
             fill_shared<SA, PA>(p.a_vector, at, kAPlane, kTileRows,
                                 min((k_valid + 15) / 16 * 2, 8),
-                                raw_at + buffer * p.raw_bytes +
-                                    static_cast<int>(k) * static_cast<int>(sizeof(SA)),
-                                row_bytes,
-                                static_cast<int>(min(p.m - tile.m0, static_cast<long long>(kTileRows))),
-                                k_valid, thread, kProducers);
-          else
+                                raw_at + c * kChunk * static_cast<int>(sizeof(SA)), row_bytes,
+                                rows, k_valid, own, kGroup);
+            if (!p.resident)
+              fill_chunk<SB, PB, BMN>(p.b_vector, at + a_bytes, b_plane, p.tile_n, b, p.b_ld,
+                                      tile.n0, p.n - tile.n0, c * kChunk, k_valid, own, kGroup);
+            tc::fence_async_proxy();
+            tc::barrier_arrive(tc::shared_address(&full[stage]));
+            advance(1);
+          }
+          if (!ok) break;
+          tc::barrier_arrive(read_bar);
+          if (own == 0 && p.tiles - t > step) {
+            if (!(ok = tc::barrier_wait(read_bar, round))) break;
+            copy_tile(t + step);
+          }
+          advance(chunks_all);  // the other group's tile
+        }
+        // no copy is in flight past this point, also after a wait that ran out
+        if (copied) ok = tc::barrier_wait(raw_bar, (copied - 1) & 1) && ok;
+      } else {
+        for (uint32_t t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+          const ProductTile tile(p, t);
+          for (long long k = tile.k0; k < tile.k1; k += kChunk) {
+            if (!(ok = tc::barrier_wait(tc::shared_address(&empty[stage]), parity))) break;
+            const uint32_t at = ring + stage * stage_bytes;
+            const int k_valid = static_cast<int>(min(tile.k1 - k, static_cast<long long>(kChunk)));
             fill_chunk<SA, PA, AMN>(p.a_vector, at, kAPlane, kTileRows, a, p.a_ld, tile.m0,
                                     p.m - tile.m0, k, k_valid, thread, kProducers);
-          if (!p.resident)
-            fill_chunk<SB, PB, BMN>(p.b_vector, at + a_bytes, b_plane, p.tile_n, b, p.b_ld,
-                                    tile.n0, p.n - tile.n0, k, k_valid, thread, kProducers);
-          tc::fence_async_proxy();
-          tc::barrier_arrive(tc::shared_address(&full[stage]));
-          if (++stage == p.stages) stage = 0, parity ^= 1;
-        }
-        if (!AMN && p.raw_bytes && ok) {
-          const uint32_t read = tc::shared_address(&raw_read[buffer]);
-          tc::barrier_arrive(read);
-          if (thread == 0 && p.tiles - t > 2ull * gridDim.x) {
-            if (!(ok = tc::barrier_wait(read, (i >> 1) & 1))) break;
-            copy_tile(t + 2 * gridDim.x, buffer);
-            ++started;
+            if (!p.resident)
+              fill_chunk<SB, PB, BMN>(p.b_vector, at + a_bytes, b_plane, p.tile_n, b, p.b_ld,
+                                      tile.n0, p.n - tile.n0, k, k_valid, thread, kProducers);
+            tc::fence_async_proxy();
+            tc::barrier_arrive(tc::shared_address(&full[stage]));
+            if (++stage == p.stages) stage = 0, parity ^= 1;
           }
         }
       }
-      // no copy is in flight past this point, also after a wait that ran out
-      for (uint32_t j = started < 2 ? 0 : started - 2; j < started; ++j)
-        ok = tc::barrier_wait(tc::shared_address(&raw_full[j & 1]), (j >> 1) & 1) && ok;
     }
   } else if (warp == product_warp) {
     // ---- one warp issues the products
