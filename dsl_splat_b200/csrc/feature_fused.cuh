@@ -14,6 +14,8 @@
 // and dy (contiguous whatever their row lengths) to shared memory; where those
 // do not fit beside the operands, the steps read global memory.
 // 16-bit types with 16-byte rows take the pass of feature_narrow.cuh instead.
+// Bound by the steps' latencies one after another: 35 -> 32 fp32 gelu over 10^6
+// rows 370 us where 408 MB take 62 us to copy.
 #pragma once
 #include "feature_product.cuh"
 
@@ -27,13 +29,19 @@ struct FusedParams {
   void* dx;        // (rows, k) or NULL
   float* partial;  // per block: (n, k) of dW, then (n) of db; NULL: neither
   int activation, x_vector, w_vector, dy_vector, dx_vector;
-  int raw;  // x and dy are copied ahead
+  // x and dy are copied ahead (training of 35 -> 64 bf16 over 10^6 rows 222 us
+  // against 250 read as needed, 35 -> 32 fp32 450 against 490)
+  int raw;
   uint32_t tiles, tmem_columns;
   int* error;
 };
 
 constexpr int kFusedThreads = 512, kFusedWarps = kFusedThreads / 32;
-constexpr int kFusedWidth = 128;        // widest k and n
+// Widest k and n: what fits in shared memory there is faster in one pass
+// (training over 500000 rows against the products: 64 -> 64 bf16 147 us against
+// 197, 128 -> 128 bf16 175 against 309, 64 -> 64 fp32 275 against 460, 128 -> 64
+// fp32 637 against 636).
+constexpr int kFusedWidth = 128;
 constexpr int kOnesBytes = 16 * 128;    // 16 rows of 64 ones
 
 template <class T>

@@ -44,15 +44,16 @@ bool make_map(CUtensorMap& map, const void* base, long long rows, long long colu
 constexpr int kOneBlockBytes = 225 * 1024, kTwoBlocksBytes = 110 * 1024,
               kThreeBlocksBytes = 73 * 1024;
 constexpr int kMaxSharedBias = 4096;  // values
-constexpr long long kFewRows = 1024;
+constexpr long long kFewRows = 16384;
 constexpr int kMaxResidentBytes = 128 * 1024;
 
 // Fills in the tiling of p (its sources, sizes and epilogue set) and launches.
 template <class SA, int PA, bool AMN, class SB, int PB, bool BMN, class TE, class TO, int EPI>
 int launch_product(ProductParams p, cudaStream_t s) {
-  // a plain product's tiles are as wide as they can be; one with arithmetic
-  // behind it is faster with two blocks' epilogues on an SM (512 -> 512 fp16
-  // gelu over 131072 rows: see the sizes in the measurements)
+  // a plain product's tiles are as wide as they can be; behind one with
+  // arithmetic two blocks' epilogues share an SM (512 -> 512 fp16 gelu over
+  // 131072 rows 103 us against 107 in 256-wide tiles, 256 -> 256 bf16 silu 39
+  // against 48)
   const int widest = PA == 1 && PB == 1 && EPI == kPlain ? 256 : 128;
   p.tiles_n = (p.n + widest - 1) / widest;
   p.tile_n = ((p.n + p.tiles_n - 1) / p.tiles_n + 31) / 32 * 32;
@@ -73,6 +74,8 @@ int launch_product(ProductParams p, cudaStream_t s) {
   // sums of several accumulators are joined in fp32 outputs; an operand row of
   // more values than kExactSum is summed in one
   p.k_per_sum = kAcc == 2 && EPI == kPlain && sizeof(TO) == 4 ? kExactSum : p.k_per_split;
+  // (35 -> 32 fp32 gelu over 10^6 rows 113 us against 154 without, 32 -> 3 bf16
+  // over 1.9 10^6 67 against 84, 64 -> 32 bf16 71 against 69)
   p.alternate = p.tile_n == 32 && p.k_per_sum >= p.k_per_split;
   p.accumulators = p.alternate ? 4 : 2;
   while (p.tmem_columns < static_cast<uint32_t>(p.accumulators * kAcc * p.tile_n))
@@ -108,12 +111,15 @@ int launch_product(ProductParams p, cudaStream_t s) {
                      BMN ? kChunk : p.tile_n);
   }
   // two tiles of A as they are in memory, where two stages fit beside them
+  // (35 -> 32 fp32 gelu over 10^6 rows 113 us against 140 read as needed,
+  // 35 -> 64 bf16 78 against 82)
   if (!p.copy_operands && !AMN && p.tiles_n == 1 && p.a_ld == p.k && host::aligned(p.a, 16)) {
     const long long raw = (kTileRows * p.k * static_cast<long long>(sizeof(SA)) + 127) / 128 * 128;
     if (fixed + 2 * stage + 2 * raw > budget && blocks == 2) blocks = 1, budget = kOneBlockBytes;
     if (fixed + 2 * stage + 2 * raw <= budget) p.raw_bytes = static_cast<int>(raw);
   }
   // blocks without register-filling producers are small enough for three
+  // (64 -> 64 bf16 with residual over 1.9 10^6 rows 121 us against 137 with two)
   if (p.copy_operands && blocks == 2 && 3 * p.tmem_columns <= 512 &&
       fixed + 2 * stage <= kThreeBlocksBytes)
     blocks = 3, budget = kThreeBlocksBytes;
@@ -140,8 +146,9 @@ int launch_product(ProductParams p, cudaStream_t s) {
 // their own type: rounded to it as x and y are, half a step relative, which is
 // what the result's own rounding costs again (and f16 gradients below 2^-24 or
 // above 65504 leave its range, as dy itself would).  A second part would undo
-// that rounding but doubles the products, and took 20 % more time in the narrow
-// layers' pass and 60 % more in the wide ones' products.
+// that rounding but doubles the products: 64 -> 64 bf16 training over 1.9 10^6
+// rows took 465 us with it and 411 without, 512 -> 512 fp16 over 131072 rows
+// 2021 (of bf16 parts, three products) and 1016.
 template <class T>
 constexpr int kOperandParts = sizeof(T) == 4 ? 3 : 1;
 
@@ -185,7 +192,10 @@ Planes split(const void* src, long long rows, int cols, void* to, cudaStream_t s
 }
 
 // Whether the wide layers' products take planes: fp32 operands, and rows that
-// are not whole 16-byte pieces.  A pass over few rows would cost its launch.
+// are not whole 16-byte pieces.  The pass that makes them pays from about
+// kFewRows on: 300 -> 300 fp32 over 4000, 16000 and 100000 rows 34, 56 and
+// 250 us with planes, 26, 58 and 288 without; 301 -> 200 bf16 over 4000 and
+// 100000 rows 34 and 75 with, 23 and 117 without (trained: 282 against 725).
 template <class T>
 bool wants_planes(long long rows, int k, int n) {
   const int whole = 16 / static_cast<int>(sizeof(T));

@@ -19,6 +19,12 @@
 // which there are two or four, so that loads, products and epilogues of
 // neighbouring tiles overlap.  Where the whole of B fits beside the ring it is
 // loaded once per block.
+//
+// Bound by memory and the epilogue's arithmetic where k and n are small (64 -> 64
+// bf16 with residual over 1600x1200 rows 121 us, 112 us of copying; 32 -> 64 silu
+// 96 us, of which two special-function instructions a value take 55), by how
+// fast operands reach shared memory where they are wide (300 -> 300 fp32 over
+// 200000 rows 400 us for 216 GFLOP of parts: the tensor pipe is busy 34 %).
 #pragma once
 #include <type_traits>
 

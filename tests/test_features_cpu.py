@@ -98,9 +98,9 @@ def test_entry_points_refuse_before_any_launch():
     assert lib.splat_feature_linear(0, 0, 1, 1, P, P, None, None, 0, P, None, 0, None) == -1
     assert lib.splat_feature_linear(0, 1, 1 << 20, 1, P, P, None, None, 0, P, None, 0, None) == -4
     assert lib.splat_feature_linear(0, 1, 1, 1, None, P, None, None, 0, P, None, 0, None) == -1
-    assert lib.splat_feature_linear(0, 5000, 300, 9, P, P, None, None, 0, P, None, 0, None) == -5
-    assert lib.splat_feature_linear_workspace_bytes(0, 5000, 300, 9) > 5000 * 300 * 6
-    assert lib.splat_feature_linear_workspace_bytes(1, 5000, 304, 9) == 16
+    assert lib.splat_feature_linear(0, 50000, 300, 9, P, P, None, None, 0, P, None, 0, None) == -5
+    assert lib.splat_feature_linear_workspace_bytes(0, 50000, 300, 9) > 50000 * 300 * 6
+    assert lib.splat_feature_linear_workspace_bytes(1, 50000, 304, 9) == 16
     assert lib.splat_feature_linear_backward(0, 8, 4, 4, P, P, None, 0, P, P, P, P, P, 0,
                                              None) == -5
     assert lib.splat_feature_linear_backward_workspace_bytes(7, 8, 4, 4, 0) == 0

@@ -136,11 +136,12 @@ def test_linear_sizes(m, k, n, dtype):
 
 
 # rows enough for several tiles of a block, and for operands laid out before
-# the products (1024): aligned and odd widths on either side of 64, 128 and 256
+# the products (16384): aligned and odd widths on either side of 64, 128 and 256
 MANY_ROWS = [(1024, 300, 17), (1500, 35, 300), (2001, 129, 130), (1300, 520, 264),
              (1100, 264, 520), (50001, 40, 3), (60000, 33, 20), (120001, 64, 64),
              (70001, 35, 64), (70000, 64, 35), (50000, 128, 128), (40000, 100, 72),
-             (30001, 96, 128), (4096, 256, 256), (9000, 16, 200)]
+             (30001, 96, 128), (4096, 256, 256), (9000, 16, 200), (17001, 300, 17),
+             (16384, 35, 300), (20000, 129, 130), (16500, 264, 200), (18000, 520, 137)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -150,7 +151,8 @@ def test_linear_many_rows(m, k, n, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("m, k, n", [(3000, 300, 200), (3000, 301, 37), (70000, 48, 32)])
+@pytest.mark.parametrize("m, k, n", [(3000, 300, 200), (3000, 301, 37), (70000, 48, 32),
+                                     (20000, 300, 200), (20000, 301, 37)])
 def test_linear_many_rows_without_activation(m, k, n, dtype):
     linear_case(m, k, n, dtype, "none", seed=21)
 
@@ -186,12 +188,13 @@ def test_linear_single_gradients(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("k, n", [(24, 40), (300, 200), (301, 33)])
-def test_linear_any_subset_of_gradients(k, n, dtype):
+@pytest.mark.parametrize("m, k, n", [(1200, 24, 40), (1200, 300, 200), (1200, 301, 33),
+                                     (17000, 301, 33)])
+def test_linear_any_subset_of_gradients(m, k, n, dtype):
     """Each subset's gradients are those of the whole set."""
     normal = draws(24)
-    tensors = [normal(*s, dtype=dtype) for s in ((1200, k), (n, k), (n,), (1200, n))]
-    dy = normal(1200, n, dtype=dtype)
+    tensors = [normal(*s, dtype=dtype) for s in ((m, k), (n, k), (n,), (m, n))]
+    dy = normal(m, n, dtype=dtype)
 
     def grads(which):
         leaves = [t.detach().clone().requires_grad_(i in which) for i, t in enumerate(tensors)]
@@ -423,7 +426,7 @@ NORM_SHAPES = [((1, 1, 1, 4), 2), ((1, 1, 1, 1), 1), ((2, 3, 5, 8), 8), ((1, 37,
                ((1, 5, 7, 2050), 2), ((4, 2, 2, 512), 32), ((300, 2, 1, 8), 2),
                ((2, 120, 160, 24), 8), ((1, 200, 300, 3), 1), ((1, 301, 211, 35), 5),
                ((2, 300, 200, 35), 7), ((1, 150, 130, 149), 1), ((1, 40, 60, 600), 1),
-               ((3, 90, 110, 66), 2)]
+               ((3, 90, 110, 66), 2), ((2, 80, 80, 32), 8), ((1, 150, 160, 40), 8)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
