@@ -49,6 +49,7 @@ constexpr int kMaxThreads = 512;
 struct NormParams {
   Layout l;
   int samples, groups, group_channels;
+  int keep;  // small samples: the values stay in shared memory, or are read again
   const void* x;
   const void* dy;
   const void* weight;  // (C) or NULL: 1
@@ -657,16 +658,20 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_backward_apply_kernel(con
 
 // ---- small samples: one launch ---------------------------------------------------
 //
-// A sample that fits in the shared memory of a cluster of up to 8 blocks is
-// read once: every thread keeps its own values there, the blocks exchange
+// One cluster of up to 8 blocks takes a sample.  Where its values fit in their
+// shared memory they are read once, every thread keeping its own; larger ones
+// are read again, out of the L2.  The blocks exchange
 // their channel sums through distributed shared memory, and each forms the
 // group's moments for itself.  One launch and no workspace: a call on
 // 37x53x35 fp32 takes 27 us against 42 in passes, on 80x80x32 fp32 (819 KB) 26
 // against 40, on 64 such samples 40 against 52 (two launches fewer, and x is
 // read once).
 
-constexpr int kSmallThreads = 256;
-constexpr int kSmallBytes = 150 * 1024;  // of a block's values
+constexpr int kSmallThreads = 512;
+constexpr size_t kMostShared = 226 * 1024;
+constexpr int kKeptBytes = 150 * 1024;   // of a block's values, kept in shared memory
+constexpr int kSmallBytes = 512 * 1024;  // or read again
+constexpr int kMaxRereadSamples = 8;
 constexpr int kSmallChannels = 1024;
 
 // Sums the threads' sums over the block and then over the cluster; all blocks
@@ -710,7 +715,7 @@ struct SmallShared {
   double2* channel;
   float2* group;  // per group: mean and rstd, or m1 and m2
   SPLAT_DEV SmallShared(unsigned char* base, const Layout& l, int arrays) {
-    base += kept_bytes(l, sizeof(Vec<T, V>), arrays);
+    base += kept_bytes(l, sizeof(Vec<T, V>), arrays);  // arrays: 0 when nothing is kept
     channel = reinterpret_cast<double2*>(base);
     per_thread = reinterpret_cast<float2*>(channel + l.channels);
     own = per_thread + l.threads * V;
@@ -730,7 +735,7 @@ __global__ void __launch_bounds__(kSmallThreads) norm_small_kernel(const NormPar
   extern __shared__ __align__(16) unsigned char shared[];
   const Layout& l = p.l;
   const Place at = place<V>(l);
-  const SmallShared<T, V> mem(shared, l, 1);
+  const SmallShared<T, V> mem(shared, l, p.keep ? 1 : 0);
   Values* kept = reinterpret_cast<Values*>(shared) + threadIdx.x;
   const T* x = static_cast<const T*>(p.x) + at.sample * l.span;
   const T* from = x + at.first;
@@ -749,7 +754,7 @@ __global__ void __launch_bounds__(kSmallThreads) norm_small_kernel(const NormPar
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (i0 + u < at.count) {
-        kept[(i0 + u) * l.threads] = v[u];
+        if (p.keep) kept[(i0 + u) * l.threads] = v[u];
         float f[V];
         widen<T, V>(v[u], f);
 #pragma unroll
@@ -762,7 +767,7 @@ __global__ void __launch_bounds__(kSmallThreads) norm_small_kernel(const NormPar
   }
   if (at.left) {
     const Values v = load_part<T, V>(from + at.count * at.stride, at.left);
-    kept[at.count * l.threads] = v;
+    if (p.keep) kept[at.count * l.threads] = v;
 #pragma unroll
     for (int j = 0; j < V; ++j)
       if (j < at.left) {
@@ -804,11 +809,23 @@ __global__ void __launch_bounds__(kSmallThreads) norm_small_kernel(const NormPar
     return round_pairs<T, V>(
         activate<ACT, V>(fma(widen_pairs<T, V>(v) + ch.minus, ch.scale, ch.bias)));
   };
-#pragma unroll 2
-  for (int i = 0; i < at.count; ++i)
-    *reinterpret_cast<Values*>(to + i * at.stride) = result(kept[i * l.threads]);
+  for (int i0 = 0; i0 < at.count; i0 += U) {
+    Values v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u < at.count)
+        v[u] = p.keep ? kept[(i0 + u) * l.threads]
+                      : *reinterpret_cast<const Values*>(from + (i0 + u) * at.stride);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u < at.count)
+        *reinterpret_cast<Values*>(to + (i0 + u) * at.stride) = result(v[u]);
+  }
   if (at.left)
-    store_part<T, V>(to + at.count * at.stride, result(kept[at.count * l.threads]), at.left);
+    store_part<T, V>(to + at.count * at.stride,
+                     result(p.keep ? kept[at.count * l.threads]
+                                   : load_part<T, V>(from + at.count * at.stride, at.left)),
+                     at.left);
 }
 
 template <class T, int V, int ACT>
@@ -818,7 +835,7 @@ __global__ void __launch_bounds__(kSmallThreads)
   extern __shared__ __align__(16) unsigned char shared[];
   const Layout& l = p.l;
   const Place at = place<V>(l);
-  const SmallShared<T, V> mem(shared, l, 2);
+  const SmallShared<T, V> mem(shared, l, p.keep ? 2 : 0);
   Values* kept_x = reinterpret_cast<Values*>(shared) + threadIdx.x;
   Values* kept_g = kept_x + l.per_block * l.threads;
   const long long offset = at.sample * l.span + at.first;
@@ -850,16 +867,20 @@ __global__ void __launch_bounds__(kSmallThreads)
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (i0 + u < at.count) {
-          kept_x[(i0 + u) * l.threads] = v[u];
-          kept_g[(i0 + u) * l.threads] = g[u];
+          if (p.keep) {
+            kept_x[(i0 + u) * l.threads] = v[u];
+            kept_g[(i0 + u) * l.threads] = g[u];
+          }
           add(v[u], g[u]);
         }
     }
     if (at.left) {
       const Values v = load_part<T, V>(from + at.count * at.stride, at.left);
       const Values g = load_part<T, V>(grad + at.count * at.stride, at.left);
-      kept_x[at.count * l.threads] = v;
-      kept_g[at.count * l.threads] = g;
+      if (p.keep) {
+        kept_x[at.count * l.threads] = v;
+        kept_g[at.count * l.threads] = g;
+      }
       add(v, g);
     }
   }
@@ -901,13 +922,31 @@ __global__ void __launch_bounds__(kSmallThreads)
     const Pairs<V> du = slope<ACT, V>(fma(d, k.scale, k.bias)) * widen_pairs<T, V>(g);
     return round_pairs<T, V>(fma(du, k.scale, fma(d, k.k2, k.k1)));
   };
-#pragma unroll 2
-  for (int i = 0; i < at.count; ++i)
-    *reinterpret_cast<Values*>(to + i * at.stride) =
-        result(kept_x[i * l.threads], kept_g[i * l.threads]);
-  if (at.left)
-    store_part<T, V>(to + at.count * at.stride,
-                     result(kept_x[at.count * l.threads], kept_g[at.count * l.threads]), at.left);
+  constexpr int U = 4;
+  for (int i0 = 0; i0 < at.count; i0 += U) {
+    Values v[U], g[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u < at.count) {
+        v[u] = p.keep ? kept_x[(i0 + u) * l.threads]
+                      : *reinterpret_cast<const Values*>(from + (i0 + u) * at.stride);
+        g[u] = p.keep ? kept_g[(i0 + u) * l.threads]
+                      : *reinterpret_cast<const Values*>(grad + (i0 + u) * at.stride);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u < at.count)
+        *reinterpret_cast<Values*>(to + (i0 + u) * at.stride) = result(v[u], g[u]);
+  }
+  if (at.left) {
+    const long long o = at.count * at.stride;
+    store_part<T, V>(to + o,
+                     result(p.keep ? kept_x[at.count * l.threads]
+                                   : load_part<T, V>(from + o, at.left),
+                            p.keep ? kept_g[at.count * l.threads]
+                                   : load_part<T, V>(grad + o, at.left)),
+                     at.left);
+  }
 }
 
 // ---- host ------------------------------------------------------------------
@@ -955,7 +994,7 @@ constexpr int kForwardBlocksPerSm = 2, kBackwardBlocksPerSm = 1;
 struct Plan {
   Layout l;
   int vector;
-  bool small;
+  bool small, keep;
   size_t shared_bytes;
 };
 
@@ -966,8 +1005,12 @@ Plan make_plan(int value_bytes, int samples, long long positions, int channels, 
   const int per_sm = backward ? kBackwardBlocksPerSm : kForwardBlocksPerSm;
   const long long bytes = positions * channels * value_bytes * (backward ? 2 : 1);
   plan.l = make_layout(samples, positions, channels, plan.vector, per_sm, kSmallThreads);
+  // values read twice by few blocks only pay where there are few samples: 1, 8,
+  // 16 and 64 of 170x170x32 fp32 30, 31, 66 and 169 us against 40, 39, 43 and
+  // 145 in passes
   plan.small = plan.l.columns == 1 && channels <= kSmallChannels &&
-               bytes <= static_cast<long long>(kMaxCluster) * kSmallBytes;
+               bytes <= static_cast<long long>(kMaxCluster) *
+                            (samples <= kMaxRereadSamples ? kSmallBytes : kKeptBytes);
   plan.shared_bytes = 0;
   if (!plan.small) {
     plan.l = make_layout(samples, positions, channels, plan.vector, per_sm, kMaxThreads);
@@ -977,7 +1020,13 @@ Plan make_plan(int value_bytes, int samples, long long positions, int channels, 
     while (blocks < kMaxCluster && blocks * 8192LL < bytes && blocks < plan.l.steps) blocks *= 2;
     plan.l.blocks = blocks;
     plan.l.per_block = (plan.l.steps + blocks - 1) / blocks;
-    plan.shared_bytes = small_bytes(plan.l, plan.vector, value_bytes, groups, backward ? 2 : 1);
+    plan.keep = bytes <= static_cast<long long>(kMaxCluster) * kKeptBytes;
+    const auto need = [&](int arrays) {
+      return small_bytes(plan.l, plan.vector, value_bytes, groups, arrays);
+    };
+    // many channels, or a last step of few vectors, can leave less room
+    if (plan.keep && need(backward ? 2 : 1) > kMostShared) plan.keep = false;
+    plan.shared_bytes = need(!plan.keep ? 0 : backward ? 2 : 1);
   }
   return plan;
 }
@@ -1083,6 +1132,7 @@ int splat_feature_norm(int dtype, int samples, long long positions, int channels
     return host::fail(kWorkspaceTooSmall, "feature_norm: workspace");
   NormParams p{};
   p.l = plan.l;
+  p.keep = plan.small && plan.keep;
   p.samples = samples;
   p.groups = groups;
   p.group_channels = channels / groups;
@@ -1141,6 +1191,7 @@ int splat_feature_norm_backward(int dtype, int samples, long long positions, int
     return host::fail(kWorkspaceTooSmall, "feature_norm_backward: workspace");
   NormParams p{};
   p.l = plan.l;
+  p.keep = plan.small && plan.keep;
   p.samples = samples;
   p.groups = groups;
   p.group_channels = channels / groups;

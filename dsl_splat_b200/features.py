@@ -54,24 +54,6 @@ def _once(backward):
     return run
 
 
-# The tensors keep their shapes up to these functions: a reshape outside would
-# be a node of its own in the autograd graph, whose visit costs more than a
-# small call's kernels.
-
-def _rows(t: Tensor | None, width: int) -> Tensor | None:
-    """(...,width) as (rows,width); the row count is explicit, since with no
-    rows a -1 dimension is ambiguous."""
-    return t if t is None or t.ndim == 2 else t.reshape(math.prod(t.shape[:-1]), width)
-
-
-def _linear_forward(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None,
-                    activation: str) -> Tensor:
-    n = weight.shape[0]
-    y = stages.feature_linear(_rows(x, weight.shape[1]), weight, bias, _rows(residual, n),
-                              activation)
-    return y if x.ndim == 2 else y.view(x.shape[:-1] + (n,))
-
-
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: Tensor, weight: Tensor, bias: Tensor | None,
@@ -79,7 +61,7 @@ class _Linear(torch.autograd.Function):
         ctx.save_for_backward(x, weight, bias)
         ctx.activation = activation
         ctx.set_materialize_grads(False)
-        return _linear_forward(x, weight, bias, residual, activation)
+        return stages.feature_linear(x, weight, bias, residual, activation)
 
     @staticmethod
     @_once
@@ -88,23 +70,20 @@ class _Linear(torch.autograd.Function):
             return (None,) * 5
         x, weight, bias = ctx.saved_tensors
         needs = ctx.needs_input_grad
-        n, k = weight.shape
         dx, dweight, dbias = stages.feature_linear_backward(
-            _rows(x, k), weight, bias, ctx.activation, _rows(upstream, n), needs[:3])
-        if dx is not None and x.ndim != 2:
-            dx = dx.view(x.shape)
+            x, weight, bias, ctx.activation, upstream, needs[:3])
         return dx, dweight, dbias, upstream if needs[3] else None, None
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx: Any, x: Tensor, weight: Tensor | None, bias: Tensor | None, groups: int,
-                eps: float, activation: str, shape: tuple[int, int, int]) -> Tensor:
-        y, moments = stages.feature_norm(x.reshape(shape), groups, weight, bias, eps, activation)
+    def forward(ctx: Any, x: Tensor, weight: Tensor | None, bias: Tensor | None, samples: int,
+                groups: int, eps: float, activation: str) -> Tensor:
+        y, moments = stages.feature_norm(x, samples, groups, weight, bias, eps, activation)
         ctx.save_for_backward(x, weight, bias, moments)
-        ctx.groups, ctx.activation, ctx.shape = groups, activation, shape
+        ctx.settings = samples, groups, activation
         ctx.set_materialize_grads(False)
-        return y.view(x.shape)
+        return y
 
     @staticmethod
     @_once
@@ -112,11 +91,10 @@ class _GroupNorm(torch.autograd.Function):
         if upstream is None:
             return (None,) * 7
         x, weight, bias, moments = ctx.saved_tensors
+        samples, groups, activation = ctx.settings
         dx, dweight, dbias = stages.feature_norm_backward(
-            x.reshape(ctx.shape), ctx.groups, weight, bias, moments, ctx.activation,
-            upstream.reshape(ctx.shape), ctx.needs_input_grad[:3])
-        if dx is not None:
-            dx = dx.view(x.shape)
+            x, samples, groups, weight, bias, moments, activation, upstream,
+            ctx.needs_input_grad[:3])
         return dx, dweight, dbias, None, None, None, None
 
 
@@ -167,7 +145,7 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *,
         raise ValueError("at most 65535 input and output features")
     if _recorded(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, residual, activation)
-    return _linear_forward(x, weight, bias, residual, activation)
+    return stages.feature_linear(x, weight, bias, residual, activation)
 
 
 def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tensor | None = None,
@@ -199,11 +177,10 @@ def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tenso
     positions = math.prod(x.shape[-1 - spatial_dims:-1])
     if positions > (1 << 31) - 1 or positions * channels > 1 << 40 or samples * channels > 1 << 30:
         raise ValueError("too many positions or samples")
-    shape, groups, eps = (samples, positions, channels), int(groups), float(eps)
+    groups, eps = int(groups), float(eps)
     if _recorded(x, weight, bias):
-        return _GroupNorm.apply(x, weight, bias, groups, eps, activation, shape)
-    y, _ = stages.feature_norm(x.reshape(shape), groups, weight, bias, eps, activation, False)
-    return y.view(x.shape)
+        return _GroupNorm.apply(x, weight, bias, samples, groups, eps, activation)
+    return stages.feature_norm(x, samples, groups, weight, bias, eps, activation, False)[0]
 
 
 @dataclass(slots=True)

@@ -718,13 +718,13 @@ def _address(t: Tensor | None) -> int | None:
 
 def feature_linear(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None,
                    activation: str) -> Tensor:
-    """act(x weight^T + bias) + residual for x (M,K), weight (N,K)."""
-    (m, k), n = x.shape, weight.shape[0]
-    y = x.new_empty((m, n))
+    """act(x weight^T + bias) + residual for x (...,K), weight (N,K)."""
+    n, k = weight.shape
+    y = x.new_empty(x.shape[:-1] + (n,))
+    m = x.numel() // k
     if m:
         dtype, device = FEATURE_DTYPES[x.dtype], x.device
-        size = _query("splat_feature_linear_workspace_bytes", device.index,
-                      dtype, m, k, n)
+        size = _query("splat_feature_linear_workspace_bytes", device.index, dtype, m, k, n)
         ws = x.new_empty((size,), dtype=torch.uint8) if size > 16 else None
         x, weight, bias, residual = _dense(x), _dense(weight), _dense(bias), _dense(residual)
         _call(lib.splat_feature_linear, "feature_linear", device, dtype, m, k, n, x.data_ptr(),
@@ -737,14 +737,16 @@ def feature_linear_backward(x: Tensor, weight: Tensor, bias: Tensor | None, acti
                             upstream: Tensor, needs: tuple[bool, bool, bool]
                             ) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
     """Gradients of x, weight and bias (None where not needed)."""
-    (m, k), n = x.shape, weight.shape[0]
+    n, k = weight.shape
+    m = x.numel() // k
     make = x.new_empty if m else x.new_zeros
-    dx = make((m, k)) if needs[0] else None
+    dx = make(x.shape) if needs[0] else None
     dweight = make((n, k)) if needs[1] else None
     dbias = make((n,)) if needs[2] else None
     if m and any(needs):
         dtype, act, device = FEATURE_DTYPES[x.dtype], _ACTIVATION_CODES[activation], x.device
-        size = _query("splat_feature_linear_backward_workspace_bytes", device.index, dtype, m, k, n, act)
+        size = _query("splat_feature_linear_backward_workspace_bytes", device.index, dtype, m, k,
+                      n, act)
         ws = x.new_empty((size,), dtype=torch.uint8)
         x, weight, bias, upstream = _dense(x), _dense(weight), _dense(bias), _dense(upstream)
         _call(lib.splat_feature_linear_backward, "feature_linear_backward", device, dtype, m, k,
@@ -753,17 +755,20 @@ def feature_linear_backward(x: Tensor, weight: Tensor, bias: Tensor | None, acti
     return dx, dweight, dbias
 
 
-def feature_norm(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None, eps: float,
-                 activation: str, save: bool = True) -> tuple[Tensor, Tensor | None]:
-    """Group norm with an activation of x (B,S,C): y, and (save) the fp32 means
-    and reciprocal deviations (2,B,groups)."""
-    samples, positions, channels = x.shape
-    y = x.new_empty((samples, positions, channels))
+def feature_norm(x: Tensor, samples: int, groups: int, weight: Tensor | None,
+                 bias: Tensor | None, eps: float, activation: str, save: bool = True
+                 ) -> tuple[Tensor, Tensor | None]:
+    """Group norm with an activation of x (...,C), whose leading dimensions hold
+    `samples` samples: y, and (save) the fp32 means and reciprocal deviations
+    (2,samples,groups)."""
+    channels = x.shape[-1]
+    y = x.new_empty(x.shape)
     moments = x.new_empty((2, samples, groups), dtype=torch.float32) if save else None
-    if samples and positions:
+    if x.numel():
         dtype, device = FEATURE_DTYPES[x.dtype], x.device
-        size = _query("splat_feature_norm_workspace_bytes", device.index,
-                      dtype, samples, positions, channels, groups, 0)
+        positions = x.numel() // (samples * channels)
+        size = _query("splat_feature_norm_workspace_bytes", device.index, dtype, samples,
+                      positions, channels, groups, 0)
         ws = x.new_empty((size,), dtype=torch.uint8) if size > 16 else None
         x, weight, bias = _dense(x), _dense(weight), _dense(bias)
         mean = rstd = None
@@ -776,20 +781,22 @@ def feature_norm(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | N
     return y, moments
 
 
-def feature_norm_backward(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None,
-                          moments: Tensor, activation: str, upstream: Tensor,
-                          needs: tuple[bool, bool, bool]
+def feature_norm_backward(x: Tensor, samples: int, groups: int, weight: Tensor | None,
+                          bias: Tensor | None, moments: Tensor, activation: str,
+                          upstream: Tensor, needs: tuple[bool, bool, bool]
                           ) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
     """Gradients of x, weight and bias (None where not needed)."""
-    samples, positions, channels = x.shape
-    values = samples and positions
+    channels = x.shape[-1]
+    values = x.numel()
     make = x.new_empty if values else x.new_zeros
-    dx = make((samples, positions, channels)) if needs[0] else None
+    dx = make(x.shape) if needs[0] else None
     dweight = make((channels,)) if needs[1] else None
     dbias = make((channels,)) if needs[2] else None
     if values and any(needs):
         dtype, device = FEATURE_DTYPES[x.dtype], x.device
-        size = _query("splat_feature_norm_workspace_bytes", device.index, dtype, samples, positions, channels, groups, 1)
+        positions = values // (samples * channels)
+        size = _query("splat_feature_norm_workspace_bytes", device.index, dtype, samples,
+                      positions, channels, groups, 1)
         ws = x.new_empty((size,), dtype=torch.uint8)
         x, weight, bias, upstream = _dense(x), _dense(weight), _dense(bias), _dense(upstream)
         mean = moments.data_ptr()

@@ -511,7 +511,7 @@ def feature_linear(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Ten
 
 @feature_linear.register_fake
 def _(x, weight, bias, residual, activation):
-    return x.new_empty((x.shape[0], weight.shape[0]))
+    return x.new_empty(x.shape[:-1] + (weight.shape[0],))
 
 
 @torch.library.custom_op(f"{_NS}::feature_linear_backward", mutates_args=())
@@ -545,7 +545,7 @@ feature_linear.register_autograd(_feature_linear_backward, setup_context=_featur
 @torch.library.custom_op(f"{_NS}::feature_norm", mutates_args=())
 def feature_norm(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None, eps: float,
                  activation: str) -> tuple[Tensor, Tensor]:
-    return stages.feature_norm(x, groups, weight, bias, eps, activation)
+    return stages.feature_norm(x, x.shape[0], groups, weight, bias, eps, activation)
 
 
 @feature_norm.register_fake
@@ -557,8 +557,8 @@ def _(x, groups, weight, bias, eps, activation):
 def feature_norm_backward(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None,
                           moments: Tensor, activation: str, upstream: Tensor
                           ) -> tuple[Tensor, Tensor, Tensor]:
-    return stages.feature_norm_backward(x, groups, weight, bias, moments, activation, upstream,
-                                        (True, True, True))
+    return stages.feature_norm_backward(x, x.shape[0], groups, weight, bias, moments, activation,
+                                        upstream, (True, True, True))
 
 
 @feature_norm_backward.register_fake
