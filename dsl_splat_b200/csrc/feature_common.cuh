@@ -162,6 +162,24 @@ SPLAT_DEV void logistic2(float& a, float& b) {
   a = fast_reciprocal(a);
   b = fast_reciprocal(b);
 }
+// normal_tail of a pair: the distribution function's values and the densities'
+// exponentials.
+SPLAT_DEV void normal2(f32x2 z, float a, float b, f32x2& cdf, f32x2& e) {
+  float u, v;
+  unpack2(mul2(mul2(z, z), splat2(-0.72134752044448170f)), u, v);
+  e = pack2(fast_exp2(u), fast_exp2(v));
+  unpack2(fma2(pack2(fabsf(a), fabsf(b)), splat2(0.23164189f), splat2(1.0f)), u, v);
+  const f32x2 t = pack2(fast_reciprocal(u), fast_reciprocal(v));
+  f32x2 q = fma2(t, splat2(0.5f * 1.061405429f), splat2(0.5f * -1.453152027f));
+  q = fma2(q, t, splat2(0.5f * 1.421413741f));
+  q = fma2(q, t, splat2(0.5f * -0.284496736f));
+  q = fma2(q, t, splat2(0.5f * 0.254829592f));
+  float ta, tb, ua, ub;
+  const f32x2 tail = mul2(mul2(q, t), e);
+  unpack2(tail, ta, tb);
+  unpack2(fma2(tail, splat2(-1.0f), splat2(1.0f)), ua, ub);
+  cdf = pack2(a < 0.0f ? ta : ua, b < 0.0f ? tb : ub);
+}
 template <int ACT>
 SPLAT_DEV void activate2(float& a, float& b) {
   if constexpr (ACT == kSilu) {
@@ -170,6 +188,11 @@ SPLAT_DEV void activate2(float& a, float& b) {
     unpack2(mul2(pack2(a, b), pack2(s, t)), a, b);
   } else if constexpr (ACT == kSigmoid) {
     logistic2(a, b);
+  } else if constexpr (ACT == kGelu) {
+    const f32x2 z = pack2(a, b);
+    f32x2 cdf, e;
+    normal2(z, a, b, cdf, e);
+    unpack2(mul2(z, cdf), a, b);
   } else {
     a = activate<ACT>(a);
     b = activate<ACT>(b);
@@ -185,6 +208,11 @@ SPLAT_DEV void slope2(float& a, float& b) {
     // s + s z (1 - s), and s (1 - s)
     const f32x2 q = fma2(pack2(-s, -t), ACT == kSilu ? z : p, ACT == kSilu ? z : p);
     unpack2(ACT == kSilu ? fma2(p, q, p) : q, a, b);
+  } else if constexpr (ACT == kGelu) {
+    const f32x2 z = pack2(a, b);
+    f32x2 cdf, e;
+    normal2(z, a, b, cdf, e);
+    unpack2(fma2(mul2(z, splat2(0.39894228040143268f)), e, cdf), a, b);
   } else {
     a = slope<ACT>(a);
     b = slope<ACT>(b);

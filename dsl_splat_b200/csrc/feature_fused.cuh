@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
   const uint32_t x_raw_at = bias_at + kFusedWidth * 4;
   const uint32_t dy_raw_at = x_raw_at + F::raw_bytes(p.k);
   const T* x = static_cast<const T*>(p.x);
-  // thread 0: copies of a tile
+  // one thread: copies of a tile
   const auto copy_rows = [&](const void* from, int width, uint32_t tile, uint32_t to,
                              unsigned long long& bar) {
     const long long m0 = static_cast<long long>(tile) * kTileRows;
