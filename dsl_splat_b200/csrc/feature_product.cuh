@@ -690,12 +690,12 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
                        raw_bar);
           ++copied;
         };
-        const auto advance = [&](int stages) {
-          for (stage += stages; stage >= p.stages; stage -= p.stages) parity ^= 1;
-        };
+        // and stages of its own, so that its waits on a stage follow one another
+        const int first_stage = group ? (p.stages + 1) / 2 : 0;
+        const int end_stage = group ? p.stages : (p.stages + 1) / 2;
+        stage = first_stage;
         const uint32_t step = 2 * gridDim.x, first = blockIdx.x + group * gridDim.x;
         if (own == 0 && first < p.tiles) copy_tile(first);
-        advance(group * chunks_all);
         uint32_t round = 0;
         for (uint32_t t = first; t < p.tiles && ok; t += step, round ^= 1) {
           const ProductTile tile(p, t);
@@ -715,7 +715,7 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
                                       tile.n0, p.n - tile.n0, c * kChunk, k_valid, own, kGroup);
             tc::fence_async_proxy();
             tc::barrier_arrive(tc::shared_address(&full[stage]));
-            advance(1);
+            if (++stage == end_stage) stage = first_stage, parity ^= 1;
           }
           if (!ok) break;
           tc::barrier_arrive(read_bar);
@@ -723,7 +723,6 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
             if (!(ok = tc::barrier_wait(read_bar, round))) break;
             copy_tile(t + step);
           }
-          advance(chunks_all);  // the other group's tile
         }
         // no copy is in flight past this point, also after a wait that ran out
         if (copied) ok = tc::barrier_wait(raw_bar, (copied - 1) & 1) && ok;
@@ -759,8 +758,11 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
       // rows of the result are not stored
       const uint32_t a_block = p.m > 64 ? kChunk * 128 : 0;
       if (p.resident) ok = tc::barrier_wait(tc::shared_address(&resident_full), 0);
-      int stage = 0;
-      uint32_t parity = 0, i_acc = 0;  // accumulators filled
+      // the stages of the one ring, or of the two groups of producers in turn
+      const int half_stages = p.raw_bytes ? (p.stages + 1) / 2 : p.stages;
+      int stage = 0, other_stage = half_stages;
+      uint32_t parity = 0, other_parity = 0, i_acc = 0;  // accumulators filled
+      int end_stage = half_stages, other_end = p.stages;
       for (uint32_t t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
         const ProductTile tile(p, t);
         int c = 0;
@@ -797,10 +799,19 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
                               steps, instruction, !first);
               }
             tc::commit(lead, tc::shared_address(&empty[stage]));
-            if (++stage == p.stages) stage = 0, parity ^= 1;
+            if (++stage == end_stage) {
+              stage = p.raw_bytes && end_stage == p.stages ? half_stages : 0;
+              parity ^= 1;
+            }
           }
           tc::commit(lead, tc::shared_address(&acc_full[acc]));
           ++i_acc;
+        }
+        if (p.raw_bytes) {  // the other group's tile is next
+          const int s = stage, e = end_stage;
+          const uint32_t q = parity;
+          stage = other_stage, end_stage = other_end, parity = other_parity;
+          other_stage = s, other_end = e, other_parity = q;
         }
       }
       // whichever way the loop ended, no product is in flight past this point

@@ -158,6 +158,17 @@ def test_linear_many_rows_without_activation(m, k, n, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k, n", [(68, 17), (128, 32), (100, 64), (185, 24), (35, 24)])
+def test_linear_very_many_tiles(k, n, dtype):
+    """Ten tiles and more to every block, of one chunk of inputs and of several."""
+    normal = draws(26)
+    x, w, b = (normal(*s, dtype=dtype) for s in ((400001, k), (n, k), (n,)))
+    for _ in range(3):
+        y = features.linear(x, w, b, activation="sigmoid")
+        check_linear(x, w, b, None, "sigmoid", y)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_very_wide(dtype):
     """A bias of more values than a block keeps, and thousands of inputs."""
     linear_case(40, 24, 5003, dtype, "silu", seed=22)
