@@ -42,12 +42,12 @@ constexpr int kFusedThreads = 512, kFusedWarps = kFusedThreads / 32;
 // 197, 128 -> 128 bf16 175 against 309, 64 -> 64 fp32 275 against 460, 128 -> 64
 // fp32 637 against 636).
 constexpr int kFusedWidth = 128;
-constexpr int kOnesBytes = 16 * 128;    // 16 rows of 64 ones
+constexpr int kJoinBytes = 4 * kFusedWidth * 4;  // db of the four blocks of rows
 
 template <class T>
 struct Fused {
   static constexpr int P = sizeof(T) == 4 ? 3 : 1;  // parts of every operand
-  static constexpr int kAcc = sizeof(T) == 4 ? 2 : 1;  // accumulators of dW and db
+  static constexpr int kAcc = sizeof(T) == 4 ? 2 : 1;  // accumulators of dW
   __host__ __device__ static int blocks64(int n) { return (n + 63) / 64; }
   // a patch of 32 x 16 values for each warp
   __host__ __device__ static int staging_bytes() { return kFusedWarps * 512 * sizeof(T); }
@@ -59,7 +59,7 @@ struct Fused {
   __host__ __device__ static int w_plane(int k, int n32) { return blocks64(k) * n32 * 128; }
   static size_t shared_bytes(int k, int n, int n32, bool raw) {
     return static_cast<size_t>(staging_bytes()) + P * x_plane(k) + P * x_plane(n) +
-           P * w_plane(k, n32) + kOnesBytes + 1024 + kFusedWidth * 4 +
+           P * w_plane(k, n32) + kJoinBytes + 1024 + kFusedWidth * 4 +
            (raw ? raw_bytes(k) + raw_bytes(n) : 0);
   }
 };
@@ -79,8 +79,8 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
   const uint32_t x_at = base + F::staging_bytes();
   const uint32_t z_at = x_at + P * x_plane;
   const uint32_t w_at = z_at + P * z_plane;
-  const uint32_t ones_at = w_at + P * w_plane;
-  const uint32_t bias_at = ones_at + kOnesBytes;
+  const uint32_t join_at = w_at + P * w_plane;
+  const uint32_t bias_at = join_at + kJoinBytes;
   const int warp = tc::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   // a warp's patches: 16 columns from 16 group on, and from 64 + 16 group on
   const int lane_block = warp & 3, group = warp >> 2;
@@ -112,16 +112,11 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
     }
   }
   if (warp == 0) tc::tmem_alloc(tc::shared_address(&tmem_base), p.tmem_columns);
-  // W, a block of ones and the bias stay for all tiles
+  // W and the bias stay for all tiles
   for (int c = 0; c * 64 < p.k; ++c)
     fill<T, P>(p.w_vector, w_at + c * p.n32 * 128, w_plane, p.n32, 8,
                 static_cast<const T*>(p.weight) + c * 64, p.k, p.n, p.k - c * 64, threadIdx.x,
                 kFusedThreads);
-  {
-    const uint32_t one = kIsF16<T> ? 0x3c003c00u : 0x3f803f80u;
-    if (threadIdx.x < kOnesBytes / 16)
-      store_shared(ones_at + threadIdx.x * 16, make_uint4(one, one, one, one));
-  }
   for (int i = threadIdx.x; i < p.n32; i += kFusedThreads)
     asm volatile("st.shared.f32 [%0], %1;" ::"r"(bias_at + i * 4),
                  "f"(p.bias && i < p.n ? to_float(static_cast<const T*>(p.bias)[i]) : 0.0f)
@@ -131,10 +126,11 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = tc::uniform(tmem_base);
-  const uint32_t acc_w = tmem + max(p.k32, p.n32), acc_b = acc_w + kAcc * p.k32;
+  const uint32_t acc_w = tmem + max(p.k32, p.n32);
 
   float sum_w[kAcc == 2 ? 2 : 1][16] = {};  // fp32: this thread's part of dW
-  float sum_b = 0.0f;
+  // db of this lane's columns, from dz before its rounding
+  float sum_b[2] = {0.0f, 0.0f};
   uint32_t parity = 0;
   bool ok = true, fresh = true;
   for (uint32_t t = blockIdx.x; t < p.tiles; t += gridDim.x, parity ^= 1) {
@@ -219,6 +215,10 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = 0.0f;
       }
+      __syncwarp();
+      const float columns = sum_rows<16>(v);
+      if (c < 64) sum_b[0] += columns;
+      else sum_b[1] += columns;
       const int row = lane_block * 32 + lane;
       const uint32_t at = z_at + (c >> 6) * kAPlane + row * 128;
 #pragma unroll
@@ -273,7 +273,6 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
         // n of up to 64 take one block of dz twice; the upper lanes are not read
         const uint32_t z_block = p.n > 64 ? kAPlane : 0;
         const uint32_t wide = tc::instruction(!kIsF16<T>, true, true, p.k32);
-        const uint32_t narrow = tc::instruction(!kIsF16<T>, true, false, 16);
         const bool start = kAcc == 2 || fresh;
 #pragma unroll
         for (int sum = P - 1; sum >= 0; --sum)
@@ -288,17 +287,6 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
                           tc::descriptor_mn_major(x_at + j * x_plane, kAPlane), tc::kStepMn,
                           tc::kStepMn, kTileRows / 16, wide, !first);
           }
-#pragma unroll
-        for (int i = P - 1; i >= 0; --i) {
-          const bool own = i == 0 && kAcc == 2;
-          const bool first = start && (own || i == P - 1);
-          for (int h = 0; h < 2; ++h)
-            tc::mma_steps(lead, acc_b + (own ? 0 : (kAcc - 1) * 32),
-                          tc::descriptor_mn_major(z_at + i * z_plane + h * 4 * tc::kStepMn,
-                                                  z_block),
-                          tc::descriptor_k_major(ones_at), tc::kStepMn, tc::kStepK, 4, narrow,
-                          !(first && h == 0));
-        }
       }
       tc::commit(lead, tc::shared_address(&dw_done));
     }
@@ -342,9 +330,6 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
             for (int j = 0; j < 16; ++j) sum_w[i][j] += v[j];
           }
         }
-        if (group == 0)
-          sum_b += tc::tmem_load1(acc_b + (lane_block << 21)) +
-                   tc::tmem_load1(acc_b + (lane_block << 21) + 32);
       }
     }
   }
@@ -372,10 +357,15 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
           }
         }
       }
-      if (group == 0) {
-        if constexpr (kAcc == 1) sum_b = tc::tmem_load1(acc_b + (lane_block << 21));
-        if (row < p.n) out[p.n * p.k + row] = sum_b;
-      }
+    }
+    // both lanes of a column have its sum
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int c = group * 16 + 64 * i + lane / 2;
+      if (lane % 2 == 0 && c < p.n)
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(join_at + (lane_block * kFusedWidth + c) * 4),
+                     "f"(sum_b[i])
+                     : "memory");
     }
   }
   if (threadIdx.x == 0) {  // nothing is in flight past this, also after a wait that ran out
@@ -393,6 +383,18 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
   if (!ok) atomicCAS(p.error, 0, kDeviceTimeout);
   tc::fence_before_sync();
   __syncthreads();
+  if (p.partial && !fresh && threadIdx.x < p.n) {
+    float s = 0.0f;
+    for (int q = 0; q < 4; ++q) {
+      float v;
+      asm volatile("ld.shared.f32 %0, [%1];"
+                   : "=f"(v)
+                   : "r"(join_at + (q * kFusedWidth + threadIdx.x) * 4)
+                   : "memory");
+      s += v;
+    }
+    p.partial[static_cast<size_t>(blockIdx.x) * p.n * (p.k + 1) + p.n * p.k + threadIdx.x] = s;
+  }
   if (warp == 0) tc::tmem_free(tmem, p.tmem_columns);
 }
 

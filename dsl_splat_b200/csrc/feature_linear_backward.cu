@@ -168,10 +168,18 @@ size_t dz_bytes(int dtype, long long rows, int n, int activation) {
   return activation == kNone ? 0 : round16(static_cast<size_t>(rows) * n * (dtype == kF32 ? 4 : 2));
 }
 
+// Sums of dz over 32 rows each, of whole tiles.
+size_t column_sums_bytes(long long rows, int n, int activation) {
+  return activation == kNone
+             ? 0
+             : round16(static_cast<size_t>((rows + kTileRows - 1) / kTileRows) * 4 * n * 4);
+}
+
 // What the wide layers' products read: the tensors, or planes of them.
 struct Sources {
   const void *x, *weight, *dz;
   Planes x_planes, weight_planes, dz_planes;  // data: NULL without planes
+  const float* column_sums;                   // NULL: dz is dy
 };
 
 // The two products of the backward.
@@ -207,7 +215,11 @@ int launch_gradients(long long rows, int k, int n, const Sources& from, void* dx
   }
   if (dbias) {
     float* sums = partial + static_cast<long long>(splits.count) * n * k;
-    const int count = sum_columns<T>(static_cast<const T*>(from.dz), rows, n, sums, s);
+    // of dy, or of the sums that the pass over z left of dz before its rounding
+    const int count =
+        from.column_sums
+            ? sum_columns<float>(from.column_sums, (rows + 31) / 32, n, sums, s)
+            : sum_columns<T>(static_cast<const T*>(from.dz), rows, n, sums, s);
     join_splits<T>(sums, n, count, n, 0, dbias, nullptr, s);
   }
   return host::check_launch("feature_linear_backward");
@@ -233,7 +245,7 @@ FusedPlan plan_fused(long long rows, int k, int n) {
   if (k > kFusedWidth || n > kFusedWidth) return plan;
   const int k32 = round32(k), n32 = round32(n);
   plan.tmem_columns = 32;
-  while (plan.tmem_columns < static_cast<uint32_t>(std::max(k32, n32) + F::kAcc * (k32 + 32)))
+  while (plan.tmem_columns < static_cast<uint32_t>(std::max(k32, n32) + F::kAcc * k32))
     plan.tmem_columns *= 2;
   const int row_align = 16 / static_cast<int>(sizeof(T));
   plan.copies = sizeof(T) == 2 && k % row_align == 0 && n % row_align == 0 && rows < 1LL << 31;
@@ -340,6 +352,7 @@ size_t splat_feature_linear_backward_workspace_bytes(int dtype, long long rows, 
   return dz_bytes(dtype, rows, n, activation) +
          round16(static_cast<size_t>(weight_splits(rows, k, n).count) * n * k * 4) +
          round16(static_cast<size_t>(kMaxColumnSplits) * n * 4) +
+         column_sums_bytes(rows, n, activation) +
          SPLAT_FEATURE_TYPE(dtype, [&] {
            return wants_planes<T>(rows, k, n) ? plane_bytes<T>(rows, k) + plane_bytes<T>(n, k) +
                                                     plane_bytes<T>(rows, n)
@@ -373,7 +386,9 @@ int splat_feature_linear_backward(int dtype, long long rows, int k, int n, const
     float* partial = reinterpret_cast<float*>(at);
     at += round16(static_cast<size_t>(weight_splits(rows, k, n).count) * n * k * 4) +
           round16(static_cast<size_t>(kMaxColumnSplits) * n * 4);
-    Sources from{x, weight, activation == kNone ? dy : dz, {}, {}, {}};
+    float* column_sums = reinterpret_cast<float*>(at);
+    at += column_sums_bytes(rows, n, activation);
+    Sources from{x, weight, activation == kNone ? dy : dz, {}, {}, {}, nullptr};
     const bool planes = wants_planes<T>(rows, k, n);
     if (planes) {
       if (dweight || activation != kNone) from.x_planes = split<T>(x, rows, k, at, s);
@@ -384,6 +399,7 @@ int splat_feature_linear_backward(int dtype, long long rows, int k, int n, const
     if (activation != kNone) {
       ProductParams p = forward_params<T>(rows, k, n, x, weight, bias, dy, activation, dz);
       if (planes) use_planes(p, from.x_planes, from.weight_planes);
+      if (dbias) from.column_sums = p.column_sums = column_sums;
       const int status = launch_product<T, P, false, T, P, false, T, T, kSlope>(p, s);
       if (status != kOk) return status;
     }

@@ -82,6 +82,7 @@ struct ProductParams {
   const void* bias;   // (n) or NULL
   const void* extra;  // residual or dy (m, n), or NULL
   void* out;          // (splits, m, n)
+  float* column_sums; // kSlope: (4 tiles_m, n) sums of dz over 32 rows each, or NULL
   int extra_vector, out_vector;  // their rows are whole 16-byte pieces
   int bias_shared;    // values of the bias kept in shared memory (0: too many)
   int* error;
@@ -497,6 +498,29 @@ SPLAT_DEV void finish_row(const Patch<TE, W>& extra, bool with_extra, float (&v)
   }
 }
 
+// The sums over a warp's rows of W columns, a lane's row each: halving steps,
+// after which lane l has column l of 32 (of 16: column l / 2, in two lanes).
+template <int HALF, int BIT, int W>
+SPLAT_DEV void fold_rows(float (&v)[W]) {
+  if constexpr (HALF > 0) {
+    const bool upper = threadIdx.x & BIT;
+#pragma unroll
+    for (int j = 0; j < HALF; ++j) {
+      const float mine = upper ? v[j + HALF] : v[j], theirs = upper ? v[j] : v[j + HALF];
+      v[j] = mine + __shfl_xor_sync(0xffffffffu, theirs, BIT);
+    }
+    fold_rows<HALF / 2, BIT / 2>(v);
+  }
+}
+template <int W>
+SPLAT_DEV float sum_rows(const float (&row)[W]) {
+  float v[W];
+#pragma unroll
+  for (int j = 0; j < W; ++j) v[j] = row[j];
+  fold_rows<W / 2, 16>(v);
+  return W == 16 ? v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1) : v[0];
+}
+
 // ---- operands as planes ----------------------------------------------------------
 
 // src (rows, cols) as `P` planes of plane_rows x ld 16-bit parts; rows behind
@@ -907,6 +931,19 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
               case kGelu: finish_row<EPI, kGelu, TE>(extra_patch, e, v); break;
               case kSigmoid: finish_row<EPI, kSigmoid, TE>(extra_patch, e, v); break;
               default: finish_row<EPI, kNone, TE>(extra_patch, e, v);
+            }
+            if constexpr (EPI == kSlope) {
+              if (p.column_sums) {  // before dz is rounded
+                if (static_cast<int>(threadIdx.x & 31) >= rows) {
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+                }
+                __syncwarp();
+                const float sum = sum_rows<32>(v);
+                const int lane = threadIdx.x & 31;
+                if (lane < cols)
+                  p.column_sums[(tile.m0 / 32 + lane_block) * p.n + col0 + lane] = sum;
+              }
             }
             if (p.copy_extra) {  // the next patch's, once this one has been read
               __syncwarp();

@@ -9,7 +9,8 @@ step) and h = eps(dtype) / 2 for the one rounding to the output's type:
 * an activation and its slope, 16 u relative, and what their argument is off
   by times their Lipschitz constants (both at most 1.2);
 * 16-bit types take dz = dy act'(z) in their own type: half a step relative
-  (and half their smallest value) of each dz, besides the above.
+  (and half their smallest value) of each dz, besides the above, in dx and dW;
+  db is summed from dz before that.
 """
 
 import math
@@ -94,6 +95,7 @@ def check_linear(x, w, b, r, act, y, grads=None, dy=None):
         e_dz = dyd.abs() * U
     if act == "relu":  # the slope jumps where z is within its own error of 0
         e_dz = dyd.abs() * ((z.abs() <= e_z).double() + U)
+    e_sum = e_dz  # db is summed from dz before its rounding
     if x.dtype != torch.float32:
         e_dz = e_dz + half_step(x.dtype) * (dz.abs() + e_dz) + smallest(x.dtype)
     dx, dw, db = grads
@@ -103,7 +105,7 @@ def check_linear(x, w, b, r, act, y, grads=None, dy=None):
         check(dw, dz.t() @ xd, (m + 8) * U * (dz.abs().t() @ xd.abs()) + e_dz.t() @ xd.abs(),
               "dw")
     if db is not None:
-        check(db, dz.sum(0), (m + 8) * U * dz.abs().sum(0) + e_dz.sum(0), "db")
+        check(db, dz.sum(0), (m + 8) * U * dz.abs().sum(0) + e_sum.sum(0), "db")
 
 
 def linear_case(m, k, n, dtype, act, bias=True, residual=False, seed=0):
