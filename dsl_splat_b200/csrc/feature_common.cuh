@@ -15,6 +15,9 @@ namespace feature {
 enum Dtype : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
 enum Activation : int { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3, kSigmoid = 4 };
 
+// Whether dy act' has more digits than dy: a slope of 0 or 1 leaves them.
+__host__ __device__ constexpr bool rounds_dz(int activation) { return activation >= kSilu; }
+
 using bf16 = __nv_bfloat16;
 using f16 = __half;
 
@@ -86,6 +89,24 @@ SPLAT_DEV void widen(const Vec<T, V>& r, float (&v)[V]) {
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = to_float(r.v[j]);
   }
+}
+
+// The first of the two values of T that stand for 16-bit layers' dz, and in v
+// what it leaves, which is rounded to T for the second: half a step squared
+// relative (2^-16 for bf16, 2^-22 for f16) and half of T's smallest value.  The
+// first one is at most T's largest, so that the second brings a v beyond it, an
+// infinity or a NaN.
+template <class T, int V>
+SPLAT_DEV Vec<T, V> take_first(float (&v)[V]) {
+  constexpr float kMost = kIsF16<T> ? 65504.0f : 3.38953138925153547590470800371e38f;
+  float o[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) o[i] = fminf(fmaxf(v[i], -kMost), kMost);
+  const Vec<T, V> first = round_values<T, V>(o);
+  widen<T, V>(first, o);
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] -= o[i];
+  return first;
 }
 
 // 2^x and 1/x in one instruction each, within 2 units of 2^-23; results below

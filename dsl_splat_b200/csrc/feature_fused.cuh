@@ -47,7 +47,8 @@ constexpr int kJoinBytes = 4 * kFusedWidth * 4;  // db of the four blocks of row
 
 template <class T>
 struct Fused {
-  static constexpr int P = sizeof(T) == 4 ? 3 : 1;  // parts of every operand
+  static constexpr int P = sizeof(T) == 4 ? 3 : 1;   // parts of x and W
+  static constexpr int PZ = sizeof(T) == 4 ? 3 : 2;  // of dz (take_first)
   static constexpr int kAcc = sizeof(T) == 4 ? 2 : 1;  // accumulators of dW
   __host__ __device__ static int blocks64(int n) { return (n + 63) / 64; }
   // a patch of 32 x 16 values for each warp
@@ -59,7 +60,7 @@ struct Fused {
   __host__ __device__ static int x_plane(int k) { return blocks64(k) * kAPlane; }
   __host__ __device__ static int w_plane(int k, int n32) { return blocks64(k) * n32 * 128; }
   static size_t shared_bytes(int k, int n, int n32, bool raw) {
-    return static_cast<size_t>(staging_bytes()) + P * x_plane(k) + P * x_plane(n) +
+    return static_cast<size_t>(staging_bytes()) + P * x_plane(k) + PZ * x_plane(n) +
            P * w_plane(k, n32) + kJoinBytes + 1024 + kFusedWidth * 4 +
            (raw ? raw_bytes(k) + raw_bytes(n) : 0);
   }
@@ -70,7 +71,7 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
     fused_backward_kernel(const __grid_constant__ FusedParams p) {
   using F = Fused<T>;
   constexpr int kAcc = F::kAcc;
-  constexpr int P = F::P;
+  constexpr int P = F::P, PZ = F::PZ;
   extern __shared__ unsigned char dynamic[];
   __shared__ alignas(8) unsigned long long z_done, dx_done, dw_done, drained, x_raw, dy_raw;
   __shared__ uint32_t tmem_base;
@@ -79,7 +80,7 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
   const uint32_t w_plane = F::w_plane(p.k, p.n32);
   const uint32_t x_at = base + F::staging_bytes();
   const uint32_t z_at = x_at + P * x_plane;
-  const uint32_t w_at = z_at + P * z_plane;
+  const uint32_t w_at = z_at + PZ * z_plane;
   const uint32_t join_at = w_at + P * w_plane;
   const uint32_t bias_at = join_at + kJoinBytes;
   const int warp = tc::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -98,6 +99,8 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
                 tc::shared_address(&bar));
   };
   const bool with_z = p.activation != kNone;
+  // parts of dz: its 16-bit values have one where dz has dy's digits
+  const int z_parts = sizeof(T) == 4 ? PZ : rounds_dz(p.activation) ? 2 : 1;
 
   if (threadIdx.x == 0) {
     tc::barrier_init(tc::shared_address(&z_done), 1);
@@ -224,21 +227,23 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
       const uint32_t at = z_at + (c >> 6) * kAPlane + row * 128;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        uint4 parts[P];
+        uint4 parts[PZ];
         if constexpr (sizeof(T) == 2) {
           float o[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) o[i] = v[j * 8 + i];
-          const Vec<T, 8> r = round_values<T, 8>(o);
+          const Vec<T, 8> r = z_parts == 1 ? round_values<T, 8>(o) : take_first<T, 8>(o);
           parts[0] = reinterpret_cast<const uint4&>(r);
+          const Vec<T, 8> second = round_values<T, 8>(o);
+          parts[1] = reinterpret_cast<const uint4&>(second);
         } else {
           Vec<float, 8> o;
 #pragma unroll
           for (int i = 0; i < 8; ++i) o.v[i] = v[j * 8 + i];
-          to_parts<float, P>(o, parts);
+          to_parts<float, PZ>(o, parts);
         }
 #pragma unroll
-        for (int q = 0; q < P; ++q)
+        for (int q = 0; q < PZ; ++q)
           store_shared(at + q * z_plane + ((((c & 63) / 8 + j) ^ (row & 7)) << 4), parts[q]);
       }
     }
@@ -254,11 +259,11 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
         const uint32_t instruction = tc::instruction(!kIsF16<T>, false, true, p.k32);
         bool first = true;
 #pragma unroll
-        for (int sum = P - 1; sum >= 0; --sum)
+        for (int sum = PZ - 1; sum >= 0; --sum)
 #pragma unroll
-          for (int i = 0; i < P; ++i) {
+          for (int i = 0; i < PZ; ++i) {
             const int j = sum - i;
-            if (j < 0 || j >= P) continue;
+            if (j < 0 || j >= P || i >= z_parts) continue;
             for (int c = 0; c * 64 < p.n; ++c) {
               tc::mma_steps(lead, tmem, tc::descriptor_k_major(z_at + i * z_plane + c * kAPlane),
                             tc::descriptor_mn_major(w_at + j * w_plane + c * 4 * tc::kStepMn,
@@ -274,15 +279,17 @@ __global__ void __launch_bounds__(kFusedThreads, sizeof(T) == 4 ? 1 : 2)
         // n of up to 64 take one block of dz twice; the upper lanes are not read
         const uint32_t z_block = p.n > 64 ? kAPlane : 0;
         const uint32_t wide = tc::instruction(!kIsF16<T>, true, true, p.k32);
-        const bool start = kAcc == 2 || fresh;
+        // the first product into an accumulator overwrites it
+        bool start = kAcc == 2 || fresh;
 #pragma unroll
-        for (int sum = P - 1; sum >= 0; --sum)
+        for (int sum = PZ - 1; sum >= 0; --sum)
 #pragma unroll
-          for (int i = 0; i < P; ++i) {
+          for (int i = 0; i < PZ; ++i) {
             const int j = sum - i;
-            if (j < 0 || j >= P) continue;
+            if (j < 0 || j >= P || i >= z_parts) continue;
             const bool own = sum == 0 && kAcc == 2;
-            const bool first = start && (own || (sum == P - 1 && i == 0));
+            const bool first = start || own;
+            if (!own) start = false;
             tc::mma_steps(lead, acc_w + (own ? 0 : (kAcc - 1) * p.k32),
                           tc::descriptor_mn_major(z_at + i * z_plane, z_block),
                           tc::descriptor_mn_major(x_at + j * x_plane, kAPlane), tc::kStepMn,

@@ -54,7 +54,7 @@ int launch_product(ProductParams p, cudaStream_t s) {
   // arithmetic two blocks' epilogues share an SM (512 -> 512 fp16 gelu over
   // 131072 rows 103 us against 107 in 256-wide tiles, 256 -> 256 bf16 silu 39
   // against 48)
-  const int widest = PA == 1 && PB == 1 && EPI == kPlain ? 256 : 128;
+  const int widest = PA <= 2 && PB == 1 && EPI == kPlain ? 256 : 128;
   p.tiles_n = (p.n + widest - 1) / widest;
   p.tile_n = ((p.n + p.tiles_n - 1) / p.tiles_n + 31) / 32 * 32;
   const long long tiles_m = (p.m + kTileRows - 1) / kTileRows;
@@ -66,7 +66,10 @@ int launch_product(ProductParams p, cudaStream_t s) {
   p.b_vector = row_vector<SB>(p.b, p.b_ld);
   p.extra_vector =
       p.n * static_cast<long long>(sizeof(TE)) % 16 == 0 && host::aligned(p.extra, 16);
-  p.out_vector = p.n * static_cast<long long>(sizeof(TO)) % 16 == 0 && host::aligned(p.out, 16);
+  if (!p.out_ld) p.out_ld = p.n;
+  p.out_vector = p.n * static_cast<long long>(sizeof(TO)) % 16 == 0 &&
+                 p.out_ld * static_cast<long long>(sizeof(TO)) % 16 == 0 &&
+                 host::aligned(p.out, 16);
   const int columns = static_cast<int>(p.tiles_n) * p.tile_n;
   p.bias_shared = p.bias && columns <= kMaxSharedBias ? columns : 0;
   p.tmem_columns = 32;
@@ -94,7 +97,16 @@ int launch_product(ProductParams p, cudaStream_t s) {
   int blocks = 2, budget = kTwoBlocksBytes;
   if (producers(PA, PB) > 128 || p.tmem_columns > 256 || fixed + 2 * stage > budget)
     blocks = 1, budget = kOneBlockBytes;
-  if (p.a_plane_rows) {
+  if constexpr (PA == 2) {
+    const long long a_rows = AMN ? p.k : p.m, a_columns = AMN ? p.m : p.k;
+    const int a_box = AMN ? kChunk : kTileRows;
+    p.copy_operands =
+        make_map<SA>(p.a_map, p.a, a_rows, a_columns, p.a_ld, kChunk, a_box) &&
+        make_map<SA>(p.a_second_map, p.a_second, a_rows, a_columns, p.a_ld, kChunk, a_box) &&
+        make_map<SB>(p.b_map, p.b, BMN ? p.k : p.n, BMN ? p.n : p.k, p.b_ld, kChunk,
+                     BMN ? kChunk : p.tile_n);
+    if (!p.copy_operands) return host::fail(kInvalidArgument, "feature_linear: operand planes");
+  } else if (p.a_plane_rows) {
     // both operands are planes; f16 ones hold f16, all others bf16 parts
     using H = std::conditional_t<kIsF16<SA>, f16, bf16>;
     p.copy_operands =
@@ -113,7 +125,7 @@ int launch_product(ProductParams p, cudaStream_t s) {
   // two tiles of A as they are in memory, where two stages fit beside them
   // (35 -> 32 fp32 gelu over 10^6 rows 113 us against 140 read as needed,
   // 35 -> 64 bf16 78 against 82)
-  if (!p.copy_operands && !AMN && p.tiles_n == 1 && p.a_ld == p.k && host::aligned(p.a, 16)) {
+  if (PA != 2 && !p.copy_operands && !AMN && p.tiles_n == 1 && p.a_ld == p.k && host::aligned(p.a, 16)) {
     const long long raw = (kTileRows * p.k * static_cast<long long>(sizeof(SA)) + 127) / 128 * 128;
     if (fixed + 2 * stage + 2 * raw > budget && blocks == 2) blocks = 1, budget = kOneBlockBytes;
     if (fixed + 2 * stage + 2 * raw <= budget) p.raw_bytes = static_cast<int>(raw);
@@ -128,7 +140,9 @@ int launch_product(ProductParams p, cudaStream_t s) {
   if (EPI != kPlain) p.copy_extra = make_map<TE>(p.extra_map, p.extra, p.m, p.n, p.n, 32, 32);
   // partial sums are added to or lie one split behind the other
   if (p.splits == 1 && p.k_per_sum >= p.k)
-    p.copy_out = make_map<TO>(p.out_map, p.out, p.m, p.n, p.n, 32, 32);
+    p.copy_out = make_map<TO>(p.out_map, p.out, p.m, p.n, p.out_ld, 32, 32) &&
+                 (!p.out_second ||
+                  make_map<TO>(p.out_second_map, p.out_second, p.m, p.n, p.out_ld, 32, 32));
   p.error = host::device_error_word();
   if (!p.error) return kCudaError;
   const int bytes = fixed + p.stages * stage + 2 * p.raw_bytes + 1024;
@@ -142,13 +156,10 @@ int launch_product(ProductParams p, cudaStream_t s) {
   return host::check_launch("feature_linear");
 }
 
-// Parts of an operand of the linear layer's products.  16-bit types take dz in
-// their own type: rounded to it as x and y are, half a step relative, which is
-// what the result's own rounding costs again (and f16 gradients below 2^-24 or
-// above 65504 leave its range, as dy itself would).  A second part would undo
-// that rounding but doubles the products: 64 -> 64 bf16 training over 1.9 10^6
-// rows took 465 us with it and 411 without, 512 -> 512 fp16 over 131072 rows
-// 2021 (of bf16 parts, three products) and 1016.
+// Parts of an operand of the linear layer's products, but for the dz of 16-bit
+// types, which has two where its activation's slope adds digits to dy's: one would
+// add half a step to each dz, which dx and dW show as much as their own rounding
+// (2.4e-3 relative instead of 1.7e-3 for bf16).
 template <class T>
 constexpr int kOperandParts = sizeof(T) == 4 ? 3 : 1;
 

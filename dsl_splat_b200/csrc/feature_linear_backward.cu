@@ -4,8 +4,8 @@
 //   dx = dz W,  dW = dz^T x,  db = sum over rows of dz,  dr = dy
 //
 // Narrow layers take one pass over the rows (feature_fused.cuh).  Wider ones
-// form dz (in x's type) and take a product each for dx and dW, the latter over
-// ranges of rows whose sums are joined in a fixed order.
+// form dz (in fp32, or in two values of a 16-bit type) and take a product each for
+// dx and dW, the latter over ranges of rows whose sums are joined in a fixed order.
 #include <algorithm>
 
 #include "feature_fused.cuh"
@@ -164,8 +164,21 @@ Splits weight_splits(long long rows, int k, int n) {
 
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
+// dz: (rows, n); of 16-bit types in two parts, planes whose rows start on 16
+// bytes.
+bool two_parts(int dtype, int activation) { return dtype != kF32 && rounds_dz(activation); }
+size_t dz_plane_bytes(long long rows, int n) {
+  return static_cast<size_t>(rows) * round_to(n, 8) * 2;
+}
 size_t dz_bytes(int dtype, long long rows, int n, int activation) {
+  if (two_parts(dtype, activation)) return 2 * dz_plane_bytes(rows, n);
   return activation == kNone ? 0 : round16(static_cast<size_t>(rows) * n * (dtype == kF32 ? 4 : 2));
+}
+// Whether x, W and a dz of one plane are laid out as planes before the products.
+// With a dz of two the products copy all their operands.
+template <class T>
+bool backward_planes(int dtype, long long rows, int k, int n, int activation) {
+  return two_parts(dtype, activation) ? k % 8 != 0 : wants_planes<T>(rows, k, n);
 }
 
 // Sums of dz over 32 rows each, of whole tiles.
@@ -177,17 +190,22 @@ size_t column_sums_bytes(long long rows, int n, int activation) {
 
 // What the wide layers' products read: the tensors, or planes of them.
 struct Sources {
-  const void *x, *weight, *dz;
+  const void *x, *weight, *dz, *dz_second;    // dz_second: NULL: one part
   Planes x_planes, weight_planes, dz_planes;  // data: NULL without planes
   const float* column_sums;                   // NULL: dz is dy
 };
 
-// The two products of the backward.
-template <class T>
+// The two products of the backward; P: parts of dz.
+template <class T, int P>
 int launch_gradients(long long rows, int k, int n, const Sources& from, void* dx, void* dweight,
                      void* dbias, float* partial, cudaStream_t s) {
-  constexpr int P = kOperandParts<T>;
+  constexpr int PB = kOperandParts<T>;
   const bool planes = from.dz_planes.data != nullptr;
+  // a dz of two parts, by the matrix of whole 16-byte rows beside it
+  const auto use_parts = [&](ProductParams& p, const Planes& b, const void* as_it_is) {
+    p.a = from.dz, p.a_second = from.dz_second, p.a_ld = round_to(n, 8);
+    p.b = b.data ? b.data : as_it_is, p.b_ld = b.data ? b.ld : k;
+  };
   if (dx) {
     ProductParams p{};
     p.m = rows, p.k = n, p.n = k;
@@ -195,8 +213,9 @@ int launch_gradients(long long rows, int k, int n, const Sources& from, void* dx
     p.b = from.weight, p.b_ld = k;
     p.k_per_split = n, p.splits = 1;
     p.out = dx;
-    if (planes) use_planes(p, from.dz_planes, from.weight_planes);
-    const int status = launch_product<T, P, false, T, P, true, T, T, kPlain>(p, s);
+    if constexpr (P == 2) use_parts(p, from.weight_planes, from.weight);
+    else if (planes) use_planes(p, from.dz_planes, from.weight_planes);
+    const int status = launch_product<T, P, false, T, PB, true, T, T, kPlain>(p, s);
     if (status != kOk) return status;
   }
   const Splits splits = weight_splits(rows, k, n);
@@ -207,8 +226,9 @@ int launch_gradients(long long rows, int k, int n, const Sources& from, void* dx
     p.b = from.x, p.b_ld = k;
     p.k_per_split = splits.rows, p.splits = splits.count;
     p.out = partial;
-    if (planes) use_planes(p, from.dz_planes, from.x_planes);
-    const int status = launch_product<T, P, true, T, P, true, float, float, kPlain>(p, s);
+    if constexpr (P == 2) use_parts(p, from.x_planes, from.x);
+    else if (planes) use_planes(p, from.dz_planes, from.x_planes);
+    const int status = launch_product<T, P, true, T, PB, true, float, float, kPlain>(p, s);
     if (status != kOk) return status;
     const long long count = static_cast<long long>(n) * k;
     join_splits<T>(partial, count, splits.count, count, 0, dweight, nullptr, s);
@@ -239,7 +259,7 @@ struct FusedPlan {
 int round32(int n) { return (n + 31) / 32 * 32; }
 
 template <class T>
-FusedPlan plan_fused(long long rows, int k, int n) {
+FusedPlan plan_fused(long long rows, int k, int n, int activation) {
   using F = Fused<T>;
   FusedPlan plan{};
   if (k > kFusedWidth || n > kFusedWidth) return plan;
@@ -251,7 +271,7 @@ FusedPlan plan_fused(long long rows, int k, int n) {
   plan.copies = sizeof(T) == 2 && k % row_align == 0 && n % row_align == 0 && rows < 1LL << 31;
   int per_sm = 1;
   if (plan.copies) {
-    plan.bytes = narrow_bytes(k, n, n32);
+    plan.bytes = narrow_bytes(k, n, n32, rounds_dz(activation));
     plan.tmem_columns = 32;
     while (plan.tmem_columns < static_cast<uint32_t>(n32 + 2 * k32)) plan.tmem_columns *= 2;
     if (k <= 64 && n <= 64) per_sm = 2;
@@ -346,7 +366,9 @@ extern "C" {
 size_t splat_feature_linear_backward_workspace_bytes(int dtype, long long rows, int k, int n,
                                                      int activation) {
   if (check_linear(dtype, rows, k, n, activation) != kOk) return 0;
-  const FusedPlan plan = SPLAT_FEATURE_TYPE(dtype, [&] { return plan_fused<T>(rows, k, n); });
+  const FusedPlan plan = SPLAT_FEATURE_TYPE(dtype, [&] {
+    return plan_fused<T>(rows, k, n, activation);
+  });
   const size_t sums = static_cast<size_t>(n) * (static_cast<size_t>(k) + 1) * 4;
   if (plan.blocks) return plan.blocks * sums;
   return dz_bytes(dtype, rows, n, activation) +
@@ -354,9 +376,10 @@ size_t splat_feature_linear_backward_workspace_bytes(int dtype, long long rows, 
          round16(static_cast<size_t>(kMaxColumnSplits) * n * 4) +
          column_sums_bytes(rows, n, activation) +
          SPLAT_FEATURE_TYPE(dtype, [&] {
-           return wants_planes<T>(rows, k, n) ? plane_bytes<T>(rows, k) + plane_bytes<T>(n, k) +
-                                                    plane_bytes<T>(rows, n)
-                                              : static_cast<size_t>(0);
+           return backward_planes<T>(dtype, rows, k, n, activation)
+                      ? plane_bytes<T>(rows, k) + plane_bytes<T>(n, k) +
+                            (two_parts(dtype, activation) ? 0 : plane_bytes<T>(rows, n))
+                      : static_cast<size_t>(0);
          });
 }
 
@@ -375,7 +398,7 @@ int splat_feature_linear_backward(int dtype, long long rows, int k, int n, const
     return host::fail(kWorkspaceTooSmall, "feature_linear_backward: workspace");
   auto s = static_cast<cudaStream_t>(stream);
   return SPLAT_FEATURE_TYPE(dtype, [&] {
-    const FusedPlan plan = plan_fused<T>(rows, k, n);
+    const FusedPlan plan = plan_fused<T>(rows, k, n, activation);
     if (plan.blocks)
       return launch_fused<T>(plan, rows, k, n, x, weight, bias, activation, dy, dx, dweight,
                              dbias, static_cast<float*>(workspace), s);
@@ -388,8 +411,16 @@ int splat_feature_linear_backward(int dtype, long long rows, int k, int n, const
           round16(static_cast<size_t>(kMaxColumnSplits) * n * 4);
     float* column_sums = reinterpret_cast<float*>(at);
     at += column_sums_bytes(rows, n, activation);
-    Sources from{x, weight, activation == kNone ? dy : dz, {}, {}, {}, nullptr};
-    const bool planes = wants_planes<T>(rows, k, n);
+    Sources from{x, weight, activation == kNone ? dy : dz, nullptr, {}, {}, {}, nullptr};
+    const bool planes = backward_planes<T>(dtype, rows, k, n, activation);
+    if (two_parts(dtype, activation)) {
+      if (rows >= 1LL << 31)
+        return host::fail(kTooLarge, "feature_linear_backward: too many rows of a wide layer");
+      if (!planes && !(host::aligned(x, 16) && host::aligned(weight, 16)))
+        return host::fail(kInvalidArgument,
+                          "feature_linear_backward: tensors must be 16-byte aligned");
+      from.dz_second = static_cast<char*>(dz) + dz_plane_bytes(rows, n);
+    }
     if (planes) {
       if (dweight || activation != kNone) from.x_planes = split<T>(x, rows, k, at, s);
       at += plane_bytes<T>(rows, k);
@@ -399,12 +430,20 @@ int splat_feature_linear_backward(int dtype, long long rows, int k, int n, const
     if (activation != kNone) {
       ProductParams p = forward_params<T>(rows, k, n, x, weight, bias, dy, activation, dz);
       if (planes) use_planes(p, from.x_planes, from.weight_planes);
+      if (from.dz_second) {
+        p.out_second = const_cast<void*>(from.dz_second);
+        p.out_ld = round_to(n, 8);
+      }
       if (dbias) from.column_sums = p.column_sums = column_sums;
       const int status = launch_product<T, P, false, T, P, false, T, T, kSlope>(p, s);
       if (status != kOk) return status;
     }
+    if constexpr (sizeof(T) == 2) {
+      if (from.dz_second)
+        return launch_gradients<T, 2>(rows, k, n, from, dx, dweight, dbias, partial, s);
+    }
     if (planes && (dx || dweight)) from.dz_planes = split<T>(from.dz, rows, n, at, s);
-    return launch_gradients<T>(rows, k, n, from, dx, dweight, dbias, partial, s);
+    return launch_gradients<T, P>(rows, k, n, from, dx, dweight, dbias, partial, s);
   });
 }
 

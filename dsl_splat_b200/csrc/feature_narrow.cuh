@@ -3,10 +3,12 @@
 // tensor copies bring x and dy to shared memory and take dx from it.
 //
 // Two tiles are in flight.  dy arrives in the layout of a tensor-core operand
-// and dz overwrites it in place.  While the eight compute warps turn dy into dz
-// for tile t, the products of tile t - 1 finish; they then store its dx while
-// the tensor core forms z of tile t + 1, dW and dx of tile t.  db is summed in
-// registers from dz before its rounding.
+// and dz overwrites it in place: its first value (take_first).  The second
+// values have one plane, which is written once the products of the tile before
+// have read it; without an activation and for ReLU dz has dy's digits and there
+// are none.  While the eight compute warps turn dy into dz for tile t, the products of tile t - 1
+// finish; they then store its dx while the tensor core forms z of tile t + 1, dW
+// and dx of tile t.  db is summed in registers from dz before its rounding.
 //
 // Bound by memory and by the latency of 16 compute warps to an SM: 64 -> 64 bf16
 // over 1600x1200 rows moves 737 MB in 152 us (112 us at the copy rate).
@@ -33,9 +35,11 @@ constexpr int kNarrowWidth = 128;
 
 __host__ __device__ inline int blocks64(int n) { return (n + 63) / 64; }
 
-// x and dy of two tiles, W, a patch per warp, the bias and db's joins.
-inline size_t narrow_bytes(int k, int n, int n32) {
-  return 2 * (blocks64(k) + blocks64(n)) * static_cast<size_t>(kAPlane) +
+// x and dy of two tiles, dz's second values, W, a patch per warp, the bias and
+// db's joins.
+inline size_t narrow_bytes(int k, int n, int n32, bool second) {
+  return (2 * (blocks64(k) + blocks64(n)) + (second ? blocks64(n) : 0)) *
+             static_cast<size_t>(kAPlane) +
          static_cast<size_t>(blocks64(k)) * n32 * 128 + 8 * 2048 + 5 * kNarrowWidth * 4 + 1024;
 }
 
@@ -50,12 +54,13 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
   __shared__ uint32_t tmem_base;
   const uint32_t base = (tc::shared_address(dynamic) + 1023u) & ~1023u;
   const uint32_t x_bytes = blocks64(p.k) * kAPlane, z_bytes = blocks64(p.n) * kAPlane;
-  const uint32_t x_at = base, z_at = x_at + 2 * x_bytes, w_at = z_at + 2 * z_bytes;
+  const bool with_z = p.activation != kNone, with_second = rounds_dz(p.activation);
+  const uint32_t x_at = base, z_at = x_at + 2 * x_bytes, second_at = z_at + 2 * z_bytes;
+  const uint32_t w_at = second_at + (with_second ? z_bytes : 0);
   const uint32_t w_block = p.n32 * 128;
   const uint32_t patch_at = w_at + blocks64(p.k) * w_block;
   const uint32_t bias_at = patch_at + 8 * 2048, join_at = bias_at + kNarrowWidth * 4;
   const int warp = tc::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const bool with_z = p.activation != kNone;
   const auto bar = [](const unsigned long long& b) { return tc::shared_address(&b); };
 
   if (threadIdx.x == 0) {
@@ -138,15 +143,21 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
           tc::mma_steps(lead, w_tmem, tc::descriptor_mn_major(z_now, z_block),
                         tc::descriptor_mn_major(x_now, kAPlane), tc::kStepMn, tc::kStepMn,
                         kTileRows / 16, w_instruction, i > 0);
+          if (with_second)
+            tc::mma_steps(lead, w_tmem, tc::descriptor_mn_major(second_at, z_block),
+                          tc::descriptor_mn_major(x_now, kAPlane), tc::kStepMn, tc::kStepMn,
+                          kTileRows / 16, w_instruction, true);
         }
         if (p.with_dx) {
           if (i > 0 && !(ok = tc::barrier_wait(bar(dx_read), (i - 1) & 1) && ok)) break;
           tc::fence_after_sync();
-          for (int c = 0; c * 64 < p.n; ++c)
-            tc::mma_steps(lead, dx_tmem, tc::descriptor_k_major(z_now + c * kAPlane),
-                          tc::descriptor_mn_major(w_at + c * 4 * tc::kStepMn, w_block),
-                          tc::kStepK, tc::kStepMn, min((p.n - c * 64 + 15) / 16, 4),
-                          dx_instruction, c > 0);
+          for (int part = 0; part <= (with_second ? 1 : 0); ++part)
+            for (int c = 0; c * 64 < p.n; ++c)
+              tc::mma_steps(lead, dx_tmem,
+                            tc::descriptor_k_major((part ? second_at : z_now) + c * kAPlane),
+                            tc::descriptor_mn_major(w_at + c * 4 * tc::kStepMn, w_block),
+                            tc::kStepK, tc::kStepMn, min((p.n - c * 64 + 15) / 16, 4),
+                            dx_instruction, part > 0 || c > 0);
         }
         tc::commit(lead, bar(dx_done));
         tc::commit(lead, bar(spent[b]));
@@ -168,7 +179,7 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
 #pragma unroll
       for (int j = 0; j < 16; ++j) sum_b[c][j] = pack2(0.0f, 0.0f);
 
-    const auto form_dz = [&](auto act, uint32_t z_row) {
+    const auto form_dz = [&](auto act, uint32_t z_row, uint32_t i_tile) {
       constexpr int ACT = decltype(act)::value;
 #pragma unroll
       for (int cc = 0; cc < C; ++cc) {
@@ -186,6 +197,7 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
           }
         }
         const uint32_t at = z_row + (c >> 1) * kAPlane;
+        const uint32_t to_second = second_at - (z_at + (i_tile & 1) * z_bytes);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t piece = at + ((((c & 1) * 4 + j) ^ turn) << 4);
@@ -201,11 +213,34 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
             }
             f32x2& sum = sum_b[cc][j * 4 + i / 2];
             sum = add2(sum, dz);
-            unpack2(dz, e[i], e[i + 1]);
+            if constexpr (ACT != kNone) unpack2(dz, v[j * 8 + i], v[j * 8 + i + 1]);
           }
-          if constexpr (ACT != kNone) {
+        }
+        if constexpr (ACT == kRelu) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = v[j * 8 + i];
             const Vec<T, 8> r = round_values<T, 8>(e);
-            store_shared(piece, reinterpret_cast<const uint4&>(r));
+            store_shared(at + ((((c & 1) * 4 + j) ^ turn) << 4), reinterpret_cast<const uint4&>(r));
+          }
+        }
+        if constexpr (rounds_dz(ACT)) {
+          // the products of the tile before have read its second values
+          if (cc == 0 && i_tile > 0 &&
+              !(ok = tc::barrier_wait(bar(dx_done), (i_tile - 1) & 1)))
+            return;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t piece = at + ((((c & 1) * 4 + j) ^ turn) << 4);
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = v[j * 8 + i];
+            const Vec<T, 8> first = take_first<T, 8>(e);
+            store_shared(piece, reinterpret_cast<const uint4&>(first));
+            const Vec<T, 8> second = round_values<T, 8>(e);
+            store_shared(piece + to_second, reinterpret_cast<const uint4&>(second));
           }
         }
       }
@@ -247,12 +282,13 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
       tc::fence_after_sync();
       const uint32_t z_row = z_at + b * z_bytes + row * 128;
       switch (p.activation) {
-        case kRelu: form_dz(std::integral_constant<int, kRelu>{}, z_row); break;
-        case kSilu: form_dz(std::integral_constant<int, kSilu>{}, z_row); break;
-        case kGelu: form_dz(std::integral_constant<int, kGelu>{}, z_row); break;
-        case kSigmoid: form_dz(std::integral_constant<int, kSigmoid>{}, z_row); break;
-        default: form_dz(std::integral_constant<int, kNone>{}, z_row);
+        case kRelu: form_dz(std::integral_constant<int, kRelu>{}, z_row, i); break;
+        case kSilu: form_dz(std::integral_constant<int, kSilu>{}, z_row, i); break;
+        case kGelu: form_dz(std::integral_constant<int, kGelu>{}, z_row, i); break;
+        case kSigmoid: form_dz(std::integral_constant<int, kSigmoid>{}, z_row, i); break;
+        default: form_dz(std::integral_constant<int, kNone>{}, z_row, i);
       }
+      if (!ok) break;
       tc::fence_async_proxy();
       tc::fence_before_sync();
       tc::barrier_arrive(bar(dz_ready[b]));

@@ -1,11 +1,11 @@
 // C(m, n) = sum_k A(m, k) B(n, k) on the tensor cores, with the epilogues of a
 // linear layer and its backward.
 //
-// Numbers.  Operands are 16-bit for tcgen05.mma.  What has more digits is
-// split into 2 or 3 bf16 parts, v = v0 + v1 + v2 with v_i rounded from what
-// v_0 .. v_{i-1} leave (8 digits each), and the products of parts i and j with
-// i + j < parts are summed: three parts reproduce an fp32 product to 2^-24, two
-// a 16-bit value exactly.  Accumulators are fp32 in tensor memory.
+// Numbers.  Operands are 16-bit for tcgen05.mma.  fp32 ones are split into three
+// bf16 parts, v = v0 + v1 + v2 with v_i rounded from what v_0 .. v_{i-1} leave (8
+// digits each), and the products of parts i and j with i + j < 3 are summed,
+// which reproduces an fp32 product to 2^-24.  The dz of 16-bit layers is two
+// values of their type (take_first).  Accumulators are fp32 in tensor memory.
 //
 // Work.  A persistent block takes 128 x NT tiles.  64-wide chunks of k go from
 // global memory into a ring of stages: 16-bit operands with 16-byte rows by
@@ -41,8 +41,9 @@ constexpr int kMaxStages = 8, kMaxAccumulators = 4;
 constexpr int kAPlane = kTileRows * 128;
 
 // Producer threads: operands that are split always pass through registers, so
-// there it is threads that keep loads in flight.
-__host__ __device__ constexpr int producers(int pa, int pb) { return pa == 1 && pb == 1 ? 128 : 256; }
+// there it is threads that keep loads in flight.  Two-part ones always lie in
+// memory as two planes and are copied.
+__host__ __device__ constexpr int producers(int pa, int pb) { return pa <= 2 && pb <= 2 ? 128 : 256; }
 // fp32 operands keep the products of lower parts in an accumulator of their
 // own: the tensor core truncates its sums, so each addition at full magnitude
 // costs up to 2^-24, and the lower products must not add to their number.
@@ -56,6 +57,7 @@ enum Epilogue : int { kForward = 0, kSlope = 1, kPlain = 2 };
 
 struct ProductParams {
   CUtensorMap a_map, b_map, extra_map, out_map;
+  CUtensorMap a_second_map, out_second_map;  // of the second of two parts
   int copy_operands, copy_extra, copy_out;  // by tensor copies
   // the operands' parts lie in memory as 16-bit planes of so many rows (0: they
   // are made on the way)
@@ -67,6 +69,7 @@ struct ProductParams {
   // row-major sources: A is (m, k) rows or, transposed, (k, m); B likewise
   const void* a;
   const void* b;
+  const void* a_second;  // A in two parts: the second's plane, like a's
   long long a_ld, b_ld;
   int a_vector, b_vector;  // bytes that every row start and chunk is aligned to
   long long k_per_split;   // a multiple of kChunk unless there is one split
@@ -81,7 +84,9 @@ struct ProductParams {
   uint32_t tmem_columns;
   const void* bias;   // (n) or NULL
   const void* extra;  // residual or dy (m, n), or NULL
-  void* out;          // (splits, m, n)
+  void* out;          // (splits, m, n), rows out_ld values apart
+  void* out_second;   // kSlope: dz in two parts, the second's plane; or NULL
+  long long out_ld;
   float* column_sums; // kSlope: (4 tiles_m, n) sums of dz over 32 rows each, or NULL
   int extra_vector, out_vector;  // their rows are whole 16-byte pieces
   int bias_shared;    // values of the bias kept in shared memory (0: too many)
@@ -324,11 +329,12 @@ SPLAT_DEV uint32_t chunk_bytes(int width, long long mn_valid) {
             : width * 128;
 }
 template <int P, bool MN>
-SPLAT_DEV void copy_chunk(const CUtensorMap* map, uint32_t dst, uint32_t plane, int plane_rows,
-                          int width, long long mn0, long long mn_valid, long long k0,
-                          uint32_t bar) {
+SPLAT_DEV void copy_chunk(const CUtensorMap* map, const CUtensorMap* second_map, uint32_t dst,
+                          uint32_t plane, int plane_rows, int width, long long mn0,
+                          long long mn_valid, long long k0, uint32_t bar) {
 #pragma unroll
   for (int i = 0; i < P; ++i, dst += plane) {
+    if (P == 2 && i == 1) map = second_map, plane_rows = 0;
     if constexpr (MN) {
       for (int b = 0; b * 64 < width && b * 64 < mn_valid; ++b)
         tc::copy_in(dst + b * (kChunk * 128), map, static_cast<int>(mn0) + b * 64,
@@ -655,8 +661,9 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
           const uint32_t bar = tc::shared_address(&resident_full);
           tc::barrier_expect(bar, chunks_all * PB * chunk_bytes<BMN>(p.tile_n, p.n));
           for (int c = 0; c < chunks_all; ++c)
-            copy_chunk<PB, BMN>(&p.b_map, resident + c * b_bytes, b_plane, p.b_plane_rows, p.tile_n,
-                                0, p.n, static_cast<long long>(c) * kChunk, bar);
+            copy_chunk<PB, BMN>(&p.b_map, nullptr, resident + c * b_bytes, b_plane,
+                                p.b_plane_rows, p.tile_n, 0, p.n,
+                                static_cast<long long>(c) * kChunk, bar);
         }
         int started = 0;  // stages that have been filled at least once
         for (uint32_t t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
@@ -668,11 +675,11 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
                                PA * chunk_bytes<AMN>(kTileRows, p.m - tile.m0) +
                                    (p.resident ? 0
                                                : PB * chunk_bytes<BMN>(p.tile_n, p.n - tile.n0)));
-            copy_chunk<PA, AMN>(&p.a_map, at, kAPlane, p.a_plane_rows, kTileRows, tile.m0,
-                                p.m - tile.m0, k, bar);
+            copy_chunk<PA, AMN>(&p.a_map, &p.a_second_map, at, kAPlane, p.a_plane_rows,
+                                kTileRows, tile.m0, p.m - tile.m0, k, bar);
             if (!p.resident)
-              copy_chunk<PB, BMN>(&p.b_map, at + a_bytes, b_plane, p.b_plane_rows, p.tile_n,
-                                  tile.n0, p.n - tile.n0, k, bar);
+              copy_chunk<PB, BMN>(&p.b_map, nullptr, at + a_bytes, b_plane, p.b_plane_rows,
+                                  p.tile_n, tile.n0, p.n - tile.n0, k, bar);
             started = max(started, stage + 1);
             if (++stage == p.stages) stage = 0, parity ^= 1;
           }
@@ -683,7 +690,7 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
         for (int i = 0; i < started; ++i)
           ok = tc::barrier_wait(tc::shared_address(&full[i]), i < stage ? parity ^ 1 : parity) && ok;
       }
-    } else {
+    } else if constexpr (PA != 2) {
       const SA* a = static_cast<const SA*>(p.a);
       const SB* b = static_cast<const SB*>(p.b);
       if (p.resident) {
@@ -773,7 +780,7 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
     // ---- one warp issues the products
     {
       const uint32_t lead = tc::elected();
-      constexpr bool kBf16 = !(PA == 1 && PB == 1 && kIsF16<SA>);
+      constexpr bool kBf16 = !kIsF16<SA>;
       constexpr int kParts = PA > PB ? PA : PB;
       // the part of A in the first product of the smallest kind
       constexpr int first_part = kParts - 1 < PB ? 0 : kParts - PB;
@@ -873,7 +880,7 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
       const ProductTile tile(p, t);
       const long long row0 = tile.m0 + lane_block * 32;
       const int rows = static_cast<int>(min(p.m - row0, 32LL));
-      TO* out = static_cast<TO*>(p.out) + (tile.split * p.m + row0) * p.n;
+      const long long out_at = (tile.split * p.m + row0) * p.out_ld;
       for (long long sum_k = tile.k0; sum_k < tile.k1; sum_k += p.k_per_sum) {
         bool waited = false;
         const uint32_t acc = i_acc & (p.accumulators - 1);
@@ -954,25 +961,44 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
                 fetch_extra(ProductTile(p, t + t_step), c_first);
             }
           }
-          if (leader && p.copy_out) tc::copies_out_read();
-          __syncwarp();  // the results before have left the patch
+          // first: round to what leaves a second value, which v becomes
+          const auto put = [&](auto first, const CUtensorMap* map, void* out) {
+            if (leader && p.copy_out) tc::copies_out_read();
+            __syncwarp();  // the results before have left the patch
 #pragma unroll
-          for (int j = 0; j < Patch<TO>::kPieces; ++j) {
-            constexpr int V = Patch<TO>::V;
-            float o[V];
+            for (int j = 0; j < Patch<TO>::kPieces; ++j) {
+              constexpr int V = Patch<TO>::V;
+              float o[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = v[j * V + i];
-            const Vec<TO, V> r = round_values<TO, V>(o);
-            store_shared(out_patch.at(threadIdx.x & 31, j), reinterpret_cast<const uint4&>(r));
+              for (int i = 0; i < V; ++i) o[i] = v[j * V + i];
+              Vec<TO, V> r;
+              if constexpr (decltype(first)::value) {
+                r = take_first<TO, V>(o);
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[j * V + i] = o[i];
+              } else {
+                r = round_values<TO, V>(o);
+              }
+              store_shared(out_patch.at(threadIdx.x & 31, j), reinterpret_cast<const uint4&>(r));
+            }
+            if (p.copy_out) {
+              tc::fence_async_proxy();
+              __syncwarp();
+              if (leader) tc::copy_out(map, col0, static_cast<int>(row0), out_patch.base);
+            } else {
+              __syncwarp();
+              out_patch.store(static_cast<TO*>(out) + out_at + col0, p.out_ld, rows, cols,
+                              p.out_vector, sum_k != tile.k0);
+            }
+          };
+          if constexpr (EPI == kSlope && sizeof(TO) == 2) {
+            if (p.out_second) {
+              put(std::true_type{}, &p.out_map, p.out);
+              put(std::false_type{}, &p.out_second_map, p.out_second);
+              continue;
+            }
           }
-          if (p.copy_out) {
-            tc::fence_async_proxy();
-            __syncwarp();
-            if (leader) tc::copy_out(&p.out_map, col0, static_cast<int>(row0), out_patch.base);
-          } else {
-            __syncwarp();
-            out_patch.store(out + col0, p.n, rows, cols, p.out_vector, sum_k != tile.k0);
-          }
+          put(std::false_type{}, &p.out_map, p.out);
         }
         if (!ok) break;
         if (!waited) {  // a warp without a patch still takes part

@@ -10,9 +10,9 @@ the per-Gaussian features that they blend from.
 Tensors are CUDA float32, bfloat16 or float16, all of one type per call (no
 autocast).  Sums are held in fp32 or more and rounded once to that type, and
 no result depends on the order in which blocks run.  The backward of a 16-bit
-`linear` takes dy act'(z) in that type, as mixed-precision training does:
-values below or above float16's range are lost there, so float16 losses want
-their usual scale.  Any strides are taken; what is not contiguous is copied
+`linear` keeps dy act'(z) as two values of that type (2^-16 relative for
+bfloat16, 2^-22 for float16, whose smallest value is 2^-24: float16 losses want
+their usual scale).  Any strides are taken; what is not contiguous is copied
 first.  First-order gradients only.  In float32 the products of non-finite
 values are NaN where IEEE arithmetic would give an infinity.
 

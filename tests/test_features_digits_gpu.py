@@ -1,0 +1,104 @@
+"""Digits of the feature operators: sums, intermediate values and activations
+at the sizes and values where they could be lost.
+
+Tolerances are bounds on roundings, counted as in test_features_gpu: u = 2^-23
+for an fp32 operation (the tensor core truncates its sums), h = eps(dtype) / 2
+for the one rounding to the output's type.
+"""
+
+import math
+
+import pytest
+import torch
+
+from dsl_splat_b200 import features
+from test_features_gpu import (ACTS, DTYPES, U, check, draws, half_step, smallest,
+                               value_and_slope)
+
+pytestmark = pytest.mark.gpu
+HALF = (torch.bfloat16, torch.float16)
+
+
+# ---- dz = dy act'(z) between the products of the backward ------------------------
+
+# the one-pass kernels (16-byte rows, other rows), the products (16-byte rows,
+# other rows of few and of many), on either side of 64 and 128 features
+DZ_SIZES = [(300, 64, 64), (700, 128, 128), (5000, 32, 24), (300, 35, 64), (513, 33, 25),
+            (700, 100, 72), (400, 127, 101), (520, 264, 200), (400, 300, 17), (300, 17, 300),
+            (333, 301, 201), (17000, 301, 33), (16500, 136, 200), (9000, 512, 512)]
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid", "relu"])
+@pytest.mark.parametrize("m, k, n", DZ_SIZES)
+def test_gradients_round_once(m, k, n, act, dtype):
+    """dx and dW of 16-bit types are off by their own rounding and little else:
+    dz is kept as two values of the type, h^2 relative (and half the type's
+    smallest value) off."""
+    normal = draws(41)
+    x, w, b = (normal(*s, dtype=dtype) for s in ((m, k), (n, k), (n,)))
+    w = w / 16
+    dy = normal(m, n, dtype=dtype)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = features.linear(*leaves, activation=act)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    xd, wd, dyd = (t.detach().double() for t in (x, w, dy))
+    z = xd @ wd.t() + b.detach().double()
+    e_z = (k + 8) * U * (xd.abs() @ wd.abs().t() + b.detach().double().abs())
+    _, rate = value_and_slope(z, act)
+    dz = dyd * rate
+    # the slope: 16 u of its terms and its argument's error; for GELU 2^-15 more,
+    # half (the largest tail) of the 2^-14 that the tails of 16-bit types may be off
+    e_dz = dyd.abs() * (1.2 * e_z + 16 * U * (1 + z.abs()) + 2.0 ** -15 * (act == "gelu"))
+    if act == "relu":
+        e_dz = dyd.abs() * ((z.abs() <= e_z).double() + U)
+    e_dz = e_dz + half_step(dtype) ** 2 * (dz.abs() + e_dz) + smallest(dtype)
+    # a product's sums truncate at most once for 16 terms of each of two parts
+    check(dx, dz @ wd, (n / 8 + 16) * U * (dz.abs() @ wd.abs()) + e_dz @ wd.abs(), "dx")
+    check(dw, dz.t() @ xd, (min(m, 8192) / 8 + 16) * U * (dz.abs().t() @ xd.abs())
+          + e_dz.t() @ xd.abs(), "dw")
+
+
+def test_gradients_beyond_the_types_range():
+    """act' is up to 1.13: a dz above fp16's largest value does not spoil what
+    is formed from it."""
+    for k, n in ((64, 64), (35, 20), (264, 200), (301, 37)):
+        x = torch.zeros(256, k, device="cuda", dtype=torch.float16)
+        x[:, 0] = 1.5
+        w = torch.zeros(n, k, device="cuda", dtype=torch.float16)
+        w[:, 0] = 1.0
+        w[:, 1] = 2.0 ** -10
+        dy = torch.zeros(256, n, device="cuda", dtype=torch.float16)
+        dy[:, 3] = 65504.0
+        x.requires_grad_()
+        y = features.linear(x, w, activation="gelu")
+        dx, = torch.autograd.grad(y, x, dy)
+        _, rate = value_and_slope(torch.tensor(1.5, dtype=torch.float64), "gelu")
+        want = 65504.0 * float(rate) * 2.0 ** -10
+        assert float(rate) > 1.1
+        # its own rounding, and that of the second part: 4 of 73857
+        assert ((dx[:, 1].double() - want).abs() <= (2.0 ** -11 + 2.0 ** -13) * want).all()
+
+
+@pytest.mark.parametrize("k, n", [(64, 64), (35, 20), (264, 200), (301, 37)])
+@pytest.mark.parametrize("dtype", HALF)
+def test_infinite_gradients_stay_infinite(k, n, dtype):
+    """An infinite dy gives infinities, as the one value dz would, and spoils
+    no other row."""
+    normal = draws(42)
+    x, w, dy = (normal(*s, dtype=dtype) for s in ((300, k), (n, k), (300, n)))
+    w = w.abs() + 0.25
+    x.requires_grad_()
+
+    def run(dy):
+        y = features.linear(x, w, activation="sigmoid")
+        return torch.autograd.grad(y, x, dy)[0]
+
+    clean = run(dy)
+    dy = dy.clone()
+    dy[130, 1] = float("inf")
+    x.data[130] = 0.01
+    spoilt = run(dy)
+    keep = torch.arange(300, device="cuda") != 130
+    assert torch.equal(spoilt[keep], clean[keep])
+    assert (spoilt[130] == float("inf")).all()
