@@ -122,13 +122,9 @@ def _recorded(*tensors: Tensor | None) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
-def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *,
-           residual: Tensor | None = None, activation: str = "none") -> Tensor:
-    """act(x weight^T + bias) + residual over the last dimension of x.
-
-    x: (...,K), weight: (N,K), bias: (N,), residual and the result: (...,N).
-    activation: "none", "relu", "silu", "gelu" (the erf form) or "sigmoid".
-    """
+def check_linear(x: Tensor, weight: Tensor, bias: Tensor | None, activation: str,
+                 **outputs: Tensor | None) -> None:
+    """Refuses what `linear` does not take; outputs: tensors of the result's shape."""
     _check_activation(activation)
     _check_input(x)
     if x.ndim < 1 or x.shape[-1] < 1:
@@ -139,13 +135,41 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *,
     n = weight.shape[0]
     _check_like(weight, x, (n, k), "weight")
     _check_like(bias, x, (n,), "bias")
-    shape = x.shape[:-1] + (n,)
-    _check_like(residual, x, shape, "residual")
+    for name, t in outputs.items():
+        _check_like(t, x, x.shape[:-1] + (n,), name)
     if k > 65535 or n > 65535:
         raise ValueError("at most 65535 input and output features")
+
+
+def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *,
+           residual: Tensor | None = None, activation: str = "none") -> Tensor:
+    """act(x weight^T + bias) + residual over the last dimension of x.
+
+    x: (...,K), weight: (N,K), bias: (N,), residual and the result: (...,N).
+    activation: "none", "relu", "silu", "gelu" (the erf form) or "sigmoid".
+    """
+    check_linear(x, weight, bias, activation, residual=residual)
     if _recorded(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, residual, activation)
     return stages.feature_linear(x, weight, bias, residual, activation)
+
+
+def check_group_norm(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None,
+                     eps: float, activation: str, samples: int, positions: int) -> None:
+    """Refuses what `group_norm` does not take, for an x of at least a dimension
+    whose leading ones hold so many samples and positions."""
+    _check_activation(activation)
+    channels = x.shape[-1]
+    if isinstance(groups, bool) or not isinstance(groups, Integral) or groups < 1:
+        raise ValueError("groups must be a positive integer")
+    if channels % groups:
+        raise ValueError(f"groups must divide the channels: {channels} channels, {groups} groups")
+    _check_like(weight, x, (channels,), "weight")
+    _check_like(bias, x, (channels,), "bias")
+    if not math.isfinite(eps) or eps <= 0:
+        raise ValueError("eps must be finite and positive")
+    if positions > (1 << 31) - 1 or positions * channels > 1 << 40 or samples * channels > 1 << 30:
+        raise ValueError("too many positions or samples")
 
 
 def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tensor | None = None,
@@ -164,19 +188,9 @@ def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tenso
         raise ValueError("spatial_dims must be an integer of at least one")
     if x.ndim < spatial_dims + 1 or x.shape[-1] < 1:
         raise ValueError("x must have spatial_dims dimensions and at least one channel last")
-    channels = x.shape[-1]
-    if isinstance(groups, bool) or not isinstance(groups, Integral) or groups < 1:
-        raise ValueError("groups must be a positive integer")
-    if channels % groups:
-        raise ValueError(f"groups must divide the channels: {channels} channels, {groups} groups")
-    _check_like(weight, x, (channels,), "weight")
-    _check_like(bias, x, (channels,), "bias")
-    if not math.isfinite(eps) or eps <= 0:
-        raise ValueError("eps must be finite and positive")
     samples = math.prod(x.shape[:-1 - spatial_dims])
     positions = math.prod(x.shape[-1 - spatial_dims:-1])
-    if positions > (1 << 31) - 1 or positions * channels > 1 << 40 or samples * channels > 1 << 30:
-        raise ValueError("too many positions or samples")
+    check_group_norm(x, groups, weight, bias, eps, activation, samples, positions)
     groups, eps = int(groups), float(eps)
     if _recorded(x, weight, bias):
         return _GroupNorm.apply(x, weight, bias, samples, groups, eps, activation)

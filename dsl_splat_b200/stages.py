@@ -799,6 +799,7 @@ def feature_norm_backward(x: Tensor, samples: int, groups: int, weight: Tensor |
                       positions, channels, groups, 1)
         ws = x.new_empty((size,), dtype=torch.uint8)
         x, weight, bias, upstream = _dense(x), _dense(weight), _dense(bias), _dense(upstream)
+        moments = _dense(moments)
         mean = moments.data_ptr()
         _call(lib.splat_feature_norm_backward, "feature_norm_backward", device, dtype, samples,
               positions, channels, groups, x.data_ptr(), _address(weight), _address(bias), mean,

@@ -6,7 +6,8 @@ fake implementation that gives output shapes and dtypes without running the
 kernels -- so the stages trace under FakeTensorMode, torch.compile and
 torch.export.  The differentiable ones (`project`, `sh_forward`, `render`)
 carry autograd formulas that call the backward operators, so a graph built
-from them stays inside torch.ops.splat200.
+from them stays inside torch.ops.splat200.  The feature operators check their
+arguments as `features` does, in their fake forms too.
 
 Binning's pair count is data-dependent: its fake kernel returns an unbacked
 size for point_list, which is what the reference's `.item()` read
@@ -33,10 +34,12 @@ Operator <- reference code it stands for:
 
 from __future__ import annotations
 
+import math
+
 import torch
 from torch import Tensor
 
-from . import stages
+from . import features, stages
 
 _NS = "splat200"
 
@@ -503,26 +506,46 @@ rade_render.register_autograd(_rade_render_backward, setup_context=_rade_render_
 
 # ---- feature operators ----------------------------------------------------------
 
+def _check_norm(x, groups, weight, bias, eps, activation):
+    features._check_input(x)
+    if x.ndim < 2 or x.shape[-1] < 1:
+        raise ValueError("x must have samples first and at least one channel last")
+    features.check_group_norm(x, groups, weight, bias, eps, activation, x.shape[0],
+                              math.prod(x.shape[1:-1]))
+
+
+def _check_norm_backward(x, groups, weight, bias, moments, activation, upstream):
+    _check_norm(x, groups, weight, bias, 1.0, activation)
+    features._check_like(upstream, x, x.shape, "upstream")
+    if (moments.dtype is not torch.float32 or moments.device != x.device
+            or moments.shape != (2, x.shape[0], groups)):
+        raise ValueError("moments must be the float32 (2,samples,groups) of feature_norm")
+
+
 @torch.library.custom_op(f"{_NS}::feature_linear", mutates_args=())
 def feature_linear(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None,
                    activation: str) -> Tensor:
+    features.check_linear(x, weight, bias, activation, residual=residual)
     return stages.feature_linear(x, weight, bias, residual, activation)
 
 
 @feature_linear.register_fake
 def _(x, weight, bias, residual, activation):
+    features.check_linear(x, weight, bias, activation, residual=residual)
     return x.new_empty(x.shape[:-1] + (weight.shape[0],))
 
 
 @torch.library.custom_op(f"{_NS}::feature_linear_backward", mutates_args=())
 def feature_linear_backward(x: Tensor, weight: Tensor, bias: Tensor | None, activation: str,
                             upstream: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    features.check_linear(x, weight, bias, activation, upstream=upstream)
     return stages.feature_linear_backward(x, weight, bias, activation, upstream,
                                           (True, True, True))
 
 
 @feature_linear_backward.register_fake
 def _(x, weight, bias, activation, upstream):
+    features.check_linear(x, weight, bias, activation, upstream=upstream)
     return x.new_empty(x.shape), weight.new_empty(weight.shape), x.new_empty((weight.shape[0],))
 
 
@@ -545,11 +568,13 @@ feature_linear.register_autograd(_feature_linear_backward, setup_context=_featur
 @torch.library.custom_op(f"{_NS}::feature_norm", mutates_args=())
 def feature_norm(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None, eps: float,
                  activation: str) -> tuple[Tensor, Tensor]:
+    _check_norm(x, groups, weight, bias, eps, activation)
     return stages.feature_norm(x, x.shape[0], groups, weight, bias, eps, activation)
 
 
 @feature_norm.register_fake
 def _(x, groups, weight, bias, eps, activation):
+    _check_norm(x, groups, weight, bias, eps, activation)
     return x.new_empty(x.shape), x.new_empty((2, x.shape[0], groups), dtype=torch.float32)
 
 
@@ -557,12 +582,14 @@ def _(x, groups, weight, bias, eps, activation):
 def feature_norm_backward(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None,
                           moments: Tensor, activation: str, upstream: Tensor
                           ) -> tuple[Tensor, Tensor, Tensor]:
+    _check_norm_backward(x, groups, weight, bias, moments, activation, upstream)
     return stages.feature_norm_backward(x, x.shape[0], groups, weight, bias, moments, activation,
                                         upstream, (True, True, True))
 
 
 @feature_norm_backward.register_fake
 def _(x, groups, weight, bias, moments, activation, upstream):
+    _check_norm_backward(x, groups, weight, bias, moments, activation, upstream)
     return (x.new_empty(x.shape), x.new_empty((x.shape[-1],)), x.new_empty((x.shape[-1],)))
 
 

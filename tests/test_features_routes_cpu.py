@@ -1,0 +1,113 @@
+"""Feature operators without a GPU: the calls that reach them by torch.ops."""
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import dsl_splat_b200  # noqa: F401  (registers the operators)
+
+ops = torch.ops.splat200
+
+
+def fake(*shape, dtype=torch.float32, device="cuda"):
+    return torch.empty(shape, device=device, dtype=dtype)
+
+
+LINEAR = dict(x=(6, 3), weight=(4, 3), bias=(4,), residual=(6, 4))
+
+
+def linear_tensors(change):
+    dtypes = {m: change.get(m + "_dtype", torch.float32) for m in LINEAR}
+    return [fake(*change.get(m, LINEAR[m]), dtype=dtypes[m],
+                 device=change.get(m + "_device", "cuda")) for m in LINEAR]
+
+
+LINEAR_CHANGES = [
+    (dict(x=(8, 6), weight=(4, 3)), "weight must have shape"),
+    (dict(weight=(4, 5)), "weight must have shape"),
+    (dict(weight=(4,)), r"weight must be \(N,K\)"),
+    (dict(bias=(1,)), "bias must have shape"),
+    (dict(residual=(3, 4)), "residual must have shape"),
+    (dict(weight_dtype=torch.bfloat16), "weight must have x's dtype"),
+    (dict(bias_dtype=torch.float16), "bias must have x's dtype"),
+    (dict(residual_dtype=torch.float64), "residual must have x's dtype"),
+    (dict(weight_device="cpu"), "weight must have x's dtype and device"),
+    (dict(x_device="cpu"), "x must be a CUDA"),
+    (dict(x_dtype=torch.float64), "x must be a CUDA"),
+    (dict(x=(1, 70000), weight=(4, 70000), residual=(1, 4)), "65535"),
+]
+
+
+@pytest.mark.parametrize("change, message", LINEAR_CHANGES)
+def test_linear_op_refusals(change, message):
+    with FakeTensorMode():
+        with pytest.raises(ValueError, match=message):
+            ops.feature_linear(*linear_tensors(change), "silu")
+
+
+def test_linear_op_refuses_unknown_activations():
+    with FakeTensorMode():
+        with pytest.raises(ValueError, match="activation"):
+            ops.feature_linear(*linear_tensors({}), "tanh")
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(x=(8, 6), weight=(4, 3)), "weight must have shape"),
+    (dict(bias=(1,)), "bias must have shape"),
+    (dict(weight_dtype=torch.bfloat16), "weight must have x's dtype"),
+    (dict(upstream=(5, 4)), "upstream must have shape"),
+    (dict(upstream_dtype=torch.float16), "upstream must have x's dtype"),
+    (dict(activation="tanh"), "activation"),
+])
+def test_linear_backward_op_refusals(change, message):
+    with FakeTensorMode():
+        x, weight, bias, _ = linear_tensors(change)
+        upstream = fake(*change.get("upstream", (6, 4)),
+                        dtype=change.get("upstream_dtype", torch.float32))
+        with pytest.raises(ValueError, match=message):
+            ops.feature_linear_backward(x, weight, bias, change.get("activation", "silu"), upstream)
+
+
+NORM_CHANGES = [
+    (dict(groups=3), "groups must divide"),
+    (dict(groups=0), "groups must be a positive"),
+    (dict(eps=-1.0), "eps must be finite"),
+    (dict(eps=float("inf")), "eps must be finite"),
+    (dict(activation="swish"), "activation"),
+    (dict(weight=(7,)), "weight must have shape"),
+    (dict(bias=(9,)), "bias must have shape"),
+    (dict(weight_dtype=torch.bfloat16), "weight must have x's dtype"),
+    (dict(x=(8,)), "x must have"),
+    (dict(x_device="cpu"), "x must be a CUDA"),
+]
+
+
+@pytest.mark.parametrize("change, message", NORM_CHANGES)
+def test_norm_op_refusals(change, message):
+    with FakeTensorMode():
+        x = fake(*change.get("x", (2, 5, 8)), device=change.get("x_device", "cuda"))
+        weight = fake(*change.get("weight", (8,)), dtype=change.get("weight_dtype", torch.float32))
+        bias = fake(*change.get("bias", (8,)))
+        with pytest.raises(ValueError, match=message):
+            ops.feature_norm(x, change.get("groups", 2), weight, bias, change.get("eps", 1e-5),
+                             change.get("activation", "silu"))
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(groups=3), "groups must divide"),
+    (dict(upstream=(2, 4, 8)), "upstream must have shape"),
+    (dict(upstream_dtype=torch.float16), "upstream must have x's dtype"),
+    (dict(moments=(2, 2, 4)), "moments must be"),
+    (dict(moments_dtype=torch.float64), "moments must be"),
+    (dict(weight=(7,)), "weight must have shape"),
+])
+def test_norm_backward_op_refusals(change, message):
+    with FakeTensorMode():
+        moments = fake(*change.get("moments", (2, 2, 2)),
+                       dtype=change.get("moments_dtype", torch.float32))
+        upstream = fake(*change.get("upstream", (2, 5, 8)),
+                        dtype=change.get("upstream_dtype", torch.float32))
+        with pytest.raises(ValueError, match=message):
+            ops.feature_norm_backward(fake(2, 5, 8), change.get("groups", 2),
+                                      fake(*change.get("weight", (8,))), None, moments, "silu",
+                                      upstream)
