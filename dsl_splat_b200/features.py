@@ -13,7 +13,8 @@ no result depends on the order in which blocks run.  The backward of a 16-bit
 `linear` keeps dy act'(z) as two values of that type (2^-16 relative for
 bfloat16, 2^-22 for float16, whose smallest value is 2^-24: float16 losses want
 their usual scale).  Any strides are taken; what is not contiguous is copied
-first.  First-order gradients only.  In float32 the products of non-finite
+first.  First-order reverse-mode gradients only; forward-mode ones and torch.func's
+transforms are refused.  In float32 the products of non-finite
 values are NaN where IEEE arithmetic would give an infinity.
 
 A device-side wait that gives up (a defect, not a user's error) sets the
@@ -37,6 +38,7 @@ from typing import Any, Iterator
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import stages
@@ -117,6 +119,14 @@ def _check_like(t: Tensor | None, x: Tensor, shape: tuple, name: str) -> None:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
+def _check_forward_mode(*tensors: Tensor | None) -> None:
+    """Refuses dual tensors: a result without a tangent would pass for a
+    derivative of zero."""
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("forward-mode derivatives of the feature operators")
+
+
 def _recorded(*tensors: Tensor | None) -> bool:
     """Whether autograd has to know of a call."""
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
@@ -149,6 +159,7 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *,
     activation: "none", "relu", "silu", "gelu" (the erf form) or "sigmoid".
     """
     check_linear(x, weight, bias, activation, residual=residual)
+    _check_forward_mode(x, weight, bias, residual)
     if _recorded(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, residual, activation)
     return stages.feature_linear(x, weight, bias, residual, activation)
@@ -191,6 +202,7 @@ def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tenso
     samples = math.prod(x.shape[:-1 - spatial_dims])
     positions = math.prod(x.shape[-1 - spatial_dims:-1])
     check_group_norm(x, groups, weight, bias, eps, activation, samples, positions)
+    _check_forward_mode(x, weight, bias)
     groups, eps = int(groups), float(eps)
     if _recorded(x, weight, bias):
         return _GroupNorm.apply(x, weight, bias, samples, groups, eps, activation)

@@ -38,6 +38,7 @@ import math
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import features, stages
 
@@ -506,7 +507,20 @@ rade_render.register_autograd(_rade_render_backward, setup_context=_rade_render_
 
 # ---- feature operators ----------------------------------------------------------
 
+def _check_forward_mode():
+    # an operator without a formula for them drops tangents; in torch.func.jvp it
+    # does not see which of its arguments had one
+    if forward_ad._current_level >= 0:
+        raise NotImplementedError("forward-mode derivatives of the feature operators")
+
+
+def _check_linear(x, weight, bias, activation, **outputs):
+    _check_forward_mode()
+    features.check_linear(x, weight, bias, activation, **outputs)
+
+
 def _check_norm(x, groups, weight, bias, eps, activation):
+    _check_forward_mode()
     features._check_input(x)
     if x.ndim < 2 or x.shape[-1] < 1:
         raise ValueError("x must have samples first and at least one channel last")
@@ -525,27 +539,27 @@ def _check_norm_backward(x, groups, weight, bias, moments, activation, upstream)
 @torch.library.custom_op(f"{_NS}::feature_linear", mutates_args=())
 def feature_linear(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None,
                    activation: str) -> Tensor:
-    features.check_linear(x, weight, bias, activation, residual=residual)
+    _check_linear(x, weight, bias, activation, residual=residual)
     return stages.feature_linear(x, weight, bias, residual, activation)
 
 
 @feature_linear.register_fake
 def _(x, weight, bias, residual, activation):
-    features.check_linear(x, weight, bias, activation, residual=residual)
+    _check_linear(x, weight, bias, activation, residual=residual)
     return x.new_empty(x.shape[:-1] + (weight.shape[0],))
 
 
 @torch.library.custom_op(f"{_NS}::feature_linear_backward", mutates_args=())
 def feature_linear_backward(x: Tensor, weight: Tensor, bias: Tensor | None, activation: str,
                             upstream: Tensor) -> tuple[Tensor, Tensor, Tensor]:
-    features.check_linear(x, weight, bias, activation, upstream=upstream)
+    _check_linear(x, weight, bias, activation, upstream=upstream)
     return stages.feature_linear_backward(x, weight, bias, activation, upstream,
                                           (True, True, True))
 
 
 @feature_linear_backward.register_fake
 def _(x, weight, bias, activation, upstream):
-    features.check_linear(x, weight, bias, activation, upstream=upstream)
+    _check_linear(x, weight, bias, activation, upstream=upstream)
     return x.new_empty(x.shape), weight.new_empty(weight.shape), x.new_empty((weight.shape[0],))
 
 

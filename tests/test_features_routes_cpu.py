@@ -1,10 +1,12 @@
-"""Feature operators without a GPU: the calls that reach them by torch.ops."""
+"""Feature operators without a GPU: the calls that reach them by torch.ops and under
+forward-mode differentiation."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 from torch._subclasses.fake_tensor import FakeTensorMode
 
-import dsl_splat_b200  # noqa: F401  (registers the operators)
+from dsl_splat_b200 import features
 
 ops = torch.ops.splat200
 
@@ -111,3 +113,28 @@ def test_norm_backward_op_refusals(change, message):
             ops.feature_norm_backward(fake(2, 5, 8), change.get("groups", 2),
                                       fake(*change.get("weight", (8,))), None, moments, "silu",
                                       upstream)
+
+
+def test_forward_mode_is_refused():
+    with FakeTensorMode(), fwAD.dual_level():
+        x, w = fake(6, 3), fake(4, 3)
+        dual = fwAD.make_dual(x, torch.ones_like(x))
+        for call in (lambda: features.linear(dual, w),
+                     lambda: features.linear(x, fwAD.make_dual(w, torch.ones_like(w))),
+                     lambda: features.linear(x, w, residual=fwAD.make_dual(fake(6, 4),
+                                                                           fake(6, 4))),
+                     lambda: features.group_norm(dual[None], 3, spatial_dims=1)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+
+
+def test_forward_mode_operators_are_refused():
+    with FakeTensorMode(), fwAD.dual_level():
+        x, w = fake(6, 3), fake(4, 3)
+        dual = fwAD.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ops.feature_linear(dual, w, None, None, "silu")
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ops.feature_norm(dual[None], 3, None, None, 1e-5, "silu")
