@@ -127,6 +127,14 @@ def _check_forward_mode(*tensors: Tensor | None) -> None:
         raise NotImplementedError("forward-mode derivatives of the feature operators")
 
 
+def _traced() -> bool:
+    """Whether a program is being recorded: then the calls go through
+    torch.ops.splat200, which it can hold (a launch through the C ABI leaves
+    only the allocation of its result in it)."""
+    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+            or torch._C._get_tracing_state() is not None)
+
+
 def _recorded(*tensors: Tensor | None) -> bool:
     """Whether autograd has to know of a call."""
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
@@ -160,6 +168,8 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *,
     """
     check_linear(x, weight, bias, activation, residual=residual)
     _check_forward_mode(x, weight, bias, residual)
+    if _traced():
+        return torch.ops.splat200.feature_linear(x, weight, bias, residual, activation)
     if _recorded(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, residual, activation)
     return stages.feature_linear(x, weight, bias, residual, activation)
@@ -204,6 +214,10 @@ def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tenso
     check_group_norm(x, groups, weight, bias, eps, activation, samples, positions)
     _check_forward_mode(x, weight, bias)
     groups, eps = int(groups), float(eps)
+    if _traced():
+        shape = (samples, positions, x.shape[-1])
+        return torch.ops.splat200.feature_norm(x.reshape(shape), groups, weight, bias, eps,
+                                               activation)[0].reshape(x.shape)
     if _recorded(x, weight, bias):
         return _GroupNorm.apply(x, weight, bias, samples, groups, eps, activation)
     return stages.feature_norm(x, samples, groups, weight, bias, eps, activation, False)[0]

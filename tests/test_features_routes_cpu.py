@@ -1,10 +1,11 @@
-"""Feature operators without a GPU: the calls that reach them by torch.ops and under
-forward-mode differentiation."""
+"""Feature operators without a GPU: the calls that reach them by torch.ops, under
+forward-mode differentiation and while a program is traced."""
 
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from dsl_splat_b200 import features
 
@@ -138,3 +139,26 @@ def test_forward_mode_operators_are_refused():
             ops.feature_linear(dual, w, None, None, "silu")
         with pytest.raises(NotImplementedError, match="forward-mode"):
             ops.feature_norm(dual[None], 3, None, None, 1e-5, "silu")
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_traced_programs_hold_the_operators(grad):
+    def run(x, w, b):
+        y = features.linear(x, w, b, activation="silu")
+        return features.group_norm(y[None], 2, spatial_dims=1)
+
+    with FakeTensorMode():
+        tensors = [fake(*s).requires_grad_(grad) for s in ((6, 3), (4, 3), (4,))]
+        graph = make_fx(run)(*tensors)
+    called = [n.target for n in graph.graph.nodes if n.op == "call_function"]
+    assert ops.feature_linear.default in called
+    assert ops.feature_norm.default in called
+
+
+def test_traced_shapes():
+    with FakeTensorMode():
+        assert features.linear(fake(2, 5, 3), fake(4, 3)).shape == (2, 5, 4)
+        assert features.linear(fake(3), fake(4, 3)).shape == (4,)
+        assert features.group_norm(fake(3, 2, 5, 7, 8), 4).shape == (3, 2, 5, 7, 8)
+        assert features.group_norm(fake(5, 8), 4, spatial_dims=1).shape == (5, 8)
+        assert features.group_norm(fake(0, 4, 4, 8), 4).shape == (0, 4, 4, 8)
