@@ -187,8 +187,8 @@ def check_group_norm(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor
         raise ValueError(f"groups must divide the channels: {channels} channels, {groups} groups")
     _check_like(weight, x, (channels,), "weight")
     _check_like(bias, x, (channels,), "bias")
-    if not math.isfinite(eps) or eps <= 0:
-        raise ValueError("eps must be finite and positive")
+    if not 2.0 ** -126 <= eps < 2.0 ** 128:  # the kernels take it in fp32
+        raise ValueError("eps must be finite and positive in float32's normal range")
     if positions > (1 << 31) - 1 or positions * channels > 1 << 40 or samples * channels > 1 << 30:
         raise ValueError("too many positions or samples")
 

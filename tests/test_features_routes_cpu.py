@@ -162,3 +162,10 @@ def test_traced_shapes():
         assert features.group_norm(fake(3, 2, 5, 7, 8), 4).shape == (3, 2, 5, 7, 8)
         assert features.group_norm(fake(5, 8), 4, spatial_dims=1).shape == (5, 8)
         assert features.group_norm(fake(0, 4, 4, 8), 4).shape == (0, 4, 4, 8)
+
+
+def test_norm_refuses_an_eps_that_float32_has_not():
+    with FakeTensorMode():
+        for eps in (1e-60, 1e60):
+            with pytest.raises(ValueError, match="eps must be finite"):
+                features.group_norm(fake(1, 3, 4, 8), 2, eps=eps)
