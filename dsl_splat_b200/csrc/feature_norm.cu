@@ -57,7 +57,8 @@ struct NormParams {
   void* out;           // y or dx
   float* mean;         // (B, G)
   float* rstd;
-  float2* partial;     // (B, blocks * columns, C)
+  // (B, blocks * columns, C): double2 of the forward, float2 of the backward
+  void* partial;
   float2* moments;     // (B, G): m1, m2
   double2* channel;    // (B, C): sums of du and du xhat
   float eps;
@@ -226,7 +227,7 @@ SPLAT_DEV void write_partial(const NormParams& p, const Place& at, const float (
   __syncthreads();
   const int first = at.column * l.threads * V;  // flat position of sums[0] in a step
   const int count = min(l.threads, l.step - at.column * l.threads) * V;
-  float2* out = p.partial +
+  float2* out = static_cast<float2*>(p.partial) +
                 ((static_cast<long long>(at.sample) * l.blocks + at.part) * l.columns + at.column) *
                     l.channels;
   for (int c = threadIdx.x; c < l.channels; c += l.threads) {
@@ -241,27 +242,138 @@ SPLAT_DEV void write_partial(const NormParams& p, const Place& at, const float (
   }
 }
 
-// Sums of x - pivot and its square per channel; the pivot is the sample's
-// first row, so that a large common offset does not cancel.
+// A thread's sums of x - pivot and its square per channel.  The pivot is the
+// thread's first value and moves to the mean of those so far after every
+// fourfold of the first few, so that the sums of squares never exceed a few
+// times the squared deviations that they hold, whichever values come first.  (A
+// pivot for the whole sample cancels where it is unlike the rest: the sample's
+// first row, 300 deviations away, cost the variance of 1600 x 1200 positions
+// 1e-3 of itself.)
+template <class T, int V>
+struct Deviations {
+  Pairs<V> minus, s1, s2;  // minus: -pivot
+  SPLAT_DEV void start(const T* first, int valid) {
+    float zero[V] = {}, pivot[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) pivot[j] = j < valid ? -to_float(first[j]) : 0.0f;
+    minus.set(pivot);
+    s1.set(zero);
+    s2.set(zero);
+  }
+  SPLAT_DEV void add(const Vec<T, V>& v) {
+    const Pairs<V> d = widen_pairs<T, V>(v) + minus;
+    s1 = s1 + d;
+    s2 = fma(d, d, s2);
+  }
+  // Sums of squares that have overflowed stay infinite.
+  static SPLAT_DEV float less(float a, float b) {
+    return a == __int_as_float(0x7f800000) ? a : a - b;
+  }
+  SPLAT_DEV void move(int count) {
+    float m[V], a[V], b[V];
+    minus.get(m);
+    s1.get(a);
+    s2.get(b);
+    const float n = static_cast<float>(count), inverse = 1.0f / n;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float to = m[j] - a[j] * inverse, by = m[j] - to, rest = a[j] - n * by;
+      b[j] = less(b[j], by * (a[j] + rest));
+      a[j] = rest;
+      m[j] = to;
+    }
+    minus.set(m);
+    s1.set(a);
+    s2.set(b);
+  }
+  // (mean - x0, sum of squared deviations) of count values and, in the channels
+  // below `left`, of a last one; x0(j): the sample's first row.
+  template <class F>
+  SPLAT_DEV void finish(int count, const T* last, int left, F x0, float2 (&r)[V]) const {
+    float m[V], a[V], b[V];
+    minus.get(m);
+    s1.get(a);
+    s2.get(b);
+    const float more = 1.0f / static_cast<float>(count + 1);
+    const float inverse = count ? 1.0f / static_cast<float>(count) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (j < left) {
+        const float d = to_float(last[j]) + m[j];
+        a[j] += d;
+        b[j] += d * d;
+      } else if (count == 0) {
+        r[j] = make_float2(0.0f, 0.0f);
+        continue;
+      }
+      const float mean = a[j] * (j < left ? more : inverse), rest = less(b[j], a[j] * mean);
+      r[j] = make_float2((-m[j] - x0(j)) + mean, rest < 0.0f ? 0.0f : rest);
+    }
+  }
+};
+
+// Joins the block's threads: for every channel their (mean - x0, sum of squared
+// deviations) in `slots`, of `count` flat positions of a step from `first` on, to
+// the sums of x - x0 and its square.  The squared deviations are the threads' and
+// those of their means from the block's, so nothing cancels in fp32.  Whole warps
+// work, up to 32 threads to a channel, in a fixed order.
+template <int V, class F>
+SPLAT_DEV void join_threads(const Layout& l, int part, int first, int count, const float2* slots,
+                            F write) {
+  const int begin = min(part * l.per_block, l.steps), end = min(begin + l.per_block, l.steps);
+  const int steps = end - begin, whole = l.threads & ~31;
+  // positions from `cut` on are one value short: the sample ends before them
+  const long long cut =
+      steps && end == l.steps ? l.span - (l.steps - 1LL) * l.step * V - first : count;
+  int lanes = 32;
+  while (lanes > 1 && l.channels * lanes > whole) lanes /= 2;
+  const int lane = threadIdx.x & (lanes - 1), groups = whole / lanes;
+  if (static_cast<int>(threadIdx.x) >= whole) return;
+  const auto sum = [&](auto v) {
+    for (int o = lanes / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
+  for (int c0 = 0; c0 < l.channels; c0 += groups) {
+    const int c = c0 + static_cast<int>(threadIdx.x) / lanes;
+    int from = c - first % l.channels;
+    if (from < 0) from += l.channels;
+    from = c < l.channels ? from + lane * l.channels : count;
+    const int by = lanes * l.channels;
+    int n = 0;
+    float a = 0.0f;
+    for (int i = from; i < count; i += by) {
+      const int ni = steps - (i >= cut ? 1 : 0);
+      n += ni;
+      a += static_cast<float>(ni) * slots[i].x;
+    }
+    n = sum(n);
+    a = sum(a);
+    const float mean = n ? a / static_cast<float>(n) : 0.0f;
+    float b = 0.0f;
+    for (int i = from; i < count; i += by) {
+      const float apart = slots[i].x - mean;
+      b += slots[i].y + static_cast<float>(steps - (i >= cut ? 1 : 0)) * (apart * apart);
+    }
+    b = sum(b);
+    if (lane == 0 && c < l.channels) {
+      const double m = mean;
+      write(c, n * m, b + n * m * m);
+    }
+  }
+}
+
 template <class T, int V>
 __global__ void __launch_bounds__(kMaxThreads, 2) norm_sums_kernel(const NormParams p) {
   using Values = Vec<T, V>;
+  __shared__ float2 slots[kMaxThreads * V];
   const Layout& l = p.l;
   const Place at = place<V>(l);
   const T* x = static_cast<const T*>(p.x) + at.sample * l.span;
-  float zero[V] = {}, pivot[V];
-  Pairs<V> minus, s1, s2;
-  s1.set(zero);
-  s2.set(zero);
-  const bool active = at.count || at.left;
-#pragma unroll
-  for (int j = 0; j < V; ++j)
-    pivot[j] =
-        active ? -to_float(x[(static_cast<long long>(at.vector) * V + j) % l.channels]) : 0.0f;
-  minus.set(pivot);
   const T* from = x + at.first;
+  Deviations<T, V> sums;
+  sums.start(from, at.count ? V : at.left);
   constexpr int U = 4;
-  int i = 0;
+  int i = 0, move = U;
   for (; i + U <= at.count; i += U) {
     Values v[U];
 #pragma unroll
@@ -269,28 +381,27 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_sums_kernel(const NormPar
       v[u] = *reinterpret_cast<const Values*>(from + u * at.stride);
     from += U * at.stride;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const Pairs<V> d = widen_pairs<T, V>(v[u]) + minus;
-      s1 = s1 + d;
-      s2 = fma(d, d, s2);
+    for (int u = 0; u < U; ++u) sums.add(v[u]);
+    if (i + U == move) {
+      sums.move(move);
+      move = move < 1 << 28 ? move * 4 : 0;
     }
   }
-  for (; i < at.count; ++i, from += at.stride) {
-    const Pairs<V> d = widen_pairs<T, V>(*reinterpret_cast<const Values*>(from)) + minus;
-    s1 = s1 + d;
-    s2 = fma(d, d, s2);
-  }
-  float a[V], b[V];
-  s1.get(a);
-  s2.get(b);
+  for (; i < at.count; ++i, from += at.stride)
+    sums.add(*reinterpret_cast<const Values*>(from));
+  float2 r[V];
+  sums.finish(at.count, from, at.left, [&](int j) {
+    return to_float(x[(static_cast<long long>(at.vector) * V + j) % l.channels]);
+  }, r);
 #pragma unroll
-  for (int j = 0; j < V; ++j)
-    if (j < at.left) {
-      const float d = to_float(from[j]) + pivot[j];
-      a[j] += d;
-      b[j] += d * d;
-    }
-  write_partial<V>(p, at, a, b);
+  for (int j = 0; j < V; ++j) slots[threadIdx.x * V + j] = r[j];
+  __syncthreads();
+  const int first = at.column * l.threads * V;  // flat position of slots[0] in a step
+  double2* out = static_cast<double2*>(p.partial) +
+                 ((static_cast<long long>(at.sample) * l.blocks + at.part) * l.columns + at.column) *
+                     l.channels;
+  join_threads<V>(l, at.part, first, min(l.threads, l.step - at.column * l.threads) * V, slots,
+                  [&](int c, double a, double b) { out[c] = make_double2(a, b); });
 }
 
 SPLAT_DEV uint32_t cluster_rank() {
@@ -310,6 +421,9 @@ SPLAT_DEV double load_cluster(const double* own, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(rank));
   asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(there) : "memory");
   return v;
+}
+SPLAT_DEV double2 load_cluster(const double2* own, uint32_t rank) {
+  return make_double2(load_cluster(&own->x, rank), load_cluster(&own->y, rank));
 }
 SPLAT_DEV float2 load_cluster(const float2* own, uint32_t rank) {
   const uint32_t here = static_cast<uint32_t>(__cvta_generic_to_shared(own));
@@ -334,23 +448,23 @@ SPLAT_DEV double warp_sum(double v) {
 // row, and the threads of a channel are added up in a fixed order.
 constexpr int kJoinThreads = 1024, kJoinChannels = 32, kMaxCluster = 8;
 
+template <class Pair>  // double2 or float2
 SPLAT_DEV void channel_sums(const NormParams& p, int sample, int c0, int count,
                             double2 (&joined)[kJoinChannels]) {
   __shared__ double2 sums[kJoinThreads];
   const int parts = p.l.blocks * p.l.columns;
-  const float2* in =
-      p.partial + static_cast<long long>(sample) * parts * p.l.channels + c0;
+  const Pair* in = static_cast<const Pair*>(p.partial) +
+                   static_cast<long long>(sample) * parts * p.l.channels + c0;
   const int lanes = kJoinThreads / count, c = threadIdx.x % count, lane = threadIdx.x / count;
   double a = 0.0, b = 0.0;
   if (lane < lanes) {
     constexpr int U = 8;  // reads in flight
     for (int i0 = lane; i0 < parts; i0 += U * lanes) {
-      float2 v[U];
+      Pair v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int i = i0 + u * lanes;
-        v[u] = i < parts ? in[static_cast<long long>(i) * p.l.channels + c]
-                         : make_float2(0.0f, 0.0f);
+        v[u] = i < parts ? in[static_cast<long long>(i) * p.l.channels + c] : Pair{};
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -376,13 +490,14 @@ SPLAT_DEV void channel_sums(const NormParams& p, int sample, int c0, int count,
   __syncthreads();
 }
 
-// A group's moments from its channels' sums of x - pivot: (count, mean, sum of
+// A group's moments from its channels' sums of x - x0 (x0: the sample's first
+// row), in doubles, where an x0 far from the rest costs nothing: (count, mean, sum of
 // squared deviations) of up to 32 channels at a time, a lane to a channel, and
 // such blocks joined by
 //   M = M_a + M_b + (mean_b - mean_a)^2 n_a n_b / (n_a + n_b).
 struct Moments {
   double n, mean, m2;
-  // Called by a whole warp; pivot and sums of lanes from `count` on are ignored.
+  // Called by a whole warp; the pivot (x0) and sums of lanes from `count` on are ignored.
   SPLAT_DEV void join(double rows, int count, double2 sums, double pivot) {
     const bool in = (threadIdx.x & 31) < count;
     const double inverse = 1.0 / rows;
@@ -419,7 +534,7 @@ __global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(const NormParam
   Moments m{};
   for (int k0 = rank * kJoinChannels; k0 < p.group_channels; k0 += blocks * kJoinChannels) {
     const int c0 = g * p.group_channels + k0, count = min(kJoinChannels, p.group_channels - k0);
-    channel_sums(p, sample, c0, count, joined);
+    channel_sums<double2>(p, sample, c0, count, joined);
     if (threadIdx.x < 32) {
       const int k = min(static_cast<int>(threadIdx.x), count - 1);
       m.join(rows, count, joined[k], to_float(x[c0 + k]));
@@ -565,7 +680,7 @@ __global__ void __launch_bounds__(kJoinThreads)
   double m1 = 0.0, m2 = 0.0;
   for (int k0 = rank * kJoinChannels; k0 < p.group_channels; k0 += blocks * kJoinChannels) {
     const int c0 = g * p.group_channels + k0, count = min(kJoinChannels, p.group_channels - k0);
-    channel_sums(p, sample, c0, count, joined);
+    channel_sums<float2>(p, sample, c0, count, joined);
     if (threadIdx.x < 32) {
       const int k = threadIdx.x;
       double2 v = joined[min(k, count - 1)];
@@ -674,8 +789,24 @@ constexpr int kSmallBytes = 512 * 1024;  // or read again
 constexpr int kMaxRereadSamples = 8;
 constexpr int kSmallChannels = 1024;
 
-// Sums the threads' sums over the block and then over the cluster; all blocks
-// end with the sample's sums per channel in `channel`.
+// The cluster's sums per channel of its blocks' in `own`; all blocks end with
+// them in `channel`.
+template <class Pair>  // double2 or float2
+SPLAT_DEV void join_cluster(const Layout& l, const Pair* own, double2* channel) {
+  cluster_sync();
+  for (int c = threadIdx.x; c < l.channels; c += l.threads) {
+    double a = 0.0, b = 0.0;
+    for (int r = 0; r < l.blocks; ++r) {
+      const Pair v = load_cluster(own + c, r);
+      a += v.x;
+      b += v.y;
+    }
+    channel[c] = make_double2(a, b);
+  }
+  cluster_sync();  // no block leaves while its sums are read
+}
+
+// Sums the threads' sums over the block and then over the cluster.
 template <int V>
 SPLAT_DEV void cluster_sums(const Layout& l, const float (&s1)[V], const float (&s2)[V],
                             float2* per_thread, float2* own, double2* channel) {
@@ -691,40 +822,32 @@ SPLAT_DEV void cluster_sums(const Layout& l, const float (&s1)[V], const float (
     }
     own[c] = make_float2(a, b);
   }
-  cluster_sync();
-  for (int c = threadIdx.x; c < l.channels; c += l.threads) {
-    double a = 0.0, b = 0.0;
-    for (int r = 0; r < l.blocks; ++r) {
-      const float2 v = load_cluster(own + c, r);
-      a += v.x;
-      b += v.y;
-    }
-    channel[c] = make_double2(a, b);
-  }
-  cluster_sync();  // no block leaves while its sums are read
+  join_cluster(l, own, channel);
 }
 
 // Shared memory of the small kernels: the values, then the sums.
 __host__ __device__ inline size_t kept_bytes(const Layout& l, int vector_bytes, int arrays) {
   return (static_cast<size_t>(arrays) * l.per_block * l.threads * vector_bytes + 15) / 16 * 16;
 }
-template <class T, int V>
+template <class T, int V, class Own>  // Own: double2 (forward) or float2
 struct SmallShared {
   float2* per_thread;
-  float2* own;
+  Own* own;
   double2* channel;
   float2* group;  // per group: mean and rstd, or m1 and m2
   SPLAT_DEV SmallShared(unsigned char* base, const Layout& l, int arrays) {
     base += kept_bytes(l, sizeof(Vec<T, V>), arrays);  // arrays: 0 when nothing is kept
     channel = reinterpret_cast<double2*>(base);
-    per_thread = reinterpret_cast<float2*>(channel + l.channels);
-    own = per_thread + l.threads * V;
-    group = own + l.channels;
+    own = reinterpret_cast<Own*>(channel + l.channels);
+    per_thread = reinterpret_cast<float2*>(own + l.channels);
+    group = per_thread + l.threads * V;
   }
 };
-size_t small_bytes(const Layout& l, int v, int value_bytes, int groups, int arrays) {
+size_t small_bytes(const Layout& l, int v, int value_bytes, int groups, int arrays,
+                   bool backward) {
   return kept_bytes(l, v * value_bytes, arrays) +
-         static_cast<size_t>(l.channels) * (sizeof(double2) + sizeof(float2)) +
+         static_cast<size_t>(l.channels) *
+             (sizeof(double2) + (backward ? sizeof(float2) : sizeof(double2))) +
          static_cast<size_t>(l.threads) * v * sizeof(float2) +
          static_cast<size_t>(groups) * sizeof(float2);
 }
@@ -735,17 +858,19 @@ __global__ void __launch_bounds__(kSmallThreads) norm_small_kernel(const NormPar
   extern __shared__ __align__(16) unsigned char shared[];
   const Layout& l = p.l;
   const Place at = place<V>(l);
-  const SmallShared<T, V> mem(shared, l, p.keep ? 1 : 0);
+  const SmallShared<T, V, double2> mem(shared, l, p.keep ? 1 : 0);
   Values* kept = reinterpret_cast<Values*>(shared) + threadIdx.x;
   const T* x = static_cast<const T*>(p.x) + at.sample * l.span;
   const T* from = x + at.first;
-  float a[V] = {}, b[V] = {}, pivot[V];
   const bool active = at.count || at.left;
+  Deviations<T, V> sums;
+  sums.start(from, at.count ? V : at.left);
+  float x0[V];
 #pragma unroll
   for (int j = 0; j < V; ++j)
-    pivot[j] = active ? to_float(x[(at.vector * V + j) % l.channels]) : 0.0f;
+    x0[j] = active ? to_float(x[(at.vector * V + j) % l.channels]) : 0.0f;
   constexpr int U = 8;  // reads in flight
-  for (int i0 = 0; i0 < at.count; i0 += U) {
+  for (int i0 = 0, move = U; i0 < at.count; i0 += U) {
     Values v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -755,28 +880,23 @@ __global__ void __launch_bounds__(kSmallThreads) norm_small_kernel(const NormPar
     for (int u = 0; u < U; ++u)
       if (i0 + u < at.count) {
         if (p.keep) kept[(i0 + u) * l.threads] = v[u];
-        float f[V];
-        widen<T, V>(v[u], f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float d = f[j] - pivot[j];
-          a[j] += d;
-          b[j] += d * d;
-        }
+        sums.add(v[u]);
       }
+    if (i0 + U == move && move <= at.count) {
+      sums.move(move);
+      move *= 4;
+    }
   }
-  if (at.left) {
-    const Values v = load_part<T, V>(from + at.count * at.stride, at.left);
-    if (p.keep) kept[at.count * l.threads] = v;
+  if (at.left && p.keep)
+    kept[at.count * l.threads] = load_part<T, V>(from + at.count * at.stride, at.left);
+  float2 r[V];
+  sums.finish(at.count, from + at.count * at.stride, at.left, [&](int j) { return x0[j]; }, r);
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (j < at.left) {
-        const float d = to_float(v.v[j]) - pivot[j];
-        a[j] += d;
-        b[j] += d * d;
-      }
-  }
-  cluster_sums<V>(l, a, b, mem.per_thread, mem.own, mem.channel);
+  for (int j = 0; j < V; ++j) mem.per_thread[threadIdx.x * V + j] = r[j];
+  __syncthreads();
+  join_threads<V>(l, at.part, 0, l.threads * V, mem.per_thread,
+                  [&](int c, double s1, double s2) { mem.own[c] = make_double2(s1, s2); });
+  join_cluster(l, mem.own, mem.channel);
   __syncthreads();
   const double rows = static_cast<double>(l.span / l.channels);
   // whole warps only (there is one: a block has more than 128 threads)
@@ -835,7 +955,7 @@ __global__ void __launch_bounds__(kSmallThreads)
   extern __shared__ __align__(16) unsigned char shared[];
   const Layout& l = p.l;
   const Place at = place<V>(l);
-  const SmallShared<T, V> mem(shared, l, p.keep ? 2 : 0);
+  const SmallShared<T, V, float2> mem(shared, l, p.keep ? 2 : 0);
   Values* kept_x = reinterpret_cast<Values*>(shared) + threadIdx.x;
   Values* kept_g = kept_x + l.per_block * l.threads;
   const long long offset = at.sample * l.span + at.first;
@@ -1022,7 +1142,7 @@ Plan make_plan(int value_bytes, int samples, long long positions, int channels, 
     plan.l.per_block = (plan.l.steps + blocks - 1) / blocks;
     plan.keep = bytes <= static_cast<long long>(kMaxCluster) * kKeptBytes;
     const auto need = [&](int arrays) {
-      return small_bytes(plan.l, plan.vector, value_bytes, groups, arrays);
+      return small_bytes(plan.l, plan.vector, value_bytes, groups, arrays, backward);
     };
     // many channels, or a last step of few vectors, can leave less room
     if (plan.keep && need(backward ? 2 : 1) > kMostShared) plan.keep = false;
@@ -1073,9 +1193,9 @@ int with_width(int v, F f) {
 
 size_t round_up(size_t n) { return (n + 15) / 16 * 16; }
 
-size_t partial_bytes(int samples, const Layout& l) {
+size_t partial_bytes(int samples, const Layout& l, bool backward) {
   return round_up(static_cast<size_t>(samples) * l.blocks * l.columns * l.channels *
-                  sizeof(float2));
+                  (backward ? sizeof(float2) : sizeof(double2)));
 }
 
 int check_norm(int dtype, int samples, long long positions, int channels, int groups,
@@ -1110,8 +1230,8 @@ size_t splat_feature_norm_workspace_bytes(int dtype, int samples, long long posi
   const Plan plan =
       make_plan(bytes_of(dtype), samples, positions, channels, groups, backward != 0);
   const size_t moments = round_up(static_cast<size_t>(samples) * groups * sizeof(float2));
-  if (!backward) return plan.small ? 16 : partial_bytes(samples, plan.l) + moments;
-  return (plan.small ? 0 : partial_bytes(samples, plan.l)) + moments +
+  if (!backward) return plan.small ? 16 : partial_bytes(samples, plan.l, false) + moments;
+  return (plan.small ? 0 : partial_bytes(samples, plan.l, true)) + moments +
          static_cast<size_t>(samples) * channels * sizeof(double2);
 }
 
@@ -1126,7 +1246,7 @@ int splat_feature_norm(int dtype, int samples, long long positions, int channels
   if (!host::aligned(x, 16) || !host::aligned(y, 16) || !host::aligned(workspace, 16))
     return host::fail(kInvalidArgument, "feature_norm: x, y and workspace must be 16-byte aligned");
   const Plan plan = make_plan(bytes_of(dtype), samples, positions, channels, groups, false);
-  const size_t partial = plan.small ? 0 : partial_bytes(samples, plan.l);
+  const size_t partial = plan.small ? 0 : partial_bytes(samples, plan.l, false);
   const size_t moments = round_up(static_cast<size_t>(samples) * groups * sizeof(float2));
   if (!plan.small && (!workspace || workspace_bytes < partial + moments))
     return host::fail(kWorkspaceTooSmall, "feature_norm: workspace");
@@ -1142,7 +1262,7 @@ int splat_feature_norm(int dtype, int samples, long long positions, int channels
   p.out = y;
   p.mean = mean;
   p.rstd = rstd;
-  p.partial = static_cast<float2*>(workspace);
+  p.partial = workspace;
   if (!mean && !plan.small) {  // the passes hand them on all the same
     p.mean = reinterpret_cast<float*>(static_cast<char*>(workspace) + partial);
     p.rstd = p.mean + static_cast<size_t>(samples) * groups;
@@ -1185,7 +1305,7 @@ int splat_feature_norm_backward(int dtype, int samples, long long positions, int
     return host::fail(kInvalidArgument,
                       "feature_norm_backward: tensors and workspace must be 16-byte aligned");
   const Plan plan = make_plan(bytes_of(dtype), samples, positions, channels, groups, true);
-  if (workspace_bytes < (plan.small ? 0 : partial_bytes(samples, plan.l)) +
+  if (workspace_bytes < (plan.small ? 0 : partial_bytes(samples, plan.l, true)) +
                             round_up(static_cast<size_t>(samples) * groups * sizeof(float2)) +
                             static_cast<size_t>(samples) * channels * sizeof(double2))
     return host::fail(kWorkspaceTooSmall, "feature_norm_backward: workspace");
@@ -1203,8 +1323,8 @@ int splat_feature_norm_backward(int dtype, int samples, long long positions, int
   p.mean = const_cast<float*>(mean);
   p.rstd = const_cast<float*>(rstd);
   char* at = static_cast<char*>(workspace);
-  p.partial = reinterpret_cast<float2*>(at);
-  at += plan.small ? 0 : partial_bytes(samples, p.l);
+  p.partial = at;
+  at += plan.small ? 0 : partial_bytes(samples, p.l, true);
   p.moments = reinterpret_cast<float2*>(at);
   at += round_up(static_cast<size_t>(samples) * groups * sizeof(float2));
   p.channel = reinterpret_cast<double2*>(at);

@@ -102,3 +102,68 @@ def test_infinite_gradients_stay_infinite(k, n, dtype):
     keep = torch.arange(300, device="cuda") != 130
     assert torch.equal(spoilt[keep], clean[keep])
     assert (spoilt[130] == float("inf")).all()
+
+# ---- group norm of samples whose first row is unlike the rest ---------------------
+
+def norm_exact(x, groups):
+    b, s, c = x.shape
+    X = x.double().reshape(b, s, groups, -1)
+    mean = X.mean((1, 3), keepdim=True)
+    var = (X - mean).square().mean((1, 3), keepdim=True)
+    return X, mean, var
+
+
+NORM_FIRST = [(1, 40 * 50, 32, 8), (2, 67 * 101, 48, 4), (1, 300 * 300, 32, 8),
+              (1, 301 * 211, 35, 5), (3, 250 * 260, 16, 16), (1, 500 * 400, 64, 16),
+              (2, 90 * 90, 600, 1), (1, 800, 2050, 2), (64, 170 * 170, 32, 8), (1, 7, 3, 1)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("apart", [30.0, 300.0, 3000.0])
+@pytest.mark.parametrize("b, s, c, groups", NORM_FIRST)
+def test_group_norm_first_row_unlike_the_rest(b, s, c, groups, apart, dtype):
+    """An empty corner of an image of far features.  The variance is joined
+    from sums of squares of one sign about means that lie among the values:
+    chains of at most 64 additions of them, each half of u, and four times
+    that for the moving mean; y is off by half of its relative error."""
+    normal = draws(45)
+    x = normal(b, s, c, dtype=dtype, shift=apart)
+    x[:, 0] = 0
+    dy = normal(b, s, c, dtype=dtype)
+    x.requires_grad_()
+    y = features.group_norm(x, groups, spatial_dims=1)
+    dx, = torch.autograd.grad(y, x, dy)
+    X, mean, var = norm_exact(x.detach(), groups)
+    rstd = (var + 1e-5).rsqrt()
+    e_rstd = 128 * U * rstd  # relative: half of 256 u
+    # the mean is kept as an fp32 value, and formed from fp32 differences to the
+    # first row and to each other
+    e_mean = U * mean.abs() + U * (X[:, :1] - mean).abs().mean(3, keepdim=True) \
+        + 64 * U * var.sqrt()
+    hat = (X - mean) * rstd
+    e_hat = (e_mean + U * (X - mean).abs()) * rstd + (X - mean).abs() * e_rstd + 4 * U * hat.abs()
+    check(y.detach(), hat.reshape(x.shape), e_hat.reshape(x.shape), "y")
+    D = dy.double().reshape(X.shape)
+
+    def avg(v):
+        return v.mean((1, 3), keepdim=True)
+
+    m1, m2 = avg(D), avg(D * hat)
+    e_m2 = avg(D.abs() * e_hat) + 520 * U * avg((D * hat).abs())
+    inner = D - m1 - hat * m2
+    e_inner = (520 * U * avg(D.abs()) + e_hat * m2.abs() + hat.abs() * e_m2
+               + 4 * U * (D.abs() + m1.abs() + (hat * m2).abs()))
+    check(dx, (rstd * inner).reshape(x.shape),
+          (rstd * e_inner + e_rstd * inner.abs()).reshape(x.shape), "dx")
+
+
+def test_group_norm_halves_apart():
+    """Values on two sides of a step: no row stands for all."""
+    for s, c in ((5000, 8), (400_000, 32)):
+        normal = draws(46)
+        x = normal(1, s, c, dtype=torch.float32)
+        x[:, s // 3:] += 1000.0
+        y = features.group_norm(x, 2, spatial_dims=1)
+        X, mean, var = norm_exact(x, 2)
+        hat = (X - mean) * (var + 1e-5).rsqrt()
+        check(y, hat.reshape(x.shape), (200 * U * (hat.abs() + 1)).reshape(x.shape), "y")
