@@ -5,9 +5,9 @@
 // for layers whose W and one 128-row tile of x and dz fit in shared memory.
 // x and dy are read once and dx is written once; the three products of a tile
 // take the same copies of x, dz and W, as K-major operands in one and MN-major
-// ones in the other.  dW stays in tensor memory (16-bit types: truncation costs
-// about 2e-8 relative an addition, and 2 10^6 rows are 424 additions a block) or
-// is added up in registers after every tile (fp32).  db is folded from the
+// ones in the other.  dW stays in tensor memory (16-bit types; a block has no more
+// tiles than kMostAdditions allow) or is added up in registers after every tile
+// (fp32).  db is folded from the
 // lanes' rows of dz before dz is rounded or split.
 //
 // A block of 16 warps does each tile's steps together: load, product,

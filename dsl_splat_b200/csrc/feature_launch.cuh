@@ -74,9 +74,11 @@ int launch_product(ProductParams p, cudaStream_t s) {
   p.bias_shared = p.bias && columns <= kMaxSharedBias ? columns : 0;
   p.tmem_columns = 32;
   constexpr int kAcc = accumulators(PA, PB);
-  // sums of several accumulators are joined in fp32 outputs; an operand row of
-  // more values than kExactSum is summed in one
-  p.k_per_sum = kAcc == 2 && EPI == kPlain && sizeof(TO) == 4 ? kExactSum : p.k_per_split;
+  // sums of several accumulators are joined in fp32 outputs
+  p.k_per_sum = kAcc == 2 && EPI == kPlain ? kExactSum
+                : EPI == kPlain && sizeof(TO) == 4
+                    ? kMostAdditions * 16 / PA
+                    : p.k_per_split;
   // (35 -> 32 fp32 gelu over 10^6 rows 113 us against 154 without, 32 -> 3 bf16
   // over 1.9 10^6 67 against 84, 64 -> 32 bf16 71 against 69)
   p.alternate = p.tile_n == 32 && p.k_per_sum >= p.k_per_split;

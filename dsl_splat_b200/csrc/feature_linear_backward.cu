@@ -18,15 +18,15 @@ namespace feature {
 
 // ---- sums over splits and rows ---------------------------------------------------
 
-// Adds the splits' partial sums, `stride` values apart, in a fixed order: 32
-// threads to a value.  The first count_a values go to a, the rest to b.
+// Adds the splits' partial sums, `stride` values apart, in a fixed order and in
+// doubles (there may be a million): 32 threads to a value.  The first count_a values go to a, the rest to b.
 constexpr int kJoinLanes = 32;
 template <class T>
 __global__ void __launch_bounds__(32 * kJoinLanes)
     join_splits_kernel(const float* partial, long long stride, int splits, long long count_a,
                        long long count_b, T* a, T* b) {
   const long long i = blockIdx.x * 32LL + threadIdx.x, count = count_a + count_b;
-  float s = 0.0f;
+  double s = 0.0;
   if (i < count) {
     constexpr int U = 8;  // reads in flight
     for (int k0 = threadIdx.y; k0 < splits; k0 += U * kJoinLanes) {
@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(32 * kJoinLanes)
       for (int u = 0; u < U; ++u) s += v[u];
     }
   }
-  __shared__ float sums[kJoinLanes][33];
+  __shared__ double sums[kJoinLanes][33];
   sums[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   // a warp to a value, its lanes' sums in a fixed tree
@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(32 * kJoinLanes)
   const long long j = blockIdx.x * 32LL + threadIdx.y;
   if (threadIdx.x == 0 && j < count) {
     T* to = j < count_a ? a : b;
-    if (to) to[j < count_a ? j : j - count_a] = from_float<T>(s);
+    if (to) to[j < count_a ? j : j - count_a] = from_float<T>(static_cast<float>(s));
   }
 }
 
@@ -283,8 +283,15 @@ FusedPlan plan_fused(long long rows, int k, int n, int activation) {
     plan.raw = raw <= static_cast<size_t>(per_sm == 2 ? kTwoBlocksBytes : kOneBlockBytes);
     if (plan.raw) plan.bytes = raw;
   }
-  plan.blocks = static_cast<int>(std::min<long long>(
-      (rows + kTileRows - 1) / kTileRows, static_cast<long long>(host::sm_count()) * per_sm));
+  // as many as are resident; of 16-bit types so many times more that no dW takes
+  // more than kMostAdditions in tensor memory
+  const long long tiles = (rows + kTileRows - 1) / kTileRows;
+  long long blocks = static_cast<long long>(host::sm_count()) * per_sm;
+  if (sizeof(T) == 2) {
+    const long long most = kMostAdditions * 16 / kTileRows / (rounds_dz(activation) ? 2 : 1);
+    blocks *= std::max(1LL, (tiles + blocks * most - 1) / (blocks * most));
+  }
+  plan.blocks = static_cast<int>(std::min(tiles, blocks));
   return plan;
 }
 

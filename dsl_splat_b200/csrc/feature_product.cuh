@@ -51,6 +51,11 @@ __host__ __device__ constexpr int producers(int pa, int pb) { return pa <= 2 && 
 __host__ __device__ constexpr int accumulators(int pa, int pb) { return pa == 3 || pb == 3 ? 2 : 1; }
 // k that such an accumulator sums before it is added up in fp32 (32 additions).
 constexpr int kExactSum = 512;
+// Additions into an accumulator of a 16-bit layer's dW, whose sums run over the
+// rows: they cost it about 2e-8 relative each and 2^-23 at most, a quarter of half
+// a step of f16 in all.  (y and dx of 16-bit layers sum up to 65535 values: at most
+// 8192 additions, 1.4e-4.)
+constexpr int kMostAdditions = 1024;
 
 // act(C + bias) + residual; dy act'(C + bias); C.
 enum Epilogue : int { kForward = 0, kSlope = 1, kPlain = 2 };

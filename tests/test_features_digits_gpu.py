@@ -167,3 +167,24 @@ def test_group_norm_halves_apart():
         X, mean, var = norm_exact(x, 2)
         hat = (X - mean) * (var + 1e-5).rsqrt()
         check(y, hat.reshape(x.shape), (200 * U * (hat.abs() + 1)).reshape(x.shape), "y")
+
+# ---- long sums -------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows, k, n, power", [(200_000_000, 8, 8, -13), (200_000_000, 9, 7, -13),
+                                               (800_000, 2048, 2048, -5)])
+def test_weight_gradient_over_many_rows(rows, k, n, power):
+    """fp16: an accumulator of dW takes 1024 additions at most (u each), and
+    what it holds is added up in fp32: 64 additions in a chain (u / 2 each).
+    The sum lies just above a value of fp16 whose step is 2^-10 of it, so that
+    a bias of half a step shows."""
+    x = torch.full((rows, k), 1285 / 1024, device="cuda", dtype=torch.float16)
+    dy = torch.full((rows, n), 2.0 ** power * 1105 / 1024, device="cuda", dtype=torch.float16)
+    value = float(x[0, 0]) * float(dy[0, 0])
+    used = math.ceil(32800 / value)
+    assert used <= rows
+    x, dy = x[:used], dy[:used]
+    w = torch.zeros(n, k, device="cuda", dtype=torch.float16, requires_grad=True)
+    y = features.linear(x, w)
+    dw, = torch.autograd.grad(y, w, dy)
+    want = torch.full((n, k), used * value, device="cuda", dtype=torch.float64)
+    check(dw, want, (1024 + 32) * U * want, "dw")
