@@ -188,3 +188,38 @@ def test_weight_gradient_over_many_rows(rows, k, n, power):
     dw, = torch.autograd.grad(y, w, dy)
     want = torch.full((n, k), used * value, device="cuda", dtype=torch.float64)
     check(dw, want, (1024 + 32) * U * want, "dw")
+
+
+# ---- whole numbers -----------------------------------------------------------------
+
+EXACT_SIZES = [(120001, 64, 64), (70001, 35, 64), (50000, 128, 128), (40000, 100, 72),
+               (30001, 96, 128), (60000, 33, 20), (50001, 40, 3), (4096, 256, 256),
+               (17001, 300, 17), (20000, 129, 130), (18000, 520, 137), (200001, 8, 8),
+               (9000, 16, 200), (1, 3, 5), (129, 64, 32)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["none", "relu"])
+@pytest.mark.parametrize("m, k, n", EXACT_SIZES)
+def test_linear_whole_numbers(m, k, n, act, dtype):
+    """Small whole numbers: every sum is one of fp32's, so each result is the
+    exact sum rounded once, to the bit; a tile that is lost, doubled or stale
+    changes it."""
+    g = torch.Generator().manual_seed(44)
+
+    def whole(*shape, most):
+        return torch.randint(-most, most + 1, shape, generator=g).to(dtype).cuda()
+
+    x, w, b = whole(m, k, most=3), whole(n, k, most=1), whole(n, most=2)
+    dy, r = whole(m, n, most=2), whole(m, n, most=3)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = features.linear(x, w, b, residual=r, activation=act)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    xd, wd, dyd = (t.detach().double() for t in (x, w, dy))
+    z = xd @ wd.t() + b.detach().double()
+    value, rate = value_and_slope(z, act)
+    dz = dyd * rate
+    for name, got, want in (("y", y, value + r.double()), ("dx", dx, dz @ wd),
+                            ("dw", dw, dz.t() @ xd), ("db", db, dz.sum(0))):
+        assert want.abs().max() < 2 ** 24, name
+        assert torch.equal(got.detach(), want.to(dtype)), name
