@@ -75,7 +75,7 @@ int launch_product(ProductParams p, cudaStream_t s) {
   p.tmem_columns = 32;
   constexpr int kAcc = accumulators(PA, PB);
   // sums of several accumulators are joined in fp32 outputs
-  p.k_per_sum = kAcc == 2 && EPI == kPlain ? kExactSum
+  p.k_per_sum = kAcc == 2 ? kExactSum
                 : EPI == kPlain && sizeof(TO) == 4
                     ? kMostAdditions * 16 / PA
                     : p.k_per_split;

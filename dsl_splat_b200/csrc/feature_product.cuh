@@ -437,6 +437,38 @@ struct Patch {
     }
   }
 
+  // Adds what this warp stored in global memory (fp32 only) onto the staging.
+  SPLAT_DEV void add(const T* src, long long ld, int rows, int cols, bool vector) const {
+    static_assert(sizeof(T) == 4);
+    const int lane = threadIdx.x & 31;
+    if (vector) {
+      constexpr int kRows = 32 / kPieces;
+      const int piece = lane % kPieces, r0 = lane / kPieces;
+      if (piece * V >= cols) return;
+      src += r0 * ld + piece * V;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i, src += kRows * ld) {
+        if (i * kRows + r0 >= rows) break;
+        const uint32_t to = at(i * kRows + r0, piece);
+        float4 v = load_shared(to);
+        const float4 o = *reinterpret_cast<const float4*>(src);
+        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+        store_shared(to, reinterpret_cast<const uint4&>(v));
+      }
+    } else {
+      constexpr int kRows = 32 / W;
+      const int col = lane % W;
+      if (col >= cols) return;
+      src += lane / W * ld + col;
+      for (int r = lane / W; r < rows; r += kRows, src += kRows * ld) {
+        const uint32_t to = at(r, col / V) + col % V * sizeof(T);
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(to) : "memory");
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(to), "f"(v + *src) : "memory");
+      }
+    }
+  }
+
   // Staging -> global memory; add (fp32 only): onto what is there.
   SPLAT_DEV void store(T* dst, long long ld, int rows, int cols, bool vector, bool add) const {
     const int lane = threadIdx.x & 31;
@@ -893,7 +925,7 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
         for (int c = c_first; c * 32 < p.tile_n; c += kEpilogueWarps / 4) {
           const int col0 = tile.n0 + c * 32, cols = min(p.n - col0, 32);
           if (cols <= 0 || rows <= 0) break;
-          if (kExtra && p.extra && !p.copy_extra) {
+          if (kExtra && p.extra && !p.copy_extra && sum_k + p.k_per_sum >= tile.k1) {
             __syncwarp();  // the patch before has been read
             extra_patch.load(static_cast<const TE*>(p.extra) + row0 * p.n + col0, p.n, rows, cols,
                              p.extra_vector);
@@ -912,6 +944,33 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
             tc::tmem_load32(from + p.tile_n, low);
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] += low[i];
+          }
+          // rows of several sums: those before the last are stored, each onto the ones
+          // before, and the last takes them from there
+          if constexpr (kExtra && kAcc == 2) {
+            if (p.k_per_sum < p.k) {
+              TO* to = static_cast<TO*>(p.out) + out_at + col0;
+              const bool last = sum_k + p.k_per_sum >= tile.k1;
+              const int lane = threadIdx.x & 31;
+              __syncwarp();  // the results before have left the patch
+#pragma unroll
+              for (int j = 0; j < Patch<TO>::kPieces; ++j)
+                store_shared(out_patch.at(lane, j),
+                             make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                                        __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3])));
+              __syncwarp();
+              if (!last) {
+                out_patch.store(to, p.out_ld, rows, cols, p.out_vector, sum_k != tile.k0);
+                continue;
+              }
+              out_patch.add(to, p.out_ld, rows, cols, p.out_vector);
+              __syncwarp();
+#pragma unroll
+              for (int j = 0; j < Patch<TO>::kPieces; ++j) {
+                const float4 s = load_shared(out_patch.at(lane, j));
+                v[4 * j] = s.x, v[4 * j + 1] = s.y, v[4 * j + 2] = s.z, v[4 * j + 3] = s.w;
+              }
+            }
           }
           if constexpr (kExtra) {
             if (p.bias) {
@@ -993,7 +1052,7 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
             } else {
               __syncwarp();
               out_patch.store(static_cast<TO*>(out) + out_at + col0, p.out_ld, rows, cols,
-                              p.out_vector, sum_k != tile.k0);
+                              p.out_vector, !kExtra && sum_k != tile.k0);
             }
           };
           if constexpr (EPI == kSlope && sizeof(TO) == 2) {

@@ -132,7 +132,7 @@ def _traced() -> bool:
     torch.ops.splat200, which it can hold (a launch through the C ABI leaves
     only the allocation of its result in it)."""
     return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
-            or torch._C._get_tracing_state() is not None)
+            or torch._C._is_tracing())
 
 
 def _recorded(*tensors: Tensor | None) -> bool:

@@ -570,7 +570,8 @@ int splat_debug_expf(int n, const float* x, float* ours, float* cuda_exp, void* 
  * tensor of a call: 0 float32, 1 bfloat16, 2 float16 (row-major, contiguous,
  * 16-byte aligned bases).  activation: 0 none, 1 relu, 2 silu, 3 gelu (erf),
  * 4 sigmoid.  Sums are held in fp32 or more and rounded once, so results do
- * not depend on the order in which blocks run. */
+ * not depend on the order in which blocks run.  No output may overlap an input
+ * (float32 layers of more than 512 inputs keep sums in y on the way). */
 
 /* y = act(x weight^T + bias) + residual; x (rows, k), weight (n, k), bias (n)
  * or NULL, residual (rows, n) or NULL, y (rows, n).  A workspace of 16 bytes

@@ -223,3 +223,30 @@ def test_linear_whole_numbers(m, k, n, act, dtype):
                             ("dw", dw, dz.t() @ xd), ("db", db, dz.sum(0))):
         assert want.abs().max() < 2 ** 24, name
         assert torch.equal(got.detach(), want.to(dtype)), name
+
+@pytest.mark.parametrize("m, k, n", [(130, 1100, 40), (130, 5003, 33), (64, 16384, 24),
+                                     (40, 65535, 9), (20, 20001, 200),
+                                     (16400, 1100, 140)])
+@pytest.mark.parametrize("act", ["none", "sigmoid"])
+def test_linear_long_rows_of_one_sign(m, k, n, act):
+    """fp32: an accumulator sums 512 inputs in 32 truncating additions (48 u
+    with those within a product), the rest is added in fp32 (u / 2 each)."""
+    g = torch.Generator().manual_seed(43)
+    x = (0.5 + torch.rand(m, k, generator=g)).cuda()
+    w = ((0.5 + torch.rand(n, k, generator=g)) / k).cuda()
+    r = torch.randn(m, n, generator=g).cuda()
+    b = torch.randn(n, generator=g).cuda()
+    z = x.double() @ w.double().t()
+    e_z = (48 + k / 1024) * U * z + 2 * U * b.double().abs()
+    z = z + b.double()
+    value, rate = value_and_slope(z, act)
+    x.requires_grad_()
+    y = features.linear(x, w, b, residual=r, activation=act)
+    want = value + r.double()
+    check(y.detach(), want, e_z + 16 * U * value.abs() + U * want.abs(), "y")
+    # dx = dy act'(z) w: z is formed again
+    dy = torch.zeros(m, n, device="cuda")
+    dy[:, 1] = 1.0
+    dx, = torch.autograd.grad(y, x, dy)
+    want = rate[:, 1:2] * w.double()[1]
+    check(dx, want, (rate[:, 1:2] * 20 * U + e_z[:, 1:2]) * w.double()[1], "dx")
