@@ -47,7 +47,7 @@ struct alignas(sizeof(T) * V) Vec {
   T v[V];
 };
 
-// The same for V values at once: 16-bit ones are rounded in pairs.
+// from_float of V values at once: 16-bit ones are rounded in pairs.
 template <class T, int V>
 SPLAT_DEV Vec<T, V> round_values(const float (&v)[V]) {
   Vec<T, V> r;
@@ -110,10 +110,15 @@ SPLAT_DEV Vec<T, V> take_first(float (&v)[V]) {
 }
 
 // 2^x and 1/x in one instruction each, within 2 units of 2^-23; results below
-// the normal range are 0.
+// the normal range are 0 (of exp2_whole: are not).
 SPLAT_DEV float fast_exp2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+SPLAT_DEV float exp2_whole(float x) {
+  float r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 SPLAT_DEV float fast_reciprocal(float x) {
@@ -122,121 +127,144 @@ SPLAT_DEV float fast_reciprocal(float x) {
   return r;
 }
 
-// 1 / (1 + exp(-z)); exp(-z) overflowing to infinity gives 0.
-SPLAT_DEV float logistic(float z) {
-  return fast_reciprocal(1.0f + fast_exp2(z * -1.44269504088896341f));
+// The activations work on packed pairs: one instruction for both where there is
+// one.  FINE is for fp32, whose results keep their digits however small they
+// are; for 16-bit types 2^-14 of a result will do.
+//
+// 2^(-h C) for C = C_0 + C_1: the rounding of h C_0 alone, 2^-24 of itself, would
+// cost the power h C 2^-24.  FINE takes that rounding, C_1 and `rest`, what h
+// leaves out of its value (0 for NULL), to first order.  hn is -h.
+template <bool FINE>
+SPLAT_DEV f32x2 exp2_of(f32x2 hn, float c0, float c1, const f32x2* rest) {
+  const f32x2 y = mul2(hn, splat2(c0));
+  float a, b;
+  unpack2(y, a, b);
+  if constexpr (FINE) {
+    const f32x2 e = pack2(exp2_whole(a), exp2_whole(b));
+    f32x2 less = fma2(hn, splat2(-c1), fma2(hn, splat2(-c0), y));
+    if (rest) less = fma2(*rest, splat2(c0), less);
+    return fma2(mul2(less, splat2(-0.693147180559945309f)), e, e);
+  } else {
+    return pack2(fast_exp2(a), fast_exp2(b));
+  }
 }
 
-// The normal distribution's upper tail at |z| and its density: with
-// x = |z| / sqrt 2 and t = 1 / (1 + 0.3275911 x), erfc(x) is
-// t (a1 + a2 t + .. + a5 t^4) exp(-x^2) within 1.5e-7 (Abramowitz and Stegun,
-// Handbook of Mathematical Functions, 7.1.26).
-SPLAT_DEV void normal_tail(float z, float& tail, float& density) {
-  const float e = fast_exp2(z * z * -0.72134752044448170f);
-  const float t = fast_reciprocal(__fmaf_rn(fabsf(z), 0.23164189f, 1.0f));
-  float q = __fmaf_rn(t, 1.061405429f, -1.453152027f);
-  q = __fmaf_rn(q, t, 1.421413741f);
-  q = __fmaf_rn(q, t, -0.284496736f);
-  q = __fmaf_rn(q, t, 0.254829592f);
-  tail = 0.5f * q * t * e;
-  density = 0.39894228040143268f * e;
+// |z|; FINE: at most a value from which every function here is 0 or 1, because
+// infinities have no rounding.  NaN stays.
+template <bool FINE>
+SPLAT_DEV float magnitude(float z, float most) {
+  return FINE && fabsf(z) > most ? most : fabsf(z);
 }
 
-// NaN passes through every activation.
-template <int ACT>
-SPLAT_DEV float activate(float z) {
-  if constexpr (ACT == kRelu) return z < 0.0f ? 0.0f : z;
-  if constexpr (ACT == kSilu) return z * logistic(z);
-  if constexpr (ACT == kGelu) {
-    float tail, density;
-    normal_tail(z, tail, density);
-    return z * (z < 0.0f ? tail : 1.0f - tail);
-  }
-  if constexpr (ACT == kSigmoid) return logistic(z);
-  return z;
-}
-
-// d activate / dz.
-template <int ACT>
-SPLAT_DEV float slope(float z) {
-  if constexpr (ACT == kRelu) return z > 0.0f ? 1.0f : 0.0f;
-  if constexpr (ACT == kSilu) {
-    const float s = logistic(z);
-    return s * (1.0f + z * (1.0f - s));
-  }
-  if constexpr (ACT == kGelu) {
-    float tail, density;
-    normal_tail(z, tail, density);
-    return (z < 0.0f ? tail : 1.0f - tail) + z * density;
-  }
-  if constexpr (ACT == kSigmoid) {
-    const float s = logistic(z);
-    return s * (1.0f - s);
-  }
-  return 1.0f;
-}
-
-// Packed pairs: one instruction for both where there is one.
-SPLAT_DEV void logistic2(float& a, float& b) {
-  unpack2(mul2(pack2(a, b), pack2(-1.44269504088896341f, -1.44269504088896341f)), a, b);
-  unpack2(add2(pack2(fast_exp2(a), fast_exp2(b)), pack2(1.0f, 1.0f)), a, b);
-  a = fast_reciprocal(a);
-  b = fast_reciprocal(b);
-}
-// normal_tail of a pair: the distribution function's values and the densities'
-// exponentials.
-SPLAT_DEV void normal2(f32x2 z, float a, float b, f32x2& cdf, f32x2& e) {
+// e = exp(-|z|) and r = 1 / (1 + e): the logistic function is r or, of negative
+// arguments, e r, and the other of them is 1 less it, without cancellation.
+template <bool FINE>
+SPLAT_DEV void logistic_parts(float a, float b, f32x2& e, f32x2& r) {
+  const f32x2 hn = pack2(-magnitude<FINE>(a, 200.0f), -magnitude<FINE>(b, 200.0f));
+  e = exp2_of<FINE>(hn, 1.44269504088896341f, 1.925962990e-8f, nullptr);
   float u, v;
-  unpack2(mul2(mul2(z, z), splat2(-0.72134752044448170f)), u, v);
-  e = pack2(fast_exp2(u), fast_exp2(v));
-  unpack2(fma2(pack2(fabsf(a), fabsf(b)), splat2(0.23164189f), splat2(1.0f)), u, v);
+  unpack2(add2(e, splat2(1.0f)), u, v);
+  r = pack2(fast_reciprocal(u), fast_reciprocal(v));
+}
+template <bool FINE>
+SPLAT_DEV void logistic2(float& a, float& b) {
+  if constexpr (FINE) {
+    f32x2 e, r;
+    logistic_parts<true>(a, b, e, r);
+    float u, v, s, t;
+    unpack2(mul2(e, r), u, v);
+    unpack2(r, s, t);
+    a = a < 0.0f ? u : s;
+    b = b < 0.0f ? v : t;
+  } else {  // exp(-z) overflowing to infinity gives 0
+    unpack2(mul2(pack2(a, b), splat2(-1.44269504088896341f)), a, b);
+    unpack2(add2(pack2(fast_exp2(a), fast_exp2(b)), splat2(1.0f)), a, b);
+    a = fast_reciprocal(a);
+    b = fast_reciprocal(b);
+  }
+}
+
+// The normal distribution function of a pair, and e = exp(-z^2 / 2).  Its tail
+// at |z| is e Q(|z|); Q(z) / t with t = 1 / (1 + p z) is a polynomial in t fitted
+// to erfc(z / sqrt 2) exp(z^2 / 2) / 2 by least squares whose weights follow the
+// relative error (Lawson's iteration): 2.5e-8 relative up to 20 (FINE), 2.9e-5
+// up to 13.5.
+template <bool FINE>
+SPLAT_DEV void normal2(float a, float b, f32x2& cdf, f32x2& e) {
+  const float x = magnitude<FINE>(a, 20.0f), y = magnitude<FINE>(b, 20.0f);
+  const f32x2 z = pack2(x, y), hn = mul2(z, pack2(-x, -y));
+  const f32x2 rest = fma2(z, z, hn);
+  e = exp2_of<FINE>(hn, 0.72134752044448170f, 9.62981495e-9f, &rest);
+  float u, v;
+  unpack2(fma2(z, splat2(FINE ? 0.27f : 0.375f), splat2(1.0f)), u, v);
   const f32x2 t = pack2(fast_reciprocal(u), fast_reciprocal(v));
-  f32x2 q = fma2(t, splat2(0.5f * 1.061405429f), splat2(0.5f * -1.453152027f));
-  q = fma2(q, t, splat2(0.5f * 1.421413741f));
-  q = fma2(q, t, splat2(0.5f * -0.284496736f));
-  q = fma2(q, t, splat2(0.5f * 0.254829592f));
+  f32x2 q;
+  if constexpr (FINE) {
+    q = fma2(t, splat2(0.0290643238f), splat2(-0.127003357f));
+    q = fma2(q, t, splat2(0.170891672f));
+    q = fma2(q, t, splat2(-0.0705219954f));
+    q = fma2(q, t, splat2(0.108767502f));
+    q = fma2(q, t, splat2(0.071631223f));
+    q = fma2(q, t, splat2(0.101922527f));
+    q = fma2(q, t, splat2(0.107526444f));
+    q = fma2(q, t, splat2(0.107721671f));
+  } else {
+    q = fma2(t, splat2(-0.0909852087f), splat2(0.201043263f));
+    q = fma2(q, t, splat2(0.0829740763f));
+    q = fma2(q, t, splat2(0.157920063f));
+    q = fma2(q, t, splat2(0.149041131f));
+  }
   float ta, tb, ua, ub;
   const f32x2 tail = mul2(mul2(q, t), e);
   unpack2(tail, ta, tb);
   unpack2(fma2(tail, splat2(-1.0f), splat2(1.0f)), ua, ub);
   cdf = pack2(a < 0.0f ? ta : ua, b < 0.0f ? tb : ub);
 }
-template <int ACT>
+
+// NaN passes through every activation.
+template <int ACT, bool FINE>
 SPLAT_DEV void activate2(float& a, float& b) {
-  if constexpr (ACT == kSilu) {
+  if constexpr (ACT == kRelu) {
+    a = a < 0.0f ? 0.0f : a;
+    b = b < 0.0f ? 0.0f : b;
+  } else if constexpr (ACT == kSilu) {
     float s = a, t = b;
-    logistic2(s, t);
+    logistic2<FINE>(s, t);
     unpack2(mul2(pack2(a, b), pack2(s, t)), a, b);
-  } else if constexpr (ACT == kSigmoid) {
-    logistic2(a, b);
   } else if constexpr (ACT == kGelu) {
-    const f32x2 z = pack2(a, b);
     f32x2 cdf, e;
-    normal2(z, a, b, cdf, e);
-    unpack2(mul2(z, cdf), a, b);
-  } else {
-    a = activate<ACT>(a);
-    b = activate<ACT>(b);
+    normal2<FINE>(a, b, cdf, e);
+    unpack2(mul2(pack2(a, b), cdf), a, b);
+  } else if constexpr (ACT == kSigmoid) {
+    logistic2<FINE>(a, b);
   }
 }
 
-template <int ACT>
+// d activate / dz.
+template <int ACT, bool FINE>
 SPLAT_DEV void slope2(float& a, float& b) {
-  if constexpr (ACT == kSilu || ACT == kSigmoid) {
-    float s = a, t = b;
-    logistic2(s, t);
-    const f32x2 p = pack2(s, t), z = pack2(a, b);
-    // s + s z (1 - s), and s (1 - s)
-    const f32x2 q = fma2(pack2(-s, -t), ACT == kSilu ? z : p, ACT == kSilu ? z : p);
-    unpack2(ACT == kSilu ? fma2(p, q, p) : q, a, b);
+  if constexpr (ACT == kRelu) {
+    a = a > 0.0f ? 1.0f : 0.0f;
+    b = b > 0.0f ? 1.0f : 0.0f;
+  } else if constexpr (ACT == kSilu || ACT == kSigmoid) {
+    f32x2 e, r;
+    logistic_parts<FINE>(a, b, e, r);
+    const f32x2 other = mul2(e, r), both = mul2(other, r);  // s (1 - s)
+    if constexpr (ACT == kSigmoid) {
+      unpack2(both, a, b);
+    } else {
+      float u, v, s, t;
+      unpack2(other, u, v);
+      unpack2(r, s, t);
+      // s + z s (1 - s)
+      unpack2(fma2(pack2(a, b), both, pack2(a < 0.0f ? u : s, b < 0.0f ? v : t)), a, b);
+    }
   } else if constexpr (ACT == kGelu) {
-    const f32x2 z = pack2(a, b);
     f32x2 cdf, e;
-    normal2(z, a, b, cdf, e);
-    unpack2(fma2(mul2(z, splat2(0.39894228040143268f)), e, cdf), a, b);
+    normal2<FINE>(a, b, cdf, e);
+    unpack2(fma2(mul2(pack2(a, b), splat2(0.39894228040143268f)), e, cdf), a, b);
   } else {
-    a = slope<ACT>(a);
-    b = slope<ACT>(b);
+    a = b = 1.0f;
   }
 }
 

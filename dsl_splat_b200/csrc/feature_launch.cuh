@@ -127,7 +127,8 @@ int launch_product(ProductParams p, cudaStream_t s) {
   // two tiles of A as they are in memory, where two stages fit beside them
   // (35 -> 32 fp32 gelu over 10^6 rows 113 us against 140 read as needed,
   // 35 -> 64 bf16 78 against 82)
-  if (PA != 2 && !p.copy_operands && !AMN && p.tiles_n == 1 && p.a_ld == p.k && host::aligned(p.a, 16)) {
+  if (PA != 2 && !p.copy_operands && !AMN && p.tiles_n == 1 && p.a_ld == p.k &&
+      host::aligned(p.a, 16)) {
     const long long raw = (kTileRows * p.k * static_cast<long long>(sizeof(SA)) + 127) / 128 * 128;
     if (fixed + 2 * stage + 2 * raw > budget && blocks == 2) blocks = 1, budget = kOneBlockBytes;
     if (fixed + 2 * stage + 2 * raw <= budget) p.raw_bytes = static_cast<int>(raw);

@@ -19,7 +19,8 @@ namespace feature {
 // ---- sums over splits and rows ---------------------------------------------------
 
 // Adds the splits' partial sums, `stride` values apart, in a fixed order and in
-// doubles (there may be a million): 32 threads to a value.  The first count_a values go to a, the rest to b.
+// doubles (there may be a million): 32 threads to a value.  The first count_a
+// values go to a, the rest to b.
 constexpr int kJoinLanes = 32;
 template <class T>
 __global__ void __launch_bounds__(32 * kJoinLanes)

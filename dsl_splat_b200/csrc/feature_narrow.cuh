@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
           for (int i = 0; i < 8; i += 2) {
             f32x2 dz = pack2(e[i], e[i + 1]);
             if constexpr (ACT != kNone) {
-              slope2<ACT>(v[j * 8 + i], v[j * 8 + i + 1]);
+              slope2<ACT, false>(v[j * 8 + i], v[j * 8 + i + 1]);
               dz = mul2(dz, pack2(v[j * 8 + i], v[j * 8 + i + 1]));
             }
             f32x2& sum = sum_b[cc][j * 4 + i / 2];

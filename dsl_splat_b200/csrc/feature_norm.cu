@@ -102,26 +102,26 @@ SPLAT_DEV Pairs<V> fma(Pairs<V> a, const Pairs<V>& b, const Pairs<V>& c) {
   for (int i = 0; i < Pairs<V>::N; ++i) a.v[i] = fma2(a.v[i], b.v[i], c.v[i]);
   return a;
 }
-template <int ACT, int V>
+template <int ACT, bool FINE, int V>
 SPLAT_DEV Pairs<V> activate(Pairs<V> x) {
 #pragma unroll
   for (int i = 0; i < Pairs<V>::N; ++i) {
     float a, b;
     unpack2(x.v[i], a, b);
-    if constexpr (V == 1) a = activate<ACT>(a);
-    else activate2<ACT>(a, b);
+    if constexpr (V == 1) b = a;
+    activate2<ACT, FINE>(a, b);
     x.v[i] = pack2(a, b);
   }
   return x;
 }
-template <int ACT, int V>
+template <int ACT, bool FINE, int V>
 SPLAT_DEV Pairs<V> slope(Pairs<V> x) {
 #pragma unroll
   for (int i = 0; i < Pairs<V>::N; ++i) {
     float a, b;
     unpack2(x.v[i], a, b);
-    if constexpr (V == 1) a = slope<ACT>(a);
-    else slope2<ACT>(a, b);
+    if constexpr (V == 1) b = a;
+    slope2<ACT, FINE>(a, b);
     x.v[i] = pack2(a, b);
   }
   return x;
@@ -397,9 +397,8 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_sums_kernel(const NormPar
   for (int j = 0; j < V; ++j) slots[threadIdx.x * V + j] = r[j];
   __syncthreads();
   const int first = at.column * l.threads * V;  // flat position of slots[0] in a step
-  double2* out = static_cast<double2*>(p.partial) +
-                 ((static_cast<long long>(at.sample) * l.blocks + at.part) * l.columns + at.column) *
-                     l.channels;
+  const long long block = (static_cast<long long>(at.sample) * l.blocks + at.part) * l.columns;
+  double2* out = static_cast<double2*>(p.partial) + (block + at.column) * l.channels;
   join_threads<V>(l, at.part, first, min(l.threads, l.step - at.column * l.threads) * V, slots,
                   [&](int c, double a, double b) { out[c] = make_double2(a, b); });
 }
@@ -601,7 +600,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_apply_kernel(const NormPa
   ch.load(p, at);
   const auto result = [&](const Values& v) {
     return round_pairs<T, V>(
-        activate<ACT, V>(fma(widen_pairs<T, V>(v) + ch.minus, ch.scale, ch.bias)));
+        activate<ACT, sizeof(T) == 4, V>(fma(widen_pairs<T, V>(v) + ch.minus, ch.scale, ch.bias)));
   };
   if (at.left) store_part<T, V>(to, result(load_part<T, V>(from, at.left)), at.left);
   constexpr int U = 4;
@@ -642,7 +641,8 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_backward_sums_kernel(cons
     ch.load(p, at);
     const auto add = [&](const Values& v, const Values& g) {
       const Pairs<V> d = widen_pairs<T, V>(v) + ch.minus;
-      const Pairs<V> du = slope<ACT, V>(fma(d, ch.scale, ch.bias)) * widen_pairs<T, V>(g);
+      const Pairs<V> du =
+          slope<ACT, sizeof(T) == 4, V>(fma(d, ch.scale, ch.bias)) * widen_pairs<T, V>(g);
       s1 = s1 + du;
       s2 = fma(du, d, s2);
     };
@@ -739,7 +739,8 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_backward_apply_kernel(con
   ch.load(p, at);
   const auto result = [&](const Values& v, const Values& g) {
     const Pairs<V> d = widen_pairs<T, V>(v) + ch.minus;
-    const Pairs<V> du = slope<ACT, V>(fma(d, ch.scale, ch.bias)) * widen_pairs<T, V>(g);
+    const Pairs<V> du =
+        slope<ACT, sizeof(T) == 4, V>(fma(d, ch.scale, ch.bias)) * widen_pairs<T, V>(g);
     return round_pairs<T, V>(fma(du, ch.scale, fma(d, ch.k2, ch.k1)));
   };
   if (at.left)
@@ -927,7 +928,7 @@ __global__ void __launch_bounds__(kSmallThreads) norm_small_kernel(const NormPar
   T* to = static_cast<T*>(p.out) + at.sample * l.span + at.first;
   const auto result = [&](const Values& v) {
     return round_pairs<T, V>(
-        activate<ACT, V>(fma(widen_pairs<T, V>(v) + ch.minus, ch.scale, ch.bias)));
+        activate<ACT, sizeof(T) == 4, V>(fma(widen_pairs<T, V>(v) + ch.minus, ch.scale, ch.bias)));
   };
   for (int i0 = 0; i0 < at.count; i0 += U) {
     Values v[U];
@@ -971,7 +972,8 @@ __global__ void __launch_bounds__(kSmallThreads)
     ch.load(p, at, nullptr, nullptr);
     const auto add = [&](const Values& v, const Values& g) {
       const Pairs<V> d = widen_pairs<T, V>(v) + ch.minus;
-      const Pairs<V> du = slope<ACT, V>(fma(d, ch.scale, ch.bias)) * widen_pairs<T, V>(g);
+      const Pairs<V> du =
+          slope<ACT, sizeof(T) == 4, V>(fma(d, ch.scale, ch.bias)) * widen_pairs<T, V>(g);
       s1 = s1 + du;
       s2 = fma(du, d, s2);
     };
@@ -1039,7 +1041,8 @@ __global__ void __launch_bounds__(kSmallThreads)
   T* to = static_cast<T*>(p.out) + offset;
   const auto result = [&](const Values& v, const Values& g) {
     const Pairs<V> d = widen_pairs<T, V>(v) + k.minus;
-    const Pairs<V> du = slope<ACT, V>(fma(d, k.scale, k.bias)) * widen_pairs<T, V>(g);
+    const Pairs<V> du =
+        slope<ACT, sizeof(T) == 4, V>(fma(d, k.scale, k.bias)) * widen_pairs<T, V>(g);
     return round_pairs<T, V>(fma(du, k.scale, fma(d, k.k2, k.k1)));
   };
   constexpr int U = 4;

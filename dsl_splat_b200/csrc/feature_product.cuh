@@ -43,7 +43,9 @@ constexpr int kAPlane = kTileRows * 128;
 // Producer threads: operands that are split always pass through registers, so
 // there it is threads that keep loads in flight.  Two-part ones always lie in
 // memory as two planes and are copied.
-__host__ __device__ constexpr int producers(int pa, int pb) { return pa <= 2 && pb <= 2 ? 128 : 256; }
+__host__ __device__ constexpr int producers(int pa, int pb) {
+  return pa <= 2 && pb <= 2 ? 128 : 256;
+}
 // fp32 operands keep the products of lower parts in an accumulator of their
 // own: the tensor core truncates its sums, so each addition at full magnitude
 // costs up to 2^-24, and the lower products must not add to their number.
@@ -522,7 +524,7 @@ SPLAT_DEV void finish_row(const Patch<TE, W>& extra, bool with_extra, float (&v)
     float* z = v + piece * V;
     if constexpr (EPI == kForward) {
 #pragma unroll
-      for (int j = 0; j < V; j += 2) activate2<ACT>(z[j], z[j + 1]);
+      for (int j = 0; j < V; j += 2) activate2<ACT, sizeof(TE) == 4>(z[j], z[j + 1]);
     }
     if (EPI == kSlope || with_extra) {
       const float4 raw = load_shared(extra.at(lane, piece));
@@ -533,7 +535,7 @@ SPLAT_DEV void finish_row(const Patch<TE, W>& extra, bool with_extra, float (&v)
         if constexpr (EPI == kForward)
           unpack2(add2(pack2(z[j], z[j + 1]), pack2(e[j], e[j + 1])), z[j], z[j + 1]);
         else {
-          slope2<ACT>(z[j], z[j + 1]);
+          slope2<ACT, sizeof(TE) == 4>(z[j], z[j + 1]);
           unpack2(mul2(pack2(z[j], z[j + 1]), pack2(e[j], e[j + 1])), z[j], z[j + 1]);
         }
       }
@@ -957,7 +959,8 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
               for (int j = 0; j < Patch<TO>::kPieces; ++j)
                 store_shared(out_patch.at(lane, j),
                              make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
-                                        __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3])));
+                                        __float_as_uint(v[4 * j + 2]),
+                                        __float_as_uint(v[4 * j + 3])));
               __syncwarp();
               if (!last) {
                 out_patch.store(to, p.out_ld, rows, cols, p.out_vector, sum_k != tile.k0);

@@ -250,3 +250,75 @@ def test_linear_long_rows_of_one_sign(m, k, n, act):
     dx, = torch.autograd.grad(y, x, dy)
     want = rate[:, 1:2] * w.double()[1]
     check(dx, want, (rate[:, 1:2] * 20 * U + e_z[:, 1:2]) * w.double()[1], "dx")
+
+# ---- activations at large arguments ------------------------------------------------
+
+def through(z, act, dtype):
+    """act and its slope of the values z through a layer of weight 1, whose
+    products and sums are exact."""
+    x = z.to(dtype).cuda().reshape(-1, 1).requires_grad_()
+    w = torch.ones(1, 1, device="cuda", dtype=dtype)
+    y = features.linear(x, w, activation=act)
+    slope, = torch.autograd.grad(y, x, torch.ones_like(y))
+    return x.detach().double(), y.detach(), slope
+
+
+def exact_activation(z, act):
+    """Value and slope without cancellation, and the slope's terms."""
+    if act == "gelu":
+        c = 0.5 * torch.special.erfc(-z / math.sqrt(2))
+        d = z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+        return z * c, c + d, c + d.abs()
+    s, t = torch.special.expit(z), torch.special.expit(-z)
+    if act == "silu":
+        return z * s, s + z * s * t, s + (z * s * t).abs()
+    return s, s * t, s * t
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+def test_activations_keep_their_digits(act):
+    """fp32: 16 u of the value itself, however small (and the smallest normal
+    value's step)."""
+    most = 13.0 if act == "gelu" else 86.0
+    z = torch.cat([torch.linspace(-most, most, 20001), torch.linspace(-1, 1, 4001),
+                   torch.tensor([0.0, -0.0, 1e-20, -1e-20, 200.0, 1e30])])
+    z, y, slope = through(z, act, torch.float32)
+    value, rate, terms = exact_activation(z, act)
+    rate = torch.where(z > 100, rate.nan_to_num(), rate)
+    check(y, value, 16 * U * value.abs() + 2.0 ** -126, "y")
+    check(slope, rate, 16 * U * terms.nan_to_num() + 2.0 ** -126, "slope")
+
+
+@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+def test_activations_below_the_normal_range(act):
+    """e^z below 2^-126 is not taken for 0."""
+    z, y, _ = through(torch.linspace(-95, -86, 901), act, torch.float32)
+    value, _, _ = exact_activation(z, act)
+    check(y, value, 16 * U * value.abs() + 16 * 2.0 ** -149 * (1 + z.abs()), "y")
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+def test_activations_of_short_types(act, dtype):
+    """2^-13 relative where the type's own step is 2^-8 or 2^-11."""
+    most = 12.0 if act == "gelu" else 80.0
+    z, y, slope = through(torch.linspace(-most, most, 60001), act, dtype)
+    value, rate, terms = exact_activation(z, act)
+    check(y, value, 2.0 ** -13 * value.abs(), "y")
+    check(slope, rate, 2.0 ** -13 * terms, "slope")
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+def test_group_norm_activations_keep_their_digits(act):
+    """The same through group norm: one group of -1 and 1, scaled by the
+    weights."""
+    c = 512
+    x = torch.ones(1, 2, 2, c, device="cuda")
+    x[:, :, 1] = -1.0
+    w = torch.linspace(0.0, 12.0, c, device="cuda")
+    y = features.group_norm(x, 1, w, eps=2.0 ** -40, activation=act)
+    # hat is +-1 to 2^-40; z = hat w, 4 u
+    z = (x.double() * w.double())
+    value, _, terms = exact_activation(z, act)
+    # an argument off by 4 u |z| changes the tails by 4 u z^2 of themselves
+    check(y, value, (16 + 4 * z.abs() + 4 * z * z) * U * value.abs() + 2.0 ** -126, "y")
