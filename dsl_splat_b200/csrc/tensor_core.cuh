@@ -154,18 +154,6 @@ SPLAT_DEV void tmem_load16(uint32_t address, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// One column of the same.
-SPLAT_DEV float tmem_load1(uint32_t address) {
-  uint32_t r;
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r)
-      : "r"(address)
-      : "memory");
-  return __uint_as_float(r);
-}
-
 // ---- matrix products ---------------------------------------------------------
 
 // Operands lie in shared memory as blocks of rows of 128 bytes (64 16-bit
