@@ -54,7 +54,10 @@ int launch_product(ProductParams p, cudaStream_t s) {
   // arithmetic two blocks' epilogues share an SM (512 -> 512 fp16 gelu over
   // 131072 rows 103 us against 107 in 256-wide tiles, 256 -> 256 bf16 silu 39
   // against 48)
-  const int widest = PA <= 2 && PB == 1 && EPI == kPlain ? 256 : 128;
+  constexpr long long kMostSum = kMostAdditions * 16 / PA;  // of a 16-bit layer's accumulator
+  // 16-bit results of more are added up in shared memory, a patch to a warp
+  p.held = sizeof(TO) == 2 && p.k > kMostSum;
+  const int widest = p.held ? 64 : PA <= 2 && PB == 1 && EPI == kPlain ? 256 : 128;
   p.tiles_n = (p.n + widest - 1) / widest;
   p.tile_n = ((p.n + p.tiles_n - 1) / p.tiles_n + 31) / 32 * 32;
   const long long tiles_m = (p.m + kTileRows - 1) / kTileRows;
@@ -75,10 +78,7 @@ int launch_product(ProductParams p, cudaStream_t s) {
   p.tmem_columns = 32;
   constexpr int kAcc = accumulators(PA, PB);
   // sums of several accumulators are joined in fp32 outputs
-  p.k_per_sum = kAcc == 2 ? kExactSum
-                : EPI == kPlain && sizeof(TO) == 4
-                    ? kMostAdditions * 16 / PA
-                    : p.k_per_split;
+  p.k_per_sum = kAcc == 2 ? kExactSum : kMostSum;
   // (35 -> 32 fp32 gelu over 10^6 rows 113 us against 154 without, 32 -> 3 bf16
   // over 1.9 10^6 67 against 84, 64 -> 32 bf16 71 against 69)
   p.alternate = p.tile_n == 32 && p.k_per_sum >= p.k_per_split;
@@ -89,7 +89,8 @@ int launch_product(ProductParams p, cudaStream_t s) {
   const long long chunks = (p.k + kChunk - 1) / kChunk;
   const long long whole_b = chunks * b_bytes;
   // a patch of results, and one of the extra values
-  p.staging = 1024 * static_cast<int>(sizeof(TO) + (p.extra ? sizeof(TE) : 0));
+  p.staging =
+      1024 * static_cast<int>(sizeof(TO) + (p.extra ? sizeof(TE) : 0) + (p.held ? 4 : 0));
   int fixed = kEpilogueWarps * p.staging + (p.bias_shared * 4 + 1023) / 1024 * 1024;
   // B stays where two stages of A fit beside it
   p.resident = p.splits == 1 && p.tiles_n == 1 && whole_b <= kMaxResidentBytes &&
@@ -142,7 +143,7 @@ int launch_product(ProductParams p, cudaStream_t s) {
   if (p.stages < 1) return host::fail(kTooLarge, "feature_linear: no room for a stage");
   if (EPI != kPlain) p.copy_extra = make_map<TE>(p.extra_map, p.extra, p.m, p.n, p.n, 32, 32);
   // partial sums are added to or lie one split behind the other
-  if (p.splits == 1 && p.k_per_sum >= p.k)
+  if (p.splits == 1 && (p.k_per_sum >= p.k || p.held))
     p.copy_out = make_map<TO>(p.out_map, p.out, p.m, p.n, p.out_ld, 32, 32) &&
                  (!p.out_second ||
                   make_map<TO>(p.out_second_map, p.out_second, p.m, p.n, p.out_ld, 32, 32));

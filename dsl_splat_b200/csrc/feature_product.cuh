@@ -53,10 +53,8 @@ __host__ __device__ constexpr int producers(int pa, int pb) {
 __host__ __device__ constexpr int accumulators(int pa, int pb) { return pa == 3 || pb == 3 ? 2 : 1; }
 // k that such an accumulator sums before it is added up in fp32 (32 additions).
 constexpr int kExactSum = 512;
-// Additions into an accumulator of a 16-bit layer's dW, whose sums run over the
-// rows: they cost it about 2e-8 relative each and 2^-23 at most, a quarter of half
-// a step of f16 in all.  (y and dx of 16-bit layers sum up to 65535 values: at most
-// 8192 additions, 1.4e-4.)
+// Additions into an accumulator of a 16-bit layer: each costs it up to 2^-23, so
+// that they stay below a quarter of half a step of f16.
 constexpr int kMostAdditions = 1024;
 
 // act(C + bias) + residual; dy act'(C + bias); C.
@@ -81,6 +79,7 @@ struct ProductParams {
   int a_vector, b_vector;  // bytes that every row start and chunk is aligned to
   long long k_per_split;   // a multiple of kChunk unless there is one split
   long long k_per_sum;     // of one accumulator; the tile's sums are added in `out` (fp32)
+  int held;                // or, of 16-bit results, in shared memory
   int splits, tile_n;
   uint32_t tiles_n, tiles_m, tiles;  // tiles = splits * tiles_m * tiles_n, below 2^31
   int stages, resident, activation;
@@ -947,7 +946,30 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] += low[i];
           }
-          // rows of several sums: those before the last are stored, each onto the ones
+          // 16-bit results of several sums: a lane holds its row's in shared memory
+          if constexpr (sizeof(TO) == 2) {
+            if (p.held) {
+              const Patch<float> held{out_patch.base + 1024 * static_cast<int>(sizeof(TO)) +
+                                      (p.extra ? 1024 * static_cast<int>(sizeof(TE)) : 0)};
+              const bool last = sum_k + p.k_per_sum >= tile.k1;
+              const int lane = threadIdx.x & 31;
+#pragma unroll
+              for (int j = 0; j < Patch<float>::kPieces; ++j) {
+                const uint32_t place = held.at(lane, j);
+                if (sum_k != tile.k0) {
+                  const float4 s = load_shared(place);
+                  v[4 * j] += s.x, v[4 * j + 1] += s.y, v[4 * j + 2] += s.z, v[4 * j + 3] += s.w;
+                }
+                if (!last)
+                  store_shared(place,
+                               make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                                          __float_as_uint(v[4 * j + 2]),
+                                          __float_as_uint(v[4 * j + 3])));
+              }
+              if (!last) continue;
+            }
+          }
+          // fp32 ones: the sums before the last are stored, each onto the ones
           // before, and the last takes them from there
           if constexpr (kExtra && kAcc == 2) {
             if (p.k_per_sum < p.k) {
@@ -1055,7 +1077,8 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
             } else {
               __syncwarp();
               out_patch.store(static_cast<TO*>(out) + out_at + col0, p.out_ld, rows, cols,
-                              p.out_vector, !kExtra && sum_k != tile.k0);
+                              p.out_vector,
+                              !kExtra && sizeof(TO) == 4 && sum_k != tile.k0);
             }
           };
           if constexpr (EPI == kSlope && sizeof(TO) == 2) {

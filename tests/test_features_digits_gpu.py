@@ -322,3 +322,46 @@ def test_group_norm_activations_keep_their_digits(act):
     value, _, terms = exact_activation(z, act)
     # an argument off by 4 u |z| changes the tails by 4 u z^2 of themselves
     check(y, value, (16 + 4 * z.abs() + 4 * z * z) * U * value.abs() + 2.0 ** -126, "y")
+
+
+@pytest.mark.parametrize("k", [16384, 20000, 40008, 65535])
+@pytest.mark.parametrize("n", [1, 33, 200])
+def test_short_types_over_long_rows(k, n):
+    """fp16: the tensor core cuts what an addition leaves below the step of its
+    accumulator.  One large product first and then sums of 1.9 steps each lose
+    nine tenths of a step an addition; 1024 additions (u each) at most lie in
+    one accumulator, the rest is added in fp32."""
+    x = torch.full((130, k), 2.0 ** -13, device="cuda", dtype=torch.float16)
+    w = torch.full((n, k), 1.9 * 2.0 ** -14, device="cuda", dtype=torch.float16)
+    x[:, 0] = 1.0
+    w[:, 0] = 1.0
+    want = x.double() @ w.double().t()
+    tolerance = (1024 + 16) * U * want
+    check(features.linear(x, w), want, tolerance, "y")
+    residual = torch.ones_like(want, dtype=torch.float16)
+    check(features.linear(x, w, residual=residual), want + 1, tolerance + U * (want + 1),
+          "y + residual")
+    # dx of a layer with so many outputs, and z in its gradient, are such sums too
+    leaf = w[:, :1].new_zeros(130, n).requires_grad_()
+    dx, = torch.autograd.grad(features.linear(leaf, w.t()), leaf, x)
+    check(dx, want, tolerance, "dx")
+    x.requires_grad_()
+    y = features.linear(x, w, activation="sigmoid")
+    dy = torch.zeros_like(y)
+    dy[:, 0] = 1.0
+    dx, = torch.autograd.grad(y, x, dy)
+    s = torch.sigmoid(want)
+    check(y.detach(), s, tolerance + 16 * U, "sigmoid")
+    rate = (s * (1 - s))[:, :1]
+    check(dx, rate * w.double()[0], (tolerance[:, :1] + 2.0 ** -13 * rate) * w.double()[0], "dx")
+
+
+def test_short_types_over_long_rows_of_two_parts():
+    """The same for dx where dz is two values: 512 additions of each."""
+    n = 65535
+    dy = torch.full((64, n), 2.0 ** -13, device="cuda", dtype=torch.bfloat16)
+    x = torch.zeros(64, 40, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    w = torch.rand(n, 40, generator=torch.Generator().manual_seed(47)).to(torch.bfloat16).cuda()
+    dx, = torch.autograd.grad(features.linear(x, w, activation="sigmoid"), x, dy)
+    want = dy.double() @ w.double() / 4  # the slope at 0
+    check(dx, want, (1024 + 16 + 16) * U * want, "dx")
