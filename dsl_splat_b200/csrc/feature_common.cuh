@@ -246,6 +246,12 @@ SPLAT_DEV void slope2(float& a, float& b) {
   if constexpr (ACT == kRelu) {
     a = a > 0.0f ? 1.0f : 0.0f;
     b = b > 0.0f ? 1.0f : 0.0f;
+  } else if constexpr (ACT == kSilu && !FINE) {
+    // s + s z (1 - s): where 1 - s cancels, it is small beside the rest
+    float s = a, t = b;
+    logistic2<false>(s, t);
+    const f32x2 p = pack2(s, t), z = pack2(a, b);
+    unpack2(fma2(p, fma2(pack2(-s, -t), z, z), p), a, b);
   } else if constexpr (ACT == kSilu || ACT == kSigmoid) {
     f32x2 e, r;
     logistic_parts<FINE>(a, b, e, r);

@@ -779,15 +779,14 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_backward_apply_kernel(con
 // are read again, out of the L2.  The blocks exchange
 // their channel sums through distributed shared memory, and each forms the
 // group's moments for itself.  One launch and no workspace: a call on
-// 37x53x35 fp32 takes 27 us against 42 in passes, on 80x80x32 fp32 (819 KB) 26
-// against 40, on 64 such samples 40 against 52 (two launches fewer, and x is
-// read once).
+// 37x53x35 fp32 takes 15 us against 22 in passes, on 80x80x32 fp32 (819 KB) 17
+// against 22.
 
 constexpr int kSmallThreads = 512;
 constexpr size_t kMostShared = 226 * 1024;
-constexpr int kKeptBytes = 150 * 1024;   // of a block's values, kept in shared memory
-constexpr int kSmallBytes = 512 * 1024;  // or read again
-constexpr int kMaxRereadSamples = 8;
+constexpr int kSmallForward = 450000, kSmallBackward = 300000;  // values of a sample
+constexpr int kFewSamples = 8;
+constexpr long long kManyBytes = 1792 * 1024;
 constexpr int kSmallChannels = 1024;
 
 // The cluster's sums per channel of its blocks' in `own`; all blocks end with
@@ -1128,12 +1127,14 @@ Plan make_plan(int value_bytes, int samples, long long positions, int channels, 
   const int per_sm = backward ? kBackwardBlocksPerSm : kForwardBlocksPerSm;
   const long long bytes = positions * channels * value_bytes * (backward ? 2 : 1);
   plan.l = make_layout(samples, positions, channels, plan.vector, per_sm, kSmallThreads);
-  // values read twice by few blocks only pay where there are few samples: 1, 8,
-  // 16 and 64 of 170x170x32 fp32 30, 31, 66 and 169 us against 40, 39, 43 and
-  // 145 in passes
+  // few samples, whose clusters run at once, or many that are quick: a cluster is
+  // slower than the passes' many blocks (forward, 1 and 4 of 100x100x32 fp32 in 19
+  // us each against 22 and 25 in passes, one of 130x130x32 25 against 22; 16 and 64
+  // of 20x20x32 21 and 49 against 23 and 35, of 10x10x32 15 and 15 against 22 and
+  // 33; backward, one of 80x80x32 19 against 20, of 100x100x32 23 against 20)
   plan.small = plan.l.columns == 1 && channels <= kSmallChannels &&
-               bytes <= static_cast<long long>(kMaxCluster) *
-                            (samples <= kMaxRereadSamples ? kSmallBytes : kKeptBytes);
+               positions * channels <= (backward ? kSmallBackward : kSmallForward) &&
+               (samples <= kFewSamples || samples * bytes <= kManyBytes);
   plan.shared_bytes = 0;
   if (!plan.small) {
     plan.l = make_layout(samples, positions, channels, plan.vector, per_sm, kMaxThreads);
@@ -1143,12 +1144,10 @@ Plan make_plan(int value_bytes, int samples, long long positions, int channels, 
     while (blocks < kMaxCluster && blocks * 8192LL < bytes && blocks < plan.l.steps) blocks *= 2;
     plan.l.blocks = blocks;
     plan.l.per_block = (plan.l.steps + blocks - 1) / blocks;
-    plan.keep = bytes <= static_cast<long long>(kMaxCluster) * kKeptBytes;
     const auto need = [&](int arrays) {
       return small_bytes(plan.l, plan.vector, value_bytes, groups, arrays, backward);
     };
-    // many channels, or a last step of few vectors, can leave less room
-    if (plan.keep && need(backward ? 2 : 1) > kMostShared) plan.keep = false;
+    plan.keep = need(backward ? 2 : 1) <= kMostShared;
     plan.shared_bytes = need(!plan.keep ? 0 : backward ? 2 : 1);
   }
   return plan;
