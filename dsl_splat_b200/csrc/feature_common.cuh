@@ -98,14 +98,20 @@ SPLAT_DEV void widen(const Vec<T, V>& r, float (&v)[V]) {
 // infinity or a NaN.
 template <class T, int V>
 SPLAT_DEV Vec<T, V> take_first(float (&v)[V]) {
-  constexpr float kMost = kIsF16<T> ? 65504.0f : 3.38953138925153547590470800371e38f;
-  float o[V];
+  Vec<T, V> first;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&first);
 #pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = fminf(fmaxf(v[i], -kMost), kMost);
-  const Vec<T, V> first = round_values<T, V>(o);
+  for (int i = 0; i < V; i += 2) {
+    if constexpr (kIsF16<T>)
+      asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(w[i / 2]) : "f"(v[i + 1]), "f"(v[i]));
+    else
+      asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(w[i / 2]) : "f"(v[i + 1]), "f"(v[i]));
+  }
+  float o[V];
   widen<T, V>(first, o);
 #pragma unroll
-  for (int i = 0; i < V; ++i) v[i] -= o[i];
+  for (int i = 0; i < V; i += 2)
+    unpack2(sub2(pack2(v[i], v[i + 1]), pack2(o[i], o[i + 1])), v[i], v[i + 1]);
   return first;
 }
 

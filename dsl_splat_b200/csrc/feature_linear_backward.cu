@@ -289,7 +289,8 @@ FusedPlan plan_fused(long long rows, int k, int n, int activation) {
   const long long tiles = (rows + kTileRows - 1) / kTileRows;
   long long blocks = static_cast<long long>(host::sm_count()) * per_sm;
   if (sizeof(T) == 2) {
-    const long long most = kMostAdditions * 16 / kTileRows / (rounds_dz(activation) ? 2 : 1);
+    const bool two = rounds_dz(activation) && !(plan.copies && n <= 64);  // products a tile
+    const long long most = kMostAdditions * 16 / kTileRows / (two ? 2 : 1);
     blocks *= std::max(1LL, (tiles + blocks * most - 1) / (blocks * most));
   }
   plan.blocks = static_cast<int>(std::min(tiles, blocks));

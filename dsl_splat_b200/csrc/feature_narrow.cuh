@@ -11,7 +11,9 @@
 // and dx of tile t.  db is summed in registers from dz before its rounding.
 //
 // Bound by memory and by the latency of 16 compute warps to an SM: 64 -> 64 bf16
-// over 1600x1200 rows moves 737 MB in 152 us (112 us at the copy rate).
+// over 1600x1200 rows moves 737 MB in 139 us without an activation and in 198 with
+// SiLU (112 us at the copy rate).  There dW's second values take the tensor core's
+// idle lanes: as a product of their own 206 us.
 #pragma once
 #include "feature_product.cuh"
 
@@ -86,6 +88,31 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
   tc::fence_after_sync();
   const uint32_t tmem = tc::uniform(tmem_base);
   const uint32_t z_tmem = tmem, dx_tmem = z_tmem + p.n32, w_tmem = dx_tmem + p.k32;
+  // a compute warp's lanes of dW to this block's sums, or added to them
+  const auto store_dw = [&](bool add) {
+    const int lane_block = warp & 3, row = lane_block * 32 + lane - (add ? 64 : 0);
+    float* out = p.partial + static_cast<size_t>(blockIdx.x) * p.n * (p.k + 1);
+#pragma unroll
+    for (int cc = 0; cc < C; ++cc) {
+      const int c = (warp >> 2) + 2 * cc;
+      if (c * 32 >= p.k32) break;
+      float v[32];
+      tc::tmem_load32(w_tmem + (lane_block << 21) + c * 32, v);
+      if (row < p.n) {
+        float* to = out + row * p.k + c * 32;
+        if (add) {
+          float o[32];  // all reads before the first write
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = c * 32 + j < p.k ? to[j] : 0.0f;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += o[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (c * 32 + j < p.k) to[j] = v[j];
+      }
+    }
+  };
   const uint32_t count = (p.tiles - blockIdx.x + gridDim.x - 1) / gridDim.x;  // of this block
   bool ok = true;
 
@@ -118,8 +145,9 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
       const uint32_t z_instruction = tc::instruction(!kIsF16<T>, false, false, p.n32);
       const uint32_t dx_instruction = tc::instruction(!kIsF16<T>, false, true, p.k32);
       const uint32_t w_instruction = tc::instruction(!kIsF16<T>, true, true, p.k32);
-      // n of up to 64 take one block of dz twice; the upper lanes are not read
-      const uint32_t z_block = p.n > 64 ? kAPlane : 0;
+      // n of up to 64 leave lanes 64 and up to the second values (or, without them,
+      // to the first ones again, which are not read)
+      const uint32_t beside = p.n <= 64 && with_second;
       const auto form_z = [&](uint32_t i) {
         const uint32_t b = i & 1;
         if (!(ok = tc::barrier_wait(bar(full[b]), (i >> 1) & 1) && ok)) return;
@@ -140,11 +168,12 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
         if (i + 1 < count) form_z(i + 1);
         const uint32_t x_now = x_at + b * x_bytes, z_now = z_at + b * z_bytes;
         if (p.partial) {
+          const uint32_t z_block = p.n > 64 ? kAPlane : beside ? second_at - z_now : 0;
           tc::mma_steps(lead, w_tmem, tc::descriptor_mn_major(z_now, z_block),
                         tc::descriptor_mn_major(x_now, kAPlane), tc::kStepMn, tc::kStepMn,
                         kTileRows / 16, w_instruction, i > 0);
-          if (with_second)
-            tc::mma_steps(lead, w_tmem, tc::descriptor_mn_major(second_at, z_block),
+          if (with_second && !beside)
+            tc::mma_steps(lead, w_tmem, tc::descriptor_mn_major(second_at, kAPlane),
                           tc::descriptor_mn_major(x_now, kAPlane), tc::kStepMn, tc::kStepMn,
                           kTileRows / 16, w_instruction, true);
         }
@@ -301,21 +330,7 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
     if (p.partial) {
       ok = tc::barrier_wait(bar(all_done), 0) && ok;
       tc::fence_after_sync();
-      float* out = p.partial + static_cast<size_t>(blockIdx.x) * p.n * (p.k + 1);
-      if (lane_block * 32 < p.n) {
-#pragma unroll
-        for (int cc = 0; cc < C; ++cc) {
-          const int c = half + 2 * cc;
-          if (c * 32 >= p.k32) break;
-          float v[32];
-          tc::tmem_load32(w_tmem + (lane_block << 21) + c * 32, v);
-          if (row < p.n) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (c * 32 + j < p.k) out[row * p.k + c * 32 + j] = v[j];
-          }
-        }
-      }
+      if (lane_block * 32 < p.n) store_dw(false);
 #pragma unroll
       for (int cc = 0; cc < C; ++cc) {
         const int c = half + 2 * cc;
@@ -341,6 +356,12 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
   if (!ok) atomicCAS(p.error, 0, kDeviceTimeout);
   tc::fence_before_sync();
   __syncthreads();
+  if (p.partial && p.n <= 64 && with_second) {  // dW of the second values, in lanes 64 and up
+    tc::fence_after_sync();
+    if (warp < 8 && (warp & 3) >= 2 && ((warp & 3) - 2) * 32 < p.n) store_dw(true);
+    tc::fence_before_sync();
+    __syncthreads();
+  }
   if (p.partial && threadIdx.x < p.n) {
     float s = 0.0f;
     for (int q = 0; q < 4; ++q) {
