@@ -16,7 +16,7 @@
 // do not fit beside the operands, the steps read global memory.
 // 16-bit types with 16-byte rows take the pass of feature_narrow.cuh instead.
 // Bound by the steps' latencies one after another: 35 -> 32 fp32 gelu over 10^6
-// rows about 330 us where 408 MB take 62 us to copy.
+// rows 365 us where 408 MB take 62 us to copy.
 #pragma once
 #include "feature_product.cuh"
 
@@ -30,8 +30,8 @@ struct FusedParams {
   void* dx;        // (rows, k) or NULL
   float* partial;  // per block: (n, k) of dW, then (n) of db; NULL: neither
   int activation, x_vector, w_vector, dy_vector, dx_vector;
-  // x and dy are copied ahead (training of 35 -> 64 bf16 over 10^6 rows 222 us
-  // against 250 read as needed, 35 -> 32 fp32 450 against 490)
+  // x and dy are copied ahead (training of 35 -> 64 bf16 over 10^6 rows 254 us
+  // against 286 read as needed, 35 -> 32 fp32 468 against 534)
   int raw;
   uint32_t tiles, tmem_columns;
   int* error;
@@ -39,9 +39,9 @@ struct FusedParams {
 
 constexpr int kFusedThreads = 512, kFusedWarps = kFusedThreads / 32;
 // Widest k and n: what fits in shared memory there is faster in one pass
-// (training over 500000 rows against the products: 64 -> 64 bf16 147 us against
-// 197, 128 -> 128 bf16 175 against 309, 64 -> 64 fp32 275 against 460, 128 -> 64
-// fp32 637 against 636).
+// (silu training over 500000 rows against the products: 64 -> 64 bf16 118 us
+// against 192, 128 -> 128 bf16 202 against 337, 64 -> 64 fp32 297 against 462,
+// 128 -> 64 fp32 636 against 648).
 constexpr int kFusedWidth = 128;
 constexpr int kJoinBytes = 4 * kFusedWidth * 4;  // db of the four blocks of rows
 

@@ -52,7 +52,7 @@ template <class SA, int PA, bool AMN, class SB, int PB, bool BMN, class TE, clas
 int launch_product(ProductParams p, cudaStream_t s) {
   // a plain product's tiles are as wide as they can be; behind one with
   // arithmetic two blocks' epilogues share an SM (512 -> 512 fp16 gelu over
-  // 131072 rows 103 us against 107 in 256-wide tiles, 256 -> 256 bf16 silu 39
+  // 131072 rows 111 us against 119 in 256-wide tiles, 256 -> 256 bf16 silu 43
   // against 48)
   constexpr long long kMostSum = kMostAdditions * 16 / PA;  // of a 16-bit layer's accumulator
   // 16-bit results of more are added up in shared memory, a patch to a warp
@@ -79,8 +79,8 @@ int launch_product(ProductParams p, cudaStream_t s) {
   constexpr int kAcc = accumulators(PA, PB);
   // sums of several accumulators are joined in fp32 outputs
   p.k_per_sum = kAcc == 2 ? kExactSum : kMostSum;
-  // (35 -> 32 fp32 gelu over 10^6 rows 113 us against 154 without, 32 -> 3 bf16
-  // over 1.9 10^6 67 against 84, 64 -> 32 bf16 71 against 69)
+  // (35 -> 32 fp32 gelu over 10^6 rows 114 us against 187 without, 32 -> 3 bf16
+  // over 1.9 10^6 66 against 85, 64 -> 32 bf16 69 against 69)
   p.alternate = p.tile_n == 32 && p.k_per_sum >= p.k_per_split;
   p.accumulators = p.alternate ? 4 : 2;
   while (p.tmem_columns < static_cast<uint32_t>(p.accumulators * kAcc * p.tile_n))
@@ -126,8 +126,8 @@ int launch_product(ProductParams p, cudaStream_t s) {
                      BMN ? kChunk : p.tile_n);
   }
   // two tiles of A as they are in memory, where two stages fit beside them
-  // (35 -> 32 fp32 gelu over 10^6 rows 113 us against 140 read as needed,
-  // 35 -> 64 bf16 78 against 82)
+  // (35 -> 32 fp32 gelu over 10^6 rows 112 us against 152 read as needed,
+  // 35 -> 64 bf16 73 against 79)
   if (PA != 2 && !p.copy_operands && !AMN && p.tiles_n == 1 && p.a_ld == p.k &&
       host::aligned(p.a, 16)) {
     const long long raw = (kTileRows * p.k * static_cast<long long>(sizeof(SA)) + 127) / 128 * 128;
@@ -135,7 +135,7 @@ int launch_product(ProductParams p, cudaStream_t s) {
     if (fixed + 2 * stage + 2 * raw <= budget) p.raw_bytes = static_cast<int>(raw);
   }
   // blocks without register-filling producers are small enough for three
-  // (64 -> 64 bf16 with residual over 1.9 10^6 rows 121 us against 137 with two)
+  // (64 -> 64 bf16 with residual over 1.9 10^6 rows 129 us against 139 with two)
   if (p.copy_operands && blocks == 2 && 3 * p.tmem_columns <= 512 &&
       fixed + 2 * stage <= kThreeBlocksBytes)
     blocks = 3, budget = kThreeBlocksBytes;
@@ -208,9 +208,9 @@ Planes split(const void* src, long long rows, int cols, void* to, cudaStream_t s
 
 // Whether the wide layers' products take planes: fp32 operands, and rows that
 // are not whole 16-byte pieces.  The pass that makes them pays from about
-// kFewRows on: 300 -> 300 fp32 over 4000, 16000 and 100000 rows 34, 56 and
-// 250 us with planes, 26, 58 and 288 without; 301 -> 200 bf16 over 4000 and
-// 100000 rows 34 and 75 with, 23 and 117 without (trained: 282 against 725).
+// kFewRows on: 300 -> 300 fp32 over 4000, 16384 and 100000 rows 29, 55 and
+// 251 us with planes, 25, 57 and 289 without; 301 -> 200 bf16 over 4000 and
+// 100000 rows 23 and 73 with, 21 and 108 without (ReLU training: 275 against 717).
 template <class T>
 bool wants_planes(long long rows, int k, int n) {
   const int whole = 16 / static_cast<int>(sizeof(T));

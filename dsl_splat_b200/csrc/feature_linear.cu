@@ -22,8 +22,8 @@ int check_linear(int dtype, long long rows, int k, int n, int activation) {
 }
 
 // The forward takes planes where its x would be converted for several tiles
-// (n above 128) or its rows are long.  Over 200000 rows: 128 -> 128 fp32 60 us
-// without against 99 with, 101 -> 128 bf16 47 against 59, 255 -> 128 bf16 109
+// (n above 128) or its rows are long.  Over 200000 rows: 128 -> 128 fp32 69 us
+// without against 106 with, 101 -> 128 bf16 46 against 56, 255 -> 128 bf16 106
 // against 96.
 template <class T>
 bool forward_planes(long long rows, int k, int n) {

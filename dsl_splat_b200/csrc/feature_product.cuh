@@ -21,10 +21,12 @@
 // loaded once per block.
 //
 // Bound by memory and the epilogue's arithmetic where k and n are small (64 -> 64
-// bf16 with residual over 1600x1200 rows 121 us, 112 us of copying; 32 -> 64 silu
-// 96 us, of which two special-function instructions a value take 55), by how
-// fast operands reach shared memory where they are wide (300 -> 300 fp32 over
-// 200000 rows 400 us for 216 GFLOP of parts: the tensor pipe is busy 34 %).
+// bf16 silu with residual over 1600x1200 rows 132 us, 112 us of copying; 32 -> 64
+// silu 96 us, 56 us of copying and 55 of two special-function instructions a
+// value).  Wide fp32 layers (300 -> 300 over 200000 rows 401 us for 216 GFLOP of
+// parts, the tensor pipe busy 34 %) have a ring of one stage: three parts of 64 k
+// of both operands are 96 KB, beside which the epilogue's patches leave no room
+// for another, so that a stage's copies wait for its products.
 #pragma once
 #include <type_traits>
 

@@ -5,7 +5,7 @@ the per-Gaussian features that they blend from.
 * `linear`: act(x W^T + b) + residual over the last dimension;
 * `group_norm`: group norm with an activation over channel-last images;
 * `FeatureDecoder`: a run of them, called on an image, or passed to
-  gs3d.rasterize / rade.rasterize as `feature_decoder`.
+  gs3d.rasterize / rade.rasterize / aaa.rasterize as `feature_decoder`.
 
 Tensors are CUDA float32, bfloat16 or float16, all of one type per call (no
 autocast).  Sums are held in fp32 or more and rounded once to that type, and
