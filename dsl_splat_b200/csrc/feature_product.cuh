@@ -150,10 +150,16 @@ SPLAT_DEV Vec<S, 8> load8(const S* p, int valid) {
   return r;
 }
 
-// Part of two values as a packed pair, and what it leaves of them.
+// Part of two values as a packed pair, and what it leaves of them.  A part that
+// others follow is at most bf16's largest value, so that the last one brings an
+// infinity, which then meets the other operand's leading part alone.
+template <bool LAST>
 SPLAT_DEV uint32_t take_part(float& a, float& b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  const uint32_t u = reinterpret_cast<const uint32_t&>(h);
+  uint32_t u;
+  if constexpr (LAST)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(b), "f"(a));
+  else
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(b), "f"(a));
   a -= __uint_as_float(u << 16);
   b -= __uint_as_float(u & 0xffff0000u);
   return u;
@@ -169,7 +175,8 @@ SPLAT_DEV void to_parts(const Vec<S, 8>& v, uint4 (&out)[P]) {
     for (int j = 0; j < 4; ++j) {
       float a = to_float(v.v[2 * j]), b = to_float(v.v[2 * j + 1]);
 #pragma unroll
-      for (int p = 0; p < P; ++p) w[p][j] = take_part(a, b);
+      for (int p = 0; p < P; ++p)
+        w[p][j] = p == P - 1 ? take_part<true>(a, b) : take_part<false>(a, b);
     }
 #pragma unroll
     for (int p = 0; p < P; ++p) out[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);

@@ -13,9 +13,10 @@ no result depends on the order in which blocks run.  The backward of a 16-bit
 `linear` keeps dy act'(z) as two values of that type (2^-16 relative for
 bfloat16, 2^-22 for float16, whose smallest value is 2^-24: float16 losses want
 their usual scale).  Any strides are taken; what is not contiguous is copied
-first.  First-order reverse-mode gradients only; forward-mode ones and torch.func's
-transforms are refused.  In float32 the products of non-finite
-values are NaN where IEEE arithmetic would give an infinity.
+first.  First-order reverse-mode gradients only; forward-mode ones and
+torch.func's transforms are refused.  float32 operands are split into three parts
+of 8 digits, of which those below 2^-133 are lost (values below 2^-110 keep
+fewer than 24).
 
 A device-side wait that gives up (a defect, not a user's error) sets the
 library's error word, which the next binning, or _native.device_error, reads.

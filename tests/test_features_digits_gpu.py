@@ -365,3 +365,42 @@ def test_short_types_over_long_rows_of_two_parts():
     dx, = torch.autograd.grad(features.linear(x, w, activation="sigmoid"), x, dy)
     want = dy.double() @ w.double() / 4  # the slope at 0
     check(dx, want, (1024 + 16 + 16) * U * want, "dx")
+
+
+# ---- the ends of fp32's range ------------------------------------------------------
+
+@pytest.mark.parametrize("m, k, n", [(70, 35, 20), (200, 64, 64), (300, 300, 200),
+                                     (17000, 300, 140)])
+def test_largest_and_infinite_fp32_values(m, k, n):
+    """Values that round to more than bf16's largest are split like others, and
+    an infinity gives what IEEE arithmetic gives."""
+    normal = draws(48)
+    x, w = normal(m, k, dtype=torch.float32), normal(n, k, dtype=torch.float32)
+    dy = normal(m, n, dtype=torch.float32)
+    most = torch.finfo(torch.float32).max
+    w = w * 2.0 ** -12
+    x[3] = 0.0
+    x[3, 5] = most
+    x[4, 1] = float("inf")
+    x[5, 2] = -float("inf")
+    x[6, 3], x[6, 4] = float("inf"), -float("inf")
+    x.requires_grad_()
+    y = features.linear(x, w)
+    want = x.double() @ w.double().t()
+    fine = want.isfinite()
+    check(y[fine].detach(), want[fine].detach(),
+          (k + 8) * U * (x.detach().nan_to_num(0, 0, 0).double().abs() @ w.double().abs().t())[fine],
+          "y")
+    for row in (4, 5, 6):
+        assert torch.equal(y[row].isnan(), want[row].float().isnan())
+        assert torch.equal(y[row].nan_to_num(0.0), want[row].float().nan_to_num(0.0))
+    # dy: its products with w, and (by way of dW) with x
+    dy[3] = 0.0
+    dy[3, 7] = most
+    dy[9, 2] = float("inf")
+    dx, = torch.autograd.grad(y, x, dy)
+    want = dy.double() @ w.double()
+    fine = want.isfinite()
+    check(dx[fine], want[fine], (n + 8) * U * (dy.nan_to_num(0, 0, 0).double().abs()
+                                               @ w.double().abs())[fine], "dx")
+    assert torch.equal(dx[9], want[9].float())
