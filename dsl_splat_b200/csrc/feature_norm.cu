@@ -784,7 +784,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_backward_apply_kernel(con
 
 constexpr int kSmallThreads = 512;
 constexpr size_t kMostShared = 226 * 1024;
-constexpr int kSmallForward = 450000, kSmallBackward = 300000;  // values of a sample
+constexpr int kSmallForward = 450000, kSmallBackward = 600000;  // values of a sample
 constexpr int kFewSamples = 8;
 constexpr long long kManyBytes = 1792 * 1024;
 constexpr int kSmallChannels = 1024;
@@ -1131,7 +1131,9 @@ Plan make_plan(int value_bytes, int samples, long long positions, int channels, 
   // slower than the passes' many blocks (forward, 1 and 4 of 100x100x32 fp32 in 19
   // us each against 22 and 25 in passes, one of 130x130x32 25 against 22; 16 and 64
   // of 20x20x32 21 and 49 against 23 and 35, of 10x10x32 15 and 15 against 22 and
-  // 33; backward, one of 80x80x32 19 against 20, of 100x100x32 23 against 20)
+  // 33).  The backward, which waits for the host in a training step, takes more for
+  // its fewer launches (2 of 67x101x48 fp32 trained 125 us against 134, where the
+  // kernels alone take 25 and 22; one of 170x170x32 bf16 39 against 25)
   plan.small = plan.l.columns == 1 && channels <= kSmallChannels &&
                positions * channels <= (backward ? kSmallBackward : kSmallForward) &&
                (samples <= kFewSamples || samples * bytes <= kManyBytes);

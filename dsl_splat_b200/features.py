@@ -123,8 +123,7 @@ def _check_like(t: Tensor | None, x: Tensor, shape: tuple, name: str) -> None:
 def _check_forward_mode(*tensors: Tensor | None) -> None:
     """Refuses dual tensors: a result without a tangent would pass for a
     derivative of zero."""
-    if forward_ad._current_level >= 0 and any(
-            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError("forward-mode derivatives of the feature operators")
 
 
@@ -142,8 +141,8 @@ def _recorded(*tensors: Tensor | None) -> bool:
 
 
 def check_linear(x: Tensor, weight: Tensor, bias: Tensor | None, activation: str,
-                 **outputs: Tensor | None) -> None:
-    """Refuses what `linear` does not take; outputs: tensors of the result's shape."""
+                 output: Tensor | None, name: str) -> None:
+    """Refuses what `linear` does not take; output: of the result's shape."""
     _check_activation(activation)
     _check_input(x)
     if x.ndim < 1 or x.shape[-1] < 1:
@@ -154,8 +153,8 @@ def check_linear(x: Tensor, weight: Tensor, bias: Tensor | None, activation: str
     n = weight.shape[0]
     _check_like(weight, x, (n, k), "weight")
     _check_like(bias, x, (n,), "bias")
-    for name, t in outputs.items():
-        _check_like(t, x, x.shape[:-1] + (n,), name)
+    if output is not None:
+        _check_like(output, x, x.shape[:-1] + (n,), name)
     if k > 65535 or n > 65535:
         raise ValueError("at most 65535 input and output features")
 
@@ -167,8 +166,9 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *,
     x: (...,K), weight: (N,K), bias: (N,), residual and the result: (...,N).
     activation: "none", "relu", "silu", "gelu" (the erf form) or "sigmoid".
     """
-    check_linear(x, weight, bias, activation, residual=residual)
-    _check_forward_mode(x, weight, bias, residual)
+    check_linear(x, weight, bias, activation, residual, "residual")
+    if forward_ad._current_level >= 0:
+        _check_forward_mode(x, weight, bias, residual)
     if _traced():
         return torch.ops.splat200.feature_linear(x, weight, bias, residual, activation)
     if _recorded(x, weight, bias, residual):
@@ -213,7 +213,8 @@ def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tenso
     samples = math.prod(x.shape[:-1 - spatial_dims])
     positions = math.prod(x.shape[-1 - spatial_dims:-1])
     check_group_norm(x, groups, weight, bias, eps, activation, samples, positions)
-    _check_forward_mode(x, weight, bias)
+    if forward_ad._current_level >= 0:
+        _check_forward_mode(x, weight, bias)
     groups, eps = int(groups), float(eps)
     if _traced():
         shape = (samples, positions, x.shape[-1])

@@ -514,9 +514,9 @@ def _check_forward_mode():
         raise NotImplementedError("forward-mode derivatives of the feature operators")
 
 
-def _check_linear(x, weight, bias, activation, **outputs):
+def _check_linear(x, weight, bias, activation, output, name):
     _check_forward_mode()
-    features.check_linear(x, weight, bias, activation, **outputs)
+    features.check_linear(x, weight, bias, activation, output, name)
 
 
 def _check_norm(x, groups, weight, bias, eps, activation):
@@ -539,27 +539,27 @@ def _check_norm_backward(x, groups, weight, bias, moments, activation, upstream)
 @torch.library.custom_op(f"{_NS}::feature_linear", mutates_args=())
 def feature_linear(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None,
                    activation: str) -> Tensor:
-    _check_linear(x, weight, bias, activation, residual=residual)
+    _check_linear(x, weight, bias, activation, residual, "residual")
     return stages.feature_linear(x, weight, bias, residual, activation)
 
 
 @feature_linear.register_fake
 def _(x, weight, bias, residual, activation):
-    _check_linear(x, weight, bias, activation, residual=residual)
+    _check_linear(x, weight, bias, activation, residual, "residual")
     return x.new_empty(x.shape[:-1] + (weight.shape[0],))
 
 
 @torch.library.custom_op(f"{_NS}::feature_linear_backward", mutates_args=())
 def feature_linear_backward(x: Tensor, weight: Tensor, bias: Tensor | None, activation: str,
                             upstream: Tensor) -> tuple[Tensor, Tensor, Tensor]:
-    _check_linear(x, weight, bias, activation, upstream=upstream)
+    _check_linear(x, weight, bias, activation, upstream, "upstream")
     return stages.feature_linear_backward(x, weight, bias, activation, upstream,
                                           (True, True, True))
 
 
 @feature_linear_backward.register_fake
 def _(x, weight, bias, activation, upstream):
-    _check_linear(x, weight, bias, activation, upstream=upstream)
+    _check_linear(x, weight, bias, activation, upstream, "upstream")
     return x.new_empty(x.shape), weight.new_empty(weight.shape), x.new_empty((weight.shape[0],))
 
 
