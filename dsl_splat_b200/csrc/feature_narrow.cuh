@@ -11,7 +11,7 @@
 // and dx of tile t.  db is summed in registers from dz before its rounding.
 //
 // Bound by memory and by the latency of 16 compute warps to an SM: 64 -> 64 bf16
-// over 1600x1200 rows moves 737 MB in 139 us without an activation and in 198 with
+// over 1600x1200 rows moves 737 MB in 140 us without an activation and in 193 with
 // SiLU (112 us at the copy rate).  There dW's second values take the tensor core's
 // idle lanes: as a product of their own 206 us.
 #pragma once
@@ -88,31 +88,6 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
   tc::fence_after_sync();
   const uint32_t tmem = tc::uniform(tmem_base);
   const uint32_t z_tmem = tmem, dx_tmem = z_tmem + p.n32, w_tmem = dx_tmem + p.k32;
-  // a compute warp's lanes of dW to this block's sums, or added to them
-  const auto store_dw = [&](bool add) {
-    const int lane_block = warp & 3, row = lane_block * 32 + lane - (add ? 64 : 0);
-    float* out = p.partial + static_cast<size_t>(blockIdx.x) * p.n * (p.k + 1);
-#pragma unroll
-    for (int cc = 0; cc < C; ++cc) {
-      const int c = (warp >> 2) + 2 * cc;
-      if (c * 32 >= p.k32) break;
-      float v[32];
-      tc::tmem_load32(w_tmem + (lane_block << 21) + c * 32, v);
-      if (row < p.n) {
-        float* to = out + row * p.k + c * 32;
-        if (add) {
-          float o[32];  // all reads before the first write
-#pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = c * 32 + j < p.k ? to[j] : 0.0f;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] += o[j];
-        }
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (c * 32 + j < p.k) to[j] = v[j];
-      }
-    }
-  };
   const uint32_t count = (p.tiles - blockIdx.x + gridDim.x - 1) / gridDim.x;  // of this block
   bool ok = true;
 
@@ -330,7 +305,48 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
     if (p.partial) {
       ok = tc::barrier_wait(bar(all_done), 0) && ok;
       tc::fence_after_sync();
-      if (lane_block * 32 < p.n) store_dw(false);
+      float* out = p.partial + static_cast<size_t>(blockIdx.x) * p.n * (p.k + 1);
+      // dW of the second values in lanes 64 and up goes by way of x's buffers
+      const bool beside = with_second && p.n <= 64;
+      const uint32_t half_at = x_at + (row & 63) * 4;
+      const auto each_chunk = [&](auto use) {
+#pragma unroll
+        for (int cc = 0; cc < C; ++cc) {
+          const int c = half + 2 * cc;
+          if (c * 32 >= p.k32) break;
+          float v[32];
+          tc::tmem_load32(w_tmem + (lane_block << 21) + c * 32, v);
+          use(c, v);
+        }
+      };
+      const bool upper = beside && lane_block >= 2;
+      if (upper)
+        each_chunk([&](int c, const float (&v)[32]) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(half_at + (c * 32 + j) * 256), "f"(v[j])
+                         : "memory");
+        });
+      if (beside) asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (!upper && lane_block * 32 < p.n)
+        each_chunk([&](int c, float (&v)[32]) {
+          if (beside) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              float second;
+              asm volatile("ld.shared.f32 %0, [%1];"
+                           : "=f"(second)
+                           : "r"(half_at + (c * 32 + j) * 256)
+                           : "memory");
+              v[j] += second;
+            }
+          }
+          if (row < p.n) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c * 32 + j < p.k) out[row * p.k + c * 32 + j] = v[j];
+          }
+        });
 #pragma unroll
       for (int cc = 0; cc < C; ++cc) {
         const int c = half + 2 * cc;
@@ -356,12 +372,6 @@ __global__ void __launch_bounds__(kNarrowThreads, WIDE ? 1 : 2)
   if (!ok) atomicCAS(p.error, 0, kDeviceTimeout);
   tc::fence_before_sync();
   __syncthreads();
-  if (p.partial && p.n <= 64 && with_second) {  // dW of the second values, in lanes 64 and up
-    tc::fence_after_sync();
-    if (warp < 8 && (warp & 3) >= 2 && ((warp & 3) - 2) * 32 < p.n) store_dw(true);
-    tc::fence_before_sync();
-    __syncthreads();
-  }
   if (p.partial && threadIdx.x < p.n) {
     float s = 0.0f;
     for (int q = 0; q < 4; ++q) {
