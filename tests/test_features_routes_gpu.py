@@ -1,5 +1,5 @@
-"""Feature operators on the GPU in recorded programs: torch.compile, torch.jit.trace
-and make_fx hold them and give what the calls themselves give."""
+"""Feature operators on the GPU in recorded programs: torch.compile, torch.jit.trace,
+make_fx and CUDA graphs hold them and give what the calls themselves give."""
 
 import pytest
 import torch
@@ -56,3 +56,40 @@ def test_under_torch_func():
                 lambda: torch.func.vmap(lambda v: features.group_norm(v, 5))(x)):
         with pytest.raises((RuntimeError, NotImplementedError)):
             run()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m, k, n, act", [(700, 512, 264, "gelu"), (700, 301, 200, "silu"),
+                                          (17000, 301, 33, "sigmoid"), (900, 64, 48, "silu"),
+                                          (40, 20001, 9, "silu"), (900, 35, 48, "relu")])
+def test_captured_layers(m, k, n, act, dtype):
+    """One training step of a layer, captured and replayed on other inputs
+    beside an eager one on another stream."""
+    normal = draws(52)
+    w, b, dy = (normal(*s, dtype=dtype) for s in ((n, k), (n,), (m, n)))
+    inputs = [normal(m, k, dtype=dtype) for _ in range(3)]
+
+    def step(x):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        y = features.linear(*leaves, activation=act)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    want = [[t.clone() for t in step(x)] for x in inputs]
+    static = inputs[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for i, x in enumerate(inputs):
+        static.copy_(x)
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            beside = step(inputs[i - 1])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(out, want[i]))
+        assert all(torch.equal(a, c) for a, c in zip(beside, want[i - 1]))
