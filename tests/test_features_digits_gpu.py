@@ -404,3 +404,16 @@ def test_largest_and_infinite_fp32_values(m, k, n):
     check(dx[fine], want[fine], (n + 8) * U * (dy.nan_to_num(0, 0, 0).double().abs()
                                                @ w.double().abs())[fine], "dx")
     assert torch.equal(dx[9], want[9].float())
+
+
+def test_training_over_more_rows_than_an_int():
+    """2^31 + 2^20 rows of one value, in many more blocks than are resident: sums
+    of powers of two are exact until they are rounded."""
+    rows = (1 << 31) + (1 << 20)
+    x = torch.ones(rows, 1, device="cuda", dtype=torch.bfloat16)
+    w = torch.zeros(1, 1, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    b = torch.zeros(1, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    y = features.linear(x, w, b, activation="sigmoid")
+    dw, db = torch.autograd.grad(y, (w, b), torch.full_like(y, 2.0 ** -20))
+    want = torch.tensor(rows * 2.0 ** -22, dtype=torch.float64).to(torch.bfloat16)
+    assert float(dw) == float(want) and float(db) == float(want)
