@@ -6,7 +6,8 @@ AAA-Gaussians rasterisers.
 dsl_splat's signatures; the compute path
 is libsplat200.so (hand-written CUDA for sm_100a) reached through the C ABI
 in include/splat200.h.  `dsl_splat_b200.features` holds the operators that
-decode the feature images which they render.
+decode the feature images which they render and train with them,
+`dsl_splat_b200.optim` the optimizer.
 """
 
 from .cameras import PinholeCamera
@@ -14,8 +15,9 @@ from .statistics import MaskedContributionCount, WeightedContributionSum
 from . import aaa
 from . import features
 from . import gs3d
+from . import optim
 from . import rade
 from . import torch_ops  # registers torch.ops.splat200.*
 
-__all__ = ["aaa", "features", "gs3d", "rade", "torch_ops", "PinholeCamera",
+__all__ = ["aaa", "features", "gs3d", "optim", "rade", "torch_ops", "PinholeCamera",
            "MaskedContributionCount", "WeightedContributionSum"]

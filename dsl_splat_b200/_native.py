@@ -21,6 +21,7 @@ _F = ctypes.c_float
 _Z = ctypes.c_size_t
 _L = ctypes.c_longlong
 _U = ctypes.c_uint
+_D = ctypes.c_double
 
 # name -> (restype, argtypes)
 SIGNATURES: dict[str, tuple] = {
@@ -104,6 +105,16 @@ SIGNATURES: dict[str, tuple] = {
     "splat_feature_norm": (_I, [_I, _I, _L, _I, _I, _P, _P, _P, _F, _I, _P, _P, _P, _P, _Z, _P]),
     "splat_feature_norm_backward": (_I, [_I, _I, _L, _I, _I, _P, _P, _P, _P, _P, _I, _P, _P, _P,
                                          _P, _P, _Z, _P]),
+    "splat_feature_layer_norm": (_I, [_I, _L, _I, _P, _P, _P, _F, _I, _P, _P]),
+    "splat_feature_layer_norm_backward_workspace_bytes": (_Z, [_I, _L, _I]),
+    "splat_feature_layer_norm_backward": (_I, [_I, _L, _I, _P, _P, _P, _F, _I, _P, _P, _P, _P,
+                                               _P, _Z, _P]),
+    "splat_feature_embedding": (_I, [_I, _I, _L, _I, _I, _P, _P, _F, _P, _P]),
+    "splat_feature_embedding_backward_workspace_bytes": (_Z, [_I, _L, _I, _I]),
+    "splat_feature_embedding_backward": (_I, [_I, _I, _L, _I, _I, _P, _P, _F, _P, _P, _Z, _P]),
+    "splat_adamw": (_I, [_I, _I, _I, _P, _I, _P]),
+    "splat_adamw_decode": (_I, [_L, _P, _P, _I, _P, _P]),
+    "splat_adamw_encode": (_I, [_L, _P, _I, _P, _P, _P]),
 }
 
 
@@ -120,6 +131,15 @@ class SplatAaaFrame(ctypes.Structure):
                 ("sort_order", _I), ("ewa", _I), ("new_aabb", _I), ("near_clipping", _I),
                 ("tile_culling", _I), ("complete", _I), ("cooperative", _I),
                 ("normalize_quats", _I)]
+
+
+class SplatAdamwTensor(ctypes.Structure):
+    """include/splat200.h SplatAdamwTensor: one tensor of an AdamW step."""
+
+    _fields_ = [("p", _P), ("g", _P), ("m", _P), ("v", _P), ("m_exponents", _P),
+                ("v_exponents", _P), ("device_step", _P), ("device_lr", _P), ("n", _L),
+                ("step", _L), ("lr", _D), ("weight_decay", _D), ("beta1", _D), ("beta2", _D),
+                ("eps", _D)]
 
 
 def _load() -> ctypes.CDLL:

@@ -36,12 +36,15 @@ SOURCES = {"splat200.cu": ["-fmad=false"],
            "aaa_backward.cu": ["-fmad=true", "-prec-div=false", "-prec-sqrt=false"],
            "feature_linear.cu": ["-fmad=true"],
            "feature_linear_backward.cu": ["-fmad=true"],
-           "feature_norm.cu": ["-fmad=true"]}
+           "feature_norm.cu": ["-fmad=true"],
+           "feature_layer_norm.cu": ["-fmad=true"],
+           "feature_embedding.cu": ["-fmad=true"],
+           "adamw.cu": ["-fmad=true"]}
 HEADERS = ["splat_common.cuh", "cameras.cuh", "project.cuh", "binning.cuh", "render.cuh",
            "footprint.cuh", "tile_modes.cuh", "host_runtime.h", "rade.cuh", "rade_project.cuh",
            "aaa.cuh", "aaa_render.cuh", "aaa_api.cuh", "aaa_blend_params.cuh",
            "aaa_backward.cuh", "feature_common.cuh", "feature_product.cuh", "feature_fused.cuh",
-           "feature_launch.cuh", "feature_narrow.cuh", "tensor_core.cuh"]
+           "feature_launch.cuh", "feature_narrow.cuh", "feature_join.cuh", "tensor_core.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -4,6 +4,9 @@ the per-Gaussian features that they blend from.
 
 * `linear`: act(x W^T + b) + residual over the last dimension;
 * `group_norm`: group norm with an activation over channel-last images;
+* `layer_norm`: layer norm with an activation over the last dimension;
+* `embedding`: rows of a table by their ids, such as a codebook that Gaussians
+  share or a code for each view;
 * `FeatureDecoder`: a run of them, called on an image, or passed to
   gs3d.rasterize / rade.rasterize / aaa.rasterize as `feature_decoder`.
 
@@ -99,6 +102,42 @@ class _GroupNorm(torch.autograd.Function):
             x, samples, groups, weight, bias, moments, activation, upstream,
             ctx.needs_input_grad[:3])
         return dx, dweight, dbias, None, None, None, None
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float,
+                activation: str) -> Tensor:
+        ctx.save_for_backward(x, weight, bias)
+        ctx.settings = eps, activation
+        ctx.set_materialize_grads(False)
+        return stages.feature_layer_norm(x, weight, bias, eps, activation)
+
+    @staticmethod
+    @_once
+    def backward(ctx: Any, upstream: Tensor | None):
+        if upstream is None:
+            return (None,) * 5
+        dx, dweight, dbias = stages.feature_layer_norm_backward(
+            *ctx.saved_tensors, *ctx.settings, upstream, ctx.needs_input_grad[:3])
+        return dx, dweight, dbias, None, None
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, ids: Tensor, table: Tensor, scale: float) -> Tensor:
+        ctx.save_for_backward(ids)
+        ctx.settings = table.shape[0], scale
+        ctx.set_materialize_grads(False)
+        return stages.feature_embedding(ids, table, scale)
+
+    @staticmethod
+    @_once
+    def backward(ctx: Any, upstream: Tensor | None):
+        if upstream is None:
+            return None, None, None
+        ids, = ctx.saved_tensors
+        return None, stages.feature_embedding_backward(ids, *ctx.settings, upstream), None
 
 
 def _check_activation(activation: str) -> None:
@@ -225,6 +264,77 @@ def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tenso
     return stages.feature_norm(x, samples, groups, weight, bias, eps, activation, False)[0]
 
 
+def check_layer_norm(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float,
+                     activation: str) -> None:
+    """Refuses what `layer_norm` does not take."""
+    _check_activation(activation)
+    _check_input(x)
+    if x.ndim < 1 or x.shape[-1] < 1:
+        raise ValueError("x must have a last dimension of at least one channel")
+    channels = x.shape[-1]
+    _check_like(weight, x, (channels,), "weight")
+    _check_like(bias, x, (channels,), "bias")
+    if not 2.0 ** -126 <= eps < 2.0 ** 128:  # the kernels take it in fp32
+        raise ValueError("eps must be finite and positive in float32's normal range")
+    if channels > 65535:
+        raise ValueError("at most 65535 channels")
+
+
+def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, *,
+               eps: float = 1e-5, activation: str = "none") -> Tensor:
+    """act((x - mean) / sqrt(var + eps) * weight + bias) over the last dimension.
+
+    Mean and biased variance are those of the last dimension of x (...,C); weight
+    and bias: (C,).  activation as in `linear`.
+    """
+    check_layer_norm(x, weight, bias, eps, activation)
+    if forward_ad._current_level >= 0:
+        _check_forward_mode(x, weight, bias)
+    eps = float(eps)
+    if _traced():
+        return torch.ops.splat200.feature_layer_norm(x, weight, bias, eps, activation)
+    if _recorded(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, eps, activation)
+    return stages.feature_layer_norm(x, weight, bias, eps, activation)
+
+
+def check_embedding(ids: Tensor, entries: int, channels: int, scale: float,
+                    values: Tensor) -> None:
+    """Refuses what `embedding` does not take; values: the table, or its rows' upstream."""
+    if (not isinstance(values, Tensor) or not values.is_cuda
+            or values.dtype not in stages.FEATURE_DTYPES):
+        raise ValueError("table must be a CUDA float32, bfloat16 or float16 tensor")
+    if entries < 1 or channels < 1:
+        raise ValueError("table must be (V,C) with V and C of at least one")
+    if not isinstance(ids, Tensor) or ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError("ids must be an int32 or int64 tensor")
+    if ids.device != values.device:
+        raise ValueError("ids must be on the table's device")
+    if not abs(scale) < 2.0 ** 128:  # the kernels take it in fp32
+        raise ValueError("scale must be finite in float32")
+    if channels > 65535 or entries > 1 << 30 or ids.numel() > 1 << 30:
+        raise ValueError("at most 65535 channels, 2^30 entries and 2^30 ids")
+
+
+def embedding(ids: Tensor, table: Tensor, *, scale: float = 1.0) -> Tensor:
+    """scale * table[ids]: the rows of a table (V,C) by ids of any shape.
+
+    ids: int32 or int64 in [0,V).  An id outside gives zeros, takes no part in the
+    gradient and sets the library's error word.
+    """
+    if not isinstance(table, Tensor) or table.ndim != 2:
+        raise ValueError("table must be (V,C) with V and C of at least one")
+    check_embedding(ids, table.shape[0], table.shape[1], scale, table)
+    if forward_ad._current_level >= 0:
+        _check_forward_mode(table)
+    scale = float(scale)
+    if _traced():
+        return torch.ops.splat200.feature_embedding(ids, table, scale)
+    if _recorded(table):
+        return _Embedding.apply(ids, table, scale)
+    return stages.feature_embedding(ids, table, scale)
+
+
 @dataclass(slots=True)
 class Linear:
     """One `linear` of a FeatureDecoder; residual=True adds the layer's own input."""
@@ -254,6 +364,19 @@ class GroupNorm:
                           activation=self.activation)
 
 
+@dataclass(slots=True)
+class LayerNorm:
+    """One `layer_norm` of a FeatureDecoder."""
+
+    weight: Tensor | None = None
+    bias: Tensor | None = None
+    eps: float = 1e-5
+    activation: str = "none"
+
+    def __call__(self, x: Tensor) -> Tensor:
+        return layer_norm(x, self.weight, self.bias, eps=self.eps, activation=self.activation)
+
+
 class FeatureDecoder:
     """Layers called one after another on a channel-last image (...,H,W,C).
 
@@ -261,9 +384,9 @@ class FeatureDecoder:
     converted to it once, at the start.
     """
 
-    def __init__(self, *layers: Linear | GroupNorm):
-        if not layers or not all(isinstance(v, (Linear, GroupNorm)) for v in layers):
-            raise ValueError("FeatureDecoder takes Linear and GroupNorm layers")
+    def __init__(self, *layers: Linear | GroupNorm | LayerNorm):
+        if not layers or not all(isinstance(v, (Linear, GroupNorm, LayerNorm)) for v in layers):
+            raise ValueError("FeatureDecoder takes Linear and GroupNorm layers, and LayerNorm")
         self.layers = layers
 
     def parameters(self) -> Iterator[Tensor]:

@@ -1,0 +1,338 @@
+"""AdamW over many tensors at once, such as a scene's Gaussians and a feature
+decoder's layers.
+
+    m' = b1 m + (1 - b1) g,  v' = b2 v + (1 - b2) g^2
+    p' = p (1 - lr wd) - lr / (1 - b1^t) m' / (sqrt(v' / (1 - b2^t)) + eps)
+
+* `adamw`: one step in place, one launch for all tensors of a device and dtype;
+* `AdamW`: the torch.optim.Optimizer that calls it;
+* `Moment8`: a moment held in 8 bits.
+
+Parameters are contiguous CUDA float32, bfloat16 or float16 tensors, their gradients of
+the same type.  Both moments are float32, or 8-bit codes with an exponent for each 256
+values of the flattened tensor: m as a sign, 4 bits of exponent and 3 of mantissa, v as
+its root with 4 and 4, both relative to the run's exponent.  Each step rounds them
+down after a dither that is a hash of the value's place and the step: off by less than
+a step of the code and right on average, so that averages which move by less than that
+are followed; the update itself takes the values before their rounding.  A run that
+holds an infinity or a NaN reads as NaN.
+
+The reference has no counterpart; its users bring their own optimizer.
+"""
+
+from __future__ import annotations
+
+import math
+from numbers import Integral, Real
+from typing import Any, Callable, Iterable, Sequence
+
+import torch
+from torch import Tensor
+
+from . import stages
+from ._native import SplatAdamwTensor
+
+RUN = 256  # values that share an exponent
+
+
+class Moment8:
+    """A moment held in 8 bits: codes of the parameter's shape and exponents, one for each
+    256 values.  squared: of the second moment, whose root the codes hold."""
+
+    __slots__ = ("codes", "exponents", "squared")
+
+    def __init__(self, codes: Tensor, exponents: Tensor, squared: bool = False):
+        if codes.dtype is not torch.uint8 or exponents.dtype is not torch.int8:
+            raise ValueError("codes must be uint8 and exponents int8")
+        if not codes.is_contiguous() or not exponents.is_contiguous():
+            raise ValueError("codes and exponents must be contiguous")
+        if exponents.shape != (-(-codes.numel() // RUN),) or exponents.device != codes.device:
+            raise ValueError("exponents must have one value for each 256 codes, on their device")
+        self.codes, self.exponents, self.squared = codes, exponents, squared
+
+    @classmethod
+    def of(cls, values: Tensor, squared: bool = False) -> Moment8:
+        """The nearest codes of float32 moments."""
+        if not values.is_cuda or values.dtype is not torch.float32:
+            raise ValueError("values must be a CUDA float32 tensor")
+        return cls(*stages.adamw_encode(values, squared), squared)
+
+    @classmethod
+    def zeros_like(cls, parameter: Tensor, squared: bool = False) -> Moment8:
+        codes = torch.zeros(parameter.shape, dtype=torch.uint8, device=parameter.device)
+        exponents = torch.full((-(-codes.numel() // RUN),), -126, dtype=torch.int8,
+                               device=parameter.device)
+        return cls(codes, exponents, squared)
+
+    def values(self) -> Tensor:
+        """The float32 moments that the codes stand for."""
+        if not self.codes.is_cuda:
+            raise ValueError("codes must be a CUDA tensor")
+        return stages.adamw_decode(self.codes, self.exponents, self.squared)
+
+
+def _check_settings(betas: tuple[float, float], eps: float, weight_decay: float) -> None:
+    if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
+        raise ValueError("betas must be two numbers of at least 0 and below 1")
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError("eps must be finite and not negative")
+    if not (weight_decay >= 0.0 and math.isfinite(weight_decay)):
+        raise ValueError("weight_decay must be finite and not negative")
+
+
+def _check_lr(lr: Any) -> None:
+    if isinstance(lr, Tensor):
+        if lr.numel() != 1 or not lr.is_cuda or lr.dtype is not torch.float32:
+            raise ValueError("lr must be a number or a CUDA float32 tensor of one value")
+    elif not isinstance(lr, Real) or not (lr >= 0.0 and math.isfinite(lr)):
+        raise ValueError("lr must be finite and not negative")
+
+
+def _check_step(step: Any) -> None:
+    if isinstance(step, Tensor):
+        if step.numel() != 1 or not step.is_cuda or step.dtype is not torch.int64:
+            raise ValueError("step must be an integer or a CUDA int64 tensor of one value")
+    elif isinstance(step, bool) or not isinstance(step, Integral) or step < 1:
+        raise ValueError("step must be an integer of at least one")
+
+
+def _check_parameter(p: Tensor) -> None:
+    if not isinstance(p, Tensor) or not p.is_cuda or p.dtype not in stages.FEATURE_DTYPES:
+        raise ValueError("parameters must be CUDA float32, bfloat16 or float16 tensors")
+    if not p.is_contiguous():
+        raise ValueError("parameters must be contiguous")
+
+
+def _check_moment(m: Any, p: Tensor, squared: bool) -> int:
+    if isinstance(m, Moment8):
+        if m.codes.shape != p.shape or m.codes.device != p.device or m.squared != squared:
+            raise ValueError("8-bit moments must have their parameter's shape and device, and "
+                             "the second ones be squared")
+        return 8
+    if (not isinstance(m, Tensor) or m.dtype is not torch.float32 or m.shape != p.shape
+            or m.device != p.device or not m.is_contiguous()):
+        raise ValueError("moments must be contiguous float32 tensors, or Moment8, of their "
+                         "parameter's shape and device")
+    return 32
+
+
+def _each(value: Any, count: int, name: str) -> Sequence:
+    if isinstance(value, (list, tuple)):
+        if len(value) != count:
+            raise ValueError(f"{name} must be one value, or one for each parameter")
+        return value
+    return (value,) * count
+
+
+class _Launches:
+    """The launches of a step, made after all of its arguments have been checked."""
+
+    def __init__(self) -> None:
+        self.records: dict[tuple, list] = {}
+        self.written: list[Tensor] = []
+        self.held: list[Tensor] = []  # until the launches
+        self.places: set[int] = set()
+
+    def add(self, p: Tensor, g: Tensor, m: Tensor | Moment8, v: Tensor | Moment8,
+            step: int | Tensor, lr: float | Tensor, decay: float, betas: tuple[float, float],
+            eps: float, maximize: bool) -> None:
+        """A parameter, whose numbers have been checked."""
+        _check_parameter(p)
+        if not isinstance(g, Tensor) or g.layout is not torch.strided:
+            raise ValueError("gradients must be dense tensors")
+        if g.dtype is not p.dtype or g.device != p.device or g.shape != p.shape:
+            raise ValueError("gradients must have their parameter's dtype, device and shape")
+        bits = _check_moment(m, p, False)
+        if _check_moment(v, p, True) != bits:
+            raise ValueError("both moments must be held in the same number of bits")
+        for t in (step, lr):
+            if isinstance(t, Tensor) and t.device != p.device:
+                raise ValueError("step and lr tensors must be on their parameter's device")
+        n = p.numel()
+        if not n:
+            return
+        if not g.is_contiguous():
+            g = g.contiguous()
+            self.held.append(g)
+        address = p.data_ptr()
+        if address in self.places:
+            raise ValueError("a parameter is listed twice")
+        self.places.add(address)
+        device_step = step.data_ptr() if isinstance(step, Tensor) else None
+        device_lr = lr.data_ptr() if isinstance(lr, Tensor) else None
+        rest = (device_step, device_lr, n, 0 if device_step else step, 0.0 if device_lr else lr,
+                decay, betas[0], betas[1], eps)
+        if bits == 8:
+            record = SplatAdamwTensor(address, g.data_ptr(), m.codes.data_ptr(),
+                                      v.codes.data_ptr(), m.exponents.data_ptr(),
+                                      v.exponents.data_ptr(), *rest)
+            self.written += (p, m.codes, v.codes, m.exponents, v.exponents)
+        else:
+            record = SplatAdamwTensor(address, g.data_ptr(), m.data_ptr(), v.data_ptr(), None,
+                                      None, *rest)
+            self.written += (p, m, v)
+        self.records.setdefault((p.device, p.dtype, bits, maximize), []).append(record)
+
+    def run(self) -> None:
+        for (device, dtype, bits, maximize), records in self.records.items():
+            stages.adamw(device, dtype, bits, records, maximize)
+        if self.written:
+            torch.autograd.graph.increment_version(self.written)
+
+
+@torch.no_grad()
+def adamw(params: Sequence[Tensor], grads: Sequence[Tensor],
+          exp_avgs: Sequence[Tensor | Moment8], exp_avg_sqs: Sequence[Tensor | Moment8], *,
+          step: int | Tensor | Sequence, lr: float | Tensor | Sequence,
+          betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+          weight_decay: float | Sequence[float] = 1e-2, maximize: bool = False) -> None:
+    """One AdamW step of all params in place, their moments with them.
+
+    step counts from 1 and is the number of this step.  step, lr and weight_decay are
+    one value or a list with one for each parameter; step may be a CUDA int64 and lr a CUDA
+    float32 tensor of one value, which the kernel reads (a captured step then follows
+    them).  A parameter must not be listed twice."""
+    count = len(params)
+    if not len(grads) == len(exp_avgs) == len(exp_avg_sqs) == count:
+        raise ValueError("params, grads, exp_avgs and exp_avg_sqs must have the same length")
+    steps, lrs = _each(step, count, "step"), _each(lr, count, "lr")
+    decays = _each(weight_decay, count, "weight_decay")
+    for s in steps if isinstance(step, (list, tuple)) else (step,):
+        _check_step(s)
+    for v in lrs if isinstance(lr, (list, tuple)) else (lr,):
+        _check_lr(v)
+    for w in decays if isinstance(weight_decay, (list, tuple)) else (weight_decay,):
+        _check_settings(betas, eps, w)
+    launches = _Launches()
+    for p, g, m, v, s, r, w in zip(params, grads, exp_avgs, exp_avg_sqs, steps, lrs, decays):
+        launches.add(p, g, m, v, s, r, w, betas, eps, maximize)
+    launches.run()
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW with one launch for all parameters of a device and dtype.
+
+    state_bits: 32 or 8.  The state of a parameter holds "step", "exp_avg" and "exp_avg_sq"
+    (with 8 bits the codes, and their "exp_avg_exponents" and "exp_avg_sq_exponents");
+    `moments` and `set_moments` take the values they stand for, whatever the bits,
+    which is what code that adds or removes Gaussians has to carry over.
+    capturable: steps are counted on the device, so that a captured step() can be
+    replayed (lr may then be a CUDA float32 tensor)."""
+
+    def __init__(self, params: Iterable, lr: float | Tensor = 1e-3,
+                 betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, *, state_bits: int = 32, maximize: bool = False,
+                 capturable: bool = False):
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                                      state_bits=state_bits, maximize=maximize,
+                                      capturable=capturable))
+
+    def add_param_group(self, param_group: dict) -> None:
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
+            _check_lr(group["lr"])
+            _check_settings(group["betas"], group["eps"], group["weight_decay"])
+            if group["state_bits"] not in (8, 32):
+                raise ValueError("state_bits must be 8 or 32")
+            for p in group["params"]:
+                _check_parameter(p)
+        except ValueError:
+            self.param_groups.pop()
+            raise
+
+    def _state(self, p: Tensor, group: dict) -> dict:
+        state = self.state[p]
+        if not state:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW makes a parameter's state in its first step, which "
+                                   "must run before a step is captured")
+            state["step"] = (torch.zeros((), dtype=torch.int64, device=p.device)
+                             if group["capturable"] else 0)
+            if group["state_bits"] == 8:
+                self._put(state, Moment8.zeros_like(p), Moment8.zeros_like(p, squared=True))
+            else:
+                self._put(state, torch.zeros_like(p, dtype=torch.float32),
+                          torch.zeros_like(p, dtype=torch.float32))
+        return state
+
+    @staticmethod
+    def _put(state: dict, m: Tensor | Moment8, v: Tensor | Moment8) -> None:
+        for name, moment in (("exp_avg", m), ("exp_avg_sq", v)):
+            if isinstance(moment, Moment8):
+                state[name], state[name + "_exponents"] = moment.codes, moment.exponents
+            else:
+                state[name] = moment
+
+    @staticmethod
+    def _get(state: dict) -> tuple:
+        if "exp_avg_exponents" not in state:
+            return state["exp_avg"], state["exp_avg_sq"]
+        return (Moment8(state["exp_avg"], state["exp_avg_exponents"]),
+                Moment8(state["exp_avg_sq"], state["exp_avg_sq_exponents"], True))
+
+    @torch.no_grad()
+    def step(self, closure: Callable | None = None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        capturing = torch.cuda.is_current_stream_capturing()
+        launches = _Launches()
+        counters, counted = [], []
+        for group in self.param_groups:
+            if capturing and not group["capturable"]:
+                raise RuntimeError("a step is captured only of an AdamW with capturable=True")
+            _check_lr(group["lr"])
+            settings = (group["lr"], group["weight_decay"], group["betas"], group["eps"],
+                        group["maximize"])
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                state = self._state(p, group)
+                step = state["step"]
+                if isinstance(step, Tensor):
+                    counters.append(step)
+                else:
+                    counted.append(state)
+                    step += 1
+                launches.add(p, p.grad, *self._get(state), step, *settings)
+        if counters:
+            torch._foreach_add_(counters, 1)
+        launches.run()
+        for state in counted:
+            state["step"] += 1
+        return loss
+
+    def moments(self, p: Tensor) -> tuple[Tensor, Tensor]:
+        """A parameter's moments as float32 (of 32 bits the state's own tensors)."""
+        if not self.state.get(p):
+            raise KeyError("the parameter has no state yet")
+        m, v = self._get(self.state[p])
+        return (m.values(), v.values()) if isinstance(m, Moment8) else (m, v)
+
+    @torch.no_grad()
+    def set_moments(self, p: Tensor, m: Tensor, v: Tensor) -> None:
+        """Replaces a parameter's moments by float32 ones of its shape; its step stays."""
+        group = next((g for g in self.param_groups if any(q is p for q in g["params"])), None)
+        if group is None:
+            raise KeyError("not a parameter of this optimizer")
+        for t in (m, v):
+            _check_moment(t, p, False)
+        state = self._state(p, group)
+        if group["state_bits"] == 8:
+            self._put(state, Moment8.of(m), Moment8.of(v, squared=True))
+        else:
+            self._put(state, m.clone(), v.clone())
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict: dict) -> None:
+        super().load_state_dict(state_dict)
+        # torch casts a state to its parameter's dtype; moments keep theirs
+        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
+        own = [p for group in self.param_groups for p in group["params"]]
+        for i, p in zip(saved, own):
+            if i in state_dict["state"]:
+                self.state[p] = {
+                    name: v.to(p.device, copy=True).contiguous() if isinstance(v, Tensor) else v
+                    for name, v in state_dict["state"][i].items()}

@@ -806,3 +806,102 @@ def feature_norm_backward(x: Tensor, samples: int, groups: int, weight: Tensor |
               mean + 4 * samples * groups, _ACTIVATION_CODES[activation], upstream.data_ptr(),
               _address(dx), _address(dweight), _address(dbias), ws.data_ptr(), size)
     return dx, dweight, dbias
+
+
+def feature_layer_norm(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float,
+                       activation: str) -> Tensor:
+    """Layer norm with an activation over the last dimension of x (...,C)."""
+    channels = x.shape[-1]
+    y = x.new_empty(x.shape)
+    rows = x.numel() // channels
+    if rows:
+        x, weight, bias = _dense(x), _dense(weight), _dense(bias)
+        _call(lib.splat_feature_layer_norm, "feature_layer_norm", x.device,
+              FEATURE_DTYPES[x.dtype], rows, channels, x.data_ptr(), _address(weight),
+              _address(bias), eps, _ACTIVATION_CODES[activation], y.data_ptr())
+    return y
+
+
+def feature_layer_norm_backward(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float,
+                                activation: str, upstream: Tensor,
+                                needs: tuple[bool, bool, bool]
+                                ) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
+    """Gradients of x, weight and bias (None where not needed)."""
+    channels = x.shape[-1]
+    rows = x.numel() // channels
+    make = x.new_empty if rows else x.new_zeros
+    dx = make(x.shape) if needs[0] else None
+    dweight = make((channels,)) if needs[1] else None
+    dbias = make((channels,)) if needs[2] else None
+    if rows and any(needs):
+        dtype, device = FEATURE_DTYPES[x.dtype], x.device
+        size = _query("splat_feature_layer_norm_backward_workspace_bytes", device.index, dtype,
+                      rows, channels)
+        ws = x.new_empty((size,), dtype=torch.uint8)
+        x, weight, bias, upstream = _dense(x), _dense(weight), _dense(bias), _dense(upstream)
+        _call(lib.splat_feature_layer_norm_backward, "feature_layer_norm_backward", device, dtype,
+              rows, channels, x.data_ptr(), _address(weight), _address(bias), eps,
+              _ACTIVATION_CODES[activation], upstream.data_ptr(), _address(dx),
+              _address(dweight), _address(dbias), ws.data_ptr(), size)
+    return dx, dweight, dbias
+
+
+def feature_embedding(ids: Tensor, table: Tensor, scale: float) -> Tensor:
+    """scale table[ids] for ids of any shape and table (V,C)."""
+    entries, channels = table.shape
+    y = table.new_empty(ids.shape + (channels,))
+    count = ids.numel()
+    if count:
+        ids, table = _dense(ids), _dense(table)
+        _call(lib.splat_feature_embedding, "feature_embedding", table.device,
+              FEATURE_DTYPES[table.dtype], ids.element_size(), count, entries, channels,
+              ids.data_ptr(), table.data_ptr(), scale, y.data_ptr())
+    return y
+
+
+def feature_embedding_backward(ids: Tensor, entries: int, scale: float,
+                               upstream: Tensor) -> Tensor:
+    """The gradient of a table (entries,C) for upstream ids.shape + (C,)."""
+    channels, count = upstream.shape[-1], ids.numel()
+    if not count:
+        return upstream.new_zeros((entries, channels))
+    dtable = upstream.new_empty((entries, channels))
+    dtype, device = FEATURE_DTYPES[upstream.dtype], upstream.device
+    size = _query("splat_feature_embedding_backward_workspace_bytes", device.index, dtype, count,
+                  entries, channels)
+    ws = upstream.new_empty((size,), dtype=torch.uint8)
+    ids, upstream = _dense(ids), _dense(upstream)
+    _call(lib.splat_feature_embedding_backward, "feature_embedding_backward", device, dtype,
+          ids.element_size(), count, entries, channels, ids.data_ptr(), upstream.data_ptr(),
+          scale, dtable.data_ptr(), ws.data_ptr(), size)
+    return dtable
+
+
+# ---- optimizer -----------------------------------------------------------------
+
+def adamw(device: torch.device, dtype: torch.dtype, bits: int, records: list, maximize: bool
+          ) -> None:
+    """One AdamW step of nv.SplatAdamwTensor records on one device, of one dtype."""
+    table = (nv.SplatAdamwTensor * len(records))(*records)
+    _call(lib.splat_adamw, "adamw", device, FEATURE_DTYPES[dtype], bits, len(records), table,
+          int(maximize))
+
+
+def adamw_decode(codes: Tensor, exponents: Tensor, squared: bool) -> Tensor:
+    """The float32 values that contiguous 8-bit codes stand for."""
+    values = codes.new_empty(codes.shape, dtype=torch.float32)
+    if codes.numel():
+        _call(lib.splat_adamw_decode, "adamw_decode", codes.device, codes.numel(),
+              codes.data_ptr(), exponents.data_ptr(), int(squared), values.data_ptr())
+    return values
+
+
+def adamw_encode(values: Tensor, squared: bool) -> tuple[Tensor, Tensor]:
+    """The nearest codes of float32 values, and their exponents."""
+    values = _dense(values)
+    codes = values.new_empty(values.shape, dtype=torch.uint8)
+    exponents = values.new_empty((-(-values.numel() // 256),), dtype=torch.int8)
+    if values.numel():
+        _call(lib.splat_adamw_encode, "adamw_encode", values.device, values.numel(),
+              values.data_ptr(), int(squared), codes.data_ptr(), exponents.data_ptr())
+    return codes, exponents

@@ -28,8 +28,9 @@ Operator <- reference code it stands for:
   rade_project_backward  rade/projection.py:475-551
   rade_render         rade/render.py:550-601 (colour, alpha, depths, normals)
   rade_render_backward   rade/render.py:604-670
-  feature_linear, feature_norm and their _backward: no counterpart (features.linear,
-                      features.group_norm)
+  feature_linear, feature_norm, feature_layer_norm, feature_embedding and their
+                      _backward: no counterpart (features.linear, .group_norm,
+                      .layer_norm, .embedding)
 """
 
 from __future__ import annotations
@@ -621,8 +622,114 @@ def _feature_norm_backward(ctx, upstream, _moments):
 
 feature_norm.register_autograd(_feature_norm_backward, setup_context=_feature_norm_setup)
 
+
+def _check_layer_norm(x, weight, bias, eps, activation, upstream=None):
+    _check_forward_mode()
+    features.check_layer_norm(x, weight, bias, eps, activation)
+    features._check_like(upstream, x, x.shape, "upstream")
+
+
+@torch.library.custom_op(f"{_NS}::feature_layer_norm", mutates_args=())
+def feature_layer_norm(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float,
+                       activation: str) -> Tensor:
+    _check_layer_norm(x, weight, bias, eps, activation)
+    return stages.feature_layer_norm(x, weight, bias, eps, activation)
+
+
+@feature_layer_norm.register_fake
+def _(x, weight, bias, eps, activation):
+    _check_layer_norm(x, weight, bias, eps, activation)
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op(f"{_NS}::feature_layer_norm_backward", mutates_args=())
+def feature_layer_norm_backward(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float,
+                                activation: str, upstream: Tensor
+                                ) -> tuple[Tensor, Tensor, Tensor]:
+    _check_layer_norm(x, weight, bias, eps, activation, upstream)
+    return stages.feature_layer_norm_backward(x, weight, bias, eps, activation, upstream,
+                                              (True, True, True))
+
+
+@feature_layer_norm_backward.register_fake
+def _(x, weight, bias, eps, activation, upstream):
+    _check_layer_norm(x, weight, bias, eps, activation, upstream)
+    return (x.new_empty(x.shape), x.new_empty((x.shape[-1],)), x.new_empty((x.shape[-1],)))
+
+
+def _feature_layer_norm_setup(ctx, inputs, output):
+    x, weight, bias, *ctx.settings = inputs
+    ctx.save_for_backward(x, weight, bias)
+
+
+def _feature_layer_norm_backward(ctx, upstream):
+    x, weight, bias = ctx.saved_tensors
+    dx, dw, db = torch.ops.splat200.feature_layer_norm_backward(x, weight, bias, *ctx.settings,
+                                                                upstream)
+    return dx, None if weight is None else dw, None if bias is None else db, None, None
+
+
+feature_layer_norm.register_autograd(_feature_layer_norm_backward,
+                                     setup_context=_feature_layer_norm_setup)
+
+
+def _check_embedding(ids, table, scale):
+    _check_forward_mode()
+    if table.ndim != 2:
+        raise ValueError("table must be (V,C) with V and C of at least one")
+    features.check_embedding(ids, table.shape[0], table.shape[1], scale, table)
+
+
+def _check_embedding_backward(ids, entries, scale, upstream):
+    _check_forward_mode()
+    if upstream.ndim != ids.ndim + 1 or upstream.shape[:-1] != ids.shape:
+        raise ValueError("upstream must have the shape of ids and channels last")
+    features.check_embedding(ids, entries, upstream.shape[-1], scale, upstream)
+
+
+@torch.library.custom_op(f"{_NS}::feature_embedding", mutates_args=())
+def feature_embedding(ids: Tensor, table: Tensor, scale: float) -> Tensor:
+    _check_embedding(ids, table, scale)
+    return stages.feature_embedding(ids, table, scale)
+
+
+@feature_embedding.register_fake
+def _(ids, table, scale):
+    _check_embedding(ids, table, scale)
+    return table.new_empty(ids.shape + (table.shape[1],))
+
+
+@torch.library.custom_op(f"{_NS}::feature_embedding_backward", mutates_args=())
+def feature_embedding_backward(ids: Tensor, entries: int, scale: float,
+                               upstream: Tensor) -> Tensor:
+    _check_embedding_backward(ids, entries, scale, upstream)
+    return stages.feature_embedding_backward(ids, entries, scale, upstream)
+
+
+@feature_embedding_backward.register_fake
+def _(ids, entries, scale, upstream):
+    _check_embedding_backward(ids, entries, scale, upstream)
+    return upstream.new_empty((entries, upstream.shape[-1]))
+
+
+def _feature_embedding_setup(ctx, inputs, output):
+    ids, table, ctx.scale = inputs
+    ctx.save_for_backward(ids)
+    ctx.entries = table.shape[0]
+
+
+def _feature_embedding_backward(ctx, upstream):
+    ids, = ctx.saved_tensors
+    return None, torch.ops.splat200.feature_embedding_backward(ids, ctx.entries, ctx.scale,
+                                                               upstream), None
+
+
+feature_embedding.register_autograd(_feature_embedding_backward,
+                                    setup_context=_feature_embedding_setup)
+
 OPERATORS = ("cameras_prepare", "project", "project_backward", "project_views",
              "project_views_backward", "sh_forward", "sh_backward", "bin_and_sort", "render",
              "render_backward", "rade_project", "rade_project_backward", "rade_render",
              "rade_render_backward", "feature_linear", "feature_linear_backward", "feature_norm",
-             "feature_norm_backward")
+             "feature_norm_backward", "feature_layer_norm", "feature_layer_norm_backward",
+             "feature_embedding", "feature_embedding_backward")

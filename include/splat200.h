@@ -611,6 +611,62 @@ int splat_feature_norm_backward(int dtype, int samples, long long positions, int
                                 const void* dy, void* dx, void* dweight, void* dbias,
                                 void* workspace, size_t workspace_bytes, void* stream);
 
+/* y = act((x - mean) rstd weight + bias) with the mean and biased variance of
+ * each row of x (rows, channels); weight, bias (channels) or NULL. */
+int splat_feature_layer_norm(int dtype, long long rows, int channels, const void* x,
+                             const void* weight, const void* bias, float eps, int activation,
+                             void* y, void* stream);
+
+/* Gradients of the above for dy: dx, dweight, dbias, each NULL to skip it.  The
+ * rows' moments are taken from x again. */
+size_t splat_feature_layer_norm_backward_workspace_bytes(int dtype, long long rows, int channels);
+int splat_feature_layer_norm_backward(int dtype, long long rows, int channels, const void* x,
+                                      const void* weight, const void* bias, float eps,
+                                      int activation, const void* dy, void* dx, void* dweight,
+                                      void* dbias, void* workspace, size_t workspace_bytes,
+                                      void* stream);
+
+/* y_i = scale table[ids_i]; ids (count) of id_bytes 4 or 8 (signed), table
+ * (entries, channels), y (count, channels).  An id outside the table gives a row of
+ * zeros, no gradient and (forward) the device error -6. */
+int splat_feature_embedding(int dtype, int id_bytes, long long count, int entries, int channels,
+                            const void* ids, const void* table, float scale, void* y,
+                            void* stream);
+
+/* dtable[v] = scale sum of dy_i over ids_i = v, all of (entries, channels). */
+size_t splat_feature_embedding_backward_workspace_bytes(int dtype, long long count, int entries,
+                                                        int channels);
+int splat_feature_embedding_backward(int dtype, int id_bytes, long long count, int entries,
+                                     int channels, const void* ids, const void* dy, float scale,
+                                     void* dtable, void* workspace, size_t workspace_bytes,
+                                     void* stream);
+
+/* ---- optimizer ---------------------------------------------------------------
+ * One AdamW step of `count` tensors in place: p and g of the dtype (as above), m
+ * and v float32 (bits 32) or 8-bit codes (bits 8: v's are of its root) with an
+ * exponent for each 256 values, ceil(n / 256) signed bytes.  step counts from 1.
+ * device_step and device_lr (NULL: step and lr are used) are read by the kernel, so
+ * that a captured launch follows them.  No two tensors may overlap. */
+typedef struct SplatAdamwTensor {
+  void* p;
+  const void* g;
+  void *m, *v;
+  void *m_exponents, *v_exponents;
+  const long long* device_step;
+  const float* device_lr;
+  long long n, step;
+  double lr, weight_decay, beta1, beta2, eps;
+} SplatAdamwTensor;
+int splat_adamw(int dtype, int bits, int count, const SplatAdamwTensor* tensors, int maximize,
+                void* stream);
+
+/* What 8-bit codes of n values stand for (squared: of v, else of m), and the
+ * nearest codes of float32 values. */
+int splat_adamw_decode(long long n, const void* codes, const void* exponents, int squared,
+                       float* values, void* stream);
+int splat_adamw_encode(long long n, const float* values, int squared, void* codes,
+                       void* exponents, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

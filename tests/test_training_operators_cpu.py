@@ -1,0 +1,210 @@
+"""The operators that train features, without a GPU: what they refuse, the shapes of
+their torch.ops forms and the C entry points' status codes."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
+
+from dsl_splat_b200 import features, optim
+from dsl_splat_b200._native import SplatAdamwTensor, lib
+
+ops = torch.ops.splat200
+P = 256  # an aligned address that is never read
+
+
+def fake(*shape, dtype=torch.float32, device="cuda"):
+    return torch.empty(shape, device=device, dtype=dtype)
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(activation="tanh"), "activation"),
+    (dict(x=()), "x must have a last dimension"),
+    (dict(x=(3, 0), weight=(0,)), "x must have a last dimension"),
+    (dict(weight=(7,)), "weight must have shape"),
+    (dict(bias=(1, 8)), "bias must have shape"),
+    (dict(dtype=torch.float64), "x must be a CUDA"),
+    (dict(weight_dtype=torch.float16), "weight must have x's dtype"),
+    (dict(device="cpu"), "x must be a CUDA"),
+    (dict(eps=0.0), "eps must be finite"),
+    (dict(eps=1e-60), "eps must be finite"),
+    (dict(x=(2, 65536), weight=(65536,), bias=(65536,)), "65535"),
+])
+def test_layer_norm_refusals(change, message):
+    with FakeTensorMode():
+        dtype, device = change.get("dtype", torch.float32), change.get("device", "cuda")
+        x = fake(*change.get("x", (5, 8)), dtype=dtype, device=device)
+        weight = fake(*change.get("weight", (8,)), dtype=change.get("weight_dtype", dtype),
+                      device=device)
+        bias = fake(*change.get("bias", (8,)), dtype=dtype, device=device)
+        eps, act = change.get("eps", 1e-5), change.get("activation", "silu")
+        for call in (lambda: features.layer_norm(x, weight, bias, eps=eps, activation=act),
+                     lambda: ops.feature_layer_norm(x, weight, bias, eps, act),
+                     lambda: ops.feature_layer_norm_backward(x, weight, bias, eps, act, x)):
+            with pytest.raises(ValueError, match=message):
+                call()
+
+
+def test_layer_norm_refuses_host_tensors():
+    with pytest.raises(ValueError, match="x must be a CUDA"):
+        features.layer_norm(torch.zeros(2, 3))
+    with FakeTensorMode(), pytest.raises(ValueError, match="upstream must have shape"):
+        ops.feature_layer_norm_backward(fake(4, 8), None, None, 1e-5, "none", fake(4, 7))
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(table=(5,)), r"table must be \(V,C\)"),
+    (dict(table=(0, 4)), r"table must be \(V,C\)"),
+    (dict(table=(5, 0)), r"table must be \(V,C\)"),
+    (dict(dtype=torch.float64), "table must be a CUDA"),
+    (dict(device="cpu"), "table must be a CUDA"),
+    (dict(ids_dtype=torch.int16), "ids must be an int32"),
+    (dict(ids_device="cpu"), "ids must be on the table's device"),
+    (dict(scale=float("nan")), "scale must be finite"),
+    (dict(scale=1e39), "scale must be finite"),
+    (dict(table=(5, 70000)), "65535"),
+])
+def test_embedding_refusals(change, message):
+    with FakeTensorMode():
+        table = fake(*change.get("table", (5, 4)), dtype=change.get("dtype", torch.float32),
+                     device=change.get("device", "cuda"))
+        ids = fake(3, 2, dtype=change.get("ids_dtype", torch.int64),
+                   device=change.get("ids_device", "cuda"))
+        scale = change.get("scale", 1.0)
+        for call in (lambda: features.embedding(ids, table, scale=scale),
+                     lambda: ops.feature_embedding(ids, table, scale)):
+            with pytest.raises(ValueError, match=message):
+                call()
+
+
+def test_embedding_backward_refusals():
+    with FakeTensorMode():
+        ids = fake(3, 2, dtype=torch.int64)
+        for upstream, entries, message in ((fake(3, 2), 5, "upstream must have the shape"),
+                                           (fake(3, 3, 4), 5, "upstream must have the shape"),
+                                           (fake(3, 2, 4), 0, r"table must be \(V,C\)")):
+            with pytest.raises(ValueError, match=message):
+                ops.feature_embedding_backward(ids, entries, 1.0, upstream)
+
+
+def test_fake_shapes():
+    with FakeTensorMode():
+        x, w = fake(4, 5, 8, dtype=torch.bfloat16), fake(8, dtype=torch.bfloat16)
+        assert features.layer_norm(x, w).shape == x.shape
+        dx, dw, db = ops.feature_layer_norm_backward(x, w, None, 1e-5, "silu", x)
+        assert dx.shape == x.shape and dw.shape == db.shape == (8,)
+        ids, table = fake(3, 2, dtype=torch.int32), fake(9, 4, dtype=torch.float16)
+        y = features.embedding(ids, table)
+        assert y.shape == (3, 2, 4) and y.dtype is torch.float16
+        assert ops.feature_embedding_backward(ids, 9, 1.0, y).shape == (9, 4)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_traced_programs_hold_the_operators(grad):
+    def run(ids, table, w):
+        return features.layer_norm(features.embedding(ids, table), w)
+
+    with FakeTensorMode():
+        tensors = [fake(*s).requires_grad_(grad) for s in ((9, 4), (4,))]
+        graph = make_fx(run)(fake(6, dtype=torch.int64), *tensors)
+    called = [n.target for n in graph.graph.nodes if n.op == "call_function"]
+    assert ops.feature_embedding.default in called
+    assert ops.feature_layer_norm.default in called
+
+
+def test_forward_mode_is_refused():
+    with FakeTensorMode(), fwAD.dual_level():
+        x, table, ids = fake(6, 4), fake(9, 4), fake(3, dtype=torch.int64)
+        for call in (lambda: features.layer_norm(fwAD.make_dual(x, torch.ones_like(x))),
+                     lambda: features.embedding(ids, fwAD.make_dual(table, fake(9, 4))),
+                     lambda: ops.feature_layer_norm(x, None, None, 1e-5, "none"),
+                     lambda: ops.feature_embedding(ids, table, 1.0)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+
+
+def test_decoder_takes_layer_norms():
+    with FakeTensorMode():
+        decoder = features.FeatureDecoder(features.Linear(fake(6, 4)),
+                                          features.LayerNorm(fake(6), fake(6)))
+        assert decoder(fake(2, 3, 4)).shape == (2, 3, 6)
+        assert len(list(decoder.parameters())) == 3
+
+
+def test_entry_points_refuse_before_any_launch():
+    before = lib.splat_launch_count()
+    norm, back = lib.splat_feature_layer_norm, lib.splat_feature_layer_norm_backward
+    assert norm(3, 1, 8, P, None, None, 1e-5, 0, P, None) == -1
+    assert norm(0, 1, 8, P, None, None, 1e-5, 5, P, None) == -1
+    assert norm(0, 0, 8, P, None, None, 1e-5, 0, P, None) == -1
+    assert norm(0, 1, 70000, P, None, None, 1e-5, 0, P, None) == -4
+    assert norm(0, 1, 8, None, None, None, 1e-5, 0, P, None) == -1
+    size = lib.splat_feature_layer_norm_backward_workspace_bytes
+    assert size(0, 10, 8) >= 64 and size(4, 10, 8) == 0
+    assert back(0, 10, 8, P, None, None, 1e-5, 0, P, P, P, P, P, 0, None) == -5
+    assert back(0, 10, 8, P, None, None, 1e-5, 0, P, P, P, P, P + 4, 1 << 20, None) == -1
+    assert back(0, 10, 8, P, None, None, 1e-5, 0, None, P, P, P, P, 1 << 20, None) == -1
+    look, grad = lib.splat_feature_embedding, lib.splat_feature_embedding_backward
+    assert look(0, 2, 1, 4, 4, P, P, 1.0, P, None) == -1
+    assert look(0, 8, 0, 4, 4, P, P, 1.0, P, None) == -1
+    assert look(0, 8, (1 << 30) + 1, 4, 4, P, P, 1.0, P, None) == -4
+    assert look(0, 8, 1, 4, 4, None, P, 1.0, P, None) == -1
+    assert lib.splat_feature_embedding_backward_workspace_bytes(0, 8, 4, 4) == 16
+    assert lib.splat_feature_embedding_backward_workspace_bytes(0, 100000, 50, 4) > 400000
+    assert grad(0, 8, 100000, 50, 4, P, P, 1.0, P, P, 100, None) == -5
+    assert grad(0, 8, 8, 4, 4, P, P, 1.0, None, P, 100, None) == -1
+    assert lib.splat_launch_count() == before
+
+
+def test_adamw_entry_points_refuse_before_any_launch():
+    before = lib.splat_launch_count()
+
+    def record(**change):
+        values = dict(p=P, g=P, m=P, v=P, n=8, step=1, lr=0.1, beta1=0.9, beta2=0.999, eps=1e-8)
+        return (SplatAdamwTensor * 1)(SplatAdamwTensor(**{**values, **change}))
+
+    assert lib.splat_adamw(3, 32, 1, record(), 0, None) == -1
+    assert lib.splat_adamw(0, 16, 1, record(), 0, None) == -1
+    assert lib.splat_adamw(0, 32, -1, record(), 0, None) == -1
+    assert lib.splat_adamw(0, 32, 1, None, 0, None) == -1
+    assert lib.splat_adamw(0, 32, 1, record(step=0), 0, None) == -1
+    assert lib.splat_adamw(0, 32, 1, record(p=None), 0, None) == -1
+    assert lib.splat_adamw(0, 8, 1, record(), 0, None) == -1
+    assert lib.splat_adamw(0, 32, 1, record(n=-1), 0, None) == -1
+    assert lib.splat_adamw(0, 32, 1, record(n=1 << 41), 0, None) == -4
+    assert lib.splat_adamw(0, 32, 0, None, 0, None) == 0
+    assert lib.splat_adamw(0, 32, 1, record(n=0), 0, None) == 0
+    assert lib.splat_adamw_decode(0, P, P, 0, P, None) == -1
+    assert lib.splat_adamw_decode(8, None, P, 0, P, None) == -1
+    assert lib.splat_adamw_encode(8, P, 0, P, None, None) == -1
+    assert lib.splat_launch_count() == before
+
+
+def test_optimizer_refuses_host_tensors_and_bad_settings():
+    with pytest.raises(ValueError, match="CUDA"):
+        optim.AdamW([torch.zeros(3, requires_grad=True)])
+    with FakeTensorMode():
+        p = fake(4, 3).requires_grad_()
+        for change, message in ((dict(lr=-1.0), "lr"), (dict(lr=float("nan")), "lr"),
+                                (dict(betas=(1.0, 0.9)), "betas"), (dict(eps=-1.0), "eps"),
+                                (dict(weight_decay=-0.1), "weight_decay"),
+                                (dict(state_bits=16), "state_bits")):
+            with pytest.raises(ValueError, match=message):
+                optim.AdamW([p], **change)
+        with pytest.raises(ValueError, match="contiguous"):
+            optim.AdamW([fake(4, 3).t().requires_grad_()])
+
+
+def test_moment8_refusals():
+    codes, exponents = torch.zeros(300, dtype=torch.uint8), torch.zeros(2, dtype=torch.int8)
+    optim.Moment8(codes, exponents)
+    for c, e, message in ((codes.int(), exponents, "uint8"), (codes, exponents.int(), "int8"),
+                          (codes, exponents[:1], "one value for each 256"),
+                          (codes[::2], exponents[:1], "contiguous")):
+        with pytest.raises(ValueError, match=message):
+            optim.Moment8(c, e)
+    with pytest.raises(ValueError, match="CUDA"):
+        optim.Moment8(codes, exponents).values()
+    with pytest.raises(ValueError, match="CUDA float32"):
+        optim.Moment8.of(torch.zeros(3))
