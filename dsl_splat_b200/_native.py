@@ -112,6 +112,11 @@ SIGNATURES: dict[str, tuple] = {
     "splat_feature_embedding": (_I, [_I, _I, _L, _I, _I, _P, _P, _F, _P, _P]),
     "splat_feature_embedding_backward_workspace_bytes": (_Z, [_I, _L, _I, _I]),
     "splat_feature_embedding_backward": (_I, [_I, _I, _L, _I, _I, _P, _P, _F, _P, _P, _Z, _P]),
+    "splat_feature_entropy_workspace_bytes": (_Z, [_I, _L, _I, _I, _I]),
+    "splat_feature_entropy": (_I, [_I, _L, _I, _I, _P, _P, _P, _I, _P, _L, _I, _P, _P, _P, _P,
+                                   _Z, _P]),
+    "splat_feature_entropy_backward": (_I, [_I, _L, _I, _I, _P, _P, _P, _I, _P, _L, _I, _P, _P,
+                                            _P, _P, _P, _P, _P, _Z, _P]),
     "splat_adamw": (_I, [_I, _I, _I, _P, _I, _P]),
     "splat_adamw_decode": (_I, [_L, _P, _P, _I, _P, _P]),
     "splat_adamw_encode": (_I, [_L, _P, _I, _P, _P, _P]),

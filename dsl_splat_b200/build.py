@@ -39,6 +39,7 @@ SOURCES = {"splat200.cu": ["-fmad=false"],
            "feature_norm.cu": ["-fmad=true"],
            "feature_layer_norm.cu": ["-fmad=true"],
            "feature_embedding.cu": ["-fmad=true"],
+           "feature_entropy.cu": ["-fmad=true"],
            "adamw.cu": ["-fmad=true"]}
 HEADERS = ["splat_common.cuh", "cameras.cuh", "project.cuh", "binning.cuh", "render.cuh",
            "footprint.cuh", "tile_modes.cuh", "host_runtime.h", "rade.cuh", "rade_project.cuh",

@@ -143,7 +143,7 @@ int launch_product(ProductParams p, cudaStream_t s) {
   if (p.stages < 1) return host::fail(kTooLarge, "feature_linear: no room for a stage");
   if (EPI != kPlain) p.copy_extra = make_map<TE>(p.extra_map, p.extra, p.m, p.n, p.n, 32, 32);
   // partial sums are added to or lie one split behind the other
-  if (p.splits == 1 && (p.k_per_sum >= p.k || p.held))
+  if (p.splits == 1 && (p.k_per_sum >= p.k || p.held) && !p.accumulate)
     p.copy_out = make_map<TO>(p.out_map, p.out, p.m, p.n, p.out_ld, 32, 32) &&
                  (!p.out_second ||
                   make_map<TO>(p.out_second_map, p.out_second, p.m, p.n, p.out_ld, 32, 32));

@@ -83,6 +83,7 @@ struct ProductParams {
   long long k_per_sum;     // of one accumulator; the tile's sums are added in `out` (fp32)
   int held;                // or, of 16-bit results, in shared memory
   int splits, tile_n;
+  int accumulate;          // fp32 results of a plain product are added to what `out` holds
   uint32_t tiles_n, tiles_m, tiles;  // tiles = splits * tiles_m * tiles_n, below 2^31
   int stages, resident, activation;
   // accumulators of a block: 2, whose columns the two groups of four epilogue
@@ -1087,7 +1088,8 @@ __global__ void __launch_bounds__(producers(PA, PB) == 128 ? 512 : 544,
               __syncwarp();
               out_patch.store(static_cast<TO*>(out) + out_at + col0, p.out_ld, rows, cols,
                               p.out_vector,
-                              !kExtra && sizeof(TO) == 4 && sum_k != tile.k0);
+                              !kExtra && sizeof(TO) == 4 &&
+                                  (sum_k != tile.k0 || p.accumulate));
             }
           };
           if constexpr (EPI == kSlope && sizeof(TO) == 2) {

@@ -7,6 +7,8 @@ the per-Gaussian features that they blend from.
 * `layer_norm`: layer norm with an activation over the last dimension;
 * `embedding`: rows of a table by their ids, such as a codebook that Gaussians
   share or a code for each view;
+* `linear_cross_entropy`: the softmax cross entropy of a linear head over a
+  vocabulary, whose logits are never kept;
 * `FeatureDecoder`: a run of them, called on an image, or passed to
   gs3d.rasterize / rade.rasterize / aaa.rasterize as `feature_decoder`.
 
@@ -138,6 +140,30 @@ class _Embedding(torch.autograd.Function):
             return None, None, None
         ids, = ctx.saved_tensors
         return None, stages.feature_embedding_backward(ids, *ctx.settings, upstream), None
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, x: Tensor, weight: Tensor, target: Tensor, bias: Tensor | None,
+                ignore_index: int, reduction: str) -> Tensor:
+        loss, lse, counted = stages.feature_entropy(x, weight, target, bias, ignore_index,
+                                                    reduction)
+        ctx.save_for_backward(x, weight, target, bias, lse, counted)
+        ctx.settings = ignore_index, reduction
+        ctx.set_materialize_grads(False)
+        return loss
+
+    @staticmethod
+    @_once
+    def backward(ctx: Any, upstream: Tensor | None):
+        if upstream is None:
+            return (None,) * 6
+        x, weight, target, bias, lse, counted = ctx.saved_tensors
+        needs = ctx.needs_input_grad
+        dx, dweight, dbias = stages.feature_entropy_backward(
+            x, weight, target, bias, *ctx.settings, lse, counted, upstream,
+            (needs[0], needs[1], needs[3]))
+        return dx, dweight, None, dbias, None, None
 
 
 def _check_activation(activation: str) -> None:
@@ -335,6 +361,53 @@ def embedding(ids: Tensor, table: Tensor, *, scale: float = 1.0) -> Tensor:
     return stages.feature_embedding(ids, table, scale)
 
 
+def check_linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, bias: Tensor | None,
+                               ignore_index: int, reduction: str) -> None:
+    """Refuses what `linear_cross_entropy` does not take."""
+    if reduction not in stages.REDUCTIONS:
+        raise ValueError(f"reduction must be one of {stages.REDUCTIONS}")
+    _check_input(x)
+    if x.ndim < 1 or x.shape[-1] < 1:
+        raise ValueError("x must have a last dimension of at least one feature")
+    if not isinstance(weight, Tensor) or weight.ndim != 2 or weight.shape[0] < 1:
+        raise ValueError("weight must be (V,K) with V of at least one")
+    vocabulary = weight.shape[0]
+    _check_like(weight, x, (vocabulary, x.shape[-1]), "weight")
+    _check_like(bias, x, (vocabulary,), "bias")
+    if not isinstance(target, Tensor) or target.dtype not in (torch.int32, torch.int64):
+        raise ValueError("target must be an int32 or int64 tensor")
+    if target.device != x.device or target.shape != x.shape[:-1]:
+        raise ValueError("target must have x's device and its leading dimensions")
+    if isinstance(ignore_index, bool) or not isinstance(ignore_index, Integral) \
+            or not -(1 << 63) <= ignore_index < 1 << 63:
+        raise ValueError("ignore_index must be an integer of 64 bits")
+    if x.shape[-1] > 65535 or vocabulary > 1 << 20 or target.numel() > 1 << 31:
+        raise ValueError("at most 65535 features, 2^20 words and 2^31 rows")
+
+
+def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, bias: Tensor | None = None,
+                         *, ignore_index: int = -100, reduction: str = "mean") -> Tensor:
+    """The softmax cross entropy of z = x weight^T + bias over a vocabulary,
+    log sum_j exp z_j - z_target, as float32; the logits are never kept.
+
+    x: (...,K), weight: (V,K), bias: (V,), target: (...) of int32 or int64 in [0,V).
+    Rows whose target is ignore_index have no loss and no gradient; so have rows with
+    another target outside, which also set the library's error word.  reduction:
+    "none" (a loss for each row), "sum" or "mean" over the rows that count (0 if none
+    does).  A bias of minus infinity takes a word out.
+    """
+    check_linear_cross_entropy(x, weight, target, bias, ignore_index, reduction)
+    if forward_ad._current_level >= 0:
+        _check_forward_mode(x, weight, bias)
+    ignore_index = int(ignore_index)
+    if _traced():
+        return torch.ops.splat200.feature_entropy(x, weight, target, bias, ignore_index,
+                                                  reduction)[0]
+    if _recorded(x, weight, bias):
+        return _LinearCrossEntropy.apply(x, weight, target, bias, ignore_index, reduction)
+    return stages.feature_entropy(x, weight, target, bias, ignore_index, reduction, False)[0]
+
+
 @dataclass(slots=True)
 class Linear:
     """One `linear` of a FeatureDecoder; residual=True adds the layer's own input."""
@@ -396,9 +469,22 @@ class FeatureDecoder:
                     yield t
 
     def __call__(self, image: Tensor) -> Tensor:
+        return self._run(image, self.layers)
+
+    def _run(self, image: Tensor, layers: tuple) -> Tensor:
         first = next(self.parameters(), None)
         if first is not None:
             image = image.to(first.dtype)
-        for layer in self.layers:
+        for layer in layers:
             image = layer(image)
         return image
+
+    def cross_entropy(self, image: Tensor, target: Tensor, *, ignore_index: int = -100,
+                      reduction: str = "mean") -> Tensor:
+        """`linear_cross_entropy` of the decoder's result, whose last layer is a Linear
+        without activation or residual, and whose values are never kept."""
+        head = self.layers[-1]
+        if not isinstance(head, Linear) or head.activation != "none" or head.residual:
+            raise ValueError("cross_entropy needs a last Linear without activation or residual")
+        return linear_cross_entropy(self._run(image, self.layers[:-1]), head.weight, target,
+                                    head.bias, ignore_index=ignore_index, reduction=reduction)

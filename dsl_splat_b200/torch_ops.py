@@ -28,9 +28,9 @@ Operator <- reference code it stands for:
   rade_project_backward  rade/projection.py:475-551
   rade_render         rade/render.py:550-601 (colour, alpha, depths, normals)
   rade_render_backward   rade/render.py:604-670
-  feature_linear, feature_norm, feature_layer_norm, feature_embedding and their
-                      _backward: no counterpart (features.linear, .group_norm,
-                      .layer_norm, .embedding)
+  feature_linear, feature_norm, feature_layer_norm, feature_embedding, feature_entropy
+                      and their _backward: no counterpart (features.linear, .group_norm,
+                      .layer_norm, .embedding, .linear_cross_entropy)
 """
 
 from __future__ import annotations
@@ -727,9 +727,75 @@ def _feature_embedding_backward(ctx, upstream):
 feature_embedding.register_autograd(_feature_embedding_backward,
                                     setup_context=_feature_embedding_setup)
 
+
+def _check_entropy(x, weight, target, bias, ignore_index, reduction):
+    _check_forward_mode()
+    features.check_linear_cross_entropy(x, weight, target, bias, ignore_index, reduction)
+
+
+def _check_entropy_backward(x, weight, target, bias, ignore_index, reduction, lse, counted,
+                            upstream):
+    _check_entropy(x, weight, target, bias, ignore_index, reduction)
+    shapes = ((target.numel(),), (1,), target.shape if reduction == "none" else ())
+    for t, shape, name in zip((lse, counted, upstream), shapes, ("lse", "counted", "upstream")):
+        if t.dtype is not torch.float32 or t.device != x.device or t.shape != shape:
+            raise ValueError(f"{name} must be float32 of shape {tuple(shape)} on x's device")
+
+
+@torch.library.custom_op(f"{_NS}::feature_entropy", mutates_args=())
+def feature_entropy(x: Tensor, weight: Tensor, target: Tensor, bias: Tensor | None,
+                    ignore_index: int, reduction: str) -> tuple[Tensor, Tensor, Tensor]:
+    _check_entropy(x, weight, target, bias, ignore_index, reduction)
+    return stages.feature_entropy(x, weight, target, bias, ignore_index, reduction)
+
+
+@feature_entropy.register_fake
+def _(x, weight, target, bias, ignore_index, reduction):
+    _check_entropy(x, weight, target, bias, ignore_index, reduction)
+    f32 = torch.float32
+    return (x.new_empty(target.shape if reduction == "none" else (), dtype=f32),
+            x.new_empty((target.numel(),), dtype=f32), x.new_empty((1,), dtype=f32))
+
+
+@torch.library.custom_op(f"{_NS}::feature_entropy_backward", mutates_args=())
+def feature_entropy_backward(x: Tensor, weight: Tensor, target: Tensor, bias: Tensor | None,
+                             ignore_index: int, reduction: str, lse: Tensor, counted: Tensor,
+                             upstream: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    _check_entropy_backward(x, weight, target, bias, ignore_index, reduction, lse, counted,
+                            upstream)
+    dx, dweight, dbias = stages.feature_entropy_backward(
+        x, weight, target, bias, ignore_index, reduction, lse, counted, upstream,
+        (True, True, True))
+    return dx, dweight, weight.new_empty((0,)) if dbias is None else dbias
+
+
+@feature_entropy_backward.register_fake
+def _(x, weight, target, bias, ignore_index, reduction, lse, counted, upstream):
+    _check_entropy_backward(x, weight, target, bias, ignore_index, reduction, lse, counted,
+                            upstream)
+    return (x.new_empty(x.shape), weight.new_empty(weight.shape),
+            weight.new_empty((0 if bias is None else weight.shape[0],)))
+
+
+def _feature_entropy_setup(ctx, inputs, output):
+    x, weight, target, bias, *ctx.settings = inputs
+    ctx.save_for_backward(x, weight, target, bias, output[1], output[2])
+
+
+def _feature_entropy_backward(ctx, upstream, _lse, _counted):
+    x, weight, target, bias, lse, counted = ctx.saved_tensors
+    dx, dw, db = torch.ops.splat200.feature_entropy_backward(
+        x, weight, target, bias, *ctx.settings, lse, counted, upstream)
+    return dx, dw, None, None if bias is None else db, None, None
+
+
+feature_entropy.register_autograd(_feature_entropy_backward,
+                                  setup_context=_feature_entropy_setup)
+
 OPERATORS = ("cameras_prepare", "project", "project_backward", "project_views",
              "project_views_backward", "sh_forward", "sh_backward", "bin_and_sort", "render",
              "render_backward", "rade_project", "rade_project_backward", "rade_render",
              "rade_render_backward", "feature_linear", "feature_linear_backward", "feature_norm",
              "feature_norm_backward", "feature_layer_norm", "feature_layer_norm_backward",
-             "feature_embedding", "feature_embedding_backward")
+             "feature_embedding", "feature_embedding_backward", "feature_entropy",
+             "feature_entropy_backward")

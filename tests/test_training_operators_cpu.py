@@ -208,3 +208,85 @@ def test_moment8_refusals():
         optim.Moment8(codes, exponents).values()
     with pytest.raises(ValueError, match="CUDA float32"):
         optim.Moment8.of(torch.zeros(3))
+
+
+ENTROPY = dict(x=(6, 4), weight=(9, 4), target=(6,), bias=(9,))
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(reduction="max"), "reduction"),
+    (dict(x=()), "x must have a last dimension"),
+    (dict(weight=(9,)), r"weight must be \(V,K\)"),
+    (dict(weight=(0, 4), bias=(0,)), r"weight must be \(V,K\)"),
+    (dict(weight=(9, 5)), "weight must have shape"),
+    (dict(weight_dtype=torch.float16), "weight must have x's dtype"),
+    (dict(bias=(8,)), "bias must have shape"),
+    (dict(target=(5,)), "target must have x's device"),
+    (dict(target=(6, 1)), "target must have x's device"),
+    (dict(target_device="cpu"), "target must have x's device"),
+    (dict(target_dtype=torch.uint8), "target must be an int32"),
+    (dict(x_dtype=torch.float64), "x must be a CUDA"),
+    (dict(ignore=1.5), "ignore_index"),
+    (dict(ignore=True), "ignore_index"),
+    (dict(ignore=1 << 63), "ignore_index"),
+    (dict(weight=((1 << 20) + 1, 4), bias=((1 << 20) + 1,)), "2\\^20 words"),
+])
+def test_entropy_refusals(change, message):
+    with FakeTensorMode():
+        dtypes = dict(target=torch.int64)
+        x, weight, target, bias = (
+            fake(*change.get(m, ENTROPY[m]),
+                 dtype=change.get(m + "_dtype", dtypes.get(m, torch.float32)),
+                 device=change.get(m + "_device", "cuda")) for m in ENTROPY)
+        with pytest.raises(ValueError, match=message):
+            features.linear_cross_entropy(x, weight, target, bias,
+                                          ignore_index=change.get("ignore", -100),
+                                          reduction=change.get("reduction", "mean"))
+
+
+def test_entropy_shapes_and_traces():
+    with FakeTensorMode():
+        x, w, b = (fake(*ENTROPY[m]).requires_grad_() for m in ("x", "weight", "bias"))
+        target = fake(6, dtype=torch.int64)
+        loss, lse, counted = ops.feature_entropy(x, w, target, b, -100, "none")
+        assert loss.shape == lse.shape == (6,) and counted.shape == (1,)
+        dx, dw, db = ops.feature_entropy_backward(x, w, target, b, -100, "none", lse, counted,
+                                                  loss)
+        assert dx.shape == x.shape and dw.shape == w.shape and db.shape == b.shape
+        with pytest.raises(ValueError, match="upstream must be float32 of shape"):
+            ops.feature_entropy_backward(x, w, target, b, -100, "mean", lse, counted, loss)
+        graph = make_fx(lambda x, w, t, b: features.linear_cross_entropy(x, w, t, b))(
+            x, w, target, b)
+        assert ops.feature_entropy.default in [n.target for n in graph.graph.nodes]
+        image = fake(2, 3, 4)
+        decoder = features.FeatureDecoder(features.LayerNorm(fake(4)), features.Linear(w, b))
+        labels = fake(2, 3, dtype=torch.int64)
+        assert decoder.cross_entropy(image, labels).shape == ()
+        assert decoder.cross_entropy(image, labels, reduction="none").shape == (2, 3)
+        for last in (features.Linear(w, b, "silu"), features.LayerNorm(fake(4))):
+            with pytest.raises(ValueError, match="last Linear"):
+                features.FeatureDecoder(features.Linear(fake(4, 4)), last).cross_entropy(image,
+                                                                                        labels)
+
+
+def test_entropy_entry_points_refuse_before_any_launch():
+    before = lib.splat_launch_count()
+    size = lib.splat_feature_entropy_workspace_bytes
+    assert size(0, 100, 8, 50, 0) > 100 * 50 * 4 and size(0, 100, 0, 50, 0) == 0
+    assert size(0, 100, 8, (1 << 20) + 1, 1) == 0
+
+    def forward(dtype=0, rows=100, k=8, v=50, x=P, id_bytes=8, reduction=0, ws=P, n=1 << 30):
+        return lib.splat_feature_entropy(dtype, rows, k, v, x, P, P, id_bytes, P, -100, reduction,
+                                         P, None, None, ws, n, None)
+
+    assert forward(dtype=5) == forward(rows=0) == forward(id_bytes=2) == forward(x=None) == -1
+    assert forward(reduction=3) == forward(ws=P + 4) == -1
+    assert forward(k=70000) == -4 and forward(n=100) == -5
+
+    def backward(reduction=0, counted=P, bias=P, up=P, n=1 << 30):
+        return lib.splat_feature_entropy_backward(0, 100, 8, 50, P, P, bias, 8, P, -100,
+                                                  reduction, P, counted, up, P, P, P, P, n, None)
+
+    assert backward(reduction=2, counted=None) == backward(bias=None) == backward(up=None) == -1
+    assert backward(n=100) == -5
+    assert lib.splat_launch_count() == before
