@@ -3,8 +3,10 @@
 //   z = x W^T + b,  lse_i = log sum_j exp z_ij,  l_i = lse_i - z_i,t_i
 //   dz_ij = u_i (exp(z_ij - lse_i) - [j = t_i]),  dx = dz W,  dW = dz^T x,  db = sum_i dz_i
 //
-// The logits are never kept: they are formed for a piece of the rows at a time, and
-// formed again in the backward.  u_i is the upstream gradient of row i's loss (divided by
+// The logits are never kept.  Those of 16-bit types never leave the chip
+// (feature_vocabulary.cuh); those of fp32, whose products take planes of three parts, are
+// formed for a piece of the rows at a time.  The backward forms them again, and dz for
+// a piece of the rows.  u_i is the upstream gradient of row i's loss (divided by
 // the number of rows that count for their mean) and 0 for the others.
 //
 // dz is held in T for the products.  It is taken relative to the power of two E that
@@ -15,55 +17,29 @@
 
 #include "feature_join.cuh"
 #include "feature_launch.cuh"
+#include "feature_vocabulary.cuh"
 #include "splat200.h"
 
 namespace splat {
 namespace feature {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr float kLog2E = 1.44269504088896341f;
-
-enum Reduction : int { kEach = 0, kSum = 1, kMean = 2 };
-
-// What the rows' kernels read.
-struct Rows {
-  long long rows;
-  int vocabulary, id_bytes, reduction;
-  long long ignored;
-  const void* target;
-  int* error;
-};
-
-// A row's label, or -1 where it does not count.
-SPLAT_DEV int label_of(const Rows& p, long long row) {
-  const long long t = p.id_bytes == 8 ? static_cast<const long long*>(p.target)[row]
-                                      : static_cast<const int*>(p.target)[row];
-  if (t == p.ignored) return -1;
-  if (t >= 0 && t < p.vocabulary) return static_cast<int>(t);
-  atomicCAS(p.error, 0, kInconsistentInput);
-  return -1;
-}
 
 // ---- softmax statistics ------------------------------------------------------------
 
-// Largest exponent so far and the sum relative to it.  A row that holds nothing but
-// minus infinities (or nothing at all) has the sum 0.
-struct Partial {
-  float top, sum;
-};
-SPLAT_DEV Partial join(Partial a, Partial b) {
-  const float top = fmaxf(a.top, b.top);  // NaN lies in the sums
-  if (top == -INFINITY) return {top, a.sum + b.sum};
-  return {top, a.sum * exp2f((a.top - top) * kLog2E) + b.sum * exp2f((b.top - top) * kLog2E)};
-}
+// Partial results of fp32 logits, whose top is the logit itself: its rounding to units of
+// log 2 would cost digits of the exponentials.
 SPLAT_DEV void take(Partial& s, float z) {
   if (z > s.top) {
-    s.sum = s.sum * exp2f((s.top - z) * kLog2E) + 1.0f;
+    s.sum = s.sum * expf(s.top - z) + 1.0f;
     s.top = z;
-  } else {
-    // -inf - -inf: nothing yet; NaN compares false and comes in here
-    s.sum += z == -INFINITY ? 0.0f : exp2f((z - s.top) * kLog2E);
+  } else {  // NaN compares false and comes in here
+    s.sum += expf(z - s.top);
   }
+}
+SPLAT_DEV Partial join_logits(Partial a, Partial b) {
+  const float top = fmaxf(a.top, b.top);  // NaN lies in the sums
+  return {top, a.sum * expf(a.top - top) + b.sum * expf(b.top - top)};
 }
 
 // Rows of logits (fp32, ld apart) -> lse and losses; a warp or a block to a row.
@@ -75,27 +51,41 @@ __global__ void __launch_bounds__(kThreads)
   const int r = BLOCK ? blockIdx.x : blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (r >= rows) return;
   const float* from = z + static_cast<long long>(r) * ld;
-  Partial s{-INFINITY, 0.0f};
+  Partial s{kLowest, 0.0f};
   for (int j = lane; j < p.vocabulary; j += lanes)
     take(s, from[j] + (bias ? to_float(bias[j]) : 0.0f));
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     const Partial other{__shfl_xor_sync(0xffffffffu, s.top, o),
                         __shfl_xor_sync(0xffffffffu, s.sum, o)};
-    s = join(s, other);
+    s = join_logits(s, other);
   }
   if constexpr (BLOCK) {
     __shared__ Partial all[kWarps];
     if ((threadIdx.x & 31) == 0) all[threadIdx.x >> 5] = s;
     __syncthreads();
     s = all[0];
-    for (int w = 1; w < kWarps; ++w) s = join(s, all[w]);
+    for (int w = 1; w < kWarps; ++w) s = join_logits(s, all[w]);
   }
   if (lane != 0) return;
   const float value = s.top + logf(s.sum);
   lse[first + r] = value;
   const int t = label_of(p, first + r);
   loss[first + r] = t < 0 ? 0.0f : value - (from[t] + (bias ? to_float(bias[t]) : 0.0f));
+}
+
+// The partial results of vocabulary_kernel -> lse and losses.
+__global__ void __launch_bounds__(kThreads)
+    join_partials_kernel(const Rows p, int partials, const Partial* from,
+                         const float* label_logits, float* lse, float* loss) {
+  const long long row = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x;
+  if (row >= p.rows) return;
+  Partial s = from[row];
+#pragma unroll 4
+  for (int i = 1; i < partials; ++i) s = join(s, from[i * p.rows + row]);
+  const float value = log_sum(s);
+  lse[row] = value;
+  loss[row] = label_of(p, row) < 0 ? 0.0f : value - label_logits[row];
 }
 
 // The losses' sum or mean and the number of rows that count, in doubles and in a fixed
@@ -143,11 +133,6 @@ __global__ void __launch_bounds__(kThreads)
 
 // ---- gradients -----------------------------------------------------------------------
 
-// Factors of the backward: of u_i on the way into dz, and of the products' results.
-struct Factors {
-  float in, out;
-};
-
 // The power of two that is not below any finite |u|.
 __global__ void __launch_bounds__(1024)
     factors_kernel(long long rows, int reduction, const float* upstream, const float* counted,
@@ -171,12 +156,6 @@ __global__ void __launch_bounds__(1024)
   e = min(max(e, -100), 126);
   factors->in = most ? __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * within : 0.0f;
   factors->out = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) / within;
-}
-
-SPLAT_DEV float upstream_of(const Rows& p, long long row, const float* upstream,
-                            const float* counted) {
-  const float u = upstream[p.reduction == kEach ? row : 0];
-  return p.reduction == kMean ? u / *counted : u;
 }
 
 // Logits -> dz of TO, rows ld_out apart; a warp or a block to a row.  May be in place.
@@ -224,15 +203,29 @@ __global__ void __launch_bounds__(kThreads)
   }
   sums[static_cast<long long>(blockIdx.y) * p.vocabulary + j] = sum;
 }
-// Adds a piece's ranges to the sums of the pieces before.
+// Adds a piece's ranges to the sums of the pieces before: eight threads to a column.
 __global__ void __launch_bounds__(kThreads)
     add_columns_kernel(int vocabulary, int ranges, const float* sums, bool begin, float* total) {
-  const int j = blockIdx.x * kThreads + threadIdx.x;
-  if (j >= vocabulary) return;
-  float sum = begin ? 0.0f : total[j];
+  const int j = blockIdx.x * 32 + threadIdx.x;
+  float sum = 0.0f;
+  if (j < vocabulary) {
 #pragma unroll 8
-  for (int r = 0; r < ranges; ++r) sum += sums[static_cast<long long>(r) * vocabulary + j];
+    for (int r = threadIdx.y; r < ranges; r += kWarps)
+      sum += sums[static_cast<long long>(r) * vocabulary + j];
+  }
+  __shared__ float all[kWarps][32];
+  all[threadIdx.y][threadIdx.x] = sum;
+  __syncthreads();
+  if (threadIdx.y || j >= vocabulary) return;
+  sum = begin ? 0.0f : total[j];
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) sum += all[w][threadIdx.x];
   total[j] = sum;
+}
+void add_columns(int vocabulary, int ranges, const float* sums, bool begin, float* total,
+                 cudaStream_t s) {
+  add_columns_kernel<<<host::blocks_for(vocabulary, 32), dim3(32, kWarps), 0, host::counted(s)>>>(
+      vocabulary, ranges, sums, begin, total);
 }
 
 // fp32 sums (of several splits, `stride` values apart) times the factor, rounded.
@@ -263,20 +256,59 @@ void finish(long long count, int splits, long long stride, const float* from,
 constexpr int kMostVocabulary = 1 << 20;
 constexpr long long kPieceBytes = 256LL << 20;
 
+// Whether the logits stay on the chip: fp32 ones would need planes of three parts, and
+// long rows several accumulators.
+template <class T>
+bool on_chip(int k) {
+  return sizeof(T) == 2 && k <= kMostAdditions * 16;
+}
+
 // The rows of a piece, and where its parts lie in the workspace.
 struct EntropyPlan {
+  bool on_chip;
   int piece, splits;
   long long split_rows;
+  // of vocabulary_kernel
+  int tile_n, tiles, ranges, tiles_per_range;
   size_t logits, dz, x_planes, w_planes, dz_planes, weight_sums, column_sums, column_total, dx,
-      losses, lse, loss_sums, factors, bytes;
+      losses, lse, loss_sums, factors, partials, label_logits, bytes;
 };
+
+// Ranges of words that make the busiest pair of blocks take the fewest tiles, a third of a
+// tile for each range's start among them.
+int word_ranges(int row_blocks, int tiles) {
+  const int pairs = std::max(1, host::sm_count() / 2);
+  int best = 1;
+  double least = 1e30;
+  for (int n = 1; n <= std::min(tiles, 64); ++n) {
+    const int per = (tiles + n - 1) / n;
+    const long long rounds = (static_cast<long long>(row_blocks) * n + pairs - 1) / pairs;
+    const double cost = rounds * (per + 0.3);
+    if (cost < least * 0.99) least = cost, best = n;
+  }
+  return best;
+}
 
 template <class T>
 EntropyPlan plan_entropy(long long rows, int k, int vocabulary, bool backward) {
   EntropyPlan plan{};
-  long long piece = std::max(1LL, kPieceBytes / 4 / vocabulary / kTileRows) * kTileRows;
-  piece = std::min({piece, rows, 1LL << 23});  // 65535 ranges of 256 rows, and below
+  plan.on_chip = on_chip<T>(k);
+  const int unit = plan.on_chip ? kPairRows : kTileRows;
+  long long piece;
+  if (plan.on_chip && !backward) {
+    piece = rows;
+  } else {
+    // bytes of a logit, or of a dz
+    const int size = plan.on_chip ? 2 : 4;
+    piece = std::max(1LL, kPieceBytes / size / vocabulary / unit) * unit;
+    piece = std::min({piece, rows, 1LL << 23});  // 65535 ranges of 256 rows, and below
+  }
   plan.piece = static_cast<int>(piece);
+  plan.tile_n = vocabulary <= 128 ? 128 : 256;
+  plan.tiles = (vocabulary + plan.tile_n - 1) / plan.tile_n;
+  plan.ranges = word_ranges(static_cast<int>((piece + kPairRows - 1) / kPairRows), plan.tiles);
+  plan.tiles_per_range = (plan.tiles + plan.ranges - 1) / plan.ranges;
+  plan.ranges = (plan.tiles + plan.tiles_per_range - 1) / plan.tiles_per_range;
   const auto take = [&](size_t n) {
     const size_t at = plan.bytes;
     plan.bytes += (n + 255) / 256 * 256;
@@ -284,12 +316,17 @@ EntropyPlan plan_entropy(long long rows, int k, int vocabulary, bool backward) {
   };
   plan.factors = take(sizeof(Factors));
   plan.loss_sums = take(sizeof(LossSum) * kLossBlocks);
-  plan.logits = take(4ull * piece * vocabulary);
-  plan.x_planes = take(plane_bytes<T>(piece, k));
-  plan.w_planes = take(plane_bytes<T>(vocabulary, k));
+  if (!plan.on_chip) plan.logits = take(4ull * piece * vocabulary);
+  // 16-bit rows that lie well need no planes, which their address decides
+  plan.x_planes = take(sizeof(T) == 2 && k % 8 == 0 ? 0 : plane_bytes<T>(piece, k));
+  plan.w_planes = take(sizeof(T) == 2 && k % 8 == 0 ? 0 : plane_bytes<T>(vocabulary, k));
   if (!backward) {
     plan.lse = take(4ull * rows);
     plan.losses = take(4ull * rows);
+    if (plan.on_chip) {
+      plan.partials = take(2ull * plan.ranges * rows * sizeof(Partial));
+      plan.label_logits = take(4ull * rows);
+    }
     return plan;
   }
   if (sizeof(T) == 2) plan.dz = take(2ull * piece * round_to(vocabulary, 8));
@@ -301,9 +338,36 @@ EntropyPlan plan_entropy(long long rows, int k, int vocabulary, bool backward) {
   plan.split_rows = round_to((piece + most - 1) / most, kChunk);
   plan.splits = static_cast<int>((piece + plan.split_rows - 1) / plan.split_rows);
   plan.weight_sums = take(4ull * plan.splits * vocabulary * k);
-  plan.column_sums = take(4ull * ((piece + kSumRows - 1) / kSumRows) * vocabulary);
+  plan.column_sums = take(plan.on_chip
+                              ? 4ull * round_to(piece, kPairRows) / 32 * vocabulary
+                              : 4ull * ((piece + kSumRows - 1) / kSumRows) * vocabulary);
   plan.column_total = take(4ull * vocabulary);
   return plan;
+}
+
+// What both launches of vocabulary_kernel share.
+template <class T, bool SLOPES>
+int launch_vocabulary(VocabularyParams& p, const EntropyPlan& plan, const Rows& r, long long first,
+                      int count, int k, const Planes& x, const Planes& w, const void* bias,
+                      cudaStream_t s) {
+  p.rows = r, p.first = first, p.count = count, p.k = k, p.bias = bias;
+  p.tile_n = plan.tile_n, p.tiles = plan.tiles;
+  p.row_blocks = static_cast<int>((count + static_cast<long long>(kPairRows) - 1) / kPairRows);
+  p.splits = plan.ranges, p.tiles_per_split = plan.tiles_per_range;
+  if (!make_map<T>(p.x_map, x.data, count, k, x.ld, 64, 128) ||
+      !make_map<T>(p.w_map, w.data, r.vocabulary, k, w.ld, 64, plan.tile_n / 2))
+    return host::fail(kInvalidArgument, "feature_entropy: operand maps");
+  const int fixed = 1024 + 4096 + (SLOPES ? 8 * 8192 : 0);
+  const int stage = 128 * 128 + plan.tile_n / 2 * 128;
+  p.stages = std::min(kPairStages, (kOneBlockBytes - fixed) / stage);
+  constexpr auto* kernel = vocabulary_kernel<T, SLOPES>;
+  if (!host::allow_shared<kernel>())
+    return host::check_launch("feature_entropy: shared memory");
+  const long long items = static_cast<long long>(p.row_blocks) * p.splits;
+  if (items >= 1LL << 31) return host::fail(kTooLarge, "feature_entropy: too many tiles");
+  const int pairs = static_cast<int>(std::min<long long>(items, host::sm_count() / 2));
+  kernel<<<2 * pairs, kPairThreads, fixed + p.stages * stage, host::counted(s)>>>(p);
+  return host::check_launch("feature_entropy");
 }
 
 // The logits of rows [first, first + rows).
@@ -333,9 +397,14 @@ int check_entropy(int dtype, long long rows, int k, int vocabulary, int id_bytes
     return host::fail(kInvalidArgument, "feature_entropy: targets are of 4 or 8 bytes");
   if (reduction < kEach || reduction > kMean)
     return host::fail(kInvalidArgument, "feature_entropy: reduction");
-  if (k > 65535 || vocabulary > kMostVocabulary || rows > 1LL << 31)
+  if (k > 65535 || vocabulary > kMostVocabulary || rows > (1LL << 31) - kPairRows)
     return host::fail(kTooLarge, "feature_entropy: too many rows, inputs or words");
   return kOk;
+}
+
+// Whether 16-bit rows that need no planes lie as the workspace's size takes them to.
+bool lies_well(int dtype, int k, const void* x, const void* weight) {
+  return dtype == kF32 || k % 8 || (host::aligned(x, 16) && host::aligned(weight, 16));
 }
 
 template <class T>
@@ -351,6 +420,19 @@ int launch_forward(const Rows& r, int k, const void* x, const void* weight, cons
     const int rows = static_cast<int>(std::min<long long>(plan.piece, r.rows - first));
     const Planes xs = split<T>(static_cast<const T*>(x) + first * k, rows, k,
                                ws + plan.x_planes, s);
+    if constexpr (sizeof(T) == 2) {
+      if (plan.on_chip) {  // all rows at once
+        VocabularyParams p{};
+        p.partials = reinterpret_cast<Partial*>(ws + plan.partials);
+        p.label_logits = reinterpret_cast<float*>(ws + plan.label_logits);
+        const int status =
+            launch_vocabulary<T, false>(p, plan, r, first, rows, k, xs, w, bias, s);
+        if (status != kOk) return status;
+        join_partials_kernel<<<host::blocks_for(rows, kThreads), kThreads, 0, host::counted(s)>>>(
+            r, 2 * plan.ranges, p.partials, p.label_logits, lse, each);
+        continue;
+      }
+    }
     const int status = launch_logits<T>(rows, k, vocabulary, xs, w, z, s);
     if (status != kOk) return status;
     by_row(rows, vocabulary, [&](auto block, int grid) {
@@ -391,26 +473,38 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
     const int rows = static_cast<int>(std::min<long long>(plan.piece, r.rows - first));
     const Planes xs = split<T>(static_cast<const T*>(x) + first * k, rows, k,
                                ws + plan.x_planes, s);
-    int status = launch_logits<T>(rows, k, vocabulary, xs, w, z, s);
+    Planes dz;
+    int status = kOk;
+    if constexpr (sizeof(T) == 2) {
+      dz.ld = static_cast<int>(round_to(vocabulary, 8));
+      dz.data = ws + plan.dz;
+      dz.rows = dz.plane_rows = rows;
+      if (plan.on_chip) {
+        VocabularyParams p{};
+        p.lse = lse, p.upstream = upstream, p.counted = counted, p.factors = factors;
+        if (dbias) p.column_sums = column_sums;
+        if (!make_map<T>(p.dz_map, dz.data, rows, vocabulary, dz.ld, 64, 32))
+          return host::fail(kInvalidArgument, "feature_entropy_backward: map");
+        status = launch_vocabulary<T, true>(p, plan, r, first, rows, k, xs, w, bias, s);
+        if (status != kOk) return status;
+        if (dbias)
+          add_columns(vocabulary, (rows + 31) / 32, column_sums, first == 0, column_total, s);
+      }
+    }
+    if (!plan.on_chip) status = launch_logits<T>(rows, k, vocabulary, xs, w, z, s);
     if (status != kOk) return status;
-    if (dbias) {
+    if (dbias && !plan.on_chip) {
       const int ranges = (rows + kSumRows - 1) / kSumRows;
       column_slopes_kernel<T>
           <<<dim3(host::blocks_for(vocabulary, kThreads), ranges), kThreads, 0,
              host::counted(s)>>>(r, first, rows, z, vocabulary, b, lse, upstream, counted,
                                  factors, column_sums);
-      add_columns_kernel<<<host::blocks_for(vocabulary, kThreads), kThreads, 0,
-                           host::counted(s)>>>(vocabulary, ranges, column_sums, first == 0,
-                                               column_total);
+      add_columns(vocabulary, ranges, column_sums, first == 0, column_total, s);
     }
     if (!dx && !dweight) continue;
-    Planes dz;
-    by_row(rows, vocabulary, [&](auto block, int grid) {
+    if (!plan.on_chip) by_row(rows, vocabulary, [&](auto block, int grid) {
       constexpr bool kBlock = decltype(block)::value;
       if constexpr (sizeof(T) == 2) {
-        dz.ld = static_cast<int>(round_to(vocabulary, 8));
-        dz.data = ws + plan.dz;
-        dz.rows = dz.plane_rows = rows;
         row_slope_kernel<T, T, kBlock><<<grid, kThreads, 0, host::counted(s)>>>(
             r, first, rows, z, vocabulary, b, lse, upstream, counted, factors,
             static_cast<T*>(dz.data), dz.ld);
@@ -479,6 +573,8 @@ int splat_feature_entropy(int dtype, long long rows, int k, int vocabulary, cons
     return host::fail(kInvalidArgument, "feature_entropy: workspace not 16-byte aligned");
   if (workspace_bytes < splat_feature_entropy_workspace_bytes(dtype, rows, k, vocabulary, 0))
     return host::fail(kWorkspaceTooSmall, "feature_entropy: workspace");
+  if (!lies_well(dtype, k, x, weight))
+    return host::fail(kInvalidArgument, "feature_entropy: x and weight must be 16-byte aligned");
   Rows r{rows, vocabulary, id_bytes, reduction, ignored, target, host::device_error_word()};
   if (!r.error) return kCudaError;
   return SPLAT_FEATURE_TYPE(dtype, [&] {
@@ -503,6 +599,8 @@ int splat_feature_entropy_backward(int dtype, long long rows, int k, int vocabul
                       "feature_entropy_backward: workspace not 16-byte aligned");
   if (workspace_bytes < splat_feature_entropy_workspace_bytes(dtype, rows, k, vocabulary, 1))
     return host::fail(kWorkspaceTooSmall, "feature_entropy_backward: workspace");
+  if (!lies_well(dtype, k, x, weight))
+    return host::fail(kInvalidArgument, "feature_entropy_backward: x and weight must be 16-byte aligned");
   Rows r{rows, vocabulary, id_bytes, reduction, ignored, target, host::device_error_word()};
   if (!r.error) return kCudaError;
   return SPLAT_FEATURE_TYPE(dtype, [&] {

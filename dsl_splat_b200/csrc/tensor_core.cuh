@@ -84,6 +84,7 @@ SPLAT_DEV void copy_out(const CUtensorMap* map, int column, int row, uint32_t sr
                : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
+SPLAT_DEV void copy_out_none() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // Contiguous bytes (a multiple of 16, both addresses 16-byte aligned).
 SPLAT_DEV void bulk_in(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile(
@@ -91,6 +92,11 @@ SPLAT_DEV void bulk_in(uint32_t dst, const void* src, uint32_t bytes, uint32_t b
           "r"(dst),
       "l"(src), "r"(bytes), "r"(bar)
       : "memory");
+}
+// Until the sources of this thread's copy_outs, but for the last N, may be written again.
+template <int N>
+SPLAT_DEV void copies_out_read_but() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
 // Until the sources of this thread's copy_outs may be written again.
 SPLAT_DEV void copies_out_read() {
@@ -229,6 +235,95 @@ SPLAT_DEV void commit(uint32_t elected, uint32_t bar) {
       "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
           bar),
       "r"(elected)
+      : "memory");
+}
+
+// ---- pairs of blocks -----------------------------------------------------------
+
+// A cluster of two blocks works on one product: 256 rows of A, of which each holds 128, and n
+// rows of B, of which each holds half.  The block of rank 0 issues; each finds the results
+// of its own rows in its tensor memory.
+SPLAT_DEV uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// The address that this block's shared memory has in the block of the given rank.
+SPLAT_DEV uint32_t address_in(uint32_t address, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(address), "r"(rank));
+  return r;
+}
+// All threads of both blocks.
+SPLAT_DEV void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+SPLAT_DEV void barrier_arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+               : "memory");
+}
+SPLAT_DEV bool barrier_poll_pair(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity), "r"(kPollSleep)
+      : "memory");
+  return done;
+}
+// barrier_wait for a barrier of this block that the other one arrives at too.
+SPLAT_DEV bool barrier_wait_pair(uint32_t bar, uint32_t parity) {
+  if (barrier_poll_pair(bar, parity)) return true;
+  const unsigned long long start = nanoseconds();
+  while (!barrier_poll_pair(bar, parity))
+    if (nanoseconds() - start > kWaitLimit) return false;
+  return true;
+}
+// copy_in whose barrier may lie in the other block.
+SPLAT_DEV void copy_in_pair(uint32_t dst, const CUtensorMap* map, int column, int row,
+                            uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(column), "r"(row), "r"(bar)
+      : "memory");
+}
+SPLAT_DEV void tmem_alloc_pair(uint32_t where, uint32_t columns) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where),
+               "r"(columns)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+}
+SPLAT_DEV void tmem_free_pair(uint32_t address, uint32_t columns) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(address),
+               "r"(columns));
+}
+__host__ __device__ constexpr uint32_t instruction_pair(bool is_bf16, bool a_mn, bool b_mn,
+                                                        int n) {
+  return (instruction(is_bf16, a_mn, b_mn, n) & ~(0x1fu << 24)) | ((256u >> 4) << 24);
+}
+SPLAT_DEV void mma_pair(uint32_t elected, uint32_t d, uint64_t a, uint64_t b,
+                        uint32_t instruction, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(instruction), "r"(static_cast<uint32_t>(accumulate)), "r"(elected)
+      : "memory");
+}
+// The barriers at this address in both blocks get an arrival when all earlier products of
+// this lane are done.
+SPLAT_DEV void commit_pair(uint32_t elected, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %2;\n\t}" ::"r"(bar),
+      "r"(elected), "h"(static_cast<unsigned short>(3))
       : "memory");
 }
 
