@@ -266,8 +266,8 @@ bool on_chip(int k) {
 // The rows of a piece, and where its parts lie in the workspace.
 struct EntropyPlan {
   bool on_chip;
-  int piece, splits;
-  long long split_rows;
+  int piece;
+  PairSplits dx_splits, dw_splits;
   // of vocabulary_kernel
   int tile_n, tiles, ranges, tiles_per_range;
   size_t logits, dz, x_planes, w_planes, dz_planes, weight_sums, column_sums, column_total, dx,
@@ -304,7 +304,7 @@ EntropyPlan plan_entropy(long long rows, int k, int vocabulary, bool backward) {
     piece = std::min({piece, rows, 1LL << 23});  // 65535 ranges of 256 rows, and below
   }
   plan.piece = static_cast<int>(piece);
-  plan.tile_n = vocabulary <= 128 ? 128 : 256;
+  plan.tile_n = pair_tile_n(vocabulary);
   plan.tiles = (vocabulary + plan.tile_n - 1) / plan.tile_n;
   plan.ranges = word_ranges(static_cast<int>((piece + kPairRows - 1) / kPairRows), plan.tiles);
   plan.tiles_per_range = (plan.tiles + plan.ranges - 1) / plan.ranges;
@@ -324,20 +324,28 @@ EntropyPlan plan_entropy(long long rows, int k, int vocabulary, bool backward) {
     plan.lse = take(4ull * rows);
     plan.losses = take(4ull * rows);
     if (plan.on_chip) {
-      plan.partials = take(2ull * plan.ranges * rows * sizeof(Partial));
+      plan.partials = take(plan.tile_n / 64 * static_cast<size_t>(plan.ranges) * rows *
+                           sizeof(Partial));
       plan.label_logits = take(4ull * rows);
     }
     return plan;
   }
   if (sizeof(T) == 2) plan.dz = take(2ull * piece * round_to(vocabulary, 8));
   else plan.dz_planes = take(plane_bytes<T>(piece, vocabulary));
-  plan.dx = take(4ull * piece * k);
-  const long long tiles = ((vocabulary + 127LL) / 128) * ((k + 127) / 128);
-  const long long wanted = std::max(1LL, 2LL * host::sm_count() / tiles);
-  const long long most = std::min(wanted, (piece + 511) / 512);
-  plan.split_rows = round_to((piece + most - 1) / most, kChunk);
-  plan.splits = static_cast<int>((piece + plan.split_rows - 1) / plan.split_rows);
-  plan.weight_sums = take(4ull * plan.splits * vocabulary * k);
+  // ranges of words for dx and of rows for dW, whose sums are joined
+  if (plan.on_chip) {
+    plan.dx_splits = pair_splits(pair_tiles(piece, k), vocabulary);
+    plan.dw_splits = pair_splits(pair_tiles(vocabulary, k), piece);
+  } else {
+    const long long tiles = ((vocabulary + 127LL) / 128) * ((k + 127) / 128);
+    const long long wanted = std::max(1LL, 2LL * host::sm_count() / tiles);
+    const long long most = std::min(wanted, (piece + 511) / 512);
+    plan.dx_splits = {1, vocabulary};
+    plan.dw_splits.k = round_to((piece + most - 1) / most, kChunk);
+    plan.dw_splits.count = static_cast<int>((piece + plan.dw_splits.k - 1) / plan.dw_splits.k);
+  }
+  plan.dx = take(4ull * plan.dx_splits.count * piece * k);
+  plan.weight_sums = take(4ull * plan.dw_splits.count * vocabulary * k);
   plan.column_sums = take(plan.on_chip
                               ? 4ull * round_to(piece, kPairRows) / 32 * vocabulary
                               : 4ull * ((piece + kSumRows - 1) / kSumRows) * vocabulary);
@@ -357,8 +365,8 @@ int launch_vocabulary(VocabularyParams& p, const EntropyPlan& plan, const Rows& 
   if (!make_map<T>(p.x_map, x.data, count, k, x.ld, 64, 128) ||
       !make_map<T>(p.w_map, w.data, r.vocabulary, k, w.ld, 64, plan.tile_n / 2))
     return host::fail(kInvalidArgument, "feature_entropy: operand maps");
-  const int fixed = 1024 + 4096 + (SLOPES ? 8 * 8192 : 0);
-  const int stage = 128 * 128 + plan.tile_n / 2 * 128;
+  const int fixed = 1024 + kVocabularyWarps * (256 + (SLOPES ? 4096 : 0));
+  const int stage = kAPlane + plan.tile_n / 2 * 128;
   p.stages = std::min(kPairStages, (kOneBlockBytes - fixed) / stage);
   constexpr auto* kernel = vocabulary_kernel<T, SLOPES>;
   if (!host::allow_shared<kernel>())
@@ -366,7 +374,7 @@ int launch_vocabulary(VocabularyParams& p, const EntropyPlan& plan, const Rows& 
   const long long items = static_cast<long long>(p.row_blocks) * p.splits;
   if (items >= 1LL << 31) return host::fail(kTooLarge, "feature_entropy: too many tiles");
   const int pairs = static_cast<int>(std::min<long long>(items, host::sm_count() / 2));
-  kernel<<<2 * pairs, kPairThreads, fixed + p.stages * stage, host::counted(s)>>>(p);
+  kernel<<<2 * pairs, kVocabularyThreads, fixed + p.stages * stage, host::counted(s)>>>(p);
   return host::check_launch("feature_entropy");
 }
 
@@ -429,7 +437,7 @@ int launch_forward(const Rows& r, int k, const void* x, const void* weight, cons
             launch_vocabulary<T, false>(p, plan, r, first, rows, k, xs, w, bias, s);
         if (status != kOk) return status;
         join_partials_kernel<<<host::blocks_for(rows, kThreads), kThreads, 0, host::counted(s)>>>(
-            r, 2 * plan.ranges, p.partials, p.label_logits, lse, each);
+            r, plan.tile_n / 64 * plan.ranges, p.partials, p.label_logits, lse, each);
         continue;
       }
     }
@@ -515,28 +523,42 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
     });
     if constexpr (sizeof(T) == 4) dz = split<T>(z, rows, vocabulary, ws + plan.dz_planes, s);
     if (dx) {
-      ProductParams p{};
-      p.m = rows, p.k = vocabulary, p.n = k;
-      use_planes(p, dz, w);
-      p.k_per_split = vocabulary, p.splits = 1;
-      p.out = dx_sums;
-      status = launch_product<T, P, false, T, P, true, float, float, kPlain>(p, s);
+      if (plan.on_chip) {
+        if constexpr (sizeof(T) == 2)
+          status = launch_pairs<T, false, true>(rows, k, vocabulary, dz.data, dz.ld, w.data, w.ld,
+                                                plan.dx_splits, dx_sums, false, s);
+      } else {
+        ProductParams p{};
+        p.m = rows, p.k = vocabulary, p.n = k;
+        use_planes(p, dz, w);
+        p.k_per_split = vocabulary, p.splits = 1;
+        p.out = dx_sums;
+        status = launch_product<T, P, false, T, P, true, float, float, kPlain>(p, s);
+      }
       if (status != kOk) return status;
-      finish<T>(static_cast<long long>(rows) * k, 1, 0, dx_sums, factors,
+      const long long values = static_cast<long long>(rows) * k;
+      finish<T>(values, plan.dx_splits.count, values, dx_sums, factors,
                 static_cast<T*>(dx) + first * k, s);
     }
     if (dweight) {
-      ProductParams p{};
-      p.m = vocabulary, p.k = rows, p.n = k;
-      use_planes(p, dz, xs);
       // a last, shorter piece has fewer splits
-      p.k_per_split = plan.split_rows;
-      p.splits = static_cast<int>((rows + plan.split_rows - 1) / plan.split_rows);
-      p.accumulate = first != 0;
-      p.out = weight_sums;
-      status = launch_product<T, P, true, T, P, true, float, float, kPlain>(p, s);
+      PairSplits dw = plan.dw_splits;
+      dw.count = static_cast<int>((rows + dw.k - 1) / dw.k);
+      if (plan.on_chip) {
+        if constexpr (sizeof(T) == 2)
+          status = launch_pairs<T, true, true>(vocabulary, k, rows, dz.data, dz.ld, xs.data,
+                                               xs.ld, dw, weight_sums, first != 0, s);
+      } else {
+        ProductParams p{};
+        p.m = vocabulary, p.k = rows, p.n = k;
+        use_planes(p, dz, xs);
+        p.k_per_split = dw.k, p.splits = dw.count;
+        p.accumulate = first != 0;
+        p.out = weight_sums;
+        status = launch_product<T, P, true, T, P, true, float, float, kPlain>(p, s);
+      }
       if (status != kOk) return status;
-      splits = std::max(splits, p.splits);
+      splits = std::max(splits, dw.count);
     }
   }
   const long long weights = static_cast<long long>(vocabulary) * k;

@@ -6,21 +6,22 @@
 //
 // A pair of blocks (tensor_core.cuh) takes 256 rows x 256 words: per SM, a chunk of 64 k
 // is 16 KB of x and 16 KB of W, half of what two blocks on their own would read from the
-// L2.  In each block one thread starts the tensor copies, and eight epilogue warps read
-// the finished accumulators (two of 256 columns, all of the tensor memory); the leading
-// block's product warp issues.  A pair stays with 256 rows over a range of words, so that
-// a row's running maximum and sum stay in a thread's registers; ranges and column halves
-// leave a partial result each, joined in a fixed order.  Exponentials take the
+// L2.  In each block one thread starts the tensor copies, and sixteen epilogue warps read
+// the finished accumulators (two of 256 columns, all of the tensor memory), 64 words of 32
+// rows each, and give them back before they work on them; the leading block's product warp
+// issues.  A pair stays with 256 rows over a range of words, so that a row's running maximum
+// and sum stay in a thread's registers; ranges and quarters of the columns leave a
+// partial result each, joined in a fixed order.  Exponentials take the
 // special-function pipe 2048 cycles a tile, the products 8 a k: the pipe binds below 256
 // features, the tensor core above.
 #pragma once
-#include "feature_product.cuh"
+#include "feature_pairs.cuh"
 
 namespace splat {
 namespace feature {
 
-constexpr int kPairRows = 256, kPairThreads = 320;  // eight epilogue warps, copies, products
-constexpr int kPairStages = 8;
+constexpr int kVocabularyWarps = 16;  // of the epilogue
+constexpr int kVocabularyThreads = 32 * kVocabularyWarps + 64;
 constexpr float kLog2E = 1.44269504088896341f;
 
 // What the rows' kernels read.
@@ -72,11 +73,11 @@ struct VocabularyParams {
   Rows rows;           // of all pieces
   long long first;     // row of the piece
   int count;           // its rows
-  int k, tile_n;       // 128 or 256 words
+  int k, tile_n;       // 64, 128 or 256 words
   int tiles, row_blocks, splits, tiles_per_split;
   int stages;
   const void* bias;
-  // statistics: (splits, 2, count), and the labels' logits (count)
+  // statistics: (splits, tile_n / 64, count), and the labels' logits (count)
   Partial* partials;
   float* label_logits;
   // slopes
@@ -86,123 +87,60 @@ struct VocabularyParams {
 };
 
 template <class T, bool SLOPES>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVocabularyThreads, 1)
     vocabulary_kernel(const __grid_constant__ VocabularyParams p) {
   extern __shared__ unsigned char dynamic[];
-  __shared__ alignas(8) unsigned long long full[kPairStages], empty[kPairStages], acc_full[2],
-      acc_empty[2], drained;
-  __shared__ uint32_t tmem_base;
+  __shared__ PairBarriers barriers;
   const uint32_t base = (tc::shared_address(dynamic) + 1023u) & ~1023u;
   const int warp = tc::uniform(threadIdx.x >> 5);
   const uint32_t rank = tc::cluster_rank();
-  const int half_n = p.tile_n / 2;
-  const uint32_t stage_bytes = 128 * 128 + half_n * 128;
+  const int half_n = p.tile_n / 2, groups = p.tile_n / 64;
+  const uint32_t stage_bytes = kAPlane + half_n * 128;
   // patches of the epilogue warps, their words' biases, the ring
-  const uint32_t bias_at = base + (SLOPES ? 8 * 8192 : 0), ring = bias_at + 4096;
-  const int chunks = (p.k + 63) / 64;
-  constexpr uint32_t kColumns = 512;
-
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < p.stages; ++i) {
-      tc::barrier_init(tc::shared_address(&full[i]), 1);
-      tc::barrier_init(tc::shared_address(&empty[i]), 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      tc::barrier_init(tc::shared_address(&acc_full[i]), 1);
-      tc::barrier_init(tc::shared_address(&acc_empty[i]), 16);  // epilogue warps of the pair
-    }
-    tc::barrier_init(tc::shared_address(&drained), 1);
-    tc::barrier_init_fence();
-  }
-  if (warp == 0) tc::tmem_alloc_pair(tc::shared_address(&tmem_base), kColumns);
-  tc::fence_before_sync();
-  __syncthreads();
-  tc::cluster_sync();
-  tc::fence_after_sync();
-  const uint32_t tmem = tc::uniform(tmem_base);
+  const uint32_t bias_at = base + (SLOPES ? kVocabularyWarps * 4096 : 0);
+  const uint32_t ring_at = bias_at + kVocabularyWarps * 256;
+  const uint32_t tmem = pair_begin(barriers, p.stages, 8 * groups);
   const int items = p.row_blocks * p.splits;
   const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
   bool ok = true;
 
-  if (warp == 8) {
-    // ---- copies
+  if (warp == kVocabularyWarps) {
     if ((threadIdx.x & 31) == 0) {
-      int stage = 0, started = 0;
-      uint32_t parity = 1;  // a fresh barrier's previous phase counts as complete
+      PairRing ring(barriers, ring_at, stage_bytes, p.stages, rank);
       for (int item = pair; item < items && ok; item += pairs) {
         const int block = item % p.row_blocks, split = item / p.row_blocks;
         const int t1 = min((split + 1) * p.tiles_per_split, p.tiles);
         const int row = block * kPairRows + rank * 128;
         for (int t = split * p.tiles_per_split; t < t1 && ok; ++t)
-          for (int c = 0; c < chunks; ++c) {
-            if (!(ok = tc::barrier_wait(tc::shared_address(&empty[stage]), parity))) break;
-            const uint32_t at = ring + stage * stage_bytes;
-            // both blocks' copies are told to the leading one's barrier
-            const uint32_t own = tc::shared_address(&full[stage]);
-            if (rank == 0) tc::barrier_expect(own, 2 * stage_bytes);
-            const uint32_t bar = tc::address_in(own, 0);
-            tc::copy_in_pair(at, &p.x_map, c * 64, row, bar);
-            tc::copy_in_pair(at + 128 * 128, &p.w_map, c * 64, t * p.tile_n + rank * half_n, bar);
-            started = max(started, stage + 1);
-            if (++stage == p.stages) stage = 0, parity ^= 1;
-          }
+          for (int k = 0; k < p.k && ok; k += kChunk)
+            ok = ring.fill([&](uint32_t at, uint32_t bar) {
+              tc::copy_in_pair(at, &p.x_map, k, row, bar);
+              tc::copy_in_pair(at + kAPlane, &p.w_map, k, t * p.tile_n + rank * half_n, bar);
+            });
       }
-      // no copy of either block is in flight past the pair's last barrier, also after a
-      // wait that ran out: parity ^ 1 is the phase of the ring's current round, parity the
-      // last one's
-      if (rank == 0)
-        for (int i = 0; i < started; ++i)
-          ok = tc::barrier_wait_pair(tc::shared_address(&full[i]),
-                                     i < stage ? parity ^ 1 : parity) && ok;
+      ok = ring.drain() && ok;
     }
-  } else if (warp == 9) {
-    // ---- products
+  } else if (warp == kVocabularyWarps + 1) {
     if (rank == 0) {
-      const uint32_t lead = tc::elected();
-      const uint32_t instruction = tc::instruction_pair(!kIsF16<T>, false, false, p.tile_n);
-      int stage = 0;
-      uint32_t parity = 0, n = 0;  // accumulators filled
+      PairIssue issue(barriers, ring_at, stage_bytes, p.stages, tmem,
+                      tc::instruction_pair(!kIsF16<T>, false, false, p.tile_n));
       for (int item = pair; item < items && ok; item += pairs) {
         const int split = item / p.row_blocks;
         const int t1 = min((split + 1) * p.tiles_per_split, p.tiles);
-        for (int t = split * p.tiles_per_split; t < t1 && ok; ++t, ++n) {
-          const uint32_t acc = n & 1;
-          if (!(ok = tc::barrier_wait_pair(tc::shared_address(&acc_empty[acc]),
-                                           ((n >> 1) & 1) ^ 1)))
-            break;
-          tc::fence_after_sync();
-          const uint32_t d = tmem + acc * 256;
-          for (int c = 0; c < chunks; ++c) {
-            if (!(ok = tc::barrier_wait_pair(tc::shared_address(&full[stage]), parity))) break;
-            tc::fence_after_sync();
-            const uint32_t at = ring + stage * stage_bytes;
-            uint64_t a = tc::descriptor_k_major(at), b = tc::descriptor_k_major(at + 128 * 128);
-            const int steps = (min(p.k - c * 64, 64) + 15) / 16;
-#pragma unroll 4
-            for (int s = 0; s < steps; ++s) {
-              tc::mma_pair(lead, d, a, b, instruction, c > 0 || s > 0);
-              a += tc::kStepK >> 4;
-              b += tc::kStepK >> 4;
-            }
-            tc::commit_pair(lead, tc::shared_address(&empty[stage]));
-            if (++stage == p.stages) stage = 0, parity ^= 1;
-          }
-          tc::commit_pair(lead, tc::shared_address(&acc_full[acc]));
-        }
+        for (int t = split * p.tiles_per_split; t < t1 && ok; ++t)
+          ok = issue.template tile<false, false>(p.k);
       }
-      // whichever way the loop ended, no product is in flight past this point
-      tc::commit_pair(lead, tc::shared_address(&drained));
-      ok = tc::barrier_wait(tc::shared_address(&drained), 0) && ok;
+      ok = issue.drain() && ok;
     }
-  } else {
-    // ---- epilogue: a thread to a row, four warps to half of the columns
-    const int lane = threadIdx.x & 31, lane_block = warp & 3, half = warp >> 2;
+  } else if (warp < 4 * groups) {
+    // a thread to a row, a warp to 64 of the tile's words
+    const int lane = threadIdx.x & 31, lane_block = warp & 3, group = warp >> 2;
     const T* bias = static_cast<const T*>(p.bias);
     const int V = p.rows.vocabulary;
     float* own_bias = reinterpret_cast<float*>(
-        dynamic + (bias_at - tc::shared_address(dynamic)) + warp * 512);
-    uint32_t n = 0;       // accumulators read
-    uint32_t patches = 0;  // written
+        dynamic + (bias_at - tc::shared_address(dynamic)) + warp * 256);
+    const uint32_t patch = base + warp * 4096;
+    uint32_t read = 0;  // accumulators
     for (int item = pair; item < items && ok; item += pairs) {
       const int block = item % p.row_blocks, split = item / p.row_blocks;
       const int t1 = min((split + 1) * p.tiles_per_split, p.tiles);
@@ -216,126 +154,112 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         less = p.lse[p.first + row] * kLog2E;
         u = upstream_of(p.rows, p.first + row, p.upstream, p.counted) * p.factors->in;
       }
-      for (int t = split * p.tiles_per_split; t < t1; ++t, ++n) {
-        const uint32_t acc = n & 1;
-        const int col0 = t * p.tile_n + half * half_n;  // of this warp
-        const bool with_bias = bias || col0 + half_n > V;
+      for (int t = split * p.tiles_per_split; t < t1; ++t, ++read) {
+        const uint32_t acc = read & 1;
+        const int col0 = t * p.tile_n + group * 64;  // of this warp
+        const bool with_bias = bias || col0 + 64 > V;
         if (with_bias) {
           // in units of log 2; words behind the last have minus infinity
           __syncwarp();  // the tile before has been read
-          for (int j = lane; j < half_n; j += 32)
+#pragma unroll
+          for (int j = lane; j < 64; j += 32)
             own_bias[j] = col0 + j >= V ? -INFINITY
                           : bias        ? to_float(bias[col0 + j]) * kLog2E
                                         : 0.0f;
           __syncwarp();
         }
-        if (!(ok = tc::barrier_wait(tc::shared_address(&acc_full[acc]), (n >> 1) & 1))) break;
+        if (!(ok = tc::barrier_wait(tc::shared_address(&barriers.acc_full[acc]), (read >> 1) & 1)))
+          break;
         tc::fence_after_sync();
-        for (int c = 0; c < half_n; c += 32) {
-          float v[32];
-          tc::tmem_load32(tmem + (lane_block << 21) + acc * 256 + half * half_n + c, v);
-          if (with_bias) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 b = *reinterpret_cast<const float4*>(own_bias + c + j);
-              v[j] = fmaf(v[j], kLog2E, b.x);
-              v[j + 1] = fmaf(v[j + 1], kLog2E, b.y);
-              v[j + 2] = fmaf(v[j + 2], kLog2E, b.z);
-              v[j + 3] = fmaf(v[j + 3], kLog2E, b.w);
-            }
-          }
-          const int at = label - (col0 + c);  // of the label among these words
-          const bool hit = at >= 0 && at < 32;
-          if constexpr (!SLOPES) {
-            if (__any_sync(0xffffffffu, hit)) {
-              float z = 0.0f;
-#pragma unroll
-              for (int j = 0; j < 32; ++j) z = j == at ? v[j] : z;
-              if (hit) p.label_logits[row] = with_bias ? z * 0.693147180559945309f : z;
-            }
-            float most = v[0];
-#pragma unroll
-            for (int j = 1; j < 32; ++j) most = fmaxf(most, v[j]);
-            if (!with_bias) most *= kLog2E;
-            if (most > s.top) {
-              s.sum *= exp2f(s.top - most);
-              s.top = most;
-            }
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (with_bias) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) sum[j & 3] += fast_exp2(v[j] - s.top);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) sum[j & 3] += fast_exp2(fmaf(v[j], kLog2E, -s.top));
-            }
-            s.sum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          } else {
-            if (with_bias) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = fast_exp2(v[j] - less);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = fast_exp2(fmaf(v[j], kLog2E, -less));
-            }
-            if (__any_sync(0xffffffffu, hit)) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = j == at ? v[j] - 1.0f : v[j];
-            }
-            // rows that do not count have no gradient, whatever their logits are
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = label < 0 ? 0.0f : v[j] * u;
-            // a patch of 32 rows and 64 words for a tensor copy, in two steps
-            const uint32_t patch = base + warp * 8192 + (patches & 1) * 4096;
-            if (!(c & 32)) {
-              if (lane == 0) tc::copies_out_read_but<1>();
-              __syncwarp();
-            }
-#pragma unroll
-            for (int piece = 0; piece < 4; ++piece) {
-              const Vec<T, 8> r = round_values<T, 8>(reinterpret_cast<const float(&)[8]>(v[piece * 8]));
-              const uint32_t to = patch + lane * 128 +
-                                  ((((c & 32) >> 3) + piece) ^ (lane & 7)) * 16;
-              const uint4& w = reinterpret_cast<const uint4&>(r);
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w.x),
-                           "r"(w.y), "r"(w.z), "r"(w.w)
-                           : "memory");
-            }
-            if (c & 32) {
-              tc::fence_async_proxy();
-              __syncwarp();
-              if (lane == 0) {
-                // patches without a copy count too, see copies_out_read_but
-                if (row0 < p.count && col0 + c - 32 < V)
-                  tc::copy_out(&p.dz_map, col0 + c - 32, row0, patch);
-                else
-                  tc::copy_out_none();
-              }
-              ++patches;
-            }
-            if (p.column_sums) {  // before dz is rounded
-              const float sum = sum_rows<32>(v);
-              if (row0 < p.count && col0 + c + lane < V)
-                p.column_sums[static_cast<long long>(row0 / 32) * V + col0 + c + lane] = sum;
-            }
-          }
-        }
+        float v[64];
+        tc::tmem_load64(tmem + (lane_block << 21) + acc * 256 + group * 64, v);
         tc::fence_before_sync();
         __syncwarp();
         if (lane == 0)
-          tc::barrier_arrive_remote(tc::address_in(tc::shared_address(&acc_empty[acc]), 0));
+          tc::barrier_arrive_remote(
+              tc::address_in(tc::shared_address(&barriers.acc_empty[acc]), 0));
+        if (with_bias) {
+#pragma unroll
+          for (int j = 0; j < 64; j += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(own_bias + j);
+            v[j] = fmaf(v[j], kLog2E, b.x);
+            v[j + 1] = fmaf(v[j + 1], kLog2E, b.y);
+            v[j + 2] = fmaf(v[j + 2], kLog2E, b.z);
+            v[j + 3] = fmaf(v[j + 3], kLog2E, b.w);
+          }
+        }
+        const int at = label - col0;  // of the label among these words
+        const bool hit = at >= 0 && at < 64;
+        if constexpr (!SLOPES) {
+          if (__any_sync(0xffffffffu, hit)) {
+            float z = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 64; ++j) z = j == at ? v[j] : z;
+            if (hit) p.label_logits[row] = with_bias ? z * 0.693147180559945309f : z;
+          }
+          float most[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+          for (int j = 4; j < 64; ++j) most[j & 3] = fmaxf(most[j & 3], v[j]);
+          most[0] = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+          if (!with_bias) most[0] *= kLog2E;
+          if (most[0] > s.top) {
+            s.sum *= exp2f(s.top - most[0]);
+            s.top = most[0];
+          }
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          if (with_bias) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) sum[j & 3] += fast_exp2(v[j] - s.top);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) sum[j & 3] += fast_exp2(fmaf(v[j], kLog2E, -s.top));
+          }
+          s.sum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        } else {
+          if (with_bias) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) v[j] = fast_exp2(v[j] - less);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) v[j] = fast_exp2(fmaf(v[j], kLog2E, -less));
+          }
+          if (__any_sync(0xffffffffu, hit)) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) v[j] = j == at ? v[j] - 1.0f : v[j];
+          }
+          // rows that do not count have no gradient, whatever their logits are
+#pragma unroll
+          for (int j = 0; j < 64; ++j) v[j] = label < 0 ? 0.0f : v[j] * u;
+          if (p.column_sums) {  // before dz is rounded
+            float* sums = p.column_sums + static_cast<long long>(row0 / 32) * V + col0 + lane;
+#pragma unroll
+            for (int c = 0; c < 64; c += 32) {
+              const float sum = sum_rows<32>(reinterpret_cast<const float(&)[32]>(v[c]));
+              if (row0 < p.count && col0 + c + lane < V) sums[c] = sum;
+            }
+          }
+          // a patch of 32 rows and 64 words for a tensor copy
+          if (lane == 0) tc::copies_out_read();
+          __syncwarp();
+#pragma unroll
+          for (int piece = 0; piece < 8; ++piece) {
+            const Vec<T, 8> r =
+                round_values<T, 8>(reinterpret_cast<const float(&)[8]>(v[piece * 8]));
+            store_shared(patch + lane * 128 + ((piece ^ (lane & 7)) << 4),
+                         reinterpret_cast<const uint4&>(r));
+          }
+          tc::fence_async_proxy();
+          __syncwarp();
+          if (lane == 0 && row0 < p.count && col0 < V)
+            tc::copy_out(&p.dz_map, col0, row0, patch);
+        }
       }
       if (!SLOPES && here)
-        p.partials[static_cast<long long>(split * 2 + half) * p.count + row] = s;
+        p.partials[static_cast<long long>(split * groups + group) * p.count + row] = s;
     }
     if (SLOPES && lane == 0) tc::copies_out_read();
   }
-  if (!ok) atomicCAS(p.rows.error, 0, kDeviceTimeout);
-  tc::fence_before_sync();
-  __syncthreads();
-  __syncwarp();
-  tc::cluster_sync();
-  if (warp == 0) tc::tmem_free_pair(tmem, kColumns);
+  pair_end(tmem, ok, p.rows.error);
 }
 
 }  // namespace feature
