@@ -1,12 +1,12 @@
 // Softmax cross entropy of a linear head over a vocabulary:
 //
-//   z = x W^T + b,  lse_i = log sum_j exp z_ij,  l_i = lse_i - z_i,t_i
-//   dz_ij = u_i (exp(z_ij - lse_i) - [j = t_i]),  dx = dz W,  dW = dz^T x,  db = sum_i dz_i
+//   z = x W^T + b,  l_i = log sum_j exp z_ij - z_i,t_i
+//   dz_ij = u_i (exp(z_ij) / sum_k exp z_ik - [j = t_i])
+//   dx = dz W,  dW = dz^T x,  db = sum_i dz_i
 //
-// The logits are never kept.  Those of 16-bit types never leave the chip
-// (feature_vocabulary.cuh); those of fp32, whose products take planes of three parts, are
-// formed for a piece of the rows at a time.  The backward forms them again, and dz for
-// a piece of the rows.  u_i is the upstream gradient of row i's loss (divided by
+// The logits are never kept.  They never leave the chip (feature_vocabulary.cuh) but those of
+// rows so long that they take several accumulators, which are formed for a piece of the
+// rows at a time.  The backward forms them again, and dz for a piece of the rows.  u_i is the upstream gradient of row i's loss (divided by
 // the number of rows that count for their mean) and 0 for the others.
 //
 // dz is held in T for the products.  It is taken relative to the power of two E that
@@ -42,11 +42,11 @@ SPLAT_DEV Partial join_logits(Partial a, Partial b) {
   return {top, a.sum * expf(a.top - top) + b.sum * expf(b.top - top)};
 }
 
-// Rows of logits (fp32, ld apart) -> lse and losses; a warp or a block to a row.
+// Rows of logits (fp32, ld apart) -> moments and losses; a warp or a block to a row.
 template <class T, bool BLOCK>
 __global__ void __launch_bounds__(kThreads)
     row_loss_kernel(const Rows p, long long first, int rows, const float* z, int ld,
-                    const T* bias, float* lse, float* loss) {
+                    const T* bias, Partial* moments, float* loss) {
   const int lane = BLOCK ? threadIdx.x : threadIdx.x & 31, lanes = BLOCK ? kThreads : 32;
   const int r = BLOCK ? blockIdx.x : blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (r >= rows) return;
@@ -68,24 +68,27 @@ __global__ void __launch_bounds__(kThreads)
     for (int w = 1; w < kWarps; ++w) s = join_logits(s, all[w]);
   }
   if (lane != 0) return;
-  const float value = s.top + logf(s.sum);
-  lse[first + r] = value;
+  moments[first + r] = s;
+  // the logits' difference first: of a label that is the largest it is 0
   const int t = label_of(p, first + r);
-  loss[first + r] = t < 0 ? 0.0f : value - (from[t] + (bias ? to_float(bias[t]) : 0.0f));
+  loss[first + r] =
+      t < 0 ? 0.0f : s.top - (from[t] + (bias ? to_float(bias[t]) : 0.0f)) + logf(s.sum);
 }
 
-// The partial results of vocabulary_kernel -> lse and losses.
+// The partial results of vocabulary_kernel -> moments and losses.
 __global__ void __launch_bounds__(kThreads)
     join_partials_kernel(const Rows p, int partials, const Partial* from,
-                         const float* label_logits, float* lse, float* loss) {
+                         const float* label_logits, Partial* moments, float* loss) {
   const long long row = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x;
   if (row >= p.rows) return;
   Partial s = from[row];
 #pragma unroll 4
   for (int i = 1; i < partials; ++i) s = join(s, from[i * p.rows + row]);
-  const float value = log_sum(s);
-  lse[row] = value;
-  loss[row] = label_of(p, row) < 0 ? 0.0f : value - label_logits[row];
+  moments[row] = s;
+  // the logits' difference first: of a label that is the largest it is 0
+  loss[row] = label_of(p, row) < 0
+                  ? 0.0f
+                  : 0.693147180559945309f * (s.top - label_logits[row] + log2f(s.sum));
 }
 
 // The losses' sum or mean and the number of rows that count, in doubles and in a fixed
@@ -162,7 +165,7 @@ __global__ void __launch_bounds__(1024)
 template <class T, class TO, bool BLOCK>
 __global__ void __launch_bounds__(kThreads)
     row_slope_kernel(const Rows p, long long first, int rows, const float* z, int ld,
-                     const T* bias, const float* lse, const float* upstream,
+                     const T* bias, const Partial* moments, const float* upstream,
                      const float* counted, const Factors* factors, TO* dz, int ld_out) {
   const int lane = BLOCK ? threadIdx.x : threadIdx.x & 31, lanes = BLOCK ? kThreads : 32;
   const int r = BLOCK ? blockIdx.x : blockIdx.x * kWarps + (threadIdx.x >> 5);
@@ -171,12 +174,13 @@ __global__ void __launch_bounds__(kThreads)
   TO* to = dz + static_cast<long long>(r) * ld_out;
   const int t = label_of(p, first + r);
   const float u = t < 0 ? 0.0f : upstream_of(p, first + r, upstream, counted) * factors->in;
-  const float less = lse[first + r];
+  const Partial s = moments[first + r];
+  const float factor = u / s.sum;
   for (int j = lane; j < ld_out; j += lanes) {
     float v = 0.0f;
     if (t >= 0 && j < p.vocabulary) {
-      v = expf(from[j] + (bias ? to_float(bias[j]) : 0.0f) - less);
-      v = (j == t ? v - 1.0f : v) * u;
+      v = expf(from[j] + (bias ? to_float(bias[j]) : 0.0f) - s.top) * factor;
+      if (j == t) v -= u;
     }
     to[j] = from_float<TO>(v);
   }
@@ -187,7 +191,7 @@ constexpr int kSumRows = 256;
 template <class T>
 __global__ void __launch_bounds__(kThreads)
     column_slopes_kernel(const Rows p, long long first, int rows, const float* z, int ld,
-                         const T* bias, const float* lse, const float* upstream,
+                         const T* bias, const Partial* moments, const float* upstream,
                          const float* counted, const Factors* factors, float* sums) {
   const int j = blockIdx.x * kThreads + threadIdx.x;
   if (j >= p.vocabulary) return;
@@ -197,35 +201,37 @@ __global__ void __launch_bounds__(kThreads)
   for (int r = begin; r < end; ++r) {
     const int t = label_of(p, first + r);
     if (t < 0) continue;
-    float v = expf(z[static_cast<long long>(r) * ld + j] + b - lse[first + r]);
-    v = j == t ? v - 1.0f : v;
-    sum = fmaf(v, upstream_of(p, first + r, upstream, counted) * factors->in, sum);
+    const Partial s = moments[first + r];
+    const float u = upstream_of(p, first + r, upstream, counted) * factors->in;
+    const float v = expf(z[static_cast<long long>(r) * ld + j] + b - s.top) * (u / s.sum);
+    sum += j == t ? v - u : v;
   }
   sums[static_cast<long long>(blockIdx.y) * p.vocabulary + j] = sum;
 }
-// Adds a piece's ranges to the sums of the pieces before: eight threads to a column.
-__global__ void __launch_bounds__(kThreads)
+// Adds a piece's ranges to the sums of the pieces before: 32 threads to a column.
+constexpr int kAddThreads = 32;
+__global__ void __launch_bounds__(32 * kAddThreads)
     add_columns_kernel(int vocabulary, int ranges, const float* sums, bool begin, float* total) {
   const int j = blockIdx.x * 32 + threadIdx.x;
   float sum = 0.0f;
   if (j < vocabulary) {
 #pragma unroll 8
-    for (int r = threadIdx.y; r < ranges; r += kWarps)
+    for (int r = threadIdx.y; r < ranges; r += kAddThreads)
       sum += sums[static_cast<long long>(r) * vocabulary + j];
   }
-  __shared__ float all[kWarps][32];
+  __shared__ float all[kAddThreads][32];
   all[threadIdx.y][threadIdx.x] = sum;
   __syncthreads();
   if (threadIdx.y || j >= vocabulary) return;
   sum = begin ? 0.0f : total[j];
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) sum += all[w][threadIdx.x];
+  for (int w = 0; w < kAddThreads; ++w) sum += all[w][threadIdx.x];
   total[j] = sum;
 }
 void add_columns(int vocabulary, int ranges, const float* sums, bool begin, float* total,
                  cudaStream_t s) {
-  add_columns_kernel<<<host::blocks_for(vocabulary, 32), dim3(32, kWarps), 0, host::counted(s)>>>(
-      vocabulary, ranges, sums, begin, total);
+  add_columns_kernel<<<host::blocks_for(vocabulary, 32), dim3(32, kAddThreads), 0,
+                       host::counted(s)>>>(vocabulary, ranges, sums, begin, total);
 }
 
 // fp32 sums (of several splits, `stride` values apart) times the factor, rounded.
@@ -256,11 +262,10 @@ void finish(long long count, int splits, long long stride, const float* from,
 constexpr int kMostVocabulary = 1 << 20;
 constexpr long long kPieceBytes = 256LL << 20;
 
-// Whether the logits stay on the chip: fp32 ones would need planes of three parts, and
-// long rows several accumulators.
+// Whether the logits stay on the chip: their sums take one accumulator.
 template <class T>
 bool on_chip(int k) {
-  return sizeof(T) == 2 && k <= kMostAdditions * 16;
+  return k <= (sizeof(T) == 2 ? kMostAdditions * 16 : kExactSum);
 }
 
 // The rows of a piece, and where its parts lie in the workspace.
@@ -270,8 +275,8 @@ struct EntropyPlan {
   PairSplits dx_splits, dw_splits;
   // of vocabulary_kernel
   int tile_n, tiles, ranges, tiles_per_range;
-  size_t logits, dz, x_planes, w_planes, dz_planes, weight_sums, column_sums, column_total, dx,
-      losses, lse, loss_sums, factors, partials, label_logits, bytes;
+  size_t logits, dz, x_planes, w_planes, weight_sums, column_sums, column_total, dx, losses,
+      moments, loss_sums, factors, partials, label_logits, bytes;
 };
 
 // Ranges of words that make the busiest pair of blocks take the fewest tiles, a third of a
@@ -291,6 +296,7 @@ int word_ranges(int row_blocks, int tiles) {
 
 template <class T>
 EntropyPlan plan_entropy(long long rows, int k, int vocabulary, bool backward) {
+  constexpr int P = kOperandParts<T>;
   EntropyPlan plan{};
   plan.on_chip = on_chip<T>(k);
   const int unit = plan.on_chip ? kPairRows : kTileRows;
@@ -299,12 +305,12 @@ EntropyPlan plan_entropy(long long rows, int k, int vocabulary, bool backward) {
     piece = rows;
   } else {
     // bytes of a logit, or of a dz
-    const int size = plan.on_chip ? 2 : 4;
+    const int size = plan.on_chip ? 2 * P : 4;
     piece = std::max(1LL, kPieceBytes / size / vocabulary / unit) * unit;
     piece = std::min({piece, rows, 1LL << 23});  // 65535 ranges of 256 rows, and below
   }
   plan.piece = static_cast<int>(piece);
-  plan.tile_n = pair_tile_n(vocabulary);
+  plan.tile_n = pair_tile_n<P>(vocabulary);
   plan.tiles = (vocabulary + plan.tile_n - 1) / plan.tile_n;
   plan.ranges = word_ranges(static_cast<int>((piece + kPairRows - 1) / kPairRows), plan.tiles);
   plan.tiles_per_range = (plan.tiles + plan.ranges - 1) / plan.ranges;
@@ -321,7 +327,7 @@ EntropyPlan plan_entropy(long long rows, int k, int vocabulary, bool backward) {
   plan.x_planes = take(sizeof(T) == 2 && k % 8 == 0 ? 0 : plane_bytes<T>(piece, k));
   plan.w_planes = take(sizeof(T) == 2 && k % 8 == 0 ? 0 : plane_bytes<T>(vocabulary, k));
   if (!backward) {
-    plan.lse = take(4ull * rows);
+    plan.moments = take(sizeof(Partial) * rows);
     plan.losses = take(4ull * rows);
     if (plan.on_chip) {
       plan.partials = take(plan.tile_n / 64 * static_cast<size_t>(plan.ranges) * rows *
@@ -330,12 +336,11 @@ EntropyPlan plan_entropy(long long rows, int k, int vocabulary, bool backward) {
     }
     return plan;
   }
-  if (sizeof(T) == 2) plan.dz = take(2ull * piece * round_to(vocabulary, 8));
-  else plan.dz_planes = take(plane_bytes<T>(piece, vocabulary));
+  plan.dz = take(plane_bytes<T>(piece, vocabulary));
   // ranges of words for dx and of rows for dW, whose sums are joined
   if (plan.on_chip) {
-    plan.dx_splits = pair_splits(pair_tiles(piece, k), vocabulary);
-    plan.dw_splits = pair_splits(pair_tiles(vocabulary, k), piece);
+    plan.dx_splits = pair_splits<P>(pair_tiles<P>(piece, k), vocabulary);
+    plan.dw_splits = pair_splits<P>(pair_tiles<P>(vocabulary, k), piece);
   } else {
     const long long tiles = ((vocabulary + 127LL) / 128) * ((k + 127) / 128);
     const long long wanted = std::max(1LL, 2LL * host::sm_count() / tiles);
@@ -362,19 +367,21 @@ int launch_vocabulary(VocabularyParams& p, const EntropyPlan& plan, const Rows& 
   p.tile_n = plan.tile_n, p.tiles = plan.tiles;
   p.row_blocks = static_cast<int>((count + static_cast<long long>(kPairRows) - 1) / kPairRows);
   p.splits = plan.ranges, p.tiles_per_split = plan.tiles_per_range;
-  if (!make_map<T>(p.x_map, x.data, count, k, x.ld, 64, 128) ||
-      !make_map<T>(p.w_map, w.data, r.vocabulary, k, w.ld, 64, plan.tile_n / 2))
+  constexpr int P = kOperandParts<T>, kEpilogue = vocabulary_warps(P);
+  p.x_plane_rows = x.plane_rows, p.w_plane_rows = w.plane_rows;
+  if (!make_operand_map<T, false>(p.x_map, x, count, k, 128) ||
+      !make_operand_map<T, false>(p.w_map, w, r.vocabulary, k, plan.tile_n / 2))
     return host::fail(kInvalidArgument, "feature_entropy: operand maps");
-  const int fixed = 1024 + kVocabularyWarps * (256 + (SLOPES ? 4096 : 0));
-  const int stage = kAPlane + plan.tile_n / 2 * 128;
+  const int fixed = 1024 + 4096 + (SLOPES ? kEpilogue * 4096 : 0);
+  const int stage = P * (kAPlane + plan.tile_n / 2 * 128);
   p.stages = std::min(kPairStages, (kOneBlockBytes - fixed) / stage);
-  constexpr auto* kernel = vocabulary_kernel<T, SLOPES>;
+  constexpr auto* kernel = vocabulary_kernel<T, P, SLOPES>;
   if (!host::allow_shared<kernel>())
     return host::check_launch("feature_entropy: shared memory");
   const long long items = static_cast<long long>(p.row_blocks) * p.splits;
   if (items >= 1LL << 31) return host::fail(kTooLarge, "feature_entropy: too many tiles");
   const int pairs = static_cast<int>(std::min<long long>(items, host::sm_count() / 2));
-  kernel<<<2 * pairs, kVocabularyThreads, fixed + p.stages * stage, host::counted(s)>>>(p);
+  kernel<<<2 * pairs, 32 * kEpilogue + 64, fixed + p.stages * stage, host::counted(s)>>>(p);
   return host::check_launch("feature_entropy");
 }
 
@@ -417,35 +424,32 @@ bool lies_well(int dtype, int k, const void* x, const void* weight) {
 
 template <class T>
 int launch_forward(const Rows& r, int k, const void* x, const void* weight, const void* bias,
-                   float* loss, float* lse, float* counted, char* ws, cudaStream_t s) {
+                   float* loss, Partial* moments, float* counted, char* ws, cudaStream_t s) {
   const int vocabulary = r.vocabulary;
   const EntropyPlan plan = plan_entropy<T>(r.rows, k, vocabulary, false);
   float* z = reinterpret_cast<float*>(ws + plan.logits);
-  if (!lse) lse = reinterpret_cast<float*>(ws + plan.lse);
+  if (!moments) moments = reinterpret_cast<Partial*>(ws + plan.moments);
   float* each = r.reduction == kEach ? loss : reinterpret_cast<float*>(ws + plan.losses);
   const Planes w = split<T>(weight, vocabulary, k, ws + plan.w_planes, s);
   for (long long first = 0; first < r.rows; first += plan.piece) {
     const int rows = static_cast<int>(std::min<long long>(plan.piece, r.rows - first));
     const Planes xs = split<T>(static_cast<const T*>(x) + first * k, rows, k,
                                ws + plan.x_planes, s);
-    if constexpr (sizeof(T) == 2) {
-      if (plan.on_chip) {  // all rows at once
-        VocabularyParams p{};
-        p.partials = reinterpret_cast<Partial*>(ws + plan.partials);
-        p.label_logits = reinterpret_cast<float*>(ws + plan.label_logits);
-        const int status =
-            launch_vocabulary<T, false>(p, plan, r, first, rows, k, xs, w, bias, s);
-        if (status != kOk) return status;
-        join_partials_kernel<<<host::blocks_for(rows, kThreads), kThreads, 0, host::counted(s)>>>(
-            r, plan.tile_n / 64 * plan.ranges, p.partials, p.label_logits, lse, each);
-        continue;
-      }
+    if (plan.on_chip) {  // all rows at once
+      VocabularyParams p{};
+      p.partials = reinterpret_cast<Partial*>(ws + plan.partials);
+      p.label_logits = reinterpret_cast<float*>(ws + plan.label_logits);
+      const int status = launch_vocabulary<T, false>(p, plan, r, first, rows, k, xs, w, bias, s);
+      if (status != kOk) return status;
+      join_partials_kernel<<<host::blocks_for(rows, kThreads), kThreads, 0, host::counted(s)>>>(
+          r, plan.tile_n / 64 * plan.ranges, p.partials, p.label_logits, moments, each);
+      continue;
     }
     const int status = launch_logits<T>(rows, k, vocabulary, xs, w, z, s);
     if (status != kOk) return status;
     by_row(rows, vocabulary, [&](auto block, int grid) {
       row_loss_kernel<T, decltype(block)::value><<<grid, kThreads, 0, host::counted(s)>>>(
-          r, first, rows, z, vocabulary, static_cast<const T*>(bias), lse, each);
+          r, first, rows, z, vocabulary, static_cast<const T*>(bias), moments, each);
     });
   }
   if (r.reduction != kEach) {
@@ -461,7 +465,7 @@ int launch_forward(const Rows& r, int k, const void* x, const void* weight, cons
 
 template <class T>
 int launch_backward(const Rows& r, int k, const void* x, const void* weight, const void* bias,
-                    const float* lse, const float* counted, const float* upstream, void* dx,
+                    const Partial* moments, const float* counted, const float* upstream, void* dx,
                     void* dweight, void* dbias, char* ws, cudaStream_t s) {
   constexpr int P = kOperandParts<T>;
   const int vocabulary = r.vocabulary;
@@ -482,22 +486,24 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
     const Planes xs = split<T>(static_cast<const T*>(x) + first * k, rows, k,
                                ws + plan.x_planes, s);
     Planes dz;
+    dz.ld = static_cast<int>(round_to(vocabulary, 8));
+    dz.data = ws + plan.dz;
+    dz.rows = rows;
+    dz.plane_rows = static_cast<int>(P == 1 ? rows : round_to(rows, 64));
     int status = kOk;
-    if constexpr (sizeof(T) == 2) {
-      dz.ld = static_cast<int>(round_to(vocabulary, 8));
-      dz.data = ws + plan.dz;
-      dz.rows = dz.plane_rows = rows;
-      if (plan.on_chip) {
-        VocabularyParams p{};
-        p.lse = lse, p.upstream = upstream, p.counted = counted, p.factors = factors;
-        if (dbias) p.column_sums = column_sums;
-        if (!make_map<T>(p.dz_map, dz.data, rows, vocabulary, dz.ld, 64, 32))
-          return host::fail(kInvalidArgument, "feature_entropy_backward: map");
-        status = launch_vocabulary<T, true>(p, plan, r, first, rows, k, xs, w, bias, s);
-        if (status != kOk) return status;
-        if (dbias)
-          add_columns(vocabulary, (rows + 31) / 32, column_sums, first == 0, column_total, s);
-      }
+    if (plan.on_chip) {
+      VocabularyParams p{};
+      p.moments = moments, p.upstream = upstream, p.counted = counted, p.factors = factors;
+      p.dz_plane_rows = dz.plane_rows;
+      if (dbias) p.column_sums = column_sums;
+      if (!make_map<PairOperand<T>>(p.dz_map, dz.data,
+                                    static_cast<long long>(dz.plane_rows) * P, vocabulary, dz.ld,
+                                    64, 32))
+        return host::fail(kInvalidArgument, "feature_entropy_backward: map");
+      status = launch_vocabulary<T, true>(p, plan, r, first, rows, k, xs, w, bias, s);
+      if (status != kOk) return status;
+      if (dbias)
+        add_columns(vocabulary, (rows + 31) / 32, column_sums, first == 0, column_total, s);
     }
     if (!plan.on_chip) status = launch_logits<T>(rows, k, vocabulary, xs, w, z, s);
     if (status != kOk) return status;
@@ -505,7 +511,7 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
       const int ranges = (rows + kSumRows - 1) / kSumRows;
       column_slopes_kernel<T>
           <<<dim3(host::blocks_for(vocabulary, kThreads), ranges), kThreads, 0,
-             host::counted(s)>>>(r, first, rows, z, vocabulary, b, lse, upstream, counted,
+             host::counted(s)>>>(r, first, rows, z, vocabulary, b, moments, upstream, counted,
                                  factors, column_sums);
       add_columns(vocabulary, ranges, column_sums, first == 0, column_total, s);
     }
@@ -514,19 +520,20 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
       constexpr bool kBlock = decltype(block)::value;
       if constexpr (sizeof(T) == 2) {
         row_slope_kernel<T, T, kBlock><<<grid, kThreads, 0, host::counted(s)>>>(
-            r, first, rows, z, vocabulary, b, lse, upstream, counted, factors,
+            r, first, rows, z, vocabulary, b, moments, upstream, counted, factors,
             static_cast<T*>(dz.data), dz.ld);
       } else {
         row_slope_kernel<T, float, kBlock><<<grid, kThreads, 0, host::counted(s)>>>(
-            r, first, rows, z, vocabulary, b, lse, upstream, counted, factors, z, vocabulary);
+            r, first, rows, z, vocabulary, b, moments, upstream, counted, factors, z, vocabulary);
       }
     });
-    if constexpr (sizeof(T) == 4) dz = split<T>(z, rows, vocabulary, ws + plan.dz_planes, s);
+    if constexpr (sizeof(T) == 4) {
+      if (!plan.on_chip) dz = split<T>(z, rows, vocabulary, ws + plan.dz, s);
+    }
     if (dx) {
       if (plan.on_chip) {
-        if constexpr (sizeof(T) == 2)
-          status = launch_pairs<T, false, true>(rows, k, vocabulary, dz.data, dz.ld, w.data, w.ld,
-                                                plan.dx_splits, dx_sums, false, s);
+        status = launch_pairs<T, false, true>(rows, k, vocabulary, dz, w, plan.dx_splits, dx_sums,
+                                              false, s);
       } else {
         ProductParams p{};
         p.m = rows, p.k = vocabulary, p.n = k;
@@ -545,9 +552,8 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
       PairSplits dw = plan.dw_splits;
       dw.count = static_cast<int>((rows + dw.k - 1) / dw.k);
       if (plan.on_chip) {
-        if constexpr (sizeof(T) == 2)
-          status = launch_pairs<T, true, true>(vocabulary, k, rows, dz.data, dz.ld, xs.data,
-                                               xs.ld, dw, weight_sums, first != 0, s);
+        status = launch_pairs<T, true, true>(vocabulary, k, rows, dz, xs, dw, weight_sums,
+                                             first != 0, s);
       } else {
         ProductParams p{};
         p.m = vocabulary, p.k = rows, p.n = k;
@@ -585,7 +591,7 @@ size_t splat_feature_entropy_workspace_bytes(int dtype, long long rows, int k, i
 
 int splat_feature_entropy(int dtype, long long rows, int k, int vocabulary, const void* x,
                           const void* weight, const void* bias, int id_bytes, const void* target,
-                          long long ignored, int reduction, float* loss, float* lse,
+                          long long ignored, int reduction, float* loss, float* moments,
                           float* counted, void* workspace, size_t workspace_bytes, void* stream) {
   const int bad = check_entropy(dtype, rows, k, vocabulary, id_bytes, reduction);
   if (bad != kOk) return bad;
@@ -600,20 +606,21 @@ int splat_feature_entropy(int dtype, long long rows, int k, int vocabulary, cons
   Rows r{rows, vocabulary, id_bytes, reduction, ignored, target, host::device_error_word()};
   if (!r.error) return kCudaError;
   return SPLAT_FEATURE_TYPE(dtype, [&] {
-    return launch_forward<T>(r, k, x, weight, bias, loss, lse, counted,
-                             static_cast<char*>(workspace), static_cast<cudaStream_t>(stream));
+    return launch_forward<T>(r, k, x, weight, bias, loss, reinterpret_cast<Partial*>(moments),
+                             counted, static_cast<char*>(workspace),
+                             static_cast<cudaStream_t>(stream));
   });
 }
 
 int splat_feature_entropy_backward(int dtype, long long rows, int k, int vocabulary,
                                    const void* x, const void* weight, const void* bias,
                                    int id_bytes, const void* target, long long ignored,
-                                   int reduction, const float* lse, const float* counted,
+                                   int reduction, const float* moments, const float* counted,
                                    const float* upstream, void* dx, void* dweight, void* dbias,
                                    void* workspace, size_t workspace_bytes, void* stream) {
   const int bad = check_entropy(dtype, rows, k, vocabulary, id_bytes, reduction);
   if (bad != kOk) return bad;
-  if (!x || !weight || !target || !lse || !upstream || !workspace ||
+  if (!x || !weight || !target || !moments || !upstream || !workspace ||
       (reduction == kMean && !counted) || (dbias && !bias))
     return host::fail(kInvalidArgument, "feature_entropy_backward: null pointer");
   if (!host::aligned(workspace, 16))
@@ -626,7 +633,7 @@ int splat_feature_entropy_backward(int dtype, long long rows, int k, int vocabul
   Rows r{rows, vocabulary, id_bytes, reduction, ignored, target, host::device_error_word()};
   if (!r.error) return kCudaError;
   return SPLAT_FEATURE_TYPE(dtype, [&] {
-    return launch_backward<T>(r, k, x, weight, bias, lse, counted, upstream, dx, dweight, dbias,
+    return launch_backward<T>(r, k, x, weight, bias, reinterpret_cast<const Partial*>(moments), counted, upstream, dx, dweight, dbias,
                               static_cast<char*>(workspace), static_cast<cudaStream_t>(stream));
   });
 }

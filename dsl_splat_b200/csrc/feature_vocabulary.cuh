@@ -1,27 +1,30 @@
-// Tiles of z = x W^T that never reach memory, for 16-bit x and W: what is left of them are the
-// rows' softmax statistics, or dz.
+// Tiles of z = x W^T that never reach memory: what is left of them are the rows' softmax
+// statistics, or dz.
 //
 //   statistics:  top_i = max_j z_ij, sum_i = sum_j exp(z_ij - top_i), z_i,t_i
-//   slopes:      dz_ij = u_i (exp(z_ij - lse_i) - [j = t_i]), and its column sums
+//   slopes:      dz_ij = u_i (exp(z_ij - top_i) / sum_i - [j = t_i]), and its column sums
 //
-// A pair of blocks (tensor_core.cuh) takes 256 rows x 256 words: per SM, a chunk of 64 k
-// is 16 KB of x and 16 KB of W, half of what two blocks on their own would read from the
-// L2.  In each block one thread starts the tensor copies, and sixteen epilogue warps read
-// the finished accumulators (two of 256 columns, all of the tensor memory), 64 words of 32
-// rows each, and give them back before they work on them; the leading block's product warp
-// issues.  A pair stays with 256 rows over a range of words, so that a row's running maximum
-// and sum stay in a thread's registers; ranges and quarters of the columns leave a
-// partial result each, joined in a fixed order.  Exponentials take the
-// special-function pipe 2048 cycles a tile, the products 8 a k: the pipe binds below 256
-// features, the tensor core above.
+// A pair of blocks (tensor_core.cuh) takes 256 rows x 256 words of 16-bit x and W, or 256 x
+// 128 of fp32 ones in three parts: per SM, a chunk of 64 k is 16 KB of x and 16 KB of W,
+// half of what two blocks on their own would read from the L2.  In each block one thread
+// starts the tensor copies, and sixteen (eight) epilogue warps read the finished
+// accumulators, 64 words of 32 rows each, and give them back before they work on them; the
+// leading block's product warp issues.  A pair stays with 256 rows over a range of words,
+// so that a row's running maximum and sum stay in a thread's registers; ranges and groups of
+// columns leave a partial result each, joined in a fixed order.  Exponentials take the
+// special-function pipe 2048 cycles a tile of 256 words, the products 8 a k: the pipe binds
+// below 256 features, the tensor core above.
+//
+// top and sum are kept apart for the slopes: rounded into one logarithm, they would cost
+// each probability 2^-24 of that logarithm.
 #pragma once
 #include "feature_pairs.cuh"
 
 namespace splat {
 namespace feature {
 
-constexpr int kVocabularyWarps = 16;  // of the epilogue
-constexpr int kVocabularyThreads = 32 * kVocabularyWarps + 64;
+// Epilogue warps: one to 64 words of 32 rows.
+__host__ __device__ constexpr int vocabulary_warps(int parts) { return parts == 1 ? 16 : 8; }
 constexpr float kLog2E = 1.44269504088896341f;
 
 // What the rows' kernels read.
@@ -66,10 +69,10 @@ SPLAT_DEV Partial join(Partial a, Partial b) {
   const float top = fmaxf(a.top, b.top);  // NaN lies in the sums
   return {top, a.sum * exp2f(a.top - top) + b.sum * exp2f(b.top - top)};
 }
-SPLAT_DEV float log_sum(Partial s) { return 0.693147180559945309f * (s.top + log2f(s.sum)); }
 
 struct VocabularyParams {
   CUtensorMap x_map, w_map, dz_map;
+  int x_plane_rows, w_plane_rows, dz_plane_rows;  // of operands in parts
   Rows rows;           // of all pieces
   long long first;     // row of the piece
   int count;           // its rows
@@ -77,36 +80,92 @@ struct VocabularyParams {
   int tiles, row_blocks, splits, tiles_per_split;
   int stages;
   const void* bias;
-  // statistics: (splits, tile_n / 64, count), and the labels' logits (count)
+  // statistics: (splits, tile_n / 64, count), and the labels' logits (count) in units of log 2
   Partial* partials;
   float* label_logits;
   // slopes
-  const float *lse, *upstream, *counted;
+  const Partial* moments;  // (rows)
+  const float *upstream, *counted;
   const Factors* factors;
   float* column_sums;  // (count / 32 rounded up to whole tiles, vocabulary) or NULL
 };
 
-template <class T, bool SLOPES>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVocabularyThreads, 1)
+// 64 logits of a row: those of parts are the sums of two accumulators.
+template <int P>
+SPLAT_DEV void load_logits(uint32_t from, float (&v)[64]) {
+  if constexpr (P == 1) {
+    tc::tmem_load64(from, v);
+  } else {
+#pragma unroll
+    for (int c = 0; c < 64; c += 32) {
+      float high[32], low[32];
+      tc::tmem_load32(from + c, high);
+      tc::tmem_load32(from + c + 128, low);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[c + j] = high[j] + low[j];
+    }
+  }
+}
+
+// v -> 2^(v scale - top), in pairs.
+SPLAT_DEV void exponentials(float (&v)[64], float scale, float top) {
+#pragma unroll
+  for (int j = 0; j < 64; j += 2) {
+    unpack2(fma2(pack2(v[j], v[j + 1]), splat2(scale), splat2(-top)), v[j], v[j + 1]);
+    v[j] = fast_exp2(v[j]);
+    v[j + 1] = fast_exp2(v[j + 1]);
+  }
+}
+
+// The sums over a warp's rows of 32 columns, through its patch: a lane stores its row, then
+// adds four columns of eight rows.  Lanes 0 to 7 get four columns' sums each.
+SPLAT_DEV float4 patch_sums(uint32_t patch, const float* v) {
+  const int lane = threadIdx.x & 31, quad = lane & 7;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    store_shared(patch + lane * 128 + ((j ^ (lane & 7)) << 4),
+                 make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                            __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3])));
+  __syncwarp();
+  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    const float4 row = load_shared(patch + ((lane & 24) + r) * 128 + ((quad ^ r) << 4));
+    sum.x += row.x, sum.y += row.y, sum.z += row.z, sum.w += row.w;
+  }
+#pragma unroll
+  for (int o = 8; o < 32; o *= 2) {
+    sum.x += __shfl_xor_sync(0xffffffffu, sum.x, o);
+    sum.y += __shfl_xor_sync(0xffffffffu, sum.y, o);
+    sum.z += __shfl_xor_sync(0xffffffffu, sum.z, o);
+    sum.w += __shfl_xor_sync(0xffffffffu, sum.w, o);
+  }
+  __syncwarp();  // the patch has been read
+  return sum;
+}
+
+template <class T, int P, bool SLOPES>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * vocabulary_warps(P) + 64, 1)
     vocabulary_kernel(const __grid_constant__ VocabularyParams p) {
+  constexpr int kEpilogue = vocabulary_warps(P);
   extern __shared__ unsigned char dynamic[];
   __shared__ PairBarriers barriers;
   const uint32_t base = (tc::shared_address(dynamic) + 1023u) & ~1023u;
   const int warp = tc::uniform(threadIdx.x >> 5);
   const uint32_t rank = tc::cluster_rank();
   const int half_n = p.tile_n / 2, groups = p.tile_n / 64;
-  const uint32_t stage_bytes = kAPlane + half_n * 128;
+  const uint32_t b_plane = half_n * 128;
   // patches of the epilogue warps, their words' biases, the ring
-  const uint32_t bias_at = base + (SLOPES ? kVocabularyWarps * 4096 : 0);
-  const uint32_t ring_at = bias_at + kVocabularyWarps * 256;
+  const uint32_t bias_at = base + (SLOPES ? kEpilogue * 4096 : 0);
+  const uint32_t ring_at = bias_at + 4096;
   const uint32_t tmem = pair_begin(barriers, p.stages, 8 * groups);
   const int items = p.row_blocks * p.splits;
   const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
   bool ok = true;
 
-  if (warp == kVocabularyWarps) {
+  if (warp == kEpilogue) {
     if ((threadIdx.x & 31) == 0) {
-      PairRing ring(barriers, ring_at, stage_bytes, p.stages, rank);
+      PairRing ring(barriers, ring_at, P * (kAPlane + b_plane), p.stages, rank);
       for (int item = pair; item < items && ok; item += pairs) {
         const int block = item % p.row_blocks, split = item / p.row_blocks;
         const int t1 = min((split + 1) * p.tiles_per_split, p.tiles);
@@ -114,21 +173,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVocabularyThreads, 
         for (int t = split * p.tiles_per_split; t < t1 && ok; ++t)
           for (int k = 0; k < p.k && ok; k += kChunk)
             ok = ring.fill([&](uint32_t at, uint32_t bar) {
-              tc::copy_in_pair(at, &p.x_map, k, row, bar);
-              tc::copy_in_pair(at + kAPlane, &p.w_map, k, t * p.tile_n + rank * half_n, bar);
+              const int word = t * p.tile_n + rank * half_n;
+#pragma unroll
+              for (int i = 0; i < P; ++i, at += kAPlane)
+                tc::copy_in_pair(at, &p.x_map, k, row + i * p.x_plane_rows, bar);
+#pragma unroll
+              for (int i = 0; i < P; ++i, at += b_plane)
+                tc::copy_in_pair(at, &p.w_map, k, word + i * p.w_plane_rows, bar);
             });
       }
       ok = ring.drain() && ok;
     }
-  } else if (warp == kVocabularyWarps + 1) {
+  } else if (warp == kEpilogue + 1) {
     if (rank == 0) {
-      PairIssue issue(barriers, ring_at, stage_bytes, p.stages, tmem,
-                      tc::instruction_pair(!kIsF16<T>, false, false, p.tile_n));
+      PairIssue<P> issue(barriers, ring_at, b_plane, p.stages, tmem,
+                         tc::instruction_pair(!kIsF16<T>, false, false, p.tile_n));
       for (int item = pair; item < items && ok; item += pairs) {
         const int split = item / p.row_blocks;
         const int t1 = min((split + 1) * p.tiles_per_split, p.tiles);
         for (int t = split * p.tiles_per_split; t < t1 && ok; ++t)
-          ok = issue.template tile<false, false>(p.k);
+          ok = issue.template sum<false, false>(p.k);
       }
       ok = issue.drain() && ok;
     }
@@ -149,10 +213,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVocabularyThreads, 
       const bool here = row < p.count;
       const int label = here ? label_of(p.rows, p.first + row) : -1;
       Partial s{kLowest, 0.0f};
-      float less = 0.0f, u = 0.0f;
-      if (SLOPES && label >= 0) {
-        less = p.lse[p.first + row] * kLog2E;
-        u = upstream_of(p.rows, p.first + row, p.upstream, p.counted) * p.factors->in;
+      float u = 0.0f, factor = 0.0f;
+      bool cleared = false;  // some rows' dz is not what 0 times their exponentials gives
+      if constexpr (SLOPES) {
+        if (here) {
+          s = p.moments[p.first + row];
+          if (label >= 0) {
+            u = upstream_of(p.rows, p.first + row, p.upstream, p.counted) * p.factors->in;
+            factor = u / s.sum;
+          }
+        }
+        // a row that does not count has no gradient, whatever its logits are
+        cleared = __any_sync(0xffffffffu, label < 0 && !(here && isfinite(s.top + s.sum)));
       }
       for (int t = split * p.tiles_per_split; t < t1; ++t, ++read) {
         const uint32_t acc = read & 1;
@@ -172,20 +244,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVocabularyThreads, 
           break;
         tc::fence_after_sync();
         float v[64];
-        tc::tmem_load64(tmem + (lane_block << 21) + acc * 256 + group * 64, v);
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0)
-          tc::barrier_arrive_remote(
-              tc::address_in(tc::shared_address(&barriers.acc_empty[acc]), 0));
+        load_logits<P>(tmem + (lane_block << 21) + acc * 256 + group * 64, v);
+        pair_release(barriers, acc);
         if (with_bias) {
 #pragma unroll
           for (int j = 0; j < 64; j += 4) {
             const float4 b = *reinterpret_cast<const float4*>(own_bias + j);
-            v[j] = fmaf(v[j], kLog2E, b.x);
-            v[j + 1] = fmaf(v[j + 1], kLog2E, b.y);
-            v[j + 2] = fmaf(v[j + 2], kLog2E, b.z);
-            v[j + 3] = fmaf(v[j + 3], kLog2E, b.w);
+            unpack2(fma2(pack2(v[j], v[j + 1]), splat2(kLog2E), pack2(b.x, b.y)), v[j], v[j + 1]);
+            unpack2(fma2(pack2(v[j + 2], v[j + 3]), splat2(kLog2E), pack2(b.z, b.w)), v[j + 2],
+                    v[j + 3]);
           }
         }
         const int at = label - col0;  // of the label among these words
@@ -195,7 +262,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVocabularyThreads, 
             float z = 0.0f;
 #pragma unroll
             for (int j = 0; j < 64; ++j) z = j == at ? v[j] : z;
-            if (hit) p.label_logits[row] = with_bias ? z * 0.693147180559945309f : z;
+            if (hit) p.label_logits[row] = with_bias ? z : z * kLog2E;
           }
           float most[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
@@ -206,52 +273,73 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVocabularyThreads, 
             s.sum *= exp2f(s.top - most[0]);
             s.top = most[0];
           }
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          if (with_bias) {
+          exponentials(v, with_bias ? 1.0f : kLog2E, s.top);
+          f32x2 sum[4] = {pack2(s.sum, 0.0f), 0, 0, 0};
 #pragma unroll
-            for (int j = 0; j < 64; ++j) sum[j & 3] += fast_exp2(v[j] - s.top);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 64; ++j) sum[j & 3] += fast_exp2(fmaf(v[j], kLog2E, -s.top));
-          }
-          s.sum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          for (int j = 0; j < 64; j += 2)
+            sum[j / 2 & 3] = add2(sum[j / 2 & 3], pack2(v[j], v[j + 1]));
+          float a, b;
+          unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), a, b);
+          s.sum = a + b;
         } else {
-          if (with_bias) {
+          exponentials(v, with_bias ? 1.0f : kLog2E, s.top);
 #pragma unroll
-            for (int j = 0; j < 64; ++j) v[j] = fast_exp2(v[j] - less);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 64; ++j) v[j] = fast_exp2(fmaf(v[j], kLog2E, -less));
-          }
+          for (int j = 0; j < 64; j += 2)
+            unpack2(mul2(pack2(v[j], v[j + 1]), splat2(factor)), v[j], v[j + 1]);
           if (__any_sync(0xffffffffu, hit)) {
 #pragma unroll
-            for (int j = 0; j < 64; ++j) v[j] = j == at ? v[j] - 1.0f : v[j];
+            for (int j = 0; j < 64; ++j) v[j] = j == at ? v[j] - u : v[j];
           }
-          // rows that do not count have no gradient, whatever their logits are
+          if (cleared) {
 #pragma unroll
-          for (int j = 0; j < 64; ++j) v[j] = label < 0 ? 0.0f : v[j] * u;
-          if (p.column_sums) {  // before dz is rounded
-            float* sums = p.column_sums + static_cast<long long>(row0 / 32) * V + col0 + lane;
-#pragma unroll
-            for (int c = 0; c < 64; c += 32) {
-              const float sum = sum_rows<32>(reinterpret_cast<const float(&)[32]>(v[c]));
-              if (row0 < p.count && col0 + c + lane < V) sums[c] = sum;
-            }
+            for (int j = 0; j < 64; ++j) v[j] = label < 0 ? 0.0f : v[j];
           }
-          // a patch of 32 rows and 64 words for a tensor copy
           if (lane == 0) tc::copies_out_read();
           __syncwarp();
+          if (p.column_sums) {  // before dz is rounded
+            float* sums = p.column_sums + static_cast<long long>(row0 / 32) * V;
 #pragma unroll
-          for (int piece = 0; piece < 8; ++piece) {
-            const Vec<T, 8> r =
-                round_values<T, 8>(reinterpret_cast<const float(&)[8]>(v[piece * 8]));
-            store_shared(patch + lane * 128 + ((piece ^ (lane & 7)) << 4),
-                         reinterpret_cast<const uint4&>(r));
+            for (int c = 0; c < 64; c += 32) {
+              const float4 sum = patch_sums(patch, v + c);
+              const int j = col0 + c + lane * 4;
+              if (lane < 8 && row0 < p.count) {
+                if (j < V) sums[j] = sum.x;
+                if (j + 1 < V) sums[j + 1] = sum.y;
+                if (j + 2 < V) sums[j + 2] = sum.z;
+                if (j + 3 < V) sums[j + 3] = sum.w;
+              }
+            }
           }
-          tc::fence_async_proxy();
-          __syncwarp();
-          if (lane == 0 && row0 < p.count && col0 < V)
-            tc::copy_out(&p.dz_map, col0, row0, patch);
+          // patches of 32 rows and 64 words for tensor copies; planes of parts have zeros in
+          // the rows behind the last
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            if (i > 0) {
+              if (lane == 0) tc::copies_out_read();
+              __syncwarp();
+            }
+#pragma unroll
+            for (int piece = 0; piece < 8; ++piece) {
+              float* o = v + piece * 8;
+              uint4 r;
+              if constexpr (P == 1) {
+                const Vec<T, 8> rounded = round_values<T, 8>(reinterpret_cast<float(&)[8]>(*o));
+                r = reinterpret_cast<const uint4&>(rounded);
+              } else {
+                r = i == P - 1 ? make_uint4(take_part<true>(o[0], o[1]), take_part<true>(o[2], o[3]),
+                                            take_part<true>(o[4], o[5]), take_part<true>(o[6], o[7]))
+                               : make_uint4(take_part<false>(o[0], o[1]),
+                                            take_part<false>(o[2], o[3]),
+                                            take_part<false>(o[4], o[5]),
+                                            take_part<false>(o[6], o[7]));
+              }
+              store_shared(patch + lane * 128 + ((piece ^ (lane & 7)) << 4), r);
+            }
+            tc::fence_async_proxy();
+            __syncwarp();
+            if (lane == 0 && row0 < (P == 1 ? p.count : p.dz_plane_rows) && col0 < V)
+              tc::copy_out(&p.dz_map, col0, row0 + i * p.dz_plane_rows, patch);
+          }
         }
       }
       if (!SLOPES && here)

@@ -84,6 +84,15 @@ SPLAT_DEV void copy_out(const CUtensorMap* map, int column, int row, uint32_t sr
                : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
+// fp32 values onto those of global memory.
+SPLAT_DEV void add_out(const CUtensorMap* map, int column, int row, uint32_t src) {
+  asm volatile(
+      "cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];" ::
+          "l"(map),
+      "r"(column), "r"(row), "r"(src)
+      : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
 // Contiguous bytes (a multiple of 16, both addresses 16-byte aligned).
 SPLAT_DEV void bulk_in(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile(

@@ -146,9 +146,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: Tensor, weight: Tensor, target: Tensor, bias: Tensor | None,
                 ignore_index: int, reduction: str) -> Tensor:
-        loss, lse, counted = stages.feature_entropy(x, weight, target, bias, ignore_index,
+        loss, moments, counted = stages.feature_entropy(x, weight, target, bias, ignore_index,
                                                     reduction)
-        ctx.save_for_backward(x, weight, target, bias, lse, counted)
+        ctx.save_for_backward(x, weight, target, bias, moments, counted)
         ctx.settings = ignore_index, reduction
         ctx.set_materialize_grads(False)
         return loss
@@ -158,10 +158,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def backward(ctx: Any, upstream: Tensor | None):
         if upstream is None:
             return (None,) * 6
-        x, weight, target, bias, lse, counted = ctx.saved_tensors
+        x, weight, target, bias, moments, counted = ctx.saved_tensors
         needs = ctx.needs_input_grad
         dx, dweight, dbias = stages.feature_entropy_backward(
-            x, weight, target, bias, *ctx.settings, lse, counted, upstream,
+            x, weight, target, bias, *ctx.settings, moments, counted, upstream,
             (needs[0], needs[1], needs[3]))
         return dx, dweight, None, dbias, None, None
 

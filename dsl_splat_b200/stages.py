@@ -884,13 +884,13 @@ def feature_entropy(x: Tensor, weight: Tensor, target: Tensor, bias: Tensor | No
                     ignore_index: int, reduction: str, save: bool = True
                     ) -> tuple[Tensor, Tensor | None, Tensor | None]:
     """Softmax cross entropy of x weight^T + bias: the float32 loss and (save) for the
-    backward the rows' log sums and the number of rows that count."""
+    backward the rows' moments (rows,2) and the number of rows that count."""
     vocabulary, k = weight.shape
     rows = target.numel()
     f32 = torch.float32
     each = reduction == "none"
     loss = x.new_empty(target.shape if each else (), dtype=f32)
-    lse = x.new_empty((rows,), dtype=f32) if save else None
+    moments = x.new_empty((rows, 2), dtype=f32) if save else None
     counted = x.new_empty((1,), dtype=f32) if save else None
     if rows:
         dtype, device = FEATURE_DTYPES[x.dtype], x.device
@@ -901,14 +901,14 @@ def feature_entropy(x: Tensor, weight: Tensor, target: Tensor, bias: Tensor | No
         _call(lib.splat_feature_entropy, "feature_entropy", device, dtype, rows, k, vocabulary,
               x.data_ptr(), weight.data_ptr(), _address(bias), target.element_size(),
               target.data_ptr(), ignore_index, REDUCTIONS.index(reduction), loss.data_ptr(),
-              _address(lse), _address(counted), ws.data_ptr(), size)
+              _address(moments), _address(counted), ws.data_ptr(), size)
     elif not each:
         loss.zero_()
-    return loss, lse, counted
+    return loss, moments, counted
 
 
 def feature_entropy_backward(x: Tensor, weight: Tensor, target: Tensor, bias: Tensor | None,
-                             ignore_index: int, reduction: str, lse: Tensor, counted: Tensor,
+                             ignore_index: int, reduction: str, moments: Tensor, counted: Tensor,
                              upstream: Tensor, needs: tuple[bool, bool, bool]
                              ) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
     """Gradients of x, weight and bias (None where not needed)."""
@@ -924,11 +924,11 @@ def feature_entropy_backward(x: Tensor, weight: Tensor, target: Tensor, bias: Te
                       vocabulary, 1)
         ws = x.new_empty((size,), dtype=torch.uint8)
         x, weight, bias, target = _dense(x), _dense(weight), _dense(bias), _dense(target)
-        upstream, lse = _dense(upstream), _dense(lse)
+        upstream, moments = _dense(upstream), _dense(moments)
         _call(lib.splat_feature_entropy_backward, "feature_entropy_backward", device, dtype, rows,
               k, vocabulary, x.data_ptr(), weight.data_ptr(), _address(bias),
               target.element_size(), target.data_ptr(), ignore_index,
-              REDUCTIONS.index(reduction), lse.data_ptr(), counted.data_ptr(),
+              REDUCTIONS.index(reduction), moments.data_ptr(), counted.data_ptr(),
               upstream.data_ptr(), _address(dx), _address(dweight), _address(dbias),
               ws.data_ptr(), size)
     return dx, dweight, dbias

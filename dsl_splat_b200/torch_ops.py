@@ -733,11 +733,11 @@ def _check_entropy(x, weight, target, bias, ignore_index, reduction):
     features.check_linear_cross_entropy(x, weight, target, bias, ignore_index, reduction)
 
 
-def _check_entropy_backward(x, weight, target, bias, ignore_index, reduction, lse, counted,
+def _check_entropy_backward(x, weight, target, bias, ignore_index, reduction, moments, counted,
                             upstream):
     _check_entropy(x, weight, target, bias, ignore_index, reduction)
-    shapes = ((target.numel(),), (1,), target.shape if reduction == "none" else ())
-    for t, shape, name in zip((lse, counted, upstream), shapes, ("lse", "counted", "upstream")):
+    shapes = ((target.numel(), 2), (1,), target.shape if reduction == "none" else ())
+    for t, shape, name in zip((moments, counted, upstream), shapes, ("moments", "counted", "upstream")):
         if t.dtype is not torch.float32 or t.device != x.device or t.shape != shape:
             raise ValueError(f"{name} must be float32 of shape {tuple(shape)} on x's device")
 
@@ -754,24 +754,24 @@ def _(x, weight, target, bias, ignore_index, reduction):
     _check_entropy(x, weight, target, bias, ignore_index, reduction)
     f32 = torch.float32
     return (x.new_empty(target.shape if reduction == "none" else (), dtype=f32),
-            x.new_empty((target.numel(),), dtype=f32), x.new_empty((1,), dtype=f32))
+            x.new_empty((target.numel(), 2), dtype=f32), x.new_empty((1,), dtype=f32))
 
 
 @torch.library.custom_op(f"{_NS}::feature_entropy_backward", mutates_args=())
 def feature_entropy_backward(x: Tensor, weight: Tensor, target: Tensor, bias: Tensor | None,
-                             ignore_index: int, reduction: str, lse: Tensor, counted: Tensor,
+                             ignore_index: int, reduction: str, moments: Tensor, counted: Tensor,
                              upstream: Tensor) -> tuple[Tensor, Tensor, Tensor]:
-    _check_entropy_backward(x, weight, target, bias, ignore_index, reduction, lse, counted,
+    _check_entropy_backward(x, weight, target, bias, ignore_index, reduction, moments, counted,
                             upstream)
     dx, dweight, dbias = stages.feature_entropy_backward(
-        x, weight, target, bias, ignore_index, reduction, lse, counted, upstream,
+        x, weight, target, bias, ignore_index, reduction, moments, counted, upstream,
         (True, True, True))
     return dx, dweight, weight.new_empty((0,)) if dbias is None else dbias
 
 
 @feature_entropy_backward.register_fake
-def _(x, weight, target, bias, ignore_index, reduction, lse, counted, upstream):
-    _check_entropy_backward(x, weight, target, bias, ignore_index, reduction, lse, counted,
+def _(x, weight, target, bias, ignore_index, reduction, moments, counted, upstream):
+    _check_entropy_backward(x, weight, target, bias, ignore_index, reduction, moments, counted,
                             upstream)
     return (x.new_empty(x.shape), weight.new_empty(weight.shape),
             weight.new_empty((0 if bias is None else weight.shape[0],)))
@@ -782,10 +782,10 @@ def _feature_entropy_setup(ctx, inputs, output):
     ctx.save_for_backward(x, weight, target, bias, output[1], output[2])
 
 
-def _feature_entropy_backward(ctx, upstream, _lse, _counted):
-    x, weight, target, bias, lse, counted = ctx.saved_tensors
+def _feature_entropy_backward(ctx, upstream, _moments, _counted):
+    x, weight, target, bias, moments, counted = ctx.saved_tensors
     dx, dw, db = torch.ops.splat200.feature_entropy_backward(
-        x, weight, target, bias, *ctx.settings, lse, counted, upstream)
+        x, weight, target, bias, *ctx.settings, moments, counted, upstream)
     return dx, dw, None, None if bias is None else db, None, None
 
 

@@ -645,14 +645,14 @@ int splat_feature_embedding_backward(int dtype, int id_bytes, long long count, i
  * k), bias (vocabulary) or NULL, target (rows) of id_bytes 4 or 8 (signed).  A row whose
  * target is `ignored` does not count; one whose target lies outside the vocabulary neither,
  * with the device error -6.  reduction: 0 none (loss of each row), 1 sum, 2 mean over the
- * rows that count (0 if none does).  loss float32; lse (rows) float32, for the backward, or
- * NULL; counted (1) float32, the rows that count (1 if none does), for the mean's
+ * rows that count (0 if none does).  loss float32; moments (rows, 2) float32, the rows'
+ * largest logits and sums in the units that the backward takes them in, or NULL; counted (1) float32, the rows that count (1 if none does), for the mean's
  * backward, or NULL. */
 size_t splat_feature_entropy_workspace_bytes(int dtype, long long rows, int k, int vocabulary,
                                              int backward);
 int splat_feature_entropy(int dtype, long long rows, int k, int vocabulary, const void* x,
                           const void* weight, const void* bias, int id_bytes, const void* target,
-                          long long ignored, int reduction, float* loss, float* lse,
+                          long long ignored, int reduction, float* loss, float* moments,
                           float* counted, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Gradients of the above for the loss's upstream gradient (float32: rows, or one):
@@ -660,7 +660,7 @@ int splat_feature_entropy(int dtype, long long rows, int k, int vocabulary, cons
 int splat_feature_entropy_backward(int dtype, long long rows, int k, int vocabulary,
                                    const void* x, const void* weight, const void* bias,
                                    int id_bytes, const void* target, long long ignored,
-                                   int reduction, const float* lse, const float* counted,
+                                   int reduction, const float* moments, const float* counted,
                                    const float* upstream, void* dx, void* dweight, void* dbias,
                                    void* workspace, size_t workspace_bytes, void* stream);
 
