@@ -85,10 +85,10 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll 4
   for (int i = 1; i < partials; ++i) s = join(s, from[i * p.rows + row]);
   moments[row] = s;
-  // the logits' difference first: of a label that is the largest it is 0
-  loss[row] = label_of(p, row) < 0
-                  ? 0.0f
-                  : 0.693147180559945309f * (s.top - label_logits[row] + log2f(s.sum));
+  // the logits' difference first, as the exponentials took it
+  loss[row] = label_of(p, row) < 0 ? 0.0f
+                                   : 0.693147180559945309f *
+                                         (log2f(s.sum) - fmaf(label_logits[row], kLog2E, -s.top));
 }
 
 // The losses' sum or mean and the number of rows that count, in doubles and in a fixed
@@ -260,7 +260,7 @@ void finish(long long count, int splits, long long stride, const float* from,
 // ---- launching -----------------------------------------------------------------------
 
 constexpr int kMostVocabulary = 1 << 20;
-constexpr long long kPieceBytes = 256LL << 20;
+constexpr long long kPieceBytes = 1LL << 30;
 
 // Whether the logits stay on the chip: their sums take one accumulator.
 template <class T>
@@ -372,7 +372,7 @@ int launch_vocabulary(VocabularyParams& p, const EntropyPlan& plan, const Rows& 
   if (!make_operand_map<T, false>(p.x_map, x, count, k, 128) ||
       !make_operand_map<T, false>(p.w_map, w, r.vocabulary, k, plan.tile_n / 2))
     return host::fail(kInvalidArgument, "feature_entropy: operand maps");
-  const int fixed = 1024 + 4096 + (SLOPES ? kEpilogue * 4096 : 0);
+  const int fixed = 1024 + (SLOPES ? kEpilogue * 4096 : 0);
   const int stage = P * (kAPlane + plan.tile_n / 2 * 128);
   p.stages = std::min(kPairStages, (kOneBlockBytes - fixed) / stage);
   constexpr auto* kernel = vocabulary_kernel<T, P, SLOPES>;
@@ -417,9 +417,11 @@ int check_entropy(int dtype, long long rows, int k, int vocabulary, int id_bytes
   return kOk;
 }
 
-// Whether 16-bit rows that need no planes lie as the workspace's size takes them to.
-bool lies_well(int dtype, int k, const void* x, const void* weight) {
-  return dtype == kF32 || k % 8 || (host::aligned(x, 16) && host::aligned(weight, 16));
+// Whether 16-bit rows that need no planes lie as the workspace's size takes them to, and
+// the bias as it is read.
+bool lies_well(int dtype, int k, const void* x, const void* weight, const void* bias) {
+  return host::aligned(bias, 16) &&
+         (dtype == kF32 || k % 8 || (host::aligned(x, 16) && host::aligned(weight, 16)));
 }
 
 template <class T>
@@ -498,7 +500,7 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
       if (dbias) p.column_sums = column_sums;
       if (!make_map<PairOperand<T>>(p.dz_map, dz.data,
                                     static_cast<long long>(dz.plane_rows) * P, vocabulary, dz.ld,
-                                    64, 32))
+                                    32, 32))
         return host::fail(kInvalidArgument, "feature_entropy_backward: map");
       status = launch_vocabulary<T, true>(p, plan, r, first, rows, k, xs, w, bias, s);
       if (status != kOk) return status;
@@ -601,8 +603,8 @@ int splat_feature_entropy(int dtype, long long rows, int k, int vocabulary, cons
     return host::fail(kInvalidArgument, "feature_entropy: workspace not 16-byte aligned");
   if (workspace_bytes < splat_feature_entropy_workspace_bytes(dtype, rows, k, vocabulary, 0))
     return host::fail(kWorkspaceTooSmall, "feature_entropy: workspace");
-  if (!lies_well(dtype, k, x, weight))
-    return host::fail(kInvalidArgument, "feature_entropy: x and weight must be 16-byte aligned");
+  if (!lies_well(dtype, k, x, weight, bias))
+    return host::fail(kInvalidArgument, "feature_entropy: x, weight and bias must be 16-byte aligned");
   Rows r{rows, vocabulary, id_bytes, reduction, ignored, target, host::device_error_word()};
   if (!r.error) return kCudaError;
   return SPLAT_FEATURE_TYPE(dtype, [&] {
@@ -628,8 +630,8 @@ int splat_feature_entropy_backward(int dtype, long long rows, int k, int vocabul
                       "feature_entropy_backward: workspace not 16-byte aligned");
   if (workspace_bytes < splat_feature_entropy_workspace_bytes(dtype, rows, k, vocabulary, 1))
     return host::fail(kWorkspaceTooSmall, "feature_entropy_backward: workspace");
-  if (!lies_well(dtype, k, x, weight))
-    return host::fail(kInvalidArgument, "feature_entropy_backward: x and weight must be 16-byte aligned");
+  if (!lies_well(dtype, k, x, weight, bias))
+    return host::fail(kInvalidArgument, "feature_entropy_backward: x, weight and bias must be 16-byte aligned");
   Rows r{rows, vocabulary, id_bytes, reduction, ignored, target, host::device_error_word()};
   if (!r.error) return kCudaError;
   return SPLAT_FEATURE_TYPE(dtype, [&] {

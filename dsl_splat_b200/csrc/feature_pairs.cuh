@@ -322,8 +322,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 }
 
 // How a pair product of so many tiles and chunks of 64 k is split: such that the busiest
-// pair takes the fewest chunks, twelve for a tile's start and end among them, and no
-// accumulator of 16-bit products more than its additions.
+// pair takes the fewest chunks, three for a tile's start among them, and no accumulator
+// of 16-bit products more than its additions.
 struct PairSplits {
   int count;
   long long k;  // of a split
@@ -338,7 +338,7 @@ PairSplits pair_splits(long long tiles, long long k) {
   double least = 1e30;
   for (long long n = fewest; n <= std::min(chunks, fewest + 31); ++n) {
     const long long per = (chunks + n - 1) / n;
-    const double cost = static_cast<double>((tiles * n + pairs - 1) / pairs) * (per + 12);
+    const double cost = static_cast<double>((tiles * n + pairs - 1) / pairs) * (per + 3);
     if (cost < least * 0.98) {
       least = cost;
       best.k = per * kChunk;

@@ -8,10 +8,12 @@
 // 128 of fp32 ones in three parts: per SM, a chunk of 64 k is 16 KB of x and 16 KB of W,
 // half of what two blocks on their own would read from the L2.  In each block one thread
 // starts the tensor copies, and sixteen (eight) epilogue warps read the finished
-// accumulators, 64 words of 32 rows each, and give them back before they work on them; the
-// leading block's product warp issues.  A pair stays with 256 rows over a range of words,
-// so that a row's running maximum and sum stay in a thread's registers; ranges and groups of
-// columns leave a partial result each, joined in a fixed order.  Exponentials take the
+// accumulators, 32 words of 32 rows at a time, and give them back before they work on the
+// last of them; the leading block's product warp issues.  One half of the epilogue takes
+// the even tiles and the other the odd ones, so that the one's exponentials run under the
+// other's waits and maxima.  A pair stays with 256 rows over a range of words, so that a
+// row's running maximum and sum stay in a thread's registers; ranges and groups of warps
+// leave a partial result each, joined in a fixed order.  Exponentials take the
 // special-function pipe 2048 cycles a tile of 256 words, the products 8 a k: the pipe binds
 // below 256 features, the tensor core above.
 //
@@ -80,7 +82,7 @@ struct VocabularyParams {
   int tiles, row_blocks, splits, tiles_per_split;
   int stages;
   const void* bias;
-  // statistics: (splits, tile_n / 64, count), and the labels' logits (count) in units of log 2
+  // statistics: (splits, tile_n / 64, count), and the labels' logits (count)
   Partial* partials;
   float* label_logits;
   // slopes
@@ -90,30 +92,48 @@ struct VocabularyParams {
   float* column_sums;  // (count / 32 rounded up to whole tiles, vocabulary) or NULL
 };
 
-// 64 logits of a row: those of parts are the sums of two accumulators.
+// 32 logits of a row: those of parts are the sums of two accumulators.
 template <int P>
-SPLAT_DEV void load_logits(uint32_t from, float (&v)[64]) {
-  if constexpr (P == 1) {
-    tc::tmem_load64(from, v);
-  } else {
+SPLAT_DEV void load_logits(uint32_t from, float (&v)[32]) {
+  tc::tmem_load32(from, v);
+  if constexpr (P > 1) {
+    float low[32];
+    tc::tmem_load32(from + 128, low);
 #pragma unroll
-    for (int c = 0; c < 64; c += 32) {
-      float high[32], low[32];
-      tc::tmem_load32(from + c, high);
-      tc::tmem_load32(from + c + 128, low);
-#pragma unroll
-      for (int j = 0; j < 32; ++j) v[c + j] = high[j] + low[j];
-    }
+    for (int j = 0; j < 32; ++j) v[j] += low[j];
   }
 }
 
-// v -> 2^(v scale - top), in pairs.
-SPLAT_DEV void exponentials(float (&v)[64], float scale, float top) {
+// v -> exp(v) 2^-top, in pairs.
+SPLAT_DEV void exponentials(float (&v)[32], float top) {
 #pragma unroll
-  for (int j = 0; j < 64; j += 2) {
-    unpack2(fma2(pack2(v[j], v[j + 1]), splat2(scale), splat2(-top)), v[j], v[j + 1]);
+  for (int j = 0; j < 32; j += 2) {
+    unpack2(fma2(pack2(v[j], v[j + 1]), splat2(kLog2E), splat2(-top)), v[j], v[j + 1]);
     v[j] = fast_exp2(v[j]);
     v[j + 1] = fast_exp2(v[j + 1]);
+  }
+}
+
+// Adds the biases of 32 words, of which so many exist: the others get minus infinity.
+template <class T>
+SPLAT_DEV void add_bias(float (&v)[32], const T* bias, int words) {
+  if (words >= 32) {
+    if (!bias) return;
+    constexpr int N = 16 / sizeof(T);
+#pragma unroll
+    for (int j = 0; j < 32; j += N) {
+      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(bias + j));
+      float b[N];
+      widen<T, N>(reinterpret_cast<const Vec<T, N>&>(raw), b);
+#pragma unroll
+      for (int i = 0; i < N; i += 2)
+        unpack2(add2(pack2(v[j + i], v[j + i + 1]), pack2(b[i], b[i + 1])), v[j + i],
+                v[j + i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      v[j] = j >= words ? -INFINITY : bias ? v[j] + to_float(bias[j]) : v[j];
   }
 }
 
@@ -155,10 +175,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * vocabulary_warp
   const uint32_t rank = tc::cluster_rank();
   const int half_n = p.tile_n / 2, groups = p.tile_n / 64;
   const uint32_t b_plane = half_n * 128;
-  // patches of the epilogue warps, their words' biases, the ring
-  const uint32_t bias_at = base + (SLOPES ? kEpilogue * 4096 : 0);
-  const uint32_t ring_at = bias_at + 4096;
-  const uint32_t tmem = pair_begin(barriers, p.stages, 8 * groups);
+  // patches of the epilogue warps, the ring
+  const uint32_t ring_at = base + (SLOPES ? kEpilogue * 4096 : 0);
+  // tiles that have two 64 words for each warp are shared by half of the warps, which
+  // take every other one
+  const bool alternate = 4 * groups == kEpilogue;
+  const int active = alternate ? kEpilogue / 2 : 4 * groups;  // warps of a tile
+  const uint32_t tmem = pair_begin(barriers, p.stages, 2 * active);
   const int items = p.row_blocks * p.splits;
   const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
   bool ok = true;
@@ -196,15 +219,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * vocabulary_warp
       }
       ok = issue.drain() && ok;
     }
-  } else if (warp < 4 * groups) {
-    // a thread to a row, a warp to 64 of the tile's words
+  } else if (alternate || warp < active) {
+    // a thread to a row, a warp to one or two 64 of the tile's words
     const int lane = threadIdx.x & 31, lane_block = warp & 3, group = warp >> 2;
+    const uint32_t own = alternate ? warp / active : 0, every = alternate ? 1 : 0;
+    const int first = alternate ? (warp % active >> 2) * 128 : group * 64;
+    const int end = first + (alternate ? 128 : 64);
     const T* bias = static_cast<const T*>(p.bias);
     const int V = p.rows.vocabulary;
-    float* own_bias = reinterpret_cast<float*>(
-        dynamic + (bias_at - tc::shared_address(dynamic)) + warp * 256);
-    const uint32_t patch = base + warp * 4096;
-    uint32_t read = 0;  // accumulators
+    const uint32_t patch_at = base + warp * 4096;
+    uint32_t read = 0, patches = 0;  // accumulators; copied out
     for (int item = pair; item < items && ok; item += pairs) {
       const int block = item % p.row_blocks, split = item / p.row_blocks;
       const int t1 = min((split + 1) * p.tiles_per_split, p.tiles);
@@ -227,81 +251,61 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * vocabulary_warp
         cleared = __any_sync(0xffffffffu, label < 0 && !(here && isfinite(s.top + s.sum)));
       }
       for (int t = split * p.tiles_per_split; t < t1; ++t, ++read) {
+        if ((read & every) != own) continue;
         const uint32_t acc = read & 1;
-        const int col0 = t * p.tile_n + group * 64;  // of this warp
-        const bool with_bias = bias || col0 + 64 > V;
-        if (with_bias) {
-          // in units of log 2; words behind the last have minus infinity
-          __syncwarp();  // the tile before has been read
-#pragma unroll
-          for (int j = lane; j < 64; j += 32)
-            own_bias[j] = col0 + j >= V ? -INFINITY
-                          : bias        ? to_float(bias[col0 + j]) * kLog2E
-                                        : 0.0f;
-          __syncwarp();
-        }
         if (!(ok = tc::barrier_wait(tc::shared_address(&barriers.acc_full[acc]), (read >> 1) & 1)))
           break;
         tc::fence_after_sync();
-        float v[64];
-        load_logits<P>(tmem + (lane_block << 21) + acc * 256 + group * 64, v);
-        pair_release(barriers, acc);
-        if (with_bias) {
+        for (int c = first; c < end; c += 32) {
+          const int col0 = t * p.tile_n + c;
+          float v[32];
+          load_logits<P>(tmem + (lane_block << 21) + acc * 256 + c, v);
+          if (c + 32 == end) pair_release(barriers, acc);
+          if (bias || col0 + 32 > V) add_bias<T>(v, bias ? bias + col0 : nullptr, V - col0);
+          const int at = label - col0;  // of the label among these words
+          const bool hit = at >= 0 && at < 32;
+          if constexpr (!SLOPES) {
+            if (__any_sync(0xffffffffu, hit)) {
+              float z = 0.0f;
 #pragma unroll
-          for (int j = 0; j < 64; j += 4) {
-            const float4 b = *reinterpret_cast<const float4*>(own_bias + j);
-            unpack2(fma2(pack2(v[j], v[j + 1]), splat2(kLog2E), pack2(b.x, b.y)), v[j], v[j + 1]);
-            unpack2(fma2(pack2(v[j + 2], v[j + 3]), splat2(kLog2E), pack2(b.z, b.w)), v[j + 2],
-                    v[j + 3]);
-          }
-        }
-        const int at = label - col0;  // of the label among these words
-        const bool hit = at >= 0 && at < 64;
-        if constexpr (!SLOPES) {
-          if (__any_sync(0xffffffffu, hit)) {
-            float z = 0.0f;
+              for (int j = 0; j < 32; ++j) z = j == at ? v[j] : z;
+              if (hit) p.label_logits[row] = z;
+            }
+            float most[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-            for (int j = 0; j < 64; ++j) z = j == at ? v[j] : z;
-            if (hit) p.label_logits[row] = with_bias ? z : z * kLog2E;
-          }
-          float most[4] = {v[0], v[1], v[2], v[3]};
+            for (int j = 4; j < 32; ++j) most[j & 3] = fmaxf(most[j & 3], v[j]);
+            most[0] = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * kLog2E;
+            if (most[0] > s.top) {
+              s.sum *= exp2f(s.top - most[0]);
+              s.top = most[0];
+            }
+            exponentials(v, s.top);
+            f32x2 sum[4] = {pack2(s.sum, 0.0f), 0, 0, 0};
 #pragma unroll
-          for (int j = 4; j < 64; ++j) most[j & 3] = fmaxf(most[j & 3], v[j]);
-          most[0] = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-          if (!with_bias) most[0] *= kLog2E;
-          if (most[0] > s.top) {
-            s.sum *= exp2f(s.top - most[0]);
-            s.top = most[0];
-          }
-          exponentials(v, with_bias ? 1.0f : kLog2E, s.top);
-          f32x2 sum[4] = {pack2(s.sum, 0.0f), 0, 0, 0};
+            for (int j = 0; j < 32; j += 2)
+              sum[j / 2 & 3] = add2(sum[j / 2 & 3], pack2(v[j], v[j + 1]));
+            float a, b;
+            unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), a, b);
+            s.sum = a + b;
+          } else {
+            exponentials(v, s.top);
 #pragma unroll
-          for (int j = 0; j < 64; j += 2)
-            sum[j / 2 & 3] = add2(sum[j / 2 & 3], pack2(v[j], v[j + 1]));
-          float a, b;
-          unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), a, b);
-          s.sum = a + b;
-        } else {
-          exponentials(v, with_bias ? 1.0f : kLog2E, s.top);
+            for (int j = 0; j < 32; j += 2)
+              unpack2(mul2(pack2(v[j], v[j + 1]), splat2(factor)), v[j], v[j + 1]);
+            if (__any_sync(0xffffffffu, hit)) {
 #pragma unroll
-          for (int j = 0; j < 64; j += 2)
-            unpack2(mul2(pack2(v[j], v[j + 1]), splat2(factor)), v[j], v[j + 1]);
-          if (__any_sync(0xffffffffu, hit)) {
+              for (int j = 0; j < 32; ++j) v[j] = j == at ? v[j] - u : v[j];
+            }
+            if (cleared) {
 #pragma unroll
-            for (int j = 0; j < 64; ++j) v[j] = j == at ? v[j] - u : v[j];
-          }
-          if (cleared) {
-#pragma unroll
-            for (int j = 0; j < 64; ++j) v[j] = label < 0 ? 0.0f : v[j];
-          }
-          if (lane == 0) tc::copies_out_read();
-          __syncwarp();
-          if (p.column_sums) {  // before dz is rounded
-            float* sums = p.column_sums + static_cast<long long>(row0 / 32) * V;
-#pragma unroll
-            for (int c = 0; c < 64; c += 32) {
-              const float4 sum = patch_sums(patch, v + c);
-              const int j = col0 + c + lane * 4;
+              for (int j = 0; j < 32; ++j) v[j] = label < 0 ? 0.0f : v[j];
+            }
+            if (p.column_sums) {  // before dz is rounded
+              if (lane == 0) tc::copies_out_read();
+              __syncwarp();
+              const float4 sum = patch_sums(patch_at, v);
+              float* sums = p.column_sums + static_cast<long long>(row0 / 32) * V;
+              const int j = col0 + lane * 4;
               if (lane < 8 && row0 < p.count) {
                 if (j < V) sums[j] = sum.x;
                 if (j + 1 < V) sums[j + 1] = sum.y;
@@ -309,36 +313,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * vocabulary_warp
                 if (j + 3 < V) sums[j + 3] = sum.w;
               }
             }
-          }
-          // patches of 32 rows and 64 words for tensor copies; planes of parts have zeros in
-          // the rows behind the last
+            // patches of 32 rows and 32 words for tensor copies, two in turn; planes of
+            // parts have zeros in the rows behind the last
 #pragma unroll
-          for (int i = 0; i < P; ++i) {
-            if (i > 0) {
-              if (lane == 0) tc::copies_out_read();
+            for (int i = 0; i < P; ++i, ++patches) {
+              const Patch<PairOperand<T>> patch{patch_at + (patches & 1) * 2048};
+              if (lane == 0) tc::copies_out_read_but<1>();
               __syncwarp();
-            }
 #pragma unroll
-            for (int piece = 0; piece < 8; ++piece) {
-              float* o = v + piece * 8;
-              uint4 r;
-              if constexpr (P == 1) {
-                const Vec<T, 8> rounded = round_values<T, 8>(reinterpret_cast<float(&)[8]>(*o));
-                r = reinterpret_cast<const uint4&>(rounded);
-              } else {
-                r = i == P - 1 ? make_uint4(take_part<true>(o[0], o[1]), take_part<true>(o[2], o[3]),
+              for (int piece = 0; piece < 4; ++piece) {
+                float* o = v + piece * 8;
+                uint4 r;
+                if constexpr (P == 1) {
+                  const Vec<T, 8> rounded = round_values<T, 8>(reinterpret_cast<float(&)[8]>(*o));
+                  r = reinterpret_cast<const uint4&>(rounded);
+                } else {
+                  constexpr bool kLast[3] = {false, false, true};
+                  r = kLast[i] ? make_uint4(take_part<true>(o[0], o[1]), take_part<true>(o[2], o[3]),
                                             take_part<true>(o[4], o[5]), take_part<true>(o[6], o[7]))
                                : make_uint4(take_part<false>(o[0], o[1]),
                                             take_part<false>(o[2], o[3]),
                                             take_part<false>(o[4], o[5]),
                                             take_part<false>(o[6], o[7]));
+                }
+                store_shared(patch.at(lane, piece), r);
               }
-              store_shared(patch + lane * 128 + ((piece ^ (lane & 7)) << 4), r);
+              tc::fence_async_proxy();
+              __syncwarp();
+              if (lane == 0) {
+                if (row0 < (P == 1 ? p.count : p.dz_plane_rows) && col0 < V)
+                  tc::copy_out(&p.dz_map, col0, row0 + i * p.dz_plane_rows, patch.base);
+                else
+                  tc::copy_out_none();  // counts too
+              }
             }
-            tc::fence_async_proxy();
-            __syncwarp();
-            if (lane == 0 && row0 < (P == 1 ? p.count : p.dz_plane_rows) && col0 < V)
-              tc::copy_out(&p.dz_map, col0, row0 + i * p.dz_plane_rows, patch);
           }
         }
       }

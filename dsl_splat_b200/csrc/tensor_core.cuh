@@ -101,6 +101,13 @@ SPLAT_DEV void bulk_in(uint32_t dst, const void* src, uint32_t bytes, uint32_t b
       "l"(src), "r"(bytes), "r"(bar)
       : "memory");
 }
+SPLAT_DEV void copy_out_none() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// Until the sources of this thread's copy_outs, but for the last N of them and of
+// copy_out_nones, may be written again.
+template <int N>
+SPLAT_DEV void copies_out_read_but() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
 // Until the sources of this thread's copy_outs may be written again.
 SPLAT_DEV void copies_out_read() {
   asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");

@@ -170,7 +170,10 @@ def test_words_taken_out(dtype, v):
         alone = torch.full_like(b, -math.inf)
         alone[word] = 1.0
         loss, grads = run(x, w, alone, torch.full_like(target, word), "none")
-        assert not loss.any()
+        # log2 of the exponential of r, less r: r is what the rounding of the largest logit to
+        # units of log 2 leaves.  The exponential is off by 2 units of 2^-23 and rounded by half
+        # a one, its logarithm and the difference (both below 2^-20) add less than one
+        assert float(loss.abs().max()) <= 2.0 ** -21
     # a target that is out has an infinite loss; nothing left is not a number
     b[int(target[5])] = -math.inf
     loss = features.linear_cross_entropy(x, w, target, b, reduction="none")
