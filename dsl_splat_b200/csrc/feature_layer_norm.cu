@@ -4,8 +4,11 @@
 //   du = dy act'(u),  d = du w
 //   dx = rstd (d - mean(d) - h mean(d h)),  dw = sum du h,  db = sum du over rows
 //
-// A row's values stay in the registers of a group of lanes (up to 1024 of them) or
-// of a block (up to 8192), so that x and dy are read once.  The mean is taken twice:
+// Rows of up to 1024 channels are staged: bulk copies bring tiles of whole rows into each
+// warp's ring in shared memory, a group of lanes holds a row in registers and puts the
+// results in its place, and bulk copies take them out.  So any channel count moves in
+// contiguous 16-byte pieces, and enough of them are in flight however few registers are left.  Longer
+// rows stay in a block's registers (up to 8192) or are read again from the caches.  The mean is taken twice:
 // the second time of the deviations from the first, whose squares give the
 // variance without a subtraction of like numbers.  The backward takes both again
 // from x, which it has to read: two floats kept per row would cost a row of 32
@@ -13,11 +16,13 @@
 // in all of its rows and adds their du and du h in registers; blocks' sums are
 // joined in a fixed order.
 #include <algorithm>
+#include <type_traits>
 
 #include "feature_common.cuh"
 #include "feature_join.cuh"
 #include "host_runtime.h"
 #include "splat200.h"
+#include "tensor_core.cuh"
 
 namespace splat {
 namespace feature {
@@ -27,6 +32,7 @@ constexpr int kMostLaneValues = 32;                              // of a row, in
 constexpr int kMostGroupChannels = 32 * kMostLaneValues;         // of a row, in a warp
 constexpr int kMostBlockChannels = kNormThreads * kMostLaneValues;
 constexpr int kMostChannels = 65535;
+constexpr int kMostNormStages = 3;
 
 struct LayerNormParams {
   long long rows;
@@ -37,6 +43,7 @@ struct LayerNormParams {
   float* moments;  // (3, rows) of rows longer than a block's registers
   float eps;
   int activation;
+  int* error;
 };
 
 // Sums over the lanes of a row, all lanes get them.
@@ -61,180 +68,397 @@ SPLAT_DEV void sum_lanes(float (&v)[K], int lanes) {
   }
 }
 
-// x of a row -> its deviations from the mean; returns rstd.
-template <bool BLOCK, int N>
-SPLAT_DEV float centre(float (&v)[N], const bool (&in)[N], int lanes, float inverse, float eps) {
-  float sum[1] = {0.0f};
+SPLAT_DEV float add_halves(f32x2 v) {
+  float a, b;
+  unpack2(v, a, b);
+  return a + b;
+}
+// Pairs of values where there are channels, zeros elsewhere.
+template <int M>
+SPLAT_DEV f32x2 masked(f32x2 v, const bool (&in)[2 * M], int i) {
+  float a, b;
+  unpack2(v, a, b);
+  return pack2(in[2 * i] ? a : 0.0f, in[2 * i + 1] ? b : 0.0f);
+}
+
+// x of a row, in pairs -> its normal form (x - mean) rstd; returns rstd.  FULL: every value
+// is a channel's.
+template <bool BLOCK, bool FULL, int M>
+SPLAT_DEV float normalise(f32x2 (&v)[M], const bool (&in)[2 * M], int lanes, float inverse,
+                          float eps) {
+  f32x2 total = v[0];
 #pragma unroll
-  for (int i = 0; i < N; ++i) sum[0] += v[i];
+  for (int i = 1; i < M; ++i) total = add2(total, v[i]);
+  float sum[1] = {add_halves(total)};
   sum_lanes<BLOCK>(sum, lanes);
-  const float mean = sum[0] * inverse;
-  float rest[2] = {0.0f, 0.0f};
+  const f32x2 mean = splat2(-sum[0] * inverse);
+  f32x2 rests = 0, squares = 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    v[i] = in[i] ? v[i] - mean : 0.0f;
-    rest[0] += v[i];
-    rest[1] += v[i] * v[i];
+  for (int i = 0; i < M; ++i) {
+    v[i] = add2(v[i], mean);
+    if constexpr (!FULL) v[i] = masked<M>(v[i], in, i);
+    rests = add2(rests, v[i]);
+    squares = fma2(v[i], v[i], squares);
   }
+  float rest[2] = {add_halves(rests), add_halves(squares)};
   sum_lanes<BLOCK>(rest, lanes);
   const float more = rest[0] * inverse;
+  const float rstd = rsqrtf(fmaxf(rest[1] * inverse - more * more, 0.0f) + eps);
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] -= more;
-  return rsqrtf(fmaxf(rest[1] * inverse - more * more, 0.0f) + eps);
+  for (int i = 0; i < M; ++i) v[i] = fma2(v[i], splat2(rstd), splat2(-more * rstd));
+  return rstd;
 }
 
-template <int N, bool FINE>
-SPLAT_DEV void activate_all(int activation, float (&u)[N]) {
+template <int ACT, int M, bool FINE, bool SLOPE>
+SPLAT_DEV void each_pair(f32x2 (&u)[M]) {
 #pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    switch (activation) {
-      case kRelu: activate2<kRelu, FINE>(u[i], u[i + 1]); break;
-      case kSilu: activate2<kSilu, FINE>(u[i], u[i + 1]); break;
-      case kGelu: activate2<kGelu, FINE>(u[i], u[i + 1]); break;
-      case kSigmoid: activate2<kSigmoid, FINE>(u[i], u[i + 1]); break;
-      default: break;
-    }
+  for (int i = 0; i < M; ++i) {
+    float a, b;
+    unpack2(u[i], a, b);
+    if constexpr (SLOPE) slope2<ACT, FINE>(a, b);
+    else activate2<ACT, FINE>(a, b);
+    u[i] = pack2(a, b);
   }
 }
-template <int N, bool FINE>
-SPLAT_DEV void slope_all(int activation, float (&u)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    switch (activation) {
-      case kRelu: slope2<kRelu, FINE>(u[i], u[i + 1]); break;
-      case kSilu: slope2<kSilu, FINE>(u[i], u[i + 1]); break;
-      case kGelu: slope2<kGelu, FINE>(u[i], u[i + 1]); break;
-      case kSigmoid: slope2<kSigmoid, FINE>(u[i], u[i + 1]); break;
-      default: u[i] = u[i + 1] = 1.0f;
-    }
+// u -> act(u), or act'(u).
+template <bool FINE, bool SLOPE, int M>
+SPLAT_DEV void all_pairs(int activation, f32x2 (&u)[M]) {
+  switch (activation) {
+    case kRelu: each_pair<kRelu, M, FINE, SLOPE>(u); break;
+    case kSilu: each_pair<kSilu, M, FINE, SLOPE>(u); break;
+    case kGelu: each_pair<kGelu, M, FINE, SLOPE>(u); break;
+    case kSigmoid: each_pair<kSigmoid, M, FINE, SLOPE>(u); break;
+    default: each_pair<kNone, M, FINE, SLOPE>(u);
   }
 }
 
-// V values a load, J loads a row and thread.
-template <class T, int V, int J, bool BLOCK, bool BACKWARD>
-__global__ void __launch_bounds__(kNormThreads) layer_norm_kernel(const LayerNormParams p) {
-  constexpr int N = V * J;
-  constexpr bool kFine = sizeof(T) == 4;
-  using Piece = Vec<T, V>;
-  const int lanes = BLOCK ? kNormThreads : p.lanes;
-  const int lane = threadIdx.x & (lanes - 1);
-  const int C = p.channels;
+template <bool FINE, bool SLOPE>
+SPLAT_DEV float one_value(int activation, float u) {
+  f32x2 pair[1] = {pack2(u, 0.0f)};
+  all_pairs<FINE, SLOPE>(activation, pair);
+  float a, b;
+  unpack2(pair[0], a, b);
+  return a;
+}
+
+// A pair of channels' weights and biases, in shared memory, where they cost fewer registers
+// and the lanes of all rows read the same; those of a row's lanes lie side by side.
+SPLAT_DEV float4 load_float4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(at));
+  return v;
+}
+struct Affine {
+  f32x2 w, b;
+};
+SPLAT_DEV Affine affine(uint32_t at, int i, int lanes) {
+  const float4 v = load_float4(at + i * lanes * 16);
+  return {pack2(v.x, v.y), pack2(v.z, v.w)};
+}
+
+// A row's x -> y, in place.
+template <class T, bool BLOCK, bool FULL, int M>
+SPLAT_DEV void norm_row(const LayerNormParams& p, f32x2 (&h)[M], const bool (&in)[2 * M],
+                        uint32_t affine_at, int lanes, float inverse) {
+  normalise<BLOCK, FULL>(h, in, lanes, inverse, p.eps);
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    const Affine a = affine(affine_at, i, lanes);
+    h[i] = fma2(h[i], a.w, a.b);
+  }
+  all_pairs<sizeof(T) == 4, false>(p.activation, h);
+}
+
+// A row's x and dy -> dx in dy's place; its du h and du are added to dw and db.
+template <class T, bool BLOCK, bool FULL, int M>
+SPLAT_DEV void norm_row_backward(const LayerNormParams& p, f32x2 (&h)[M], f32x2 (&g)[M],
+                                 const bool (&in)[2 * M], uint32_t affine_at, int lanes,
+                                 float inverse, f32x2 (&dw)[M], f32x2 (&db)[M]) {
+  const float rstd = normalise<BLOCK, FULL>(h, in, lanes, inverse, p.eps);
+  if (p.activation != kNone) {
+    f32x2 u[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      const Affine a = affine(affine_at, i, lanes);
+      u[i] = fma2(h[i], a.w, a.b);
+    }
+    all_pairs<sizeof(T) == 4, true>(p.activation, u);
+#pragma unroll
+    for (int i = 0; i < M; ++i) g[i] = mul2(g[i], u[i]);
+  }
+  f32x2 less2 = 0, along2 = 0;
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    db[i] = add2(db[i], g[i]);
+    dw[i] = fma2(g[i], h[i], dw[i]);
+    g[i] = mul2(g[i], affine(affine_at, i, lanes).w);
+    less2 = add2(less2, g[i]);
+    along2 = fma2(g[i], h[i], along2);
+  }
+  if (!p.dx) return;
+  float sums[2] = {add_halves(less2), add_halves(along2)};
+  sum_lanes<BLOCK>(sums, lanes);
+  // rstd (d - mean(d) - h mean(d h))
+  const f32x2 less = splat2(-sums[0] * inverse * rstd), along = splat2(-sums[1] * inverse * rstd);
+#pragma unroll
+  for (int i = 0; i < M; ++i) g[i] = fma2(g[i], splat2(rstd), fma2(h[i], along, less));
+}
+
+// The channels of a thread: V neighbouring ones of each of N / V pieces.
+template <int V, int N>
+SPLAT_DEV int channel_of(int i, int lane, int lanes) {
+  return (i / V * lanes + lane) * V + i % V;
+}
+// TIGHT: N is the least of its kind for the row (plan_norm), so that all but the last
+// values are channels'.
+template <int V, int N, bool TIGHT>
+SPLAT_DEV void own_channels(int channels, int lane, int lanes, bool (&in)[N]) {
+  constexpr int kSure = !TIGHT || N <= 8 ? 0 : N - (V > 1 ? 8 : N > 16 ? 4 : 2);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    in[i] = i < kSure || channel_of<V, N>(i, lane, lanes) < channels;
+}
+// Lays out the block's weights and biases for affine(), which a thread calls with the place
+// of the first plus lane * 16.
+template <class T, int V, int N>
+SPLAT_DEV void lay_out_affine(const LayerNormParams& p, int lanes, float* to) {
+  for (int k = threadIdx.x; k < lanes * N; k += blockDim.x) {
+    const int lane = k / N, i = k % N, c = channel_of<V, N>(i, lane, lanes);
+    const bool in = c < p.channels;
+    float* pair = to + (i / 2 * lanes + lane) * 4 + i % 2;
+    pair[0] = in && p.weight ? to_float(static_cast<const T*>(p.weight)[c]) : 1.0f;
+    pair[2] = in && p.bias ? to_float(static_cast<const T*>(p.bias)[c]) : 0.0f;
+  }
+}
+
+// A thread's values of a row, in pairs: zeros where there are none.
+template <class T, int V, int N>
+SPLAT_DEV void load_row(const T* row, int lane, int lanes, bool here, const bool (&in)[N],
+                        f32x2 (&v)[N / 2]) {
+  float f[N];
+#pragma unroll
+  for (int j = 0; j < N; j += V) {
+    Vec<T, V> raw{};
+    if (here && in[j]) raw = *reinterpret_cast<const Vec<T, V>*>(row + (j / V * lanes + lane) * V);
+    widen<T, V>(raw, reinterpret_cast<float(&)[V]>(f[j]));
+  }
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) v[i] = pack2(f[2 * i], f[2 * i + 1]);
+}
+template <class T, int V, int N>
+SPLAT_DEV void store_row(T* row, int lane, int lanes, bool here, const bool (&in)[N],
+                         const f32x2 (&v)[N / 2]) {
+  float f[N];
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) unpack2(v[i], f[2 * i], f[2 * i + 1]);
+#pragma unroll
+  for (int j = 0; j < N; j += V)
+    if (here && in[j])
+      *reinterpret_cast<Vec<T, V>*>(row + (j / V * lanes + lane) * V) =
+          round_values<T, V>(reinterpret_cast<const float(&)[V]>(f[j]));
+}
+
+// ---- rows of up to 1024 channels ----------------------------------------------------
+
+// Each warp's ring of stages of shared memory: a tile of x (and of dy), whose results go
+// out of it.  Warps do not wait for one another.
+struct Staging {
+  int rows, stages;  // of a tile; of a ring
+  int bytes;         // of a tile, a multiple of 16
+  long long tiles;
+};
+
+// What the last whole 16 bytes of a run of bytes leave -> shared memory.
+SPLAT_DEV void copy_rest(uint32_t to, const void* from, int bytes) {
+  for (int i = bytes & ~15; i < bytes; i += 2)
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + i),
+                 "h"(*reinterpret_cast<const unsigned short*>(static_cast<const char*>(from) + i))
+                 : "memory");
+}
+
+// Blocks of 256 threads that an SM holds at once.
+constexpr int resident_blocks(int values, bool backward) {
+  return values > 16 ? (backward ? 1 : 2) : backward ? 2 : 3;
+}
+
+template <class T, int V, int N, bool FULL, bool BACKWARD>
+__global__ void __launch_bounds__(kNormThreads, resident_blocks(N, BACKWARD))
+    staged_norm_kernel(const LayerNormParams p, const Staging ring) {
+  extern __shared__ unsigned char dynamic[];
+  __shared__ alignas(8) unsigned long long barriers[kNormThreads / 32][kMostNormStages];
+  constexpr int M = N / 2;
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const bool leader = (threadIdx.x & 31) == 0;
+  const uint32_t base = (tc::shared_address(dynamic) + 15u) & ~15u;
+  const int stage_bytes = (BACKWARD ? 2 : 1) * ring.bytes;
+  const uint32_t own_at = base + warp * ring.stages * stage_bytes;
+  const uint32_t rings_end = base + warps * ring.stages * stage_bytes;
+  unsigned char* own = dynamic + (own_at - tc::shared_address(dynamic));
+  const uint32_t full = tc::shared_address(barriers[warp]);
+  const int lanes = p.lanes, lane = threadIdx.x & (lanes - 1), groups = 32 / lanes;
+  const int group = (threadIdx.x & 31) / lanes, C = p.channels;
+  const float inverse = 1.0f / static_cast<float>(C);
+  bool in[N], ok = true;
+  f32x2 dw[BACKWARD ? M : 1] = {}, db[BACKWARD ? M : 1] = {};
+  const T* x = static_cast<const T*>(p.x);
+  const T* dy = static_cast<const T*>(p.dy);
+  T* out = static_cast<T*>(BACKWARD ? p.dx : p.y);
+  const long long first = static_cast<long long>(blockIdx.x) * warps + warp;
+  const long long step = static_cast<long long>(gridDim.x) * warps;
+  const auto rows_of = [&](long long tile) {
+    return static_cast<int>(min(p.rows - tile * ring.rows, static_cast<long long>(ring.rows)));
+  };
+  int started = 0;  // by the leader
+  const auto fetch = [&](long long tile, int stage) {
+    const uint32_t bar = full + stage * 8, to = own_at + stage * stage_bytes;
+    const int bytes = rows_of(tile) * C * static_cast<int>(sizeof(T)), whole = bytes & ~15;
+    const long long at = tile * ring.rows * C;
+    copy_rest(to, x + at, bytes);
+    if constexpr (BACKWARD) copy_rest(to + ring.bytes, dy + at, bytes);
+    tc::barrier_expect(bar, (BACKWARD ? 2 : 1) * whole);
+    if (whole) {
+      tc::bulk_in(to, x + at, whole, bar);
+      if constexpr (BACKWARD) tc::bulk_in(to + ring.bytes, dy + at, whole, bar);
+    }
+    ++started;
+  };
+  if (leader) {
+    for (int i = 0; i < ring.stages; ++i) tc::barrier_init(full + i * 8, 1);
+    tc::barrier_init_fence();
+    long long tile = first;
+    for (int i = 0; i < ring.stages - 1 && tile < ring.tiles; ++i, tile += step) fetch(tile, i);
+  }
+  own_channels<V, N, true>(C, lane, lanes, in);
+  lay_out_affine<T, V, N>(p, lanes, reinterpret_cast<float*>(
+                                        dynamic + (rings_end - tc::shared_address(dynamic))));
+  const uint32_t affine_at = rings_end + lane * 16;
+  __syncthreads();
+  int stage = 0, waited = 0;
+  uint32_t parity = 0;
+  for (long long tile = first; tile < ring.tiles; tile += step) {
+    if (!(ok = tc::barrier_wait(full + stage * 8, parity))) break;
+    ++waited;
+    const int rows = rows_of(tile);
+    unsigned char* at = own + stage * stage_bytes;
+    for (int r0 = 0; r0 < rows; r0 += groups) {
+      const int r = r0 + group;
+      const bool here = r < rows;
+      T* row = reinterpret_cast<T*>(at) + r * C;
+      f32x2 h[M];
+      load_row<T, V>(row, lane, lanes, here, in, h);
+      if constexpr (BACKWARD) {
+        f32x2 g[M];
+        load_row<T, V>(reinterpret_cast<const T*>(at + ring.bytes) + r * C, lane, lanes, here, in,
+                       g);
+        norm_row_backward<T, false, FULL>(p, h, g, in, affine_at, lanes, inverse, dw, db);
+        if (out) store_row<T, V>(row, lane, lanes, here, in, g);
+      } else {
+        norm_row<T, false, FULL>(p, h, in, affine_at, lanes, inverse);
+        store_row<T, V>(row, lane, lanes, here, in, h);
+      }
+    }
+    tc::fence_async_proxy();
+    __syncwarp();
+    if (leader) {
+      if (out) {
+        const int bytes = rows * C * static_cast<int>(sizeof(T)), whole = bytes & ~15;
+        char* to = reinterpret_cast<char*>(out + tile * ring.rows * C);
+        if (whole) tc::bulk_out(to, own_at + stage * stage_bytes, whole);
+        for (int i = whole; i < bytes; i += 2)
+          *reinterpret_cast<unsigned short*>(to + i) =
+              *reinterpret_cast<const unsigned short*>(at + i);
+      }
+      // the stage before this one is free once its results have been read
+      const long long next = tile + (ring.stages - 1) * step;
+      if (next < ring.tiles) {
+        if (out) tc::copies_out_read_but<1>();
+        fetch(next, stage ? stage - 1 : ring.stages - 1);
+      }
+    }
+    if (++stage == ring.stages) stage = 0, parity ^= 1;
+  }
+  if (leader) {
+    // no copy is in flight past this point, also after a wait that ran out
+    for (int i = waited; i < started; ++i) {
+      ok = tc::barrier_wait(full + stage * 8, parity) && ok;
+      if (++stage == ring.stages) stage = 0, parity ^= 1;
+    }
+    if (out) tc::copies_out_read();
+  }
+  if (!ok) atomicCAS(p.error, 0, kDeviceTimeout);
+  if constexpr (BACKWARD) {
+    if (!p.partial) return;
+    __syncthreads();
+    // the groups of a warp, then the warps one after another
+    float* sums = reinterpret_cast<float*>(dynamic + (base - tc::shared_address(dynamic)));
+    for (int o = lanes; o < 32; o *= 2)
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        dw[i] = add2(dw[i], __shfl_xor_sync(0xffffffffu, dw[i], o));
+        db[i] = add2(db[i], __shfl_xor_sync(0xffffffffu, db[i], o));
+      }
+    for (int k = 0; k < warps; ++k) {
+      if (warp == k && group == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (!in[i]) continue;
+          const int c = channel_of<V, N>(i, lane, lanes);
+          float a[2], d[2];
+          unpack2(dw[i / 2], a[0], a[1]);
+          unpack2(db[i / 2], d[0], d[1]);
+          sums[c] = (k ? sums[c] : 0.0f) + a[i % 2];
+          sums[C + c] = (k ? sums[C + c] : 0.0f) + d[i % 2];
+        }
+      }
+      __syncthreads();
+    }
+    float* to = p.partial + 2LL * blockIdx.x * C;
+    for (int c = threadIdx.x; c < 2 * C; c += blockDim.x) to[c] = sums[c];
+  }
+}
+
+// ---- rows of up to 8192 channels: a block each ----------------------------------------
+
+template <class T, int V, bool BACKWARD>
+__global__ void __launch_bounds__(kNormThreads) block_norm_kernel(const LayerNormParams p) {
+  constexpr int N = kMostLaneValues, M = N / 2;
+  const int lane = threadIdx.x, lanes = kNormThreads, C = p.channels;
   const float inverse = 1.0f / static_cast<float>(C);
   bool in[N];
-  float w[N], b[N];
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const int c = (j * lanes + lane) * V;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      in[j * V + i] = c < C;  // C is a multiple of V
-      w[j * V + i] = c < C && p.weight ? to_float(static_cast<const T*>(p.weight)[c + i]) : 1.0f;
-      b[j * V + i] = c < C && p.bias ? to_float(static_cast<const T*>(p.bias)[c + i]) : 0.0f;
-    }
-  }
-  float dw[BACKWARD ? N : 1] = {}, db[BACKWARD ? N : 1] = {};
-  // a warp's groups step together
-  const int groups = BLOCK ? 1 : 32 / lanes;
-  const int group = BLOCK ? 0 : (threadIdx.x & 31) / lanes;
-  const long long first =
-      BLOCK ? blockIdx.x : (blockIdx.x * (kNormThreads / 32LL) + (threadIdx.x >> 5)) * groups;
-  const long long step = BLOCK ? gridDim.x : gridDim.x * (kNormThreads / 32LL) * groups;
-  for (long long row0 = first; row0 < p.rows; row0 += step) {
-    const long long row = row0 + group, at = row * C;
-    const bool here = row < p.rows;
-    Piece raw[J], up[BACKWARD ? J : 1];
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      raw[j] = Piece{};
-      if (here && in[j * V])
-        raw[j] = *reinterpret_cast<const Piece*>(static_cast<const T*>(p.x) + at +
-                                                 (j * lanes + lane) * V);
-    }
+  f32x2 dw[BACKWARD ? M : 1] = {}, db[BACKWARD ? M : 1] = {};
+  extern __shared__ float4 weights[];
+  own_channels<V, N, false>(C, lane, lanes, in);
+  lay_out_affine<T, V, N>(p, lanes, reinterpret_cast<float*>(weights));
+  const uint32_t affine_at = tc::shared_address(weights) + lane * 16;
+  __syncthreads();
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const long long at = row * C;
+    f32x2 h[M];
+    load_row<T, V>(static_cast<const T*>(p.x) + at, lane, lanes, true, in, h);
     if constexpr (BACKWARD) {
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        up[j] = Piece{};
-        if (here && in[j * V])
-          up[j] = *reinterpret_cast<const Piece*>(static_cast<const T*>(p.dy) + at +
-                                                  (j * lanes + lane) * V);
-      }
-    }
-    float h[N], u[N];
-#pragma unroll
-    for (int j = 0; j < J; ++j) widen<T, V>(raw[j], reinterpret_cast<float(&)[V]>(h[j * V]));
-    const float rstd = centre<BLOCK>(h, in, lanes, inverse, p.eps);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      h[i] *= rstd;
-      u[i] = fmaf(h[i], w[i], b[i]);
-    }
-    if constexpr (!BACKWARD) {
-      activate_all<N, kFine>(p.activation, u);
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-        if (here && in[j * V])
-          *reinterpret_cast<Piece*>(static_cast<T*>(p.y) + at + (j * lanes + lane) * V) =
-              round_values<T, V>(reinterpret_cast<const float(&)[V]>(u[j * V]));
+      f32x2 g[M];
+      load_row<T, V>(static_cast<const T*>(p.dy) + at, lane, lanes, true, in, g);
+      norm_row_backward<T, true, false>(p, h, g, in, affine_at, lanes, inverse, dw, db);
+      if (p.dx) store_row<T, V>(static_cast<T*>(p.dx) + at, lane, lanes, true, in, g);
     } else {
-      float g[N], sums[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int j = 0; j < J; ++j) widen<T, V>(up[j], reinterpret_cast<float(&)[V]>(g[j * V]));
-      slope_all<N, kFine>(p.activation, u);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        g[i] *= u[i];
-        db[i] += g[i];
-        dw[i] = fmaf(g[i], h[i], dw[i]);
-        g[i] *= w[i];
-        sums[0] += g[i];
-        sums[1] = fmaf(g[i], h[i], sums[1]);
-      }
-      if (p.dx) {
-        sum_lanes<BLOCK>(sums, lanes);
-        const float less = sums[0] * inverse, along = sums[1] * inverse;
-#pragma unroll
-        for (int i = 0; i < N; ++i) g[i] = rstd * (g[i] - fmaf(h[i], along, less));
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-          if (here && in[j * V])
-            *reinterpret_cast<Piece*>(static_cast<T*>(p.dx) + at + (j * lanes + lane) * V) =
-                round_values<T, V>(reinterpret_cast<const float(&)[V]>(g[j * V]));
-      }
+      norm_row<T, true, false>(p, h, in, affine_at, lanes, inverse);
+      store_row<T, V>(static_cast<T*>(p.y) + at, lane, lanes, true, in, h);
     }
   }
   if constexpr (BACKWARD) {
     if (!p.partial) return;
     float* to = p.partial + 2LL * blockIdx.x * C;
-    if constexpr (BLOCK) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (!in[i]) continue;
-        const int c = (i / V * lanes + lane) * V + i % V;
-        to[c] = dw[i];
-        to[C + c] = db[i];
-      }
-    } else {
-      // the groups of a warp, then the warps one after another
-      __shared__ float sums[2 * kMostGroupChannels];
-      for (int o = lanes; o < 32; o *= 2)
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
-          db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
-        }
-      for (int k = 0; k < kNormThreads / 32; ++k) {
-        if (static_cast<int>(threadIdx.x >> 5) == k && group == 0) {
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            if (!in[i]) continue;
-            const int c = (i / V * lanes + lane) * V + i % V;
-            sums[c] = (k ? sums[c] : 0.0f) + dw[i];
-            sums[C + c] = (k ? sums[C + c] : 0.0f) + db[i];
-          }
-        }
-        __syncthreads();
-      }
-      for (int c = threadIdx.x; c < 2 * C; c += kNormThreads) to[c] = sums[c];
+    for (int i = 0; i < N; ++i) {
+      if (!in[i]) continue;
+      const int c = channel_of<V, N>(i, lane, lanes);
+      float a[2], d[2];
+      unpack2(dw[i / 2], a[0], a[1]);
+      unpack2(db[i / 2], d[0], d[1]);
+      to[c] = a[i % 2];
+      to[C + c] = d[i % 2];
     }
   }
 }
@@ -275,13 +499,12 @@ __global__ void __launch_bounds__(kNormThreads) long_rows_kernel(const LayerNorm
       float sums[2] = {0.0f, 0.0f};
       for (int c = threadIdx.x; c < C; c += kNormThreads) {
         const float h = (to_float(x[c]) - mean - more) * rstd, scale = w ? to_float(w[c]) : 1.0f;
-        float u[2] = {fmaf(h, scale, b ? to_float(b[c]) : 0.0f), 0.0f};
+        const float u = fmaf(h, scale, b ? to_float(b[c]) : 0.0f);
         if constexpr (!BACKWARD) {
-          activate_all<2, kFine>(p.activation, u);
-          static_cast<T*>(p.y)[row * C + c] = from_float<T>(u[0]);
+          static_cast<T*>(p.y)[row * C + c] = from_float<T>(one_value<kFine, false>(p.activation, u));
         } else {
-          slope_all<2, kFine>(p.activation, u);
-          const float g = to_float(dy[c]) * u[0] * scale;
+          const float g =
+              to_float(dy[c]) * one_value<kFine, true>(p.activation, u) * scale;
           if (pass == 0) {
             sums[0] += g;
             sums[1] = fmaf(g, h, sums[1]);
@@ -316,9 +539,8 @@ __global__ void __launch_bounds__(kNormThreads)
     const float h = (to_float(static_cast<const T*>(p.x)[row * C + c]) - p.moments[row] -
                      p.moments[p.rows + row]) *
                     p.moments[2 * p.rows + row];
-    float u[2] = {fmaf(h, w, b), 0.0f};
-    slope_all<2, kFine>(p.activation, u);
-    const float g = to_float(static_cast<const T*>(p.dy)[row * C + c]) * u[0];
+    const float g = to_float(static_cast<const T*>(p.dy)[row * C + c]) *
+                    one_value<kFine, true>(p.activation, fmaf(h, w, b));
     db += g;
     dw = fmaf(g, h, dw);
   }
@@ -331,15 +553,24 @@ __global__ void __launch_bounds__(kNormThreads)
 
 struct LayerNormPlan {
   int blocks, lanes;  // lanes: 0: a block to a row
+  bool vector;        // rows are whole 16-byte pieces
+  int values;         // of a lane
+  int warps;          // of a block
+  Staging ring;
+  size_t shared;
   bool longer;        // than a block's registers
   long long range;    // of rows, of their columns' sums
 };
+
+// Bytes of a warp's tile, that three stages for all of an SM's warps fit.
+constexpr int kTileBytes = 2900, kBackwardTileBytes = 2250;
 
 template <class T>
 LayerNormPlan plan_norm(long long rows, int channels, bool backward) {
   constexpr int V = 16 / sizeof(T);
   LayerNormPlan plan{};
   const int sms = host::sm_count();
+  plan.vector = channels % V == 0;
   plan.longer = channels > kMostBlockChannels;
   if (plan.longer) {
     plan.blocks = static_cast<int>(std::min<long long>(rows, 4LL * sms));
@@ -347,44 +578,104 @@ LayerNormPlan plan_norm(long long rows, int channels, bool backward) {
     plan.range = (rows + most - 1) / most;
     return plan;
   }
-  long long rows_at_once = 1;
-  if (channels <= kMostGroupChannels) {
-    // eight values a lane, where rows are whole 16-byte pieces and where not
-    const int width = channels % V == 0 ? std::max(V, 8) : 8;
-    plan.lanes = 1;
-    while (plan.lanes < 32 && plan.lanes * width < channels) plan.lanes *= 2;
-    rows_at_once = kNormThreads / plan.lanes;
+  if (channels > kMostGroupChannels) {
+    plan.blocks = static_cast<int>(std::min<long long>(rows, (backward ? 1LL : 4LL) * sms));
+    return plan;
   }
-  plan.blocks = static_cast<int>(std::min<long long>((rows + rows_at_once - 1) / rows_at_once,
-                                                     (backward ? 4LL : 8LL) * sms));
+  // up to 16 values a lane, of which the last piece may be idle; more in whole warps
+  plan.lanes = 1;
+  while (plan.lanes < 32 && plan.lanes * 16 < channels) plan.lanes *= 2;
+  const int each = (channels + plan.lanes - 1) / plan.lanes;
+  plan.values = plan.vector ? (each <= 8 ? 8 : each <= 16 ? 16 : each <= 24 ? 24 : 32)
+                : each <= 8 ? 8 : each <= 16 ? (each + 1) / 2 * 2 : (each + 3) / 4 * 4;
+  // tiles of whole passes that start on 16 bytes
+  const int at_once = 32 / plan.lanes, row_bytes = channels * static_cast<int>(sizeof(T));
+  int unit = at_once;
+  while (unit * row_bytes % 16) unit *= 2;
+  const int most = 
+      std::max(1, (backward ? kBackwardTileBytes : kTileBytes) / (unit * row_bytes));
+  // no longer than what there is for a warp
+  const long long wanted = (rows + 16LL * sms * unit - 1) / (16LL * sms * unit);
+  plan.ring.rows = unit * static_cast<int>(std::min<long long>(most, wanted));
+  plan.ring.bytes = (plan.ring.rows * row_bytes + 15) / 16 * 16;
+  plan.ring.tiles = (rows + plan.ring.rows - 1) / plan.ring.rows;
+  // three stages a warp, in half of an SM's shared memory at most
+  const int stage = (backward ? 2 : 1) * plan.ring.bytes;
+  plan.ring.stages = kMostNormStages;
+  plan.warps = kNormThreads / 32;
+  while (plan.warps > 1 && plan.warps * plan.ring.stages * stage > 100 * 1024) plan.warps /= 2;
+  plan.shared = 16 + static_cast<size_t>(std::max(plan.warps * plan.ring.stages * stage,
+                                                  8 * channels)) +
+                8 * plan.lanes * plan.values;
+  const int fit = static_cast<int>(220 * 1024 / (plan.shared + 1024));
+  // no more blocks than run at once: each takes its share of the tiles
+  const int resident = std::max(
+      1, std::min(fit, resident_blocks(plan.values, backward) * kNormThreads / 32 / plan.warps));
+  plan.blocks = static_cast<int>(std::min<long long>(
+      (plan.ring.tiles + plan.warps - 1) / plan.warps, static_cast<long long>(resident) * sms));
   return plan;
 }
 
 template <class T, bool BACKWARD>
-void launch_norm(const LayerNormPlan& plan, LayerNormParams& p, cudaStream_t s) {
+int launch_norm(const LayerNormPlan& plan, LayerNormParams& p, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
   p.lanes = plan.lanes;
-  const auto run = [&](auto* kernel) {
-    kernel<<<plan.blocks, kNormThreads, 0, host::counted(s)>>>(p);
-  };
-  if (plan.longer) return run(long_rows_kernel<T, BACKWARD>);
-  const int lanes = plan.lanes ? plan.lanes : kNormThreads;
-  const int each = (p.channels + lanes - 1) / lanes;  // values a lane
-  const bool vector = p.channels % V == 0 && host::aligned(p.x, 16) && host::aligned(p.y, 16) &&
-                      host::aligned(p.dy, 16) && host::aligned(p.dx, 16);
-  if (!plan.lanes) {
-    if (vector) run(layer_norm_kernel<T, V, 32 / V, true, BACKWARD>);
-    else run(layer_norm_kernel<T, 1, 32, true, BACKWARD>);
-  } else if (each <= 8) {
-    if (vector) run(layer_norm_kernel<T, V, 8 / V, false, BACKWARD>);
-    else run(layer_norm_kernel<T, 1, 8, false, BACKWARD>);
-  } else if (each <= 16) {
-    if (vector) run(layer_norm_kernel<T, V, 16 / V, false, BACKWARD>);
-    else run(layer_norm_kernel<T, 1, 16, false, BACKWARD>);
-  } else {
-    if (vector) run(layer_norm_kernel<T, V, 32 / V, false, BACKWARD>);
-    else run(layer_norm_kernel<T, 1, 32, false, BACKWARD>);
+  if (plan.longer) {
+    long_rows_kernel<T, BACKWARD><<<plan.blocks, kNormThreads, 0, host::counted(s)>>>(p);
+    return kOk;
   }
+  const bool aligned = host::aligned(p.x, 16) && host::aligned(p.y, 16) &&
+                       host::aligned(p.dy, 16) && host::aligned(p.dx, 16);
+  if (!plan.lanes) {
+    constexpr auto* wide = block_norm_kernel<T, V, BACKWARD>;
+    constexpr auto* narrow = block_norm_kernel<T, 1, BACKWARD>;
+    if (!host::allow_shared<wide>() || !host::allow_shared<narrow>())
+      return host::check_launch("feature_layer_norm: shared memory");
+    (plan.vector && aligned ? wide : narrow)<<<plan.blocks, kNormThreads, 8 * kMostBlockChannels,
+                                               host::counted(s)>>>(p);
+    return kOk;
+  }
+  if (!aligned)
+    return host::fail(kInvalidArgument, "feature_layer_norm: tensors must be 16-byte aligned");
+  p.error = host::device_error_word();
+  if (!p.error) return kCudaError;
+  const auto run = [&](auto width, auto values) {
+    constexpr int kWidth = decltype(width)::value, kValues = decltype(values)::value;
+    const auto launch = [&](auto full) {
+      constexpr auto* kernel =
+          staged_norm_kernel<T, kWidth, kValues, decltype(full)::value, BACKWARD>;
+      if (!host::allow_shared<kernel>())
+        return host::check_launch("feature_layer_norm: shared memory");
+      kernel<<<plan.blocks, 32 * plan.warps, plan.shared, host::counted(s)>>>(p, plan.ring);
+      return static_cast<int>(kOk);
+    };
+    if constexpr (kWidth > 1) {
+      if (plan.lanes * kValues == p.channels) return launch(std::true_type{});
+    }
+    return launch(std::false_type{});
+  };
+#define SPLAT_NORM_VALUES(width, n) \
+  case n: return run(std::integral_constant<int, width>{}, std::integral_constant<int, n>{})
+  if (plan.vector) {
+    switch (plan.values) {
+      SPLAT_NORM_VALUES(V, 8);
+      SPLAT_NORM_VALUES(V, 16);
+      SPLAT_NORM_VALUES(V, 24);
+      default: return run(std::integral_constant<int, V>{}, std::integral_constant<int, 32>{});
+    }
+  }
+  switch (plan.values) {
+    SPLAT_NORM_VALUES(1, 8);
+    SPLAT_NORM_VALUES(1, 10);
+    SPLAT_NORM_VALUES(1, 12);
+    SPLAT_NORM_VALUES(1, 14);
+    SPLAT_NORM_VALUES(1, 16);
+    SPLAT_NORM_VALUES(1, 20);
+    SPLAT_NORM_VALUES(1, 24);
+    SPLAT_NORM_VALUES(1, 28);
+    default: return run(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{});
+  }
+#undef SPLAT_NORM_VALUES
 }
 
 int check_layer_norm(int dtype, long long rows, int channels, int activation) {
@@ -424,9 +715,9 @@ int splat_feature_layer_norm(int dtype, long long rows, int channels, const void
     p.rows = rows, p.channels = channels;
     p.x = x, p.weight = weight, p.bias = bias, p.y = y;
     p.eps = eps, p.activation = activation;
-    launch_norm<T, false>(plan_norm<T>(rows, channels, false), p,
-                          static_cast<cudaStream_t>(stream));
-    return host::check_launch("feature_layer_norm");
+    const int status = launch_norm<T, false>(plan_norm<T>(rows, channels, false), p,
+                                             static_cast<cudaStream_t>(stream));
+    return status != kOk ? status : host::check_launch("feature_layer_norm");
   });
 }
 
@@ -463,7 +754,8 @@ int splat_feature_layer_norm_backward(int dtype, long long rows, int channels, c
     if (dweight || dbias)
       p.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                            moments_bytes(plan, rows));
-    launch_norm<T, true>(plan, p, s);
+    const int status = launch_norm<T, true>(plan, p, s);
+    if (status != kOk) return status;
     if (p.partial) {
       const int count = sums(plan, rows);
       if (plan.longer)

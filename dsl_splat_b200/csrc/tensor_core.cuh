@@ -101,6 +101,13 @@ SPLAT_DEV void bulk_in(uint32_t dst, const void* src, uint32_t bytes, uint32_t b
       "l"(src), "r"(bytes), "r"(bar)
       : "memory");
 }
+// Contiguous bytes, as bulk_in.
+SPLAT_DEV void bulk_out(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src),
+               "r"(bytes)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
 SPLAT_DEV void copy_out_none() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // Until the sources of this thread's copy_outs, but for the last N of them and of
 // copy_out_nones, may be written again.
