@@ -43,6 +43,7 @@ constexpr int kThreads = 256;
 constexpr int kMostTensors = 96;
 constexpr int kRun = 256;           // values that share an exponent
 constexpr int kPiece = 4096;        // values of a block
+constexpr int kPiece8 = 16384;      // with states in 8 bits, whose blocks load ahead
 constexpr int kNotFinite = -128;    // exponent of a run with infinities or NaN: all are NaN
 
 struct Tensor {
@@ -54,6 +55,7 @@ struct Tensor {
   const float* device_lr;        // or NULL: the host knew the learning rate
   double lr, decay, beta1, beta2;
   long long n;
+  float b1, c1, b2, c2;             // the betas and 1 - them
   float shrink, rate, unbias, eps;  // 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
   uint32_t step, first_block;
   int vector;  // every base lies on 16 bytes
@@ -100,22 +102,16 @@ SPLAT_DEV int tensor_of(const Table& table) {
   return low;
 }
 
-struct Betas {
-  float b1, c1, b2, c2;
-  SPLAT_DEV explicit Betas(const Tensor& t)
-      : b1(static_cast<float>(t.beta1)),
-        c1(static_cast<float>(1.0 - t.beta1)),
-        b2(static_cast<float>(t.beta2)),
-        c2(static_cast<float>(1.0 - t.beta2)) {}
-};
-
-// One value: m and v become m' and the root of v'; returns p'.
-SPLAT_DEV float update(float p, float g, float& m, float& v, float& root, const Betas& b,
-                       const Rates& r, float eps) {
-  m = __fadd_rn(__fmul_rn(m, b.b1), __fmul_rn(g, b.c1));
-  v = __fadd_rn(__fmul_rn(v, b.b2), __fmul_rn(__fmul_rn(g, b.c2), g));
+// One value: m and v become m' and v', root that of v'; returns p'.  FAST: the quotient
+// is off by two units of 2^-23 instead of a half (the root is at least 2^-75 or 0).
+template <bool FAST>
+SPLAT_DEV float update(float p, float g, float& m, float& v, float& root, const Tensor& t,
+                       const Rates& r) {
+  m = __fadd_rn(__fmul_rn(m, t.b1), __fmul_rn(g, t.c1));
+  v = __fadd_rn(__fmul_rn(v, t.b2), __fmul_rn(__fmul_rn(g, t.c2), g));
   root = __fsqrt_rn(v);
-  return p * r.shrink - m / fmaf(root, r.unbias, eps) * r.rate;
+  const float below = fmaf(root, r.unbias, t.eps);
+  return fmaf(p, r.shrink, -(FAST ? __fdividef(m, below) : m / below) * r.rate);
 }
 
 // ---- states in 32 bits ---------------------------------------------------------------
@@ -124,7 +120,6 @@ template <class T>
 __global__ void __launch_bounds__(kThreads) step32_kernel(const __grid_constant__ Table table) {
   const Tensor& t = table.t[tensor_of(table)];
   const Rates r = rates_of(t);
-  const Betas betas(t);
   const long long begin = static_cast<long long>(blockIdx.x - t.first_block) * kPiece;
   const long long end = min(begin + kPiece, t.n);
   T* p = static_cast<T*>(t.p);
@@ -145,7 +140,7 @@ __global__ void __launch_bounds__(kThreads) step32_kernel(const __grid_constant_
       float* vf = reinterpret_cast<float*>(&vv);
 #pragma unroll
       for (int k = 0; k < V; ++k)
-        pf[k] = update(pf[k], gf[k] * table.ascend, mf[k], vf[k], root, betas, r, t.eps);
+        pf[k] = update<false>(pf[k], gf[k] * table.ascend, mf[k], vf[k], root, t, r);
       *reinterpret_cast<Vec<T, V>*>(p + i) = round_values<T, V>(pf);
       *reinterpret_cast<float4*>(m + i) = mv;
       *reinterpret_cast<float4*>(v + i) = vv;
@@ -154,14 +149,14 @@ __global__ void __launch_bounds__(kThreads) step32_kernel(const __grid_constant_
     const long long i = whole + threadIdx.x;
     if (i < end) {
       float root;
-      p[i] = from_float<T>(update(to_float(p[i]), to_float(g[i]) * table.ascend, m[i], v[i], root,
-                                  betas, r, t.eps));
+      p[i] = from_float<T>(update<false>(to_float(p[i]), to_float(g[i]) * table.ascend, m[i], v[i], root,
+                                  t, r));
     }
   } else {
     for (long long i = begin + threadIdx.x; i < end; i += kThreads) {
       float root;
-      p[i] = from_float<T>(update(to_float(p[i]), to_float(g[i]) * table.ascend, m[i], v[i], root,
-                                  betas, r, t.eps));
+      p[i] = from_float<T>(update<false>(to_float(p[i]), to_float(g[i]) * table.ascend, m[i], v[i], root,
+                                  t, r));
     }
   }
 }
@@ -182,16 +177,31 @@ SPLAT_DEV uint32_t dither(long long i, uint32_t step) {
   return h ^ (h >> 16);
 }
 
-// What a code of M bits of mantissa stands for in a run of the given factor; the
-// shifted code is an fp32 number 2^112 below it.
-template <int M>
-SPLAT_DEV float decode(uint32_t c, float factor) {
-  const uint32_t size = M == 3 ? c & 127u : c;
-  const float v = __uint_as_float(size << (23 - M)) * 0x1p112f * factor;
-  return M == 3 && (c & 128u) ? -v : v;
+// What a code of M bits of mantissa stands for in a run of the given factor: the shifted
+// code is an fp32 number 2^112 below it.  Both powers of two are exact, but for results
+// below fp32's normal range, which are rounded once.
+struct Factor {
+  float near, far;  // 2^(112 + E), of which far is what fp32 cannot hold
+};
+SPLAT_DEV Factor factor_of(int exponent) {
+  if (exponent == kNotFinite) return {__uint_as_float(0x7fc00000u), 1.0f};
+  const int near = min(exponent, 15);
+  return {power(112 + near), power(exponent - near)};
 }
-SPLAT_DEV float factor_of(int exponent) {
-  return exponent == kNotFinite ? __uint_as_float(0x7fc00000u) : power(exponent);
+// The four codes of a word.
+template <int M>
+SPLAT_DEV void decode4(uint32_t word, const Factor& factor, float* v) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t top = word << (24 - 8 * k);  // the code in the highest byte
+    const uint32_t bits = M == 3 ? static_cast<uint32_t>(static_cast<int>(top) >> 4) & 0x87f00000u
+                                 : (top >> 5) & 0x07f80000u;
+    v[k] = __uint_as_float(bits) * factor.near;
+  }
+  if (factor.far != 1.0f) {  // of a whole run
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] *= factor.far;
+  }
 }
 
 // The run's exponent from its largest magnitude's bits.
@@ -203,109 +213,179 @@ SPLAT_DEV int exponent_of(uint32_t most) {
   return min(max(e, -126), 127);
 }
 
-// The code of x; noise: 16 bits of a step, the half of which rounds to the nearest.
+// The code of |x| 2^-E = y; noise: 16 bits of a step, the half of which rounds to the
+// nearest.  That of y below the normal codes is taken apart because it is rare.
 template <int M>
-SPLAT_DEV uint32_t encode(float x, float inverse, uint32_t noise) {
+SPLAT_DEV uint32_t encode_normal(float y, uint32_t noise) {
   constexpr int kDrop = 23 - M;
-  const float y = fabsf(x) * inverse;
-  const uint32_t normal =
-      ((__float_as_uint(y) + (noise << (kDrop - 16))) >> kDrop) - (112u << M);
-  const uint32_t small = static_cast<uint32_t>(
-      floorf(__fadd_rn(y * static_cast<float>(1 << (14 + M)), static_cast<float>(noise) * 0x1p-16f)));
-  uint32_t c = y < 0x1p-14f ? small : normal;
-  if constexpr (M == 3) {
-    return min(c, 127u) | (x < 0.0f ? 128u : 0u);
-  } else {
-    c = min(c, 255u);
-    return c == 0 && x > 0.0f ? 1u : c;
-  }
+  return min((__float_as_uint(y) + (noise << (kDrop - 16)) - (112u << 23)) >> kDrop,
+             M == 3 ? 127u : 255u);
 }
-
-// A warp's run: eight values to a lane.
-constexpr int kLane = kRun / 32;
-
-template <class S>
-SPLAT_DEV void load_lane(const S* from, bool vector, int valid, S (&to)[kLane]) {
-  if (vector && valid == kLane) {
-    constexpr int B = sizeof(S) * kLane > 16 ? 16 : sizeof(S) * kLane, V = B / sizeof(S);
-#pragma unroll
-    for (int k = 0; k < kLane; k += V)
-      reinterpret_cast<Vec<S, V>&>(to[k]) = *reinterpret_cast<const Vec<S, V>*>(from + k);
-  } else {
-#pragma unroll
-    for (int k = 0; k < kLane; ++k) to[k] = k < valid ? from[k] : S(0.0f);
-  }
-}
-template <class S>
-SPLAT_DEV void store_lane(S* to, bool vector, int valid, const S (&from)[kLane]) {
-  if (vector && valid == kLane) {
-    constexpr int B = sizeof(S) * kLane > 16 ? 16 : sizeof(S) * kLane, V = B / sizeof(S);
-#pragma unroll
-    for (int k = 0; k < kLane; k += V)
-      *reinterpret_cast<Vec<S, V>*>(to + k) = reinterpret_cast<const Vec<S, V>&>(from[k]);
-  } else {
-#pragma unroll
-    for (int k = 0; k < kLane; ++k)
-      if (k < valid) to[k] = from[k];
-  }
-}
-
-// The codes of a run and its exponent.
 template <int M>
+SPLAT_DEV uint32_t encode_small(float y, uint32_t noise) {
+  const uint32_t c = static_cast<uint32_t>(floorf(__fadd_rn(
+      y * static_cast<float>(1 << (14 + M)), static_cast<float>(noise) * 0x1p-16f)));
+  return M == 4 && c == 0 && y > 0.0f ? 1u : c;
+}
+constexpr float kLeastNormal = 0x1p-14f;
+
+// A warp's run: eight values to a lane, four of each half, so that every access of the
+// warp is contiguous.
+constexpr int kLane = kRun / 32;
+SPLAT_DEV int place_of(int k) { return (k >> 2) * 128 + (threadIdx.x & 31) * 4 + (k & 3); }
+
+// left: values of the run.
+template <class S>
+SPLAT_DEV void load_lane(const S* run, bool vector, int left, S (&to)[kLane]) {
+#pragma unroll
+  for (int k = 0; k < kLane; k += 4) {
+    const int at = place_of(k);
+    if (vector && at + 4 <= left) {
+      reinterpret_cast<Vec<S, 4>&>(to[k]) = *reinterpret_cast<const Vec<S, 4>*>(run + at);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) to[k + j] = at + j < left ? run[at + j] : S(0.0f);
+    }
+  }
+}
+template <class S>
+SPLAT_DEV void store_lane(S* run, bool vector, int left, const S (&from)[kLane]) {
+#pragma unroll
+  for (int k = 0; k < kLane; k += 4) {
+    const int at = place_of(k);
+    if (vector && at + 4 <= left) {
+      *reinterpret_cast<Vec<S, 4>*>(run + at) = reinterpret_cast<const Vec<S, 4>&>(from[k]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (at + j < left) run[at + j] = from[k + j];
+    }
+  }
+}
+SPLAT_DEV int left_of(long long n, long long run) {
+  return static_cast<int>(max(0LL, min(n - run * kRun, static_cast<long long>(kRun))));
+}
+
+// A lane's codes, four to a word.
+SPLAT_DEV void load_codes(const unsigned char* run, bool vector, int left, uint32_t (&w)[2]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int at = place_of(4 * h);
+    w[h] = 0;
+    if (vector && at + 4 <= left) {
+      w[h] = *reinterpret_cast<const uint32_t*>(run + at);
+    } else {
+      for (int j = 0; j < 4; ++j)
+        if (at + j < left) w[h] |= static_cast<uint32_t>(run[at + j]) << (8 * j);
+    }
+  }
+}
+SPLAT_DEV void store_codes(unsigned char* run, bool vector, int left, const uint32_t (&w)[2]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int at = place_of(4 * h);
+    if (vector && at + 4 <= left) {
+      *reinterpret_cast<uint32_t*>(run + at) = w[h];
+    } else {
+      for (int j = 0; j < 4; ++j)
+        if (at + j < left) run[at + j] = static_cast<unsigned char>(w[h] >> (8 * j));
+    }
+  }
+}
+
+// The codes of a run and its exponent; SHIFT: of 16 bits of noise in each word.  Values
+// behind the run's last are zeros.
+template <int M, int SHIFT>
 SPLAT_DEV void store_run(const float (&x)[kLane], const uint32_t (&noise)[kLane], bool vector,
-                         int valid, unsigned char* codes, signed char* exponent) {
+                         int left, unsigned char* codes, signed char* exponent) {
   uint32_t most = 0;
 #pragma unroll
-  for (int k = 0; k < kLane; ++k)
-    if (k < valid) most = max(most, __float_as_uint(x[k]) & 0x7fffffffu);
+  for (int k = 0; k < kLane; ++k) most = max(most, __float_as_uint(x[k]) & 0x7fffffffu);
   most = __reduce_max_sync(0xffffffffu, most);
   const int e = exponent_of<M>(most);
   const float inverse = power(e == kNotFinite ? 0 : -e);
-  alignas(16) unsigned char c[kLane];
+  uint32_t w[2];
+  float least = INFINITY;
 #pragma unroll
-  for (int k = 0; k < kLane; ++k)
-    c[k] = static_cast<unsigned char>(encode<M>(x[k], inverse, noise[k]));
-  store_lane(codes, vector, valid, c);
+  for (int h = 0; h < 2; ++h) {
+    uint32_t c[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = 4 * h + j;
+      const float y = fabsf(x[k]) * inverse;
+      least = fminf(least, y);
+      c[j] = encode_normal<M>(y, noise[k] >> SHIFT & 0xffffu);
+      if (M == 3) c[j] |= __float_as_uint(x[k]) >> 24 & 128u;
+    }
+    w[h] = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+  }
+  if (__any_sync(0xffffffffu, least < kLeastNormal)) {
+#pragma unroll
+    for (int k = 0; k < kLane; ++k) {
+      const float y = fabsf(x[k]) * inverse;
+      const uint32_t c = encode_small<M>(y, noise[k] >> SHIFT & 0xffffu) |
+                         (M == 3 && x[k] < 0.0f ? 128u : 0u);
+      const int at = 8 * (k & 3);
+      if (y < kLeastNormal) w[k >> 2] = (w[k >> 2] & ~(255u << at)) | c << at;
+    }
+  }
+  store_codes(codes, vector, left, w);
   if ((threadIdx.x & 31) == 0) *exponent = static_cast<signed char>(e);
 }
 
+// What a warp reads of a run.
 template <class T>
-__global__ void __launch_bounds__(kThreads) step8_kernel(const __grid_constant__ Table table) {
+struct Run {
+  alignas(16) T p[kLane];
+  alignas(16) T g[kLane];
+  uint32_t m[2], v[2];
+  int m_exponent, v_exponent;
+  SPLAT_DEV void load(const Tensor& t, long long run) {
+    const int left = left_of(t.n, run);
+    const long long i = run * kRun;
+    load_lane(static_cast<const T*>(t.p) + i, t.vector, left, p);
+    load_lane(static_cast<const T*>(t.g) + i, t.vector, left, g);
+    load_codes(static_cast<const unsigned char*>(t.m) + i, t.vector, left, m);
+    load_codes(static_cast<const unsigned char*>(t.v) + i, t.vector, left, v);
+    m_exponent = left ? t.m_exponents[run] : 0;
+    v_exponent = left ? t.v_exponents[run] : 0;
+  }
+};
+
+template <class T>
+__global__ void __launch_bounds__(kThreads, 3) step8_kernel(const __grid_constant__ Table table) {
   const Tensor& t = table.t[tensor_of(table)];
   const Rates r = rates_of(t);
-  const Betas betas(t);
-  const long long block = blockIdx.x - t.first_block;
-  const int lane = threadIdx.x & 31;
-  for (int k = threadIdx.x >> 5; k < kPiece / kRun; k += kThreads / 32) {
-    const long long run = block * (kPiece / kRun) + k;
+  constexpr int kWarps = kThreads / 32;
+  long long run = static_cast<long long>(blockIdx.x - t.first_block) * (kPiece8 / kRun) +
+                  (threadIdx.x >> 5);
+  Run<T> next;
+  next.load(t, run);
+  for (int k = 0; k < kPiece8 / kRun; k += kWarps, run += kWarps) {
     if (run * kRun >= t.n) break;
-    const long long i = run * kRun + lane * kLane;
-    const int valid = static_cast<int>(max(0LL, min(t.n - i, static_cast<long long>(kLane))));
-    alignas(16) T p[kLane], g[kLane];
-    alignas(16) unsigned char mc[kLane], vc[kLane];
-    load_lane(static_cast<const T*>(t.p) + i, t.vector, valid, p);
-    load_lane(static_cast<const T*>(t.g) + i, t.vector, valid, g);
-    load_lane(static_cast<const unsigned char*>(t.m) + i, t.vector, valid, mc);
-    load_lane(static_cast<const unsigned char*>(t.v) + i, t.vector, valid, vc);
-    const float mf = factor_of(t.m_exponents[run]), vf = factor_of(t.v_exponents[run]);
+    Run<T> now = next;
+    if (k + kWarps < kPiece8 / kRun) next.load(t, run + kWarps);
+    const long long i = run * kRun;
+    const int left = left_of(t.n, run);
+    const Factor mf = factor_of(now.m_exponent), vf = factor_of(now.v_exponent);
     float m[kLane], root[kLane];
-    uint32_t low[kLane], high[kLane];
+    uint32_t noise[kLane];
+    decode4<3>(now.m[0], mf, m);
+    decode4<3>(now.m[1], mf, m + 4);
+    decode4<4>(now.v[0], vf, root);
+    decode4<4>(now.v[1], vf, root + 4);
 #pragma unroll
     for (int j = 0; j < kLane; ++j) {
-      m[j] = decode<3>(mc[j], mf);
-      const float before = decode<4>(vc[j], vf);
-      float v = __fmul_rn(before, before);
-      p[j] = from_float<T>(update(to_float(p[j]), to_float(g[j]) * table.ascend, m[j], v, root[j],
-                                  betas, r, t.eps));
-      const uint32_t h = dither(i + j, r.step);
-      low[j] = h & 0xffffu;
-      high[j] = h >> 16;
+      float v = __fmul_rn(root[j], root[j]);
+      now.p[j] = from_float<T>(update<true>(to_float(now.p[j]), to_float(now.g[j]) * table.ascend,
+                                            m[j], v, root[j], t, r));
+      noise[j] = dither(i + place_of(j), r.step);
     }
-    store_lane(static_cast<T*>(t.p) + i, t.vector, valid, p);
-    store_run<3>(m, low, t.vector, valid, static_cast<unsigned char*>(t.m) + i,
-                 t.m_exponents + run);
-    store_run<4>(root, high, t.vector, valid, static_cast<unsigned char*>(t.v) + i,
-                 t.v_exponents + run);
+    store_lane(static_cast<T*>(t.p) + i, t.vector, left, now.p);
+    store_run<3, 0>(m, noise, t.vector, left, static_cast<unsigned char*>(t.m) + i,
+                    t.m_exponents + run);
+    store_run<4, 16>(root, noise, t.vector, left, static_cast<unsigned char*>(t.v) + i,
+                     t.v_exponents + run);
   }
 }
 
@@ -314,43 +394,49 @@ template <bool SQUARED>
 __global__ void __launch_bounds__(kThreads)
     decode_kernel(long long n, const unsigned char* codes, const signed char* exponents,
                   bool vector, float* values) {
-  const int lane = threadIdx.x & 31;
+  constexpr int U = 2;  // runs in flight
   const long long runs = (n + kRun - 1) / kRun, step = gridDim.x * (kThreads / 32LL);
-  for (long long run = blockIdx.x * (kThreads / 32LL) + (threadIdx.x >> 5); run < runs;
-       run += step) {
-    const long long i = run * kRun + lane * kLane;
-    const int valid = static_cast<int>(max(0LL, min(n - i, static_cast<long long>(kLane))));
-    alignas(16) unsigned char c[kLane];
-    alignas(16) float v[kLane];
-    load_lane(codes + i, vector, valid, c);
-    const float factor = factor_of(exponents[run]);
+  for (long long run0 = blockIdx.x * (kThreads / 32LL) + (threadIdx.x >> 5); run0 < runs;
+       run0 += U * step) {
+    uint32_t c[U][2];
+    int e[U], left[U];
 #pragma unroll
-    for (int k = 0; k < kLane; ++k) {
-      v[k] = decode<SQUARED ? 4 : 3>(c[k], factor);
-      if (SQUARED) v[k] = __fmul_rn(v[k], v[k]);
+    for (int u = 0; u < U; ++u) {
+      const long long run = run0 + u * step;
+      left[u] = left_of(n, run);
+      load_codes(codes + run * kRun, vector, left[u], c[u]);
+      e[u] = run < runs ? exponents[run] : 0;
     }
-    store_lane(values + i, vector, valid, v);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const Factor factor = factor_of(e[u]);
+      alignas(16) float v[kLane];
+      decode4<SQUARED ? 4 : 3>(c[u][0], factor, v);
+      decode4<SQUARED ? 4 : 3>(c[u][1], factor, v + 4);
+      if (SQUARED)
+#pragma unroll
+        for (int k = 0; k < kLane; ++k) v[k] = __fmul_rn(v[k], v[k]);
+      store_lane(values + (run0 + u * step) * kRun, vector, left[u], v);
+    }
   }
 }
 template <bool SQUARED>
 __global__ void __launch_bounds__(kThreads)
     encode_kernel(long long n, const float* values, bool vector, unsigned char* codes,
                   signed char* exponents) {
-  const int lane = threadIdx.x & 31;
   const long long runs = (n + kRun - 1) / kRun, step = gridDim.x * (kThreads / 32LL);
   for (long long run = blockIdx.x * (kThreads / 32LL) + (threadIdx.x >> 5); run < runs;
        run += step) {
-    const long long i = run * kRun + lane * kLane;
-    const int valid = static_cast<int>(max(0LL, min(n - i, static_cast<long long>(kLane))));
+    const int left = left_of(n, run);
     alignas(16) float v[kLane];
     uint32_t half[kLane];
-    load_lane(values + i, vector, valid, v);
+    load_lane(values + run * kRun, vector, left, v);
 #pragma unroll
     for (int k = 0; k < kLane; ++k) {
       if (SQUARED) v[k] = __fsqrt_rn(v[k]);
       half[k] = 0x8000u;
     }
-    store_run<SQUARED ? 4 : 3>(v, half, vector, valid, codes + i, exponents + run);
+    store_run<SQUARED ? 4 : 3, 0>(v, half, vector, left, codes + run * kRun, exponents + run);
   }
 }
 
@@ -406,7 +492,8 @@ int splat_adamw(int dtype, int bits, int count, const SplatAdamwTensor* tensors,
     for (; next < count && table.count < kMostTensors; ++next) {
       const SplatAdamwTensor& from = tensors[next];
       if (!from.n) continue;
-      const long long more = (from.n + kPiece - 1) / kPiece;
+      const int piece = bits == 8 ? kPiece8 : kPiece;
+      const long long more = (from.n + piece - 1) / piece;
       if (blocks && blocks + more >= 1LL << 31) break;
       Tensor& t = table.t[table.count++];
       t.p = from.p, t.g = from.g, t.m = from.m, t.v = from.v;
@@ -414,6 +501,8 @@ int splat_adamw(int dtype, int bits, int count, const SplatAdamwTensor* tensors,
       t.v_exponents = static_cast<signed char*>(from.v_exponents);
       t.device_step = from.device_step, t.device_lr = from.device_lr;
       t.lr = from.lr, t.decay = from.weight_decay, t.beta1 = from.beta1, t.beta2 = from.beta2;
+      t.b1 = static_cast<float>(t.beta1), t.c1 = static_cast<float>(1.0 - t.beta1);
+      t.b2 = static_cast<float>(t.beta2), t.c2 = static_cast<float>(1.0 - t.beta2);
       t.n = from.n, t.eps = static_cast<float>(from.eps);
       t.step = static_cast<uint32_t>(from.step);
       t.shrink = static_cast<float>(1.0 - t.lr * t.decay);
