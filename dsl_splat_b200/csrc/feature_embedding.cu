@@ -2,8 +2,8 @@
 //
 //   y_i = s T[id_i]          dT[v] = s sum of dy_i over id_i = v
 //
-// Bound by memory.  The gradient sorts the rows' indices by id (a stable counting
-// sort of up to 13 bits of the id a pass), walks them in that order and adds up
+// Bound by memory.  The gradient sorts the rows by id (a stable counting
+// sort of up to 10 bits of the id a pass), walks them in that order and adds up
 // each entry's run in fp32: a group of lanes to a few rows, the runs that cross
 // groups joined in shared memory and those that cross blocks by a second kernel,
 // all in the order of the rows, so that no result depends on the order of blocks.
@@ -28,47 +28,52 @@ SPLAT_DEV int id_at(const void* ids, long long i, int entries) {
 
 // ---- forward -----------------------------------------------------------------------
 
-// Rows of `units` pieces of V values, `lanes` threads to a row.
+// Rows of `units` pieces of V values, `lanes` threads to a row; a warp takes 32 rows, whose
+// ids its lanes read at once.
 template <class T, class I, int V>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 5)
     lookup_kernel(long long count, int entries, int channels, int units, int lanes,
                   const void* ids, const T* table, float scale, T* y, int* error) {
   constexpr int U = 4;  // rows in flight
   using Piece = Vec<T, V>;
-  const int lane = threadIdx.x & (lanes - 1);
-  const long long groups = static_cast<long long>(gridDim.x) * (kThreads / lanes);
-  const long long first = blockIdx.x * static_cast<long long>(kThreads / lanes) +
-                          threadIdx.x / lanes;
-  for (long long i0 = first; i0 < count; i0 += U * groups) {
-    int id[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      id[u] = -1;
-      if (i0 + u * groups < count) {
-        id[u] = id_at<I>(ids, i0 + u * groups, entries);
-        if (id[u] < 0 && lane == 0) atomicCAS(error, 0, kInconsistentInput);
-      }
+  const int lane = threadIdx.x & (lanes - 1), group = (threadIdx.x & 31) / lanes;
+  const int groups = 32 / lanes;
+  const long long step = gridDim.x * static_cast<long long>(kThreads);
+  for (long long row0 = blockIdx.x * static_cast<long long>(kThreads) + (threadIdx.x & ~31u);
+       row0 < count; row0 += step) {
+    const long long own = row0 + (threadIdx.x & 31);
+    int id = -1;
+    if (own < count) {
+      id = id_at<I>(ids, own, entries);
+      if (id < 0) atomicCAS(error, 0, kInconsistentInput);
     }
-    for (int q = lane; q < units; q += lanes) {
-      Piece v[U];
+    const int rows = static_cast<int>(min(count - row0, 32LL));
+    for (int r0 = group; r0 < 32; r0 += U * groups) {
+      int at[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        v[u] = Piece{};
-        if (id[u] >= 0)
-          v[u] = *reinterpret_cast<const Piece*>(table + static_cast<long long>(id[u]) * channels +
-                                                 q * V);
-      }
+      for (int u = 0; u < U; ++u)
+        at[u] = __shfl_sync(0xffffffffu, id, (r0 + u * groups) & 31);
+      for (int q = lane; q < units; q += lanes) {
+        Piece v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (scale != 1.0f) {
-          float f[V];
-          widen<T, V>(v[u], f);
-#pragma unroll
-          for (int k = 0; k < V; ++k) f[k] *= scale;
-          v[u] = round_values<T, V>(f);
+        for (int u = 0; u < U; ++u) {
+          v[u] = Piece{};
+          if (r0 + u * groups < rows && at[u] >= 0)
+            v[u] = *reinterpret_cast<const Piece*>(
+                table + static_cast<long long>(at[u]) * channels + q * V);
         }
-        if (i0 + u * groups < count)
-          *reinterpret_cast<Piece*>(y + (i0 + u * groups) * channels + q * V) = v[u];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (scale != 1.0f) {
+            float f[V];
+            widen<T, V>(v[u], f);
+#pragma unroll
+            for (int k = 0; k < V; ++k) f[k] *= scale;
+            v[u] = round_values<T, V>(f);
+          }
+          if (r0 + u * groups < rows)
+            *reinterpret_cast<Piece*>(y + (row0 + r0 + u * groups) * channels + q * V) = v[u];
+        }
       }
     }
   }
@@ -76,25 +81,35 @@ __global__ void __launch_bounds__(kThreads)
 
 // ---- sorting indices by id ---------------------------------------------------------
 
-constexpr int kMostBits = 13;  // of a pass: 160 KB of counters in place_kernel
+// Bits of a pass.  A million rows of 13 bits in one pass, whose 8192 counters for each
+// warp leave an SM one block, took 50 us, in two passes of 7 and 6 bits 45.
+constexpr int kMostBits = 10;
+
+// A row and its id.
+struct Sorted {
+  int row, id;
+};
 
 struct SortPass {
   const void* ids;
-  const int* order;       // of the pass before; NULL: as they lie
+  const Sorted* order;    // of the pass before; NULL: as they lie
   const int* valid;       // how many of them (with `order`)
   long long count;
   int entries, shift, bins;
-  int* counts;            // (blocks, bins)
+  int* counts;            // (bins, blocks)
   int* totals;            // (bins)
-  int* out;
+  Sorted* out;
   int* out_valid;
 };
 
+// id: -1 outside the table, and from `end` on.
 template <class I>
-SPLAT_DEV int sort_key(const SortPass& p, long long i, int& index) {
-  index = p.order ? p.order[i] : static_cast<int>(i);
-  return id_at<I>(p.ids, index, p.entries);
+SPLAT_DEV Sorted sort_item(const SortPass& p, long long i, long long end) {
+  if (i >= end) return {0, -1};
+  if (p.order) return p.order[i];
+  return {static_cast<int>(i), id_at<I>(p.ids, i, p.entries)};
 }
+constexpr int kAhead = 8;  // items that a thread reads at once
 
 // Rows of a block: whole warps' worth to each warp.
 SPLAT_DEV long long rows_per_warp(long long count) {
@@ -104,90 +119,117 @@ SPLAT_DEV long long rows_per_warp(long long count) {
 
 template <class I>
 __global__ void __launch_bounds__(kThreads) count_digits_kernel(const SortPass p) {
-  extern __shared__ int bins[];
+  extern __shared__ __align__(16) int bins[];
   const long long count = p.order ? *p.valid : p.count;
   for (int d = threadIdx.x; d < p.bins; d += kThreads) bins[d] = 0;
   __syncthreads();
   const long long per = rows_per_warp(count) * kWarps;
   const long long begin = blockIdx.x * per, end = min(begin + per, count);
-#pragma unroll 4
-  for (long long i = begin + threadIdx.x; i < end; i += kThreads) {
-    int index;
-    const int key = sort_key<I>(p, i, index);
-    if (key >= 0) atomicAdd(&bins[(key >> p.shift) & (p.bins - 1)], 1);
+  for (long long i0 = begin + threadIdx.x; i0 < end; i0 += kAhead * kThreads) {
+    Sorted v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) v[u] = sort_item<I>(p, i0 + u * kThreads, end);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (v[u].id >= 0) atomicAdd(&bins[(v[u].id >> p.shift) & (p.bins - 1)], 1);
   }
   __syncthreads();
   for (int d = threadIdx.x; d < p.bins; d += kThreads)
-    p.counts[static_cast<long long>(blockIdx.x) * p.bins + d] = bins[d];
+    p.counts[static_cast<long long>(d) * gridDim.x + blockIdx.x] = bins[d];
 }
 
-// Of each digit, what the blocks before have.
+// Of each digit, what the blocks before have: a warp to a digit.
 __global__ void __launch_bounds__(kThreads) digit_prefix_kernel(const SortPass p, int blocks) {
-  const int d = blockIdx.x * kThreads + threadIdx.x;
+  const int d = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (d >= p.bins) return;
-  int sum = 0;
-  constexpr int U = 16;
-  for (int b0 = 0; b0 < blocks; b0 += U) {
-    int v[U];
+  int* counts = p.counts + static_cast<long long>(d) * blocks;
+  int carry = 0;
+  for (int b0 = 0; b0 < blocks; b0 += 32 * kAhead) {
+    int v[kAhead];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      v[u] = b0 + u < blocks ? p.counts[static_cast<long long>(b0 + u) * p.bins + d] : 0;
+    for (int u = 0; u < kAhead; ++u) {
+      const int b = b0 + u * 32 + lane;
+      v[u] = b < blocks ? counts[b] : 0;
+    }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (b0 + u < blocks) p.counts[static_cast<long long>(b0 + u) * p.bins + d] = sum;
-      sum += v[u];
+    for (int u = 0; u < kAhead; ++u) {
+      int upto = v[u];
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int before = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += before;
+      }
+      const int b = b0 + u * 32 + lane;
+      if (b < blocks) counts[b] = carry + upto - v[u];
+      carry += __shfl_sync(0xffffffffu, upto, 31);
     }
   }
-  p.totals[d] = sum;
+  if (lane == 0) p.totals[d] = carry;
 }
 
 // Places a block's indices: each warp takes consecutive rows in their order, so
 // that equal digits keep it.
 template <class I>
 __global__ void __launch_bounds__(kThreads) place_kernel(const SortPass p) {
-  extern __shared__ int bins[];                                            // first places
-  unsigned short* own = reinterpret_cast<unsigned short*>(bins + p.bins);  // (warps, bins)
+  extern __shared__ __align__(16) int bins[];  // first places
+  unsigned short* own = reinterpret_cast<unsigned short*>(bins + (p.bins + 3) / 4 * 4);  // (warps, bins)
   __shared__ int warp_sums[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long count = p.order ? *p.valid : p.count;
   const long long per = rows_per_warp(count);
   const long long begin = (static_cast<long long>(blockIdx.x) * kWarps + warp) * per;
   const long long end = min(begin + per, count);
-  // the digits' first places: an exclusive sum of the totals
-  const int each = (p.bins + kThreads - 1) / kThreads;
-  int sum = 0;
-  for (int k = 0; k < each; ++k) {
-    const int d = threadIdx.x * each + k;
-    if (d < p.bins) sum += p.totals[d];
-  }
-  int upto = sum;
+  // the digits' first places: an exclusive sum of the totals, of which each warp takes a part
+  const int part = (p.bins + 32 * kWarps - 1) / (32 * kWarps) * 32;
+  const int part_begin = min(warp * part, p.bins), part_end = min(part_begin + part, p.bins);
+  int carry = 0;
+  for (int d0 = part_begin; d0 < part_end; d0 += 32 * kAhead) {
+    int v[kAhead];
 #pragma unroll
-  for (int o = 1; o < 32; o *= 2) {
-    const int v = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += v;
+    for (int u = 0; u < kAhead; ++u) {
+      const int d = d0 + u * 32 + lane;
+      v[u] = d < part_end ? p.totals[d] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      int upto = v[u];
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int before = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += before;
+      }
+      const int d = d0 + u * 32 + lane;
+      if (d < part_end) bins[d] = carry + upto - v[u];
+      carry += __shfl_sync(0xffffffffu, upto, 31);
+    }
   }
-  if (lane == 31) warp_sums[warp] = upto;
-  for (int i = threadIdx.x; i < kWarps * p.bins / 2; i += kThreads)
-    reinterpret_cast<int*>(own)[i] = 0;
+  if (lane == 0) warp_sums[warp] = carry;
+  uint4* zeros = reinterpret_cast<uint4*>(own);
+  for (int i = threadIdx.x; i < kWarps * p.bins / 8; i += kThreads)
+    zeros[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
-  int place = upto - sum;
-  for (int w = 0; w < warp; ++w) place += warp_sums[w];
-  if (blockIdx.x == 0 && threadIdx.x == kThreads - 1) *p.out_valid = place + sum;
-  for (int k = 0; k < each; ++k) {
-    const int d = threadIdx.x * each + k;
-    if (d >= p.bins) break;
-    bins[d] = place + p.counts[static_cast<long long>(blockIdx.x) * p.bins + d];
-    place += p.totals[d];
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    int all = 0;
+    for (int w = 0; w < kWarps; ++w) all += warp_sums[w];
+    *p.out_valid = all;
+  }
+  for (int d = threadIdx.x; d < p.bins; d += kThreads) {
+    int place = bins[d] + p.counts[static_cast<long long>(d) * gridDim.x + blockIdx.x];
+    for (int w = 0; w < d / part; ++w) place += warp_sums[w];
+    bins[d] = place;
   }
   // the warps' counts, two to a word (a block has less than 2^16 rows, see plan_sort)
   int* words = reinterpret_cast<int*>(own + static_cast<long long>(warp) * p.bins);
-#pragma unroll 4
-  for (long long i = begin + lane; i < end; i += 32) {
-    int index;
-    const int key = sort_key<I>(p, i, index);
-    if (key < 0) continue;
-    const int d = (key >> p.shift) & (p.bins - 1);
-    atomicAdd(&words[d >> 1], 1 << ((d & 1) * 16));
+  for (long long i0 = begin + lane; i0 < end; i0 += kAhead * 32) {
+    Sorted v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) v[u] = sort_item<I>(p, i0 + u * 32, end);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (v[u].id < 0) continue;
+      const int d = (v[u].id >> p.shift) & (p.bins - 1);
+      atomicAdd(&words[d >> 1], 1 << ((d & 1) * 16));
+    }
   }
   __syncthreads();
   for (int d = threadIdx.x; d < p.bins; d += kThreads) {
@@ -201,18 +243,22 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const SortPass p) {
   }
   __syncthreads();
   unsigned short* next = own + static_cast<long long>(warp) * p.bins;
-  for (long long i0 = begin; i0 < end; i0 += 32) {
-    int index = 0, key = -1;
-    if (i0 + lane < end) key = sort_key<I>(p, i0 + lane, index);
-    const int d = key >= 0 ? (key >> p.shift) & (p.bins - 1) : -1;
-    const uint32_t peers = __match_any_sync(0xffffffffu, d);
-    const int rank = __popc(peers & lanemask_lt());
-    int first = 0;
-    if (key >= 0) first = next[d];
-    __syncwarp();
-    if (key >= 0 && rank == 0) next[d] = static_cast<unsigned short>(first + __popc(peers));
-    __syncwarp();
-    if (key >= 0) p.out[bins[d] + first + rank] = index;
+  for (long long i0 = begin; i0 < end; i0 += kAhead * 32) {
+    Sorted v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) v[u] = sort_item<I>(p, i0 + u * 32 + lane, end);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int d = v[u].id >= 0 ? (v[u].id >> p.shift) & (p.bins - 1) : -1;
+      const uint32_t peers = __match_any_sync(0xffffffffu, d);
+      const int rank = __popc(peers & lanemask_lt());
+      int first = 0;
+      if (d >= 0) first = next[d];
+      __syncwarp();
+      if (d >= 0 && rank == 0) next[d] = static_cast<unsigned short>(first + __popc(peers));
+      __syncwarp();
+      if (d >= 0) p.out[bins[d] + first + rank] = v[u];
+    }
   }
 }
 
@@ -225,10 +271,9 @@ constexpr int kHead = 1, kThrough = 2, kTail = 4;
 constexpr int kMostBlockRows = 2048;
 
 struct RunParams {
-  const void* ids;
-  const int* order;
+  const Sorted* order;
   const int* valid;
-  int entries, channels, lanes, rows;  // rows of a group
+  int channels, lanes, rows;  // rows of a group
   const void* dy;
   float scale;
   void* dtable;
@@ -236,8 +281,8 @@ struct RunParams {
   int* flags;            // (blocks)
 };
 
-template <class T, class I, int V>
-__global__ void __launch_bounds__(kThreads) sum_runs_kernel(const RunParams p) {
+template <class T, int V>
+__global__ void __launch_bounds__(kThreads, 4) sum_runs_kernel(const RunParams p) {
   using Piece = Vec<T, V>;
   __shared__ int index[kMostBlockRows], key_at[kMostBlockRows + 2];
   __shared__ float head[kThreads * V], tail[kThreads * V];
@@ -255,9 +300,9 @@ __global__ void __launch_bounds__(kThreads) sum_runs_kernel(const RunParams p) {
     const int at = begin + i - 1;
     int key = -1;
     if (at >= 0 && at < count) {
-      const int row = p.order[at];
-      key = id_at<I>(p.ids, row, p.entries);
-      if (i > 0 && i <= rows) index[i - 1] = row;
+      const Sorted v = p.order[at];
+      key = v.id;
+      if (i > 0 && i <= rows) index[i - 1] = v.row;
     }
     key_at[i] = key;
   }
@@ -356,7 +401,7 @@ __global__ void __launch_bounds__(kThreads) sum_runs_kernel(const RunParams p) {
 }
 
 // The runs across blocks.
-template <class T, class I>
+template <class T>
 __global__ void __launch_bounds__(kThreads) join_runs_kernel(const RunParams p, int block_rows) {
   if (!(p.flags[blockIdx.x] & kTail)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -372,8 +417,7 @@ __global__ void __launch_bounds__(kThreads) join_runs_kernel(const RunParams p, 
     }
     end += 32;
   }
-  const int key = id_at<I>(
-      p.ids, p.order[static_cast<long long>(blockIdx.x + 1) * block_rows - 1], p.entries);
+  const int key = p.order[static_cast<long long>(blockIdx.x + 1) * block_rows - 1].id;
   __shared__ float sums[kWarps][32];
   for (int c0 = blockIdx.y * 32; c0 < p.channels; c0 += gridDim.y * 32) {
     const int c = c0 + lane;
@@ -437,9 +481,12 @@ int check_embedding(int dtype, int id_bytes, long long count, int entries, int c
   return kOk;
 }
 
+// Whether each entry looks for its rows: 64 rows of 8192 entries x 512 (2^18 steps of a
+// warp) take 17 us, sorting them 47, most of which is the launches'; 256 rows of 65536 x 32
+// (2^19) about as long as sorted.
 bool scans(long long count, int entries, int channels) {
   return count <= kMostScanned &&
-         (count + 31) / 32 * entries * ((channels + 31) / 32) <= 1LL << 18;
+         (count + 31) / 32 * entries * ((channels + 31) / 32) <= 1LL << 19;
 }
 
 struct EmbeddingPlan {
@@ -458,7 +505,7 @@ EmbeddingPlan plan_embedding(long long count, int entries, int channels, int val
     plan.bits[i] = bits / plan.passes + (i < bits % plan.passes);
   // 2^15 rows to a block at most: its warps count in 16 bits
   plan.sort_blocks = static_cast<int>(std::max<long long>(
-      std::min<long long>((count + 2047) / 2048, host::sm_count()), (count + 32767) / 32768));
+      std::min<long long>((count + 2047) / 2048, 8LL * host::sm_count()), (count + 32767) / 32768));
   const int units = (channels + values - 1) / values;
   plan.lanes = 1;
   while (plan.lanes < 32 && plan.lanes < units) plan.lanes *= 2;
@@ -473,8 +520,8 @@ EmbeddingPlan plan_embedding(long long count, int entries, int channels, int val
     return at;
   };
   plan.flags = take(4ull * plan.run_blocks);
-  plan.order = take(4ull * count);
-  plan.order2 = plan.passes > 1 ? take(4ull * count) : plan.order;
+  plan.order = take(sizeof(Sorted) * count);
+  plan.order2 = plan.passes > 1 ? take(sizeof(Sorted) * count) : plan.order;
   plan.counts = take(4ull * plan.sort_blocks << kMostBits);
   plan.totals = take(4ull << kMostBits);
   plan.valid = take(16);
@@ -502,9 +549,8 @@ int launch_lookup(long long count, int entries, int channels, const void* ids, c
   const int units = channels / v;
   int lanes = 1;
   while (lanes < 32 && lanes < units) lanes *= 2;
-  const long long rows = kThreads / lanes;
   const unsigned grid = static_cast<unsigned>(
-      std::min<long long>((count + rows - 1) / rows, 16LL * host::sm_count()));
+      std::min<long long>((count + kThreads - 1) / kThreads, 1LL << 30));
   const auto run = [&](auto* kernel) {
     kernel<<<grid, kThreads, 0, host::counted(s)>>>(count, entries, channels, units, lanes, ids,
                                                     static_cast<const T*>(table), scale,
@@ -532,14 +578,12 @@ int launch_gradient(long long count, int entries, int channels, const void* ids,
   constexpr int V = 16 / sizeof(T);
   const int v = piece_values<T>(channels, dy, dtable) == V ? V : 1;
   const EmbeddingPlan plan = plan_embedding(count, entries, channels, v);
-  if (!host::allow_shared<place_kernel<I>>())
-    return host::check_launch("feature_embedding_backward: shared memory");
   if (cudaMemsetAsync(dtable, 0, sizeof(T) * entries * static_cast<size_t>(channels), s) !=
           cudaSuccess ||
       cudaMemsetAsync(ws + plan.flags, 0, 4ull * plan.run_blocks, s) != cudaSuccess)
     return host::check_launch("feature_embedding_backward: zeros");
   int shift = 0;
-  const int* order = nullptr;
+  const Sorted* order = nullptr;
   int* valid = reinterpret_cast<int*>(ws + plan.valid);
   for (int i = 0; i < plan.passes; ++i) {
     SortPass p{};
@@ -548,26 +592,27 @@ int launch_gradient(long long count, int entries, int channels, const void* ids,
     p.shift = shift, p.bins = 1 << plan.bits[i];
     p.counts = reinterpret_cast<int*>(ws + plan.counts);
     p.totals = reinterpret_cast<int*>(ws + plan.totals);
-    p.out = reinterpret_cast<int*>(ws + (i % 2 ? plan.order2 : plan.order));
+    p.out = reinterpret_cast<Sorted*>(ws + (i % 2 ? plan.order2 : plan.order));
     count_digits_kernel<I><<<plan.sort_blocks, kThreads, 4 * p.bins, host::counted(s)>>>(p);
-    digit_prefix_kernel<<<host::blocks_for(p.bins, kThreads), kThreads, 0, host::counted(s)>>>(
+    digit_prefix_kernel<<<host::blocks_for(p.bins, kWarps), kThreads, 0, host::counted(s)>>>(
         p, plan.sort_blocks);
-    place_kernel<I><<<plan.sort_blocks, kThreads, (4 + 2 * kWarps) * p.bins, host::counted(s)>>>(p);
+    place_kernel<I><<<plan.sort_blocks, kThreads, 4 * ((p.bins + 3) / 4 * 4) + 2 * kWarps * p.bins,
+                      host::counted(s)>>>(p);
     order = p.out;
     shift += plan.bits[i];
   }
   RunParams r{};
-  r.ids = ids, r.order = order, r.valid = valid + (plan.passes - 1) % 2;
-  r.entries = entries, r.channels = channels, r.lanes = plan.lanes, r.rows = plan.rows;
+  r.order = order, r.valid = valid + (plan.passes - 1) % 2;
+  r.channels = channels, r.lanes = plan.lanes, r.rows = plan.rows;
   r.dy = dy, r.scale = scale, r.dtable = dtable;
   r.heads = reinterpret_cast<float*>(ws + plan.heads);
   r.tails = reinterpret_cast<float*>(ws + plan.tails);
   r.flags = reinterpret_cast<int*>(ws + plan.flags);
   const dim3 grid(plan.run_blocks, plan.columns);
-  if (v == V) sum_runs_kernel<T, I, V><<<grid, kThreads, 0, host::counted(s)>>>(r);
-  else sum_runs_kernel<T, I, 1><<<grid, kThreads, 0, host::counted(s)>>>(r);
+  if (v == V) sum_runs_kernel<T, V><<<grid, kThreads, 0, host::counted(s)>>>(r);
+  else sum_runs_kernel<T, 1><<<grid, kThreads, 0, host::counted(s)>>>(r);
   const dim3 join_grid(plan.run_blocks, std::min((channels + 31) / 32, 64));
-  join_runs_kernel<T, I><<<join_grid, kThreads, 0, host::counted(s)>>>(r, plan.block_rows);
+  join_runs_kernel<T><<<join_grid, kThreads, 0, host::counted(s)>>>(r, plan.block_rows);
   return host::check_launch("feature_embedding_backward");
 }
 

@@ -234,27 +234,38 @@ void add_columns(int vocabulary, int ranges, const float* sums, bool begin, floa
                        host::counted(s)>>>(vocabulary, ranges, sums, begin, total);
 }
 
-// fp32 sums (of several splits, `stride` values apart) times the factor, rounded.
-template <class T>
+// fp32 sums (of several splits, `stride` values apart) times the factor, rounded; V of
+// them to an access.
+template <class T, int V>
 __global__ void __launch_bounds__(kThreads)
     finish_kernel(long long count, int splits, long long stride, const float* from,
                   const Factors* factors, T* to) {
   const float factor = factors->out;
-  for (long long i = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i < count;
-       i += static_cast<long long>(kThreads) * gridDim.x) {
-    float sum = 0.0f;
+  const long long step = static_cast<long long>(kThreads) * gridDim.x * V;
+  for (long long i = (blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x) * V; i < count;
+       i += step) {
+    float sum[V] = {};
 #pragma unroll 4
-    for (int s = 0; s < splits; ++s) sum += from[s * stride + i];
-    to[i] = from_float<T>(sum * factor);
+    for (int s = 0; s < splits; ++s) {
+      const Vec<float, V> v = *reinterpret_cast<const Vec<float, V>*>(from + s * stride + i);
+#pragma unroll
+      for (int k = 0; k < V; ++k) sum[k] += v.v[k];
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) sum[k] *= factor;
+    *reinterpret_cast<Vec<T, V>*>(to + i) = round_values<T, V>(sum);
   }
 }
 template <class T>
 void finish(long long count, int splits, long long stride, const float* from,
             const Factors* factors, void* to, cudaStream_t s) {
+  const bool vector = count % 4 == 0 && stride % 4 == 0 && host::aligned(to, 4 * sizeof(T));
+  const int per_block = kThreads * (vector ? 4 : 1);
   const unsigned grid = static_cast<unsigned>(
-      std::min<long long>((count + kThreads - 1) / kThreads, 16LL * host::sm_count()));
-  finish_kernel<T><<<grid, kThreads, 0, host::counted(s)>>>(count, splits, stride, from, factors,
-                                                            static_cast<T*>(to));
+      std::min<long long>((count + per_block - 1) / per_block, 1LL << 30));
+  auto* kernel = vector ? finish_kernel<T, 4> : finish_kernel<T, 1>;
+  kernel<<<grid, kThreads, 0, host::counted(s)>>>(count, splits, stride, from, factors,
+                                                  static_cast<T*>(to));
 }
 
 // ---- launching -----------------------------------------------------------------------
