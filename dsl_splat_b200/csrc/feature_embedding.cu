@@ -655,7 +655,7 @@ int splat_feature_embedding_backward(int dtype, int id_bytes, long long count, i
                                      void* stream) {
   const int bad = check_embedding(dtype, id_bytes, count, entries, channels);
   if (bad != kOk) return bad;
-  if (!ids || !dy || !dtable || !workspace)
+  if (!ids || !dy || !dtable || (!workspace && !scans(count, entries, channels)))
     return host::fail(kInvalidArgument, "feature_embedding_backward: null pointer");
   if (!host::aligned(workspace, 16))
     return host::fail(kInvalidArgument,

@@ -54,12 +54,20 @@ cudaStream_t counted(cudaStream_t s) {
   return s;
 }
 
+// What never changes in a process is asked for once per device.
+constexpr int kMostDevices = 64;
+
 int* device_error_word() {
-  void* word = nullptr;
+  static void* words[kMostDevices] = {};
+  int dev = -1;
+  const bool kept = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMostDevices;
+  void* word = kept ? __atomic_load_n(&words[dev], __ATOMIC_RELAXED) : nullptr;
+  if (word) return static_cast<int*>(word);
   if (cudaGetSymbolAddress(&word, g_splat_device_error) != cudaSuccess) {
     check_launch("device_error_word");
     return nullptr;
   }
+  if (kept) __atomic_store_n(&words[dev], word, __ATOMIC_RELAXED);
   return static_cast<int*>(word);
 }
 
@@ -91,9 +99,14 @@ bool encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, lo
 }
 
 int sm_count() {
-  int sms = 148, dev = 0;
-  if (cudaGetDevice(&dev) == cudaSuccess)
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  static int counts[kMostDevices] = {};
+  int sms = 148, dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess) return sms;
+  const bool kept = dev >= 0 && dev < kMostDevices;
+  const int known = kept ? __atomic_load_n(&counts[dev], __ATOMIC_RELAXED) : 0;
+  if (known) return known;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && kept)
+    __atomic_store_n(&counts[dev], sms, __ATOMIC_RELAXED);
   return sms;
 }
 

@@ -23,6 +23,7 @@ The reference has no counterpart; its users bring their own optimizer.
 from __future__ import annotations
 
 import math
+import struct
 from numbers import Integral, Real
 from typing import Any, Callable, Iterable, Sequence
 
@@ -30,9 +31,9 @@ import torch
 from torch import Tensor
 
 from . import stages
-from ._native import SplatAdamwTensor
 
 RUN = 256  # values that share an exponent
+_RECORD = struct.Struct("=10q5d")  # a SplatAdamwTensor of include/splat200.h
 
 
 class Moment8:
@@ -81,6 +82,8 @@ def _check_settings(betas: tuple[float, float], eps: float, weight_decay: float)
 
 
 def _check_lr(lr: Any) -> None:
+    if type(lr) is float and 0.0 <= lr < math.inf:
+        return
     if isinstance(lr, Tensor):
         if lr.numel() != 1 or not lr.is_cuda or lr.dtype is not torch.float32:
             raise ValueError("lr must be a number or a CUDA float32 tensor of one value")
@@ -89,6 +92,8 @@ def _check_lr(lr: Any) -> None:
 
 
 def _check_step(step: Any) -> None:
+    if type(step) is int and step >= 1:
+        return
     if isinstance(step, Tensor):
         if step.numel() != 1 or not step.is_cuda or step.dtype is not torch.int64:
             raise ValueError("step must be an integer or a CUDA int64 tensor of one value")
@@ -105,12 +110,13 @@ def _check_parameter(p: Tensor) -> None:
 
 def _check_moment(m: Any, p: Tensor, squared: bool) -> int:
     if isinstance(m, Moment8):
-        if m.codes.shape != p.shape or m.codes.device != p.device or m.squared != squared:
+        if (m.codes.shape != p.shape or m.codes.get_device() != p.get_device()
+                or m.squared != squared):
             raise ValueError("8-bit moments must have their parameter's shape and device, and "
                              "the second ones be squared")
         return 8
     if (not isinstance(m, Tensor) or m.dtype is not torch.float32 or m.shape != p.shape
-            or m.device != p.device or not m.is_contiguous()):
+            or m.get_device() != p.get_device() or not m.is_contiguous()):
         raise ValueError("moments must be contiguous float32 tensors, or Moment8, of their "
                          "parameter's shape and device")
     return 32
@@ -140,14 +146,21 @@ class _Launches:
         _check_parameter(p)
         if not isinstance(g, Tensor) or g.layout is not torch.strided:
             raise ValueError("gradients must be dense tensors")
-        if g.dtype is not p.dtype or g.device != p.device or g.shape != p.shape:
+        index = p.get_device()
+        if g.dtype is not p.dtype or g.get_device() != index or g.shape != p.shape:
             raise ValueError("gradients must have their parameter's dtype, device and shape")
         bits = _check_moment(m, p, False)
         if _check_moment(v, p, True) != bits:
             raise ValueError("both moments must be held in the same number of bits")
-        for t in (step, lr):
-            if isinstance(t, Tensor) and t.device != p.device:
+        device_step = device_lr = 0
+        if isinstance(step, Tensor):
+            if step.get_device() != index:
                 raise ValueError("step and lr tensors must be on their parameter's device")
+            device_step, step = step.data_ptr(), 0
+        if isinstance(lr, Tensor):
+            if lr.get_device() != index:
+                raise ValueError("step and lr tensors must be on their parameter's device")
+            device_lr, lr = lr.data_ptr(), 0.0
         n = p.numel()
         if not n:
             return
@@ -158,24 +171,20 @@ class _Launches:
         if address in self.places:
             raise ValueError("a parameter is listed twice")
         self.places.add(address)
-        device_step = step.data_ptr() if isinstance(step, Tensor) else None
-        device_lr = lr.data_ptr() if isinstance(lr, Tensor) else None
-        rest = (device_step, device_lr, n, 0 if device_step else step, 0.0 if device_lr else lr,
-                decay, betas[0], betas[1], eps)
         if bits == 8:
-            record = SplatAdamwTensor(address, g.data_ptr(), m.codes.data_ptr(),
-                                      v.codes.data_ptr(), m.exponents.data_ptr(),
-                                      v.exponents.data_ptr(), *rest)
+            record = (address, g.data_ptr(), m.codes.data_ptr(), v.codes.data_ptr(),
+                      m.exponents.data_ptr(), v.exponents.data_ptr())
             self.written += (p, m.codes, v.codes, m.exponents, v.exponents)
         else:
-            record = SplatAdamwTensor(address, g.data_ptr(), m.data_ptr(), v.data_ptr(), None,
-                                      None, *rest)
+            record = (address, g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0)
             self.written += (p, m, v)
-        self.records.setdefault((p.device, p.dtype, bits, maximize), []).append(record)
+        record = _RECORD.pack(*record, device_step, device_lr, n, step, lr, decay, betas[0],
+                              betas[1], eps)
+        self.records.setdefault((index, p.dtype, bits, maximize), []).append(record)
 
     def run(self) -> None:
-        for (device, dtype, bits, maximize), records in self.records.items():
-            stages.adamw(device, dtype, bits, records, maximize)
+        for (index, dtype, bits, maximize), records in self.records.items():
+            stages.adamw(index, dtype, bits, records, maximize)
         if self.written:
             torch.autograd.graph.increment_version(self.written)
 

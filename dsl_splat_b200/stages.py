@@ -869,11 +869,11 @@ def feature_embedding_backward(ids: Tensor, entries: int, scale: float,
     dtype, device = FEATURE_DTYPES[upstream.dtype], upstream.device
     size = _query("splat_feature_embedding_backward_workspace_bytes", device.index, dtype, count,
                   entries, channels)
-    ws = upstream.new_empty((size,), dtype=torch.uint8)
+    ws = upstream.new_empty((size,), dtype=torch.uint8) if size > 16 else None
     ids, upstream = _dense(ids), _dense(upstream)
     _call(lib.splat_feature_embedding_backward, "feature_embedding_backward", device, dtype,
           ids.element_size(), count, entries, channels, ids.data_ptr(), upstream.data_ptr(),
-          scale, dtable.data_ptr(), ws.data_ptr(), size)
+          scale, dtable.data_ptr(), _address(ws), size)
     return dtable
 
 
@@ -936,12 +936,11 @@ def feature_entropy_backward(x: Tensor, weight: Tensor, target: Tensor, bias: Te
 
 # ---- optimizer -----------------------------------------------------------------
 
-def adamw(device: torch.device, dtype: torch.dtype, bits: int, records: list, maximize: bool
+def adamw(index: int, dtype: torch.dtype, bits: int, records: list[bytes], maximize: bool
           ) -> None:
-    """One AdamW step of nv.SplatAdamwTensor records on one device, of one dtype."""
-    table = (nv.SplatAdamwTensor * len(records))(*records)
-    _call(lib.splat_adamw, "adamw", device, FEATURE_DTYPES[dtype], bits, len(records), table,
-          int(maximize))
+    """One AdamW step of packed SplatAdamwTensor records on one device, of one dtype."""
+    _call(lib.splat_adamw, "adamw", torch.device("cuda", index), FEATURE_DTYPES[dtype], bits,
+          len(records), b"".join(records), int(maximize))
 
 
 def adamw_decode(codes: Tensor, exponents: Tensor, squared: bool) -> Tensor:

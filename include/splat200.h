@@ -633,7 +633,8 @@ int splat_feature_embedding(int dtype, int id_bytes, long long count, int entrie
                             const void* ids, const void* table, float scale, void* y,
                             void* stream);
 
-/* dtable[v] = scale sum of dy_i over ids_i = v, all of (entries, channels). */
+/* dtable[v] = scale sum of dy_i over ids_i = v, all of (entries, channels).  A workspace
+ * of 16 bytes or less may be NULL. */
 size_t splat_feature_embedding_backward_workspace_bytes(int dtype, long long count, int entries,
                                                         int channels);
 int splat_feature_embedding_backward(int dtype, int id_bytes, long long count, int entries,
