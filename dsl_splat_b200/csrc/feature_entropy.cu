@@ -271,6 +271,7 @@ void finish(long long count, int splits, long long stride, const float* from,
 // ---- launching -----------------------------------------------------------------------
 
 constexpr int kMostVocabulary = 1 << 20;
+constexpr long long kMostRows = 1 << 29;  // three planes of them have 2^31 rows at most
 constexpr long long kPieceBytes = 1LL << 30;
 
 // Whether the logits stay on the chip: their sums take one accumulator.
@@ -315,9 +316,9 @@ EntropyPlan plan_entropy(long long rows, int k, int vocabulary, bool backward) {
   if (plan.on_chip && !backward) {
     piece = rows;
   } else {
-    // bytes of a logit, or of a dz
-    const int size = plan.on_chip ? 2 * P : 4;
-    piece = std::max(1LL, kPieceBytes / size / vocabulary / unit) * unit;
+    // bytes of a row's logits, or of its dz, and of its dx before the rounding
+    const long long row = std::max(vocabulary * (plan.on_chip ? 2LL * P : 4LL), 4LL * k);
+    piece = std::max(1LL, kPieceBytes / row / unit) * unit;
     piece = std::min({piece, rows, 1LL << 23});  // 65535 ranges of 256 rows, and below
   }
   plan.piece = static_cast<int>(piece);
@@ -423,7 +424,7 @@ int check_entropy(int dtype, long long rows, int k, int vocabulary, int id_bytes
     return host::fail(kInvalidArgument, "feature_entropy: targets are of 4 or 8 bytes");
   if (reduction < kEach || reduction > kMean)
     return host::fail(kInvalidArgument, "feature_entropy: reduction");
-  if (k > 65535 || vocabulary > kMostVocabulary || rows > (1LL << 31) - kPairRows)
+  if (k > 65535 || vocabulary > kMostVocabulary || rows > kMostRows)
     return host::fail(kTooLarge, "feature_entropy: too many rows, inputs or words");
   return kOk;
 }

@@ -421,9 +421,15 @@ __global__ void __launch_bounds__(kNormThreads, resident_blocks(N, BACKWARD))
 
 // ---- rows of up to 8192 channels: a block each ----------------------------------------
 
-template <class T, int V, bool BACKWARD>
-__global__ void __launch_bounds__(kNormThreads) block_norm_kernel(const LayerNormParams p) {
-  constexpr int N = kMostLaneValues, M = N / 2;
+// Of them, that an SM holds at once: a block's sums wait for all of its warps.
+constexpr int resident_rows(int values, bool backward) {
+  return (values <= 8 ? 6 : values <= 16 ? 4 : 2) / (backward ? 2 : 1);
+}
+
+template <class T, int V, int N, bool BACKWARD>
+__global__ void __launch_bounds__(kNormThreads, resident_rows(N, BACKWARD))
+    block_norm_kernel(const LayerNormParams p) {
+  constexpr int M = N / 2;
   const int lane = threadIdx.x, lanes = kNormThreads, C = p.channels;
   const float inverse = 1.0f / static_cast<float>(C);
   bool in[N];
@@ -579,7 +585,10 @@ LayerNormPlan plan_norm(long long rows, int channels, bool backward) {
     return plan;
   }
   if (channels > kMostGroupChannels) {
-    plan.blocks = static_cast<int>(std::min<long long>(rows, (backward ? 1LL : 4LL) * sms));
+    const int each = (channels + kNormThreads - 1) / kNormThreads;
+    plan.values = each <= 8 ? 8 : each <= 16 ? 16 : 32;
+    plan.blocks = static_cast<int>(
+        std::min<long long>(rows, static_cast<long long>(resident_rows(plan.values, backward)) * sms));
     return plan;
   }
   // up to 16 values a lane, of which the last piece may be idle; more in whole warps
@@ -627,13 +636,19 @@ int launch_norm(const LayerNormPlan& plan, LayerNormParams& p, cudaStream_t s) {
   const bool aligned = host::aligned(p.x, 16) && host::aligned(p.y, 16) &&
                        host::aligned(p.dy, 16) && host::aligned(p.dx, 16);
   if (!plan.lanes) {
-    constexpr auto* wide = block_norm_kernel<T, V, BACKWARD>;
-    constexpr auto* narrow = block_norm_kernel<T, 1, BACKWARD>;
-    if (!host::allow_shared<wide>() || !host::allow_shared<narrow>())
-      return host::check_launch("feature_layer_norm: shared memory");
-    (plan.vector && aligned ? wide : narrow)<<<plan.blocks, kNormThreads, 8 * kMostBlockChannels,
-                                               host::counted(s)>>>(p);
-    return kOk;
+    const auto run = [&](auto values) {
+      constexpr int kValues = decltype(values)::value;
+      constexpr auto* wide = block_norm_kernel<T, V, kValues, BACKWARD>;
+      constexpr auto* narrow = block_norm_kernel<T, 1, kValues, BACKWARD>;
+      if (!host::allow_shared<wide>() || !host::allow_shared<narrow>())
+        return host::check_launch("feature_layer_norm: shared memory");
+      (plan.vector && aligned ? wide : narrow)<<<plan.blocks, kNormThreads,
+                                                 8 * kNormThreads * kValues, host::counted(s)>>>(p);
+      return static_cast<int>(kOk);
+    };
+    if (plan.values == 8) return run(std::integral_constant<int, 8>{});
+    if (plan.values == 16) return run(std::integral_constant<int, 16>{});
+    return run(std::integral_constant<int, 32>{});
   }
   if (!aligned)
     return host::fail(kInvalidArgument, "feature_layer_norm: tensors must be 16-byte aligned");

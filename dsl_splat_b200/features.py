@@ -381,8 +381,8 @@ def check_linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, bias: 
     if isinstance(ignore_index, bool) or not isinstance(ignore_index, Integral) \
             or not -(1 << 63) <= ignore_index < 1 << 63:
         raise ValueError("ignore_index must be an integer of 64 bits")
-    if x.shape[-1] > 65535 or vocabulary > 1 << 20 or target.numel() > 1 << 31:
-        raise ValueError("at most 65535 features, 2^20 words and 2^31 rows")
+    if x.shape[-1] > 65535 or vocabulary > 1 << 20 or target.numel() > 1 << 29:
+        raise ValueError("at most 65535 features, 2^20 words and 2^29 rows")
 
 
 def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, bias: Tensor | None = None,

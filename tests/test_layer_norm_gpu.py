@@ -214,3 +214,11 @@ def test_streams_and_graphs():
     assert torch.equal(y, want)
     for g, f in zip(grads, first):
         assert torch.equal(g, f)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_weight_or_bias_alone(dtype):
+    for c in (24, 25, 1500, 9000):
+        x, w, b, dy = make(90, c, dtype, 12)
+        run(x, w, None, "silu", dy)
+        run(x, None, b, "gelu", dy)
