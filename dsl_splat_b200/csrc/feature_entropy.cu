@@ -342,7 +342,7 @@ EntropyPlan plan_entropy(long long rows, int k, int vocabulary, bool backward) {
     plan.moments = take(sizeof(Partial) * rows);
     plan.losses = take(4ull * rows);
     if (plan.on_chip) {
-      plan.partials = take(plan.tile_n / 64 * static_cast<size_t>(plan.ranges) * rows *
+      plan.partials = take(kVocabularyParts * static_cast<size_t>(plan.ranges) * rows *
                            sizeof(Partial));
       plan.label_logits = take(4ull * rows);
     }
@@ -379,12 +379,12 @@ int launch_vocabulary(VocabularyParams& p, const EntropyPlan& plan, const Rows& 
   p.tile_n = plan.tile_n, p.tiles = plan.tiles;
   p.row_blocks = static_cast<int>((count + static_cast<long long>(kPairRows) - 1) / kPairRows);
   p.splits = plan.ranges, p.tiles_per_split = plan.tiles_per_range;
-  constexpr int P = kOperandParts<T>, kEpilogue = vocabulary_warps(P);
+  constexpr int P = kOperandParts<T>;
   p.x_plane_rows = x.plane_rows, p.w_plane_rows = w.plane_rows;
   if (!make_operand_map<T, false>(p.x_map, x, count, k, 128) ||
       !make_operand_map<T, false>(p.w_map, w, r.vocabulary, k, plan.tile_n / 2))
     return host::fail(kInvalidArgument, "feature_entropy: operand maps");
-  const int fixed = 1024 + (SLOPES ? kEpilogue * 4096 : 0);
+  const int fixed = 1024 + (SLOPES ? kVocabularyWarps * 4096 : 0);
   const int stage = P * (kAPlane + plan.tile_n / 2 * 128);
   p.stages = std::min(kPairStages, (kOneBlockBytes - fixed) / stage);
   constexpr auto* kernel = vocabulary_kernel<T, P, SLOPES>;
@@ -393,7 +393,7 @@ int launch_vocabulary(VocabularyParams& p, const EntropyPlan& plan, const Rows& 
   const long long items = static_cast<long long>(p.row_blocks) * p.splits;
   if (items >= 1LL << 31) return host::fail(kTooLarge, "feature_entropy: too many tiles");
   const int pairs = static_cast<int>(std::min<long long>(items, host::sm_count() / 2));
-  kernel<<<2 * pairs, 32 * kEpilogue + 64, fixed + p.stages * stage, host::counted(s)>>>(p);
+  kernel<<<2 * pairs, kVocabularyThreads, fixed + p.stages * stage, host::counted(s)>>>(p);
   return host::check_launch("feature_entropy");
 }
 
@@ -456,7 +456,7 @@ int launch_forward(const Rows& r, int k, const void* x, const void* weight, cons
       const int status = launch_vocabulary<T, false>(p, plan, r, first, rows, k, xs, w, bias, s);
       if (status != kOk) return status;
       join_partials_kernel<<<host::blocks_for(rows, kThreads), kThreads, 0, host::counted(s)>>>(
-          r, plan.tile_n / 64 * plan.ranges, p.partials, p.label_logits, moments, each);
+          r, kVocabularyParts * plan.ranges, p.partials, p.label_logits, moments, each);
       continue;
     }
     const int status = launch_logits<T>(rows, k, vocabulary, xs, w, z, s);

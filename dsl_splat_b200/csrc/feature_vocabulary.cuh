@@ -7,7 +7,7 @@
 // A pair of blocks (tensor_core.cuh) takes 256 rows x 256 words of 16-bit x and W, or 256 x
 // 128 of fp32 ones in three parts: per SM, a chunk of 64 k is 16 KB of x and 16 KB of W,
 // half of what two blocks on their own would read from the L2.  In each block one thread
-// starts the tensor copies, and sixteen (eight) epilogue warps read the finished
+// starts the tensor copies, and sixteen epilogue warps read the finished
 // accumulators, 32 words of 32 rows at a time, and give them back before they work on the
 // last of them; the leading block's product warp issues.  One half of the epilogue takes
 // the even tiles and the other the odd ones, so that the one's exponentials run under the
@@ -25,8 +25,9 @@
 namespace splat {
 namespace feature {
 
-// Epilogue warps: one to 64 words of 32 rows.
-__host__ __device__ constexpr int vocabulary_warps(int parts) { return parts == 1 ? 16 : 8; }
+// Epilogue warps.  Half of them take a tile: four the rows, two the halves of its words.
+constexpr int kVocabularyWarps = 16, kVocabularyThreads = 32 * kVocabularyWarps + 64;
+constexpr int kVocabularyParts = 4;  // partial results of a row in a range of words
 constexpr float kLog2E = 1.44269504088896341f;
 
 // What the rows' kernels read.
@@ -82,7 +83,7 @@ struct VocabularyParams {
   int tiles, row_blocks, splits, tiles_per_split;
   int stages;
   const void* bias;
-  // statistics: (splits, tile_n / 64, count), and the labels' logits (count)
+  // statistics: (splits, kVocabularyParts, count), and the labels' logits (count)
   Partial* partials;
   float* label_logits;
   // slopes
@@ -165,23 +166,19 @@ SPLAT_DEV float4 patch_sums(uint32_t patch, const float* v) {
 }
 
 template <class T, int P, bool SLOPES>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * vocabulary_warps(P) + 64, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVocabularyThreads, 1)
     vocabulary_kernel(const __grid_constant__ VocabularyParams p) {
-  constexpr int kEpilogue = vocabulary_warps(P);
+  constexpr int kEpilogue = kVocabularyWarps;
   extern __shared__ unsigned char dynamic[];
   __shared__ PairBarriers barriers;
   const uint32_t base = (tc::shared_address(dynamic) + 1023u) & ~1023u;
   const int warp = tc::uniform(threadIdx.x >> 5);
   const uint32_t rank = tc::cluster_rank();
-  const int half_n = p.tile_n / 2, groups = p.tile_n / 64;
+  const int half_n = p.tile_n / 2;
   const uint32_t b_plane = half_n * 128;
   // patches of the epilogue warps, the ring
   const uint32_t ring_at = base + (SLOPES ? kEpilogue * 4096 : 0);
-  // tiles that have two 64 words for each warp are shared by half of the warps, which
-  // take every other one
-  const bool alternate = 4 * groups == kEpilogue;
-  const int active = alternate ? kEpilogue / 2 : 4 * groups;  // warps of a tile
-  const uint32_t tmem = pair_begin(barriers, p.stages, 2 * active);
+  const uint32_t tmem = pair_begin(barriers, p.stages, kEpilogue);
   const int items = p.row_blocks * p.splits;
   const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
   bool ok = true;
@@ -219,12 +216,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * vocabulary_warp
       }
       ok = issue.drain() && ok;
     }
-  } else if (alternate || warp < active) {
-    // a thread to a row, a warp to one or two 64 of the tile's words
-    const int lane = threadIdx.x & 31, lane_block = warp & 3, group = warp >> 2;
-    const uint32_t own = alternate ? warp / active : 0, every = alternate ? 1 : 0;
-    const int first = alternate ? (warp % active >> 2) * 128 : group * 64;
-    const int end = first + (alternate ? 128 : 64);
+  } else {
+    // a thread to a row; the first eight warps take the even tiles, the others the odd ones
+    const int lane = threadIdx.x & 31, lane_block = warp & 3, part = warp >> 2;
+    const uint32_t own = part >> 1;
+    const int first = (part & 1) * half_n, end = first + half_n;
     const T* bias = static_cast<const T*>(p.bias);
     const int V = p.rows.vocabulary;
     const uint32_t patch_at = base + warp * 4096;
@@ -251,7 +247,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * vocabulary_warp
         cleared = __any_sync(0xffffffffu, label < 0 && !(here && isfinite(s.top + s.sum)));
       }
       for (int t = split * p.tiles_per_split; t < t1; ++t, ++read) {
-        if ((read & every) != own) continue;
+        if ((read & 1) != own) continue;
         const uint32_t acc = read & 1;
         if (!(ok = tc::barrier_wait(tc::shared_address(&barriers.acc_full[acc]), (read >> 1) & 1)))
           break;
@@ -351,7 +347,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * vocabulary_warp
         }
       }
       if (!SLOPES && here)
-        p.partials[static_cast<long long>(split * groups + group) * p.count + row] = s;
+        p.partials[static_cast<long long>(split * kVocabularyParts + part) * p.count + row] = s;
     }
     if (SLOPES && lane == 0) tc::copies_out_read();
   }
