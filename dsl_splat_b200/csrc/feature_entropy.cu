@@ -9,10 +9,10 @@
 // rows at a time.  The backward forms them again, and dz for a piece of the rows.  u_i is the upstream gradient of row i's loss (divided by
 // the number of rows that count for their mean) and 0 for the others.
 //
-// dz is held in T for the products.  It is taken relative to the power of two E that
-// is not below any |u_i|, times 2^15 of float16, whose smallest value would otherwise
-// swallow the tail of a large vocabulary; the products' fp32 results are multiplied by the
-// inverse before their rounding.
+// dz is held in T for the products.  A u that all rows share is multiplied to the products'
+// fp32 results before their rounding; of u_i of their own dz is taken relative to the power of two
+// that is not below any |u_i|, and the results are multiplied by that.  float16, whose
+// smallest value would otherwise swallow the tail of a large vocabulary, has 2^15 times dz.
 #include <algorithm>
 
 #include "feature_join.cuh"
@@ -136,16 +136,20 @@ __global__ void __launch_bounds__(kThreads)
 
 // ---- gradients -----------------------------------------------------------------------
 
-// The power of two that is not below any finite |u|.
+// The factors: of rows' own u the power of two that is not below any finite one's
+// magnitude.
 __global__ void __launch_bounds__(1024)
     factors_kernel(long long rows, int reduction, const float* upstream, const float* counted,
                    float within, Factors* factors) {
+  if (reduction != kEach) {
+    if (threadIdx.x) return;
+    factors->in = within;
+    factors->out = (reduction == kMean ? *upstream / *counted : *upstream) / within;
+    return;
+  }
   uint32_t most = 0;
-  const long long n = reduction == kEach ? rows : 1;
-  for (long long i = threadIdx.x; i < n; i += 1024) {
-    float u = upstream[i];
-    if (reduction == kMean) u /= *counted;
-    const uint32_t bits = __float_as_uint(u) & 0x7fffffffu;
+  for (long long i = threadIdx.x; i < rows; i += 1024) {
+    const uint32_t bits = __float_as_uint(upstream[i]) & 0x7fffffffu;
     if (bits < 0x7f800000u) most = max(most, bits);
   }
   most = __reduce_max_sync(0xffffffffu, most);
@@ -166,14 +170,14 @@ template <class T, class TO, bool BLOCK>
 __global__ void __launch_bounds__(kThreads)
     row_slope_kernel(const Rows p, long long first, int rows, const float* z, int ld,
                      const T* bias, const Partial* moments, const float* upstream,
-                     const float* counted, const Factors* factors, TO* dz, int ld_out) {
+                     const Factors* factors, TO* dz, int ld_out) {
   const int lane = BLOCK ? threadIdx.x : threadIdx.x & 31, lanes = BLOCK ? kThreads : 32;
   const int r = BLOCK ? blockIdx.x : blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (r >= rows) return;
   const float* from = z + static_cast<long long>(r) * ld;
   TO* to = dz + static_cast<long long>(r) * ld_out;
   const int t = label_of(p, first + r);
-  const float u = t < 0 ? 0.0f : upstream_of(p, first + r, upstream, counted) * factors->in;
+  const float u = t < 0 ? 0.0f : upstream_of(p, first + r, upstream, factors);
   const Partial s = moments[first + r];
   const float factor = u / s.sum;
   for (int j = lane; j < ld_out; j += lanes) {
@@ -192,7 +196,7 @@ template <class T>
 __global__ void __launch_bounds__(kThreads)
     column_slopes_kernel(const Rows p, long long first, int rows, const float* z, int ld,
                          const T* bias, const Partial* moments, const float* upstream,
-                         const float* counted, const Factors* factors, float* sums) {
+                         const Factors* factors, float* sums) {
   const int j = blockIdx.x * kThreads + threadIdx.x;
   if (j >= p.vocabulary) return;
   const int begin = blockIdx.y * kSumRows, end = min(begin + kSumRows, rows);
@@ -202,7 +206,7 @@ __global__ void __launch_bounds__(kThreads)
     const int t = label_of(p, first + r);
     if (t < 0) continue;
     const Partial s = moments[first + r];
-    const float u = upstream_of(p, first + r, upstream, counted) * factors->in;
+    const float u = upstream_of(p, first + r, upstream, factors);
     const float v = expf(z[static_cast<long long>(r) * ld + j] + b - s.top) * (u / s.sum);
     sum += j == t ? v - u : v;
   }
@@ -507,7 +511,7 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
     int status = kOk;
     if (plan.on_chip) {
       VocabularyParams p{};
-      p.moments = moments, p.upstream = upstream, p.counted = counted, p.factors = factors;
+      p.moments = moments, p.upstream = upstream, p.factors = factors;
       p.dz_plane_rows = dz.plane_rows;
       if (dbias) p.column_sums = column_sums;
       if (!make_map<PairOperand<T>>(p.dz_map, dz.data,
@@ -525,8 +529,8 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
       const int ranges = (rows + kSumRows - 1) / kSumRows;
       column_slopes_kernel<T>
           <<<dim3(host::blocks_for(vocabulary, kThreads), ranges), kThreads, 0,
-             host::counted(s)>>>(r, first, rows, z, vocabulary, b, moments, upstream, counted,
-                                 factors, column_sums);
+             host::counted(s)>>>(r, first, rows, z, vocabulary, b, moments, upstream, factors,
+                                 column_sums);
       add_columns(vocabulary, ranges, column_sums, first == 0, column_total, s);
     }
     if (!dx && !dweight) continue;
@@ -534,11 +538,11 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
       constexpr bool kBlock = decltype(block)::value;
       if constexpr (sizeof(T) == 2) {
         row_slope_kernel<T, T, kBlock><<<grid, kThreads, 0, host::counted(s)>>>(
-            r, first, rows, z, vocabulary, b, moments, upstream, counted, factors,
+            r, first, rows, z, vocabulary, b, moments, upstream, factors,
             static_cast<T*>(dz.data), dz.ld);
       } else {
         row_slope_kernel<T, float, kBlock><<<grid, kThreads, 0, host::counted(s)>>>(
-            r, first, rows, z, vocabulary, b, moments, upstream, counted, factors, z, vocabulary);
+            r, first, rows, z, vocabulary, b, moments, upstream, factors, z, vocabulary);
       }
     });
     if constexpr (sizeof(T) == 4) {

@@ -51,14 +51,15 @@ SPLAT_DEV int label_of(const Rows& p, long long row) {
 
 enum Reduction : int { kEach = 0, kSum = 1, kMean = 2 };
 
-// Factors of the backward: of u_i on the way into dz, and of the products' results.
+// Factors of the backward: of u_i on the way into dz, and of the products' results.  Where
+// all rows have the same u it is left to the results: rounded to 16 bits with each label's
+// dz, which is nearly -u, it would cost all of dx and dW the same error.
 struct Factors {
   float in, out;
 };
 SPLAT_DEV float upstream_of(const Rows& p, long long row, const float* upstream,
-                            const float* counted) {
-  const float u = upstream[p.reduction == kEach ? row : 0];
-  return p.reduction == kMean ? u / *counted : u;
+                            const Factors* factors) {
+  return p.reduction == kEach ? upstream[row] * factors->in : factors->in;
 }
 
 // A row's largest logit in units of log 2 so far, and the sum of powers of two relative
@@ -88,7 +89,7 @@ struct VocabularyParams {
   float* label_logits;
   // slopes
   const Partial* moments;  // (rows)
-  const float *upstream, *counted;
+  const float* upstream;
   const Factors* factors;
   float* column_sums;  // (count / 32 rounded up to whole tiles, vocabulary) or NULL
 };
@@ -239,7 +240,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVocabularyThreads, 
         if (here) {
           s = p.moments[p.first + row];
           if (label >= 0) {
-            u = upstream_of(p.rows, p.first + row, p.upstream, p.counted) * p.factors->in;
+            u = upstream_of(p.rows, p.first + row, p.upstream, p.factors);
             factor = u / s.sum;
           }
         }
