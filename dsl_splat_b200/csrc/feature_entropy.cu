@@ -13,6 +13,9 @@
 // fp32 results before their rounding; of u_i of their own dz is taken relative to the power of two
 // that is not below any |u_i|, and the results are multiplied by that.  float16, whose
 // smallest value would otherwise swallow the tail of a large vocabulary, has 2^15 times dz.
+// 16-bit types hold dz with u_i of their own as two values (2.4e-3 instead of 1.7e-3
+// relative error of dx and dW for bf16 with one), whose products cost twice the time; without,
+// a label's dz is nearly 1 and the others are small beside it.
 #include <algorithm>
 
 #include "feature_join.cuh"
@@ -310,9 +313,19 @@ int word_ranges(int row_blocks, int tiles) {
   return best;
 }
 
+// What a workspace is for.
+enum Purpose : int { kForwardLoss = 0, kSharedUpstream = 1, kOwnUpstreams = 2 };
+int purpose_of(int reduction) { return reduction == kEach ? kOwnUpstreams : kSharedUpstream; }
+// Parts of dz.
 template <class T>
-EntropyPlan plan_entropy(long long rows, int k, int vocabulary, bool backward) {
+constexpr int dz_parts(bool each) {
+  return sizeof(T) == 4 ? 3 : each ? 2 : 1;
+}
+
+template <class T>
+EntropyPlan plan_entropy(long long rows, int k, int vocabulary, int purpose) {
   constexpr int P = kOperandParts<T>;
+  const bool backward = purpose != kForwardLoss, each = purpose == kOwnUpstreams;
   EntropyPlan plan{};
   plan.on_chip = on_chip<T>(k);
   const int unit = plan.on_chip ? kPairRows : kTileRows;
@@ -321,7 +334,7 @@ EntropyPlan plan_entropy(long long rows, int k, int vocabulary, bool backward) {
     piece = rows;
   } else {
     // bytes of a row's logits, or of its dz, and of its dx before the rounding
-    const long long row = std::max(vocabulary * (plan.on_chip ? 2LL * P : 4LL), 4LL * k);
+    const long long row = std::max(vocabulary * (plan.on_chip ? 2LL * dz_parts<T>(each) : 4LL), 4LL * k);
     piece = std::max(1LL, kPieceBytes / row / unit) * unit;
     piece = std::min({piece, rows, 1LL << 23});  // 65535 ranges of 256 rows, and below
   }
@@ -352,11 +365,17 @@ EntropyPlan plan_entropy(long long rows, int k, int vocabulary, bool backward) {
     }
     return plan;
   }
-  plan.dz = take(plane_bytes<T>(piece, vocabulary));
+  plan.dz = take(2ull * dz_parts<T>(each) * round_to(piece, 64) * round_to(vocabulary, 8));
   // ranges of words for dx and of rows for dW, whose sums are joined
   if (plan.on_chip) {
-    plan.dx_splits = pair_splits<P>(pair_tiles<P>(piece, k), vocabulary);
-    plan.dw_splits = pair_splits<P>(pair_tiles<P>(vocabulary, k), piece);
+    const long long dx_tiles = pair_tiles<P>(piece, k), dw_tiles = pair_tiles<P>(vocabulary, k);
+    const auto split = [&](auto parts) {
+      constexpr int DZ = decltype(parts)::value;
+      plan.dx_splits = pair_splits<DZ, P>(dx_tiles, vocabulary);
+      plan.dw_splits = pair_splits<DZ, P>(dw_tiles, piece);
+    };
+    if (each) split(std::integral_constant<int, dz_parts<T>(true)>{});
+    else split(std::integral_constant<int, dz_parts<T>(false)>{});
   } else {
     const long long tiles = ((vocabulary + 127LL) / 128) * ((k + 127) / 128);
     const long long wanted = std::max(1LL, 2LL * host::sm_count() / tiles);
@@ -375,7 +394,7 @@ EntropyPlan plan_entropy(long long rows, int k, int vocabulary, bool backward) {
 }
 
 // What both launches of vocabulary_kernel share.
-template <class T, bool SLOPES>
+template <class T, int DZ>
 int launch_vocabulary(VocabularyParams& p, const EntropyPlan& plan, const Rows& r, long long first,
                       int count, int k, const Planes& x, const Planes& w, const void* bias,
                       cudaStream_t s) {
@@ -385,13 +404,13 @@ int launch_vocabulary(VocabularyParams& p, const EntropyPlan& plan, const Rows& 
   p.splits = plan.ranges, p.tiles_per_split = plan.tiles_per_range;
   constexpr int P = kOperandParts<T>;
   p.x_plane_rows = x.plane_rows, p.w_plane_rows = w.plane_rows;
-  if (!make_operand_map<T, false>(p.x_map, x, count, k, 128) ||
-      !make_operand_map<T, false>(p.w_map, w, r.vocabulary, k, plan.tile_n / 2))
+  if (!make_operand_map<T, P, false>(p.x_map, x, count, k, 128) ||
+      !make_operand_map<T, P, false>(p.w_map, w, r.vocabulary, k, plan.tile_n / 2))
     return host::fail(kInvalidArgument, "feature_entropy: operand maps");
-  const int fixed = 1024 + (SLOPES ? kVocabularyWarps * 4096 : 0);
+  const int fixed = 1024 + (DZ ? kVocabularyWarps * 4096 : 0);
   const int stage = P * (kAPlane + plan.tile_n / 2 * 128);
   p.stages = std::min(kPairStages, (kOneBlockBytes - fixed) / stage);
-  constexpr auto* kernel = vocabulary_kernel<T, P, SLOPES>;
+  constexpr auto* kernel = vocabulary_kernel<T, P, DZ>;
   if (!host::allow_shared<kernel>())
     return host::check_launch("feature_entropy: shared memory");
   const long long items = static_cast<long long>(p.row_blocks) * p.splits;
@@ -444,7 +463,7 @@ template <class T>
 int launch_forward(const Rows& r, int k, const void* x, const void* weight, const void* bias,
                    float* loss, Partial* moments, float* counted, char* ws, cudaStream_t s) {
   const int vocabulary = r.vocabulary;
-  const EntropyPlan plan = plan_entropy<T>(r.rows, k, vocabulary, false);
+  const EntropyPlan plan = plan_entropy<T>(r.rows, k, vocabulary, kForwardLoss);
   float* z = reinterpret_cast<float*>(ws + plan.logits);
   if (!moments) moments = reinterpret_cast<Partial*>(ws + plan.moments);
   float* each = r.reduction == kEach ? loss : reinterpret_cast<float*>(ws + plan.losses);
@@ -457,7 +476,7 @@ int launch_forward(const Rows& r, int k, const void* x, const void* weight, cons
       VocabularyParams p{};
       p.partials = reinterpret_cast<Partial*>(ws + plan.partials);
       p.label_logits = reinterpret_cast<float*>(ws + plan.label_logits);
-      const int status = launch_vocabulary<T, false>(p, plan, r, first, rows, k, xs, w, bias, s);
+      const int status = launch_vocabulary<T, 0>(p, plan, r, first, rows, k, xs, w, bias, s);
       if (status != kOk) return status;
       join_partials_kernel<<<host::blocks_for(rows, kThreads), kThreads, 0, host::counted(s)>>>(
           r, kVocabularyParts * plan.ranges, p.partials, p.label_logits, moments, each);
@@ -487,7 +506,7 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
                     void* dweight, void* dbias, char* ws, cudaStream_t s) {
   constexpr int P = kOperandParts<T>;
   const int vocabulary = r.vocabulary;
-  const EntropyPlan plan = plan_entropy<T>(r.rows, k, vocabulary, true);
+  const EntropyPlan plan = plan_entropy<T>(r.rows, k, vocabulary, purpose_of(r.reduction));
   float* z = reinterpret_cast<float*>(ws + plan.logits);
   auto* factors = reinterpret_cast<Factors*>(ws + plan.factors);
   float* weight_sums = reinterpret_cast<float*>(ws + plan.weight_sums);
@@ -507,7 +526,9 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
     dz.ld = static_cast<int>(round_to(vocabulary, 8));
     dz.data = ws + plan.dz;
     dz.rows = rows;
-    dz.plane_rows = static_cast<int>(P == 1 ? rows : round_to(rows, 64));
+    const bool each = plan.on_chip && r.reduction == kEach;
+    const int parts = dz_parts<T>(each);
+    dz.plane_rows = static_cast<int>(parts == 1 ? rows : round_to(rows, 64));
     int status = kOk;
     if (plan.on_chip) {
       VocabularyParams p{};
@@ -515,10 +536,13 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
       p.dz_plane_rows = dz.plane_rows;
       if (dbias) p.column_sums = column_sums;
       if (!make_map<PairOperand<T>>(p.dz_map, dz.data,
-                                    static_cast<long long>(dz.plane_rows) * P, vocabulary, dz.ld,
+                                    static_cast<long long>(dz.plane_rows) * parts, vocabulary, dz.ld,
                                     32, 32))
         return host::fail(kInvalidArgument, "feature_entropy_backward: map");
-      status = launch_vocabulary<T, true>(p, plan, r, first, rows, k, xs, w, bias, s);
+      status = each ? launch_vocabulary<T, dz_parts<T>(true)>(p, plan, r, first, rows, k, xs, w,
+                                                              bias, s)
+                    : launch_vocabulary<T, dz_parts<T>(false)>(p, plan, r, first, rows, k, xs, w,
+                                                               bias, s);
       if (status != kOk) return status;
       if (dbias)
         add_columns(vocabulary, (rows + 31) / 32, column_sums, first == 0, column_total, s);
@@ -550,8 +574,10 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
     }
     if (dx) {
       if (plan.on_chip) {
-        status = launch_pairs<T, false, true>(rows, k, vocabulary, dz, w, plan.dx_splits, dx_sums,
-                                              false, s);
+        status = each ? launch_pairs<T, dz_parts<T>(true), false, true>(
+                            rows, k, vocabulary, dz, w, plan.dx_splits, dx_sums, false, s)
+                      : launch_pairs<T, dz_parts<T>(false), false, true>(
+                            rows, k, vocabulary, dz, w, plan.dx_splits, dx_sums, false, s);
       } else {
         ProductParams p{};
         p.m = rows, p.k = vocabulary, p.n = k;
@@ -570,8 +596,10 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
       PairSplits dw = plan.dw_splits;
       dw.count = static_cast<int>((rows + dw.k - 1) / dw.k);
       if (plan.on_chip) {
-        status = launch_pairs<T, true, true>(vocabulary, k, rows, dz, xs, dw, weight_sums,
-                                             first != 0, s);
+        status = each ? launch_pairs<T, dz_parts<T>(true), true, true>(
+                            vocabulary, k, rows, dz, xs, dw, weight_sums, first != 0, s)
+                      : launch_pairs<T, dz_parts<T>(false), true, true>(
+                            vocabulary, k, rows, dz, xs, dw, weight_sums, first != 0, s);
       } else {
         ProductParams p{};
         p.m = vocabulary, p.k = rows, p.n = k;
@@ -601,9 +629,11 @@ extern "C" {
 
 size_t splat_feature_entropy_workspace_bytes(int dtype, long long rows, int k, int vocabulary,
                                              int backward) {
-  if (check_entropy(dtype, rows, k, vocabulary, 8, 0) != kOk) return 0;
+  if (backward < kForwardLoss || backward > kOwnUpstreams ||
+      check_entropy(dtype, rows, k, vocabulary, 8, 0) != kOk)
+    return 0;
   return SPLAT_FEATURE_TYPE(dtype, [&] {
-    return plan_entropy<T>(rows, k, vocabulary, backward != 0).bytes;
+    return plan_entropy<T>(rows, k, vocabulary, backward).bytes;
   });
 }
 
@@ -644,7 +674,8 @@ int splat_feature_entropy_backward(int dtype, long long rows, int k, int vocabul
   if (!host::aligned(workspace, 16))
     return host::fail(kInvalidArgument,
                       "feature_entropy_backward: workspace not 16-byte aligned");
-  if (workspace_bytes < splat_feature_entropy_workspace_bytes(dtype, rows, k, vocabulary, 1))
+  if (workspace_bytes < splat_feature_entropy_workspace_bytes(dtype, rows, k, vocabulary,
+                                                              purpose_of(reduction)))
     return host::fail(kWorkspaceTooSmall, "feature_entropy_backward: workspace");
   if (!lies_well(dtype, k, x, weight, bias))
     return host::fail(kInvalidArgument, "feature_entropy_backward: x, weight and bias must be 16-byte aligned");

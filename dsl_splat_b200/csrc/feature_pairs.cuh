@@ -1,6 +1,7 @@
 // C(m, n) = sum_k A(m, k) B(n, k) on pairs of blocks (tensor_core.cuh): the long products of
-// a vocabulary's gradients.  Operands are 16-bit, or fp32 as planes of three bf16 parts
-// (feature_product.cuh); results are fp32 sums over ranges of k.
+// a vocabulary's gradients.  Operands are 16-bit, A in one plane or in two whose sum it is,
+// or fp32 as planes of three bf16 parts (feature_product.cuh); results are fp32 sums over
+// ranges of k.
 //
 // A pair takes 256 x tile_n tiles; each of its blocks copies its 128 rows of A and its half
 // of B's in chunks of 64 k, half of what a block on its own would read for the same work.
@@ -103,8 +104,8 @@ struct PairRing {
   }
 };
 
-// The leading block's product warp.  P: parts of the operands.
-template <int P>
+// The leading block's product warp.  PA, PB: parts of the operands.
+template <int PA, int PB>
 struct PairIssue {
   PairBarriers& b;
   uint32_t base, stage_bytes, b_plane, tmem, lead, instruction;
@@ -113,7 +114,7 @@ struct PairIssue {
 
   SPLAT_DEV PairIssue(PairBarriers& b, uint32_t base, uint32_t b_plane, int stages,
                       uint32_t tmem, uint32_t instruction)
-      : b(b), base(base), stage_bytes(P * (kAPlane + b_plane)), b_plane(b_plane), tmem(tmem),
+      : b(b), base(base), stage_bytes(PA * kAPlane + PB * b_plane), b_plane(b_plane), tmem(tmem),
         lead(tc::elected()), instruction(instruction), stages(stages) {}
 
   // One accumulator of a tile, over `length` k; that of the lower products of parts lies
@@ -128,19 +129,21 @@ struct PairIssue {
     for (long long k = 0; k < length; k += kChunk) {
       if (!tc::barrier_wait_pair(tc::shared_address(&b.full[stage]), parity)) return false;
       tc::fence_after_sync();
-      const uint32_t a_at = base + stage * stage_bytes, b_at = a_at + P * kAPlane;
+      const uint32_t a_at = base + stage * stage_bytes, b_at = a_at + PA * kAPlane;
       const int steps = static_cast<int>((min(length - k, static_cast<long long>(kChunk)) + 15) / 16);
-      // products of parts i and j with i + j < P, the smallest first
+      // products of parts i and j with i + j < PA, the smallest first
 #pragma unroll
-      for (int part = P - 1; part >= 0; --part)
+      for (int part = PA - 1; part >= 0; --part)
 #pragma unroll
         for (int i = 0; i <= part; ++i) {
+          if (part - i >= PB) continue;
           const uint32_t ao = a_at + i * kAPlane, bo = b_at + (part - i) * b_plane;
           uint64_t a = AMN ? tc::descriptor_mn_major(ao, kChunk * 128) : tc::descriptor_k_major(ao);
           uint64_t v = BMN ? tc::descriptor_mn_major(bo, kChunk * 128) : tc::descriptor_k_major(bo);
-          const uint32_t to = d + (P > 1 && part > 0 ? 128 : 0);
+          const uint32_t to = d + (PB > 1 && part > 0 ? 128 : 0);
           // the first product into an accumulator overwrites it
-          const bool first = k == 0 && i == 0 && (part == 0 || part == P - 1);
+          const bool first = k == 0 && (PB > 1 ? i == 0 && (part == 0 || part == PA - 1)
+                                               : part == PA - 1);
 #pragma unroll 4
           for (int s = 0; s < steps; ++s) {
             tc::mma_pair(lead, to, a, v, instruction, !first || s > 0);
@@ -174,7 +177,11 @@ SPLAT_DEV void pair_release(PairBarriers& b, uint32_t acc) {
 template <class T>
 using PairOperand = std::conditional_t<kIsF16<T>, f16, bf16>;
 
-template <class T, int P, bool AMN, bool BMN>
+// k of an accumulator.
+template <int PA, int PB>
+constexpr long long kPairSum = PB > 1 ? kExactSum : kMostAdditions * 16 / PA;
+
+template <class T, int PA, int PB, bool AMN, bool BMN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     pair_product_kernel(const __grid_constant__ PairParams p) {
   extern __shared__ unsigned char dynamic[];
@@ -185,7 +192,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   const uint32_t rank = tc::cluster_rank();
   const int half_n = p.tile_n / 2;
   const uint32_t b_plane = b_plane_bytes<BMN>(half_n);
-  constexpr long long kSum = P == 1 ? kMostAdditions * 16 : kExactSum;  // of an accumulator
+  constexpr long long kSum = kPairSum<PA, PB>;
   const uint32_t tmem = pair_begin(barriers, p.stages, 16);
   const int tiles_mn = p.tiles_m * p.tiles_n, tiles = tiles_mn * p.splits;
   const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
@@ -193,7 +200,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
   if (warp == 8) {
     if ((threadIdx.x & 31) == 0) {
-      PairRing ring(barriers, ring_at, P * (kAPlane + b_plane), p.stages, rank);
+      PairRing ring(barriers, ring_at, PA * kAPlane + PB * b_plane, p.stages, rank);
       for (int t = pair; t < tiles && ok; t += pairs) {
         const int split = t / tiles_mn, rest = t % tiles_mn;
         const int m0 = rest / p.tiles_n * kPairRows + rank * 128;
@@ -203,7 +210,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           ok = ring.fill([&](uint32_t at, uint32_t bar) {
             const int k0 = static_cast<int>(k);
 #pragma unroll
-            for (int i = 0; i < P; ++i, at += kAPlane) {
+            for (int i = 0; i < PA; ++i, at += kAPlane) {
               if constexpr (AMN) {
                 tc::copy_in_pair(at, &p.a_map, m0, k0 + i * p.a_plane_rows, bar);
                 tc::copy_in_pair(at + kChunk * 128, &p.a_map, m0 + 64, k0 + i * p.a_plane_rows,
@@ -213,7 +220,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
               }
             }
 #pragma unroll
-            for (int i = 0; i < P; ++i, at += b_plane) {
+            for (int i = 0; i < PB; ++i, at += b_plane) {
               if constexpr (BMN) {
                 for (int j = 0; j * 64 < half_n; ++j)
                   tc::copy_in_pair(at + j * (kChunk * 128), &p.b_map, n0 + j * 64,
@@ -228,7 +235,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
   } else if (warp == 9) {
     if (rank == 0) {
-      PairIssue<P> issue(barriers, ring_at, b_plane, p.stages, tmem,
+      PairIssue<PA, PB> issue(barriers, ring_at, b_plane, p.stages, tmem,
                          tc::instruction_pair(!kIsF16<T>, AMN, BMN, p.tile_n));
       for (int t = pair; t < tiles && ok; t += pairs) {
         const long long k0 = t / tiles_mn * p.k_per_split, k1 = min(k0 + p.k_per_split, p.k);
@@ -276,7 +283,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           patch.store(p.out + out_row * p.n + col0 + c, p.n, rows, cols, vector, p.accumulate);
         }
       };
-      if constexpr (P == 1) {
+      if constexpr (PB == 1) {  // a split is one sum
         const uint32_t acc = read & 1;
         if (!(ok = tc::barrier_wait(tc::shared_address(&barriers.acc_full[acc]), (read >> 1) & 1)))
           break;
@@ -328,12 +335,12 @@ struct PairSplits {
   int count;
   long long k;  // of a split
 };
-template <int P>
+template <int PA, int PB>
 PairSplits pair_splits(long long tiles, long long k) {
   const int pairs = std::max(1, host::sm_count() / 2);
   const long long chunks = (k + kChunk - 1) / kChunk;
-  const long long most = kMostAdditions * 16 / kChunk;
-  const long long fewest = P == 1 ? (chunks + most - 1) / most : 1;
+  const long long most = kPairSum<PA, PB> / kChunk;
+  const long long fewest = PB == 1 ? (chunks + most - 1) / most : 1;
   PairSplits best{};
   double least = 1e30;
   for (long long n = fewest; n <= std::min(chunks, fewest + 31); ++n) {
@@ -359,37 +366,36 @@ long long pair_tiles(long long m, int n) {
   return (m + kPairRows - 1) / kPairRows * ((n + tile_n - 1) / tile_n);
 }
 
-// The map of an operand: planes of its parts (16-bit ones: of one), whose rows are k or,
-// MN, m or n.
-template <class T, bool MN>
+// The map of an operand: planes of its parts (one alone has as many rows as there are),
+// whose rows are k or, MN, m or n.
+template <class T, int P, bool MN>
 bool make_operand_map(CUtensorMap& map, const Planes& x, int mn, long long k, int box_rows) {
-  constexpr int P = kOperandParts<T>;
   const long long rows = P == 1 ? (MN ? k : mn) : static_cast<long long>(x.plane_rows) * P;
   return make_map<PairOperand<T>>(map, x.data, rows, MN ? mn : k, x.ld, 64, MN ? kChunk : box_rows);
 }
 
-// a: (m, k) rows or, AMN, (k, m); b: (n, k) or, BMN, (k, n); out (splits, m, n).
-template <class T, bool AMN, bool BMN>
+// a: (m, k) rows or, AMN, (k, m), of PA parts; b: (n, k) or, BMN, (k, n); out (splits, m, n).
+template <class T, int PA, bool AMN, bool BMN>
 int launch_pairs(int m, int n, long long k, const Planes& a, const Planes& b,
                  const PairSplits& splits, float* out, bool accumulate, cudaStream_t s) {
-  constexpr int P = kOperandParts<T>;
+  constexpr int PB = kOperandParts<T>;
   PairParams p{};
   p.m = m, p.n = n, p.k = k, p.k_per_split = splits.k, p.splits = splits.count;
-  p.tile_n = pair_tile_n<P>(n);
+  p.tile_n = pair_tile_n<PB>(n);
   p.tiles_m = (m + kPairRows - 1) / kPairRows;
   p.tiles_n = (n + p.tile_n - 1) / p.tile_n;
   p.out = out, p.accumulate = accumulate;
   p.a_plane_rows = a.plane_rows, p.b_plane_rows = b.plane_rows;
-  if (!make_operand_map<T, AMN>(p.a_map, a, m, k, 128) ||
-      !make_operand_map<T, BMN>(p.b_map, b, n, k, p.tile_n / 2))
+  if (!make_operand_map<T, PA, AMN>(p.a_map, a, m, k, 128) ||
+      !make_operand_map<T, PB, BMN>(p.b_map, b, n, k, p.tile_n / 2))
     return host::fail(kInvalidArgument, "feature products: operand maps");
   p.copy_out = make_map<float>(p.out_map, out, static_cast<long long>(splits.count) * m, n, n, 32,
                                32);
   p.error = host::device_error_word();
   if (!p.error) return kCudaError;
-  const int stage = P * (kAPlane + b_plane_bytes<BMN>(p.tile_n / 2));
+  const int stage = PA * kAPlane + PB * b_plane_bytes<BMN>(p.tile_n / 2);
   p.stages = std::min(kPairStages, (kOneBlockBytes - 1024 - kPairPatches) / stage);
-  constexpr auto* kernel = pair_product_kernel<T, P, AMN, BMN>;
+  constexpr auto* kernel = pair_product_kernel<T, PA, PB, AMN, BMN>;
   if (!host::allow_shared<kernel>())
     return host::check_launch("feature products: shared memory");
   const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n * p.splits;

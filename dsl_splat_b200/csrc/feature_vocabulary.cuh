@@ -166,10 +166,12 @@ SPLAT_DEV float4 patch_sums(uint32_t patch, const float* v) {
   return sum;
 }
 
-template <class T, int P, bool SLOPES>
+// P: parts of x and W; DZ: parts of dz, 0 for the statistics.
+template <class T, int P, int DZ>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVocabularyThreads, 1)
     vocabulary_kernel(const __grid_constant__ VocabularyParams p) {
   constexpr int kEpilogue = kVocabularyWarps;
+  constexpr bool SLOPES = DZ > 0;
   extern __shared__ unsigned char dynamic[];
   __shared__ PairBarriers barriers;
   const uint32_t base = (tc::shared_address(dynamic) + 1023u) & ~1023u;
@@ -207,7 +209,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVocabularyThreads, 
     }
   } else if (warp == kEpilogue + 1) {
     if (rank == 0) {
-      PairIssue<P> issue(barriers, ring_at, b_plane, p.stages, tmem,
+      PairIssue<P, P> issue(barriers, ring_at, b_plane, p.stages, tmem,
                          tc::instruction_pair(!kIsF16<T>, false, false, p.tile_n));
       for (int item = pair; item < items && ok; item += pairs) {
         const int split = item / p.row_blocks;
@@ -313,8 +315,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVocabularyThreads, 
             // patches of 32 rows and 32 words for tensor copies, two in turn; planes of
             // parts have zeros in the rows behind the last
 #pragma unroll
-            for (int i = 0; i < P; ++i, ++patches) {
+            for (int i = 0; i < DZ; ++i, ++patches) {
               const Patch<PairOperand<T>> patch{patch_at + (patches & 1) * 2048};
+              constexpr bool kLasts[3] = {DZ == 1, DZ == 2, true};
               if (lane == 0) tc::copies_out_read_but<1>();
               __syncwarp();
 #pragma unroll
@@ -322,23 +325,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVocabularyThreads, 
                 float* o = v + piece * 8;
                 uint4 r;
                 if constexpr (P == 1) {
-                  const Vec<T, 8> rounded = round_values<T, 8>(reinterpret_cast<float(&)[8]>(*o));
+                  const Vec<T, 8> rounded =
+                      kLasts[i] ? round_values<T, 8>(reinterpret_cast<float(&)[8]>(*o))
+                                : take_first<T, 8>(reinterpret_cast<float(&)[8]>(*o));
                   r = reinterpret_cast<const uint4&>(rounded);
                 } else {
-                  constexpr bool kLast[3] = {false, false, true};
-                  r = kLast[i] ? make_uint4(take_part<true>(o[0], o[1]), take_part<true>(o[2], o[3]),
-                                            take_part<true>(o[4], o[5]), take_part<true>(o[6], o[7]))
-                               : make_uint4(take_part<false>(o[0], o[1]),
-                                            take_part<false>(o[2], o[3]),
-                                            take_part<false>(o[4], o[5]),
-                                            take_part<false>(o[6], o[7]));
+                  r = kLasts[i] ? make_uint4(take_part<true>(o[0], o[1]), take_part<true>(o[2], o[3]),
+                                             take_part<true>(o[4], o[5]), take_part<true>(o[6], o[7]))
+                                : make_uint4(take_part<false>(o[0], o[1]),
+                                             take_part<false>(o[2], o[3]),
+                                             take_part<false>(o[4], o[5]),
+                                             take_part<false>(o[6], o[7]));
                 }
                 store_shared(patch.at(lane, piece), r);
               }
               tc::fence_async_proxy();
               __syncwarp();
               if (lane == 0) {
-                if (row0 < (P == 1 ? p.count : p.dz_plane_rows) && col0 < V)
+                if (row0 < (DZ == 1 ? p.count : p.dz_plane_rows) && col0 < V)
                   tc::copy_out(&p.dz_map, col0, row0 + i * p.dz_plane_rows, patch.base);
                 else
                   tc::copy_out_none();  // counts too

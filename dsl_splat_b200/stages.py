@@ -921,7 +921,7 @@ def feature_entropy_backward(x: Tensor, weight: Tensor, target: Tensor, bias: Te
     if rows and any(t is not None for t in (dx, dweight, dbias)):
         dtype, device = FEATURE_DTYPES[x.dtype], x.device
         size = _query("splat_feature_entropy_workspace_bytes", device.index, dtype, rows, k,
-                      vocabulary, 1)
+                      vocabulary, 2 if reduction == "none" else 1)
         ws = x.new_empty((size,), dtype=torch.uint8)
         x, weight, bias, target = _dense(x), _dense(weight), _dense(bias), _dense(target)
         upstream, moments = _dense(upstream), _dense(moments)
