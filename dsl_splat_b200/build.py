@@ -1,6 +1,6 @@
 """Builds libsplat200.so in place for sm_100a (nvcc, no JIT cache).
 
-Six translation units, compiled in parallel and linked into one library:
+Translation units, compiled in parallel and linked into one library:
 
 * splat200.cu (entry points, forward kernels, binning, blending) with
   -fmad=false: every multiply-add stays two IEEE roundings unless the source
@@ -11,9 +11,9 @@ Six translation units, compiled in parallel and linked into one library:
   -prec-sqrt=false: their outputs are gradients, compared within a relative
   tolerance, and contraction plus the approximate divide and square root (a
   few ulp) remove a large part of their arithmetic;
-* feature_linear.cu, feature_linear_backward.cu and feature_norm.cu (the
-  feature operators) with -fmad=true: their results are compared within their
-  types' rounding.
+* the feature operators (feature_*.cu) and the optimizer (adamw.cu) with
+  -fmad=true: their results are compared within their types' rounding; where a
+  code in 8 bits depends on the order of operations, the source asks for each.
 
 splat200.cu keeps IEEE-rounded division and square root (the nvcc defaults
 -prec-div=true -prec-sqrt=true); nothing is built with --use_fast_math.

@@ -13,9 +13,10 @@
 // fp32 results before their rounding; of u_i of their own dz is taken relative to the power of two
 // that is not below any |u_i|, and the results are multiplied by that.  float16, whose
 // smallest value would otherwise swallow the tail of a large vocabulary, has 2^15 times dz.
-// 16-bit types hold dz with u_i of their own as two values (2.4e-3 instead of 1.7e-3
-// relative error of dx and dW for bf16 with one), whose products cost twice the time; without,
-// a label's dz is nearly 1 and the others are small beside it.
+// 16-bit types hold dz with u_i of their own as two values, whose products take twice the time:
+// with one, dx and dW would be off by 2.4e-3 instead of 1.7e-3 (bf16, relative), since a label's
+// dz would take the rounding of its u.  With a shared u one is enough, since a label's dz is
+// nearly 1 then.  Layers beyond on_chip() keep the one.
 #include <algorithm>
 
 #include "feature_join.cuh"
@@ -334,7 +335,8 @@ EntropyPlan plan_entropy(long long rows, int k, int vocabulary, int purpose) {
     piece = rows;
   } else {
     // bytes of a row's logits, or of its dz, and of its dx before the rounding
-    const long long row = std::max(vocabulary * (plan.on_chip ? 2LL * dz_parts<T>(each) : 4LL), 4LL * k);
+    const long long slopes = plan.on_chip ? 2LL * dz_parts<T>(each) : 4LL;
+    const long long row = std::max(vocabulary * slopes, 4LL * k);
     piece = std::max(1LL, kPieceBytes / row / unit) * unit;
     piece = std::min({piece, rows, 1LL << 23});  // 65535 ranges of 256 rows, and below
   }
@@ -535,9 +537,8 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
       p.moments = moments, p.upstream = upstream, p.factors = factors;
       p.dz_plane_rows = dz.plane_rows;
       if (dbias) p.column_sums = column_sums;
-      if (!make_map<PairOperand<T>>(p.dz_map, dz.data,
-                                    static_cast<long long>(dz.plane_rows) * parts, vocabulary, dz.ld,
-                                    32, 32))
+      const long long dz_rows = static_cast<long long>(dz.plane_rows) * parts;
+      if (!make_map<PairOperand<T>>(p.dz_map, dz.data, dz_rows, vocabulary, dz.ld, 32, 32))
         return host::fail(kInvalidArgument, "feature_entropy_backward: map");
       status = each ? launch_vocabulary<T, dz_parts<T>(true)>(p, plan, r, first, rows, k, xs, w,
                                                               bias, s)
@@ -650,7 +651,8 @@ int splat_feature_entropy(int dtype, long long rows, int k, int vocabulary, cons
   if (workspace_bytes < splat_feature_entropy_workspace_bytes(dtype, rows, k, vocabulary, 0))
     return host::fail(kWorkspaceTooSmall, "feature_entropy: workspace");
   if (!lies_well(dtype, k, x, weight, bias))
-    return host::fail(kInvalidArgument, "feature_entropy: x, weight and bias must be 16-byte aligned");
+    return host::fail(kInvalidArgument,
+                      "feature_entropy: x, weight and bias must be 16-byte aligned");
   Rows r{rows, vocabulary, id_bytes, reduction, ignored, target, host::device_error_word()};
   if (!r.error) return kCudaError;
   return SPLAT_FEATURE_TYPE(dtype, [&] {
@@ -678,11 +680,13 @@ int splat_feature_entropy_backward(int dtype, long long rows, int k, int vocabul
                                                               purpose_of(reduction)))
     return host::fail(kWorkspaceTooSmall, "feature_entropy_backward: workspace");
   if (!lies_well(dtype, k, x, weight, bias))
-    return host::fail(kInvalidArgument, "feature_entropy_backward: x, weight and bias must be 16-byte aligned");
+    return host::fail(kInvalidArgument,
+                      "feature_entropy_backward: x, weight and bias must be 16-byte aligned");
   Rows r{rows, vocabulary, id_bytes, reduction, ignored, target, host::device_error_word()};
   if (!r.error) return kCudaError;
   return SPLAT_FEATURE_TYPE(dtype, [&] {
-    return launch_backward<T>(r, k, x, weight, bias, reinterpret_cast<const Partial*>(moments), counted, upstream, dx, dweight, dbias,
+    return launch_backward<T>(r, k, x, weight, bias, reinterpret_cast<const Partial*>(moments),
+                              counted, upstream, dx, dweight, dbias,
                               static_cast<char*>(workspace), static_cast<cudaStream_t>(stream));
   });
 }

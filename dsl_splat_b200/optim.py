@@ -168,18 +168,19 @@ class _Launches:
             g = g.contiguous()
             self.held.append(g)
         address = p.data_ptr()
-        if address in self.places:
-            raise ValueError("a parameter is listed twice")
-        self.places.add(address)
         if bits == 8:
             record = (address, g.data_ptr(), m.codes.data_ptr(), v.codes.data_ptr(),
                       m.exponents.data_ptr(), v.exponents.data_ptr())
             self.written += (p, m.codes, v.codes, m.exponents, v.exponents)
         else:
-            record = (address, g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0)
+            record = (address, g.data_ptr(), m.data_ptr(), v.data_ptr())
             self.written += (p, m, v)
-        record = _RECORD.pack(*record, device_step, device_lr, n, step, lr, decay, betas[0],
-                              betas[1], eps)
+        written = {address, *record[2:]}
+        if len(written) < len(record) - 1 or not written.isdisjoint(self.places):
+            raise ValueError("a parameter or a moment is listed twice")
+        self.places |= written
+        record = _RECORD.pack(*record, *(0,) * (6 - len(record)), device_step, device_lr, n, step,
+                              lr, decay, betas[0], betas[1], eps)
         self.records.setdefault((index, p.dtype, bits, maximize), []).append(record)
 
     def run(self) -> None:
@@ -200,7 +201,7 @@ def adamw(params: Sequence[Tensor], grads: Sequence[Tensor],
     step counts from 1 and is the number of this step.  step, lr and weight_decay are
     one value or a list with one for each parameter; step may be a CUDA int64 and lr a CUDA
     float32 tensor of one value, which the kernel reads (a captured step then follows
-    them).  A parameter must not be listed twice."""
+    them).  No parameter or moment may be listed twice or share memory with another."""
     count = len(params)
     if not len(grads) == len(exp_avgs) == len(exp_avg_sqs) == count:
         raise ValueError("params, grads, exp_avgs and exp_avg_sqs must have the same length")

@@ -736,8 +736,9 @@ def _check_entropy(x, weight, target, bias, ignore_index, reduction):
 def _check_entropy_backward(x, weight, target, bias, ignore_index, reduction, moments, counted,
                             upstream):
     _check_entropy(x, weight, target, bias, ignore_index, reduction)
-    shapes = ((target.numel(), 2), (1,), target.shape if reduction == "none" else ())
-    for t, shape, name in zip((moments, counted, upstream), shapes, ("moments", "counted", "upstream")):
+    upstream_shape = target.shape if reduction == "none" else ()
+    for t, shape, name in ((moments, (target.numel(), 2), "moments"), (counted, (1,), "counted"),
+                           (upstream, upstream_shape, "upstream")):
         if t.dtype is not torch.float32 or t.device != x.device or t.shape != shape:
             raise ValueError(f"{name} must be float32 of shape {tuple(shape)} on x's device")
 

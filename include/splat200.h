@@ -646,10 +646,11 @@ int splat_feature_embedding_backward(int dtype, int id_bytes, long long count, i
  * k), bias (vocabulary) or NULL, target (rows) of id_bytes 4 or 8 (signed).  A row whose
  * target is `ignored` does not count; one whose target lies outside the vocabulary neither,
  * with the device error -6.  reduction: 0 none (loss of each row), 1 sum, 2 mean over the
- * rows that count (0 if none does).  A workspace is asked for with `backward` 0 for the
- * forward, 1 for the backward of a sum or mean, 2 for that of the rows' losses.  loss float32; moments (rows, 2) float32, the rows'
- * largest logits and sums in the units that the backward takes them in, or NULL; counted (1) float32, the rows that count (1 if none does), for the mean's
- * backward, or NULL. */
+ * rows that count (0 if none does).  loss float32; moments (rows, 2) float32, the rows'
+ * largest logits and sums in the units that the backward takes them in, or NULL; counted (1)
+ * float32, the rows that count (1 if none does), for the mean's backward, or NULL.  A workspace
+ * is asked for with `backward` 0 for the forward, 1 for the backward of a sum or a mean, 2 for
+ * that of the rows' losses. */
 size_t splat_feature_entropy_workspace_bytes(int dtype, long long rows, int k, int vocabulary,
                                              int backward);
 int splat_feature_entropy(int dtype, long long rows, int k, int vocabulary, const void* x,

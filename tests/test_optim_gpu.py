@@ -447,6 +447,11 @@ def test_refusals():
 
     refused("same length", [p], [g], [m], [])
     refused("listed twice", [p, p], [g, g], [m, m], [v, v])
+    refused("listed twice", [p, p.clone()], [g, g], [m, m], [v, v.clone()])
+    refused("listed twice", [p], [g], [m], [m])
+    first, second = optim.Moment8.zeros_like(p), optim.Moment8.zeros_like(p, squared=True)
+    refused("listed twice", [p], [g], [first],
+            [optim.Moment8(second.codes, first.exponents, squared=True)])
     refused("contiguous", [draw(3, 4, 5).t()], [draw(4, 5, 4)], [m], [v])
     refused("gradients must have", [p], [g.half()], [m], [v])
     refused("gradients must have", [p], [g[:9]], [m], [v])
