@@ -19,9 +19,9 @@
 //
 // 65536 x 512 bf16 features and 32768 words: statistics 1.42 ms (1550 TFLOP/s, tensor pipe 78 %
 // of cycles), slopes 1.97 (1120, 59 %: 4.3 GB of dz go out beside the exponentials).  307200 x 64
-// and 4096: 540 us (special-function pipe 56 %: waits for accumulators take the rest) and
-// 960 (32 %: the patches' shared memory, 59 %, and the 2.5 GB that leave).  Direct stores of dz
-// instead of patches took longer; so did chunks of 64 words, whose registers spill.
+// and 4096: 540 us (special-function pipe 56 %) and 850 (36 %), without a bias 450 and 620:
+// its addition and db's sums take issue slots.  Direct stores of dz instead of patches took
+// longer; so did chunks of 64 words, whose registers spill, and biases loaded before the logits.
 //
 // top and sum are kept apart for the slopes: rounded into one logarithm, they would cost
 // each probability 2^-24 of that logarithm.
@@ -145,31 +145,23 @@ SPLAT_DEV void add_bias(float (&v)[32], const T* bias, int words) {
   }
 }
 
-// The sums over a warp's rows of 32 columns, through its patch: a lane stores its row, then
-// adds four columns of eight rows.  Lanes 0 to 7 get four columns' sums each.
-SPLAT_DEV float4 patch_sums(uint32_t patch, const float* v) {
-  const int lane = threadIdx.x & 31, quad = lane & 7;
+// The sums over a warp's rows of 32 columns: lane j gets column j's.  Every step halves the
+// columns of a lane.  Through shared memory, whose wavefronts they then were most of, the
+// slopes of 307200 rows and 4096 words took 955 us instead of 850.
+template <int N>
+SPLAT_DEV float column_sum(const float (&v)[N]) {
+  if constexpr (N == 1) {
+    return v[0];
+  } else {
+    const bool upper = threadIdx.x & (N / 2);
+    float half[N / 2];
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    store_shared(patch + lane * 128 + ((j ^ (lane & 7)) << 4),
-                 make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
-                            __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3])));
-  __syncwarp();
-  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    const float4 row = load_shared(patch + ((lane & 24) + r) * 128 + ((quad ^ r) << 4));
-    sum.x += row.x, sum.y += row.y, sum.z += row.z, sum.w += row.w;
+    for (int i = 0; i < N / 2; ++i) {
+      const float sent = __shfl_xor_sync(0xffffffffu, upper ? v[i] : v[i + N / 2], N / 2);
+      half[i] = (upper ? v[i + N / 2] : v[i]) + sent;
+    }
+    return column_sum(half);
   }
-#pragma unroll
-  for (int o = 8; o < 32; o *= 2) {
-    sum.x += __shfl_xor_sync(0xffffffffu, sum.x, o);
-    sum.y += __shfl_xor_sync(0xffffffffu, sum.y, o);
-    sum.z += __shfl_xor_sync(0xffffffffu, sum.z, o);
-    sum.w += __shfl_xor_sync(0xffffffffu, sum.w, o);
-  }
-  __syncwarp();  // the patch has been read
-  return sum;
 }
 
 // P: parts of x and W; DZ: parts of dz, 0 for the statistics.
@@ -306,17 +298,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kVocabularyThreads, 
               for (int j = 0; j < 32; ++j) v[j] = label < 0 ? 0.0f : v[j];
             }
             if (p.column_sums) {  // before dz is rounded
-              if (lane == 0) tc::copies_out_read();
-              __syncwarp();
-              const float4 sum = patch_sums(patch_at, v);
-              float* sums = p.column_sums + static_cast<long long>(row0 / 32) * V;
-              const int j = col0 + lane * 4;
-              if (lane < 8 && row0 < p.count) {
-                if (j < V) sums[j] = sum.x;
-                if (j + 1 < V) sums[j + 1] = sum.y;
-                if (j + 2 < V) sums[j + 2] = sum.z;
-                if (j + 3 < V) sums[j + 3] = sum.w;
-              }
+              const float sum = column_sum(v);
+              if (row0 < p.count && col0 + lane < V)
+                p.column_sums[static_cast<long long>(row0 / 32) * V + col0 + lane] = sum;
             }
             // patches of 32 rows and 32 words for tensor copies, two in turn; planes of
             // parts have zeros in the rows behind the last
