@@ -8,8 +8,9 @@
 // No accumulator takes more than kMostAdditions of 16-bit products; those of parts take
 // kExactSum k in two accumulators, which the epilogue adds up in registers.
 //
-// 65536 x 512 bf16 features and 32768 words: dx 1.46 ms (1510 TFLOP/s), dW 1.6 (1370), tensor
-// pipe 71 and 67 % of cycles at the 1.5 to 1.6 GHz that the power allows.  307200 x 64 and
+// 65536 x 512 bf16 features and 32768 words: dx 1.46 ms (1510 TFLOP/s), dW 1.6 (1370) at the
+// 1.5 to 1.6 GHz that the power allows; a piece of it on its own has the tensor pipe 92 and 84 %
+// busy.  307200 x 64 and
 // 4096: 450 and 400 us, of which reading dz (2.5 GB) is the most: DRAM 73 and 77 %.
 #pragma once
 #include <algorithm>

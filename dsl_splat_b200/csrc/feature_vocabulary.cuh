@@ -17,8 +17,8 @@
 // special-function pipe 2048 cycles a tile of 256 words, the products 8 a k: the pipe binds
 // below 256 features, the tensor core above.
 //
-// 65536 x 512 bf16 features and 32768 words: statistics 1.42 ms (1550 TFLOP/s, tensor pipe 78 %
-// of cycles), slopes 1.97 (1120, 59 %: 4.3 GB of dz go out beside the exponentials).  307200 x 64
+// 65536 x 512 bf16 features and 32768 words: statistics 1.41 ms (1560 TFLOP/s, tensor pipe 85 %
+// of a piece's cycles), slopes 1.96 (1125, 59 %: 4.3 GB of dz go out beside the exponentials).  307200 x 64
 // and 4096: 540 us (special-function pipe 56 %) and 850 (36 %), without a bias 450 and 620:
 // its addition and db's sums take issue slots.  Direct stores of dz instead of patches took
 // longer; so did chunks of 64 words, whose registers spill, and biases loaded before the logits.
