@@ -11,7 +11,8 @@
 // accumulators, 32 words of 32 rows at a time, and give them back before they work on the
 // last of them; the leading block's product warp issues.  One half of the epilogue takes
 // the even tiles and the other the odd ones, so that the one's exponentials run under the
-// other's waits and maxima.  A pair stays with 256 rows over a range of words, so that a
+// other's waits and maxima (slopes of 65536 rows and 8192 words 258 to 314 us with
+// 64 to 256 bf16 features; 290 to 347 with all warps on each tile; as long at 512).  A pair stays with 256 rows over a range of words, so that a
 // row's running maximum and sum stay in a thread's registers; ranges and groups of warps
 // leave a partial result each, joined in a fixed order.  Exponentials take the
 // special-function pipe 2048 cycles a tile of 256 words, the products 8 a k: the pipe binds
