@@ -11,18 +11,19 @@
 // accumulators, 32 words of 32 rows at a time, and give them back before they work on the
 // last of them; the leading block's product warp issues.  One half of the epilogue takes
 // the even tiles and the other the odd ones, so that the one's exponentials run under the
-// other's waits and maxima (slopes of 65536 rows and 8192 words 258 to 314 us with
-// 64 to 256 bf16 features; 290 to 347 with all warps on each tile; as long at 512).  A pair stays with 256 rows over a range of words, so that a
-// row's running maximum and sum stay in a thread's registers; ranges and groups of warps
-// leave a partial result each, joined in a fixed order.  Exponentials take the
-// special-function pipe 2048 cycles a tile of 256 words, the products 8 a k: the pipe binds
-// below 256 features, the tensor core above.
+// other's waits and maxima (slopes of 65536 rows and 8192 words 258 to 314 us with 64 to
+// 256 bf16 features; 290 to 347 with all warps on each tile; as long at 512).  A pair stays
+// with 256 rows over a range of words, so that a row's running maximum and sum stay in a
+// thread's registers; ranges and groups of warps leave a partial result each, joined in a
+// fixed order.  Exponentials take the special-function pipe 2048 cycles a tile of 256 words,
+// the products 8 a k: the pipe binds below 256 features, the tensor core above.
 //
 // 65536 x 512 bf16 features and 32768 words: statistics 1.41 ms (1560 TFLOP/s, tensor pipe 85 %
-// of a piece's cycles), slopes 1.96 (1125, 59 %: 4.3 GB of dz go out beside the exponentials).  307200 x 64
-// and 4096: 540 us (special-function pipe 56 %) and 850 (36 %), without a bias 450 and 620:
-// its addition and db's sums take issue slots.  Direct stores of dz instead of patches took
-// longer; so did chunks of 64 words, whose registers spill, and biases loaded before the logits.
+// of a piece's cycles), slopes 1.96 (1125, 59 %: 4.3 GB of dz go out beside the
+// exponentials).  307200 x 64 and 4096: 540 us (special-function pipe 56 %) and 850 (36 %),
+// without a bias 450 and 620: its addition and db's sums take issue slots.  Direct stores of dz
+// instead of patches took longer; so did chunks of 64 words, whose registers spill, and
+// biases loaded before the logits.
 //
 // top and sum are kept apart for the slopes: rounded into one logarithm, they would cost
 // each probability 2^-24 of that logarithm.

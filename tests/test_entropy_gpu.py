@@ -119,6 +119,13 @@ def test_several_pieces(m, k, v, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_pieces_of_a_large_vocabulary(reduction, dtype):
+    """dz takes 1.2 GB at least: two to four pieces, the last one short."""
+    run(*make(4500, 24, 1 << 17, dtype, 27), reduction=reduction)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_wide_features(dtype):
     """More inputs than one accumulator takes."""
     run(*make(70, 5000, 90, dtype, 4))
@@ -224,6 +231,28 @@ def test_rows_do_not_meet():
             assert torch.equal(a[rest], c[rest])
             assert not a[7].isfinite().any()
         assert not got[0][130].isfinite()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_upstreams_that_are_not_finite(dtype):
+    """They reach their rows' dx, and no other's."""
+    x, w, b, target = make(300, 64, 300, dtype, 28, ignored=0.1)
+    target[5], target[9] = -100, 3
+    up = draws(29)(300, dtype=torch.float32)
+
+    def dx():
+        leaf = x.detach().clone().requires_grad_()
+        loss = features.linear_cross_entropy(leaf, w, target, b, reduction="none")
+        return torch.autograd.grad(loss, leaf, up)[0]
+
+    want = dx()
+    up[[5, 9, 200]] = torch.tensor([math.nan, math.inf, math.nan], device="cuda")
+    target[200] = 4
+    got = dx()
+    rest = torch.ones(300, dtype=torch.bool)
+    rest[[9, 200]] = False
+    assert torch.equal(got[rest], want[rest]) and not got[5].any()
+    assert not got[9].isfinite().any() and not got[200].isfinite().any()
 
 
 def test_targets_outside_the_vocabulary():
