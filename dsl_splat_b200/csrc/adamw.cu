@@ -154,15 +154,13 @@ __global__ void __launch_bounds__(kThreads) step32_kernel(const __grid_constant_
     if (i < end) {
       float root;
       p[i] = from_float<T>(update<false>(to_float(p[i]), to_float(g[i]) * table.ascend, m[i], v[i],
-                                         root,
-                                  t, r));
+                                         root, t, r));
     }
   } else {
     for (long long i = begin + threadIdx.x; i < end; i += kThreads) {
       float root;
       p[i] = from_float<T>(update<false>(to_float(p[i]), to_float(g[i]) * table.ascend, m[i], v[i],
-                                         root,
-                                  t, r));
+                                         root, t, r));
     }
   }
 }

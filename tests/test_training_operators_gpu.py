@@ -198,3 +198,49 @@ def test_operators_by_name():
                     ops.feature_entropy_backward(x, words, target, bias, -100, "mean", moments,
                                                  counted, up)):
         assert torch.equal(g, h)
+
+
+def test_offsets_beyond_32_bits():
+    """The last rows of more than 2^31 values are those that they are on their own."""
+    rows, tail = (1 << 25) + 1001, 700
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.empty(rows, 64, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    end = x[-tail:].clone()
+    w, b = x[0].clone(), x[1].clone()
+
+    def norm(t, dy):
+        t = t.detach().requires_grad_()
+        y = features.layer_norm(t, w, b, activation="silu")
+        return y.detach(), torch.autograd.grad(y, t, dy)[0]
+
+    for whole, alone in zip(norm(x, x), norm(end, end)):
+        assert torch.equal(whole[-tail:], alone)
+
+    words = x[:40].clone()
+    target = torch.randint(0, 40, (rows,), device="cuda", generator=g, dtype=torch.int32)
+
+    def entropy(t, target):
+        t = t.detach().requires_grad_()
+        loss = features.linear_cross_entropy(t, words, target, reduction="none")
+        return loss.detach(), torch.autograd.grad(loss.sum(), t)[0]
+
+    for whole, alone in zip(entropy(x, target), entropy(end, target[-tail:].clone())):
+        assert torch.equal(whole[-tail:], alone)
+
+    table = x[:40].clone().requires_grad_()
+    y = features.embedding(target, table)
+    assert torch.equal(y.detach()[-tail:], table.detach()[target[-tail:]])
+    # whole numbers below 2^24, whose sums in fp32 are exact
+    got, = torch.autograd.grad(y, table, torch.ones_like(y))
+    count = torch.bincount(target.long(), minlength=40)
+    assert torch.equal(got, count.to(got.dtype)[:, None].expand_as(got))
+    del y
+
+    def step(p, g):
+        m, v = torch.zeros_like(p, dtype=torch.float32), torch.ones_like(p, dtype=torch.float32)
+        optim.adamw([p], [g], [m], [v], step=3, lr=0.1)
+        return p[-tail:], m[-tail:], v[-tail:]
+
+    gradient = x.flip(0)
+    alone = step(end.clone(), gradient[-tail:].clone())
+    assert all(torch.equal(a, c) for a, c in zip(step(x, gradient), alone))
