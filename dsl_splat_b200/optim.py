@@ -219,6 +219,63 @@ def adamw(params: Sequence[Tensor], grads: Sequence[Tensor],
     launches.run()
 
 
+def _check_loaded_group(group: dict, own: dict) -> None:
+    """Refuses a saved group that this optimizer would not follow; own: the group that
+    takes it over."""
+    for name in ("amsgrad", "differentiable"):
+        if group.get(name):
+            raise ValueError(f"a state of {name}=True has no counterpart here")
+    # L2 decay, which goes through the moments
+    if not group.get("decoupled_weight_decay", True) and group["weight_decay"]:
+        raise ValueError("a state whose weight decay is not decoupled has no counterpart here")
+    _check_settings(group["betas"], group["eps"], group["weight_decay"])
+    if group.get("state_bits", own["state_bits"]) not in (8, 32):
+        raise ValueError("state_bits must be 8 or 32")
+
+
+def _counted(step: Any) -> int:
+    """The steps of a state: an integer, or a tensor of one, which torch.optim holds in
+    float32."""
+    if isinstance(step, Tensor):
+        if step.numel() != 1:
+            raise ValueError("a state's step must be one number")
+        step = step.item()
+    if isinstance(step, bool) or not isinstance(step, Real) or not 0 <= step < 1 << 63 \
+            or step != int(step):
+        raise ValueError("a state's step must be a number of steps")
+    return int(step)
+
+
+def _loaded_state(saved: dict, p: Tensor, bits: int, capturable: bool) -> dict:
+    """A parameter's saved state as `AdamW` holds it: of its own or of torch.optim.AdamW."""
+    if "max_exp_avg_sq" in saved:
+        raise ValueError("a state of amsgrad=True has no counterpart here")
+    state = {name: v.to(p.device, copy=True).contiguous() if isinstance(v, Tensor) else v
+             for name, v in saved.items() if name != "step"}
+    if "step" in saved:
+        step = _counted(saved["step"])
+        state["step"] = (torch.full((), step, dtype=torch.int64, device=p.device) if capturable
+                         else step)
+    for name, squared in (("exp_avg", False), ("exp_avg_sq", True)):
+        if name not in saved:
+            continue
+        if not isinstance(state[name], Tensor) or state[name].shape != p.shape:
+            raise ValueError(f"a state's {name} must have its parameter's shape")
+        if name + "_exponents" in saved:
+            moment = Moment8(state[name], state[name + "_exponents"], squared)
+            if bits == 32:
+                state[name] = moment.values()
+                del state[name + "_exponents"]
+        elif not state[name].is_floating_point():
+            raise ValueError(f"a state's {name} must hold floating-point values")
+        else:
+            state[name] = state[name].float()
+            if bits == 8:
+                moment = Moment8.of(state[name], squared)
+                state[name], state[name + "_exponents"] = moment.codes, moment.exponents
+    return state
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW with one launch for all parameters of a device and dtype.
 
@@ -227,7 +284,10 @@ class AdamW(torch.optim.Optimizer):
     `moments` and `set_moments` take the values they stand for, whatever the bits,
     which is what code that adds or removes Gaussians has to carry over.
     capturable: steps are counted on the device, so that a captured step() can be
-    replayed (lr may then be a CUDA float32 tensor)."""
+    replayed (lr may then be a CUDA float32 tensor).
+
+    load_state_dict takes torch.optim.AdamW's state too, but for amsgrad: its steps are
+    converted and its moments held in float32, or in 8 bits where the group has them."""
 
     def __init__(self, params: Iterable, lr: float | Tensor = 1e-3,
                  betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -302,6 +362,7 @@ class AdamW(torch.optim.Optimizer):
                 state = self._state(p, group)
                 step = state["step"]
                 if isinstance(step, Tensor):
+                    _check_step(step)  # the kernel reads it as it lies
                     counters.append(step)
                 else:
                     counted.append(state)
@@ -337,12 +398,33 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict: dict) -> None:
-        super().load_state_dict(state_dict)
-        # torch casts a state to its parameter's dtype; moments keep theirs
-        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
-        own = [p for group in self.param_groups for p in group["params"]]
-        for i, p in zip(saved, own):
-            if i in state_dict["state"]:
-                self.state[p] = {
-                    name: v.to(p.device, copy=True).contiguous() if isinstance(v, Tensor) else v
-                    for name, v in state_dict["state"][i].items()}
+        states: list[tuple[Tensor, dict]] = []
+        # a saved group of torch.optim.AdamW lacks some of the settings
+        settings = [{name: group[name] for name in self.defaults} for group in self.param_groups]
+
+        def read(_, saved: dict) -> None:
+            """The whole state, before anything of this optimizer changes."""
+            for group, own in zip(saved["param_groups"], self.param_groups):
+                _check_loaded_group(group, own)
+                bits = group.get("state_bits", own["state_bits"])
+                capturable = group.get("capturable", own["capturable"])
+                for i, p in zip(group["params"], own["params"]):
+                    if i in saved["state"]:
+                        states.append((p, _loaded_state(saved["state"][i], p, bits, capturable)))
+
+        def take(_) -> None:
+            for group, own in zip(self.param_groups, settings):
+                for name, value in own.items():
+                    group.setdefault(name, value)
+            # torch casts a state to its parameter's dtype; moments keep theirs
+            for p, state in states:
+                self.state[p] = state
+
+        # behind the hooks that change what is loaded, before those that look at the result
+        hooks = (self.register_load_state_dict_pre_hook(read),
+                 self.register_load_state_dict_post_hook(take, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()

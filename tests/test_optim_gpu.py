@@ -324,6 +324,78 @@ def test_state_dict(bits, dtype):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["host", "capturable", "fused"])
+def test_state_of_torch(kind, dtype, bits):
+    """A checkpoint of torch.optim.AdamW is followed by the step that its formula asks for."""
+    params = scene(9, dtype=dtype)
+    theirs = torch.optim.AdamW([{"params": params[:3], "lr": 0.01},
+                                {"params": params[3:], "lr": 0.002}], weight_decay=0.1,
+                               **({kind: True} if kind != "host" else {}))
+    for step in range(5):
+        set_grads(params, 40 * step)
+        theirs.step()
+    saved = copy.deepcopy(theirs.state_dict())
+    ours = optim.AdamW([{"params": params[:3]}, {"params": params[3:]}], lr=0.5, state_bits=bits)
+    ours.load_state_dict(saved)
+    for i, group in enumerate(ours.param_groups):
+        assert group["lr"] == (0.01, 0.002)[i] and group["state_bits"] == bits
+    moments = [tuple(t.clone() for t in ours.moments(p)) for p in params]
+    for i, (p, (m, v)) in enumerate(zip(params, moments)):
+        state = saved["state"][i]
+        if bits == 32:
+            assert torch.equal(m, state["exp_avg"].float())
+            assert torch.equal(v, state["exp_avg_sq"].float())
+        step = ours.state[p]["step"]
+        assert int(step) == 5 and isinstance(step, torch.Tensor) == (kind == "capturable")
+    before = [p.detach().clone() for p in params]
+    set_grads(params, 900)
+    ours.step()
+    for p, b, (m, v), lr in zip(params, before, moments, [0.01] * 3 + [0.002] * 3):
+        want, tolerance = reference(b, p.grad, m, v, 6, lr, (0.9, 0.999), 1e-8, 0.1)
+        close(p.detach(), want[0], tolerance[0], "p")
+        assert int(ours.state[p]["step"]) == 6
+    # a state of its own that has been through torch.optim's again
+    twin = optim.AdamW([{"params": params[:3]}, {"params": params[3:]}])
+    twin.load_state_dict(copy.deepcopy(ours.state_dict()))
+    for p in params:
+        for a, c in zip(ours.moments(p), twin.moments(p)):
+            assert torch.equal(a, c)
+
+
+def test_states_that_are_refused_change_nothing():
+    params = scene(10)
+    twins = [p.detach().clone().requires_grad_() for p in params]
+    theirs = torch.optim.AdamW(twins, amsgrad=True)
+    ours = optim.AdamW(params, lr=0.03)
+    for p in (*params, *twins):
+        p.grad = torch.ones_like(p)
+    theirs.step()
+    ours.step()
+    before = [tuple(t.clone() for t in ours.moments(p)) for p in params]
+    with pytest.raises(ValueError, match="amsgrad"):
+        ours.load_state_dict(theirs.state_dict())
+    assert ours.param_groups[0]["lr"] == 0.03
+    for p, was in zip(params, before):
+        assert all(torch.equal(a, c) for a, c in zip(ours.moments(p), was))
+
+
+def test_hooks_of_a_loaded_state():
+    """A hook that changes what is loaded is heard, one behind it sees the result."""
+    p, q = draw(1, 40).requires_grad_(), draw(2, 40).requires_grad_()
+    ours, twin = optim.AdamW([p]), optim.AdamW([q])
+    p.grad = torch.ones_like(p)
+    ours.step()
+    seen = []
+    twin.register_load_state_dict_pre_hook(
+        lambda _, s: {**s, "state": {0: {**s["state"][0], "step": 41}}})
+    twin.register_load_state_dict_post_hook(lambda o: seen.append(o.state[q]["step"]))
+    twin.load_state_dict(ours.state_dict())
+    assert seen == [41] and twin.state[q]["step"] == 41
+    assert torch.equal(twin.moments(q)[0], ours.moments(p)[0])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_fewer_and_more_gaussians(bits):
     """What a densification does: new tensors take over rows of the moments."""
     p = draw(4, 300, 3).requires_grad_()

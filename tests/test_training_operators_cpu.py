@@ -210,6 +210,78 @@ def test_moment8_refusals():
         optim.Moment8.of(torch.zeros(3))
 
 
+def torch_state(cls=torch.optim.AdamW, steps=3, dtype=torch.float32, **options):
+    """A parameter and torch's state_dict of it after some steps."""
+    p = torch.linspace(-1, 1, 12, dtype=dtype).reshape(4, 3).requires_grad_()
+    optimizer = cls([p], **options)
+    for step in range(steps):
+        p.grad = torch.full_like(p, 0.5 + step)
+        optimizer.step()
+    return p, optimizer.state_dict()
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_loaded_states_of_torch(dtype, capturable):
+    """torch counts its steps in float32 and holds moments in their parameter's type."""
+    p, saved = torch_state(dtype=dtype)
+    state = saved["state"][0]
+    assert state["step"].dtype is torch.float32
+    got = optim._loaded_state(state, p, 32, capturable)
+    if capturable:
+        assert got["step"].dtype is torch.int64 and got["step"].shape == ()
+    else:
+        assert type(got["step"]) is int
+    assert int(got["step"]) == 3
+    for name in ("exp_avg", "exp_avg_sq"):
+        assert got[name].dtype is torch.float32 and got[name].is_contiguous()
+        assert torch.equal(got[name], state[name].float())
+        assert got[name].data_ptr() != state[name].data_ptr()
+    # and this optimizer's own counts, of either kind
+    for step in (3, torch.tensor(3)):
+        assert int(optim._loaded_state({**state, "step": step}, p, 32, capturable)["step"]) == 3
+    assert optim._loaded_state({}, p, 32, capturable) == {}
+
+
+def test_loaded_states_that_are_refused():
+    p, saved = torch_state(amsgrad=True)
+    with pytest.raises(ValueError, match="amsgrad"):
+        optim._loaded_state(saved["state"][0], p, 32, False)
+    own = dict(state_bits=32)
+    with pytest.raises(ValueError, match="amsgrad"):
+        optim._check_loaded_group(saved["param_groups"][0], own)
+    p, saved = torch_state()
+    group, state = saved["param_groups"][0], saved["state"][0]
+    optim._check_loaded_group(group, own)
+    for change, message in ((dict(differentiable=True), "differentiable"),
+                            (dict(decoupled_weight_decay=False), "decoupled"),
+                            (dict(betas=(0.9, 1.0)), "betas"), (dict(state_bits=16), "state_bits")):
+        with pytest.raises(ValueError, match=message):
+            optim._check_loaded_group({**group, **change}, own)
+    optim._check_loaded_group({**group, "decoupled_weight_decay": False, "weight_decay": 0.0}, own)
+    for change, message in ((dict(step=torch.tensor(1.5)), "step"), (dict(step=-1), "step"),
+                            (dict(step=torch.ones(2)), "step"), (dict(step=None), "step"),
+                            (dict(step=torch.tensor(float("nan"))), "step"),
+                            (dict(exp_avg=torch.zeros(3, 4)), "exp_avg must"),
+                            (dict(exp_avg_sq=torch.zeros(4, 3, dtype=torch.uint8)), "exp_avg_sq"),
+                            (dict(exp_avg=None), "exp_avg must")):
+        with pytest.raises(ValueError, match=message):
+            optim._loaded_state({**state, **change}, p, 32, False)
+
+
+def test_steps_of_another_type_are_not_read(monkeypatch):
+    """A state's counter on the device is read as 64-bit integers lie."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    with FakeTensorMode():
+        for step in (fake(), fake(2, dtype=torch.int64), fake(dtype=torch.int64, device="cpu")):
+            p = fake(4, 3).requires_grad_()
+            p.grad = fake(4, 3)
+            optimizer = optim.AdamW([p])
+            optimizer.state[p] = {"step": step, "exp_avg": fake(4, 3), "exp_avg_sq": fake(4, 3)}
+            with pytest.raises(ValueError, match="step must be"):
+                optimizer.step()
+
+
 ENTROPY = dict(x=(6, 4), weight=(9, 4), target=(6,), bias=(9,))
 
 
