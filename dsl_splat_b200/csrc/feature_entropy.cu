@@ -242,12 +242,29 @@ void add_columns(int vocabulary, int ranges, const float* sums, bool begin, floa
                        host::counted(s)>>>(vocabulary, ranges, sums, begin, total);
 }
 
+// What dW is formed of: x without the rows that do not count, which may hold infinities and
+// NaN (0 times them would reach every word; 20 us of 2390 for 307200 x 64 bf16).  `from`: rows of 16-byte pieces, which are copied; or NULL: planes of parts, in place.
+__global__ void __launch_bounds__(kThreads)
+    keep_counted_kernel(const Rows p, long long first, int rows, int pieces, const uint4* from,
+                        int parts, long long plane_pieces, uint4* to) {
+  // a piece's values are below 2^30 (plan_entropy)
+  const uint32_t i = blockIdx.x * static_cast<uint32_t>(kThreads) + threadIdx.x;
+  const int row = static_cast<int>(i / static_cast<uint32_t>(pieces));
+  if (row >= rows) return;
+  const bool counts = label_of(p, first + row) >= 0;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  if (from) to[i] = counts ? from[i] : zero;
+  else if (!counts)
+    for (int part = 0; part < parts; ++part) to[part * plane_pieces + i] = zero;
+}
+
 // fp32 sums (of several splits, `stride` values apart) times the factor, rounded; V of
-// them to an access.
+// them to an access.  columns: of dx's rows, of which those that do not count get zeros whatever
+// W and the factor are; 0 for sums over rows, of which those of nothing are 0 for any factor.
 template <class T, int V>
 __global__ void __launch_bounds__(kThreads)
     finish_kernel(long long count, int splits, long long stride, const float* from,
-                  const Factors* factors, T* to) {
+                  const Factors* factors, const Rows p, long long first, int columns, T* to) {
   const float factor = factors->out;
   const long long step = static_cast<long long>(kThreads) * gridDim.x * V;
   for (long long i = (blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x) * V; i < count;
@@ -260,20 +277,28 @@ __global__ void __launch_bounds__(kThreads)
       for (int k = 0; k < V; ++k) sum[k] += v.v[k];
     }
 #pragma unroll
-    for (int k = 0; k < V; ++k) sum[k] *= factor;
+    for (int k = 0; k < V; ++k) {
+      const float plain = sum[k];
+      sum[k] *= factor;
+      // rows that do not count have sums of 0, or of 0 times what W has
+      if (!isfinite(sum[k]) &&
+          (columns ? label_of(p, first + (i + k) / columns) < 0 : plain == 0.0f))
+        sum[k] = 0.0f;
+    }
     *reinterpret_cast<Vec<T, V>*>(to + i) = round_values<T, V>(sum);
   }
 }
 template <class T>
 void finish(long long count, int splits, long long stride, const float* from,
-            const Factors* factors, void* to, cudaStream_t s) {
+            const Factors* factors, void* to, cudaStream_t s, const Rows& rows = {},
+            long long first = 0, int columns = 0) {
   const bool vector = count % 4 == 0 && stride % 4 == 0 && host::aligned(to, 4 * sizeof(T));
   const int per_block = kThreads * (vector ? 4 : 1);
   const unsigned grid = static_cast<unsigned>(
       std::min<long long>((count + per_block - 1) / per_block, 1LL << 30));
   auto* kernel = vector ? finish_kernel<T, 4> : finish_kernel<T, 1>;
-  kernel<<<grid, kThreads, 0, host::counted(s)>>>(count, splits, stride, from, factors,
-                                                  static_cast<T*>(to));
+  kernel<<<grid, kThreads, 0, host::counted(s)>>>(count, splits, stride, from, factors, rows,
+                                                  first, columns, static_cast<T*>(to));
 }
 
 // ---- launching -----------------------------------------------------------------------
@@ -354,8 +379,9 @@ EntropyPlan plan_entropy(long long rows, int k, int vocabulary, int purpose) {
   plan.factors = take(sizeof(Factors));
   plan.loss_sums = take(sizeof(LossSum) * kLossBlocks);
   if (!plan.on_chip) plan.logits = take(4ull * piece * vocabulary);
-  // 16-bit rows that lie well need no planes, which their address decides
-  plan.x_planes = take(sizeof(T) == 2 && k % 8 == 0 ? 0 : plane_bytes<T>(piece, k));
+  // 16-bit rows that lie well need no planes, which their address decides; those of x have a
+  // copy for dW
+  plan.x_planes = take(sizeof(T) == 2 && k % 8 == 0 && !backward ? 0 : plane_bytes<T>(piece, k));
   plan.w_planes = take(sizeof(T) == 2 && k % 8 == 0 ? 0 : plane_bytes<T>(vocabulary, k));
   if (!backward) {
     plan.moments = take(sizeof(Partial) * rows);
@@ -433,6 +459,21 @@ int launch_logits(int rows, int k, int vocabulary, const Planes& x, const Planes
   p.k_per_split = k, p.splits = 1;
   p.out = z;
   return launch_product<T, P, false, T, P, false, float, float, kPlain>(p, s);
+}
+
+// keep_counted_kernel of a piece's x, whose planes lie in the workspace or are x itself.
+template <class T>
+Planes keep_counted(const Rows& r, long long first, int rows, const Planes& xs, void* to,
+                    cudaStream_t s) {
+  const bool copies = xs.data != to;
+  const int pieces = xs.ld / 8;
+  keep_counted_kernel<<<host::blocks_for(static_cast<long long>(rows) * pieces, kThreads),
+                        kThreads, 0, host::counted(s)>>>(
+      r, first, rows, pieces, copies ? static_cast<const uint4*>(xs.data) : nullptr,
+      kOperandParts<T>, static_cast<long long>(xs.plane_rows) * pieces, static_cast<uint4*>(to));
+  Planes kept = xs;
+  kept.data = to;
+  return kept;
 }
 
 template <class F>
@@ -590,21 +631,22 @@ int launch_backward(const Rows& r, int k, const void* x, const void* weight, con
       if (status != kOk) return status;
       const long long values = static_cast<long long>(rows) * k;
       finish<T>(values, plan.dx_splits.count, values, dx_sums, factors,
-                static_cast<T*>(dx) + first * k, s);
+                static_cast<T*>(dx) + first * k, s, r, first, k);
     }
     if (dweight) {
       // a last, shorter piece has fewer splits
       PairSplits dw = plan.dw_splits;
       dw.count = static_cast<int>((rows + dw.k - 1) / dw.k);
+      const Planes counted_xs = keep_counted<T>(r, first, rows, xs, ws + plan.x_planes, s);
       if (plan.on_chip) {
         status = each ? launch_pairs<T, dz_parts<T>(true), true, true>(
-                            vocabulary, k, rows, dz, xs, dw, weight_sums, first != 0, s)
+                            vocabulary, k, rows, dz, counted_xs, dw, weight_sums, first != 0, s)
                       : launch_pairs<T, dz_parts<T>(false), true, true>(
-                            vocabulary, k, rows, dz, xs, dw, weight_sums, first != 0, s);
+                            vocabulary, k, rows, dz, counted_xs, dw, weight_sums, first != 0, s);
       } else {
         ProductParams p{};
         p.m = vocabulary, p.k = rows, p.n = k;
-        use_planes(p, dz, xs);
+        use_planes(p, dz, counted_xs);
         p.k_per_split = dw.k, p.splits = dw.count;
         p.accumulate = first != 0;
         p.out = weight_sums;

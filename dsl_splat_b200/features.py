@@ -391,10 +391,11 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, bias: Tensor
     log sum_j exp z_j - z_target, as float32; the logits are never kept.
 
     x: (...,K), weight: (V,K), bias: (V,), target: (...) of int32 or int64 in [0,V).
-    Rows whose target is ignore_index have no loss and no gradient; so have rows with
-    another target outside, which also set the library's error word.  reduction:
-    "none" (a loss for each row), "sum" or "mean" over the rows that count (0 if none
-    does).  A bias of minus infinity takes a word out.
+    Rows whose target is ignore_index have no loss and no gradient, nor a part in those of
+    weight and bias, whatever x holds there; so have rows with another target outside, which
+    also set the library's error word.  reduction: "none" (a loss for each row), "sum" or
+    "mean" over the rows that count (0 if none does).  A bias of minus infinity takes a word
+    out (its weight is finite all the same).  Logits are below 2^127 in magnitude.
     """
     check_linear_cross_entropy(x, weight, target, bias, ignore_index, reduction)
     if forward_ad._current_level >= 0:

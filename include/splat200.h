@@ -644,8 +644,8 @@ int splat_feature_embedding_backward(int dtype, int id_bytes, long long count, i
 
 /* Softmax cross entropy of z = x weight^T + bias: x (rows, k), weight (vocabulary,
  * k), bias (vocabulary) or NULL, target (rows) of id_bytes 4 or 8 (signed).  A row whose
- * target is `ignored` does not count; one whose target lies outside the vocabulary neither,
- * with the device error -6.  reduction: 0 none (loss of each row), 1 sum, 2 mean over the
+ * target is `ignored` does not count, whatever x holds there; one whose target lies outside
+ * the vocabulary neither, with the device error -6.  reduction: 0 none (loss of each row), 1 sum, 2 mean over the
  * rows that count (0 if none does).  loss float32; moments (rows, 2) float32, the rows'
  * largest logits and sums in the units that the backward takes them in, or NULL; counted (1)
  * float32, the rows that count (1 if none does), for the mean's backward, or NULL.  A workspace

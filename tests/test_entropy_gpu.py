@@ -383,3 +383,58 @@ def test_upstreams_cost_no_digits(rows, reduction, dtype):
     for got, (want, _) in zip(grads, reference(x, w, None, target, -100, reduction, up)[1:3]):
         off = float((got.double() - want).norm() / want.norm())
         assert off < 1.2 * half_step(dtype) / math.sqrt(3)
+
+
+def gradients(x, w, b, target, reduction, up):
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    loss = features.linear_cross_entropy(*leaves[:2], target, leaves[2], reduction=reduction)
+    return loss.detach(), torch.autograd.grad(loss, leaves, up)
+
+
+# on the chip of whole 16-byte rows and of odd ones, and rows of several accumulators
+WIDTHS = [(700, 64, 300), (700, 35, 300), (300, 520, 260), (70, 16392, 40)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("m, k, v", WIDTHS)
+def test_rows_that_do_not_count_may_hold_anything(m, k, v, reduction, dtype):
+    """Infinities and NaN of padded rows reach no loss and no gradient."""
+    x, w, b, target = make(m, k, v, dtype, 30, ignored=0.3)
+    target[5], target[6], target[-1] = -100, v, -100
+    up = draws(31)(*([m] if reduction == "none" else []), dtype=torch.float32, shift=1.0)
+    want = gradients(x, w, b, target, reduction, up)
+    out = (target < 0) | (target >= v)
+    x[out] = torch.tensor([math.nan, math.inf, -math.inf], device="cuda").to(dtype).repeat(m)[
+        :int(out.sum())][:, None]
+    got = gradients(x, w, b, target, reduction, up)
+    assert torch.equal(got[0], want[0])
+    for a, c in zip(got[1], want[1]):
+        assert torch.equal(a, c)
+    assert not got[1][0][out].any()
+    assert _native.device_error(torch.device("cuda", torch.cuda.current_device())) == -6
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m, k, v", WIDTHS)
+def test_weights_that_are_not_finite_leave_rows_that_do_not_count(m, k, v, dtype):
+    x, w, b, target = make(m, k, v, dtype, 32, ignored=0.3)
+    w[3], w[7, 2] = math.nan, math.inf
+    _, (dx, _, _) = gradients(x, w, b, target, "mean", torch.ones((), device="cuda"))
+    assert not dx[target < 0].any() and not dx[target >= 0].isfinite().any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["sum", "mean"])
+@pytest.mark.parametrize("up", [math.nan, math.inf])
+def test_a_shared_upstream_that_is_not_finite(up, reduction, dtype):
+    """It reaches the rows that count, and nothing where none does."""
+    up = torch.tensor(up, device="cuda")
+    for m, k, v in WIDTHS:
+        x, w, b, target = make(m, k, v, dtype, 33, ignored=0.3)
+        _, (dx, dw, db) = gradients(x, w, b, target, reduction, up)
+        assert not dx[target < 0].any() and not dx[target >= 0].isfinite().any()
+        assert not dw[target[target >= 0]].isfinite().any()
+        assert not db[target[target >= 0]].isfinite().any()
+        _, grads = gradients(x, w, b, target.fill_(-100), reduction, up)
+        assert not any(g.any() for g in grads)
