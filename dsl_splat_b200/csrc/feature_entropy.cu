@@ -6,17 +6,29 @@
 //
 // The logits are never kept.  They never leave the chip (feature_vocabulary.cuh) but those of
 // rows so long that they take several accumulators, which are formed for a piece of the
-// rows at a time.  The backward forms them again, and dz for a piece of the rows.  u_i is the upstream gradient of row i's loss (divided by
-// the number of rows that count for their mean) and 0 for the others.
+// rows at a time.  The backward forms them again, and dz for a piece of the rows.  u_i is
+// the upstream gradient of row i's loss (divided by the number of rows that count for their
+// mean) and 0 for the others.
 //
 // dz is held in T for the products.  A u that all rows share is multiplied to the products'
 // fp32 results before their rounding; of u_i of their own dz is taken relative to the power of two
 // that is not below any |u_i|, and the results are multiplied by that.  float16, whose
 // smallest value would otherwise swallow the tail of a large vocabulary, has 2^15 times dz.
-// 16-bit types hold dz with u_i of their own as two values, whose products take twice the time:
-// with one, dx and dW would be off by 2.4e-3 instead of 1.7e-3 (bf16, relative), since a label's
-// dz would take the rounding of its u.  With a shared u one is enough, since a label's dz is
-// nearly 1 then.  Layers beyond on_chip() keep the one.
+//
+// What dz's rounding costs, as relative 2-norms of dx's error over those of its own rounding
+// (bf16 1.66e-3, fp16 2.07e-4; 2048 rows x 64 over 512 words, logits of deviation 4; dW is
+// alike):
+//
+//                                  labels: random   drawn from the softmax   the largest logit
+//   one value, u shared                     1.12            1.34                   1.45
+//   one value, u of the rows' own           1.40            1.45                   1.45
+//   two values                              1.00            1.00                   1.00
+//
+// A shared u takes one: p - 1 of a head that has learnt nothing is nearly -1, whose rounding is
+// small, and that of one that has costs as much as dx's own.  Two would take 3550 us instead of
+// 2390 (307200 x 64 over 4096 words, bf16, training) and 11900 instead of 7700 (65536 x
+// 512 over 32768).  u of the rows' own takes two, because every label's dz has the full
+// rounding there.  Layers beyond on_chip() keep the one.
 #include <algorithm>
 
 #include "feature_join.cuh"

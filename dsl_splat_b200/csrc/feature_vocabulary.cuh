@@ -61,7 +61,7 @@ enum Reduction : int { kEach = 0, kSum = 1, kMean = 2 };
 
 // Factors of the backward: of u_i on the way into dz, and of the products' results.  Where
 // all rows have the same u it is left to the results: rounded to 16 bits with each label's
-// dz, which is nearly -u, it would cost all of dx and dW the same error.
+// dz, which is nearly -u before a head has learnt, it would cost all of dx and dW the same error.
 struct Factors {
   float in, out;
 };

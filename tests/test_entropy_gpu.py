@@ -438,3 +438,43 @@ def test_a_shared_upstream_that_is_not_finite(up, reduction, dtype):
         assert not db[target[target >= 0]].isfinite().any()
         _, grads = gradients(x, w, b, target.fill_(-100), reduction, up)
         assert not any(g.any() for g in grads)
+
+
+def labels_of(kind, x, w, seed):
+    """Those of a head that has learnt nothing, of one whose softmax they follow, and of one
+    that is always right."""
+    z = (x.double() @ w.double().t()).cpu()
+    g = torch.Generator().manual_seed(seed)
+    return {"random": lambda: torch.randint(0, z.shape[1], (len(z),), generator=g),
+            "drawn": lambda: torch.multinomial(torch.softmax(z, 1), 1, generator=g)[:, 0],
+            "largest": lambda: z.argmax(1)}[kind]().to(x.device)
+
+
+def digits(x, w, target, reduction, up, got):
+    """The relative 2-norms of dx's and dW's errors, over those of their own rounding."""
+    for have, (want, _) in zip(got, reference(x, w, None, target, -100, reduction, up)[1:3]):
+        own = (want.to(have.dtype).double() - want).norm()
+        yield float((have.double() - want).norm() / own)
+
+
+# dz as two values is off by 2^-17 (bf16), and the logits by four additions of 2^-23 of some
+# 2^4: 2^-17 relative of the exponentials.  Over fp16's own rounding (2^-11 / sqrt 6) that
+# is 0.04, and as much again for the other sums.
+TWO_VALUES = 1.1
+# one value's rounding is of the size of the results' own: sqrt 2 where all of dz has it and
+# rows of W are unlike, and that of the largest of 2048 such sums
+ONE_VALUE = 1.55
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("kind", ["random", "drawn", "largest"])
+def test_digits_of_gradients(kind, reduction, dtype):
+    x, w, _, _ = make(2048, 64, 512, dtype, 34, bias=False, scale=4.0)
+    target = labels_of(kind, x, w, 35)
+    up = torch.full((2048,) if reduction == "none" else (), 1.0 + 2.0 ** -9, device="cuda")
+    if reduction == "none":
+        up = up + draws(36)(2048, dtype=torch.float32).abs()
+    _, got = gradients(x, w, torch.zeros_like(w[:, 0]), target, reduction, up)
+    for off in digits(x, w, target, reduction, up, got[:2]):
+        assert off <= (TWO_VALUES if reduction == "none" else ONE_VALUE)

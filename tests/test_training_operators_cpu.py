@@ -364,3 +364,34 @@ def test_entropy_entry_points_refuse_before_any_launch():
     assert backward(reduction=2, counted=None) == backward(bias=None) == backward(up=None) == -1
     assert backward(n=100) == -5
     assert lib.splat_launch_count() == before
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", ["random", "drawn", "largest"])
+def test_the_bound_on_digits_tells_one_value_from_two(kind, dtype):
+    """The bounds on the cross entropy's 16-bit gradients, on gradients in 64 bits whose dz alone
+    is rounded: with upstreams of the rows' own one value of the type is refused and two pass;
+    with a shared one, which is left to the results, one passes."""
+    from test_entropy_gpu import ONE_VALUE, TWO_VALUES, digits, labels_of
+
+    g = torch.Generator().manual_seed(37)
+    x = torch.randn(2048, 64, generator=g).to(dtype)
+    w = (torch.randn(512, 64, generator=g) / 2).to(dtype)
+    target = labels_of(kind, x, w, 38)
+    hit = torch.nn.functional.one_hot(target, 512).double()
+    p_hit = torch.softmax(x.double() @ w.double().t(), 1) - hit
+
+    def worst(up, within, values):
+        dz = p_hit * up * within
+        held = dz.to(dtype).double()
+        if values == 2:
+            held = held + (dz - held).to(dtype).double()
+        held = held / within
+        got = (held @ w.double()).to(dtype), (held.t() @ x.double()).to(dtype)
+        return max(digits(x, w, target, "none", up.reshape(-1).float().expand(2048), got))
+
+    scale = 2.0 ** 13 if dtype == torch.float16 else 0.25
+    own = (1 + torch.randn(2048, generator=g).abs()).float().double()[:, None]
+    assert worst(own, scale, 2) <= TWO_VALUES < worst(own, scale, 1)
+    shared = torch.ones(1, 1, dtype=torch.float64)
+    assert worst(shared, 4 * scale, 1) <= ONE_VALUE
