@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const SortPass p) {
     for (int w = 0; w < d / part; ++w) place += warp_sums[w];
     bins[d] = place;
   }
-  // the warps' counts, two to a word (a block has less than 2^16 rows, see plan_sort)
+  // the warps' counts, two to a word (a block has less than 2^16 rows, see plan_embedding)
   int* words = reinterpret_cast<int*>(own + static_cast<long long>(warp) * p.bins);
   for (long long i0 = begin + lane; i0 < end; i0 += kAhead * 32) {
     Sorted v[kAhead];
@@ -447,8 +447,9 @@ __global__ void __launch_bounds__(kThreads) join_runs_kernel(const RunParams p, 
 
 // ---- few rows: each entry looks for its own --------------------------------------------
 
-constexpr int kMostScanned = 2048;
+constexpr int kMostScanned = 1024;
 
+// A warp to an entry and every gridDim.y-th 32 of its channels.
 template <class T, class I>
 __global__ void __launch_bounds__(kThreads)
     scan_ids_kernel(int count, int entries, int channels, const void* ids, const T* dy,
@@ -458,14 +459,29 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   const int lane = threadIdx.x & 31;
   for (int v = blockIdx.x * kWarps + (threadIdx.x >> 5); v < entries; v += gridDim.x * kWarps)
-    for (int c0 = 0; c0 < channels; c0 += 32) {
+    for (int c0 = blockIdx.y * 32; c0 < channels; c0 += gridDim.y * 32) {
       const int c = c0 + lane;
       float sum = 0.0f;
       for (int i0 = 0; i0 < count; i0 += 32) {
         uint32_t hits = __ballot_sync(0xffffffffu, i0 + lane < count && id[i0 + lane] == v);
-        for (; hits; hits &= hits - 1)
-          if (c < channels)
-            sum += to_float(dy[static_cast<long long>(i0 + __ffs(hits) - 1) * channels + c]);
+        if (!hits || c >= channels) continue;
+        const T* rows = dy + static_cast<long long>(i0) * channels + c;
+        if (__popc(hits) > 4) {  // a common entry's loads are in flight together
+          constexpr int U = 16;
+          for (int r0 = 0; r0 < 32; r0 += U) {
+            T raw[U];
+#pragma unroll
+            for (int r = 0; r < U; ++r) {
+              raw[r] = from_float<T>(0.0f);
+              if (hits >> (r0 + r) & 1) raw[r] = rows[static_cast<long long>(r0 + r) * channels];
+            }
+#pragma unroll
+            for (int r = 0; r < U; ++r) sum += to_float(raw[r]);
+          }
+        } else {
+          for (; hits; hits &= hits - 1)
+            sum += to_float(rows[static_cast<long long>(__ffs(hits) - 1) * channels]);
+        }
       }
       if (c < channels)
         dtable[static_cast<long long>(v) * channels + c] = from_float<T>(sum * scale);
@@ -485,9 +501,11 @@ int check_embedding(int dtype, int id_bytes, long long count, int entries, int c
   return kOk;
 }
 
-// Whether each entry looks for its rows: 64 rows of 8192 entries x 512 (2^18 steps of a
-// warp) take 17 us, sorting them 47, most of which is the launches'; 256 rows of 65536 x 32
-// (2^19) about as long as sorted.
+// Whether each entry looks for its rows.  What bounds it is either all warps' steps together
+// (64 rows of 8192 entries x 512, 2^18 steps, take 15 us where sorting takes 29; 256 rows,
+// 2^20, 32 where it takes 29) or the warp of the commonest entry, which the sizes do not tell: rows
+// that are all alike take 10 us for 256 of them and 37 for 1024, unlike ones of 300 entries x
+// 512 take 8, and sorting 1024 takes 22 to 25 (47 where its launches are not captured).
 bool scans(long long count, int entries, int channels) {
   return count <= kMostScanned &&
          (count + 31) / 32 * entries * ((channels + 31) / 32) <= 1LL << 19;
@@ -573,7 +591,10 @@ template <class T, class I>
 int launch_gradient(long long count, int entries, int channels, const void* ids, const void* dy,
                     float scale, void* dtable, char* ws, cudaStream_t s) {
   if (scans(count, entries, channels)) {
-    const int grid = std::min((entries + kWarps - 1) / kWarps, 8 * host::sm_count());
+    // the channels of few entries are spread over blocks
+    const int wanted = 8 * host::sm_count(), columns = (channels + 31) / 32;
+    const int blocks = std::min((entries + kWarps - 1) / kWarps, wanted);
+    const dim3 grid(blocks, std::min(columns, std::max(1, wanted / blocks)));
     scan_ids_kernel<T, I><<<grid, kThreads, 0, host::counted(s)>>>(
         static_cast<int>(count), entries, channels, ids, static_cast<const T*>(dy), scale,
         static_cast<T*>(dtable));

@@ -90,6 +90,28 @@ def test_rows_in_order():
         assert torch.equal(grad.double(), want)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("count", [5, 33, 1000, 1024, 1025])
+@pytest.mark.parametrize("entries", [1, 2, 300])
+def test_few_rows(entries, count, dtype):
+    """Up to those that each entry looks for itself: of like and of unlike ids, whole and
+    partial pieces of 32 channels."""
+    for channels in (3, 32, 70, 512):
+        table = draws(20)(entries, channels, dtype=dtype)
+        run(ids_of(count, entries, 21), table, 0.5)
+        run(torch.full((count,), entries - 1, device="cuda"), table, 1.0)
+
+
+def test_few_rows_in_order():
+    """Sums of whole numbers, whose order has to be the rows' where they are not exact."""
+    dy = torch.ones(1024, 40, device="cuda")
+    dy[0], dy[-1] = 2.0 ** 24, -(2.0 ** 24)  # a one is lost on the way wherever it comes
+    table = torch.zeros(2, 40, device="cuda", requires_grad=True)
+    ids = torch.ones(1024, dtype=torch.int64, device="cuda")
+    grad, = torch.autograd.grad(features.embedding(ids, table), table, dy)
+    assert not grad.any()
+
+
 def test_shapes_and_strides():
     table = draws(10)(50, 24, dtype=torch.float16)
     ids = ids_of(120, 50, 11).reshape(5, 4, 6)

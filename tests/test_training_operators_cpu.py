@@ -157,6 +157,17 @@ def test_entry_points_refuse_before_any_launch():
     assert lib.splat_launch_count() == before
 
 
+def test_embedding_gradients_of_common_entries_are_sorted():
+    """No entry looks for more than 1024 rows of its own, however few entries there are."""
+    size = lib.splat_feature_embedding_backward_workspace_bytes
+    for dtype in range(3):
+        for entries, channels in ((1, 1), (2, 512), (300, 32)):
+            assert size(dtype, 1024, entries, channels) == 16
+            assert size(dtype, 1025, entries, channels) > 16
+    # nor are more steps than sorting takes spread over the device
+    assert size(0, 64, 8192, 512) == 16 and size(0, 256, 8192, 512) > 16
+
+
 def test_adamw_entry_points_refuse_before_any_launch():
     before = lib.splat_launch_count()
 
