@@ -22,7 +22,6 @@ The reference has no counterpart; its users bring their own optimizer.
 
 from __future__ import annotations
 
-import math
 import struct
 from numbers import Integral, Real
 from typing import Any, Callable, Iterable, Sequence
@@ -72,23 +71,28 @@ class Moment8:
         return stages.adamw_decode(self.codes, self.exponents, self.squared)
 
 
+# The kernel takes these in fp32.
+_LARGEST = 2.0 ** 128
+_BELOW_ONE = 1.0 - 2.0 ** -24
+
+
 def _check_settings(betas: tuple[float, float], eps: float, weight_decay: float) -> None:
-    if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
-        raise ValueError("betas must be two numbers of at least 0 and below 1")
-    if not (eps >= 0.0 and math.isfinite(eps)):
-        raise ValueError("eps must be finite and not negative")
-    if not (weight_decay >= 0.0 and math.isfinite(weight_decay)):
-        raise ValueError("weight_decay must be finite and not negative")
+    if len(betas) != 2 or not all(0.0 <= b <= _BELOW_ONE for b in betas):
+        raise ValueError("betas must be two numbers of at least 0 and below 1 in float32")
+    if not (eps == 0.0 or 2.0 ** -126 <= eps < _LARGEST):
+        raise ValueError("eps must be 0, or finite and positive in float32's normal range")
+    if not 0.0 <= weight_decay < _LARGEST:
+        raise ValueError("weight_decay must be finite in float32 and not negative")
 
 
 def _check_lr(lr: Any) -> None:
-    if type(lr) is float and 0.0 <= lr < math.inf:
+    if type(lr) is float and 0.0 <= lr < _LARGEST:
         return
     if isinstance(lr, Tensor):
         if lr.numel() != 1 or not lr.is_cuda or lr.dtype is not torch.float32:
             raise ValueError("lr must be a number or a CUDA float32 tensor of one value")
-    elif not isinstance(lr, Real) or not (lr >= 0.0 and math.isfinite(lr)):
-        raise ValueError("lr must be finite and not negative")
+    elif not isinstance(lr, Real) or not 0.0 <= lr < _LARGEST:
+        raise ValueError("lr must be finite in float32 and not negative")
 
 
 def _check_step(step: Any) -> None:

@@ -207,6 +207,24 @@ def test_optimizer_refuses_host_tensors_and_bad_settings():
             optim.AdamW([fake(4, 3).t().requires_grad_()])
 
 
+@pytest.mark.parametrize("change, message", [
+    (dict(eps=1e-50), "eps"), (dict(eps=1e-40), "eps"), (dict(eps=1e39), "eps"),
+    (dict(eps=float("nan")), "eps"), (dict(lr=1e39), "lr"),
+    (dict(weight_decay=1e39), "weight_decay"), (dict(betas=(0.9, 1 - 2.0 ** -26)), "betas"),
+])
+def test_settings_that_float32_has_not(change, message):
+    """They would become 0, infinity or 1 on the way to the kernel."""
+    with FakeTensorMode():
+        p = fake(4, 3).requires_grad_()
+        with pytest.raises(ValueError, match=message):
+            optim.AdamW([p], **change)
+        settings = {"step": 1, "lr": 0.1, **change}
+        with pytest.raises(ValueError, match=message):
+            optim.adamw([p], [p], [p], [p], **settings)
+        for eps in (0.0, 2.0 ** -126, 1e-15):
+            optim.AdamW([p], eps=eps, betas=(0.0, 1 - 2.0 ** -24))
+
+
 def test_moment8_refusals():
     codes, exponents = torch.zeros(300, dtype=torch.uint8), torch.zeros(2, dtype=torch.int8)
     optim.Moment8(codes, exponents)
