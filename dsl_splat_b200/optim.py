@@ -332,11 +332,20 @@ class AdamW(torch.optim.Optimizer):
 
     @staticmethod
     def _put(state: dict, m: Tensor | Moment8, v: Tensor | Moment8) -> None:
+        """Into the state's own tensors where they fit, which a captured step may hold."""
         for name, moment in (("exp_avg", m), ("exp_avg_sq", v)):
             if isinstance(moment, Moment8):
-                state[name], state[name + "_exponents"] = moment.codes, moment.exponents
+                parts = {name: moment.codes, name + "_exponents": moment.exponents}
             else:
-                state[name] = moment
+                parts = {name: moment}
+                state.pop(name + "_exponents", None)
+            for key, value in parts.items():
+                held = state.get(key)
+                if isinstance(held, Tensor) and held.shape == value.shape \
+                        and held.dtype is value.dtype and held.device == value.device:
+                    held.copy_(value)
+                else:
+                    state[key] = value
 
     @staticmethod
     def _get(state: dict) -> tuple:
@@ -388,12 +397,14 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def set_moments(self, p: Tensor, m: Tensor, v: Tensor) -> None:
-        """Replaces a parameter's moments by float32 ones of its shape; its step stays."""
+        """Replaces the values of a parameter's moments by float32 ones of its shape; its step
+        stays."""
         group = next((g for g in self.param_groups if any(q is p for q in g["params"])), None)
         if group is None:
             raise KeyError("not a parameter of this optimizer")
         for t in (m, v):
-            _check_moment(t, p, False)
+            if _check_moment(t, p, False) != 32:
+                raise ValueError("moments are set from float32 tensors")
         state = self._state(p, group)
         if group["state_bits"] == 8:
             self._put(state, Moment8.of(m), Moment8.of(v, squared=True))

@@ -481,6 +481,41 @@ def test_captured_steps(bits):
                 assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_moments_set_between_replays(bits):
+    """A captured step holds the state's tensors: what is set later is what it goes on from."""
+    p = draw(11, 700, 3).requires_grad_()
+    p.grad = draw(12, 700, 3)
+    optimizer = optim.AdamW([p], lr=0.01, state_bits=bits, capturable=True)
+    optimizer.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        optimizer.step()
+    graph.replay()
+    m, v = (t.clone() for t in optimizer.moments(p))
+    optimizer.set_moments(p, 0.5 * m, 2.0 * v)
+    m, v = (t.clone() for t in optimizer.moments(p))
+    before = p.detach().clone()
+    graph.replay()
+    want, tolerance = reference(before, p.grad, m, v, 3, 0.01, (0.9, 0.999), 1e-8, 0.01)
+    close(p.detach(), want[0], tolerance[0], "p")
+    if bits == 32:
+        for got, w, t in zip(optimizer.moments(p), want[1:], tolerance[1:]):
+            close(got, w, t, "moment")
+    else:  # one step of a code below, at most
+        for got, w, mantissa in zip(optimizer.moments(p), want[1:], (8, 8)):
+            assert bool(((got - w).abs() <= 2.0 * w.abs() / mantissa
+                         + float(w.abs().max()) * 2.0 ** -14).all())
+            assert not torch.equal(got, m)
+    # its own tensors, one in the other's place
+    first, second = optimizer.moments(p)
+    swapped = second.clone(), first.abs()
+    optimizer.set_moments(p, second, first.abs())
+    got = optimizer.moments(p)
+    if bits == 32:
+        assert torch.equal(got[0], swapped[0]) and torch.equal(got[1], swapped[1])
+
+
 def test_capture_refusals():
     p = draw(1, 8).requires_grad_()
     p.grad = torch.ones_like(p)
