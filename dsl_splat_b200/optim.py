@@ -328,6 +328,13 @@ class AdamW(torch.optim.Optimizer):
             else:
                 self._put(state, torch.zeros_like(p, dtype=torch.float32),
                           torch.zeros_like(p, dtype=torch.float32))
+        elif group["capturable"] and not isinstance(state["step"], Tensor):
+            # a captured step would hold the number that it has now
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW moves a parameter's step to the device in its first "
+                                   "capturable step, which must run before a step is captured")
+            state["step"] = torch.full((), _counted(state["step"]), dtype=torch.int64,
+                                       device=p.device)
         return state
 
     @staticmethod

@@ -516,6 +516,29 @@ def test_moments_set_between_replays(bits):
         assert torch.equal(got[0], swapped[0]) and torch.equal(got[1], swapped[1])
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_that_becomes_capturable(bits):
+    """A state that counted on the host, in a group that has been made capturable."""
+    p, q = draw(13, 300).requires_grad_(), draw(13, 300).requires_grad_()
+    p.grad, q.grad = draw(14, 300), draw(14, 300)
+    ours = optim.AdamW([p], lr=0.01, state_bits=bits)
+    eager = optim.AdamW([q], lr=0.01, state_bits=bits)
+    ours.step()
+    ours.param_groups[0]["capturable"] = True
+    with pytest.raises(RuntimeError, match="before a step is captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ours.step()
+    ours.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ours.step()
+    for _ in range(3):
+        graph.replay()
+    for _ in range(5):
+        eager.step()
+    assert torch.equal(p, q) and int(ours.state[p]["step"]) == 5
+
+
 def test_capture_refusals():
     p = draw(1, 8).requires_grad_()
     p.grad = torch.ones_like(p)

@@ -207,6 +207,21 @@ def test_optimizer_refuses_host_tensors_and_bad_settings():
             optim.AdamW([fake(4, 3).t().requires_grad_()])
 
 
+def test_a_step_counted_on_the_host_is_not_captured(monkeypatch):
+    """A replay would repeat its number."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with FakeTensorMode():
+        p = fake(4, 3).requires_grad_()
+        p.grad = fake(4, 3)
+        optimizer = optim.AdamW([p], capturable=True)
+        optimizer.state[p] = {"step": 3, "exp_avg": fake(4, 3), "exp_avg_sq": fake(4, 3)}
+        with pytest.raises(RuntimeError, match="before a step is captured"):
+            optimizer.step()
+        with pytest.raises(ValueError, match="float32 tensors"):
+            optimizer.set_moments(p, optim.Moment8(fake(4, 3, dtype=torch.uint8),
+                                                   fake(1, dtype=torch.int8)), fake(4, 3))
+
+
 @pytest.mark.parametrize("change, message", [
     (dict(eps=1e-50), "eps"), (dict(eps=1e-40), "eps"), (dict(eps=1e39), "eps"),
     (dict(eps=float("nan")), "eps"), (dict(lr=1e39), "lr"),
