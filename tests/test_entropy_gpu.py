@@ -478,3 +478,37 @@ def test_digits_of_gradients(kind, reduction, dtype):
     _, got = gradients(x, w, torch.zeros_like(w[:, 0]), target, reduction, up)
     for off in digits(x, w, target, reduction, up, got[:2]):
         assert off <= (TWO_VALUES if reduction == "none" else ONE_VALUE)
+
+
+def pieces_of(m, k, v, dtype, reduction):
+    """How many pieces the backward takes, and the last one's rows.  Its workspace holds what
+    a piece needs, and so stops growing with the rows where they are one."""
+    def size(rows):
+        return _native.lib.splat_feature_entropy_workspace_bytes(
+            {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype], rows, k, v,
+            2 if reduction == "none" else 1)
+
+    low, high = 1, 1 << 29  # size(high) is that of a whole piece
+    while low < high:
+        middle = (low + high) // 2
+        if size(middle) == size(1 << 29):
+            high = middle
+        else:
+            low = middle + 1
+    return -(-m // low), m - (m - 1) // low * low
+
+
+@pytest.mark.parametrize("m, k, v, dtype, reduction, pieces", [
+    # on the chip, dW in several ranges of rows, of which the last piece has fewer
+    (300000, 64, 2000, torch.float32, "mean", 4), (300000, 64, 2000, torch.bfloat16, "none", 3),
+    (300000, 64, 2000, torch.float16, "mean", 2),
+    # logits in memory: a range, and several
+    (4500, 520, 1 << 17, torch.float32, "none", 3), (4500, 520, 1 << 17, torch.float32, "mean", 3),
+    (200000, 520, 2000, torch.float32, "none", 2), (200000, 520, 2000, torch.float32, "mean", 2),
+    (20000, 16392, 100, torch.bfloat16, "none", 2), (20000, 16392, 100, torch.bfloat16, "mean", 2),
+    (20000, 16392, 100, torch.float16, "mean", 2)])
+def test_pieces_with_a_short_last_one(m, k, v, dtype, reduction, pieces):
+    count, last = pieces_of(m, k, v, dtype, reduction)
+    assert count == pieces and last < m // count
+    run(*make(m, k, v, dtype, 40), reduction=reduction)
+    torch.cuda.empty_cache()
