@@ -180,3 +180,33 @@ def test_captured_on_another_stream():
     check(first, *reference(other.flip(0), 300, dy, 1.0), "dtable")
     check(grad, *reference(other, 300, dy, 1.0), "dtable")
     assert want.shape == grad.shape
+
+
+@pytest.mark.parametrize("count", [700, 9000])
+def test_replays_give_what_calls_give(count):
+    """A captured step replayed with other ids and upstreams gives those of calls, to the bit."""
+    table = draws(22)(300, 32, dtype=torch.float32)
+    side = torch.cuda.Stream()
+
+    def call(ids, dy):
+        leaf = table.detach().requires_grad_()
+        y = features.embedding(ids, leaf, scale=0.5)
+        return y.detach().clone(), torch.autograd.grad(y, leaf, dy)[0]
+
+    inputs = [(ids_of(count, 300, 23 + i, power=1.0 + i), draws(26 + i)(count, 32,
+                                                                       dtype=torch.float32))
+              for i in range(3)]
+    want = [call(*pair) for pair in inputs]
+    ids, dy = (torch.zeros_like(t) for t in inputs[0])
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            leaf = table.detach().requires_grad_()
+            y = features.embedding(ids, leaf, scale=0.5)
+            grad, = torch.autograd.grad(y, leaf, dy)
+        for (new_ids, new_dy), (value, gradient) in zip(inputs, want):
+            ids.copy_(new_ids)
+            dy.copy_(new_dy)
+            graph.replay()
+            assert torch.equal(y.detach(), value) and torch.equal(grad, gradient)

@@ -199,6 +199,46 @@ def test_steps_in_8_bits(n, dtype):
         assert torch.equal(second.codes.long(), torch.where(v1 > 0, c.clamp(min=1), c))
 
 
+def behind(t, offset):
+    """The same values from `offset` elements behind an aligned address on."""
+    flat = torch.empty(t.numel() + offset, dtype=t.dtype, device=t.device)[offset:]
+    return flat.copy_(t.reshape(-1)).view(t.shape)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("which", ["all", "p", "g", "m", "v"])
+def test_8_bit_steps_of_unaligned_tensors(which, dtype):
+    """More tensors than a launch takes, of which any may lie off 16 bytes: the same bits as
+    those that lie on them."""
+    sizes = [1, 3, 255, 256, 257, 1000, 16384, 16385, 40000] + [130 + i for i in range(100)]
+    p = [draw(i, n).to(dtype) for i, n in enumerate(sizes)]
+    g = [draw(1000 + i, n).to(dtype) for i, n in enumerate(sizes)]
+    first = [optim.Moment8.of(0.1 * draw(2000 + i, n)) for i, n in enumerate(sizes)]
+    second = [optim.Moment8.of(draw(3000 + i, n).square(), squared=True)
+              for i, n in enumerate(sizes)]
+
+    def moved(name, t, i):
+        return behind(t, 1 + i % 7 if which in ("all", name) else 0)
+
+    twins = [moved("p", t, i) for i, t in enumerate(p)], [moved("g", t, i) for i, t in enumerate(g)]
+    moments = [[optim.Moment8(moved(name, t.codes, i), moved(name, t.exponents, i), t.squared)
+                for i, t in enumerate(group)] for name, group in (("m", first), ("v", second))]
+    for step in (1, 9):
+        optim.adamw(p, g, first, second, step=step, lr=0.01)
+        optim.adamw(*twins, *moments, step=step, lr=0.01)
+    for a, c in zip(p, twins[0]):
+        assert torch.equal(a, c)
+    for group, others in zip((first, second), moments):
+        for a, c in zip(group, others):
+            assert torch.equal(a.codes, c.codes) and torch.equal(a.exponents, c.exponents)
+            assert torch.equal(a.values(), c.values())
+    # and encoding and decoding
+    for t in (0.1 * draw(1, 1001), draw(2, 1001).square()):
+        for squared in (False, True):
+            a, c = optim.Moment8.of(t.abs(), squared), optim.Moment8.of(behind(t.abs(), 3), squared)
+            assert torch.equal(a.codes, c.codes) and torch.equal(a.exponents, c.exponents)
+
+
 def test_8_bit_averages_follow_small_steps():
     """A constant gradient: v' moves by a thousandth of what it lacks, less than any
     code's step; over 3000 steps it has to come within a twentieth of its limit."""
