@@ -142,6 +142,7 @@ class _Launches:
         self.written: list[Tensor] = []
         self.held: list[Tensor] = []  # until the launches
         self.places: set[int] = set()
+        self.read: set[int] = set()
 
     def add(self, p: Tensor, g: Tensor, m: Tensor | Moment8, v: Tensor | Moment8,
             step: int | Tensor, lr: float | Tensor, decay: float, betas: tuple[float, float],
@@ -171,23 +172,29 @@ class _Launches:
         if not g.is_contiguous():
             g = g.contiguous()
             self.held.append(g)
-        address = p.data_ptr()
+        address, gradient = p.data_ptr(), g.data_ptr()
         if bits == 8:
-            record = (address, g.data_ptr(), m.codes.data_ptr(), v.codes.data_ptr(),
+            record = (address, gradient, m.codes.data_ptr(), v.codes.data_ptr(),
                       m.exponents.data_ptr(), v.exponents.data_ptr())
             self.written += (p, m.codes, v.codes, m.exponents, v.exponents)
         else:
-            record = (address, g.data_ptr(), m.data_ptr(), v.data_ptr())
+            record = (address, gradient, m.data_ptr(), v.data_ptr())
             self.written += (p, m, v)
         written = {address, *record[2:]}
         if len(written) < len(record) - 1 or not written.isdisjoint(self.places):
             raise ValueError("a parameter or a moment is listed twice")
         self.places |= written
+        self.read.add(gradient)
         record = _RECORD.pack(*record, *(0,) * (6 - len(record)), device_step, device_lr, n, step,
                               lr, decay, betas[0], betas[1], eps)
         self.records.setdefault((index, p.dtype, bits, maximize), []).append(record)
 
-    def run(self) -> None:
+    def run(self, counters: Sequence[Tensor] = ()) -> None:
+        """counters: device steps, which the launches read one on."""
+        if not self.read.isdisjoint(self.places):
+            raise ValueError("a gradient is a parameter or a moment of the same step")
+        if counters:
+            torch._foreach_add_(counters, 1)
         for (index, dtype, bits, maximize), records in self.records.items():
             stages.adamw(index, dtype, bits, records, maximize)
         if self.written:
@@ -205,7 +212,8 @@ def adamw(params: Sequence[Tensor], grads: Sequence[Tensor],
     step counts from 1 and is the number of this step.  step, lr and weight_decay are
     one value or a list with one for each parameter; step may be a CUDA int64 and lr a CUDA
     float32 tensor of one value, which the kernel reads (a captured step then follows
-    them).  No parameter or moment may be listed twice or share memory with another."""
+    them).  No parameter or moment may be listed twice or share memory with another or with
+    a gradient."""
     count = len(params)
     if not len(grads) == len(exp_avgs) == len(exp_avg_sqs) == count:
         raise ValueError("params, grads, exp_avgs and exp_avg_sqs must have the same length")
@@ -388,9 +396,7 @@ class AdamW(torch.optim.Optimizer):
                     counted.append(state)
                     step += 1
                 launches.add(p, p.grad, *self._get(state), step, *settings)
-        if counters:
-            torch._foreach_add_(counters, 1)
-        launches.run()
+        launches.run(counters)
         for state in counted:
             state["step"] += 1
         return loss

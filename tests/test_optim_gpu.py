@@ -636,3 +636,16 @@ def test_refusals():
     refused("lr must be", [p], [g], [m], [v], lr=torch.ones((), device="cuda").double())
     refused("one for each", [p], [g], [m], [v], lr=[0.1, 0.2])
     refused("dense", [p], [g.to_sparse()], [m], [v])
+
+
+def test_gradients_that_are_written():
+    """Other blocks of the same launch would read them while they change."""
+    p, q, g = draw(1, 10), draw(2, 10), draw(3, 10)
+    moments = [torch.zeros(10, device="cuda") for _ in range(4)]
+    before = p.clone(), q.clone()
+    for grads in ([q, g], [g, p], [g, moments[2]]):
+        with pytest.raises(ValueError, match="a gradient is"):
+            optim.adamw([p, q], grads, moments[:2], moments[2:], step=1, lr=0.1)
+    assert torch.equal(p, before[0]) and torch.equal(q, before[1])
+    optim.adamw([p, q], [g, g], moments[:2], moments[2:], step=1, lr=0.1)
+    assert not torch.equal(p, before[0]) and not torch.equal(q, before[1])
