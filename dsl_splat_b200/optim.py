@@ -299,7 +299,9 @@ class AdamW(torch.optim.Optimizer):
     replayed (lr may then be a CUDA float32 tensor).
 
     load_state_dict takes torch.optim.AdamW's state too, but for amsgrad: its steps are
-    converted and its moments held in float32, or in 8 bits where the group has them."""
+    converted and its moments held in float32, or in 8 bits where the group has them.  What
+    it loads are new tensors, which a step captured before does not follow; moments that
+    set_moments takes are written into those that it does."""
 
     def __init__(self, params: Iterable, lr: float | Tensor = 1e-3,
                  betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -444,6 +446,8 @@ class AdamW(torch.optim.Optimizer):
             for group, own in zip(self.param_groups, settings):
                 for name, value in own.items():
                     group.setdefault(name, value)
+                if isinstance(group["lr"], Tensor) and group["params"]:  # read on the host
+                    group["lr"] = group["lr"].to(group["params"][0].device, torch.float32)
             # torch casts a state to its parameter's dtype; moments keep theirs
             for p, state in states:
                 self.state[p] = state

@@ -2,6 +2,7 @@
 their definition bit by bit."""
 
 import copy
+import io
 import math
 
 import pytest
@@ -400,6 +401,31 @@ def test_state_of_torch(kind, dtype, bits):
     twin.load_state_dict(copy.deepcopy(ours.state_dict()))
     for p in params:
         for a, c in zip(ours.moments(p), twin.moments(p)):
+            assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_read_on_the_host(bits):
+    """What torch.load(map_location="cpu") gives, a learning rate on the device with it."""
+    params = scene(15)
+    optimizer = optim.AdamW(params, lr=torch.tensor(0.01, device="cuda"), state_bits=bits,
+                            capturable=True)
+    set_grads(params, 1)
+    optimizer.step()
+    file = io.BytesIO()
+    torch.save(optimizer.state_dict(), file)
+    file.seek(0)
+    twins = [p.detach().clone().requires_grad_() for p in params]
+    twin = optim.AdamW(twins, state_bits=bits)
+    twin.load_state_dict(torch.load(file, map_location="cpu"))
+    set_grads(params, 2)
+    set_grads(twins, 2)
+    optimizer.step()
+    twin.step()
+    assert twin.param_groups[0]["lr"].is_cuda and twin.param_groups[0]["capturable"]
+    for p, t in zip(params, twins):
+        assert torch.equal(p, t) and int(twin.state[t]["step"]) == 2
+        for a, c in zip(optimizer.moments(p), twin.moments(t)):
             assert torch.equal(a, c)
 
 
