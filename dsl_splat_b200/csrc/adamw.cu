@@ -22,9 +22,10 @@
 // could follow.  The states' arithmetic is single fp32 operations in a fixed order,
 // because a code depends on which side of a border its value lies.
 //
-// 59 million fp32 values: 246 us with states in 32 bits (6.7 TB/s); 255 in 8 (3.7 TB/s), of
-// which the codes' arithmetic takes its part (ALU pipe 58 %, DRAM 43 % of its cycles), while the
-// states take 118 MB instead of 472.  Reading both moments back takes 135.
+// 59 million fp32 values: 246 us with states in 32 bits (6.7 TB/s); 256 in 8 (3.7 TB/s), of
+// which the codes' arithmetic takes its part (ALU pipe 56 %, DRAM 41 % of its cycles), while the
+// states take 118 MB instead of 472.  Reading both moments back takes 135.  Steps and rates on
+// the device cost each block two powers in 64 bits: 2 us and 12.
 #include <algorithm>
 #include <cmath>
 

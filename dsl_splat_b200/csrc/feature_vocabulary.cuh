@@ -20,7 +20,7 @@
 //
 // 65536 x 512 bf16 features and 32768 words: statistics 1.41 ms (1560 TFLOP/s, tensor pipe 85 %
 // of a piece's cycles), slopes 1.96 (1125, 59 %: 4.3 GB of dz go out beside the
-// exponentials).  307200 x 64 and 4096: 540 us (special-function pipe 56 %) and 850 (36 %),
+// exponentials).  307200 x 64 and 4096: 540 us (special-function pipe 56 %) and 840 (36 %),
 // without a bias 450 and 620: its addition and db's sums take issue slots.  Direct stores of dz
 // instead of patches took longer; so did chunks of 64 words, whose registers spill, and
 // biases loaded before the logits.
@@ -149,7 +149,7 @@ SPLAT_DEV void add_bias(float (&v)[32], const T* bias, int words) {
 
 // The sums over a warp's rows of 32 columns: lane j gets column j's.  Every step halves the
 // columns of a lane.  Through shared memory, whose wavefronts they then were most of, the
-// slopes of 307200 rows and 4096 words took 955 us instead of 850.
+// slopes of 307200 rows and 4096 words took 955 us instead of 840.
 template <int N>
 SPLAT_DEV float column_sum(const float (&v)[N]) {
   if constexpr (N == 1) {

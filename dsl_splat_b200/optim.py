@@ -15,7 +15,9 @@ its root with 4 and 4, both relative to the run's exponent.  Each step rounds th
 down after a dither that is a hash of the value's place and the step: off by less than
 a step of the code and right on average, so that averages which move by less than that
 are followed; the update itself takes the values before their rounding.  A run that
-holds an infinity or a NaN reads as NaN.
+holds an infinity or a NaN reads as NaN, and makes its parameters NaN in the next step:
+gradients that may not be finite are looked at before the step, as torch.amp.GradScaler
+does.
 
 The reference has no counterpart; its users bring their own optimizer.
 """
