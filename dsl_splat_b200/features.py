@@ -399,7 +399,8 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, bias: Tensor
     weight and bias, whatever x holds there; so have rows with another target outside, which
     also set the library's error word.  reduction: "none" (a loss for each row), "sum" or
     "mean" over the rows that count (0 if none does).  A bias of minus infinity takes a word
-    out (its weight is finite all the same).  Logits are below 2^127 in magnitude.
+    out (its weight is finite all the same), as does one of the type's lowest value beside
+    others; a row's largest logit is below 2^127 in magnitude.
     """
     check_linear_cross_entropy(x, weight, target, bias, ignore_index, reduction)
     if forward_ad._current_level >= 0:
