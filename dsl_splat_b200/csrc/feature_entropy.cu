@@ -255,7 +255,8 @@ void add_columns(int vocabulary, int ranges, const float* sums, bool begin, floa
 }
 
 // What dW is formed of: x without the rows that do not count, which may hold infinities and
-// NaN (0 times them would reach every word; 20 us of 2410 for 307200 x 64 bf16).  `from`: rows of 16-byte pieces, which are copied; or NULL: planes of parts, in place.
+// NaN (0 times them would reach every word; 20 us of 2410 for 307200 x 64 bf16).  `from`:
+// rows of 16-byte pieces, which are copied; or NULL: planes of parts, in place.
 __global__ void __launch_bounds__(kThreads)
     keep_counted_kernel(const Rows p, long long first, int rows, int pieces, const uint4* from,
                         int parts, long long plane_pieces, uint4* to) {
